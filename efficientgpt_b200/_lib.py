@@ -14,7 +14,7 @@ HEADER_PATH = _PKG.parent / 'include' / 'egpt_b200.h'
 
 EGPT_OK, EGPT_ERR_SHAPE, EGPT_ERR_DTYPE, EGPT_ERR_ALIGN, EGPT_ERR_LAUNCH, EGPT_ERR_TIMEOUT, EGPT_ERR_ARG, \
     EGPT_ERR_WORKSPACE = range(8)
-EGPT_F32, EGPT_BF16 = 0, 1
+EGPT_F32, EGPT_BF16, EGPT_I8 = 0, 1, 2
 EPI_NONE, EPI_RESIDUAL, EPI_SILU_MUL, EPI_GELU = 0, 1, 2, 3
 FLAG_DOUBLE_ROUND, FLAG_RMSNORM, FLAG_PDL, FLAG_EMBED, FLAG_ADVANCE, FLAG_APPEND, FLAG_NO_TMA = 1, 2, 4, 8, 16, 32, 64
 FLAG_REF_SOFTMAX = 128
@@ -71,6 +71,13 @@ SIGNATURES = {
                                U32, P]),
     'egpt_attn_decode_noalloc': (I32, [P, I64, P, I64, P, P, I64, P, I64, I32, I32, I32, P, P, F32, P, P, F32, I32,
                                        I32, U32, P]),
+    'egpt_kv_append_q8': (I32, [P, P, P, P, I64, P, I64, P, I64, P, I64, I32, I32, I32, P, I64, P, I64, I32, P, P, F32, P,
+                                P, I64, U32, P]),
+    'egpt_kv_read_q8': (I32, [P, P, I64, I32, P, P, P, P, I64, I64, I32, I64, P, I32, I64, U32, P]),
+    'egpt_attn_q8_ws_bytes': (SZ, [I64, I32, I32, I32]),
+    'egpt_attn_decode_q8': (I32, [P, I64, P, I64, P, P, P, P, I64, P, I64, I32, I32, I32, F32, P, SZ, U32, P]),
+    'egpt_attn_shared_prefix': (I32, [P, I64, P, I64, P, P, P, P, I64, I64, P, P, P, P, I64, P, I64, I32, I32, I32, F32,
+                                      I32, P, SZ, U32, P]),
     'egpt_argmax_rows': (I32, [P, P, I64, I64, I64, I32, P]),
     'egpt_sample_ws_bytes': (SZ, [I64]),
     'egpt_attn_prefill': (I32, [P, I64, P, I64, P, P, I64, I64, I64, I32, I32, I32, F32, P]),

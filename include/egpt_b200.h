@@ -40,6 +40,7 @@ extern "C" {
 /* ---- dtypes ---------------------------------------------------------------------------------------- */
 #define EGPT_F32 0
 #define EGPT_BF16 1
+#define EGPT_I8 2 /* int8 codes with one fp32 scale per row (the int8 KV cache)                          */
 
 /* ---- GEMV epilogues -------------------------------------------------------------------------------- */
 #define EGPT_EPI_NONE 0     /* y = round(acc * s[n]) (+ bias[n])                                          */
@@ -185,6 +186,53 @@ EGPT_API int egpt_attn_decode_noalloc(void *out, int64_t ldo, const void *q, int
 EGPT_API int egpt_attn_prefill(void *out, int64_t ldo, const void *q, int64_t ldq, const void *k_cache,
                                const void *v_cache, int64_t cap, int64_t pos0, int64_t m, int nq, int nkv, int d,
                                float scale, void *stream);
+
+/* ---- int8 KV cache: written, read back, attended to ------------------------------------------------------
+ * No counterpart in the reference (its static cache holds the activations' dtype). A cache is int8 codes
+ * [heads][cap][d] and fp32 scales [heads][cap], a pair of them for keys and for values: row r of head h stands for
+ * scale[h][r] * codes[h][r], with the weights' quantiser s = max(max|x| / 127, 1e-12), q = clamp(rint(x / s), -127,
+ * 127) (egpt_quantize_rows). d is 32, 64 or 128; codes 16-byte aligned. Values are expected finite.
+ *
+ * egpt_kv_append_q8: rows i < m of k [m][ldk] and v [m][ldv] (head g at columns g d; dtype bf16 or fp32; 16-byte
+ *   aligned rows) into slot *position + i, or with EGPT_FLAG_RAGGED row i into slot position[i] of its own cache heads
+ *   [i nkv, (i + 1) nkv); position[i] = -1 is an idle slot and writes nothing. With q (bf16 [m][ldq], nq heads) the
+ *   decode step's prologue runs first: q/k RMSNorm (weights nullable) and RoPE (nullable tables bf16 [rows][d/2],
+ *   rows >= rope_base + cap; the angle is that of position rope_base + slot) at the rounding points of
+ *   egpt_qk_norm_rope_kv_append, rotated q to q_out [m][ldqo] (zeros for an idle row), and the codes are those of the
+ *   bf16 rows that call would cache. Slots outside the cache: EGPT_ERR_SHAPE through egpt_device_error.
+ * egpt_kv_read_q8: k_out, v_out [heads][count][d] (bf16 or fp32, out_head_stride elements between heads) = the values
+ *   of rows start .. start + count - 1. With starts (device int64, one per heads_per_start heads) rows begin at
+ *   start + starts[h / heads_per_start]; slots outside the cache then read as zeros.
+ * egpt_attn_decode_q8: out[i, h] = softmax(scale * q[i, h] . K_i) V_i over the L_i = position[i] + 1 keys of sequence
+ *   i's own cache (heads [i nkv, (i + 1) nkv)); position[i] = -1 (an idle slot) gives zeros. q, out bf16 rows
+ *   (16-byte aligned), m <= 512 sequences, at most 16 query heads per kv head.
+ * egpt_attn_shared_prefix: the same over prefix_len keys that all m sequences share (caches [nkv][prefix_cap][d]) and
+ *   then sequence i's own position[i] + 1 keys (its tail; position counts the tail's slots). cache_dtype EGPT_I8, or
+ *   EGPT_BF16 with all scales NULL, for prefix and tails alike. The prefix is read once for the whole batch.
+ * The work is cut into equal parts on the device, so a captured graph follows the positions. ws holds
+ * egpt_attn_q8_ws_bytes(m, nq, nkv, d) bytes, 16-byte aligned, zero-filled once; calls that can overlap on the GPU
+ * need workspaces of their own. Scores, sums and accumulators are fp32, one rounding of the output. */
+EGPT_API int egpt_kv_append_q8(int8_t *k_cache, float *k_scale, int8_t *v_cache, float *v_scale, int64_t cap,
+                               const void *k, int64_t ldk, const void *v, int64_t ldv, const int64_t *position,
+                               int64_t m, int nkv, int d, int dtype, void *q_out, int64_t ldqo, const void *q,
+                               int64_t ldq, int nq, const void *q_norm_w, const void *k_norm_w, float eps,
+                               const void *rope_cos, const void *rope_sin, int64_t rope_base, unsigned flags,
+                               void *stream);
+EGPT_API int egpt_kv_read_q8(void *k_out, void *v_out, int64_t out_head_stride, int dtype, const int8_t *k_cache,
+                             const float *k_scale, const int8_t *v_cache, const float *v_scale, int64_t cap,
+                             int64_t heads, int d, int64_t start, const int64_t *starts, int heads_per_start,
+                             int64_t count, unsigned flags, void *stream);
+EGPT_API size_t egpt_attn_q8_ws_bytes(int64_t m, int nq, int nkv, int d);
+EGPT_API int egpt_attn_decode_q8(void *out, int64_t ldo, const void *q, int64_t ldq, const int8_t *k_cache,
+                                 const float *k_scale, const int8_t *v_cache, const float *v_scale, int64_t cap,
+                                 const int64_t *position, int64_t m, int nq, int nkv, int d, float scale, void *ws,
+                                 size_t ws_bytes, unsigned flags, void *stream);
+EGPT_API int egpt_attn_shared_prefix(void *out, int64_t ldo, const void *q, int64_t ldq, const void *pk,
+                                     const float *pk_scale, const void *pv, const float *pv_scale, int64_t prefix_cap,
+                                     int64_t prefix_len, const void *tk, const float *tk_scale, const void *tv,
+                                     const float *tv_scale, int64_t cap, const int64_t *position, int64_t m, int nq,
+                                     int nkv, int d, float scale, int cache_dtype, void *ws, size_t ws_bytes,
+                                     unsigned flags, void *stream);
 
 /* ---- argmax over rows of bf16/fp32 logits -----------------------------------------------------------
  * replaces: logits[:, -1].argmax(-1) (research/realmodel/fast_decode.py:48,84): first index on ties. */
