@@ -47,6 +47,8 @@ struct Params {
   int m, nkv, group, row_tiles;  // row_tiles: 16-row tiles of a kv head's (sequence, head) rows under the prefix
   float scale_log2;
   float *ws;       // partial records
+  const float *pre;  // records of attn_prefix_kernel (null: the prefix's segments are in the flat list)
+  int pre_seqs, pre_tiles, pre_pairs, pre_ranges;
   unsigned *cnt;   // arrivals per (sequence, kv head); zero between calls
 };
 
@@ -609,19 +611,28 @@ __global__ void __launch_bounds__(kThreads) combine_kernel(const Params p, int g
   float M = -INFINITY, lsum = 0.f, a[N];
 #pragma unroll
   for (int e = 0; e < N; ++e) a[e] = 0.f;
+  auto add_record = [&](const float *rec, int rows, int r) {
+    const float mc = __ldcg(rec + rows * D + r), lc = __ldcg(rec + rows * D + rows + r);
+    if (lc == 0.f) return;  // no keys: nothing was accumulated
+    const float m_new = fmaxf(M, mc), mz = m_new == -INFINITY ? 0.f : m_new;
+    const float fo = ex2(M - mz), fc = ex2(mc - mz);
+    M = m_new;
+    lsum = lsum * fo + lc * fc;
+#pragma unroll
+    for (int e = 0; e < N; ++e) a[e] = a[e] * fo + __ldcg(rec + r * D + lane + 32 * e) * fc;
+  };
   auto add = [&](const Seg &s, int r) {
     if (s.start >= s.end) return;
-    for (int c = s.start / lay.chunk; c <= (s.end - 1) / lay.chunk; ++c) {
-      const float *rec = record<D>(p, c + s.index);
-      const float mc = __ldcg(rec + kRows * D + r), lc = __ldcg(rec + kRows * D + kRows + r);
-      const float m_new = fmaxf(M, mc), mz = m_new == -INFINITY ? 0.f : m_new;
-      const float fo = ex2(M - mz), fc = ex2(mc - mz);
-      M = m_new;
-      lsum = lsum * fo + lc * fc;
-#pragma unroll
-      for (int e = 0; e < N; ++e) a[e] = a[e] * fo + __ldcg(rec + r * D + lane + 32 * e) * fc;
-    }
+    for (int c = s.start / lay.chunk; c <= (s.end - 1) / lay.chunk; ++c) add_record(record<D>(p, c + s.index), kRows, r);
   };
+  if (D == apx::kD && p.pre) {
+    const int tile = i / p.pre_seqs, pair = tile / 2;
+    const bool two = 2 * pair + 1 < p.pre_tiles;  // the pair's streams are two tiles, or both this one
+    const float *rec = p.pre + (int64_t)(g * p.pre_pairs + pair) * p.pre_ranges * 2 * apx::kRecord;
+    for (int c = 0; c < 2 * p.pre_ranges; ++c)
+      if (!two || (c & 1) == (tile & 1))
+        add_record(rec + (int64_t)c * apx::kRecord, apx::kRowsT, (i % p.pre_seqs) * p.group + j);
+  }
   if (lay.prefix_segs) {
     const int flat = i * p.group + j;
     add(prefix_seg(p, lay, g * p.row_tiles + flat / kRows), flat % kRows);
@@ -658,6 +669,10 @@ static cudaError_t launch_d(const Params &p, int d, cudaStream_t st, bool pdl) {
                   : (d == 64 ? launch<64, Q8, NR, SHARED>(p, st, pdl) : launch<32, Q8, NR, SHARED>(p, st, pdl));
 }
 
+// Whether the prefix goes to attn_prefix_kernel: bf16, head_dim 128, more rows than one tile of the mma.sync kernel.
+static bool prefix_on_tcgen05(const Params &p, int d, bool q8) {
+  return !q8 && d == apx::kD && p.prefix > 0 && p.scale_log2 > 0.f && p.m * p.group > kRows;
+}
 static int row_tiles(int64_t m, int group) { return (int)((m * group + kRows - 1) / kRows); }
 static size_t counter_bytes(int64_t m, int nkv) { return ((size_t)m * nkv * 4 + 255) / 256 * 256; }
 
@@ -687,7 +702,8 @@ extern "C" size_t egpt_attn_q8_ws_bytes(int64_t m, int nq, int nkv, int d) {
   if (m < 1 || nkv < 1 || nq < nkv || d < 1) return 0;
   // counters, then a record for every (CTA, segment) pair: CTA c and segment s keep theirs at c + s
   const size_t records = (size_t)2 * num_sms() + (size_t)nkv * aq8::row_tiles(m, nq / nkv) + (size_t)m * nkv;
-  return aq8::counter_bytes(m, nkv) + std::max(records, (size_t)4 * num_sms()) * aq8::kRows * ((size_t)d + 2) * 4;
+  const size_t prefix = d == apx::kD && nq / nkv <= aq8::kRows ? apx::record_floats(m, nq / nkv, nkv) * 4 : 0;
+  return aq8::counter_bytes(m, nkv) + std::max(records, (size_t)4 * num_sms()) * aq8::kRows * ((size_t)d + 2) * 4 + prefix;
 }
 
 extern "C" int egpt_attn_decode_q8(void *out, int64_t ldo, const void *q, int64_t ldq, const int8_t *k_cache,
@@ -740,6 +756,22 @@ extern "C" int egpt_attn_shared_prefix(void *out, int64_t ldo, const void *q, in
   const bool pdl = (flags & EGPT_FLAG_PDL) != 0;
   const cudaStream_t st = (cudaStream_t)stream;
   cudaError_t e;
+  if (aq8::prefix_on_tcgen05(p, d, q8)) {
+    apx::Args A{};
+    const apx::Shape sh = apx::shape_of(m, p.group, nkv, prefix_len);
+    // its records lie behind those of the tails
+    const size_t head = egpt_attn_q8_ws_bytes(m, nq, nkv, d) - apx::record_floats(m, p.group, nkv) * 4;
+    A.ws = (float *)((char *)ws + head);
+    A.prefix = prefix_len, A.m = (int)m, A.nkv = nkv, A.group = p.group, A.scale_log2 = p.scale_log2;
+    bool maps_ok = false;
+    e = apx::launch(A, q, ldq, pk, pv, prefix_cap, sh, st, pdl, maps_ok);
+    if (!maps_ok) return set_error(EGPT_ERR_ALIGN, "attn_shared_prefix: tensor maps rejected");
+    if (e != cudaSuccess) return check_launch(e, "attn_prefix_kernel");
+    p.pre = A.ws, p.pre_seqs = sh.seqs, p.pre_tiles = sh.tiles, p.pre_pairs = sh.pairs, p.pre_ranges = sh.ranges;
+    p.prefix = 0;  // what is left in the flat list are the tails
+    e = p.group <= 8 ? aq8::launch<128, false, 8, true>(p, st, true) : aq8::launch<128, false, 16, true>(p, st, true);
+    return check_launch(e, "attn_shared_prefix_kernel");
+  }
   if (m * p.group <= 8) e = q8 ? aq8::launch_d<true, 8, true>(p, d, st, pdl) : aq8::launch_d<false, 8, true>(p, d, st, pdl);
   else e = q8 ? aq8::launch_d<true, 16, true>(p, d, st, pdl) : aq8::launch_d<false, 16, true>(p, d, st, pdl);
   return check_launch(e, "attn_shared_prefix_kernel");
