@@ -8,14 +8,21 @@
 //
 // Work: a segment is one cache head with the query rows that read it: (i, g) with the group's rows for a sequence's
 // own cache, (g, 16 query rows) for the shared prefix, whose rows are all (sequence, head) pairs of kv head g in a
-// row. A segment's keys are cut into tiles of kTile keys and all tiles of the call into equal contiguous ranges, one
-// per CTA: a batch of one token next to a document leaves no CTA idle, and no length is known to the host. Within a
-// range a warp takes every fourth tile through a ring of its own in shared memory (cp.async, rows past the
-// segment's end filled with zeros), so warps only meet at a segment's end.
+// row. A segment's keys are cut into tiles of kTile keys and the tiles of a launch into contiguous ranges, one per CTA,
+// on the device, so no length is known to the host. Where the segments allow it ranges are parts of one
+// segment each (split by the smallest range length that gives every CTA at most one); else they are equal
+// stretches of the flat list of all tiles and may hold several segments, so that a batch of one token next to a document
+// leaves no CTA idle. Within a range a warp takes every kWarps-th tile through a ring of its own in shared memory
+// (cp.async, rows past the segment's end filled with zeros), so warps only meet at a segment's end.
 //
-// Arithmetic: mma.sync m16n8k16 with the query rows as M. Scores of int8 keys: the codes become f16 exactly (0x6400 |
-// (q + 128) is 1152 + q), and q, scaled by a power of two per row to at most 2^15, too, so the scores are those of the
-// codes in fp32 and ks_j multiplies them. P.V is in bf16, whose exponents hold every weight times vs_j; its 8 bits
+// A prefix runs first, in a launch of its own that leaves partial records (here, or in attn_prefix.cu); the launch over
+// the sequences' own keys is a dependent one that starts beside it and waits only before it adds those records up.
+//
+// Arithmetic: mma.sync with the query rows as M. Scores of int8 keys, up to 8 rows: q as fixed point X 2^(e - 29), |X| <=
+// 2^30, in four balanced base-256 digits, two of them in the MMA's rows 0-7 and 8-15, so two int8 MMAs per 32 dims
+// give the exact dot products with the codes as they lie in memory, and ks_j multiplies their fp32 value. 16 rows: the
+// codes become f16 exactly (0x6400 | (q + 128) is 1152 + q), and q, scaled by a power of two per row to at most 2^15,
+// too, so the sums are those of the codes in fp32. P.V is in bf16, whose exponents hold every weight times vs_j; its 8 bits
 // would cost a weight 2^-9 of itself, so a weight enters as the sum of two bf16 values (16 bits). With 8 query rows
 // or fewer the second values ride in the MMA's upper 8 rows, which are idle otherwise; 16 rows take a second MMA.
 // Codes become bf16 exactly as (128 + low seven bits) - (128 + sign bit). Sums, maxima and accumulators are fp32; the
@@ -29,7 +36,9 @@ namespace aq8 {
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kMaxBatch = 512;
-constexpr int kRows = 16;  // query rows per tile (the M of the MMA), and rows of a partial record
+constexpr int kRows = 16;              // query rows per tile (the M of the MMA), and rows of a partial record
+constexpr int kCtasPerSm = 2;
+constexpr int kMinChunk = 2 * kWarps;  // tiles of a range at least
 
 struct Cache {
   const uint8_t *k, *v;
@@ -37,29 +46,35 @@ struct Cache {
   int64_t cap;
 };
 
+// The prefix's partial records, by the kernel that made them.
+struct Prefix {
+  const float *rec;                // null: no prefix
+  int big;                         // 1: attn_prefix_kernel's
+  int seqs, tiles, pairs, ranges;  // its shape
+  int row_tiles, pad, chunk, seg_tiles;  // else the list of prefix segments, cut as below
+};
+
 struct Params {
   uint16_t *out;
   const uint16_t *q;
   int64_t ldo, ldq;
-  Cache own, shared;
-  int64_t prefix;  // keys of the shared prefix (0: none)
+  Cache cache;
   const int64_t *position;
-  int m, nkv, group, row_tiles;  // row_tiles: 16-row tiles of a kv head's (sequence, head) rows under the prefix
+  int m, nkv, group;
   float scale_log2;
-  float *ws;       // partial records
-  const float *pre;  // records of attn_prefix_kernel (null: the prefix's segments are in the flat list)
-  int pre_seqs, pre_tiles, pre_pairs, pre_ranges;
-  unsigned *cnt;   // arrivals per (sequence, kv head); zero between calls
+  float *ws;      // partial records of this launch
+  unsigned *cnt;  // arrivals per (sequence, kv head); zero between calls
+  int keys;       // keys of the shared prefix (the launch over it)
+  Prefix pre;     // of the launch over the sequences' own keys: records to add up; of the prefix's: how it is cut
 };
 
-// Where the tiles of the call lie in its flat list: the prefix's segments first, then the sequences'.
+// How the tiles of the launch are cut: a segment takes up round_up(tiles, pad) places of the flat list, a CTA `chunk`.
 struct Layout {
-  int prefix_tiles, prefix_segs, prefix_end;  // tiles per prefix segment, its segments, and the list's place after them
-  int total, chunk;                           // tiles of the call, tiles per CTA
+  int total, chunk, pad;  // pad = chunk: every range lies in one segment; pad = 1: equal stretches
 };
 struct Seg {
   int index, start, end;  // its number and its tiles in the flat list
-  int seq, g, tile;       // sequence (-1: prefix), kv head, row tile
+  int seq, g, tile;       // sequence, kv head; row tile (prefix)
   int len;                // keys
 };
 
@@ -86,11 +101,14 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ void cp16(void *dst, const void *src, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes) : "memory");
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ void cp4(void *dst, const void *src, int bytes) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes) : "memory");
+__device__ __forceinline__ void cp16z(uint32_t dst, const void *src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp4(uint32_t dst, const void *src, int bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -118,6 +136,11 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_i8(int (&c)[4], const uint32_t *a, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
 // The f16 values of two bytes of (codes ^ 0x80): bytes 0x64 above them make 1024 + byte, less 1152 the code, exactly.
 __device__ __forceinline__ uint32_t codes_f16(uint32_t biased, uint32_t select) {
   uint32_t r;
@@ -137,80 +160,107 @@ __device__ __forceinline__ uint32_t codes_bf16(uint32_t codes, uint32_t select) 
 
 __device__ __forceinline__ int seq_len(const Params &p, int i) {
   const int64_t pos = p.position[i];
-  if (pos < -1 || pos >= p.own.cap) {
+  if (pos < -1 || pos >= p.cache.cap) {
     set_device_error(EGPT_ERR_SHAPE);
     return 0;
   }
   return (int)(pos + 1);
 }
 
-// cum[i] = tiles of the sequences before i (one kv head); every thread of the CTA (kThreads) calls it.
+__host__ __device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
+
+// Tiles of an equal stretch: not below the segments' average, up to kMinChunk (splitting a short segment costs more in
+// adding the parts up than it gains).
+__host__ __device__ __forceinline__ int even_share(int tiles, int segs, int grid) {
+  const int least = ceil_div(tiles, segs) < kMinChunk ? ceil_div(tiles, segs) : kMinChunk;
+  const int share = ceil_div(tiles, grid);
+  return share > least ? share : (least > 1 ? least : 1);
+}
+// cum[i] = places of the sequences before i (one kv head). The ranges: with up to 32 sequences the lanes try range lengths
+// from the even share of the tiles up to 1.5 times it, and the smallest that gives at most one range per CTA is taken;
+// failing that, and for more sequences, even shares. Every thread of the CTA calls it.
 template <int TILE>
 __device__ Layout make_layout(const Params &p, int *cum, int *scratch) {
-  constexpr int kPer = kMaxBatch / kThreads;
-  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-  int tiles[kPer], sum = 0;
-#pragma unroll
-  for (int e = 0; e < kPer; ++e) {
-    const int i = t * kPer + e;
-    tiles[e] = i < p.m ? (seq_len(p, i) + TILE - 1) / TILE : 0;
-    sum += tiles[e];
-  }
-  int inc = sum;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int up = __shfl_up_sync(0xffffffffu, inc, o);
-    if (lane >= o) inc += up;
-  }
-  if (lane == 31) scratch[warp] = inc;
-  __syncthreads();
-  int before = inc - sum;
-  for (int w = 0; w < warp; ++w) before += scratch[w];
-#pragma unroll
-  for (int e = 0; e < kPer; ++e) {
-    if (t * kPer + e <= p.m) cum[t * kPer + e] = before;
-    before += tiles[e];
-  }
-  if (t == kThreads - 1) cum[kMaxBatch] = before;
-  __syncthreads();
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5, grid = (int)gridDim.x;
   Layout l;
-  l.prefix_tiles = (int)((p.prefix + TILE - 1) / TILE);
-  l.prefix_segs = l.prefix_tiles ? p.nkv * p.row_tiles : 0;
-  l.prefix_end = l.prefix_segs * l.prefix_tiles;
-  l.total = l.prefix_end + p.nkv * cum[p.m];
-  l.chunk = max((l.total + (int)gridDim.x - 1) / (int)gridDim.x, kWarps);
+  if (p.m <= 32) {  // every warp for itself
+    const int tiles = lane < p.m ? ceil_div(seq_len(p, lane), TILE) : 0;
+    const int all = p.nkv * __reduce_add_sync(0xffffffffu, tiles);
+    const int least = max(kMinChunk, ceil_div(all, grid)), len = least + ceil_div(least * lane, 64);
+    int parts = 0;
+    for (int i = 0; i < p.m; ++i) parts += ceil_div(__shfl_sync(0xffffffffu, tiles, i), len);
+    const unsigned fits = __ballot_sync(0xffffffffu, p.nkv * parts <= grid);
+    l.chunk = fits ? __shfl_sync(0xffffffffu, len, __ffs(fits) - 1) : even_share(all, p.nkv * p.m, grid);
+    l.pad = fits ? l.chunk : 1;
+    const int places = ceil_div(tiles, l.pad) * l.pad;
+    int inc = places;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += up;
+    }
+    if (warp == 0) {
+      cum[lane] = inc - places;
+      if (lane == 31) cum[32] = inc;
+    }
+    __syncthreads();
+  } else {
+    constexpr int kPer = kMaxBatch / kThreads;
+    int tiles[kPer], sum = 0;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      const int i = t * kPer + e;
+      tiles[e] = i < p.m ? ceil_div(seq_len(p, i), TILE) : 0;
+      sum += tiles[e];
+    }
+    int inc = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += up;
+    }
+    if (lane == 31) scratch[warp] = inc;
+    __syncthreads();
+    int before = inc - sum;
+    for (int w = 0; w < warp; ++w) before += scratch[w];
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      cum[t * kPer + e] = before;
+      before += tiles[e];
+    }
+    if (t == kThreads - 1) cum[kMaxBatch] = before;
+    __syncthreads();
+    l.pad = 1;
+    l.chunk = even_share(p.nkv * cum[p.m], p.nkv * p.m, grid);
+  }
+  l.total = p.nkv * cum[p.m];
   return l;
 }
-__device__ __forceinline__ Seg own_seg(const Params &p, const Layout &l, const int *cum, int i, int g) {
-  Seg s;
-  const int tiles = cum[i + 1] - cum[i];
-  s.index = l.prefix_segs + i * p.nkv + g;
-  s.start = l.prefix_end + p.nkv * cum[i] + g * tiles;
-  s.end = s.start + tiles;
-  s.seq = i, s.g = g, s.tile = 0;
-  s.len = (int)p.position[i] + 1;
-  return s;
-}
-__device__ __forceinline__ Seg prefix_seg(const Params &p, const Layout &l, int index) {
-  Seg s;
-  s.index = index;
-  s.start = index * l.prefix_tiles, s.end = s.start + l.prefix_tiles;
-  s.seq = -1, s.g = index / p.row_tiles, s.tile = index % p.row_tiles;
-  s.len = (int)p.prefix;
-  return s;
-}
-// The segment that holds tile x < total.
+// The segment that holds place x < total.
+template <int TILE, bool PREFIX>
 __device__ __forceinline__ Seg find_seg(const Params &p, const Layout &l, const int *cum, int x) {
-  if (x < l.prefix_end) return prefix_seg(p, l, x / l.prefix_tiles);
-  int lo = 0, hi = p.m - 1;  // the last sequence whose tiles start at or before x and that has any
-  const int y = x - l.prefix_end;
+  Seg s;
+  if (PREFIX) {
+    const int places = ceil_div(p.pre.seg_tiles, l.pad) * l.pad;
+    s.index = x / places;
+    s.start = s.index * places, s.end = s.start + p.pre.seg_tiles;
+    s.seq = -1, s.g = s.index / p.pre.row_tiles, s.tile = s.index % p.pre.row_tiles;
+    s.len = p.keys;
+    return s;
+  }
+  int lo = 0, hi = p.m - 1;  // the last sequence whose places start at or before x: it has some
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (p.nkv * cum[mid] <= y) lo = mid;
+    if (p.nkv * cum[mid] <= x) lo = mid;
     else hi = mid - 1;
   }
-  const int tiles = cum[lo + 1] - cum[lo];
-  return own_seg(p, l, cum, lo, (y - p.nkv * cum[lo]) / tiles);
+  const int places = cum[lo + 1] - cum[lo];
+  s.seq = lo, s.g = (x - p.nkv * cum[lo]) / places, s.tile = 0;
+  s.index = lo * p.nkv + s.g;
+  s.start = p.nkv * cum[lo] + s.g * places;
+  s.len = (int)p.position[lo] + 1;
+  s.end = s.start + ceil_div(s.len, TILE);
+  return s;
 }
 // A partial record: kRows rows of (D accumulators), then kRows maxima and kRows sums.
 template <int D>
@@ -218,64 +268,193 @@ __device__ __forceinline__ float *record(const Params &p, int index) {
   return p.ws + (int64_t)index * kRows * (D + 2);
 }
 
+// What one (sequence, head) row's parts add up to, one warp per row or per share of a row's records.
+template <int D>
+struct Finish {
+  float m[kRows], l[kRows];
+  float a[kRows][D];
+};
+
 template <int D, bool Q8, int NR, int STAGES>
 struct Smem {
   uint8_t ring[kWarps][STAGES][Geo<D, Q8>::kStageBytes];
-  float merge[2][NR / 8 * (D / 4 + 2)][32];  // two warps' accumulators, maxima and sums
+  union {
+    float merge[kWarps / 2][NR / 8 * (D / 4 + 2)][32];  // half of the warps' accumulators, maxima and sums
+    Finish<D> fin;
+  };
   int cum[kMaxBatch + 1];
   int scratch[kWarps];
   int last;
 };
 
-// NR: query rows in use, 8 or 16. SHARED: segments of the prefix as well, and every (CTA, segment) pair leaves a record
-// for combine_kernel; else one CTA's segment goes straight to the output and the last CTA of a split one combines it.
-template <int D, bool Q8, int NR, bool SHARED, int STAGES>
+// out[i, heads of g] = the own_n records of the sequence's own keys (the first in slot `first`, then slots
+// 2 (c0 + k)) and the prefix's, added up. A warp takes a row, or with fewer rows than warps every parts-th record of a
+// row: lanes read up to 32 records' maxima and sums at once, then the accumulators follow with independent loads. The
+// order is fixed by the shapes. Every thread of the CTA calls it.
+template <int D>
+__device__ void finish(const Params &p, Finish<D> &f, int i, int g, int own_n, int first, int c0) {
+  constexpr int N = D / 32;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int parts = max(1, kWarps / p.group);
+  if (p.pre.rec) pdl_wait();  // the launch over the prefix has finished
+  for (int unit = warp; unit < p.group * parts; unit += kWarps) {
+    const int j = unit % p.group, part = unit / p.group;
+    int pre_n = 0, pre_row = 0, pre_rows = kRows;
+    int64_t pre_step = 0;
+    const float *pre0 = nullptr;
+    if (p.pre.rec) {
+      if (p.pre.big) {
+        const int tile = i / p.pre.seqs, pair = tile / 2;
+        const bool two = 2 * pair + 1 < p.pre.tiles;  // the pair's streams are two tiles, or both this one
+        pre_n = two ? p.pre.ranges : 2 * p.pre.ranges;
+        pre_step = two ? 2 * apx::kRecord : apx::kRecord;
+        pre0 = p.pre.rec + ((int64_t)(g * p.pre.pairs + pair) * p.pre.ranges * 2 + (two ? tile & 1 : 0)) * apx::kRecord;
+        pre_row = (i % p.pre.seqs) * p.group + j, pre_rows = apx::kRowsT;
+      } else {
+        const int flat = i * p.group + j, seg = g * p.pre.row_tiles + flat / kRows;
+        const int start = seg * ceil_div(p.pre.seg_tiles, p.pre.pad) * p.pre.pad;
+        const int pc0 = start / p.pre.chunk;
+        pre_n = (start + p.pre.seg_tiles - 1) / p.pre.chunk - pc0 + 1;
+        pre_step = kRows * (D + 2);
+        pre0 = p.pre.rec + (int64_t)(pc0 + seg) * pre_step;
+        pre_row = flat % kRows;
+      }
+    }
+    const int n = own_n + pre_n;
+    float M = -INFINITY, lsum = 0.f, a[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) a[e] = 0.f;
+    for (int k0 = part; k0 < n; k0 += 32 * parts) {
+      const int k = k0 + lane * parts;
+      const float *row = p.ws;
+      float mk = -INFINITY, lk = 0.f;
+      if (k < n) {
+        const bool own = k < own_n;
+        const int rows = own ? kRows : pre_rows, r = own ? j : pre_row;
+        const float *rec = own ? p.ws + (int64_t)(k == 0 ? first : 2 * (c0 + k)) * kRows * (D + 2)
+                               : pre0 + (int64_t)(k - own_n) * pre_step;
+        mk = __ldcg(rec + rows * D + r), lk = __ldcg(rec + rows * D + rows + r);
+        row = rec + r * D;
+      }
+      const float mx = fmaxf(M, warp_max(lk != 0.f ? mk : -INFINITY));
+      const float mz = mx == -INFINITY ? 0.f : mx;
+      const float fk = lk != 0.f ? ex2(mk - mz) : 0.f, fo = ex2(M - mz);  // a record without keys has no accumulators
+      M = mx;
+      lsum = lsum * fo + warp_sum(lk * fk);
+#pragma unroll
+      for (int e = 0; e < N; ++e) a[e] *= fo;
+      const int cnt = min(32, ceil_div(n - k0, parts));
+#pragma unroll 4
+      for (int c = 0; c < cnt; ++c) {
+        const float fc = __shfl_sync(0xffffffffu, fk, c);
+        const float *src = (const float *)__shfl_sync(0xffffffffu, (unsigned long long)row, c) + N * lane;
+        float v[N];
+        if constexpr (N == 4) {
+          const float4 t = __ldcg((const float4 *)src);
+          v[0] = t.x, v[1] = t.y, v[2] = t.z, v[3] = t.w;
+        } else if constexpr (N == 2) {
+          const float2 t = __ldcg((const float2 *)src);
+          v[0] = t.x, v[1] = t.y;
+        } else {
+          v[0] = __ldcg(src);
+        }
+#pragma unroll
+        for (int e = 0; e < N; ++e) a[e] += fc == 0.f ? 0.f : v[e] * fc;
+      }
+    }
+    if (parts > 1) {
+      if (lane == 0) f.m[unit] = M, f.l[unit] = lsum;
+#pragma unroll
+      for (int e = 0; e < N; ++e) f.a[unit][N * lane + e] = a[e];
+    } else {
+      const float inv = lsum == 0.f ? 0.f : 1.f / lsum;  // no keys at all: zeros
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        p.out[i * p.ldo + (int64_t)(g * p.group + j) * D + N * lane + e] = f32_to_bf16_bits(a[e] * inv);
+    }
+  }
+  if (parts == 1) return;
+  __syncthreads();
+  for (int e = threadIdx.x; e < p.group * D; e += kThreads) {
+    const int j = e / D, dd = e - j * D;
+    float M = -INFINITY, lsum = 0.f, a = 0.f;
+    for (int part = 0; part < parts; ++part) M = fmaxf(M, f.m[part * p.group + j]);
+    const float mz = M == -INFINITY ? 0.f : M;
+    for (int part = 0; part < parts; ++part) {
+      const float fp = ex2(f.m[part * p.group + j] - mz);
+      lsum += f.l[part * p.group + j] * fp;
+      a += f.a[part * p.group + j][dd] * fp;
+    }
+    p.out[i * p.ldo + (int64_t)(g * p.group + j) * D + dd] = f32_to_bf16_bits(lsum == 0.f ? 0.f : a / lsum);
+  }
+  __syncthreads();  // f is free again
+}
+
+// NR: query rows in use, 8 or 16. PREFIX: the segments of the shared prefix, every (CTA, segment) pair leaving a record in
+// slot CTA + segment; else the sequences' own keys, a CTA's at most two split segments leaving theirs in slots 2 CTA
+// and 2 CTA + 1, and the last CTA of a segment adding all of it up.
+template <int D, bool Q8, int NR, bool PREFIX, int STAGES>
 __global__ void __launch_bounds__(kThreads) attn_kernel(const Params p) {
   using G = Geo<D, Q8>;
   using S = Smem<D, Q8, NR, STAGES>;
   constexpr int TILE = G::kTile, NT = TILE / 8, ND = D / 8, NC = NR == 16 ? 4 : 2;  // NC: accumulators kept
+  constexpr bool PLANES = Q8 && NR == 8;  // scores by int8 MMAs on the digits of q
   extern __shared__ __align__(16) uint8_t smem_raw[];
   S &sm = *(S *)smem_raw;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  pdl_wait();
+  // beside the prefix's launch only finish() waits: what precedes that launch is done once it has started
+  if (PREFIX || !p.pre.rec) pdl_wait();
   pdl_launch_dependents();
-  const Layout lay = make_layout<TILE>(p, sm.cum, sm.scratch);
-
-  if (!SHARED)  // sequences without keys
-    for (int i = blockIdx.x; i < p.m; i += gridDim.x)
-      if (sm.cum[i + 1] == sm.cum[i])
-        for (int e = threadIdx.x; e < p.nkv * p.group * D; e += kThreads) p.out[i * p.ldo + e] = 0;
-
+  Layout lay;
+  if (PREFIX) {
+    lay.chunk = p.pre.chunk, lay.pad = p.pre.pad;
+    lay.total = p.nkv * p.pre.row_tiles * ceil_div(p.pre.seg_tiles, lay.pad) * lay.pad;
+  } else {
+    lay = make_layout<TILE>(p, sm.cum, sm.scratch);
+    for (int e = blockIdx.x; e < p.m * p.nkv; e += gridDim.x)  // sequences without keys of their own
+      if (sm.cum[e / p.nkv + 1] == sm.cum[e / p.nkv]) finish<D>(p, sm.fin, e / p.nkv, e % p.nkv, 0, 0, 0);
+  }
   const int x0 = (int)min((int64_t)lay.total, (int64_t)blockIdx.x * lay.chunk);
-  const int x1 = (int)min((int64_t)lay.total, (int64_t)x0 + lay.chunk);
-  if (x0 >= x1) return;
+  if (x0 >= lay.total) return;
+  Seg seg = find_seg<TILE, PREFIX>(p, lay, sm.cum, x0);
+  const int x1 = min(lay.pad > 1 ? seg.end : lay.total, x0 + lay.chunk);
 
-  // ---- this warp's loads: every fourth tile of the range, STAGES - 1 tiles ahead
+  // ---- this warp's loads: every kWarps-th tile of the range, STAGES - 1 tiles ahead. 32 lanes take 512 consecutive bytes
+  // of a full tile at a time; the swizzles split into a part of the lane and one of the step.
   int lx = x0 + warp, lcount = 0;
-  Seg ls = find_seg(p, lay, sm.cum, min(lx, x1 - 1));
+  Seg ls = seg;
+  constexpr int kStep = 32 / G::kChunks;  // rows per 512 bytes
+  const int lr = lane / G::kChunks, lc = lane % G::kChunks;
+  const uint32_t ring = smem_u32(sm.ring[warp][0]);
+  const uint32_t k_dst = ring + lr * G::kRowBytes + ((lc ^ G::k_swz(lr)) * 16);
+  const uint32_t v_dst = lr * G::kRowBytes + ((lc ^ G::v_swz(lr)) * 16);
   auto load_next = [&]() {
     if (lx < x1) {
-      if (lx >= ls.end) ls = find_seg(p, lay, sm.cum, lx);
-      uint8_t *st = sm.ring[warp][lcount % STAGES];
-      const bool shared = SHARED && ls.seq < 0;
-      const Cache &c = shared ? p.shared : p.own;
-      const int64_t head = shared ? ls.g : (int64_t)ls.seq * p.nkv + ls.g;
-      const int key0 = (lx - ls.start) * TILE;
-      const int64_t row0 = head * c.cap + key0;
-      const uint8_t *kb = c.k + row0 * G::kRowBytes, *vb = c.v + row0 * G::kRowBytes;
+      if (lx >= ls.end) ls = find_seg<TILE, PREFIX>(p, lay, sm.cum, lx);
+      const uint32_t st = (uint32_t)((lcount % STAGES) * G::kStageBytes);
+      const Cache &c = p.cache;
+      const int key0 = (lx - ls.start) * TILE, left = ls.len - key0;
+      const int64_t row0 = (PREFIX ? ls.g : (int64_t)ls.seq * p.nkv + ls.g) * c.cap + key0;
+      const uint8_t *kb = c.k + row0 * G::kRowBytes + lane * 16, *vb = c.v + row0 * G::kRowBytes + lane * 16;
 #pragma unroll
-      for (int it = 0; it < TILE * G::kChunks / 32; ++it) {
-        const int i = it * 32 + lane, r = i / G::kChunks, ch = i % G::kChunks;
-        const bool in = key0 + r < ls.len;
-        const int64_t off = in ? (int64_t)r * G::kRowBytes + ch * 16 : 0;
-        cp16(st + r * G::kRowBytes + ((ch ^ G::k_swz(r)) * 16), kb + off, in ? 16 : 0);
-        cp16(st + TILE * G::kRowBytes + r * G::kRowBytes + ((ch ^ G::v_swz(r)) * 16), vb + off, in ? 16 : 0);
+      for (int it = 0; it < TILE / kStep; ++it) {
+        // v_swz(it kStep + lr) = v_swz(it kStep) ^ v_swz(lr) (the row bits it uses do not carry)
+        const uint32_t kd = st + k_dst + it * 512;
+        const uint32_t vd = st + ring + TILE * G::kRowBytes + (v_dst ^ (G::v_swz(it * kStep) * 16)) + it * 512;
+        if (left >= TILE) {
+          cp16(kd, kb + it * 512);
+          cp16(vd, vb + it * 512);
+        } else {
+          const bool in = it * kStep + lr < left;
+          cp16z(kd, in ? kb + it * 512 : c.k, in ? 16 : 0);
+          cp16z(vd, in ? vb + it * 512 : c.v, in ? 16 : 0);
+        }
       }
       if (Q8) {
-        const bool in = lane < TILE && key0 + lane < ls.len;
-        float *sc = (float *)(st + 2 * TILE * G::kRowBytes);
-        cp4(sc + lane, c.ks + row0 + (in ? lane : 0), in ? 4 : 0);
-        cp4(sc + TILE + lane, c.vs + row0 + (in ? lane : 0), in ? 4 : 0);
+        const bool in = lane < left;
+        const uint32_t sc = ring + st + 2 * TILE * G::kRowBytes + lane * 4;
+        cp4(sc, c.ks + row0 + (in ? lane : 0), in ? 4 : 0);
+        cp4(sc + TILE * 4, c.vs + row0 + (in ? lane : 0), in ? 4 : 0);
       }
     }
     cp_commit();
@@ -286,54 +465,74 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const Params p) {
   for (int s = 0; s < STAGES - 1; ++s) load_next();
 
   int x = x0 + warp, ccount = 0;
-  Seg seg = find_seg(p, lay, sm.cum, x0);
   const int first_seg = seg.index;
   for (;;) {
-    // ---- the segment's query rows as MMA fragments: row r of the tile, dims d0 .. d0 + 3 of step w
-    uint32_t qa[D / 16][4];
-    float rowfac[2];  // scale log2(e), and for int8 the power of two that q was divided by
+    // ---- the segment's query rows as MMA fragments
+    uint32_t qa[PLANES ? D / 32 : D / 16][PLANES ? 8 : 4];
+    float rowfac[2] = {p.scale_log2, p.scale_log2};  // and for int8 the power of two that q was divided by
 #pragma unroll
-    for (int hh = 0; hh < 2; ++hh) {
+    for (int hh = 0; hh < NR / 8; ++hh) {
       const int r = g + 8 * hh;
       int64_t tok = -1;
       int h = 0;
-      if (SHARED && seg.seq < 0) {
+      if (PREFIX) {
         const int flat = seg.tile * kRows + r;
         if (flat < p.m * p.group) tok = flat / p.group, h = seg.g * p.group + flat % p.group;
       } else if (r < p.group) {
         tok = seg.seq, h = seg.g * p.group + r;
       }
-      const bool live = tok >= 0 && 8 * hh < NR;
-      const uint16_t *qr = p.q + (live ? tok * p.ldq + (int64_t)h * D : 0);
-      uint2 w[D / 16];
-      float amax = 0.f;
+      const uint16_t *qr = p.q + (tok >= 0 ? tok * p.ldq + (int64_t)h * D : 0);
+      uint2 w[D / 16];  // dims d0 .. d0 + 3 of every 16-dim step: those of the key words that this thread loads
+      uint32_t amax2 = 0u;  // the largest magnitudes of the even and odd elements, as bf16 bits (NaN above infinity)
 #pragma unroll
       for (int s = 0; s < D / 16; ++s) {
         const int d0 = Q8 ? (D == 32 ? 8 * t + 4 * s : 16 * (t + 4 * (s / 4)) + 4 * (s % 4))
                           : 8 * (t + 4 * (s / 2)) + 4 * (s % 2);
-        w[s] = live ? *(const uint2 *)(qr + d0) : make_uint2(0u, 0u);
-        if (Q8)
-          amax = fmaxf(amax, fmaxf(fmaxf(fabsf(bf16_lo(w[s].x)), fabsf(bf16_hi(w[s].x))),
-                                   fmaxf(fabsf(bf16_lo(w[s].y)), fabsf(bf16_hi(w[s].y)))));
+        w[s] = tok >= 0 ? *(const uint2 *)(qr + d0) : make_uint2(0u, 0u);
+        if (Q8) amax2 = __vmaxu2(amax2, __vmaxu2(w[s].x & 0x7fff7fffu, w[s].y & 0x7fff7fffu));
       }
-      rowfac[hh] = p.scale_log2;
       if (Q8) {
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-        // 2^e <= amax < 2^(e + 1) becomes 2^14 <= . < 2^15: bf16's 8 bits stay exact in f16 for elements down to
-        // 2^-28 of the row's largest. (The exponent is kept where both factors are normal numbers.)
-        const int e = min(max((int)(__float_as_uint(amax) >> 23) - 127, -112), 127);
-        const float up = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
-        rowfac[hh] *= __uint_as_float((uint32_t)(127 - 14 + e) << 23);
+        amax2 = __vmaxu2(amax2, __shfl_xor_sync(0xffffffffu, amax2, 1));
+        amax2 = __vmaxu2(amax2, __shfl_xor_sync(0xffffffffu, amax2, 2));
+        const int amax = (int)max(amax2 & 0xffffu, amax2 >> 16);
+        // a largest magnitude in [2^e, 2^(e + 1)) becomes one in [2^B, 2^(B + 1)): as fixed point (B = 29) bf16's 8 bits stay exact for
+        // elements down to 2^-22 of the row's largest, in f16 (B = 14) down to 2^-28. (The exponent is kept where both
+        // factors are normal numbers.)
+        constexpr int B = PLANES ? 29 : 14;
+        const int e = min(max((amax >> 7) - 127, B - 126), 127);
+        const float up = __uint_as_float((uint32_t)(127 + B - e) << 23);
+        rowfac[hh] *= __uint_as_float((uint32_t)(127 - B + e) << 23);
+        if (amax >= 0x7f80) rowfac[hh] = NAN;  // an infinity or NaN in the row: its scores are NaN
 #pragma unroll
         for (int s = 0; s < D / 16; ++s) {
-          qa[s][hh] = f16x2(bf16_lo(w[s].x) * up, bf16_hi(w[s].x) * up);
-          qa[s][hh + 2] = f16x2(bf16_lo(w[s].y) * up, bf16_hi(w[s].y) * up);
+          const float y[4] = {bf16_lo(w[s].x) * up, bf16_hi(w[s].x) * up, bf16_lo(w[s].y) * up, bf16_hi(w[s].y) * up};
+          if constexpr (PLANES) {
+            uint32_t d[4] = {0u, 0u, 0u, 0u};  // digit planes, lowest first: a byte for each of the four dims
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              int X = __float2int_rn(y[i]);
+#pragma unroll
+              for (int b = 0; b < 4; ++b) {
+                const int dig = (int)(int8_t)(X & 0xff);
+                d[b] |= (uint32_t)(dig & 0xff) << (8 * i);
+                X = (X - dig) >> 8;
+              }
+            }
+            // MMA 0: planes 3 and 2 in rows g and g + 8; MMA 1: planes 1 and 0
+            const int c = 2 * (s & 1);
+            qa[s / 2][c] = d[3], qa[s / 2][c + 1] = d[2], qa[s / 2][4 + c] = d[1], qa[s / 2][4 + c + 1] = d[0];
+          } else {
+            qa[s][hh] = f16x2(y[0], y[1]), qa[s][hh + 2] = f16x2(y[2], y[3]);
+          }
         }
       } else {
 #pragma unroll
         for (int s = 0; s < D / 16; ++s) qa[s][hh] = w[s].x, qa[s][hh + 2] = w[s].y;
       }
+    }
+    if (NR == 8 && !PLANES) {
+#pragma unroll
+      for (int s = 0; s < D / 16; ++s) qa[s][1] = qa[s][3] = 0u;
     }
     float m_run[2] = {-INFINITY, -INFINITY}, l_part[2] = {0.f, 0.f};
     float acc[ND][4];
@@ -350,11 +549,12 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const Params p) {
       const float *ksc = (const float *)(vt + TILE * G::kRowBytes), *vsc = ksc + TILE;
       const int left = seg.len - (x - seg.start) * TILE;  // keys from the tile's first to the segment's end
 
-      // ---- scores: n-tile nt holds keys 8 nt .. 8 nt + 7 (this thread loads key 8 nt + g)
+      // ---- scores in log2 units: n-tile nt holds keys 8 nt .. 8 nt + 7 (this thread loads key 8 nt + g and gets rows g,
+      // g + 8 of keys 8 nt + 2t, 8 nt + 2t + 1)
       float sc[NT][4];
+      float2 vs[NT];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
         const int r = 8 * nt + g;
         const uint8_t *row = kt + r * G::kRowBytes;
         constexpr int NW = G::kRowBytes / 16;  // words of the row that this thread takes
@@ -369,41 +569,51 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const Params p) {
             kw[4 * c] = a.x, kw[4 * c + 1] = a.y, kw[4 * c + 2] = a.z, kw[4 * c + 3] = a.w;
           }
         }
+        float2 ks = make_float2(1.f, 1.f);
+        if (Q8) ks = *(const float2 *)(ksc + 8 * nt + 2 * t), vs[nt] = *(const float2 *)(vsc + 8 * nt + 2 * t);
+        if constexpr (PLANES) {
+          int hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
 #pragma unroll
-        for (int s = 0; s < D / 16; ++s) {
-          if (Q8) {
-            const uint32_t b = kw[s] ^ 0x80808080u;
-            mma<true>(sc[nt], qa[s], codes_f16(b, 0x4140), codes_f16(b, 0x4342));
-          } else {
-            mma<false>(sc[nt], qa[s], kw[(2 * s) % NW], kw[(2 * s + 1) % NW]);
+          for (int s = 0; s < D / 32; ++s) {
+            mma_i8(hi, qa[s], kw[2 * s], kw[2 * s + 1]);
+            mma_i8(lo, qa[s] + 4, kw[2 * s], kw[2 * s + 1]);
           }
+          // |digit sums| <= 2^21, so both halves of the 32-bit digits' sum fit an int
+          sc[nt][0] = fmaf((float)(hi[0] * 256 + hi[2]), 65536.f, (float)(lo[0] * 256 + lo[2])) * (rowfac[0] * ks.x);
+          sc[nt][1] = fmaf((float)(hi[1] * 256 + hi[3]), 65536.f, (float)(lo[1] * 256 + lo[3])) * (rowfac[0] * ks.y);
+          sc[nt][2] = sc[nt][3] = 0.f;
+        } else {
+          sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+#pragma unroll
+          for (int s = 0; s < D / 16; ++s) {
+            if (Q8) {
+              const uint32_t b = kw[s] ^ 0x80808080u;
+              mma<true>(sc[nt], qa[s], codes_f16(b, 0x4140), codes_f16(b, 0x4342));
+            } else {
+              mma<false>(sc[nt], qa[s], kw[(2 * s) % NW], kw[(2 * s + 1) % NW]);
+            }
+          }
+#pragma unroll
+          for (int hh = 0; hh < NR / 8; ++hh) sc[nt][2 * hh] *= rowfac[hh] * ks.x, sc[nt][2 * hh + 1] *= rowfac[hh] * ks.y;
         }
       }
-      // ---- softmax: this thread has rows g, g + 8 of keys 8 nt + 2t, 8 nt + 2t + 1
-      float mx[2] = {-INFINITY, -INFINITY};
-      float vs[NT][2];
+      if (left < TILE) {  // the segment's last tile
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int key = 8 * nt + 2 * t + e;
-          const bool in = key < left;
-          const float kf = Q8 ? ksc[key] : 1.f;
-          vs[nt][e] = Q8 && in ? vsc[key] : 0.f;
-#pragma unroll
-          for (int hh = 0; hh < NR / 8; ++hh) {
-            float &v = sc[nt][2 * hh + e];
-            v = in ? v * (rowfac[hh] * kf) : -INFINITY;
-            mx[hh] = fmaxf(mx[hh], v);
-          }
+        for (int nt = 0; nt < NT; ++nt) {
+          const int key = 8 * nt + 2 * t;
+          if (key >= left) sc[nt][0] = sc[nt][2] = -INFINITY;
+          if (key + 1 >= left) sc[nt][1] = sc[nt][3] = -INFINITY;
         }
       }
       float ms[2], alpha[2] = {1.f, 1.f};
 #pragma unroll
       for (int hh = 0; hh < NR / 8; ++hh) {
-        mx[hh] = fmaxf(mx[hh], __shfl_xor_sync(0xffffffffu, mx[hh], 1));
-        mx[hh] = fmaxf(mx[hh], __shfl_xor_sync(0xffffffffu, mx[hh], 2));
-        const float m_new = fmaxf(m_run[hh], mx[hh]);
+        float mx = -INFINITY;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) mx = fmaxf(mx, fmaxf(sc[nt][2 * hh], sc[nt][2 * hh + 1]));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const float m_new = fmaxf(m_run[hh], mx);
         ms[hh] = m_new == -INFINITY ? 0.f : m_new;
         alpha[hh] = ex2(m_run[hh] - ms[hh]);
         m_run[hh] = m_new;
@@ -417,7 +627,7 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const Params p) {
         for (int hh = 0; hh < NR / 8; ++hh) {
           float p0 = ex2(sc[nt][2 * hh] - ms[hh]), p1 = ex2(sc[nt][2 * hh + 1] - ms[hh]);
           l_part[hh] += p0 + p1;
-          if (Q8) p0 *= vs[nt][0], p1 *= vs[nt][1];
+          if (Q8) p0 *= vs[nt].x, p1 *= vs[nt].y;  // (past the segment's end both are zeros)
           const uint32_t hi = bf16x2(p0, p1), lo = bf16x2(p0 - bf16_lo(hi), p1 - bf16_hi(hi));
           pa[nt / 2][2 * (nt % 2) + hh] = hi;
           if (NR == 16) pb[nt / 2][2 * (nt % 2) + hh] = lo;
@@ -482,7 +692,7 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const Params p) {
 #pragma unroll
       for (int j = 0; j < ND; ++j) acc[j][0] += acc[j][2], acc[j][1] += acc[j][3];
     }
-    // ---- the segment is done: the four warps' states meet in warp 0 (2, 3 -> 0, 1, then 1 -> 0)
+    // ---- the segment is done: the warps' states meet in warp 0, the upper half of them handing theirs down each time
 #pragma unroll
     for (int hh = 0; hh < NR / 8; ++hh) {
       l_part[hh] += __shfl_xor_sync(0xffffffffu, l_part[hh], 1);
@@ -518,9 +728,9 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const Params p) {
           for (int c = 0; c < NC; ++c) acc[j][c] = acc[j][c] * fa[c / 2] + b[j * NC + c][lane] * fb[c / 2];
       }
     }
-    const bool whole = !SHARED && seg.start >= x0 && seg.end <= x1;
+    const bool whole = seg.start >= x0 && seg.end <= x1;
     if (warp == 0) {
-      if (whole) {
+      if (!PREFIX && whole && !p.pre.rec) {
 #pragma unroll
         for (int hh = 0; hh < NR / 8; ++hh) {
           const int r = g + 8 * hh;
@@ -538,8 +748,8 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const Params p) {
           }
         }
       } else {
-        float *rec = record<D>(p, SHARED ? (int)blockIdx.x + seg.index : 2 * (int)blockIdx.x + (seg.index != first_seg));
-        const int rows = (SHARED && seg.seq < 0) ? kRows : p.group;
+        float *rec = record<D>(p, PREFIX ? (int)blockIdx.x + seg.index : 2 * (int)blockIdx.x + (seg.index != first_seg));
+        const int rows = PREFIX ? kRows : p.group;
 #pragma unroll
         for (int hh = 0; hh < NR / 8; ++hh) {
           const int r = g + 8 * hh;
@@ -556,97 +766,40 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const Params p) {
         }
       }
     }
-    if (!SHARED && !whole) {
-      // the last CTA of a segment that several share adds their records up
+    if (!PREFIX && (!whole || p.pre.rec)) {
       const int c0 = seg.start / lay.chunk, c1 = (seg.end - 1) / lay.chunk;
-      __threadfence();
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        unsigned *cnt = p.cnt + seg.index;
-        const bool last = atomicAdd(cnt, 1u) == (unsigned)(c1 - c0);
-        if (last) *cnt = 0u;
-        sm.last = last;
-      }
-      __syncthreads();
-      if (sm.last) {
+      bool last = true;
+      if (!whole) {  // the last CTA of a split segment adds the parts up
         __threadfence();
-        for (int e = threadIdx.x; e < p.group * D; e += kThreads) {
-          const int r = e / D, dd = e - r * D;
-          float M = -INFINITY, lsum = 0.f, a = 0.f;
-          for (int c = c0; c <= c1; ++c) {
-            const float *rec = record<D>(p, 2 * c + (c == c0 && seg.start != c0 * lay.chunk));
-            const float mc = __ldcg(rec + kRows * D + r);
-            const float lc = __ldcg(rec + kRows * D + kRows + r), ac = __ldcg(rec + r * D + dd);
-            const float m_new = fmaxf(M, mc), mz = m_new == -INFINITY ? 0.f : m_new;
-            const float fo = ex2(M - mz), fc = ex2(mc - mz);
-            M = m_new;
-            lsum = lsum * fo + lc * fc;
-            a = a * fo + ac * fc;
-          }
-          p.out[seg.seq * p.ldo + (int64_t)(seg.g * p.group + r) * D + dd] = f32_to_bf16_bits(a / lsum);
+        __syncthreads();
+        if (threadIdx.x == 0) {
+          unsigned *cnt = p.cnt + seg.index;
+          sm.last = atomicAdd(cnt, 1u) == (unsigned)(c1 - c0);
+          if (sm.last) *cnt = 0u;
         }
+        __syncthreads();
+        last = sm.last;
+        __threadfence();
+      } else {
+        __syncthreads();  // warp 0's record is written
+      }
+      if (last) {
+        // (a whole segment's one record is in this CTA's slot, a split one's first part in the last slot of its CTA
+        // if that began with another segment)
+        const int first = whole ? 2 * (int)blockIdx.x + (seg.index != first_seg) : 2 * c0 + (seg.start != c0 * lay.chunk);
+        finish<D>(p, sm.fin, seg.seq, seg.g, c1 - c0 + 1, first, c0);
       }
     }
-    if (seg.end >= x1) break;
-    seg = find_seg(p, lay, sm.cum, seg.end);
+    if (seg_end >= x1) break;
+    seg = find_seg<TILE, PREFIX>(p, lay, sm.cum, seg.end);
   }
   cp_wait<0>();
 }
 
-// One (sequence, head) row per warp: its records of the prefix's and of its own segment, added up.
-template <int D, int TILE>
-__global__ void __launch_bounds__(kThreads) combine_kernel(const Params p, int grid) {
-  __shared__ int cum[kMaxBatch + 1];
-  __shared__ int scratch[kWarps];
-  constexpr int N = D / 32;
-  pdl_wait();
-  pdl_launch_dependents();
-  Layout lay = make_layout<TILE>(p, cum, scratch);
-  lay.chunk = max((lay.total + grid - 1) / grid, kWarps);  // as the attention kernel's grid cut it
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int row = blockIdx.x * kWarps + warp;
-  const int nq = p.nkv * p.group;
-  if (row >= p.m * nq) return;
-  const int i = row / nq, h = row - i * nq, g = h / p.group, j = h - g * p.group;
-  float M = -INFINITY, lsum = 0.f, a[N];
-#pragma unroll
-  for (int e = 0; e < N; ++e) a[e] = 0.f;
-  auto add_record = [&](const float *rec, int rows, int r) {
-    const float mc = __ldcg(rec + rows * D + r), lc = __ldcg(rec + rows * D + rows + r);
-    if (lc == 0.f) return;  // no keys: nothing was accumulated
-    const float m_new = fmaxf(M, mc), mz = m_new == -INFINITY ? 0.f : m_new;
-    const float fo = ex2(M - mz), fc = ex2(mc - mz);
-    M = m_new;
-    lsum = lsum * fo + lc * fc;
-#pragma unroll
-    for (int e = 0; e < N; ++e) a[e] = a[e] * fo + __ldcg(rec + r * D + lane + 32 * e) * fc;
-  };
-  auto add = [&](const Seg &s, int r) {
-    if (s.start >= s.end) return;
-    for (int c = s.start / lay.chunk; c <= (s.end - 1) / lay.chunk; ++c) add_record(record<D>(p, c + s.index), kRows, r);
-  };
-  if (D == apx::kD && p.pre) {
-    const int tile = i / p.pre_seqs, pair = tile / 2;
-    const bool two = 2 * pair + 1 < p.pre_tiles;  // the pair's streams are two tiles, or both this one
-    const float *rec = p.pre + (int64_t)(g * p.pre_pairs + pair) * p.pre_ranges * 2 * apx::kRecord;
-    for (int c = 0; c < 2 * p.pre_ranges; ++c)
-      if (!two || (c & 1) == (tile & 1))
-        add_record(rec + (int64_t)c * apx::kRecord, apx::kRowsT, (i % p.pre_seqs) * p.group + j);
-  }
-  if (lay.prefix_segs) {
-    const int flat = i * p.group + j;
-    add(prefix_seg(p, lay, g * p.row_tiles + flat / kRows), flat % kRows);
-  }
-  add(own_seg(p, lay, cum, i, g), j);
-  const float inv = lsum == 0.f ? 0.f : 1.f / lsum;  // no keys at all: zeros
-#pragma unroll
-  for (int e = 0; e < N; ++e) p.out[i * p.ldo + (int64_t)h * D + lane + 32 * e] = f32_to_bf16_bits(a[e] * inv);
-}
-
-template <int D, bool Q8, int NR, bool SHARED>
-static cudaError_t launch(const Params &p, cudaStream_t st, bool pdl) {
+template <int D, bool Q8, int NR, bool PREFIX>
+static cudaError_t launch(const Params &p, int grid, cudaStream_t st, bool pdl) {
   constexpr int kStages = NR == 16 ? 2 : 3;
-  auto fn = attn_kernel<D, Q8, NR, SHARED, kStages>;
+  auto fn = attn_kernel<D, Q8, NR, PREFIX, kStages>;
   const size_t smem = sizeof(Smem<D, Q8, NR, kStages>);
   static int configured[64] = {0};  // the shared-memory opt-in, per device
   int dev = 0;
@@ -656,24 +809,46 @@ static cudaError_t launch(const Params &p, cudaStream_t st, bool pdl) {
     if (e != cudaSuccess) return e;
     configured[dev] = 1;
   }
-  const int grid = 2 * num_sms();
-  const cudaError_t e = launch_kernel((const void *)fn, dim3(grid), dim3(kThreads), smem, st, pdl, p);
-  if (e != cudaSuccess || !SHARED) return e;
-  const unsigned rows = (unsigned)(p.m * p.nkv * p.group);
-  return launch_kernel((const void *)combine_kernel<D, Geo<D, Q8>::kTile>, dim3((rows + kWarps - 1) / kWarps),
-                       dim3(kThreads), 0, st, true, p, grid);
+  return launch_kernel((const void *)fn, dim3(grid), dim3(kThreads), smem, st, pdl, p);
 }
-template <bool Q8, int NR, bool SHARED>
-static cudaError_t launch_d(const Params &p, int d, cudaStream_t st, bool pdl) {
-  return d == 128 ? launch<128, Q8, NR, SHARED>(p, st, pdl)
-                  : (d == 64 ? launch<64, Q8, NR, SHARED>(p, st, pdl) : launch<32, Q8, NR, SHARED>(p, st, pdl));
+template <bool Q8, int NR, bool PREFIX>
+static cudaError_t launch_d(const Params &p, int d, int grid, cudaStream_t st, bool pdl) {
+  return d == 128 ? launch<128, Q8, NR, PREFIX>(p, grid, st, pdl)
+                  : (d == 64 ? launch<64, Q8, NR, PREFIX>(p, grid, st, pdl) : launch<32, Q8, NR, PREFIX>(p, grid, st, pdl));
+}
+template <bool PREFIX>
+static cudaError_t launch_any(const Params &p, int d, bool q8, int rows, int grid, cudaStream_t st, bool pdl) {
+  if (rows <= 8) return q8 ? launch_d<true, 8, PREFIX>(p, d, grid, st, pdl) : launch_d<false, 8, PREFIX>(p, d, grid, st, pdl);
+  return q8 ? launch_d<true, 16, PREFIX>(p, d, grid, st, pdl) : launch_d<false, 16, PREFIX>(p, d, grid, st, pdl);
 }
 
+static int row_tiles(int64_t m, int group) { return (int)((m * group + kRows - 1) / kRows); }
+static int tile_keys(bool q8) { return q8 ? 32 : 16; }
+static int max_grid() { return kCtasPerSm * num_sms(); }
+// CTAs that the sequences' own keys can need: no more ranges than segments and kMinChunk tiles allow.
+static int own_grid(const Params &p, bool q8) {
+  const int64_t most = ((p.cache.cap + tile_keys(q8) - 1) / tile_keys(q8) + kMinChunk - 1) / kMinChunk;
+  return (int)std::min<int64_t>(max_grid(), most * p.m * p.nkv);
+}
+// How the prefix's segments are cut: as make_layout does it, on the host.
+static void cut_prefix(Params &p, int64_t prefix_len, bool q8, int grid) {
+  Prefix &c = p.pre;
+  c.row_tiles = row_tiles(p.m, p.group);
+  c.seg_tiles = (int)((prefix_len + tile_keys(q8) - 1) / tile_keys(q8));
+  const int segs = p.nkv * c.row_tiles, least = std::max(kMinChunk, ceil_div(segs * c.seg_tiles, grid));
+  c.pad = 1, c.chunk = even_share(segs * c.seg_tiles, segs, grid);
+  for (int j = 0; j < 32; ++j) {
+    const int len = least + ceil_div(least * j, 64);
+    if ((int64_t)segs * ceil_div(c.seg_tiles, len) <= grid) {
+      c.pad = c.chunk = len;
+      break;
+    }
+  }
+}
 // Whether the prefix goes to attn_prefix_kernel: bf16, head_dim 128, more rows than one tile of the mma.sync kernel.
 static bool prefix_on_tcgen05(const Params &p, int d, bool q8) {
-  return !q8 && d == apx::kD && p.prefix > 0 && p.scale_log2 > 0.f && p.m * p.group > kRows;
+  return !q8 && d == apx::kD && p.scale_log2 > 0.f && p.m * p.group > kRows;
 }
-static int row_tiles(int64_t m, int group) { return (int)((m * group + kRows - 1) / kRows); }
 static size_t counter_bytes(int64_t m, int nkv) { return ((size_t)m * nkv * 4 + 255) / 256 * 256; }
 
 static int check(const char *what, int64_t ldo, int64_t ldq, const void *out, const void *q, int64_t cap, int64_t m,
@@ -700,10 +875,12 @@ using namespace egpt;
 
 extern "C" size_t egpt_attn_q8_ws_bytes(int64_t m, int nq, int nkv, int d) {
   if (m < 1 || nkv < 1 || nq < nkv || d < 1) return 0;
-  // counters, then a record for every (CTA, segment) pair: CTA c and segment s keep theirs at c + s
-  const size_t records = (size_t)2 * num_sms() + (size_t)nkv * aq8::row_tiles(m, nq / nkv) + (size_t)m * nkv;
-  const size_t prefix = d == apx::kD && nq / nkv <= aq8::kRows ? apx::record_floats(m, nq / nkv, nkv) * 4 : 0;
-  return aq8::counter_bytes(m, nkv) + std::max(records, (size_t)4 * num_sms()) * aq8::kRows * ((size_t)d + 2) * 4 + prefix;
+  // arrival counters; two records for every CTA of the launch over the sequences' own keys; the prefix's records: one for
+  // every (CTA, segment) pair of attn_kernel (CTA c and segment s keep theirs at c + s), or attn_prefix_kernel's
+  const size_t rec = aq8::kRows * ((size_t)d + 2) * 4;
+  const size_t small = ((size_t)aq8::max_grid() + (size_t)nkv * aq8::row_tiles(m, nq / nkv)) * rec;
+  const size_t big = d == apx::kD && nq / nkv <= aq8::kRows ? apx::record_floats(m, nq / nkv, nkv) * 4 : 0;
+  return aq8::counter_bytes(m, nkv) + 2 * (size_t)aq8::max_grid() * rec + std::max(small, big);
 }
 
 extern "C" int egpt_attn_decode_q8(void *out, int64_t ldo, const void *q, int64_t ldq, const int8_t *k_cache,
@@ -718,12 +895,11 @@ extern "C" int egpt_attn_decode_q8(void *out, int64_t ldo, const void *q, int64_
     return set_error(EGPT_ERR_ALIGN, "attn_decode_q8: caches must be 16-byte aligned");
   aq8::Params p{};
   p.out = (uint16_t *)out, p.ldo = ldo, p.q = (const uint16_t *)q, p.ldq = ldq;
-  p.own = {(const uint8_t *)k_cache, (const uint8_t *)v_cache, k_scale, v_scale, cap};
+  p.cache = {(const uint8_t *)k_cache, (const uint8_t *)v_cache, k_scale, v_scale, cap};
   p.position = position, p.m = (int)m, p.nkv = nkv, p.group = nq / nkv, p.scale_log2 = scale * 1.4426950408889634f;
   p.cnt = (unsigned *)ws, p.ws = (float *)((char *)ws + aq8::counter_bytes(m, nkv));
-  const bool pdl = (flags & EGPT_FLAG_PDL) != 0;
-  return check_launch(p.group <= 8 ? aq8::launch_d<true, 8, false>(p, d, (cudaStream_t)stream, pdl)
-                                   : aq8::launch_d<true, 16, false>(p, d, (cudaStream_t)stream, pdl),
+  return check_launch(aq8::launch_any<false>(p, d, true, p.group, aq8::own_grid(p, true), (cudaStream_t)stream,
+                                             (flags & EGPT_FLAG_PDL) != 0),
                       "attn_decode_q8_kernel");
 }
 
@@ -741,38 +917,42 @@ extern "C" int egpt_attn_shared_prefix(void *out, int64_t ldo, const void *q, in
   if (q8 && (!pk_scale || !pv_scale || !tk_scale || !tv_scale))
     return set_error(EGPT_ERR_ARG, "attn_shared_prefix: int8 caches need their scales");
   if (int rc = aq8::check("attn_shared_prefix", ldo, ldq, out, q, cap, m, nq, nkv, d, scale, ws, ws_bytes)) return rc;
-  if (prefix_cap < 1 || prefix_len < 0 || prefix_len > prefix_cap ||
-      (int64_t)nkv * (aq8::row_tiles(m, nq / nkv) * ((prefix_len + 15) / 16) + m * ((cap + 15) / 16)) > 0x3fffffff)
-    return set_error(EGPT_ERR_SHAPE, "attn_shared_prefix: bad prefix_len (0 to prefix_cap) or caches too long");
+  if (prefix_cap < 1 || prefix_len < 0 || prefix_len > prefix_cap || prefix_len > 0x3fffffff ||
+      (int64_t)nkv * aq8::row_tiles(m, nq / nkv) * ((prefix_len + 15) / 16) > 0x1fffffff)
+    return set_error(EGPT_ERR_SHAPE, "attn_shared_prefix: bad prefix_len (0 to prefix_cap), or too long for the batch");
   if ((uintptr_t)pk % 16 || (uintptr_t)pv % 16 || (uintptr_t)tk % 16 || (uintptr_t)tv % 16)
     return set_error(EGPT_ERR_ALIGN, "attn_shared_prefix: caches must be 16-byte aligned");
+  const cudaStream_t st = (cudaStream_t)stream;
+  bool pdl = (flags & EGPT_FLAG_PDL) != 0;
   aq8::Params p{};
   p.out = (uint16_t *)out, p.ldo = ldo, p.q = (const uint16_t *)q, p.ldq = ldq;
-  p.own = {(const uint8_t *)tk, (const uint8_t *)tv, tk_scale, tv_scale, cap};
-  p.shared = {(const uint8_t *)pk, (const uint8_t *)pv, pk_scale, pv_scale, prefix_cap};
-  p.prefix = prefix_len, p.position = position, p.m = (int)m, p.nkv = nkv, p.group = nq / nkv;
-  p.row_tiles = aq8::row_tiles(m, p.group), p.scale_log2 = scale * 1.4426950408889634f;
+  p.position = position, p.m = (int)m, p.nkv = nkv, p.group = nq / nkv, p.scale_log2 = scale * 1.4426950408889634f;
   p.cnt = (unsigned *)ws, p.ws = (float *)((char *)ws + aq8::counter_bytes(m, nkv));
-  const bool pdl = (flags & EGPT_FLAG_PDL) != 0;
-  const cudaStream_t st = (cudaStream_t)stream;
-  cudaError_t e;
-  if (aq8::prefix_on_tcgen05(p, d, q8)) {
-    apx::Args A{};
-    const apx::Shape sh = apx::shape_of(m, p.group, nkv, prefix_len);
-    // its records lie behind those of the tails
-    const size_t head = egpt_attn_q8_ws_bytes(m, nq, nkv, d) - apx::record_floats(m, p.group, nkv) * 4;
-    A.ws = (float *)((char *)ws + head);
-    A.prefix = prefix_len, A.m = (int)m, A.nkv = nkv, A.group = p.group, A.scale_log2 = p.scale_log2;
-    bool maps_ok = false;
-    e = apx::launch(A, q, ldq, pk, pv, prefix_cap, sh, st, pdl, maps_ok);
-    if (!maps_ok) return set_error(EGPT_ERR_ALIGN, "attn_shared_prefix: tensor maps rejected");
-    if (e != cudaSuccess) return check_launch(e, "attn_prefix_kernel");
-    p.pre = A.ws, p.pre_seqs = sh.seqs, p.pre_tiles = sh.tiles, p.pre_pairs = sh.pairs, p.pre_ranges = sh.ranges;
-    p.prefix = 0;  // what is left in the flat list are the tails
-    e = p.group <= 8 ? aq8::launch<128, false, 8, true>(p, st, true) : aq8::launch<128, false, 16, true>(p, st, true);
-    return check_launch(e, "attn_shared_prefix_kernel");
+  float *pre_rec = p.ws + 2 * (size_t)aq8::max_grid() * aq8::kRows * (d + 2);
+  if (prefix_len > 0) {
+    if (aq8::prefix_on_tcgen05(p, d, q8)) {
+      apx::Args A{};
+      const apx::Shape sh = apx::shape_of(m, p.group, nkv, prefix_len);
+      A.ws = pre_rec, A.prefix = prefix_len, A.m = (int)m, A.nkv = nkv, A.group = p.group, A.scale_log2 = p.scale_log2;
+      bool maps_ok = false;
+      const cudaError_t e = apx::launch(A, q, ldq, pk, pv, prefix_cap, sh, st, pdl, maps_ok);
+      if (!maps_ok) return set_error(EGPT_ERR_ALIGN, "attn_shared_prefix: tensor maps rejected");
+      if (e != cudaSuccess) return check_launch(e, "attn_prefix_kernel");
+      p.pre.big = 1, p.pre.seqs = sh.seqs, p.pre.tiles = sh.tiles, p.pre.pairs = sh.pairs, p.pre.ranges = sh.ranges;
+    } else {
+      aq8::Params a = p;
+      a.cache = {(const uint8_t *)pk, (const uint8_t *)pv, pk_scale, pv_scale, prefix_cap};
+      a.keys = (int)prefix_len, a.ws = pre_rec;
+      aq8::cut_prefix(a, prefix_len, q8, aq8::max_grid());
+      const int64_t places = (int64_t)nkv * a.pre.row_tiles * aq8::ceil_div(a.pre.seg_tiles, a.pre.pad) * a.pre.pad;
+      const cudaError_t e = aq8::launch_any<true>(a, d, q8, (int)m * p.group, (int)((places + a.pre.chunk - 1) / a.pre.chunk),
+                                                  st, pdl);
+      if (e != cudaSuccess) return check_launch(e, "attn_shared_prefix_kernel (prefix)");
+      p.pre = a.pre;
+    }
+    p.pre.rec = pre_rec;
+    pdl = true;
   }
-  if (m * p.group <= 8) e = q8 ? aq8::launch_d<true, 8, true>(p, d, st, pdl) : aq8::launch_d<false, 8, true>(p, d, st, pdl);
-  else e = q8 ? aq8::launch_d<true, 16, true>(p, d, st, pdl) : aq8::launch_d<false, 16, true>(p, d, st, pdl);
-  return check_launch(e, "attn_shared_prefix_kernel");
+  p.cache = {(const uint8_t *)tk, (const uint8_t *)tv, tk_scale, tv_scale, cap};
+  return check_launch(aq8::launch_any<false>(p, d, q8, p.group, aq8::own_grid(p, q8), st, pdl), "attn_shared_prefix_kernel");
 }

@@ -243,6 +243,24 @@ def test_decode_score_sizes_and_scale_spread(cuda, factor):
     _check(out, q, nq, nkv, d, d ** -0.5, lengths, own)
 
 
+def test_nan_and_infinity_in_a_query_row_stay_in_its_heads(cuda):
+    ops = _ops()
+    gen = _gen(12)
+    nq, nkv, d, m, cap = 8, 2, 128, 2, 300
+    own = _cache_q8(gen, m * nkv, cap, d)
+    q = _randn(gen, m, nq * d).bfloat16()
+    bad = q.clone()
+    bad[0, 3 * d + 7] = float('nan')
+    bad[1, 6 * d] = float('inf')
+    pos = torch.tensor([299, 40], device=cuda)
+    want = ops.attn_decode_q8(q, *own, pos, nq, nkv, d, scale=0.1).view(m, nq, d)
+    got = ops.attn_decode_q8(bad, *own, pos, nq, nkv, d, scale=0.1).view(m, nq, d)
+    for i, h in ((0, 3), (1, 6)):
+        assert got[i, h].isnan().all()
+        got[i, h] = want[i, h]
+    assert torch.equal(got, want)
+
+
 def test_decode_positions_are_read_on_the_device(cuda):
     """A captured graph follows the positions; a position past the cache is reported and gives zeros."""
     from efficientgpt_b200 import _lib as L
