@@ -11,9 +11,11 @@
 // row. A segment's keys are cut into tiles of kTile keys and the tiles of a launch into contiguous ranges, one per CTA,
 // on the device, so no length is known to the host. Where the segments allow it ranges are parts of one
 // segment each (split by the smallest range length that gives every CTA at most one); else they are equal
-// stretches of the flat list of all tiles and may hold several segments, so that a batch of one token next to a document
-// leaves no CTA idle. Within a range a warp takes every kWarps-th tile through a ring of its own in shared memory
-// (cp.async, rows past the segment's end filled with zeros), so warps only meet at a segment's end.
+// stretches of the flat list of all tiles and may hold several segments (each counted with kExtra tiles more, about
+// what its start and end cost), cut inside a segment only if that is a long one, so that neither many short sequences
+// nor one token next to a document leave CTAs idle. Of a segment's part a warp takes every kWarps-th tile, through
+// a ring of its own in shared memory (cp.async, rows past the segment's end filled with zeros), running ahead into the
+// next segment; warps only meet at a segment's end.
 //
 // A prefix runs first, in a launch of its own that leaves partial records (here, or in attn_prefix.cu); the launch over
 // the sequences' own keys is a dependent one that starts beside it and waits only before it adds those records up.
@@ -33,12 +35,13 @@
 namespace egpt {
 namespace aq8 {
 
-constexpr int kWarps = 4;
+constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
 constexpr int kMaxBatch = 512;
 constexpr int kRows = 16;              // query rows per tile (the M of the MMA), and rows of a partial record
-constexpr int kCtasPerSm = 2;
+constexpr int kCtasPerSm = 1;
 constexpr int kMinChunk = 2 * kWarps;  // tiles of a range at least
+constexpr int kExtra = 16;             // what a segment's start and end cost, in tiles
 
 struct Cache {
   const uint8_t *k, *v;
@@ -68,12 +71,14 @@ struct Params {
   Prefix pre;     // of the launch over the sequences' own keys: records to add up; of the prefix's: how it is cut
 };
 
-// How the tiles of the launch are cut: a segment takes up round_up(tiles, pad) places of the flat list, a CTA `chunk`.
+// How the tiles of the launch are cut: a CTA takes `chunk` places of the flat list of segments.
 struct Layout {
-  int total, chunk, pad;  // pad = chunk: every range lies in one segment; pad = 1: equal stretches
+  int total, chunk;
+  int pad;    // > 1: a segment takes up a multiple of pad (= chunk) places and every range lies in one segment
+  int uncut;  // else equal stretches, and the tiles up to which a segment is not split
 };
 struct Seg {
-  int index, start, end;  // its number and its tiles in the flat list
+  int index, start, end, next;  // its number, its tiles in the flat list, and the place after it
   int seq, g, tile;       // sequence, kv head; row tile (prefix)
   int len;                // keys
 };
@@ -169,30 +174,23 @@ __device__ __forceinline__ int seq_len(const Params &p, int i) {
 
 __host__ __device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
-// Tiles of an equal stretch: not below the segments' average, up to kMinChunk (splitting a short segment costs more in
-// adding the parts up than it gains).
-__host__ __device__ __forceinline__ int even_share(int tiles, int segs, int grid) {
-  const int least = ceil_div(tiles, segs) < kMinChunk ? ceil_div(tiles, segs) : kMinChunk;
-  const int share = ceil_div(tiles, grid);
-  return share > least ? share : (least > 1 ? least : 1);
-}
 // cum[i] = places of the sequences before i (one kv head). The ranges: with up to 32 sequences the lanes try range lengths
 // from the even share of the tiles up to 1.5 times it, and the smallest that gives at most one range per CTA is taken;
-// failing that, and for more sequences, even shares. Every thread of the CTA calls it.
+// failing that, and for more sequences, equal stretches. Every thread of the CTA calls it.
 template <int TILE>
 __device__ Layout make_layout(const Params &p, int *cum, int *scratch) {
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, grid = (int)gridDim.x;
   Layout l;
+  l.pad = 1;
   if (p.m <= 32) {  // every warp for itself
     const int tiles = lane < p.m ? ceil_div(seq_len(p, lane), TILE) : 0;
-    const int all = p.nkv * __reduce_add_sync(0xffffffffu, tiles);
-    const int least = max(kMinChunk, ceil_div(all, grid)), len = least + ceil_div(least * lane, 64);
+    const int least = max(kMinChunk, ceil_div(p.nkv * __reduce_add_sync(0xffffffffu, tiles), grid));
+    const int len = least + ceil_div(least * lane, 64);
     int parts = 0;
     for (int i = 0; i < p.m; ++i) parts += ceil_div(__shfl_sync(0xffffffffu, tiles, i), len);
     const unsigned fits = __ballot_sync(0xffffffffu, p.nkv * parts <= grid);
-    l.chunk = fits ? __shfl_sync(0xffffffffu, len, __ffs(fits) - 1) : even_share(all, p.nkv * p.m, grid);
-    l.pad = fits ? l.chunk : 1;
-    const int places = ceil_div(tiles, l.pad) * l.pad;
+    if (fits) l.pad = __shfl_sync(0xffffffffu, len, __ffs(fits) - 1);
+    const int places = fits ? ceil_div(tiles, l.pad) * l.pad : (tiles ? tiles + kExtra : 0);
     int inc = places;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -206,12 +204,12 @@ __device__ Layout make_layout(const Params &p, int *cum, int *scratch) {
     __syncthreads();
   } else {
     constexpr int kPer = kMaxBatch / kThreads;
-    int tiles[kPer], sum = 0;
+    int places[kPer], sum = 0;
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
-      const int i = t * kPer + e;
-      tiles[e] = i < p.m ? ceil_div(seq_len(p, i), TILE) : 0;
-      sum += tiles[e];
+      const int i = t * kPer + e, tiles = i < p.m ? ceil_div(seq_len(p, i), TILE) : 0;
+      places[e] = tiles ? tiles + kExtra : 0;
+      sum += places[e];
     }
     int inc = sum;
 #pragma unroll
@@ -226,41 +224,69 @@ __device__ Layout make_layout(const Params &p, int *cum, int *scratch) {
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
       cum[t * kPer + e] = before;
-      before += tiles[e];
+      before += places[e];
     }
     if (t == kThreads - 1) cum[kMaxBatch] = before;
     __syncthreads();
-    l.pad = 1;
-    l.chunk = even_share(p.nkv * cum[p.m], p.nkv * p.m, grid);
   }
   l.total = p.nkv * cum[p.m];
+  l.chunk = l.pad > 1 ? l.pad : max(1, ceil_div(l.total, grid));
+  l.uncut = max(kMinChunk, l.chunk / 2);
   return l;
+}
+template <int TILE>
+__device__ __forceinline__ Seg own_seg(const Params &p, const int *cum, int i, int g) {
+  Seg s;
+  const int places = cum[i + 1] - cum[i];
+  s.seq = i, s.g = g, s.tile = 0;
+  s.index = i * p.nkv + g;
+  s.start = p.nkv * cum[i] + g * places, s.next = s.start + places;
+  s.len = (int)p.position[i] + 1;
+  s.end = s.start + ceil_div(s.len, TILE);
+  return s;
+}
+__device__ __forceinline__ Seg prefix_seg(const Params &p, int index) {
+  Seg s;
+  const int places = ceil_div(p.pre.seg_tiles, p.pre.pad) * p.pre.pad;
+  s.index = index;
+  s.start = index * places, s.end = s.start + p.pre.seg_tiles, s.next = s.start + places;
+  s.seq = -1, s.g = index / p.pre.row_tiles, s.tile = index % p.pre.row_tiles;
+  s.len = p.keys;
+  return s;
 }
 // The segment that holds place x < total.
 template <int TILE, bool PREFIX>
-__device__ __forceinline__ Seg find_seg(const Params &p, const Layout &l, const int *cum, int x) {
-  Seg s;
-  if (PREFIX) {
-    const int places = ceil_div(p.pre.seg_tiles, l.pad) * l.pad;
-    s.index = x / places;
-    s.start = s.index * places, s.end = s.start + p.pre.seg_tiles;
-    s.seq = -1, s.g = s.index / p.pre.row_tiles, s.tile = s.index % p.pre.row_tiles;
-    s.len = p.keys;
-    return s;
-  }
+__device__ __forceinline__ Seg find_seg(const Params &p, const int *cum, int x) {
+  if (PREFIX) return prefix_seg(p, x / (ceil_div(p.pre.seg_tiles, p.pre.pad) * p.pre.pad));
   int lo = 0, hi = p.m - 1;  // the last sequence whose places start at or before x: it has some
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
     if (p.nkv * cum[mid] <= x) lo = mid;
     else hi = mid - 1;
   }
-  const int places = cum[lo + 1] - cum[lo];
-  s.seq = lo, s.g = (x - p.nkv * cum[lo]) / places, s.tile = 0;
-  s.index = lo * p.nkv + s.g;
-  s.start = p.nkv * cum[lo] + s.g * places;
-  s.len = (int)p.position[lo] + 1;
-  s.end = s.start + ceil_div(s.len, TILE);
-  return s;
+  return own_seg<TILE>(p, cum, lo, (x - p.nkv * cum[lo]) / (cum[lo + 1] - cum[lo]));
+}
+// The segment after s, whose next is < total.
+template <int TILE, bool PREFIX>
+__device__ __forceinline__ Seg next_seg(const Params &p, const int *cum, const Seg &s) {
+  if (PREFIX) return prefix_seg(p, s.index + 1);
+  if (s.g + 1 < p.nkv) {
+    Seg r = s;
+    const int places = s.next - s.start;
+    ++r.g, ++r.index, r.start += places, r.end += places, r.next += places;
+    return r;
+  }
+  int i = s.seq + 1;
+  while (cum[i + 1] == cum[i]) ++i;
+  return own_seg<TILE>(p, cum, i, 0);
+}
+// Where a stretch whose even cut is place x begins: not past the tiles of a segment, nor inside a short one.
+template <int TILE, bool PREFIX>
+__device__ __forceinline__ int cut_at(const Params &p, const Layout &l, const int *cum, int64_t x) {
+  if (x >= l.total) return l.total;
+  if (l.pad > 1) return (int)x;
+  const Seg s = find_seg<TILE, PREFIX>(p, cum, (int)x);
+  return x >= s.end || (x > s.start && s.end - s.start <= l.uncut) ? s.next : (int)x;
 }
 // A partial record: kRows rows of (D accumulators), then kRows maxima and kRows sums.
 template <int D>
@@ -325,7 +351,7 @@ __device__ void finish(const Params &p, Finish<D> &f, int i, int g, int own_n, i
 #pragma unroll
     for (int e = 0; e < N; ++e) a[e] = 0.f;
     for (int k0 = part; k0 < n; k0 += 32 * parts) {
-      const int k = k0 + lane * parts;
+      const int k = k0 + lane * parts, cnt = min(32, ceil_div(n - k0, parts));
       const float *row = p.ws;
       float mk = -INFINITY, lk = 0.f;
       if (k < n) {
@@ -336,6 +362,24 @@ __device__ void finish(const Params &p, Finish<D> &f, int i, int g, int own_n, i
         mk = __ldcg(rec + rows * D + r), lk = __ldcg(rec + rows * D + rows + r);
         row = rec + r * D;
       }
+      constexpr int kBatch = 8;  // records in flight: the first of them beside the maxima and sums
+      float v[kBatch][N];
+      auto fetch = [&](int c) {
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {  // (lanes past the count have a readable address, and factor zero)
+          const float *src = (const float *)__shfl_sync(0xffffffffu, (unsigned long long)row, (c + b) & 31) + N * lane;
+          if constexpr (N == 4) {
+            const float4 t = __ldcg((const float4 *)src);
+            v[b][0] = t.x, v[b][1] = t.y, v[b][2] = t.z, v[b][3] = t.w;
+          } else if constexpr (N == 2) {
+            const float2 t = __ldcg((const float2 *)src);
+            v[b][0] = t.x, v[b][1] = t.y;
+          } else {
+            v[b][0] = __ldcg(src);
+          }
+        }
+      };
+      fetch(0);
       const float mx = fmaxf(M, warp_max(lk != 0.f ? mk : -INFINITY));
       const float mz = mx == -INFINITY ? 0.f : mx;
       const float fk = lk != 0.f ? ex2(mk - mz) : 0.f, fo = ex2(M - mz);  // a record without keys has no accumulators
@@ -343,23 +387,14 @@ __device__ void finish(const Params &p, Finish<D> &f, int i, int g, int own_n, i
       lsum = lsum * fo + warp_sum(lk * fk);
 #pragma unroll
       for (int e = 0; e < N; ++e) a[e] *= fo;
-      const int cnt = min(32, ceil_div(n - k0, parts));
-#pragma unroll 4
-      for (int c = 0; c < cnt; ++c) {
-        const float fc = __shfl_sync(0xffffffffu, fk, c);
-        const float *src = (const float *)__shfl_sync(0xffffffffu, (unsigned long long)row, c) + N * lane;
-        float v[N];
-        if constexpr (N == 4) {
-          const float4 t = __ldcg((const float4 *)src);
-          v[0] = t.x, v[1] = t.y, v[2] = t.z, v[3] = t.w;
-        } else if constexpr (N == 2) {
-          const float2 t = __ldcg((const float2 *)src);
-          v[0] = t.x, v[1] = t.y;
-        } else {
-          v[0] = __ldcg(src);
-        }
+      for (int c = 0; c < cnt; c += kBatch) {
+        if (c) fetch(c);
 #pragma unroll
-        for (int e = 0; e < N; ++e) a[e] += fc == 0.f ? 0.f : v[e] * fc;
+        for (int b = 0; b < kBatch; ++b) {
+          const float fc = __shfl_sync(0xffffffffu, fk, (c + b) & 31);
+#pragma unroll
+          for (int e = 0; e < N; ++e) a[e] += fc == 0.f ? 0.f : v[b][e] * fc;
+        }
       }
     }
     if (parts > 1) {
@@ -407,21 +442,22 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const Params p) {
   pdl_launch_dependents();
   Layout lay;
   if (PREFIX) {
-    lay.chunk = p.pre.chunk, lay.pad = p.pre.pad;
+    lay.chunk = p.pre.chunk, lay.pad = p.pre.pad, lay.uncut = 0;
     lay.total = p.nkv * p.pre.row_tiles * ceil_div(p.pre.seg_tiles, lay.pad) * lay.pad;
   } else {
     lay = make_layout<TILE>(p, sm.cum, sm.scratch);
     for (int e = blockIdx.x; e < p.m * p.nkv; e += gridDim.x)  // sequences without keys of their own
       if (sm.cum[e / p.nkv + 1] == sm.cum[e / p.nkv]) finish<D>(p, sm.fin, e / p.nkv, e % p.nkv, 0, 0, 0);
   }
-  const int x0 = (int)min((int64_t)lay.total, (int64_t)blockIdx.x * lay.chunk);
-  if (x0 >= lay.total) return;
-  Seg seg = find_seg<TILE, PREFIX>(p, lay, sm.cum, x0);
-  const int x1 = min(lay.pad > 1 ? seg.end : lay.total, x0 + lay.chunk);
+  const int x0 = cut_at<TILE, PREFIX>(p, lay, sm.cum, (int64_t)blockIdx.x * lay.chunk);
+  int x1 = cut_at<TILE, PREFIX>(p, lay, sm.cum, (int64_t)(blockIdx.x + 1) * lay.chunk);
+  if (x0 >= x1) return;
+  Seg seg = find_seg<TILE, PREFIX>(p, sm.cum, x0);
+  if (lay.pad > 1) x1 = min(x1, seg.end);
 
-  // ---- this warp's loads: every kWarps-th tile of the range, STAGES - 1 tiles ahead. 32 lanes take 512 consecutive bytes
+  // ---- this warp's loads: every kWarps-th tile of a segment's part, STAGES - 1 tiles ahead. 32 lanes take 512 consecutive bytes
   // of a full tile at a time; the swizzles split into a part of the lane and one of the step.
-  int lx = x0 + warp, lcount = 0;
+  int lx = x0 + warp, lslot = 0;
   Seg ls = seg;
   constexpr int kStep = 32 / G::kChunks;  // rows per 512 bytes
   const int lr = lane / G::kChunks, lc = lane % G::kChunks;
@@ -429,9 +465,12 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const Params p) {
   const uint32_t k_dst = ring + lr * G::kRowBytes + ((lc ^ G::k_swz(lr)) * 16);
   const uint32_t v_dst = lr * G::kRowBytes + ((lc ^ G::v_swz(lr)) * 16);
   auto load_next = [&]() {
-    if (lx < x1) {
-      if (lx >= ls.end) ls = find_seg<TILE, PREFIX>(p, lay, sm.cum, lx);
-      const uint32_t st = (uint32_t)((lcount % STAGES) * G::kStageBytes);
+    while (lx >= ls.end && ls.next < x1) {
+      ls = next_seg<TILE, PREFIX>(p, sm.cum, ls);
+      lx = ls.start + warp;
+    }
+    if (lx < min(ls.end, x1)) {
+      const uint32_t st = (uint32_t)(lslot * G::kStageBytes);
       const Cache &c = p.cache;
       const int key0 = (lx - ls.start) * TILE, left = ls.len - key0;
       const int64_t row0 = (PREFIX ? ls.g : (int64_t)ls.seq * p.nkv + ls.g) * c.cap + key0;
@@ -459,12 +498,12 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const Params p) {
     }
     cp_commit();
     lx += kWarps;
-    ++lcount;
+    lslot = lslot + 1 == STAGES ? 0 : lslot + 1;
   };
 #pragma unroll
   for (int s = 0; s < STAGES - 1; ++s) load_next();
 
-  int x = x0 + warp, ccount = 0;
+  int cslot = 0;
   const int first_seg = seg.index;
   for (;;) {
     // ---- the segment's query rows as MMA fragments
@@ -507,17 +546,15 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const Params p) {
         for (int s = 0; s < D / 16; ++s) {
           const float y[4] = {bf16_lo(w[s].x) * up, bf16_hi(w[s].x) * up, bf16_lo(w[s].y) * up, bf16_hi(w[s].y) * up};
           if constexpr (PLANES) {
-            uint32_t d[4] = {0u, 0u, 0u, 0u};  // digit planes, lowest first: a byte for each of the four dims
+            // bytes of X + 0x80808080 are the digits plus 128; a 4 x 4 byte transpose makes words of one digit (d[0] the
+            // lowest) of the four dims
+            uint32_t Y[4], d[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              int X = __float2int_rn(y[i]);
-#pragma unroll
-              for (int b = 0; b < 4; ++b) {
-                const int dig = (int)(int8_t)(X & 0xff);
-                d[b] |= (uint32_t)(dig & 0xff) << (8 * i);
-                X = (X - dig) >> 8;
-              }
-            }
+            for (int i = 0; i < 4; ++i) Y[i] = ((uint32_t)__float2int_rn(y[i]) + 0x80808080u) ^ 0x80808080u;
+            const uint32_t lo01 = __byte_perm(Y[0], Y[1], 0x5140), hi01 = __byte_perm(Y[0], Y[1], 0x7362);
+            const uint32_t lo23 = __byte_perm(Y[2], Y[3], 0x5140), hi23 = __byte_perm(Y[2], Y[3], 0x7362);
+            d[0] = __byte_perm(lo01, lo23, 0x5410), d[1] = __byte_perm(lo01, lo23, 0x7632);
+            d[2] = __byte_perm(hi01, hi23, 0x5410), d[3] = __byte_perm(hi01, hi23, 0x7632);
             // MMA 0: planes 3 and 2 in rows g and g + 8; MMA 1: planes 1 and 0
             const int c = 2 * (s & 1);
             qa[s / 2][c] = d[3], qa[s / 2][c + 1] = d[2], qa[s / 2][4 + c] = d[1], qa[s / 2][4 + c + 1] = d[0];
@@ -540,11 +577,12 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const Params p) {
     for (int j = 0; j < ND; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
 
     const int seg_end = min(seg.end, x1);
-    for (; x < seg_end; x += kWarps, ++ccount) {
+    for (int x = max(x0, seg.start) + warp; x < seg_end; x += kWarps) {
       load_next();
       cp_wait<STAGES - 1>();
       __syncwarp();
-      const uint8_t *kt = sm.ring[warp][ccount % STAGES];
+      const uint8_t *kt = sm.ring[warp][cslot];
+      cslot = cslot + 1 == STAGES ? 0 : cslot + 1;
       const uint8_t *vt = kt + TILE * G::kRowBytes;
       const float *ksc = (const float *)(vt + TILE * G::kRowBytes), *vsc = ksc + TILE;
       const int left = seg.len - (x - seg.start) * TILE;  // keys from the tile's first to the segment's end
@@ -770,28 +808,31 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const Params p) {
       const int c0 = seg.start / lay.chunk, c1 = (seg.end - 1) / lay.chunk;
       bool last = true;
       if (!whole) {  // the last CTA of a split segment adds the parts up
-        __threadfence();
-        __syncthreads();
-        if (threadIdx.x == 0) {
-          unsigned *cnt = p.cnt + seg.index;
-          sm.last = atomicAdd(cnt, 1u) == (unsigned)(c1 - c0);
-          if (sm.last) *cnt = 0u;
+        if (warp == 0) {  // warp 0 wrote the record
+          __syncwarp();
+          if (lane == 0) {
+            unsigned *cnt = p.cnt + seg.index;
+            __threadfence();
+            sm.last = atomicAdd(cnt, 1u) == (unsigned)(c1 - c0);
+            if (sm.last) *cnt = 0u;
+            __threadfence();
+          }
         }
         __syncthreads();
         last = sm.last;
-        __threadfence();
       } else {
         __syncthreads();  // warp 0's record is written
       }
       if (last) {
         // (a whole segment's one record is in this CTA's slot, a split one's first part in the last slot of its CTA
         // if that began with another segment)
-        const int first = whole ? 2 * (int)blockIdx.x + (seg.index != first_seg) : 2 * c0 + (seg.start != c0 * lay.chunk);
-        finish<D>(p, sm.fin, seg.seq, seg.g, c1 - c0 + 1, first, c0);
+        const int first = whole ? 2 * (int)blockIdx.x + (seg.index != first_seg)
+                                : 2 * c0 + (seg.start != cut_at<TILE, PREFIX>(p, lay, sm.cum, (int64_t)c0 * lay.chunk));
+        finish<D>(p, sm.fin, seg.seq, seg.g, whole ? 1 : c1 - c0 + 1, first, c0);
       }
     }
-    if (seg_end >= x1) break;
-    seg = find_seg<TILE, PREFIX>(p, lay, sm.cum, seg.end);
+    if (seg.next >= x1) break;
+    seg = next_seg<TILE, PREFIX>(p, sm.cum, seg);
   }
   cp_wait<0>();
 }
@@ -835,8 +876,8 @@ static void cut_prefix(Params &p, int64_t prefix_len, bool q8, int grid) {
   Prefix &c = p.pre;
   c.row_tiles = row_tiles(p.m, p.group);
   c.seg_tiles = (int)((prefix_len + tile_keys(q8) - 1) / tile_keys(q8));
-  const int segs = p.nkv * c.row_tiles, least = std::max(kMinChunk, ceil_div(segs * c.seg_tiles, grid));
-  c.pad = 1, c.chunk = even_share(segs * c.seg_tiles, segs, grid);
+  const int segs = p.nkv * c.row_tiles, share = ceil_div(segs * c.seg_tiles, grid), least = std::max(kMinChunk, share);
+  c.pad = 1, c.chunk = share;
   for (int j = 0; j < 32; ++j) {
     const int len = least + ceil_div(least * j, 64);
     if ((int64_t)segs * ceil_div(c.seg_tiles, len) <= grid) {
