@@ -35,13 +35,10 @@
 namespace egpt {
 namespace aq8 {
 
-constexpr int kWarps = 8;
-constexpr int kThreads = kWarps * 32;
 constexpr int kMaxBatch = 512;
 constexpr int kRows = 16;              // query rows per tile (the M of the MMA), and rows of a partial record
-constexpr int kCtasPerSm = 1;
-constexpr int kMinChunk = 2 * kWarps;  // tiles of a range at least
-constexpr int kExtra = 16;             // what a segment's start and end cost, in tiles
+constexpr int kMinKeys = 512;    // keys of a range at least
+constexpr int kExtraKeys = 512;  // what a segment's start and end cost, in keys
 
 struct Cache {
   const uint8_t *k, *v;
@@ -64,6 +61,7 @@ struct Params {
   Cache cache;
   const int64_t *position;
   int m, nkv, group;
+  int head_share;  // CTAs per kv head
   float scale_log2;
   float *ws;      // partial records of this launch
   unsigned *cnt;  // arrivals per (sequence, kv head); zero between calls
@@ -83,11 +81,20 @@ struct Seg {
   int len;                // keys
 };
 
-template <int D, bool Q8>
+// Shape of a CTA (one per SM) by type and query rows.
+template <bool Q8, int NR>
+struct Cfg {
+  static constexpr int kWarps = 8;
+  static constexpr int kThreads = 32 * kWarps;
+  static constexpr int kTile = Q8 ? 32 : 16;  // keys per warp tile: K and V 4 KB each at d = 128
+  static constexpr int kStages = NR == 8 ? 3 : 2;
+  static constexpr int kMinChunk = kMinKeys / kTile, kExtra = kExtraKeys / kTile;
+};
+template <int D, bool Q8, int NR>
 struct Geo {
   static constexpr int kRowBytes = Q8 ? D : 2 * D;
   static constexpr int kChunks = kRowBytes / 16;
-  static constexpr int kTile = Q8 ? 32 : 16;  // keys per warp tile: K and V 4 KB each at d = 128
+  static constexpr int kTile = Cfg<Q8, NR>::kTile;
   static constexpr int kStageBytes = 2 * kTile * kRowBytes + (Q8 ? 2 * kTile * 4 : 0);
   static constexpr int kRun = (!Q8 && D == 128) ? 8 : D / 8;  // consecutive output dims of one thread
   // chunk permutations of a row so that the fragment reads of 8 lanes hit 8 different 16-byte banks
@@ -159,7 +166,8 @@ __device__ __forceinline__ uint32_t codes_f16(uint32_t biased, uint32_t select) 
 __device__ __forceinline__ uint32_t codes_bf16(uint32_t codes, uint32_t select) {
   uint32_t r;
   const uint32_t pasted = __byte_perm(codes, 0x43434343u, select);
-  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(pasted & 0xff7fff7fu), "r"(pasted & 0xff80ff80u));
+  // (the second part with its sign set: a sum is one instruction, a difference two)
+  asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(pasted & 0xff7fff7fu), "r"((pasted & 0xff80ff80u) | 0x80008000u));
   return r;
 }
 
@@ -173,24 +181,37 @@ __device__ __forceinline__ int seq_len(const Params &p, int i) {
 }
 
 __host__ __device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
+// The same for 0 <= a, 0 < b, a + b <= 2^24, where a float quotient is off by one at most.
+__device__ __forceinline__ int ceil_div_small(int a, int b) {
+  const int n = a + b - 1;
+  int q = (int)((float)n * __frcp_rn((float)b));
+  const int r = n - q * b;
+  return q + (r >= b) - (r < 0);
+}
 
 // cum[i] = places of the sequences before i (one kv head). The ranges: with up to 32 sequences the lanes try range lengths
 // from the even share of the tiles up to 1.5 times it, and the smallest that gives at most one range per CTA is taken;
 // failing that, and for more sequences, equal stretches. Every thread of the CTA calls it.
-template <int TILE>
-__device__ Layout make_layout(const Params &p, int *cum, int *scratch) {
+template <typename C>
+__device__ __forceinline__ Layout make_layout(const Params &p, int *cum, int *len_of, int *scratch) {
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, grid = (int)gridDim.x;
   Layout l;
   l.pad = 1;
   if (p.m <= 32) {  // every warp for itself
-    const int tiles = lane < p.m ? ceil_div(seq_len(p, lane), TILE) : 0;
-    const int least = max(kMinChunk, ceil_div(p.nkv * __reduce_add_sync(0xffffffffu, tiles), grid));
-    const int len = least + ceil_div(least * lane, 64);
-    int parts = 0;
-    for (int i = 0; i < p.m; ++i) parts += ceil_div(__shfl_sync(0xffffffffu, tiles, i), len);
-    const unsigned fits = __ballot_sync(0xffffffffu, p.nkv * parts <= grid);
-    if (fits) l.pad = __shfl_sync(0xffffffffu, len, __ffs(fits) - 1);
-    const int places = fits ? ceil_div(tiles, l.pad) * l.pad : (tiles ? tiles + kExtra : 0);
+    const int keys = lane < p.m ? seq_len(p, lane) : 0, tiles = ceil_div(keys, C::kTile);
+    bool fits = true;
+    if (p.m == 1 && p.head_share) {  // all CTAs of a head for its one segment
+      l.pad = max(C::kMinChunk, ceil_div_small(__shfl_sync(0xffffffffu, tiles, 0), p.head_share));
+    } else {
+      const int share = ceil_div(p.nkv * __reduce_add_sync(0xffffffffu, tiles), grid);
+      const int least = max(C::kMinChunk, share), len = least + (least * lane + 63) / 64;
+      int parts = 0;
+      for (int i = 0; i < p.m; ++i) parts += ceil_div_small(__shfl_sync(0xffffffffu, tiles, i), len);
+      const unsigned good = __ballot_sync(0xffffffffu, p.nkv * parts <= grid);
+      fits = good != 0u;
+      if (fits) l.pad = __shfl_sync(0xffffffffu, len, __ffs(good) - 1);
+    }
+    const int places = fits ? ceil_div_small(tiles, l.pad) * l.pad : (tiles ? tiles + C::kExtra : 0);
     int inc = places;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -198,17 +219,18 @@ __device__ Layout make_layout(const Params &p, int *cum, int *scratch) {
       if (lane >= o) inc += up;
     }
     if (warp == 0) {
-      cum[lane] = inc - places;
+      cum[lane] = inc - places, len_of[lane] = keys;
       if (lane == 31) cum[32] = inc;
     }
     __syncthreads();
   } else {
-    constexpr int kPer = kMaxBatch / kThreads;
+    constexpr int kPer = kMaxBatch / C::kThreads;
     int places[kPer], sum = 0;
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
-      const int i = t * kPer + e, tiles = i < p.m ? ceil_div(seq_len(p, i), TILE) : 0;
-      places[e] = tiles ? tiles + kExtra : 0;
+      const int i = t * kPer + e, keys = i < p.m ? seq_len(p, i) : 0, tiles = ceil_div(keys, C::kTile);
+      len_of[i] = keys;
+      places[e] = tiles ? tiles + C::kExtra : 0;
       sum += places[e];
     }
     int inc = sum;
@@ -226,22 +248,22 @@ __device__ Layout make_layout(const Params &p, int *cum, int *scratch) {
       cum[t * kPer + e] = before;
       before += places[e];
     }
-    if (t == kThreads - 1) cum[kMaxBatch] = before;
+    if (t == C::kThreads - 1) cum[kMaxBatch] = before;
     __syncthreads();
   }
   l.total = p.nkv * cum[p.m];
   l.chunk = l.pad > 1 ? l.pad : max(1, ceil_div(l.total, grid));
-  l.uncut = max(kMinChunk, l.chunk / 2);
+  l.uncut = max(C::kMinChunk, l.chunk / 2);
   return l;
 }
 template <int TILE>
-__device__ __forceinline__ Seg own_seg(const Params &p, const int *cum, int i, int g) {
+__device__ __forceinline__ Seg own_seg(const Params &p, const int *cum, const int *len_of, int i, int g) {
   Seg s;
   const int places = cum[i + 1] - cum[i];
   s.seq = i, s.g = g, s.tile = 0;
   s.index = i * p.nkv + g;
   s.start = p.nkv * cum[i] + g * places, s.next = s.start + places;
-  s.len = (int)p.position[i] + 1;
+  s.len = len_of[i];
   s.end = s.start + ceil_div(s.len, TILE);
   return s;
 }
@@ -256,7 +278,7 @@ __device__ __forceinline__ Seg prefix_seg(const Params &p, int index) {
 }
 // The segment that holds place x < total.
 template <int TILE, bool PREFIX>
-__device__ __forceinline__ Seg find_seg(const Params &p, const int *cum, int x) {
+__device__ __forceinline__ Seg find_seg(const Params &p, const int *cum, const int *len_of, int x) {
   if (PREFIX) return prefix_seg(p, x / (ceil_div(p.pre.seg_tiles, p.pre.pad) * p.pre.pad));
   int lo = 0, hi = p.m - 1;  // the last sequence whose places start at or before x: it has some
   while (lo < hi) {
@@ -264,11 +286,11 @@ __device__ __forceinline__ Seg find_seg(const Params &p, const int *cum, int x) 
     if (p.nkv * cum[mid] <= x) lo = mid;
     else hi = mid - 1;
   }
-  return own_seg<TILE>(p, cum, lo, (x - p.nkv * cum[lo]) / (cum[lo + 1] - cum[lo]));
+  return own_seg<TILE>(p, cum, len_of, lo, (x - p.nkv * cum[lo]) / (cum[lo + 1] - cum[lo]));
 }
 // The segment after s, whose next is < total.
 template <int TILE, bool PREFIX>
-__device__ __forceinline__ Seg next_seg(const Params &p, const int *cum, const Seg &s) {
+__device__ __forceinline__ Seg next_seg(const Params &p, const int *cum, const int *len_of, const Seg &s) {
   if (PREFIX) return prefix_seg(p, s.index + 1);
   if (s.g + 1 < p.nkv) {
     Seg r = s;
@@ -278,14 +300,13 @@ __device__ __forceinline__ Seg next_seg(const Params &p, const int *cum, const S
   }
   int i = s.seq + 1;
   while (cum[i + 1] == cum[i]) ++i;
-  return own_seg<TILE>(p, cum, i, 0);
+  return own_seg<TILE>(p, cum, len_of, i, 0);
 }
 // Where a stretch whose even cut is place x begins: not past the tiles of a segment, nor inside a short one.
 template <int TILE, bool PREFIX>
-__device__ __forceinline__ int cut_at(const Params &p, const Layout &l, const int *cum, int64_t x) {
+__device__ __noinline__ int cut_at(const Params &p, const Layout &l, const int *cum, const int *len_of, int64_t x) {
   if (x >= l.total) return l.total;
-  if (l.pad > 1) return (int)x;
-  const Seg s = find_seg<TILE, PREFIX>(p, cum, (int)x);
+  const Seg s = find_seg<TILE, PREFIX>(p, cum, len_of, (int)x);
   return x >= s.end || (x > s.start && s.end - s.start <= l.uncut) ? s.next : (int)x;
 }
 // A partial record: kRows rows of (D accumulators), then kRows maxima and kRows sums.
@@ -294,115 +315,124 @@ __device__ __forceinline__ float *record(const Params &p, int index) {
   return p.ws + (int64_t)index * kRows * (D + 2);
 }
 
-// What one (sequence, head) row's parts add up to, one warp per row or per share of a row's records.
-template <int D>
+// A row's records, added up by the warps that share it.
+template <int D, int WARPS>
 struct Finish {
-  float m[kRows], l[kRows];
-  float a[kRows][D];
+  float a[WARPS][D];
 };
 
-template <int D, bool Q8, int NR, int STAGES>
+template <int D, bool Q8, int NR>
 struct Smem {
-  uint8_t ring[kWarps][STAGES][Geo<D, Q8>::kStageBytes];
+  static constexpr int kWarps = Cfg<Q8, NR>::kWarps, kPass = NR / 2;
+  uint8_t ring[kWarps][Cfg<Q8, NR>::kStages][Geo<D, Q8, NR>::kStageBytes];
   union {
-    float merge[kWarps / 2][NR / 8 * (D / 4 + 2)][32];  // half of the warps' accumulators, maxima and sums
-    Finish<D> fin;
+    float merge[kWarps][kPass][D];  // the warps' accumulators, kPass rows at a time
+    Finish<D, kWarps> fin;
   };
-  int cum[kMaxBatch + 1];
+  float warp_m[kWarps][NR], warp_l[kWarps][NR];  // their maxima and sums
+  float row_m[NR], row_l[NR];                    // and the CTA's
+  int cum[kMaxBatch + 1], len[kMaxBatch];
   int scratch[kWarps];
   int last;
 };
 
 // out[i, heads of g] = the own_n records of the sequence's own keys (the first in slot `first`, then slots
-// 2 (c0 + k)) and the prefix's, added up. A warp takes a row, or with fewer rows than warps every parts-th record of a
-// row: lanes read up to 32 records' maxima and sums at once, then the accumulators follow with independent loads. The
-// order is fixed by the shapes. Every thread of the CTA calls it.
-template <int D>
-__device__ void finish(const Params &p, Finish<D> &f, int i, int g, int own_n, int first, int c0) {
+// 2 (c0 + k)) and the prefix's, added up: a warp takes a row, or with fewer rows than warps every parts-th record of
+// one. Lanes read the maxima and sums of 32 records at once while the first accumulators are on their way, so a short
+// list costs one round trip. The order is fixed by the shapes. Every thread of the CTA calls it.
+template <int D, int WARPS>
+__device__ __noinline__ void finish(const Params &p, Finish<D, WARPS> &f, int i, int g, int own_n, int first, int c0) {
   constexpr int N = D / 32;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int parts = max(1, kWarps / p.group);
+  const int parts = p.group < WARPS ? WARPS / p.group : 1;
+  const int part = parts > 1 ? warp / p.group : 0;
   if (p.pre.rec) pdl_wait();  // the launch over the prefix has finished
-  for (int unit = warp; unit < p.group * parts; unit += kWarps) {
-    const int j = unit % p.group, part = unit / p.group;
-    int pre_n = 0, pre_row = 0, pre_rows = kRows;
+#pragma unroll 1
+  for (int j = warp - part * p.group; j < p.group && part < parts; j += WARPS) {
+    const float *pre0 = nullptr;  // row j's accumulators in the prefix's first record
+    int pre_n = 0, pre_rows = kRows, pre_row = 0;
     int64_t pre_step = 0;
-    const float *pre0 = nullptr;
     if (p.pre.rec) {
       if (p.pre.big) {
         const int tile = i / p.pre.seqs, pair = tile / 2;
         const bool two = 2 * pair + 1 < p.pre.tiles;  // the pair's streams are two tiles, or both this one
         pre_n = two ? p.pre.ranges : 2 * p.pre.ranges;
         pre_step = two ? 2 * apx::kRecord : apx::kRecord;
-        pre0 = p.pre.rec + ((int64_t)(g * p.pre.pairs + pair) * p.pre.ranges * 2 + (two ? tile & 1 : 0)) * apx::kRecord;
-        pre_row = (i % p.pre.seqs) * p.group + j, pre_rows = apx::kRowsT;
+        pre_row = (i - tile * p.pre.seqs) * p.group + j, pre_rows = apx::kRowsT;
+        pre0 = p.pre.rec + ((int64_t)(g * p.pre.pairs + pair) * p.pre.ranges * 2 + (two ? tile & 1 : 0)) * apx::kRecord +
+               pre_row * D;
       } else {
         const int flat = i * p.group + j, seg = g * p.pre.row_tiles + flat / kRows;
         const int start = seg * ceil_div(p.pre.seg_tiles, p.pre.pad) * p.pre.pad;
         const int pc0 = start / p.pre.chunk;
         pre_n = (start + p.pre.seg_tiles - 1) / p.pre.chunk - pc0 + 1;
         pre_step = kRows * (D + 2);
-        pre0 = p.pre.rec + (int64_t)(pc0 + seg) * pre_step;
         pre_row = flat % kRows;
+        pre0 = p.pre.rec + (int64_t)(pc0 + seg) * pre_step + pre_row * D;
       }
     }
+    auto row_of = [&](int k) -> const float * {  // row j's accumulators in record k
+      return k < own_n ? p.ws + (int64_t)(k == 0 ? first : 2 * (c0 + k)) * (kRows * (D + 2)) + j * D
+                       : pre0 + (int64_t)(k - own_n) * pre_step;
+    };
     const int n = own_n + pre_n;
     float M = -INFINITY, lsum = 0.f, a[N];
 #pragma unroll
     for (int e = 0; e < N; ++e) a[e] = 0.f;
-    for (int k0 = part; k0 < n; k0 += 32 * parts) {
-      const int k = k0 + lane * parts, cnt = min(32, ceil_div(n - k0, parts));
-      const float *row = p.ws;
+#pragma unroll 1
+    for (int k0 = 0; k0 < n; k0 += 32) {
       float mk = -INFINITY, lk = 0.f;
-      if (k < n) {
-        const bool own = k < own_n;
+      if (k0 + lane < n) {
+        const bool own = k0 + lane < own_n;
         const int rows = own ? kRows : pre_rows, r = own ? j : pre_row;
-        const float *rec = own ? p.ws + (int64_t)(k == 0 ? first : 2 * (c0 + k)) * kRows * (D + 2)
-                               : pre0 + (int64_t)(k - own_n) * pre_step;
-        mk = __ldcg(rec + rows * D + r), lk = __ldcg(rec + rows * D + rows + r);
-        row = rec + r * D;
+        const float *stat = row_of(k0 + lane) + (rows - r) * D + r;  // past the accumulators: maxima, then sums
+        mk = __ldcg(stat), lk = __ldcg(stat + rows);
       }
-      constexpr int kBatch = 8;  // records in flight: the first of them beside the maxima and sums
-      float v[kBatch][N];
-      auto fetch = [&](int c) {
-#pragma unroll
-        for (int b = 0; b < kBatch; ++b) {  // (lanes past the count have a readable address, and factor zero)
-          const float *src = (const float *)__shfl_sync(0xffffffffu, (unsigned long long)row, (c + b) & 31) + N * lane;
-          if constexpr (N == 4) {
-            const float4 t = __ldcg((const float4 *)src);
-            v[b][0] = t.x, v[b][1] = t.y, v[b][2] = t.z, v[b][3] = t.w;
-          } else if constexpr (N == 2) {
-            const float2 t = __ldcg((const float2 *)src);
-            v[b][0] = t.x, v[b][1] = t.y;
-          } else {
-            v[b][0] = __ldcg(src);
-          }
-        }
-      };
-      fetch(0);
-      const float mx = fmaxf(M, warp_max(lk != 0.f ? mk : -INFINITY));
-      const float mz = mx == -INFINITY ? 0.f : mx;
-      const float fk = lk != 0.f ? ex2(mk - mz) : 0.f, fo = ex2(M - mz);  // a record without keys has no accumulators
-      M = mx;
-      lsum = lsum * fo + warp_sum(lk * fk);
-#pragma unroll
-      for (int e = 0; e < N; ++e) a[e] *= fo;
-      for (int c = 0; c < cnt; c += kBatch) {
-        if (c) fetch(c);
+      const int cnt = min(32, n - k0);
+      float fk = 0.f;
+      int c = part;
+      do {
+        constexpr int kBatch = 8;
+        float v[kBatch][N];
 #pragma unroll
         for (int b = 0; b < kBatch; ++b) {
-          const float fc = __shfl_sync(0xffffffffu, fk, (c + b) & 31);
-#pragma unroll
-          for (int e = 0; e < N; ++e) a[e] += fc == 0.f ? 0.f : v[b][e] * fc;
+          if (c + b * parts < cnt) {
+            const float *src = row_of(k0 + c + b * parts) + N * lane;
+            if constexpr (N == 4) {
+              const float4 t = __ldcg((const float4 *)src);
+              v[b][0] = t.x, v[b][1] = t.y, v[b][2] = t.z, v[b][3] = t.w;
+            } else if constexpr (N == 2) {
+              const float2 t = __ldcg((const float2 *)src);
+              v[b][0] = t.x, v[b][1] = t.y;
+            } else {
+              v[b][0] = __ldcg(src);
+            }
+          }
         }
-      }
-    }
-    if (parts > 1) {
-      if (lane == 0) f.m[unit] = M, f.l[unit] = lsum;
+        if (c == part) {  // a record without keys (sum 0) has no accumulators
+          const float mx = fmaxf(M, warp_max(lk != 0.f ? mk : -INFINITY)), mz = mx == -INFINITY ? 0.f : mx;
+          const float fo = ex2(M - mz);
+          fk = lk != 0.f ? ex2(mk - mz) : 0.f;
+          M = mx;
+          lsum = lsum * fo + warp_sum(lk * fk);
 #pragma unroll
-      for (int e = 0; e < N; ++e) f.a[unit][N * lane + e] = a[e];
+          for (int e = 0; e < N; ++e) a[e] *= fo;
+        }
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+          const float fc = __shfl_sync(0xffffffffu, fk, (c + b * parts) & 31);
+          if (c + b * parts < cnt && fc != 0.f)
+#pragma unroll
+            for (int e = 0; e < N; ++e) a[e] += v[b][e] * fc;
+        }
+        c += kBatch * parts;
+      } while (c < cnt);
+    }
+    const float inv = lsum == 0.f ? 0.f : 1.f / lsum;  // no keys at all: zeros
+    if (parts > 1) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) f.a[part * p.group + j][N * lane + e] = a[e] * inv;
     } else {
-      const float inv = lsum == 0.f ? 0.f : 1.f / lsum;  // no keys at all: zeros
 #pragma unroll
       for (int e = 0; e < N; ++e)
         p.out[i * p.ldo + (int64_t)(g * p.group + j) * D + N * lane + e] = f32_to_bf16_bits(a[e] * inv);
@@ -410,17 +440,11 @@ __device__ void finish(const Params &p, Finish<D> &f, int i, int g, int own_n, i
   }
   if (parts == 1) return;
   __syncthreads();
-  for (int e = threadIdx.x; e < p.group * D; e += kThreads) {
-    const int j = e / D, dd = e - j * D;
-    float M = -INFINITY, lsum = 0.f, a = 0.f;
-    for (int part = 0; part < parts; ++part) M = fmaxf(M, f.m[part * p.group + j]);
-    const float mz = M == -INFINITY ? 0.f : M;
-    for (int part = 0; part < parts; ++part) {
-      const float fp = ex2(f.m[part * p.group + j] - mz);
-      lsum += f.l[part * p.group + j] * fp;
-      a += f.a[part * p.group + j][dd] * fp;
-    }
-    p.out[i * p.ldo + (int64_t)(g * p.group + j) * D + dd] = f32_to_bf16_bits(lsum == 0.f ? 0.f : a / lsum);
+#pragma unroll 1
+  for (int e = threadIdx.x; e < p.group * D; e += 32 * WARPS) {
+    float a = 0.f;
+    for (int q = 0; q < parts; ++q) a += f.a[q * p.group + e / D][e % D];
+    p.out[i * p.ldo + (int64_t)g * p.group * D + e] = f32_to_bf16_bits(a);
   }
   __syncthreads();  // f is free again
 }
@@ -428,10 +452,12 @@ __device__ void finish(const Params &p, Finish<D> &f, int i, int g, int own_n, i
 // NR: query rows in use, 8 or 16. PREFIX: the segments of the shared prefix, every (CTA, segment) pair leaving a record in
 // slot CTA + segment; else the sequences' own keys, a CTA's at most two split segments leaving theirs in slots 2 CTA
 // and 2 CTA + 1, and the last CTA of a segment adding all of it up.
-template <int D, bool Q8, int NR, bool PREFIX, int STAGES>
-__global__ void __launch_bounds__(kThreads) attn_kernel(const Params p) {
-  using G = Geo<D, Q8>;
-  using S = Smem<D, Q8, NR, STAGES>;
+template <int D, bool Q8, int NR, bool PREFIX>
+__global__ void __launch_bounds__(Cfg<Q8, NR>::kThreads, 1) attn_kernel(const Params p) {
+  using C = Cfg<Q8, NR>;
+  using G = Geo<D, Q8, NR>;
+  using S = Smem<D, Q8, NR>;
+  constexpr int kWarps = C::kWarps, STAGES = C::kStages;
   constexpr int TILE = G::kTile, NT = TILE / 8, ND = D / 8, NC = NR == 16 ? 4 : 2;  // NC: accumulators kept
   constexpr bool PLANES = Q8 && NR == 8;  // scores by int8 MMAs on the digits of q
   extern __shared__ __align__(16) uint8_t smem_raw[];
@@ -445,14 +471,17 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const Params p) {
     lay.chunk = p.pre.chunk, lay.pad = p.pre.pad, lay.uncut = 0;
     lay.total = p.nkv * p.pre.row_tiles * ceil_div(p.pre.seg_tiles, lay.pad) * lay.pad;
   } else {
-    lay = make_layout<TILE>(p, sm.cum, sm.scratch);
+    lay = make_layout<C>(p, sm.cum, sm.len, sm.scratch);
     for (int e = blockIdx.x; e < p.m * p.nkv; e += gridDim.x)  // sequences without keys of their own
-      if (sm.cum[e / p.nkv + 1] == sm.cum[e / p.nkv]) finish<D>(p, sm.fin, e / p.nkv, e % p.nkv, 0, 0, 0);
+      if (sm.cum[e / p.nkv + 1] == sm.cum[e / p.nkv]) finish<D, kWarps>(p, sm.fin, e / p.nkv, e % p.nkv, 0, 0, 0);
   }
-  const int x0 = cut_at<TILE, PREFIX>(p, lay, sm.cum, (int64_t)blockIdx.x * lay.chunk);
-  int x1 = cut_at<TILE, PREFIX>(p, lay, sm.cum, (int64_t)(blockIdx.x + 1) * lay.chunk);
+  int x0 = (int)min((int64_t)lay.total, (int64_t)blockIdx.x * lay.chunk), x1 = min(lay.total, x0 + lay.chunk);
+  if (lay.pad == 1) {
+    x0 = cut_at<TILE, PREFIX>(p, lay, sm.cum, sm.len, x0);
+    x1 = cut_at<TILE, PREFIX>(p, lay, sm.cum, sm.len, (int64_t)(blockIdx.x + 1) * lay.chunk);
+  }
   if (x0 >= x1) return;
-  Seg seg = find_seg<TILE, PREFIX>(p, sm.cum, x0);
+  Seg seg = find_seg<TILE, PREFIX>(p, sm.cum, sm.len, x0);
   if (lay.pad > 1) x1 = min(x1, seg.end);
 
   // ---- this warp's loads: every kWarps-th tile of a segment's part, STAGES - 1 tiles ahead. 32 lanes take 512 consecutive bytes
@@ -466,7 +495,7 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const Params p) {
   const uint32_t v_dst = lr * G::kRowBytes + ((lc ^ G::v_swz(lr)) * 16);
   auto load_next = [&]() {
     while (lx >= ls.end && ls.next < x1) {
-      ls = next_seg<TILE, PREFIX>(p, sm.cum, ls);
+      ls = next_seg<TILE, PREFIX>(p, sm.cum, sm.len, ls);
       lx = ls.start + warp;
     }
     if (lx < min(ls.end, x1)) {
@@ -475,23 +504,25 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const Params p) {
       const int key0 = (lx - ls.start) * TILE, left = ls.len - key0;
       const int64_t row0 = (PREFIX ? ls.g : (int64_t)ls.seq * p.nkv + ls.g) * c.cap + key0;
       const uint8_t *kb = c.k + row0 * G::kRowBytes + lane * 16, *vb = c.v + row0 * G::kRowBytes + lane * 16;
+      // v_swz(it kStep + lr) = v_swz(it kStep) ^ v_swz(lr) (the row bits it uses do not carry)
+      const uint32_t kd = st + k_dst, vd = st + ring + TILE * G::kRowBytes;
+      if (left >= TILE) {
 #pragma unroll
-      for (int it = 0; it < TILE / kStep; ++it) {
-        // v_swz(it kStep + lr) = v_swz(it kStep) ^ v_swz(lr) (the row bits it uses do not carry)
-        const uint32_t kd = st + k_dst + it * 512;
-        const uint32_t vd = st + ring + TILE * G::kRowBytes + (v_dst ^ (G::v_swz(it * kStep) * 16)) + it * 512;
-        if (left >= TILE) {
-          cp16(kd, kb + it * 512);
-          cp16(vd, vb + it * 512);
-        } else {
+        for (int it = 0; it < TILE / kStep; ++it) {
+          cp16(kd + it * 512, kb + it * 512);
+          cp16(vd + (v_dst ^ (G::v_swz(it * kStep) * 16)) + it * 512, vb + it * 512);
+        }
+      } else {
+#pragma unroll 1
+        for (int it = 0; it < TILE / kStep; ++it) {
           const bool in = it * kStep + lr < left;
-          cp16z(kd, in ? kb + it * 512 : c.k, in ? 16 : 0);
-          cp16z(vd, in ? vb + it * 512 : c.v, in ? 16 : 0);
+          cp16z(kd + it * 512, in ? kb + it * 512 : c.k, in ? 16 : 0);
+          cp16z(vd + (v_dst ^ (G::v_swz(it * kStep) * 16)) + it * 512, in ? vb + it * 512 : c.v, in ? 16 : 0);
         }
       }
       if (Q8) {
+        const uint32_t sc = ring + st + 2 * TILE * G::kRowBytes + lane * 4;  // [ks of the tile][vs of the tile]
         const bool in = lane < left;
-        const uint32_t sc = ring + st + 2 * TILE * G::kRowBytes + lane * 4;
         cp4(sc, c.ks + row0 + (in ? lane : 0), in ? 4 : 0);
         cp4(sc + TILE * 4, c.vs + row0 + (in ? lane : 0), in ? 4 : 0);
       }
@@ -500,7 +531,31 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const Params p) {
     lx += kWarps;
     lslot = lslot + 1 == STAGES ? 0 : lslot + 1;
   };
+  // the segment's query rows, dims d0 .. d0 + 3 of every 16-dim step: those of the key words that this thread loads
+  uint2 qw[NR / 8][D / 16];
+  auto load_q = [&](const Seg &sg) {
 #pragma unroll
+    for (int hh = 0; hh < NR / 8; ++hh) {
+      const int r = g + 8 * hh;
+      int64_t tok = -1;
+      int h = 0;
+      if (PREFIX) {
+        const int flat = sg.tile * kRows + r;
+        if (flat < p.m * p.group) tok = flat / p.group, h = sg.g * p.group + flat % p.group;
+      } else if (r < p.group) {
+        tok = sg.seq, h = sg.g * p.group + r;
+      }
+      const uint16_t *qr = p.q + (tok >= 0 ? tok * p.ldq + (int64_t)h * D : 0);
+#pragma unroll
+      for (int s = 0; s < D / 16; ++s) {
+        const int d0 = Q8 ? (D == 32 ? 8 * t + 4 * s : 16 * (t + 4 * (s / 4)) + 4 * (s % 4))
+                          : 8 * (t + 4 * (s / 2)) + 4 * (s % 2);
+        qw[hh][s] = tok >= 0 ? *(const uint2 *)(qr + d0) : make_uint2(0u, 0u);
+      }
+    }
+  };
+  load_q(seg);  // before the keys and values queue up in front of it
+#pragma unroll 1
   for (int s = 0; s < STAGES - 1; ++s) load_next();
 
   int cslot = 0;
@@ -511,25 +566,11 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const Params p) {
     float rowfac[2] = {p.scale_log2, p.scale_log2};  // and for int8 the power of two that q was divided by
 #pragma unroll
     for (int hh = 0; hh < NR / 8; ++hh) {
-      const int r = g + 8 * hh;
-      int64_t tok = -1;
-      int h = 0;
-      if (PREFIX) {
-        const int flat = seg.tile * kRows + r;
-        if (flat < p.m * p.group) tok = flat / p.group, h = seg.g * p.group + flat % p.group;
-      } else if (r < p.group) {
-        tok = seg.seq, h = seg.g * p.group + r;
-      }
-      const uint16_t *qr = p.q + (tok >= 0 ? tok * p.ldq + (int64_t)h * D : 0);
-      uint2 w[D / 16];  // dims d0 .. d0 + 3 of every 16-dim step: those of the key words that this thread loads
+      const uint2(&w)[D / 16] = qw[hh];
       uint32_t amax2 = 0u;  // the largest magnitudes of the even and odd elements, as bf16 bits (NaN above infinity)
 #pragma unroll
-      for (int s = 0; s < D / 16; ++s) {
-        const int d0 = Q8 ? (D == 32 ? 8 * t + 4 * s : 16 * (t + 4 * (s / 4)) + 4 * (s % 4))
-                          : 8 * (t + 4 * (s / 2)) + 4 * (s % 2);
-        w[s] = tok >= 0 ? *(const uint2 *)(qr + d0) : make_uint2(0u, 0u);
+      for (int s = 0; s < D / 16; ++s)
         if (Q8) amax2 = __vmaxu2(amax2, __vmaxu2(w[s].x & 0x7fff7fffu, w[s].y & 0x7fff7fffu));
-      }
       if (Q8) {
         amax2 = __vmaxu2(amax2, __shfl_xor_sync(0xffffffffu, amax2, 1));
         amax2 = __vmaxu2(amax2, __shfl_xor_sync(0xffffffffu, amax2, 2));
@@ -730,118 +771,105 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const Params p) {
 #pragma unroll
       for (int j = 0; j < ND; ++j) acc[j][0] += acc[j][2], acc[j][1] += acc[j][3];
     }
-    // ---- the segment is done: the warps' states meet in warp 0, the upper half of them handing theirs down each time
+    // ---- the segment is done: the warps' states, each relative to the largest maximum, are added up in shared memory
 #pragma unroll
     for (int hh = 0; hh < NR / 8; ++hh) {
       l_part[hh] += __shfl_xor_sync(0xffffffffu, l_part[hh], 1);
       l_part[hh] += __shfl_xor_sync(0xffffffffu, l_part[hh], 2);
+      if (t == 0) sm.warp_m[warp][g + 8 * hh] = m_run[hh], sm.warp_l[warp][g + 8 * hh] = l_part[hh];
     }
+    __syncthreads();
+    float fac[NR / 8];
 #pragma unroll
-    for (int half = kWarps / 2; half >= 1; half >>= 1) {
-      __syncthreads();  // the buffer's last readers are done
-      if (warp >= half && warp < 2 * half) {
-        float(*b)[32] = sm.merge[warp - half];
+    for (int hh = 0; hh < NR / 8; ++hh) {
+      float mx = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < ND; ++j)
+      for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, sm.warp_m[w][g + 8 * hh]);
+      fac[hh] = ex2(m_run[hh] - (mx == -INFINITY ? 0.f : mx));
+    }
+    if (threadIdx.x < NR) {
+      float mx = -INFINITY, l = 0.f;
 #pragma unroll
-          for (int c = 0; c < NC; ++c) b[j * NC + c][lane] = acc[j][c];
+      for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, sm.warp_m[w][threadIdx.x]);
 #pragma unroll
-        for (int hh = 0; hh < NR / 8; ++hh) b[ND * NC + 2 * hh][lane] = m_run[hh], b[ND * NC + 2 * hh + 1][lane] = l_part[hh];
-      }
-      __syncthreads();
-      if (warp < half) {
-        float(*b)[32] = sm.merge[warp];
-        float fa[2], fb[2];
-#pragma unroll
-        for (int hh = 0; hh < NR / 8; ++hh) {
-          const float mo = b[ND * NC + 2 * hh][lane], m_new = fmaxf(m_run[hh], mo);
-          const float mz = m_new == -INFINITY ? 0.f : m_new;
-          fa[hh] = ex2(m_run[hh] - mz), fb[hh] = ex2(mo - mz);
-          m_run[hh] = m_new;
-          l_part[hh] = l_part[hh] * fa[hh] + b[ND * NC + 2 * hh + 1][lane] * fb[hh];
-        }
-#pragma unroll
-        for (int j = 0; j < ND; ++j)
-#pragma unroll
-          for (int c = 0; c < NC; ++c) acc[j][c] = acc[j][c] * fa[c / 2] + b[j * NC + c][lane] * fb[c / 2];
-      }
+      for (int w = 0; w < kWarps; ++w)
+        l += sm.warp_l[w][threadIdx.x] * ex2(sm.warp_m[w][threadIdx.x] - (mx == -INFINITY ? 0.f : mx));
+      sm.row_m[threadIdx.x] = mx, sm.row_l[threadIdx.x] = l;
     }
     const bool whole = seg.start >= x0 && seg.end <= x1;
-    if (warp == 0) {
-      if (!PREFIX && whole && !p.pre.rec) {
+    const bool final = !PREFIX && whole && !p.pre.rec;
+    const int rows = PREFIX ? kRows : p.group;
+    float *rec = record<D>(p, PREFIX ? (int)blockIdx.x + seg.index : 2 * (int)blockIdx.x + (seg.index != first_seg));
+    constexpr int kPass = S::kPass;
+#pragma unroll 1
+    for (int r0 = 0; r0 < rows; r0 += kPass) {
+      if (r0) __syncthreads();  // the last pass has been read
 #pragma unroll
-        for (int hh = 0; hh < NR / 8; ++hh) {
-          const int r = g + 8 * hh;
-          if (r < p.group) {
-            const float inv = 1.f / l_part[hh];
-            uint16_t *dst = p.out + seg.seq * p.ldo + (int64_t)(seg.g * p.group + r) * D;
+      for (int hh = 0; hh < NR / 8; ++hh) {
+        const int r = g + 8 * hh - r0;
+        if (r >= 0 && r < kPass && r + r0 < rows) {
 #pragma unroll
-            for (int j = 0; j < ND; j += 4)
+          for (int j = 0; j < ND; j += 4)
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const int c = 2 * hh + e;
-                *(uint2 *)(dst + G::out_dim(j, e, t)) = make_uint2(bf16x2(acc[j][c] * inv, acc[j + 1][c] * inv),
-                                                                   bf16x2(acc[j + 2][c] * inv, acc[j + 3][c] * inv));
-              }
-          }
-        }
-      } else {
-        float *rec = record<D>(p, PREFIX ? (int)blockIdx.x + seg.index : 2 * (int)blockIdx.x + (seg.index != first_seg));
-        const int rows = PREFIX ? kRows : p.group;
-#pragma unroll
-        for (int hh = 0; hh < NR / 8; ++hh) {
-          const int r = g + 8 * hh;
-          if (r < rows) {
-#pragma unroll
-            for (int j = 0; j < ND; j += 4)
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const int c = 2 * hh + e;
-                *(float4 *)(rec + r * D + G::out_dim(j, e, t)) = make_float4(acc[j][c], acc[j + 1][c], acc[j + 2][c], acc[j + 3][c]);
-              }
-            if (t == 0) rec[kRows * D + r] = m_run[hh], rec[kRows * D + kRows + r] = l_part[hh];
-          }
+            for (int e = 0; e < 2; ++e) {
+              const int c = 2 * hh + e;
+              *(float4 *)&sm.merge[warp][r][G::out_dim(j, e, t)] =
+                  make_float4(acc[j][c] * fac[hh], acc[j + 1][c] * fac[hh], acc[j + 2][c] * fac[hh], acc[j + 3][c] * fac[hh]);
+            }
         }
       }
+      __syncthreads();
+#pragma unroll 1
+      for (int e = threadIdx.x; e < min(kPass, rows - r0) * D; e += C::kThreads) {
+        float a = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) a += sm.merge[w][e / D][e % D];
+        if (final) p.out[seg.seq * p.ldo + (int64_t)(seg.g * p.group + r0) * D + e] = f32_to_bf16_bits(a / sm.row_l[r0 + e / D]);
+        else rec[r0 * D + e] = a;
+      }
+    }
+    if (!final && threadIdx.x < rows) {
+      rec[kRows * D + threadIdx.x] = sm.row_m[threadIdx.x];
+      rec[kRows * D + kRows + threadIdx.x] = sm.row_l[threadIdx.x];
     }
     if (!PREFIX && (!whole || p.pre.rec)) {
       const int c0 = seg.start / lay.chunk, c1 = (seg.end - 1) / lay.chunk;
       bool last = true;
       if (!whole) {  // the last CTA of a split segment adds the parts up
-        if (warp == 0) {  // warp 0 wrote the record
-          __syncwarp();
-          if (lane == 0) {
-            unsigned *cnt = p.cnt + seg.index;
-            __threadfence();
-            sm.last = atomicAdd(cnt, 1u) == (unsigned)(c1 - c0);
-            if (sm.last) *cnt = 0u;
+        __threadfence();
+        __syncthreads();
+        if (threadIdx.x == 0) {
+          unsigned *cnt = p.cnt + seg.index;
+          sm.last = atomicAdd(cnt, 1u) == (unsigned)(c1 - c0);
+          if (sm.last) {
+            *cnt = 0u;
             __threadfence();
           }
         }
         __syncthreads();
         last = sm.last;
       } else {
-        __syncthreads();  // warp 0's record is written
+        __syncthreads();  // the record is written
       }
       if (last) {
         // (a whole segment's one record is in this CTA's slot, a split one's first part in the last slot of its CTA
         // if that began with another segment)
         const int first = whole ? 2 * (int)blockIdx.x + (seg.index != first_seg)
-                                : 2 * c0 + (seg.start != cut_at<TILE, PREFIX>(p, lay, sm.cum, (int64_t)c0 * lay.chunk));
-        finish<D>(p, sm.fin, seg.seq, seg.g, whole ? 1 : c1 - c0 + 1, first, c0);
+                                : 2 * c0 + (lay.pad == 1 && seg.start != cut_at<TILE, PREFIX>(p, lay, sm.cum, sm.len, (int64_t)c0 * lay.chunk));
+        finish<D, kWarps>(p, sm.fin, seg.seq, seg.g, whole ? 1 : c1 - c0 + 1, first, c0);
       }
     }
     if (seg.next >= x1) break;
-    seg = next_seg<TILE, PREFIX>(p, sm.cum, seg);
+    seg = next_seg<TILE, PREFIX>(p, sm.cum, sm.len, seg);
+    load_q(seg);
   }
   cp_wait<0>();
 }
 
 template <int D, bool Q8, int NR, bool PREFIX>
 static cudaError_t launch(const Params &p, int grid, cudaStream_t st, bool pdl) {
-  constexpr int kStages = NR == 16 ? 2 : 3;
-  auto fn = attn_kernel<D, Q8, NR, PREFIX, kStages>;
-  const size_t smem = sizeof(Smem<D, Q8, NR, kStages>);
+  auto fn = attn_kernel<D, Q8, NR, PREFIX>;
+  const size_t smem = sizeof(Smem<D, Q8, NR>);
   static int configured[64] = {0};  // the shared-memory opt-in, per device
   int dev = 0;
   cudaGetDevice(&dev);
@@ -850,33 +878,25 @@ static cudaError_t launch(const Params &p, int grid, cudaStream_t st, bool pdl) 
     if (e != cudaSuccess) return e;
     configured[dev] = 1;
   }
-  return launch_kernel((const void *)fn, dim3(grid), dim3(kThreads), smem, st, pdl, p);
-}
-template <bool Q8, int NR, bool PREFIX>
-static cudaError_t launch_d(const Params &p, int d, int grid, cudaStream_t st, bool pdl) {
-  return d == 128 ? launch<128, Q8, NR, PREFIX>(p, grid, st, pdl)
-                  : (d == 64 ? launch<64, Q8, NR, PREFIX>(p, grid, st, pdl) : launch<32, Q8, NR, PREFIX>(p, grid, st, pdl));
-}
-template <bool PREFIX>
-static cudaError_t launch_any(const Params &p, int d, bool q8, int rows, int grid, cudaStream_t st, bool pdl) {
-  if (rows <= 8) return q8 ? launch_d<true, 8, PREFIX>(p, d, grid, st, pdl) : launch_d<false, 8, PREFIX>(p, d, grid, st, pdl);
-  return q8 ? launch_d<true, 16, PREFIX>(p, d, grid, st, pdl) : launch_d<false, 16, PREFIX>(p, d, grid, st, pdl);
+  return launch_kernel((const void *)fn, dim3(grid), dim3(Cfg<Q8, NR>::kThreads), smem, st, pdl, p);
 }
 
 static int row_tiles(int64_t m, int group) { return (int)((m * group + kRows - 1) / kRows); }
-static int tile_keys(bool q8) { return q8 ? 32 : 16; }
-static int max_grid() { return kCtasPerSm * num_sms(); }
-// CTAs that the sequences' own keys can need: no more ranges than segments and kMinChunk tiles allow.
-static int own_grid(const Params &p, bool q8) {
-  const int64_t most = ((p.cache.cap + tile_keys(q8) - 1) / tile_keys(q8) + kMinChunk - 1) / kMinChunk;
+static int max_grid() { return num_sms(); }
+// CTAs that the sequences' own keys can need: no more than their ranges if each has the fewest keys a range may have.
+template <typename C>
+static int own_grid(const Params &p) {
+  const int64_t most = ((p.cache.cap + C::kTile - 1) / C::kTile + C::kMinChunk - 1) / C::kMinChunk;
   return (int)std::min<int64_t>(max_grid(), most * p.m * p.nkv);
 }
-// How the prefix's segments are cut: as make_layout does it, on the host.
-static void cut_prefix(Params &p, int64_t prefix_len, bool q8, int grid) {
+// How the prefix's segments are cut: as make_layout does it, on the host; returns the grid.
+template <typename C>
+static int cut_prefix(Params &p) {
   Prefix &c = p.pre;
+  const int grid = max_grid();
   c.row_tiles = row_tiles(p.m, p.group);
-  c.seg_tiles = (int)((prefix_len + tile_keys(q8) - 1) / tile_keys(q8));
-  const int segs = p.nkv * c.row_tiles, share = ceil_div(segs * c.seg_tiles, grid), least = std::max(kMinChunk, share);
+  c.seg_tiles = ceil_div(p.keys, C::kTile);
+  const int segs = p.nkv * c.row_tiles, share = ceil_div(segs * c.seg_tiles, grid), least = std::max(C::kMinChunk, share);
   c.pad = 1, c.chunk = share;
   for (int j = 0; j < 32; ++j) {
     const int len = least + ceil_div(least * j, 64);
@@ -885,6 +905,19 @@ static void cut_prefix(Params &p, int64_t prefix_len, bool q8, int grid) {
       break;
     }
   }
+  return ceil_div(segs * ceil_div(c.seg_tiles, c.pad) * c.pad, c.chunk);
+}
+template <bool Q8, int NR, bool PREFIX>
+static cudaError_t launch_d(Params &p, int d, cudaStream_t st, bool pdl) {
+  const int grid = PREFIX ? cut_prefix<Cfg<Q8, NR>>(p) : own_grid<Cfg<Q8, NR>>(p);
+  p.head_share = grid / p.nkv;
+  return d == 128 ? launch<128, Q8, NR, PREFIX>(p, grid, st, pdl)
+                  : (d == 64 ? launch<64, Q8, NR, PREFIX>(p, grid, st, pdl) : launch<32, Q8, NR, PREFIX>(p, grid, st, pdl));
+}
+template <bool PREFIX>
+static cudaError_t launch_any(Params &p, int d, bool q8, int rows, cudaStream_t st, bool pdl) {
+  if (rows <= 8) return q8 ? launch_d<true, 8, PREFIX>(p, d, st, pdl) : launch_d<false, 8, PREFIX>(p, d, st, pdl);
+  return q8 ? launch_d<true, 16, PREFIX>(p, d, st, pdl) : launch_d<false, 16, PREFIX>(p, d, st, pdl);
 }
 // Whether the prefix goes to attn_prefix_kernel: bf16, head_dim 128, more rows than one tile of the mma.sync kernel.
 static bool prefix_on_tcgen05(const Params &p, int d, bool q8) {
@@ -897,7 +930,7 @@ static int check(const char *what, int64_t ldo, int64_t ldq, const void *out, co
   if (d != 32 && d != 64 && d != 128) return set_error(EGPT_ERR_SHAPE, "%s: head_dim must be 32, 64 or 128", what);
   if (nq < 1 || nkv < 1 || nq % nkv || nq / nkv > kRows)
     return set_error(EGPT_ERR_SHAPE, "%s: nq must be a multiple of nkv, at most %d to one", what, kRows);
-  if (m < 1 || m > kMaxBatch || cap < 1 || cap > 0x3fffffff || ldq < (int64_t)nq * d || ldo < (int64_t)nq * d)
+  if (m < 1 || m > kMaxBatch || cap < 1 || cap > (1 << 27) || ldq < (int64_t)nq * d || ldo < (int64_t)nq * d)
     return set_error(EGPT_ERR_SHAPE, "%s: bad m (1 to %d), cap or leading dimension", what, kMaxBatch);
   if (m * nkv * ((cap + 15) / 16) > 0x3fffffff) return set_error(EGPT_ERR_SHAPE, "%s: cache too long for the batch", what);
   if (!(fabsf(scale) <= 3e38f)) return set_error(EGPT_ERR_ARG, "%s: scale must be finite", what);
@@ -939,8 +972,7 @@ extern "C" int egpt_attn_decode_q8(void *out, int64_t ldo, const void *q, int64_
   p.cache = {(const uint8_t *)k_cache, (const uint8_t *)v_cache, k_scale, v_scale, cap};
   p.position = position, p.m = (int)m, p.nkv = nkv, p.group = nq / nkv, p.scale_log2 = scale * 1.4426950408889634f;
   p.cnt = (unsigned *)ws, p.ws = (float *)((char *)ws + aq8::counter_bytes(m, nkv));
-  return check_launch(aq8::launch_any<false>(p, d, true, p.group, aq8::own_grid(p, true), (cudaStream_t)stream,
-                                             (flags & EGPT_FLAG_PDL) != 0),
+  return check_launch(aq8::launch_any<false>(p, d, true, p.group, (cudaStream_t)stream, (flags & EGPT_FLAG_PDL) != 0),
                       "attn_decode_q8_kernel");
 }
 
@@ -958,7 +990,7 @@ extern "C" int egpt_attn_shared_prefix(void *out, int64_t ldo, const void *q, in
   if (q8 && (!pk_scale || !pv_scale || !tk_scale || !tv_scale))
     return set_error(EGPT_ERR_ARG, "attn_shared_prefix: int8 caches need their scales");
   if (int rc = aq8::check("attn_shared_prefix", ldo, ldq, out, q, cap, m, nq, nkv, d, scale, ws, ws_bytes)) return rc;
-  if (prefix_cap < 1 || prefix_len < 0 || prefix_len > prefix_cap || prefix_len > 0x3fffffff ||
+  if (prefix_cap < 1 || prefix_len < 0 || prefix_len > prefix_cap || prefix_len > (1 << 27) ||
       (int64_t)nkv * aq8::row_tiles(m, nq / nkv) * ((prefix_len + 15) / 16) > 0x1fffffff)
     return set_error(EGPT_ERR_SHAPE, "attn_shared_prefix: bad prefix_len (0 to prefix_cap), or too long for the batch");
   if ((uintptr_t)pk % 16 || (uintptr_t)pv % 16 || (uintptr_t)tk % 16 || (uintptr_t)tv % 16)
@@ -984,10 +1016,7 @@ extern "C" int egpt_attn_shared_prefix(void *out, int64_t ldo, const void *q, in
       aq8::Params a = p;
       a.cache = {(const uint8_t *)pk, (const uint8_t *)pv, pk_scale, pv_scale, prefix_cap};
       a.keys = (int)prefix_len, a.ws = pre_rec;
-      aq8::cut_prefix(a, prefix_len, q8, aq8::max_grid());
-      const int64_t places = (int64_t)nkv * a.pre.row_tiles * aq8::ceil_div(a.pre.seg_tiles, a.pre.pad) * a.pre.pad;
-      const cudaError_t e = aq8::launch_any<true>(a, d, q8, (int)m * p.group, (int)((places + a.pre.chunk - 1) / a.pre.chunk),
-                                                  st, pdl);
+      const cudaError_t e = aq8::launch_any<true>(a, d, q8, (int)m * p.group, st, pdl);
       if (e != cudaSuccess) return check_launch(e, "attn_shared_prefix_kernel (prefix)");
       p.pre = a.pre;
     }
@@ -995,5 +1024,5 @@ extern "C" int egpt_attn_shared_prefix(void *out, int64_t ldo, const void *q, in
     pdl = true;
   }
   p.cache = {(const uint8_t *)tk, (const uint8_t *)tv, tk_scale, tv_scale, cap};
-  return check_launch(aq8::launch_any<false>(p, d, q8, p.group, aq8::own_grid(p, q8), st, pdl), "attn_shared_prefix_kernel");
+  return check_launch(aq8::launch_any<false>(p, d, q8, p.group, st, pdl), "attn_shared_prefix_kernel");
 }
