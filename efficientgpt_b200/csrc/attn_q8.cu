@@ -189,8 +189,8 @@ __device__ __forceinline__ int ceil_div_small(int a, int b) {
   return q + (r >= b) - (r < 0);
 }
 
-// cum[i] = places of the sequences before i (one kv head). The ranges: with up to 32 sequences the lanes try range lengths
-// from the even share of the tiles up to 1.5 times it, and the smallest that gives at most one range per CTA is taken;
+// cum[i] = places of the sequences before i (one kv head). The ranges: with up to 32 sequences the lanes try eight range
+// lengths from the even share of the tiles to 1.5 times it, and the smallest that gives at most one range per CTA is taken;
 // failing that, and for more sequences, equal stretches. Every thread of the CTA calls it.
 template <typename C>
 __device__ __forceinline__ Layout make_layout(const Params &p, int *cum, int *len_of, int *scratch) {
@@ -203,10 +203,15 @@ __device__ __forceinline__ Layout make_layout(const Params &p, int *cum, int *le
     if (p.m == 1 && p.head_share) {  // all CTAs of a head for its one segment
       l.pad = max(C::kMinChunk, ceil_div_small(__shfl_sync(0xffffffffu, tiles, 0), p.head_share));
     } else {
+      // lane: length number lane % 8, every fourth sequence from lane / 8 on
       const int share = ceil_div(p.nkv * __reduce_add_sync(0xffffffffu, tiles), grid);
-      const int least = max(C::kMinChunk, share), len = least + (least * lane + 63) / 64;
+      const int least = max(C::kMinChunk, share), len = least + (least * (lane & 7) + 13) / 14;
       int parts = 0;
-      for (int i = 0; i < p.m; ++i) parts += ceil_div_small(__shfl_sync(0xffffffffu, tiles, i), len);
+#pragma unroll 4
+      for (int i = lane >> 3; i < ((p.m + 3) & ~3); i += 4)
+        parts += ceil_div_small(__shfl_sync(0xffffffffu, tiles, i), len);
+      parts += __shfl_xor_sync(0xffffffffu, parts, 8);
+      parts += __shfl_xor_sync(0xffffffffu, parts, 16);
       const unsigned good = __ballot_sync(0xffffffffu, p.nkv * parts <= grid);
       fits = good != 0u;
       if (fits) l.pad = __shfl_sync(0xffffffffu, len, __ffs(good) - 1);
@@ -315,10 +320,10 @@ __device__ __forceinline__ float *record(const Params &p, int index) {
   return p.ws + (int64_t)index * kRows * (D + 2);
 }
 
-// A row's records, added up by the warps that share it.
-template <int D, int WARPS>
-struct Finish {
-  float a[WARPS][D];
+// Segments whose records a CTA has to add up: records slot .. slot + n - 1.
+constexpr int kTodo = 16;
+struct Todo {
+  int seq, g, slot, n;
 };
 
 template <int D, bool Q8, int NR>
@@ -327,28 +332,31 @@ struct Smem {
   uint8_t ring[kWarps][Cfg<Q8, NR>::kStages][Geo<D, Q8, NR>::kStageBytes];
   union {
     float merge[kWarps][kPass][D];  // the warps' accumulators, kPass rows at a time
-    Finish<D, kWarps> fin;
+    float fin[kWarps][D];           // shares of a row's records
   };
   float warp_m[kWarps][NR], warp_l[kWarps][NR];  // their maxima and sums
   float row_m[NR], row_l[NR];                    // and the CTA's
   int cum[kMaxBatch + 1], len[kMaxBatch];
   int scratch[kWarps];
-  int last;
+  Todo todo[kTodo];
+  int last[2];
 };
 
-// out[i, heads of g] = the own_n records of the sequence's own keys (the first in slot `first`, then slots
-// 2 (c0 + k)) and the prefix's, added up: a warp takes a row, or with fewer rows than warps every parts-th record of
-// one. Lanes read the maxima and sums of 32 records at once while the first accumulators are on their way, so a short
-// list costs one round trip. The order is fixed by the shapes. Every thread of the CTA calls it.
+// out[seq, heads of g] of the list's segments: their records and the prefix's, added up. A warp takes a row, or with fewer
+// rows than warps every parts-th record of one. Lanes read the maxima and sums of 32 records at once while the first
+// accumulators are on their way, so a short list costs one round trip. The order is fixed by the shapes. Every thread
+// of the CTA calls it, the list and the CTA's own records being visible to it.
 template <int D, int WARPS>
-__device__ __noinline__ void finish(const Params &p, Finish<D, WARPS> &f, int i, int g, int own_n, int first, int c0) {
+__device__ __noinline__ void finish(const Params &p, float (*f)[D], const Todo *todo, int todos) {
   constexpr int N = D / 32;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int parts = p.group < WARPS ? WARPS / p.group : 1;
-  const int part = parts > 1 ? warp / p.group : 0;
+  const int units = todos * p.group, parts = units < WARPS ? WARPS / units : 1;
   if (p.pre.rec) pdl_wait();  // the launch over the prefix has finished
 #pragma unroll 1
-  for (int j = warp - part * p.group; j < p.group && part < parts; j += WARPS) {
+  for (int u = warp; u < units * parts; u += WARPS) {
+    const int part = parts > 1 ? u / units : 0, unit = u - part * units;
+    const int entry = unit / p.group, j = unit - entry * p.group;
+    const int i = todo[entry].seq, g = todo[entry].g, own_n = todo[entry].n, slot = todo[entry].slot;
     const float *pre0 = nullptr;  // row j's accumulators in the prefix's first record
     int pre_n = 0, pre_rows = kRows, pre_row = 0;
     int64_t pre_step = 0;
@@ -372,7 +380,7 @@ __device__ __noinline__ void finish(const Params &p, Finish<D, WARPS> &f, int i,
       }
     }
     auto row_of = [&](int k) -> const float * {  // row j's accumulators in record k
-      return k < own_n ? p.ws + (int64_t)(k == 0 ? first : 2 * (c0 + k)) * (kRows * (D + 2)) + j * D
+      return k < own_n ? p.ws + (int64_t)(slot + k) * (kRows * (D + 2)) + j * D
                        : pre0 + (int64_t)(k - own_n) * pre_step;
     };
     const int n = own_n + pre_n;
@@ -431,34 +439,37 @@ __device__ __noinline__ void finish(const Params &p, Finish<D, WARPS> &f, int i,
     const float inv = lsum == 0.f ? 0.f : 1.f / lsum;  // no keys at all: zeros
     if (parts > 1) {
 #pragma unroll
-      for (int e = 0; e < N; ++e) f.a[part * p.group + j][N * lane + e] = a[e] * inv;
+      for (int e = 0; e < N; ++e) f[u][N * lane + e] = a[e] * inv;
     } else {
 #pragma unroll
       for (int e = 0; e < N; ++e)
         p.out[i * p.ldo + (int64_t)(g * p.group + j) * D + N * lane + e] = f32_to_bf16_bits(a[e] * inv);
     }
   }
-  if (parts == 1) return;
-  __syncthreads();
+  if (parts > 1) {
+    __syncthreads();
 #pragma unroll 1
-  for (int e = threadIdx.x; e < p.group * D; e += 32 * WARPS) {
-    float a = 0.f;
-    for (int q = 0; q < parts; ++q) a += f.a[q * p.group + e / D][e % D];
-    p.out[i * p.ldo + (int64_t)g * p.group * D + e] = f32_to_bf16_bits(a);
+    for (int e = threadIdx.x; e < units * D; e += 32 * WARPS) {
+      const int unit = e / D, entry = unit / p.group, j = unit - entry * p.group;
+      float a = 0.f;
+      for (int q = 0; q < parts; ++q) a += f[q * units + unit][e % D];
+      p.out[todo[entry].seq * p.ldo + (int64_t)(todo[entry].g * p.group + j) * D + e % D] = f32_to_bf16_bits(a);
+    }
   }
-  __syncthreads();  // f is free again
+  __syncthreads();  // f and the list are free again
 }
 
-// NR: query rows in use, 8 or 16. PREFIX: the segments of the shared prefix, every (CTA, segment) pair leaving a record in
-// slot CTA + segment; else the sequences' own keys, a CTA's at most two split segments leaving theirs in slots 2 CTA
-// and 2 CTA + 1, and the last CTA of a segment adding all of it up.
+// NR: query rows in use, 8 or 16. PREFIX: the segments of the shared prefix, else the sequences' own keys. A (CTA, segment)
+// pair leaves its record in slot CTA + segment: both only grow along the list, so slots are the pairs' own. Without
+// a prefix a segment that one CTA holds goes straight to the output; the rest is added up at the CTA's end, a split
+// segment's by the last of its CTAs to get there.
 template <int D, bool Q8, int NR, bool PREFIX>
 __global__ void __launch_bounds__(Cfg<Q8, NR>::kThreads, 1) attn_kernel(const Params p) {
   using C = Cfg<Q8, NR>;
   using G = Geo<D, Q8, NR>;
   using S = Smem<D, Q8, NR>;
   constexpr int kWarps = C::kWarps, STAGES = C::kStages;
-  constexpr int TILE = G::kTile, NT = TILE / 8, ND = D / 8, NC = NR == 16 ? 4 : 2;  // NC: accumulators kept
+  constexpr int TILE = G::kTile, NT = TILE / 8, ND = D / 8;
   constexpr bool PLANES = Q8 && NR == 8;  // scores by int8 MMAs on the digits of q
   extern __shared__ __align__(16) uint8_t smem_raw[];
   S &sm = *(S *)smem_raw;
@@ -472,15 +483,24 @@ __global__ void __launch_bounds__(Cfg<Q8, NR>::kThreads, 1) attn_kernel(const Pa
     lay.total = p.nkv * p.pre.row_tiles * ceil_div(p.pre.seg_tiles, lay.pad) * lay.pad;
   } else {
     lay = make_layout<C>(p, sm.cum, sm.len, sm.scratch);
-    for (int e = blockIdx.x; e < p.m * p.nkv; e += gridDim.x)  // sequences without keys of their own
-      if (sm.cum[e / p.nkv + 1] == sm.cum[e / p.nkv]) finish<D, kWarps>(p, sm.fin, e / p.nkv, e % p.nkv, 0, 0, 0);
   }
   int x0 = (int)min((int64_t)lay.total, (int64_t)blockIdx.x * lay.chunk), x1 = min(lay.total, x0 + lay.chunk);
-  if (lay.pad == 1) {
-    x0 = cut_at<TILE, PREFIX>(p, lay, sm.cum, sm.len, x0);
-    x1 = cut_at<TILE, PREFIX>(p, lay, sm.cum, sm.len, (int64_t)(blockIdx.x + 1) * lay.chunk);
+  if (lay.pad == 1) {  // both cuts at once, in the even and in the odd lanes
+    const int cut = cut_at<TILE, PREFIX>(p, lay, sm.cum, sm.len, (int64_t)(blockIdx.x + (lane & 1)) * lay.chunk);
+    x0 = __shfl_sync(0xffffffffu, cut, 0), x1 = __shfl_sync(0xffffffffu, cut, 1);
   }
-  if (x0 >= x1) return;
+  int todos = 0;                // entries of sm.todo
+  int split_n = 0;  // segments that this CTA shares with others: its first, its last
+  Todo split[2] = {};
+  auto add_todo = [&](const Todo &e) {  // all threads; the entry is visible after the next barrier
+    if (threadIdx.x == 0) sm.todo[todos] = e;
+    if (++todos == kTodo) {
+      __syncthreads();
+      finish<D, kWarps>(p, sm.fin, sm.todo, todos);
+      todos = 0;
+    }
+  };
+  if (x0 < x1) {
   Seg seg = find_seg<TILE, PREFIX>(p, sm.cum, sm.len, x0);
   if (lay.pad > 1) x1 = min(x1, seg.end);
 
@@ -559,7 +579,6 @@ __global__ void __launch_bounds__(Cfg<Q8, NR>::kThreads, 1) attn_kernel(const Pa
   for (int s = 0; s < STAGES - 1; ++s) load_next();
 
   int cslot = 0;
-  const int first_seg = seg.index;
   for (;;) {
     // ---- the segment's query rows as MMA fragments
     uint32_t qa[PLANES ? D / 32 : D / 16][PLANES ? 8 : 4];
@@ -799,7 +818,7 @@ __global__ void __launch_bounds__(Cfg<Q8, NR>::kThreads, 1) attn_kernel(const Pa
     const bool whole = seg.start >= x0 && seg.end <= x1;
     const bool final = !PREFIX && whole && !p.pre.rec;
     const int rows = PREFIX ? kRows : p.group;
-    float *rec = record<D>(p, PREFIX ? (int)blockIdx.x + seg.index : 2 * (int)blockIdx.x + (seg.index != first_seg));
+    float *rec = record<D>(p, (int)blockIdx.x + seg.index);
     constexpr int kPass = S::kPass;
 #pragma unroll 1
     for (int r0 = 0; r0 < rows; r0 += kPass) {
@@ -832,31 +851,13 @@ __global__ void __launch_bounds__(Cfg<Q8, NR>::kThreads, 1) attn_kernel(const Pa
       rec[kRows * D + threadIdx.x] = sm.row_m[threadIdx.x];
       rec[kRows * D + kRows + threadIdx.x] = sm.row_l[threadIdx.x];
     }
-    if (!PREFIX && (!whole || p.pre.rec)) {
+    if (!PREFIX && !final) {
       const int c0 = seg.start / lay.chunk, c1 = (seg.end - 1) / lay.chunk;
-      bool last = true;
-      if (!whole) {  // the last CTA of a split segment adds the parts up
-        __threadfence();
-        __syncthreads();
-        if (threadIdx.x == 0) {
-          unsigned *cnt = p.cnt + seg.index;
-          sm.last = atomicAdd(cnt, 1u) == (unsigned)(c1 - c0);
-          if (sm.last) {
-            *cnt = 0u;
-            __threadfence();
-          }
-        }
-        __syncthreads();
-        last = sm.last;
+      if (whole) {
+        add_todo({seg.seq, seg.g, (int)blockIdx.x + seg.index, 1});
       } else {
-        __syncthreads();  // the record is written
-      }
-      if (last) {
-        // (a whole segment's one record is in this CTA's slot, a split one's first part in the last slot of its CTA
-        // if that began with another segment)
-        const int first = whole ? 2 * (int)blockIdx.x + (seg.index != first_seg)
-                                : 2 * c0 + (lay.pad == 1 && seg.start != cut_at<TILE, PREFIX>(p, lay, sm.cum, sm.len, (int64_t)c0 * lay.chunk));
-        finish<D, kWarps>(p, sm.fin, seg.seq, seg.g, whole ? 1 : c1 - c0 + 1, first, c0);
+        (split_n ? split[1] : split[0]) = {seg.seq, seg.g, c0 + seg.index, c1 - c0 + 1};
+        ++split_n;
       }
     }
     if (seg.next >= x1) break;
@@ -864,6 +865,31 @@ __global__ void __launch_bounds__(Cfg<Q8, NR>::kThreads, 1) attn_kernel(const Pa
     load_q(seg);
   }
   cp_wait<0>();
+  }
+  if (PREFIX) return;
+  if (split_n) {  // the last CTA of a split segment adds the parts up
+    __threadfence();
+    __syncthreads();
+    if ((int)threadIdx.x < split_n) {
+      const Todo e = threadIdx.x ? split[1] : split[0];
+      unsigned *cnt = p.cnt + e.seq * p.nkv + e.g;
+      const bool last = atomicAdd(cnt, 1u) == (unsigned)(e.n - 1);
+      if (last) {
+        *cnt = 0u;
+        __threadfence();
+      }
+      sm.last[threadIdx.x] = last;
+    }
+    __syncthreads();
+    for (int e = 0; e < split_n; ++e)
+      if (sm.last[e]) add_todo(split[e]);
+  }
+  for (int e = blockIdx.x; e < p.m * p.nkv; e += gridDim.x)  // sequences without keys of their own
+    if (sm.len[e / p.nkv] == 0) add_todo({e / p.nkv, e % p.nkv, 0, 0});
+  if (todos) {
+    __syncthreads();
+    finish<D, kWarps>(p, sm.fin, sm.todo, todos);
+  }
 }
 
 template <int D, bool Q8, int NR, bool PREFIX>
@@ -949,12 +975,12 @@ using namespace egpt;
 
 extern "C" size_t egpt_attn_q8_ws_bytes(int64_t m, int nq, int nkv, int d) {
   if (m < 1 || nkv < 1 || nq < nkv || d < 1) return 0;
-  // arrival counters; two records for every CTA of the launch over the sequences' own keys; the prefix's records: one for
-  // every (CTA, segment) pair of attn_kernel (CTA c and segment s keep theirs at c + s), or attn_prefix_kernel's
+  // arrival counters; a record for every (CTA, segment) pair of the launch over the sequences' own keys; the prefix's
+  // records: attn_kernel's, one for every pair again, or attn_prefix_kernel's
   const size_t rec = aq8::kRows * ((size_t)d + 2) * 4;
   const size_t small = ((size_t)aq8::max_grid() + (size_t)nkv * aq8::row_tiles(m, nq / nkv)) * rec;
   const size_t big = d == apx::kD && nq / nkv <= aq8::kRows ? apx::record_floats(m, nq / nkv, nkv) * 4 : 0;
-  return aq8::counter_bytes(m, nkv) + 2 * (size_t)aq8::max_grid() * rec + std::max(small, big);
+  return aq8::counter_bytes(m, nkv) + ((size_t)aq8::max_grid() + (size_t)m * nkv) * rec + std::max(small, big);
 }
 
 extern "C" int egpt_attn_decode_q8(void *out, int64_t ldo, const void *q, int64_t ldq, const int8_t *k_cache,
@@ -1001,7 +1027,7 @@ extern "C" int egpt_attn_shared_prefix(void *out, int64_t ldo, const void *q, in
   p.out = (uint16_t *)out, p.ldo = ldo, p.q = (const uint16_t *)q, p.ldq = ldq;
   p.position = position, p.m = (int)m, p.nkv = nkv, p.group = nq / nkv, p.scale_log2 = scale * 1.4426950408889634f;
   p.cnt = (unsigned *)ws, p.ws = (float *)((char *)ws + aq8::counter_bytes(m, nkv));
-  float *pre_rec = p.ws + 2 * (size_t)aq8::max_grid() * aq8::kRows * (d + 2);
+  float *pre_rec = p.ws + ((size_t)aq8::max_grid() + (size_t)m * nkv) * aq8::kRows * (d + 2);
   if (prefix_len > 0) {
     if (aq8::prefix_on_tcgen05(p, d, q8)) {
       apx::Args A{};

@@ -47,53 +47,64 @@ __device__ __forceinline__ int code_of(float x, float s) {
   return (int)fminf(fmaxf(rintf(__fdiv_rn(x, s)), -127.f), 127.f);
 }
 
-// Rows as they are: D / 8 lanes hold one row, 16 bytes (bf16) or 32 bytes (fp32) each, so a row is read once and its
-// maximum needs a few shuffles; K and V of all rows and heads are one flat list.
+// Rows as they are: D / 8 lanes hold a row, 16 bytes (bf16) or 32 bytes (fp32) each, so it is read once and its maximum
+// needs a few shuffles; a thread takes the same piece of kRowsPerThread rows of the flat list of (row, head) and of both K
+// and V, whose loads are all on their way before the first is used.
+constexpr int kRowsPerThread = 2;
 template <int D, bool F32>
 __global__ void __launch_bounds__(kThreads) append_kernel(AppendParams p) {
-  constexpr int kLanes = D / 8;
+  constexpr int kLanes = D / 8, kRows = kThreads / kLanes;
   pdl_wait();
   pdl_launch_dependents();
-  const int64_t item = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / kLanes;
-  const int64_t per_row = 2 * (int64_t)p.nkv;
-  const bool live = item < p.m * per_row;
-  const int64_t row = live ? item / per_row : 0;
-  const int rest = live ? (int)(item - row * per_row) : 0;
-  const bool is_v = rest >= p.nkv;
-  const int head = is_v ? rest - p.nkv : rest;
   const int e0 = (int)(threadIdx.x % kLanes) * 8;
-  float x[8];
+  const unsigned items = (unsigned)(p.m * p.nkv);
+  float x[kRowsPerThread][2][8];
+  unsigned row[kRowsPerThread], head[kRowsPerThread];
+  bool live[kRowsPerThread];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = 0.f;
-  if (live) {
-    const int64_t at = row * (is_v ? p.ldv : p.ldk) + (int64_t)head * D + e0;
-    if (F32) {
-      const float4 *src = (const float4 *)((const float *)(is_v ? p.v : p.k) + at);
-      const float4 a = src[0], b = src[1];
-      x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-    } else {
-      const uint4 a = *(const uint4 *)((const uint16_t *)(is_v ? p.v : p.k) + at);
-      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+  for (int i = 0; i < kRowsPerThread; ++i) {
+    const unsigned item = (blockIdx.x * kRowsPerThread + i) * kRows + threadIdx.x / kLanes;
+    live[i] = item < items;
+    row[i] = live[i] ? item / (unsigned)p.nkv : 0;
+    head[i] = live[i] ? item - row[i] * (unsigned)p.nkv : 0;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[2 * e] = bf16_lo(w[e]), x[2 * e + 1] = bf16_hi(w[e]);
+    for (int kv = 0; kv < 2; ++kv) {
+      const int64_t at = (int64_t)row[i] * (kv ? p.ldv : p.ldk) + (int64_t)head[i] * D + e0;  // (row 0 if not live)
+      if (F32) {
+        const float4 *src = (const float4 *)((const float *)(kv ? p.v : p.k) + at);
+        const float4 a = src[0], b = src[1];
+        const float y[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[i][kv][e] = y[e];
+      } else {
+        const uint4 a = *(const uint4 *)((const uint16_t *)(kv ? p.v : p.k) + at);
+        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[i][kv][2 * e] = bf16_lo(w[e]), x[i][kv][2 * e + 1] = bf16_hi(w[e]);
+      }
     }
   }
-  float amax = 0.f;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(x[e]));
+  for (int i = 0; i < kRowsPerThread; ++i) {
+    int64_t head0 = 0;
+    const int64_t slot = live[i] ? slot_of(p, row[i], head0) : -1;
+    const int64_t dst = (head0 + head[i]) * p.cap + slot;
 #pragma unroll
-  for (int o = kLanes / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-  if (!live) return;
-  int64_t head0;
-  const int64_t slot = slot_of(p, row, head0);
-  if (slot < 0) return;
-  const float s = row_scale(amax);
-  uint32_t w[2] = {0u, 0u};
+    for (int kv = 0; kv < 2; ++kv) {
+      float amax = 0.f;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) w[e / 4] |= (uint32_t)(code_of(x[e], s) & 0xff) << (8 * (e % 4));
-  const int64_t dst = (head0 + head) * p.cap + slot;
-  *(uint2 *)((is_v ? p.v_cache : p.k_cache) + dst * D + e0) = make_uint2(w[0], w[1]);
-  if (e0 == 0) (is_v ? p.v_scale : p.k_scale)[dst] = s;
+      for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(x[i][kv][e]));
+#pragma unroll
+      for (int o = kLanes / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+      if (slot < 0) continue;
+      const float s = row_scale(amax);
+      uint32_t w[2] = {0u, 0u};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[e / 4] |= (uint32_t)(code_of(x[i][kv][e], s) & 0xff) << (8 * (e % 4));
+      *(uint2 *)((kv ? p.v_cache : p.k_cache) + dst * D + e0) = make_uint2(w[0], w[1]);
+      if (e0 == 0) (kv ? p.v_scale : p.k_scale)[dst] = s;
+    }
+  }
 }
 
 // With the decode step's prologue: one warp per head vector of q, k or v (lane l: elements l + 32 i). The norm's sum
@@ -177,43 +188,54 @@ struct ReadParams {
   int group;
 };
 
-// out[h][r] = q s of row start + r of head h: 16 codes (one 16-byte load) per thread, D / 16 threads to a row.
+// out[h][r] = q s of row start + r of head h (blockIdx.y; K, then V, in blockIdx.z): 16 codes (one 16-byte load) per
+// thread and row, D / 16 threads to a row, kReadRows rows' loads on their way at once.
+constexpr int kReadRows = 4;
 template <int D, bool F32>
 __global__ void __launch_bounds__(kThreads) read_kernel(ReadParams p) {
-  constexpr int kLanes = D / 16;
+  constexpr int kLanes = D / 16, kStep = kThreads / kLanes;
   pdl_wait();
   pdl_launch_dependents();
-  const int64_t rows = p.heads * p.count;
-  for (int64_t i = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / kLanes; i < 2 * rows;
-       i += (int64_t)gridDim.x * kThreads / kLanes) {
-    const bool is_v = i >= rows;
-    const int64_t j = is_v ? i - rows : i;
-    const int64_t h = j / p.count, r = j - h * p.count;
-    const int64_t slot = p.start + r + (p.starts ? p.starts[h / p.group] : 0);
-    const int e0 = (int)(threadIdx.x % kLanes) * 16;
-    uint4 c = make_uint4(0u, 0u, 0u, 0u);
-    float s = 0.f;
-    if (slot >= 0 && slot < p.cap) {  // slots outside the cache read as zeros
-      c = *(const uint4 *)((is_v ? p.v_cache : p.k_cache) + (h * p.cap + slot) * D + e0);
-      s = (is_v ? p.v_scale : p.k_scale)[h * p.cap + slot];
-    }
-    const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-    float x[16];
+  const int e0 = (int)(threadIdx.x % kLanes) * 16;
+  const bool is_v = blockIdx.z != 0;
+  for (int64_t h = blockIdx.y; h < p.heads; h += gridDim.y) {
+    const int64_t start = p.start + (p.starts ? p.starts[h / p.group] : 0);
+    const int8_t *codes = (is_v ? p.v_cache : p.k_cache) + h * p.cap * D + e0;
+    const float *scales = (is_v ? p.v_scale : p.k_scale) + h * p.cap;
+    for (int64_t r0 = (int64_t)blockIdx.x * kStep * kReadRows + threadIdx.x / kLanes; r0 < p.count;
+         r0 += (int64_t)gridDim.x * kStep * kReadRows) {
+      uint4 c[kReadRows];
+      float s[kReadRows];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) x[e] = (float)(int8_t)(w[e / 4] >> (8 * (e % 4))) * s;
-    const int64_t at = h * p.out_head + r * D + e0;
-    if (F32) {
-      float4 *dst = (float4 *)((float *)(is_v ? p.v_out : p.k_out) + at);
+      for (int i = 0; i < kReadRows; ++i) {
+        const int64_t r = r0 + i * kStep, slot = start + r;
+        const bool in = r < p.count && slot >= 0 && slot < p.cap;  // slots outside the cache read as zeros
+        c[i] = in ? __ldcs((const uint4 *)(codes + slot * D)) : make_uint4(0u, 0u, 0u, 0u);
+        s[i] = in ? scales[slot] : 0.f;
+      }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) dst[e] = make_float4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
-    } else {
-      uint32_t y[8];
+      for (int i = 0; i < kReadRows; ++i) {
+        const int64_t r = r0 + i * kStep;
+        if (r >= p.count) break;
+        const uint32_t w[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
+        float x[16];
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        y[e] = (uint32_t)f32_to_bf16_bits(x[2 * e]) | ((uint32_t)f32_to_bf16_bits(x[2 * e + 1]) << 16);
-      uint4 *dst = (uint4 *)((uint16_t *)(is_v ? p.v_out : p.k_out) + at);
-      dst[0] = make_uint4(y[0], y[1], y[2], y[3]);
-      dst[1] = make_uint4(y[4], y[5], y[6], y[7]);
+        for (int e = 0; e < 16; ++e) x[e] = (float)(int8_t)(w[e / 4] >> (8 * (e % 4))) * s[i];
+        const int64_t at = h * p.out_head + r * D + e0;
+        if (F32) {
+          float4 *dst = (float4 *)((float *)(is_v ? p.v_out : p.k_out) + at);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) dst[e] = make_float4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
+        } else {
+          uint32_t y[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            y[e] = (uint32_t)f32_to_bf16_bits(x[2 * e]) | ((uint32_t)f32_to_bf16_bits(x[2 * e + 1]) << 16);
+          uint4 *dst = (uint4 *)((uint16_t *)(is_v ? p.v_out : p.k_out) + at);
+          dst[0] = make_uint4(y[0], y[1], y[2], y[3]);
+          dst[1] = make_uint4(y[4], y[5], y[6], y[7]);
+        }
+      }
     }
   }
 }
@@ -273,10 +295,10 @@ extern "C" int egpt_kv_append_q8(int8_t *k_cache, float *k_scale, int8_t *v_cach
   }
   if (q_out || q_norm_w || k_norm_w || rope_cos || rope_sin)
     return set_error(EGPT_ERR_ARG, "kv_append_q8: norm and RoPE need q");
-  const int64_t threads = 2 * m * nkv * (d / 8);
+  const int64_t per_cta = (int64_t)kvq::kRowsPerThread * kvq::kThreads / (d / 8);  // (row, head) pairs
   const void *fn = d == 128 ? kvq::append_fn<128>(f32) : (d == 64 ? kvq::append_fn<64>(f32) : kvq::append_fn<32>(f32));
-  return check_launch(launch_kernel(fn, dim3((unsigned)((threads + kvq::kThreads - 1) / kvq::kThreads)),
-                                    dim3(kvq::kThreads), 0, (cudaStream_t)stream, pdl, p),
+  return check_launch(launch_kernel(fn, dim3((unsigned)((m * nkv + per_cta - 1) / per_cta)), dim3(kvq::kThreads), 0,
+                                    (cudaStream_t)stream, pdl, p),
                       "kv_append_q8_kernel");
 }
 
@@ -302,10 +324,11 @@ extern "C" int egpt_kv_read_q8(void *k_out, void *v_out, int64_t out_head_stride
   p.k_out = k_out, p.v_out = v_out, p.out_head = out_head_stride, p.k_cache = k_cache, p.v_cache = v_cache;
   p.k_scale = k_scale, p.v_scale = v_scale, p.cap = cap, p.start = start, p.count = count, p.heads = heads;
   p.starts = starts, p.group = starts ? heads_per_start : 1;
-  const int64_t threads = 2 * heads * count * (d / 16);
-  const unsigned grid = (unsigned)std::min<int64_t>((threads + kvq::kThreads - 1) / kvq::kThreads, (int64_t)num_sms() * 64);
+  const int64_t per_cta = (int64_t)kvq::kReadRows * kvq::kThreads / (d / 16);
+  const dim3 grid((unsigned)std::min<int64_t>((count + per_cta - 1) / per_cta, 1 << 16),
+                  (unsigned)std::min<int64_t>(heads, 65535), 2);
   const void *fn = d == 128 ? kvq::read_fn<128>(f32) : (d == 64 ? kvq::read_fn<64>(f32) : kvq::read_fn<32>(f32));
-  return check_launch(launch_kernel(fn, dim3(grid), dim3(kvq::kThreads), 0, (cudaStream_t)stream,
+  return check_launch(launch_kernel(fn, grid, dim3(kvq::kThreads), 0, (cudaStream_t)stream,
                                     (flags & EGPT_FLAG_PDL) != 0, p),
                       "kv_read_q8_kernel");
 }

@@ -268,6 +268,12 @@ def silu_mul(gu, inter, out=None):
 
 
 # ---- int8 KV cache: written, read back, attended to ----
+# A decode step calls these once or twice per layer, so the wrappers keep to a few microseconds: one pass over the tensors'
+# attributes, plain integers for the pointers, and the raw handle of the current stream.
+
+def _raw_stream():
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+
 
 def kv_cache_q8(heads, cap, d, device):
     """An empty int8 KV cache: (k codes int8 [heads, cap, d], k scales fp32 [heads, cap], v codes, v scales); code c of a
@@ -276,21 +282,21 @@ def kv_cache_q8(heads, cap, d, device):
                                                torch.zeros(heads, cap, dtype=torch.float32, device=device)))
 
 
-def _cache_q8(what, k_cache, k_scale, v_cache, v_scale):
-    """Checks an int8 cache pair; -> (heads, cap, d)."""
-    shape = k_cache.shape
-    if len(shape) != 3 or v_cache.shape != shape or k_scale.shape != shape[:2] or v_scale.shape != shape[:2]:
-        raise ValueError(f'{what}: codes [heads, cap, d] and scales [heads, cap] expected')
-    if not (k_cache.dtype == v_cache.dtype == torch.int8 and k_scale.dtype == v_scale.dtype == torch.float32):
+def _cache_q8(what, k, ks, v, vs):
+    """Checks an int8 cache pair; -> its shape (heads, cap, d)."""
+    shape = k.shape
+    if not (k.dtype is torch.int8 and v.dtype is torch.int8 and ks.dtype is torch.float32
+            and vs.dtype is torch.float32):
         raise ValueError(f'{what}: int8 codes and fp32 scales expected')
-    if not (k_cache.is_contiguous() and v_cache.is_contiguous() and k_scale.is_contiguous()
-            and v_scale.is_contiguous()):
+    if len(shape) != 3 or v.shape != shape or ks.shape != shape[:2] or vs.shape != shape[:2]:
+        raise ValueError(f'{what}: codes [heads, cap, d] and scales [heads, cap] expected')
+    if not (k.is_contiguous() and ks.is_contiguous() and v.is_contiguous() and vs.is_contiguous()):
         raise ValueError(f'{what}: caches must be contiguous')
     return shape
 
 
 def _positions(what, position, n):
-    if position.dtype != torch.int64 or position.numel() != n or not position.is_contiguous():
+    if position.dtype is not torch.int64 or position.numel() != n or not position.is_contiguous():
         raise ValueError(f'{what}: position must be a contiguous int64 tensor of {n}')
 
 
@@ -300,37 +306,40 @@ def kv_append_q8(k, v, k_cache, k_scale, v_cache, v_scale, position, *, ragged=F
     *position + i of caches [nkv, cap, d], or (ragged) to slot position[i] of its own heads of caches [M * nkv, cap,
     d] (-1: an idle slot, nothing is written). With q [M, nq * d] the q/k RMSNorm and RoPE of a decode step come first
     (the angle of position rope_base + slot) and the rotated q is returned."""
-    _cuda(k, v, k_cache, k_scale, v_cache, v_scale, position, q, q_norm_w, k_norm_w, rope_cos, rope_sin, q_out)
+    _cuda(k, v, k_cache, k_scale, v_cache, v_scale, position)
     heads, cap, d = _cache_q8('kv_append_q8', k_cache, k_scale, v_cache, v_scale)
-    _contig_rows(k, 'k')
-    _contig_rows(v, 'v')
+    if k.dim() != 2 or k.stride(1) != 1 or v.stride(-1) != 1:
+        raise ValueError('kv_append_q8: k and v must be 2-D tensors with unit column stride')
     m, width = k.shape
     nkv = width // d
-    if v.shape != k.shape or v.dtype != k.dtype or nkv * d != width or heads != nkv * (m if ragged else 1):
+    if v.shape != k.shape or v.dtype is not k.dtype or nkv * d != width or heads != (nkv * m if ragged else nkv):
         raise ValueError('kv_append_q8: k and v [M, nkv * d] do not fit the caches')
     _positions('kv_append_q8', position, m if ragged else 1)
-    nq = 0
+    prologue = (None, 0, None, 0, 0, None, None, eps, None, None, 0)
     if q is not None:
+        _cuda(q, q_norm_w, k_norm_w, rope_cos, rope_sin, q_out)
         _contig_rows(q, 'q')
-        if q.dtype != torch.bfloat16 or q.shape[0] != m or q.shape[1] % d:
+        if q.dtype is not torch.bfloat16 or q.shape[0] != m or q.shape[1] % d:
             raise ValueError('kv_append_q8: q must be bf16 [M, nq * d]')
-        nq = q.shape[1] // d
-        if rope_cos is not None and (rope_sin is None or rope_cos.shape != rope_sin.shape or not rope_cos.is_contiguous()
-                                     or not rope_sin.is_contiguous() or rope_cos.dtype != torch.bfloat16
-                                     or rope_sin.dtype != torch.bfloat16 or rope_cos.shape[-1] != d // 2
-                                     or rope_cos.shape[0] < rope_base + cap):
+        for w in (q_norm_w, k_norm_w):
+            if w is not None and (w.dtype is not torch.bfloat16 or w.numel() != d or not w.is_contiguous()):
+                raise ValueError('kv_append_q8: norm weights must be bf16 [d]')
+        if rope_cos is not None and (
+                rope_sin is None or rope_cos.shape != rope_sin.shape or rope_cos.dtype is not torch.bfloat16
+                or rope_sin.dtype is not torch.bfloat16 or not rope_cos.is_contiguous() or not rope_sin.is_contiguous()
+                or rope_cos.shape[-1] != d // 2 or rope_cos.shape[0] < rope_base + cap):
             raise ValueError('kv_append_q8: RoPE tables must be bf16 [>= rope_base + cap, d / 2]')
         if q_out is None:
-            q_out = torch.empty((m, nq * d), dtype=q.dtype, device=q.device)
-        _contig_rows(q_out, 'q_out')
-        if q_out.dtype != torch.bfloat16 or q_out.shape != q.shape:
-            raise ValueError('kv_append_q8: q_out must be bf16 of the shape of q')
-    L.check(L.load().egpt_kv_append_q8(k_cache.data_ptr(), k_scale.data_ptr(), v_cache.data_ptr(), v_scale.data_ptr(),
-                                       cap, k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), position.data_ptr(),
-                                       m, nkv, d, _dt(k), _p(q_out), 0 if q is None else q_out.stride(0), _p(q),
-                                       0 if q is None else q.stride(0), nq, _p(q_norm_w), _p(k_norm_w), eps,
-                                       _p(rope_cos), _p(rope_sin), rope_base, L.FLAG_RAGGED if ragged else 0,
-                                       torch.cuda.current_stream().cuda_stream), 'kv_append_q8')
+            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        elif q_out.dtype is not torch.bfloat16 or q_out.shape != q.shape or q_out.stride(1) != 1:
+            raise ValueError('kv_append_q8: q_out must be bf16 rows of the shape of q')
+        prologue = (q_out.data_ptr(), q_out.stride(0), q.data_ptr(), q.stride(0), q.shape[1] // d, _p(q_norm_w),
+                    _p(k_norm_w), eps, _p(rope_cos), _p(rope_sin), rope_base)
+    rc = L.load().egpt_kv_append_q8(k_cache.data_ptr(), k_scale.data_ptr(), v_cache.data_ptr(), v_scale.data_ptr(), cap,
+                                    k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), position.data_ptr(), m, nkv,
+                                    d, _dt(k), *prologue, L.FLAG_RAGGED if ragged else 0, _raw_stream())
+    if rc:
+        L.check(rc, 'kv_append_q8')
     return q_out
 
 
@@ -340,23 +349,29 @@ def kv_read_q8(k_cache, k_scale, v_cache, v_scale, start, count, *, dtype=torch.
     slots outside the cache read as zeros). out: the (k, v) tensors to fill, rows contiguous, one head stride."""
     _cuda(k_cache, k_scale, v_cache, v_scale)
     heads, cap, d = _cache_q8('kv_read_q8', k_cache, k_scale, v_cache, v_scale)
-    k, v = out if out is not None else torch.empty((2, heads, count, d), dtype=dtype, device=k_cache.device).unbind(0)
-    if out is not None:
+    if out is None:
+        k, v = torch.empty((2, heads, count, d), dtype=dtype, device=k_cache.device).unbind(0)
+        stride = count * d
+    else:
+        k, v = out
         _cuda(k, v)
-        if (k.shape != (heads, count, d) or v.shape != k.shape or k.stride() != v.stride() or k.dtype != v.dtype
+        if (k.shape != (heads, count, d) or v.shape != k.shape or k.stride() != v.stride() or k.dtype is not v.dtype
                 or (count > 1 and k.stride(1) != d) or k.stride(2) != 1):
             raise ValueError('kv_read_q8: out must be two tensors [heads, count, d] with contiguous rows')
+        stride = k.stride(0) if heads > 1 else count * d
     starts, group = None, 0
     if torch.is_tensor(start):
         _cuda(start)
-        _positions('kv_read_q8', start, start.numel())
-        if start.numel() < 1 or heads % start.numel():
+        n = start.numel()
+        _positions('kv_read_q8', start, n)
+        if n < 1 or heads % n:
             raise ValueError('kv_read_q8: one start for each sequence of the cache')
-        starts, group, start = start.data_ptr(), heads // start.numel(), 0
-    L.check(L.load().egpt_kv_read_q8(k.data_ptr(), v.data_ptr(), max(k.stride(0), count * d) if heads == 1 else
-                                     k.stride(0), _dt(k), k_cache.data_ptr(), k_scale.data_ptr(), v_cache.data_ptr(),
-                                     v_scale.data_ptr(), cap, heads, d, start, starts, group, count, 0,
-                                     torch.cuda.current_stream().cuda_stream), 'kv_read_q8')
+        starts, group, start = start.data_ptr(), heads // n, 0
+    rc = L.load().egpt_kv_read_q8(k.data_ptr(), v.data_ptr(), stride, _dt(k), k_cache.data_ptr(), k_scale.data_ptr(),
+                                  v_cache.data_ptr(), v_scale.data_ptr(), cap, heads, d, start, starts, group, count, 0,
+                                  _raw_stream())
+    if rc:
+        L.check(rc, 'kv_read_q8')
     return k, v
 
 
@@ -366,33 +381,34 @@ def attn_q8_ws(m, nq, nkv, d, device):
 
 
 def _attn_rows(what, q, out, nq, d):
-    _contig_rows(q, 'q')
-    if q.dtype != torch.bfloat16 or q.shape[1] != nq * d:
-        raise ValueError(f'{what}: q must be bf16 [M, nq * d]')
+    """Checks q (and out); -> (rows, out)."""
+    shape = q.shape
+    if q.dtype is not torch.bfloat16 or len(shape) != 2 or shape[1] != nq * d or q.stride(1) != 1:
+        raise ValueError(f'{what}: q must be bf16 [M, nq * d] with unit column stride')
     if out is None:
-        return torch.empty((q.shape[0], nq * d), dtype=q.dtype, device=q.device)
-    _contig_rows(out, 'out')
-    if out.dtype != torch.bfloat16 or out.shape != q.shape:
-        raise ValueError(f'{what}: out must be bf16 of the shape of q')
-    return out
+        out = torch.empty_like(q)
+    elif out.dtype is not torch.bfloat16 or out.shape != shape or out.stride(1) != 1:
+        raise ValueError(f'{what}: out must be bf16 rows of the shape of q')
+    return shape[0], out
 
 
 def attn_decode_q8(q, k_cache, k_scale, v_cache, v_scale, position, nq, nkv, d, *, scale, ws=None, out=None):
     """Decode attention over int8 caches [M * nkv, cap, d]: row i of q bf16 [M, nq * d] over the position[i] + 1 keys of
     its own sequence (int64 [M] on the device; -1: an idle slot, zeros) -> bf16 [M, nq * d]."""
     _cuda(q, k_cache, k_scale, v_cache, v_scale, position, ws, out)
-    out = _attn_rows('attn_decode_q8', q, out, nq, d)
-    m = q.shape[0]
+    m, out = _attn_rows('attn_decode_q8', q, out, nq, d)
     heads, cap, dc = _cache_q8('attn_decode_q8', k_cache, k_scale, v_cache, v_scale)
     if dc != d or heads != m * nkv:
         raise ValueError('attn_decode_q8: caches must be [M * nkv, cap, d]')
     _positions('attn_decode_q8', position, m)
     if ws is None:
         ws = attn_q8_ws(m, nq, nkv, d, q.device)
-    L.check(L.load().egpt_attn_decode_q8(out.data_ptr(), out.stride(0), q.data_ptr(), q.stride(0), k_cache.data_ptr(),
-                                         k_scale.data_ptr(), v_cache.data_ptr(), v_scale.data_ptr(), cap,
-                                         position.data_ptr(), m, nq, nkv, d, scale, ws.data_ptr(), ws.numel(), 0,
-                                         torch.cuda.current_stream().cuda_stream), 'attn_decode_q8')
+    rc = L.load().egpt_attn_decode_q8(out.data_ptr(), out.stride(0), q.data_ptr(), q.stride(0), k_cache.data_ptr(),
+                                      k_scale.data_ptr(), v_cache.data_ptr(), v_scale.data_ptr(), cap,
+                                      position.data_ptr(), m, nq, nkv, d, scale, ws.data_ptr(), ws.numel(), 0,
+                                      _raw_stream())
+    if rc:
+        L.check(rc, 'attn_decode_q8')
     return out
 
 
@@ -401,10 +417,10 @@ def _cache_pair(what, cache, d):
     _cuda(*cache)
     if len(cache) == 4:
         heads, cap, dc = _cache_q8(what, *cache)
-        dt, ptrs = L.EGPT_I8, tuple(t.data_ptr() for t in cache)
+        dt, ptrs = L.EGPT_I8, [t.data_ptr() for t in cache]
     elif len(cache) == 2:
         k, v = cache
-        if k.dim() != 3 or k.shape != v.shape or not (k.dtype == v.dtype == torch.bfloat16) or not (
+        if k.dim() != 3 or k.shape != v.shape or k.dtype is not torch.bfloat16 or v.dtype is not torch.bfloat16 or not (
                 k.is_contiguous() and v.is_contiguous()):
             raise ValueError(f'{what}: bf16 caches must be contiguous [heads, cap, d]')
         heads, cap, dc = k.shape
@@ -422,8 +438,7 @@ def attn_shared_prefix(q, prefix, tails, position, prefix_len, nq, nkv, d, *, sc
     (`tails`, caches [M * nkv, cap, d]; position int64 [M] counts the tail's slots, -1: none yet). Both are (k, v) in
     bf16 or (k, k_scale, v, v_scale) in int8."""
     _cuda(q, position, ws, out)
-    out = _attn_rows('attn_shared_prefix', q, out, nq, d)
-    m = q.shape[0]
+    m, out = _attn_rows('attn_shared_prefix', q, out, nq, d)
     ph, pcap, pdt, pp = _cache_pair('attn_shared_prefix', prefix, d)
     th, cap, tdt, tp = _cache_pair('attn_shared_prefix', tails, d)
     if pdt != tdt or ph != nkv or th != m * nkv:
@@ -431,8 +446,9 @@ def attn_shared_prefix(q, prefix, tails, position, prefix_len, nq, nkv, d, *, sc
     _positions('attn_shared_prefix', position, m)
     if ws is None:
         ws = attn_q8_ws(m, nq, nkv, d, q.device)
-    L.check(L.load().egpt_attn_shared_prefix(out.data_ptr(), out.stride(0), q.data_ptr(), q.stride(0), *pp, pcap,
-                                             prefix_len, *tp, cap, position.data_ptr(), m, nq, nkv, d, scale, pdt,
-                                             ws.data_ptr(), ws.numel(), 0, torch.cuda.current_stream().cuda_stream),
-            'attn_shared_prefix')
+    rc = L.load().egpt_attn_shared_prefix(out.data_ptr(), out.stride(0), q.data_ptr(), q.stride(0), *pp, pcap, prefix_len,
+                                          *tp, cap, position.data_ptr(), m, nq, nkv, d, scale, pdt, ws.data_ptr(),
+                                          ws.numel(), 0, _raw_stream())
+    if rc:
+        L.check(rc, 'attn_shared_prefix')
     return out
