@@ -18,7 +18,8 @@
 // next segment; warps only meet at a segment's end.
 //
 // A prefix runs first, in a launch of its own that leaves partial records (here, or in attn_prefix.cu); the launch over
-// the sequences' own keys is a dependent one that starts beside it and waits only before it adds those records up.
+// the sequences' own keys is a dependent one that starts beside it and leaves records too, and a third adds both up,
+// a warp to a row.
 //
 // Arithmetic: mma.sync with the query rows as M. Scores of int8 keys, up to 8 rows: q as fixed point X 2^(e - 29), |X| <=
 // 2^30, in four balanced base-256 digits, two of them in the MMA's rows 0-7 and 8-15, so two int8 MMAs per 32 dims
@@ -65,6 +66,7 @@ struct Params {
   float scale_log2;
   float *ws;      // partial records of this launch
   unsigned *cnt;  // arrivals per (sequence, kv head); zero between calls
+  int2 *parts;    // beside a prefix: first record and records of each (sequence, kv head)
   int keys;       // keys of the shared prefix (the launch over it)
   Prefix pre;     // of the launch over the sequences' own keys: records to add up; of the prefix's: how it is cut
 };
@@ -320,12 +322,6 @@ __device__ __forceinline__ float *record(const Params &p, int index) {
   return p.ws + (int64_t)index * kRows * (D + 2);
 }
 
-// Segments whose records a CTA has to add up: records slot .. slot + n - 1.
-constexpr int kTodo = 16;
-struct Todo {
-  int seq, g, slot, n;
-};
-
 template <int D, bool Q8, int NR>
 struct Smem {
   static constexpr int kWarps = Cfg<Q8, NR>::kWarps, kPass = NR / 2;
@@ -338,144 +334,103 @@ struct Smem {
   float row_m[NR], row_l[NR];                    // and the CTA's
   int cum[kMaxBatch + 1], len[kMaxBatch];
   int scratch[kWarps];
-  Todo todo[kTodo];
   int last[2];
 };
 
-// out[seq, heads of g] of the list's segments: their records and the prefix's, added up. A warp takes a row, or with fewer
-// rows than warps every parts-th record of one. Lanes read the maxima and sums of 32 records at once while the first
-// accumulators are on their way, so a short list costs one round trip. The order is fixed by the shapes. Every thread
-// of the CTA calls it, the list and the CTA's own records being visible to it.
-template <int D, int WARPS>
-__device__ __noinline__ void finish(const Params &p, float (*f)[D], const Todo *todo, int todos) {
+// Adds up a row's records: own_n of this launch (own0: the row's accumulators in the first) and, with PRE, pre_n of the
+// prefix's (records of pre_rows rows, pre_step floats apart). A warp takes every parts-th of them, all of their maxima and
+// sums: lanes read 32 of those at once while the first accumulators are on their way, so a short list costs one
+// round trip. The order is fixed by the shapes. -> the share's accumulators over the whole sum (zeros without any key).
+template <int D, bool PRE, int BATCH>
+__device__ __forceinline__ void add_records(const float *own0, int own_n, int row, const float *pre0, int pre_n,
+                                            int64_t pre_step, int pre_row, int pre_rows, int part, int parts,
+                                            float (&a)[D / 32]) {
   constexpr int N = D / 32;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int units = todos * p.group, parts = units < WARPS ? WARPS / units : 1;
-  if (p.pre.rec) pdl_wait();  // the launch over the prefix has finished
+  const int lane = threadIdx.x & 31, n = own_n + (PRE ? pre_n : 0);
+  auto row_of = [&](int k) -> const float * {
+    return !PRE || k < own_n ? own0 + (int64_t)k * (kRows * (D + 2)) : pre0 + (int64_t)(k - own_n) * pre_step;
+  };
+  float M = -INFINITY, lsum = 0.f;
+#pragma unroll
+  for (int e = 0; e < N; ++e) a[e] = 0.f;
 #pragma unroll 1
-  for (int u = warp; u < units * parts; u += WARPS) {
-    const int part = parts > 1 ? u / units : 0, unit = u - part * units;
-    const int entry = unit / p.group, j = unit - entry * p.group;
-    const int i = todo[entry].seq, g = todo[entry].g, own_n = todo[entry].n, slot = todo[entry].slot;
-    const float *pre0 = nullptr;  // row j's accumulators in the prefix's first record
-    int pre_n = 0, pre_rows = kRows, pre_row = 0;
-    int64_t pre_step = 0;
-    if (p.pre.rec) {
-      if (p.pre.big) {
-        const int tile = i / p.pre.seqs, pair = tile / 2;
-        const bool two = 2 * pair + 1 < p.pre.tiles;  // the pair's streams are two tiles, or both this one
-        pre_n = two ? p.pre.ranges : 2 * p.pre.ranges;
-        pre_step = two ? 2 * apx::kRecord : apx::kRecord;
-        pre_row = (i - tile * p.pre.seqs) * p.group + j, pre_rows = apx::kRowsT;
-        pre0 = p.pre.rec + ((int64_t)(g * p.pre.pairs + pair) * p.pre.ranges * 2 + (two ? tile & 1 : 0)) * apx::kRecord +
-               pre_row * D;
-      } else {
-        const int flat = i * p.group + j, seg = g * p.pre.row_tiles + flat / kRows;
-        const int start = seg * ceil_div(p.pre.seg_tiles, p.pre.pad) * p.pre.pad;
-        const int pc0 = start / p.pre.chunk;
-        pre_n = (start + p.pre.seg_tiles - 1) / p.pre.chunk - pc0 + 1;
-        pre_step = kRows * (D + 2);
-        pre_row = flat % kRows;
-        pre0 = p.pre.rec + (int64_t)(pc0 + seg) * pre_step + pre_row * D;
-      }
+  for (int k0 = 0; k0 < n; k0 += 32) {
+    float mk = -INFINITY, lk = 0.f;
+    if (k0 + lane < n) {
+      const bool own = !PRE || k0 + lane < own_n;
+      const int rows = own ? kRows : pre_rows, r = own ? row : pre_row;
+      const float *stat = row_of(k0 + lane) + (rows - r) * D + r;  // past the accumulators: maxima, then sums
+      mk = __ldcg(stat), lk = __ldcg(stat + rows);
     }
-    auto row_of = [&](int k) -> const float * {  // row j's accumulators in record k
-      return k < own_n ? p.ws + (int64_t)(slot + k) * (kRows * (D + 2)) + j * D
-                       : pre0 + (int64_t)(k - own_n) * pre_step;
-    };
-    const int n = own_n + pre_n;
-    float M = -INFINITY, lsum = 0.f, a[N];
+    const int cnt = min(32, n - k0);
+    float fk = 0.f;
+    int c = part;
+    do {
+      float v[BATCH][N];
 #pragma unroll
-    for (int e = 0; e < N; ++e) a[e] = 0.f;
-#pragma unroll 1
-    for (int k0 = 0; k0 < n; k0 += 32) {
-      float mk = -INFINITY, lk = 0.f;
-      if (k0 + lane < n) {
-        const bool own = k0 + lane < own_n;
-        const int rows = own ? kRows : pre_rows, r = own ? j : pre_row;
-        const float *stat = row_of(k0 + lane) + (rows - r) * D + r;  // past the accumulators: maxima, then sums
-        mk = __ldcg(stat), lk = __ldcg(stat + rows);
-      }
-      const int cnt = min(32, n - k0);
-      float fk = 0.f;
-      int c = part;
-      do {
-        constexpr int kBatch = 8;
-        float v[kBatch][N];
-#pragma unroll
-        for (int b = 0; b < kBatch; ++b) {
-          if (c + b * parts < cnt) {
-            const float *src = row_of(k0 + c + b * parts) + N * lane;
-            if constexpr (N == 4) {
-              const float4 t = __ldcg((const float4 *)src);
-              v[b][0] = t.x, v[b][1] = t.y, v[b][2] = t.z, v[b][3] = t.w;
-            } else if constexpr (N == 2) {
-              const float2 t = __ldcg((const float2 *)src);
-              v[b][0] = t.x, v[b][1] = t.y;
-            } else {
-              v[b][0] = __ldcg(src);
-            }
+      for (int b = 0; b < BATCH; ++b) {
+        if (c + b * parts < cnt) {
+          const float *src = row_of(k0 + c + b * parts) + N * lane;
+          if constexpr (N == 4) {
+            const float4 t = __ldcg((const float4 *)src);
+            v[b][0] = t.x, v[b][1] = t.y, v[b][2] = t.z, v[b][3] = t.w;
+          } else if constexpr (N == 2) {
+            const float2 t = __ldcg((const float2 *)src);
+            v[b][0] = t.x, v[b][1] = t.y;
+          } else {
+            v[b][0] = __ldcg(src);
           }
         }
-        if (c == part) {  // a record without keys (sum 0) has no accumulators
-          const float mx = fmaxf(M, warp_max(lk != 0.f ? mk : -INFINITY)), mz = mx == -INFINITY ? 0.f : mx;
-          const float fo = ex2(M - mz);
-          fk = lk != 0.f ? ex2(mk - mz) : 0.f;
-          M = mx;
-          lsum = lsum * fo + warp_sum(lk * fk);
+      }
+      if (c == part) {  // a record without keys (sum 0) has no accumulators
+        const float mx = fmaxf(M, warp_max(lk != 0.f ? mk : -INFINITY)), mz = mx == -INFINITY ? 0.f : mx;
+        const float fo = ex2(M - mz);
+        fk = lk != 0.f ? ex2(mk - mz) : 0.f;
+        M = mx;
+        lsum = lsum * fo + warp_sum(lk * fk);
 #pragma unroll
-          for (int e = 0; e < N; ++e) a[e] *= fo;
-        }
+        for (int e = 0; e < N; ++e) a[e] *= fo;
+      }
 #pragma unroll
-        for (int b = 0; b < kBatch; ++b) {
-          const float fc = __shfl_sync(0xffffffffu, fk, (c + b * parts) & 31);
-          if (c + b * parts < cnt && fc != 0.f)
+      for (int b = 0; b < BATCH; ++b) {
+        const float fc = __shfl_sync(0xffffffffu, fk, (c + b * parts) & 31);
+        if (c + b * parts < cnt && fc != 0.f)
 #pragma unroll
-            for (int e = 0; e < N; ++e) a[e] += v[b][e] * fc;
-        }
-        c += kBatch * parts;
-      } while (c < cnt);
-    }
-    const float inv = lsum == 0.f ? 0.f : 1.f / lsum;  // no keys at all: zeros
-    if (parts > 1) {
-#pragma unroll
-      for (int e = 0; e < N; ++e) f[u][N * lane + e] = a[e] * inv;
-    } else {
-#pragma unroll
-      for (int e = 0; e < N; ++e)
-        p.out[i * p.ldo + (int64_t)(g * p.group + j) * D + N * lane + e] = f32_to_bf16_bits(a[e] * inv);
-    }
+          for (int e = 0; e < N; ++e) a[e] += v[b][e] * fc;
+      }
+      c += BATCH * parts;
+    } while (c < cnt);
   }
-  if (parts > 1) {
-    __syncthreads();
-#pragma unroll 1
-    for (int e = threadIdx.x; e < units * D; e += 32 * WARPS) {
-      const int unit = e / D, entry = unit / p.group, j = unit - entry * p.group;
-      float a = 0.f;
-      for (int q = 0; q < parts; ++q) a += f[q * units + unit][e % D];
-      p.out[todo[entry].seq * p.ldo + (int64_t)(todo[entry].g * p.group + j) * D + e % D] = f32_to_bf16_bits(a);
-    }
-  }
-  __syncthreads();  // f and the list are free again
+  const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
+#pragma unroll
+  for (int e = 0; e < N; ++e) a[e] *= inv;
+}
+template <int N>
+__device__ __forceinline__ void store_row(uint16_t *dst, const float (&a)[N]) {
+  if constexpr (N == 4) *(uint2 *)dst = make_uint2(bf16x2(a[0], a[1]), bf16x2(a[2], a[3]));
+  else if constexpr (N == 2) *(uint32_t *)dst = bf16x2(a[0], a[1]);
+  else *dst = f32_to_bf16_bits(a[0]);
 }
 
-// NR: query rows in use, 8 or 16. PREFIX: the segments of the shared prefix, else the sequences' own keys. A (CTA, segment)
-// pair leaves its record in slot CTA + segment: both only grow along the list, so slots are the pairs' own. Without
-// a prefix a segment that one CTA holds goes straight to the output; the rest is added up at the CTA's end, a split
-// segment's by the last of its CTAs to get there.
-template <int D, bool Q8, int NR, bool PREFIX>
+// The keys of a launch: the sequences' own, alone or beside a prefix, or the prefix's.
+enum Mode { kOwn, kBeside, kPrefix };
+
+// NR: query rows in use, 8 or 16. A (CTA, segment) pair leaves its record in slot CTA + segment: both only grow along the
+// list, so slots are the pairs' own and a segment's are consecutive. Alone, a segment that one CTA holds goes
+// straight to the output, and a split one's records are added up by the last of its CTAs to get there.
+template <int D, bool Q8, int NR, Mode MODE>
 __global__ void __launch_bounds__(Cfg<Q8, NR>::kThreads, 1) attn_kernel(const Params p) {
   using C = Cfg<Q8, NR>;
   using G = Geo<D, Q8, NR>;
   using S = Smem<D, Q8, NR>;
   constexpr int kWarps = C::kWarps, STAGES = C::kStages;
   constexpr int TILE = G::kTile, NT = TILE / 8, ND = D / 8;
+  constexpr bool PREFIX = MODE == kPrefix;
   constexpr bool PLANES = Q8 && NR == 8;  // scores by int8 MMAs on the digits of q
   extern __shared__ __align__(16) uint8_t smem_raw[];
   S &sm = *(S *)smem_raw;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  // beside the prefix's launch only finish() waits: what precedes that launch is done once it has started
-  if (PREFIX || !p.pre.rec) pdl_wait();
+  if (MODE != kBeside) pdl_wait();  // (what precedes the prefix's launch is done once that has started)
   pdl_launch_dependents();
   Layout lay;
   if (PREFIX) {
@@ -489,17 +444,8 @@ __global__ void __launch_bounds__(Cfg<Q8, NR>::kThreads, 1) attn_kernel(const Pa
     const int cut = cut_at<TILE, PREFIX>(p, lay, sm.cum, sm.len, (int64_t)(blockIdx.x + (lane & 1)) * lay.chunk);
     x0 = __shfl_sync(0xffffffffu, cut, 0), x1 = __shfl_sync(0xffffffffu, cut, 1);
   }
-  int todos = 0;                // entries of sm.todo
   int split_n = 0;  // segments that this CTA shares with others: its first, its last
-  Todo split[2] = {};
-  auto add_todo = [&](const Todo &e) {  // all threads; the entry is visible after the next barrier
-    if (threadIdx.x == 0) sm.todo[todos] = e;
-    if (++todos == kTodo) {
-      __syncthreads();
-      finish<D, kWarps>(p, sm.fin, sm.todo, todos);
-      todos = 0;
-    }
-  };
+  int2 split[2] = {};  // their number and first CTA
   if (x0 < x1) {
   Seg seg = find_seg<TILE, PREFIX>(p, sm.cum, sm.len, x0);
   if (lay.pad > 1) x1 = min(x1, seg.end);
@@ -816,7 +762,7 @@ __global__ void __launch_bounds__(Cfg<Q8, NR>::kThreads, 1) attn_kernel(const Pa
       sm.row_m[threadIdx.x] = mx, sm.row_l[threadIdx.x] = l;
     }
     const bool whole = seg.start >= x0 && seg.end <= x1;
-    const bool final = !PREFIX && whole && !p.pre.rec;
+    const bool final = MODE == kOwn && whole;
     const int rows = PREFIX ? kRows : p.group;
     float *rec = record<D>(p, (int)blockIdx.x + seg.index);
     constexpr int kPass = S::kPass;
@@ -851,13 +797,13 @@ __global__ void __launch_bounds__(Cfg<Q8, NR>::kThreads, 1) attn_kernel(const Pa
       rec[kRows * D + threadIdx.x] = sm.row_m[threadIdx.x];
       rec[kRows * D + kRows + threadIdx.x] = sm.row_l[threadIdx.x];
     }
-    if (!PREFIX && !final) {
+    if (MODE != kPrefix && !final) {
       const int c0 = seg.start / lay.chunk, c1 = (seg.end - 1) / lay.chunk;
-      if (whole) {
-        add_todo({seg.seq, seg.g, (int)blockIdx.x + seg.index, 1});
-      } else {
-        (split_n ? split[1] : split[0]) = {seg.seq, seg.g, c0 + seg.index, c1 - c0 + 1};
+      if (MODE == kOwn) {
+        (split_n ? split[1] : split[0]) = make_int2(seg.index, c0);
         ++split_n;
+      } else if (seg.start >= x0 && threadIdx.x == 0) {  // (a short segment lies in one CTA wherever the even cuts are)
+        p.parts[seg.index] = make_int2(whole ? (int)blockIdx.x + seg.index : c0 + seg.index, whole ? 1 : c1 - c0 + 1);
       }
     }
     if (seg.next >= x1) break;
@@ -866,35 +812,101 @@ __global__ void __launch_bounds__(Cfg<Q8, NR>::kThreads, 1) attn_kernel(const Pa
   }
   cp_wait<0>();
   }
-  if (PREFIX) return;
-  if (split_n) {  // the last CTA of a split segment adds the parts up
-    __threadfence();
-    __syncthreads();
-    if ((int)threadIdx.x < split_n) {
-      const Todo e = threadIdx.x ? split[1] : split[0];
-      unsigned *cnt = p.cnt + e.seq * p.nkv + e.g;
-      const bool last = atomicAdd(cnt, 1u) == (unsigned)(e.n - 1);
-      if (last) {
-        *cnt = 0u;
-        __threadfence();
-      }
-      sm.last[threadIdx.x] = last;
-    }
-    __syncthreads();
-    for (int e = 0; e < split_n; ++e)
-      if (sm.last[e]) add_todo(split[e]);
+  if (MODE == kBeside) {
+    for (int e = blockIdx.x * C::kThreads + threadIdx.x; e < p.m * p.nkv; e += gridDim.x * C::kThreads)
+      if (sm.len[e / p.nkv] == 0) p.parts[e] = make_int2(0, 0);
+    pdl_wait();  // the prefix's launch: what waits for this one has waited for both
   }
-  for (int e = blockIdx.x; e < p.m * p.nkv; e += gridDim.x)  // sequences without keys of their own
-    if (sm.len[e / p.nkv] == 0) add_todo({e / p.nkv, e % p.nkv, 0, 0});
-  if (todos) {
+  if (MODE != kOwn) return;
+  for (int e = blockIdx.x; e < p.m * p.nkv; e += gridDim.x)  // sequences without keys
+    if (sm.len[e / p.nkv] == 0)
+      for (int c = threadIdx.x; c < p.group * D; c += C::kThreads)
+        p.out[(e / p.nkv) * p.ldo + (int64_t)(e % p.nkv) * p.group * D + c] = 0;
+  if (!split_n) return;
+  __threadfence();
+  __syncthreads();
+  if ((int)threadIdx.x < split_n) {
+    const int2 e = threadIdx.x ? split[1] : split[0];
+    const Seg sg = own_seg<TILE>(p, sm.cum, sm.len, e.x / p.nkv, e.x % p.nkv);
+    const int n = (sg.end - 1) / lay.chunk - e.y + 1;
+    const bool last = atomicAdd(p.cnt + e.x, 1u) == (unsigned)(n - 1);
+    if (last) {
+      p.cnt[e.x] = 0u;
+      __threadfence();
+    }
+    sm.last[threadIdx.x] = last ? n : 0;
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int s = 0; s < split_n; ++s) {
+    const int n = sm.last[s];
+    if (!n) continue;
+    // a warp takes a row, or with fewer rows than warps every parts-th record of one
+    const int2 e = s ? split[1] : split[0];
+    const int parts = p.group < kWarps ? kWarps / p.group : 1, part = parts > 1 ? warp / p.group : 0;
+    uint16_t *out = p.out + (e.x / p.nkv) * p.ldo + (int64_t)(e.x % p.nkv) * p.group * D;
+    const float *rec = record<D>(p, e.y + e.x);
+#pragma unroll 1
+    for (int j = warp - part * p.group; j < p.group && part < parts; j += kWarps) {
+      float a[D / 32];
+      add_records<D, false, 8>(rec + j * D, n, j, nullptr, 0, 0, 0, 0, part, parts, a);
+      if (parts == 1) {
+        store_row(out + j * D + D / 32 * lane, a);
+      } else {
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) sm.fin[warp][D / 32 * lane + i] = a[i];
+      }
+    }
+    if (parts == 1) continue;
     __syncthreads();
-    finish<D, kWarps>(p, sm.fin, sm.todo, todos);
+    for (int i = threadIdx.x; i < p.group * D; i += C::kThreads) {
+      float v = 0.f;
+      for (int q = 0; q < parts; ++q) v += sm.fin[q * p.group + i / D][i % D];
+      out[i] = f32_to_bf16_bits(v);
+    }
+    __syncthreads();  // sm.fin is free again
   }
 }
 
-template <int D, bool Q8, int NR, bool PREFIX>
+// Beside a prefix: one (sequence, head) row per warp, its own records and the prefix's.
+constexpr int kAddWarps = 4;
+template <int D>
+__global__ void __launch_bounds__(32 * kAddWarps) add_kernel(const Params p) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int lane = threadIdx.x & 31, unit = blockIdx.x * kAddWarps + (threadIdx.x >> 5);
+  const int nq = p.nkv * p.group;
+  if (unit >= p.m * nq) return;
+  const int i = unit / nq, h = unit - i * nq, g = h / p.group, j = h - g * p.group;
+  const int2 own = p.parts[i * p.nkv + g];
+  const float *pre0;  // the row's accumulators in the prefix's first record
+  int pre_n, pre_rows = kRows, pre_row;
+  int64_t pre_step;
+  if (p.pre.big) {
+    const int tile = i / p.pre.seqs, pair = tile / 2;
+    const bool two = 2 * pair + 1 < p.pre.tiles;  // the pair's streams are two tiles, or both this one
+    pre_n = two ? p.pre.ranges : 2 * p.pre.ranges;
+    pre_step = two ? 2 * apx::kRecord : apx::kRecord;
+    pre_row = (i - tile * p.pre.seqs) * p.group + j, pre_rows = apx::kRowsT;
+    pre0 = p.pre.rec + ((int64_t)(g * p.pre.pairs + pair) * p.pre.ranges * 2 + (two ? tile & 1 : 0)) * apx::kRecord;
+  } else {
+    const int flat = i * p.group + j, seg = g * p.pre.row_tiles + flat / kRows;
+    const int start = seg * ceil_div(p.pre.seg_tiles, p.pre.pad) * p.pre.pad;
+    const int c0 = start / p.pre.chunk;
+    pre_n = (start + p.pre.seg_tiles - 1) / p.pre.chunk - c0 + 1;
+    pre_step = kRows * (D + 2);
+    pre_row = flat % kRows;
+    pre0 = p.pre.rec + (int64_t)(c0 + seg) * pre_step;
+  }
+  float a[D / 32];
+  add_records<D, true, 16>(record<D>(p, own.x) + j * D, own.y, j, pre0 + pre_row * D, pre_n, pre_step, pre_row, pre_rows,
+                           0, 1, a);
+  store_row(p.out + i * p.ldo + (int64_t)h * D + D / 32 * lane, a);
+}
+
+template <int D, bool Q8, int NR, Mode MODE>
 static cudaError_t launch(const Params &p, int grid, cudaStream_t st, bool pdl) {
-  auto fn = attn_kernel<D, Q8, NR, PREFIX>;
+  auto fn = attn_kernel<D, Q8, NR, MODE>;
   const size_t smem = sizeof(Smem<D, Q8, NR>);
   static int configured[64] = {0};  // the shared-memory opt-in, per device
   int dev = 0;
@@ -933,23 +945,24 @@ static int cut_prefix(Params &p) {
   }
   return ceil_div(segs * ceil_div(c.seg_tiles, c.pad) * c.pad, c.chunk);
 }
-template <bool Q8, int NR, bool PREFIX>
+template <bool Q8, int NR, Mode MODE>
 static cudaError_t launch_d(Params &p, int d, cudaStream_t st, bool pdl) {
-  const int grid = PREFIX ? cut_prefix<Cfg<Q8, NR>>(p) : own_grid<Cfg<Q8, NR>>(p);
+  const int grid = MODE == kPrefix ? cut_prefix<Cfg<Q8, NR>>(p) : own_grid<Cfg<Q8, NR>>(p);
   p.head_share = grid / p.nkv;
-  return d == 128 ? launch<128, Q8, NR, PREFIX>(p, grid, st, pdl)
-                  : (d == 64 ? launch<64, Q8, NR, PREFIX>(p, grid, st, pdl) : launch<32, Q8, NR, PREFIX>(p, grid, st, pdl));
+  return d == 128 ? launch<128, Q8, NR, MODE>(p, grid, st, pdl)
+                  : (d == 64 ? launch<64, Q8, NR, MODE>(p, grid, st, pdl) : launch<32, Q8, NR, MODE>(p, grid, st, pdl));
 }
-template <bool PREFIX>
+template <Mode MODE>
 static cudaError_t launch_any(Params &p, int d, bool q8, int rows, cudaStream_t st, bool pdl) {
-  if (rows <= 8) return q8 ? launch_d<true, 8, PREFIX>(p, d, st, pdl) : launch_d<false, 8, PREFIX>(p, d, st, pdl);
-  return q8 ? launch_d<true, 16, PREFIX>(p, d, st, pdl) : launch_d<false, 16, PREFIX>(p, d, st, pdl);
+  if (rows <= 8) return q8 ? launch_d<true, 8, MODE>(p, d, st, pdl) : launch_d<false, 8, MODE>(p, d, st, pdl);
+  return q8 ? launch_d<true, 16, MODE>(p, d, st, pdl) : launch_d<false, 16, MODE>(p, d, st, pdl);
 }
 // Whether the prefix goes to attn_prefix_kernel: bf16, head_dim 128, more rows than one tile of the mma.sync kernel.
 static bool prefix_on_tcgen05(const Params &p, int d, bool q8) {
   return !q8 && d == apx::kD && p.scale_log2 > 0.f && p.m * p.group > kRows;
 }
-static size_t counter_bytes(int64_t m, int nkv) { return ((size_t)m * nkv * 4 + 255) / 256 * 256; }
+// Arrival counters, then the (first record, records) pairs of the segments.
+static size_t counter_bytes(int64_t m, int nkv) { return ((size_t)m * nkv * 16 + 255) / 256 * 256; }
 
 static int check(const char *what, int64_t ldo, int64_t ldq, const void *out, const void *q, int64_t cap, int64_t m,
                  int nq, int nkv, int d, float scale, const void *ws, size_t ws_bytes) {
@@ -997,8 +1010,9 @@ extern "C" int egpt_attn_decode_q8(void *out, int64_t ldo, const void *q, int64_
   p.out = (uint16_t *)out, p.ldo = ldo, p.q = (const uint16_t *)q, p.ldq = ldq;
   p.cache = {(const uint8_t *)k_cache, (const uint8_t *)v_cache, k_scale, v_scale, cap};
   p.position = position, p.m = (int)m, p.nkv = nkv, p.group = nq / nkv, p.scale_log2 = scale * 1.4426950408889634f;
-  p.cnt = (unsigned *)ws, p.ws = (float *)((char *)ws + aq8::counter_bytes(m, nkv));
-  return check_launch(aq8::launch_any<false>(p, d, true, p.group, (cudaStream_t)stream, (flags & EGPT_FLAG_PDL) != 0),
+  p.cnt = (unsigned *)ws, p.parts = (int2 *)((char *)ws + (size_t)m * nkv * 8);
+  p.ws = (float *)((char *)ws + aq8::counter_bytes(m, nkv));
+  return check_launch(aq8::launch_any<aq8::kOwn>(p, d, true, p.group, (cudaStream_t)stream, (flags & EGPT_FLAG_PDL) != 0),
                       "attn_decode_q8_kernel");
 }
 
@@ -1022,11 +1036,12 @@ extern "C" int egpt_attn_shared_prefix(void *out, int64_t ldo, const void *q, in
   if ((uintptr_t)pk % 16 || (uintptr_t)pv % 16 || (uintptr_t)tk % 16 || (uintptr_t)tv % 16)
     return set_error(EGPT_ERR_ALIGN, "attn_shared_prefix: caches must be 16-byte aligned");
   const cudaStream_t st = (cudaStream_t)stream;
-  bool pdl = (flags & EGPT_FLAG_PDL) != 0;
+  const bool pdl = (flags & EGPT_FLAG_PDL) != 0;
   aq8::Params p{};
   p.out = (uint16_t *)out, p.ldo = ldo, p.q = (const uint16_t *)q, p.ldq = ldq;
   p.position = position, p.m = (int)m, p.nkv = nkv, p.group = nq / nkv, p.scale_log2 = scale * 1.4426950408889634f;
-  p.cnt = (unsigned *)ws, p.ws = (float *)((char *)ws + aq8::counter_bytes(m, nkv));
+  p.cnt = (unsigned *)ws, p.parts = (int2 *)((char *)ws + (size_t)m * nkv * 8);
+  p.ws = (float *)((char *)ws + aq8::counter_bytes(m, nkv));
   float *pre_rec = p.ws + ((size_t)aq8::max_grid() + (size_t)m * nkv) * aq8::kRows * (d + 2);
   if (prefix_len > 0) {
     if (aq8::prefix_on_tcgen05(p, d, q8)) {
@@ -1042,13 +1057,20 @@ extern "C" int egpt_attn_shared_prefix(void *out, int64_t ldo, const void *q, in
       aq8::Params a = p;
       a.cache = {(const uint8_t *)pk, (const uint8_t *)pv, pk_scale, pv_scale, prefix_cap};
       a.keys = (int)prefix_len, a.ws = pre_rec;
-      const cudaError_t e = aq8::launch_any<true>(a, d, q8, (int)m * p.group, st, pdl);
+      const cudaError_t e = aq8::launch_any<aq8::kPrefix>(a, d, q8, (int)m * p.group, st, pdl);
       if (e != cudaSuccess) return check_launch(e, "attn_shared_prefix_kernel (prefix)");
       p.pre = a.pre;
     }
     p.pre.rec = pre_rec;
-    pdl = true;
   }
   p.cache = {(const uint8_t *)tk, (const uint8_t *)tv, tk_scale, tv_scale, cap};
-  return check_launch(aq8::launch_any<false>(p, d, q8, p.group, st, pdl), "attn_shared_prefix_kernel");
+  if (!p.pre.rec)
+    return check_launch(aq8::launch_any<aq8::kOwn>(p, d, q8, p.group, st, pdl), "attn_shared_prefix_kernel");
+  const cudaError_t e = aq8::launch_any<aq8::kBeside>(p, d, q8, p.group, st, true);
+  if (e != cudaSuccess) return check_launch(e, "attn_shared_prefix_kernel");
+  const void *fn = d == 128 ? (const void *)aq8::add_kernel<128>
+                            : (d == 64 ? (const void *)aq8::add_kernel<64> : (const void *)aq8::add_kernel<32>);
+  return check_launch(launch_kernel(fn, dim3((unsigned)((m * nq + aq8::kAddWarps - 1) / aq8::kAddWarps)),
+                                    dim3(32 * aq8::kAddWarps), 0, st, true, p),
+                      "attn_shared_prefix_add_kernel");
 }

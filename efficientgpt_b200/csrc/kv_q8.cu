@@ -47,63 +47,71 @@ __device__ __forceinline__ int code_of(float x, float s) {
   return (int)fminf(fmaxf(rintf(__fdiv_rn(x, s)), -127.f), 127.f);
 }
 
+// Codes of eight elements, one to a byte. A product with 1 / s is within 2^-15 of the quotient, so it decides every code
+// whose quotient is not that near to a half; the others (about one in ten thousand) take the division. The rounding is
+// that of a sum with 1.5 2^23, whose low byte is the code (|x / s| < 127.5 by the choice of s: nothing to clamp).
+__device__ __forceinline__ uint2 codes_of(const float (&x)[8], float s) {
+  constexpr float kMagic = 12582912.f;
+  const float r = __frcp_rn(s);
+  float near = 0.f;
+  uint32_t b[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float y = x[e] * r, m = y + kMagic;
+    near = fmaxf(near, fabsf(y - (m - kMagic)));
+    b[e] = __float_as_uint(m);
+  }
+  if (near > 0.4999f) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) b[e] = (uint32_t)code_of(x[e], s);
+  }
+  return make_uint2(__byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410),
+                    __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410));
+}
+
 // Rows as they are: D / 8 lanes hold a row, 16 bytes (bf16) or 32 bytes (fp32) each, so it is read once and its maximum
-// needs a few shuffles; a thread takes the same piece of kRowsPerThread rows of the flat list of (row, head) and of both K
-// and V, whose loads are all on their way before the first is used.
-constexpr int kRowsPerThread = 2;
+// needs a few shuffles; a thread takes the K and the V piece of one (row, head), heads innermost as they lie in the rows
+// (4096 rows of 8 heads: 12 us; with the rows innermost, as they lie in the cache, 16).
 template <int D, bool F32>
 __global__ void __launch_bounds__(kThreads) append_kernel(AppendParams p) {
   constexpr int kLanes = D / 8, kRows = kThreads / kLanes;
   pdl_wait();
   pdl_launch_dependents();
   const int e0 = (int)(threadIdx.x % kLanes) * 8;
-  const unsigned items = (unsigned)(p.m * p.nkv);
-  float x[kRowsPerThread][2][8];
-  unsigned row[kRowsPerThread], head[kRowsPerThread];
-  bool live[kRowsPerThread];
+  const unsigned item = blockIdx.x * kRows + threadIdx.x / kLanes, nkv = (unsigned)p.nkv;
+  const bool live = item < (unsigned)p.m * nkv;
+  const unsigned row = live ? item / nkv : 0, head = live ? item - row * nkv : 0;
+  float x[2][8];
 #pragma unroll
-  for (int i = 0; i < kRowsPerThread; ++i) {
-    const unsigned item = (blockIdx.x * kRowsPerThread + i) * kRows + threadIdx.x / kLanes;
-    live[i] = item < items;
-    row[i] = live[i] ? item / (unsigned)p.nkv : 0;
-    head[i] = live[i] ? item - row[i] * (unsigned)p.nkv : 0;
+  for (int kv = 0; kv < 2; ++kv) {
+    const int64_t at = (int64_t)row * (kv ? p.ldv : p.ldk) + (int64_t)head * D + e0;  // (row 0 if not live)
+    if (F32) {
+      const float4 *src = (const float4 *)((const float *)(kv ? p.v : p.k) + at);
+      const float4 a = src[0], b = src[1];
+      const float y[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
-    for (int kv = 0; kv < 2; ++kv) {
-      const int64_t at = (int64_t)row[i] * (kv ? p.ldv : p.ldk) + (int64_t)head[i] * D + e0;  // (row 0 if not live)
-      if (F32) {
-        const float4 *src = (const float4 *)((const float *)(kv ? p.v : p.k) + at);
-        const float4 a = src[0], b = src[1];
-        const float y[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+      for (int e = 0; e < 8; ++e) x[kv][e] = y[e];
+    } else {
+      const uint4 a = *(const uint4 *)((const uint16_t *)(kv ? p.v : p.k) + at);
+      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[i][kv][e] = y[e];
-      } else {
-        const uint4 a = *(const uint4 *)((const uint16_t *)(kv ? p.v : p.k) + at);
-        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[i][kv][2 * e] = bf16_lo(w[e]), x[i][kv][2 * e + 1] = bf16_hi(w[e]);
-      }
+      for (int e = 0; e < 4; ++e) x[kv][2 * e] = bf16_lo(w[e]), x[kv][2 * e + 1] = bf16_hi(w[e]);
     }
   }
+  int64_t head0 = 0;
+  const int64_t slot = live ? slot_of(p, row, head0) : -1;
+  const int64_t dst = (head0 + head) * p.cap + slot;
 #pragma unroll
-  for (int i = 0; i < kRowsPerThread; ++i) {
-    int64_t head0 = 0;
-    const int64_t slot = live[i] ? slot_of(p, row[i], head0) : -1;
-    const int64_t dst = (head0 + head[i]) * p.cap + slot;
+  for (int kv = 0; kv < 2; ++kv) {
+    float amax = 0.f;
 #pragma unroll
-    for (int kv = 0; kv < 2; ++kv) {
-      float amax = 0.f;
+    for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(x[kv][e]));
 #pragma unroll
-      for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(x[i][kv][e]));
-#pragma unroll
-      for (int o = kLanes / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-      if (slot < 0) continue;
-      const float s = row_scale(amax);
-      uint32_t w[2] = {0u, 0u};
-#pragma unroll
-      for (int e = 0; e < 8; ++e) w[e / 4] |= (uint32_t)(code_of(x[i][kv][e], s) & 0xff) << (8 * (e % 4));
-      *(uint2 *)((kv ? p.v_cache : p.k_cache) + dst * D + e0) = make_uint2(w[0], w[1]);
-      if (e0 == 0) (kv ? p.v_scale : p.k_scale)[dst] = s;
-    }
+    for (int o = kLanes / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    if (slot < 0) continue;
+    const float s = row_scale(amax);
+    *(uint2 *)((kv ? p.v_cache : p.k_cache) + dst * D + e0) = codes_of(x[kv], s);
+    if (e0 == 0) (kv ? p.v_scale : p.k_scale)[dst] = s;
   }
 }
 
@@ -189,9 +197,9 @@ struct ReadParams {
 };
 
 // out[h][r] = q s of row start + r of head h (blockIdx.y; K, then V, in blockIdx.z): 16 codes (one 16-byte load) per
-// thread and row, D / 16 threads to a row, kReadRows rows' loads on their way at once.
-constexpr int kReadRows = 4;
-template <int D, bool F32>
+// thread and row, D / 16 threads to a row, ROWS rows' loads on their way at once: four where that still fills the GPU
+// (32768 rows of 8 heads: 37.9 us, 43.0 with one), one for short stretches (257 rows of 6 heads: 2.2 us, 3.1 with four).
+template <int D, bool F32, int ROWS>
 __global__ void __launch_bounds__(kThreads) read_kernel(ReadParams p) {
   constexpr int kLanes = D / 16, kStep = kThreads / kLanes;
   pdl_wait();
@@ -202,19 +210,19 @@ __global__ void __launch_bounds__(kThreads) read_kernel(ReadParams p) {
     const int64_t start = p.start + (p.starts ? p.starts[h / p.group] : 0);
     const int8_t *codes = (is_v ? p.v_cache : p.k_cache) + h * p.cap * D + e0;
     const float *scales = (is_v ? p.v_scale : p.k_scale) + h * p.cap;
-    for (int64_t r0 = (int64_t)blockIdx.x * kStep * kReadRows + threadIdx.x / kLanes; r0 < p.count;
-         r0 += (int64_t)gridDim.x * kStep * kReadRows) {
-      uint4 c[kReadRows];
-      float s[kReadRows];
+    for (int64_t r0 = (int64_t)blockIdx.x * kStep * ROWS + threadIdx.x / kLanes; r0 < p.count;
+         r0 += (int64_t)gridDim.x * kStep * ROWS) {
+      uint4 c[ROWS];
+      float s[ROWS];
 #pragma unroll
-      for (int i = 0; i < kReadRows; ++i) {
+      for (int i = 0; i < ROWS; ++i) {
         const int64_t r = r0 + i * kStep, slot = start + r;
         const bool in = r < p.count && slot >= 0 && slot < p.cap;  // slots outside the cache read as zeros
         c[i] = in ? __ldcs((const uint4 *)(codes + slot * D)) : make_uint4(0u, 0u, 0u, 0u);
         s[i] = in ? scales[slot] : 0.f;
       }
 #pragma unroll
-      for (int i = 0; i < kReadRows; ++i) {
+      for (int i = 0; i < ROWS; ++i) {
         const int64_t r = r0 + i * kStep;
         if (r >= p.count) break;
         const uint32_t w[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
@@ -245,8 +253,9 @@ static const void *append_fn(bool f32) {
   return f32 ? (const void *)append_kernel<D, true> : (const void *)append_kernel<D, false>;
 }
 template <int D>
-static const void *read_fn(bool f32) {
-  return f32 ? (const void *)read_kernel<D, true> : (const void *)read_kernel<D, false>;
+static const void *read_fn(bool f32, bool four) {
+  if (four) return f32 ? (const void *)read_kernel<D, true, 4> : (const void *)read_kernel<D, false, 4>;
+  return f32 ? (const void *)read_kernel<D, true, 1> : (const void *)read_kernel<D, false, 1>;
 }
 
 }  // namespace kvq
@@ -295,7 +304,7 @@ extern "C" int egpt_kv_append_q8(int8_t *k_cache, float *k_scale, int8_t *v_cach
   }
   if (q_out || q_norm_w || k_norm_w || rope_cos || rope_sin)
     return set_error(EGPT_ERR_ARG, "kv_append_q8: norm and RoPE need q");
-  const int64_t per_cta = (int64_t)kvq::kRowsPerThread * kvq::kThreads / (d / 8);  // (row, head) pairs
+  const int64_t per_cta = kvq::kThreads / (d / 8);  // (head, row) pairs
   const void *fn = d == 128 ? kvq::append_fn<128>(f32) : (d == 64 ? kvq::append_fn<64>(f32) : kvq::append_fn<32>(f32));
   return check_launch(launch_kernel(fn, dim3((unsigned)((m * nkv + per_cta - 1) / per_cta)), dim3(kvq::kThreads), 0,
                                     (cudaStream_t)stream, pdl, p),
@@ -324,10 +333,12 @@ extern "C" int egpt_kv_read_q8(void *k_out, void *v_out, int64_t out_head_stride
   p.k_out = k_out, p.v_out = v_out, p.out_head = out_head_stride, p.k_cache = k_cache, p.v_cache = v_cache;
   p.k_scale = k_scale, p.v_scale = v_scale, p.cap = cap, p.start = start, p.count = count, p.heads = heads;
   p.starts = starts, p.group = starts ? heads_per_start : 1;
-  const int64_t per_cta = (int64_t)kvq::kReadRows * kvq::kThreads / (d / 16);
+  const bool four = 2 * heads * count * (d / 16) >= (int64_t)num_sms() * 4 * 4 * kvq::kThreads;
+  const int64_t per_cta = (int64_t)(four ? 4 : 1) * kvq::kThreads / (d / 16);
   const dim3 grid((unsigned)std::min<int64_t>((count + per_cta - 1) / per_cta, 1 << 16),
                   (unsigned)std::min<int64_t>(heads, 65535), 2);
-  const void *fn = d == 128 ? kvq::read_fn<128>(f32) : (d == 64 ? kvq::read_fn<64>(f32) : kvq::read_fn<32>(f32));
+  const void *fn = d == 128 ? kvq::read_fn<128>(f32, four)
+                              : (d == 64 ? kvq::read_fn<64>(f32, four) : kvq::read_fn<32>(f32, four));
   return check_launch(launch_kernel(fn, grid, dim3(kvq::kThreads), 0, (cudaStream_t)stream,
                                     (flags & EGPT_FLAG_PDL) != 0, p),
                       "kv_read_q8_kernel");
