@@ -447,424 +447,425 @@ __global__ void __launch_bounds__(Cfg<Q8, NR>::kThreads, 1) attn_kernel(const Pa
   int split_n = 0;  // segments that this CTA shares with others: its first, its last
   int2 split[2] = {};  // their number and first CTA
   if (x0 < x1) {
-  Seg seg = find_seg<TILE, PREFIX>(p, sm.cum, sm.len, x0);
-  if (lay.pad > 1) x1 = min(x1, seg.end);
+    Seg seg = find_seg<TILE, PREFIX>(p, sm.cum, sm.len, x0);
+    if (lay.pad > 1) x1 = min(x1, seg.end);
 
-  // ---- this warp's loads: every kWarps-th tile of a segment's part, STAGES - 1 tiles ahead. 32 lanes take 512 consecutive bytes
-  // of a full tile at a time; the swizzles split into a part of the lane and one of the step.
-  int lx = x0 + warp, lslot = 0;
-  Seg ls = seg;
-  constexpr int kStep = 32 / G::kChunks;  // rows per 512 bytes
-  const int lr = lane / G::kChunks, lc = lane % G::kChunks;
-  const uint32_t ring = smem_u32(sm.ring[warp][0]);
-  const uint32_t k_dst = ring + lr * G::kRowBytes + ((lc ^ G::k_swz(lr)) * 16);
-  const uint32_t v_dst = lr * G::kRowBytes + ((lc ^ G::v_swz(lr)) * 16);
-  auto load_next = [&]() {
-    while (lx >= ls.end && ls.next < x1) {
-      ls = next_seg<TILE, PREFIX>(p, sm.cum, sm.len, ls);
-      lx = ls.start + warp;
-    }
-    if (lx < min(ls.end, x1)) {
-      const uint32_t st = (uint32_t)(lslot * G::kStageBytes);
-      const Cache &c = p.cache;
-      const int key0 = (lx - ls.start) * TILE, left = ls.len - key0;
-      const int64_t row0 = (PREFIX ? ls.g : (int64_t)ls.seq * p.nkv + ls.g) * c.cap + key0;
-      const uint8_t *kb = c.k + row0 * G::kRowBytes + lane * 16, *vb = c.v + row0 * G::kRowBytes + lane * 16;
-      // v_swz(it kStep + lr) = v_swz(it kStep) ^ v_swz(lr) (the row bits it uses do not carry)
-      const uint32_t kd = st + k_dst, vd = st + ring + TILE * G::kRowBytes;
-      if (left >= TILE) {
+    // ---- this warp's loads: every kWarps-th tile of a segment's part, STAGES - 1 tiles ahead. 32 lanes take 512 consecutive bytes
+    // of a full tile at a time; the swizzles split into a part of the lane and one of the step.
+    int lx = x0 + warp, lslot = 0;
+    Seg ls = seg;
+    constexpr int kStep = 32 / G::kChunks;  // rows per 512 bytes
+    const int lr = lane / G::kChunks, lc = lane % G::kChunks;
+    const uint32_t ring = smem_u32(sm.ring[warp][0]);
+    const uint32_t k_dst = ring + lr * G::kRowBytes + ((lc ^ G::k_swz(lr)) * 16);
+    const uint32_t v_dst = lr * G::kRowBytes + ((lc ^ G::v_swz(lr)) * 16);
+    auto load_next = [&]() {
+      while (lx >= ls.end && ls.next < x1) {
+        ls = next_seg<TILE, PREFIX>(p, sm.cum, sm.len, ls);
+        lx = ls.start + warp;
+      }
+      if (lx < min(ls.end, x1)) {
+        const uint32_t st = (uint32_t)(lslot * G::kStageBytes);
+        const Cache &c = p.cache;
+        const int key0 = (lx - ls.start) * TILE, left = ls.len - key0;
+        const int64_t row0 = (PREFIX ? ls.g : (int64_t)ls.seq * p.nkv + ls.g) * c.cap + key0;
+        const uint8_t *kb = c.k + row0 * G::kRowBytes + lane * 16, *vb = c.v + row0 * G::kRowBytes + lane * 16;
+        // v_swz(it kStep + lr) = v_swz(it kStep) ^ v_swz(lr) (the row bits it uses do not carry)
+        const uint32_t kd = st + k_dst, vd = st + ring + TILE * G::kRowBytes;
+        if (left >= TILE) {
 #pragma unroll
-        for (int it = 0; it < TILE / kStep; ++it) {
-          cp16(kd + it * 512, kb + it * 512);
-          cp16(vd + (v_dst ^ (G::v_swz(it * kStep) * 16)) + it * 512, vb + it * 512);
-        }
-      } else {
+          for (int it = 0; it < TILE / kStep; ++it) {
+            cp16(kd + it * 512, kb + it * 512);
+            cp16(vd + (v_dst ^ (G::v_swz(it * kStep) * 16)) + it * 512, vb + it * 512);
+          }
+        } else {
 #pragma unroll 1
-        for (int it = 0; it < TILE / kStep; ++it) {
-          const bool in = it * kStep + lr < left;
-          cp16z(kd + it * 512, in ? kb + it * 512 : c.k, in ? 16 : 0);
-          cp16z(vd + (v_dst ^ (G::v_swz(it * kStep) * 16)) + it * 512, in ? vb + it * 512 : c.v, in ? 16 : 0);
+          for (int it = 0; it < TILE / kStep; ++it) {
+            const bool in = it * kStep + lr < left;
+            cp16z(kd + it * 512, in ? kb + it * 512 : c.k, in ? 16 : 0);
+            cp16z(vd + (v_dst ^ (G::v_swz(it * kStep) * 16)) + it * 512, in ? vb + it * 512 : c.v, in ? 16 : 0);
+          }
+        }
+        if (Q8) {
+          const uint32_t sc = ring + st + 2 * TILE * G::kRowBytes + lane * 4;  // [ks of the tile][vs of the tile]
+          const bool in = lane < left;
+          cp4(sc, c.ks + row0 + (in ? lane : 0), in ? 4 : 0);
+          cp4(sc + TILE * 4, c.vs + row0 + (in ? lane : 0), in ? 4 : 0);
         }
       }
-      if (Q8) {
-        const uint32_t sc = ring + st + 2 * TILE * G::kRowBytes + lane * 4;  // [ks of the tile][vs of the tile]
-        const bool in = lane < left;
-        cp4(sc, c.ks + row0 + (in ? lane : 0), in ? 4 : 0);
-        cp4(sc + TILE * 4, c.vs + row0 + (in ? lane : 0), in ? 4 : 0);
-      }
-    }
-    cp_commit();
-    lx += kWarps;
-    lslot = lslot + 1 == STAGES ? 0 : lslot + 1;
-  };
-  // the segment's query rows, dims d0 .. d0 + 3 of every 16-dim step: those of the key words that this thread loads
-  uint2 qw[NR / 8][D / 16];
-  auto load_q = [&](const Seg &sg) {
+      cp_commit();
+      lx += kWarps;
+      lslot = lslot + 1 == STAGES ? 0 : lslot + 1;
+    };
+    // the segment's query rows, dims d0 .. d0 + 3 of every 16-dim step: those of the key words that this thread loads
+    uint2 qw[NR / 8][D / 16];
+    auto load_q = [&](const Seg &sg) {
 #pragma unroll
-    for (int hh = 0; hh < NR / 8; ++hh) {
-      const int r = g + 8 * hh;
-      int64_t tok = -1;
-      int h = 0;
-      if (PREFIX) {
-        const int flat = sg.tile * kRows + r;
-        if (flat < p.m * p.group) tok = flat / p.group, h = sg.g * p.group + flat % p.group;
-      } else if (r < p.group) {
-        tok = sg.seq, h = sg.g * p.group + r;
-      }
-      const uint16_t *qr = p.q + (tok >= 0 ? tok * p.ldq + (int64_t)h * D : 0);
-#pragma unroll
-      for (int s = 0; s < D / 16; ++s) {
-        const int d0 = Q8 ? (D == 32 ? 8 * t + 4 * s : 16 * (t + 4 * (s / 4)) + 4 * (s % 4))
-                          : 8 * (t + 4 * (s / 2)) + 4 * (s % 2);
-        qw[hh][s] = tok >= 0 ? *(const uint2 *)(qr + d0) : make_uint2(0u, 0u);
-      }
-    }
-  };
-  load_q(seg);  // before the keys and values queue up in front of it
-#pragma unroll 1
-  for (int s = 0; s < STAGES - 1; ++s) load_next();
-
-  int cslot = 0;
-  for (;;) {
-    // ---- the segment's query rows as MMA fragments
-    uint32_t qa[PLANES ? D / 32 : D / 16][PLANES ? 8 : 4];
-    float rowfac[2] = {p.scale_log2, p.scale_log2};  // and for int8 the power of two that q was divided by
-#pragma unroll
-    for (int hh = 0; hh < NR / 8; ++hh) {
-      const uint2(&w)[D / 16] = qw[hh];
-      uint32_t amax2 = 0u;  // the largest magnitudes of the even and odd elements, as bf16 bits (NaN above infinity)
-#pragma unroll
-      for (int s = 0; s < D / 16; ++s)
-        if (Q8) amax2 = __vmaxu2(amax2, __vmaxu2(w[s].x & 0x7fff7fffu, w[s].y & 0x7fff7fffu));
-      if (Q8) {
-        amax2 = __vmaxu2(amax2, __shfl_xor_sync(0xffffffffu, amax2, 1));
-        amax2 = __vmaxu2(amax2, __shfl_xor_sync(0xffffffffu, amax2, 2));
-        const int amax = (int)max(amax2 & 0xffffu, amax2 >> 16);
-        // a largest magnitude in [2^e, 2^(e + 1)) becomes one in [2^B, 2^(B + 1)): as fixed point (B = 29) bf16's 8 bits stay exact for
-        // elements down to 2^-22 of the row's largest, in f16 (B = 14) down to 2^-28. (The exponent is kept where both
-        // factors are normal numbers.)
-        constexpr int B = PLANES ? 29 : 14;
-        const int e = min(max((amax >> 7) - 127, B - 126), 127);
-        const float up = __uint_as_float((uint32_t)(127 + B - e) << 23);
-        rowfac[hh] *= __uint_as_float((uint32_t)(127 - B + e) << 23);
-        if (amax >= 0x7f80) rowfac[hh] = NAN;  // an infinity or NaN in the row: its scores are NaN
+      for (int hh = 0; hh < NR / 8; ++hh) {
+        const int r = g + 8 * hh;
+        int64_t tok = -1;
+        int h = 0;
+        if (PREFIX) {
+          const int flat = sg.tile * kRows + r;
+          if (flat < p.m * p.group) tok = flat / p.group, h = sg.g * p.group + flat % p.group;
+        } else if (r < p.group) {
+          tok = sg.seq, h = sg.g * p.group + r;
+        }
+        const uint16_t *qr = p.q + (tok >= 0 ? tok * p.ldq + (int64_t)h * D : 0);
 #pragma unroll
         for (int s = 0; s < D / 16; ++s) {
-          const float y[4] = {bf16_lo(w[s].x) * up, bf16_hi(w[s].x) * up, bf16_lo(w[s].y) * up, bf16_hi(w[s].y) * up};
-          if constexpr (PLANES) {
-            // bytes of X + 0x80808080 are the digits plus 128; a 4 x 4 byte transpose makes words of one digit (d[0] the
-            // lowest) of the four dims
-            uint32_t Y[4], d[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) Y[i] = ((uint32_t)__float2int_rn(y[i]) + 0x80808080u) ^ 0x80808080u;
-            const uint32_t lo01 = __byte_perm(Y[0], Y[1], 0x5140), hi01 = __byte_perm(Y[0], Y[1], 0x7362);
-            const uint32_t lo23 = __byte_perm(Y[2], Y[3], 0x5140), hi23 = __byte_perm(Y[2], Y[3], 0x7362);
-            d[0] = __byte_perm(lo01, lo23, 0x5410), d[1] = __byte_perm(lo01, lo23, 0x7632);
-            d[2] = __byte_perm(hi01, hi23, 0x5410), d[3] = __byte_perm(hi01, hi23, 0x7632);
-            // MMA 0: planes 3 and 2 in rows g and g + 8; MMA 1: planes 1 and 0
-            const int c = 2 * (s & 1);
-            qa[s / 2][c] = d[3], qa[s / 2][c + 1] = d[2], qa[s / 2][4 + c] = d[1], qa[s / 2][4 + c + 1] = d[0];
-          } else {
-            qa[s][hh] = f16x2(y[0], y[1]), qa[s][hh + 2] = f16x2(y[2], y[3]);
-          }
+          const int d0 = Q8 ? (D == 32 ? 8 * t + 4 * s : 16 * (t + 4 * (s / 4)) + 4 * (s % 4))
+                            : 8 * (t + 4 * (s / 2)) + 4 * (s % 2);
+          qw[hh][s] = tok >= 0 ? *(const uint2 *)(qr + d0) : make_uint2(0u, 0u);
         }
-      } else {
-#pragma unroll
-        for (int s = 0; s < D / 16; ++s) qa[s][hh] = w[s].x, qa[s][hh + 2] = w[s].y;
       }
-    }
-    if (NR == 8 && !PLANES) {
-#pragma unroll
-      for (int s = 0; s < D / 16; ++s) qa[s][1] = qa[s][3] = 0u;
-    }
-    float m_run[2] = {-INFINITY, -INFINITY}, l_part[2] = {0.f, 0.f};
-    float acc[ND][4];
-#pragma unroll
-    for (int j = 0; j < ND; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+    };
+    load_q(seg);  // before the keys and values queue up in front of it
+#pragma unroll 1
+    for (int s = 0; s < STAGES - 1; ++s) load_next();
 
-    const int seg_end = min(seg.end, x1);
-    for (int x = max(x0, seg.start) + warp; x < seg_end; x += kWarps) {
-      load_next();
-      cp_wait<STAGES - 1>();
-      __syncwarp();
-      const uint8_t *kt = sm.ring[warp][cslot];
-      cslot = cslot + 1 == STAGES ? 0 : cslot + 1;
-      const uint8_t *vt = kt + TILE * G::kRowBytes;
-      const float *ksc = (const float *)(vt + TILE * G::kRowBytes), *vsc = ksc + TILE;
-      const int left = seg.len - (x - seg.start) * TILE;  // keys from the tile's first to the segment's end
-
-      // ---- scores in log2 units: n-tile nt holds keys 8 nt .. 8 nt + 7 (this thread loads key 8 nt + g and gets rows g,
-      // g + 8 of keys 8 nt + 2t, 8 nt + 2t + 1)
-      float sc[NT][4];
-      float2 vs[NT];
+    int cslot = 0;
+    for (;;) {
+      // ---- the segment's query rows as MMA fragments
+      uint32_t qa[PLANES ? D / 32 : D / 16][PLANES ? 8 : 4];
+      float rowfac[2] = {p.scale_log2, p.scale_log2};  // and for int8 the power of two that q was divided by
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const int r = 8 * nt + g;
-        const uint8_t *row = kt + r * G::kRowBytes;
-        constexpr int NW = G::kRowBytes / 16;  // words of the row that this thread takes
-        uint32_t kw[NW];
-        if constexpr (Q8 && D == 32) {
-          const uint2 a = *(const uint2 *)(row + 8 * t);
-          kw[0] = a.x, kw[1] = a.y;
-        } else {
+      for (int hh = 0; hh < NR / 8; ++hh) {
+        const uint2(&w)[D / 16] = qw[hh];
+        uint32_t amax2 = 0u;  // the largest magnitudes of the even and odd elements, as bf16 bits (NaN above infinity)
 #pragma unroll
-          for (int c = 0; c < NW / 4; ++c) {
-            const uint4 a = *(const uint4 *)(row + (((t + 4 * c) ^ G::k_swz(r)) * 16));
-            kw[4 * c] = a.x, kw[4 * c + 1] = a.y, kw[4 * c + 2] = a.z, kw[4 * c + 3] = a.w;
-          }
-        }
-        float2 ks = make_float2(1.f, 1.f);
-        if (Q8) ks = *(const float2 *)(ksc + 8 * nt + 2 * t), vs[nt] = *(const float2 *)(vsc + 8 * nt + 2 * t);
-        if constexpr (PLANES) {
-          int hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
-#pragma unroll
-          for (int s = 0; s < D / 32; ++s) {
-            mma_i8(hi, qa[s], kw[2 * s], kw[2 * s + 1]);
-            mma_i8(lo, qa[s] + 4, kw[2 * s], kw[2 * s + 1]);
-          }
-          // |digit sums| <= 2^21, so both halves of the 32-bit digits' sum fit an int
-          sc[nt][0] = fmaf((float)(hi[0] * 256 + hi[2]), 65536.f, (float)(lo[0] * 256 + lo[2])) * (rowfac[0] * ks.x);
-          sc[nt][1] = fmaf((float)(hi[1] * 256 + hi[3]), 65536.f, (float)(lo[1] * 256 + lo[3])) * (rowfac[0] * ks.y);
-          sc[nt][2] = sc[nt][3] = 0.f;
-        } else {
-          sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+        for (int s = 0; s < D / 16; ++s)
+          if (Q8) amax2 = __vmaxu2(amax2, __vmaxu2(w[s].x & 0x7fff7fffu, w[s].y & 0x7fff7fffu));
+        if (Q8) {
+          amax2 = __vmaxu2(amax2, __shfl_xor_sync(0xffffffffu, amax2, 1));
+          amax2 = __vmaxu2(amax2, __shfl_xor_sync(0xffffffffu, amax2, 2));
+          const int amax = (int)max(amax2 & 0xffffu, amax2 >> 16);
+          // a largest magnitude in [2^e, 2^(e + 1)) becomes one in [2^B, 2^(B + 1)): as fixed point (B = 29) bf16's 8 bits stay exact for
+          // elements down to 2^-22 of the row's largest, in f16 (B = 14) down to 2^-28. (The exponent is kept where both
+          // factors are normal numbers.)
+          constexpr int B = PLANES ? 29 : 14;
+          const int e = min(max((amax >> 7) - 127, B - 126), 127);
+          const float up = __uint_as_float((uint32_t)(127 + B - e) << 23);
+          rowfac[hh] *= __uint_as_float((uint32_t)(127 - B + e) << 23);
+          if (amax >= 0x7f80) rowfac[hh] = NAN;  // an infinity or NaN in the row: its scores are NaN
 #pragma unroll
           for (int s = 0; s < D / 16; ++s) {
-            if (Q8) {
-              const uint32_t b = kw[s] ^ 0x80808080u;
-              mma<true>(sc[nt], qa[s], codes_f16(b, 0x4140), codes_f16(b, 0x4342));
+            const float y[4] = {bf16_lo(w[s].x) * up, bf16_hi(w[s].x) * up, bf16_lo(w[s].y) * up, bf16_hi(w[s].y) * up};
+            if constexpr (PLANES) {
+              // bytes of X + 0x80808080 are the digits plus 128; a 4 x 4 byte transpose makes words of one digit (d[0] the
+              // lowest) of the four dims
+              uint32_t Y[4], d[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) Y[i] = ((uint32_t)__float2int_rn(y[i]) + 0x80808080u) ^ 0x80808080u;
+              const uint32_t lo01 = __byte_perm(Y[0], Y[1], 0x5140), hi01 = __byte_perm(Y[0], Y[1], 0x7362);
+              const uint32_t lo23 = __byte_perm(Y[2], Y[3], 0x5140), hi23 = __byte_perm(Y[2], Y[3], 0x7362);
+              d[0] = __byte_perm(lo01, lo23, 0x5410), d[1] = __byte_perm(lo01, lo23, 0x7632);
+              d[2] = __byte_perm(hi01, hi23, 0x5410), d[3] = __byte_perm(hi01, hi23, 0x7632);
+              // MMA 0: planes 3 and 2 in rows g and g + 8; MMA 1: planes 1 and 0
+              const int c = 2 * (s & 1);
+              qa[s / 2][c] = d[3], qa[s / 2][c + 1] = d[2], qa[s / 2][4 + c] = d[1], qa[s / 2][4 + c + 1] = d[0];
             } else {
-              mma<false>(sc[nt], qa[s], kw[(2 * s) % NW], kw[(2 * s + 1) % NW]);
+              qa[s][hh] = f16x2(y[0], y[1]), qa[s][hh + 2] = f16x2(y[2], y[3]);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int s = 0; s < D / 16; ++s) qa[s][hh] = w[s].x, qa[s][hh + 2] = w[s].y;
+        }
+      }
+      if (NR == 8 && !PLANES) {
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s) qa[s][1] = qa[s][3] = 0u;
+      }
+      float m_run[2] = {-INFINITY, -INFINITY}, l_part[2] = {0.f, 0.f};
+      float acc[ND][4];
+#pragma unroll
+      for (int j = 0; j < ND; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+
+      const int seg_end = min(seg.end, x1);
+      for (int x = max(x0, seg.start) + warp; x < seg_end; x += kWarps) {
+        load_next();
+        cp_wait<STAGES - 1>();
+        __syncwarp();
+        const uint8_t *kt = sm.ring[warp][cslot];
+        cslot = cslot + 1 == STAGES ? 0 : cslot + 1;
+        const uint8_t *vt = kt + TILE * G::kRowBytes;
+        const float *ksc = (const float *)(vt + TILE * G::kRowBytes), *vsc = ksc + TILE;
+        const int left = seg.len - (x - seg.start) * TILE;  // keys from the tile's first to the segment's end
+
+        // ---- scores in log2 units: n-tile nt holds keys 8 nt .. 8 nt + 7 (this thread loads key 8 nt + g and gets rows g,
+        // g + 8 of keys 8 nt + 2t, 8 nt + 2t + 1)
+        float sc[NT][4];
+        float2 vs[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const int r = 8 * nt + g;
+          const uint8_t *row = kt + r * G::kRowBytes;
+          constexpr int NW = G::kRowBytes / 16;  // words of the row that this thread takes
+          uint32_t kw[NW];
+          if constexpr (Q8 && D == 32) {
+            const uint2 a = *(const uint2 *)(row + 8 * t);
+            kw[0] = a.x, kw[1] = a.y;
+          } else {
+#pragma unroll
+            for (int c = 0; c < NW / 4; ++c) {
+              const uint4 a = *(const uint4 *)(row + (((t + 4 * c) ^ G::k_swz(r)) * 16));
+              kw[4 * c] = a.x, kw[4 * c + 1] = a.y, kw[4 * c + 2] = a.z, kw[4 * c + 3] = a.w;
+            }
+          }
+          float2 ks = make_float2(1.f, 1.f);
+          if (Q8) ks = *(const float2 *)(ksc + 8 * nt + 2 * t), vs[nt] = *(const float2 *)(vsc + 8 * nt + 2 * t);
+          if constexpr (PLANES) {
+            int hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int s = 0; s < D / 32; ++s) {
+              mma_i8(hi, qa[s], kw[2 * s], kw[2 * s + 1]);
+              mma_i8(lo, qa[s] + 4, kw[2 * s], kw[2 * s + 1]);
+            }
+            // |digit sums| <= 2^21, so both halves of the 32-bit digits' sum fit an int
+            sc[nt][0] = fmaf((float)(hi[0] * 256 + hi[2]), 65536.f, (float)(lo[0] * 256 + lo[2])) * (rowfac[0] * ks.x);
+            sc[nt][1] = fmaf((float)(hi[1] * 256 + hi[3]), 65536.f, (float)(lo[1] * 256 + lo[3])) * (rowfac[0] * ks.y);
+            sc[nt][2] = sc[nt][3] = 0.f;
+          } else {
+            sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+#pragma unroll
+            for (int s = 0; s < D / 16; ++s) {
+              if (Q8) {
+                const uint32_t b = kw[s] ^ 0x80808080u;
+                mma<true>(sc[nt], qa[s], codes_f16(b, 0x4140), codes_f16(b, 0x4342));
+              } else {
+                mma<false>(sc[nt], qa[s], kw[(2 * s) % NW], kw[(2 * s + 1) % NW]);
+              }
+            }
+#pragma unroll
+            for (int hh = 0; hh < NR / 8; ++hh) sc[nt][2 * hh] *= rowfac[hh] * ks.x, sc[nt][2 * hh + 1] *= rowfac[hh] * ks.y;
+          }
+        }
+        if (left < TILE) {  // the segment's last tile
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const int key = 8 * nt + 2 * t;
+            if (key >= left) sc[nt][0] = sc[nt][2] = -INFINITY;
+            if (key + 1 >= left) sc[nt][1] = sc[nt][3] = -INFINITY;
+          }
+        }
+        float ms[2], alpha[2] = {1.f, 1.f};
+#pragma unroll
+        for (int hh = 0; hh < NR / 8; ++hh) {
+          float mx = -INFINITY;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mx = fmaxf(mx, fmaxf(sc[nt][2 * hh], sc[nt][2 * hh + 1]));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+          const float m_new = fmaxf(m_run[hh], mx);
+          ms[hh] = m_new == -INFINITY ? 0.f : m_new;
+          alpha[hh] = ex2(m_run[hh] - ms[hh]);
+          m_run[hh] = m_new;
+          l_part[hh] *= alpha[hh];
+        }
+        // weights as sums of two bf16 values: pa the first (NR 8: the second in rows 8 .. 15), pb the second (NR 16)
+        uint32_t pa[NT / 2][4], pb[NR == 16 ? NT / 2 : 1][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+          for (int hh = 0; hh < NR / 8; ++hh) {
+            float p0 = ex2(sc[nt][2 * hh] - ms[hh]), p1 = ex2(sc[nt][2 * hh + 1] - ms[hh]);
+            l_part[hh] += p0 + p1;
+            if (Q8) p0 *= vs[nt].x, p1 *= vs[nt].y;  // (past the segment's end both are zeros)
+            const uint32_t hi = bf16x2(p0, p1), lo = bf16x2(p0 - bf16_lo(hi), p1 - bf16_hi(hi));
+            pa[nt / 2][2 * (nt % 2) + hh] = hi;
+            if (NR == 16) pb[nt / 2][2 * (nt % 2) + hh] = lo;
+            else pa[nt / 2][2 * (nt % 2) + 1] = lo;
+          }
+        }
+        if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+#pragma unroll
+          for (int j = 0; j < ND; ++j)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) acc[j][c] *= alpha[NR == 16 ? c / 2 : 0];
+        }
+        // ---- P.V: step u takes keys 16 u .. 16 u + 15; this thread's pairs are keys 2t, 2t + 1 and 2t + 8, 2t + 9 of them
+#pragma unroll
+        for (int u = 0; u < NT / 2; ++u) {
+          constexpr int NW = G::kRowBytes / 32;  // words of a row that this thread takes
+          uint32_t vw[4][NW];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r = 16 * u + 2 * t + (i & 1) + 8 * (i >> 1);
+            const uint8_t *row = vt + r * G::kRowBytes;
+            if constexpr (NW == 1) {
+              vw[i][0] = *(const uint32_t *)(row + 4 * g);
+            } else if constexpr (NW == 2) {
+              const uint2 a = *(const uint2 *)(row + (((g >> 1) ^ G::v_swz(r)) * 16) + 8 * (g & 1));
+              vw[i][0] = a.x, vw[i][1] = a.y;
+            } else {
+#pragma unroll
+              for (int c = 0; c < NW / 4; ++c) {
+                const uint4 a = *(const uint4 *)(row + (((g + 8 * c) ^ G::v_swz(r)) * 16));
+                vw[i][4 * c] = a.x, vw[i][4 * c + 1] = a.y, vw[i][4 * c + 2] = a.z, vw[i][4 * c + 3] = a.w;
+              }
             }
           }
 #pragma unroll
-          for (int hh = 0; hh < NR / 8; ++hh) sc[nt][2 * hh] *= rowfac[hh] * ks.x, sc[nt][2 * hh + 1] *= rowfac[hh] * ks.y;
-        }
-      }
-      if (left < TILE) {  // the segment's last tile
+          for (int w = 0; w < NW; ++w) {
+            if (Q8) {  // four dims of two key pairs: interleave the pair's bytes, then widen two at a time
+              const uint32_t pair[2][2] = {{__byte_perm(vw[0][w], vw[1][w], 0x5140), __byte_perm(vw[0][w], vw[1][w], 0x7362)},
+                                           {__byte_perm(vw[2][w], vw[3][w], 0x5140), __byte_perm(vw[2][w], vw[3][w], 0x7362)}};
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          const int key = 8 * nt + 2 * t;
-          if (key >= left) sc[nt][0] = sc[nt][2] = -INFINITY;
-          if (key + 1 >= left) sc[nt][1] = sc[nt][3] = -INFINITY;
+              for (int e = 0; e < 4; ++e) {
+                const uint32_t select = e & 1 ? 0x4342 : 0x4140;
+                const uint32_t b0 = codes_bf16(pair[0][e / 2], select), b1 = codes_bf16(pair[1][e / 2], select);
+                mma<false>(acc[4 * w + e], pa[u], b0, b1);
+                if (NR == 16) mma<false>(acc[4 * w + e], pb[u % (NR == 16 ? NT / 2 : 1)], b0, b1);
+              }
+            } else {
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const uint32_t select = e ? 0x7632 : 0x5410;
+                const uint32_t b0 = __byte_perm(vw[0][w], vw[1][w], select), b1 = __byte_perm(vw[2][w], vw[3][w], select);
+                mma<false>(acc[(2 * w + e) % ND], pa[u], b0, b1);
+                if (NR == 16) mma<false>(acc[(2 * w + e) % ND], pb[u % (NR == 16 ? NT / 2 : 1)], b0, b1);
+              }
+            }
+          }
         }
+        __syncwarp();  // the stage is read before the load that reuses it
       }
-      float ms[2], alpha[2] = {1.f, 1.f};
+
+      if (NR == 8) {  // the two parts of the weights
+#pragma unroll
+        for (int j = 0; j < ND; ++j) acc[j][0] += acc[j][2], acc[j][1] += acc[j][3];
+      }
+      // ---- the segment is done: the warps' states, each relative to the largest maximum, are added up in shared memory
+#pragma unroll
+      for (int hh = 0; hh < NR / 8; ++hh) {
+        l_part[hh] += __shfl_xor_sync(0xffffffffu, l_part[hh], 1);
+        l_part[hh] += __shfl_xor_sync(0xffffffffu, l_part[hh], 2);
+        if (t == 0) sm.warp_m[warp][g + 8 * hh] = m_run[hh], sm.warp_l[warp][g + 8 * hh] = l_part[hh];
+      }
+      __syncthreads();
+      float fac[NR / 8];
 #pragma unroll
       for (int hh = 0; hh < NR / 8; ++hh) {
         float mx = -INFINITY;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) mx = fmaxf(mx, fmaxf(sc[nt][2 * hh], sc[nt][2 * hh + 1]));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float m_new = fmaxf(m_run[hh], mx);
-        ms[hh] = m_new == -INFINITY ? 0.f : m_new;
-        alpha[hh] = ex2(m_run[hh] - ms[hh]);
-        m_run[hh] = m_new;
-        l_part[hh] *= alpha[hh];
+        for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, sm.warp_m[w][g + 8 * hh]);
+        fac[hh] = ex2(m_run[hh] - (mx == -INFINITY ? 0.f : mx));
       }
-      // weights as sums of two bf16 values: pa the first (NR 8: the second in rows 8 .. 15), pb the second (NR 16)
-      uint32_t pa[NT / 2][4], pb[NR == 16 ? NT / 2 : 1][4];
+      if (threadIdx.x < NR) {
+        float mx = -INFINITY, l = 0.f;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
+        for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, sm.warp_m[w][threadIdx.x]);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w)
+          l += sm.warp_l[w][threadIdx.x] * ex2(sm.warp_m[w][threadIdx.x] - (mx == -INFINITY ? 0.f : mx));
+        sm.row_m[threadIdx.x] = mx, sm.row_l[threadIdx.x] = l;
+      }
+      const bool whole = seg.start >= x0 && seg.end <= x1;
+      const bool final = MODE == kOwn && whole;
+      const int rows = PREFIX ? kRows : p.group;
+      float *rec = record<D>(p, (int)blockIdx.x + seg.index);
+      constexpr int kPass = S::kPass;
+#pragma unroll 1
+      for (int r0 = 0; r0 < rows; r0 += kPass) {
+        if (r0) __syncthreads();  // the last pass has been read
 #pragma unroll
         for (int hh = 0; hh < NR / 8; ++hh) {
-          float p0 = ex2(sc[nt][2 * hh] - ms[hh]), p1 = ex2(sc[nt][2 * hh + 1] - ms[hh]);
-          l_part[hh] += p0 + p1;
-          if (Q8) p0 *= vs[nt].x, p1 *= vs[nt].y;  // (past the segment's end both are zeros)
-          const uint32_t hi = bf16x2(p0, p1), lo = bf16x2(p0 - bf16_lo(hi), p1 - bf16_hi(hi));
-          pa[nt / 2][2 * (nt % 2) + hh] = hi;
-          if (NR == 16) pb[nt / 2][2 * (nt % 2) + hh] = lo;
-          else pa[nt / 2][2 * (nt % 2) + 1] = lo;
-        }
-      }
-      if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+          const int r = g + 8 * hh - r0;
+          if (r >= 0 && r < kPass && r + r0 < rows) {
 #pragma unroll
-        for (int j = 0; j < ND; ++j)
+            for (int j = 0; j < ND; j += 4)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) acc[j][c] *= alpha[NR == 16 ? c / 2 : 0];
-      }
-      // ---- P.V: step u takes keys 16 u .. 16 u + 15; this thread's pairs are keys 2t, 2t + 1 and 2t + 8, 2t + 9 of them
-#pragma unroll
-      for (int u = 0; u < NT / 2; ++u) {
-        constexpr int NW = G::kRowBytes / 32;  // words of a row that this thread takes
-        uint32_t vw[4][NW];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = 16 * u + 2 * t + (i & 1) + 8 * (i >> 1);
-          const uint8_t *row = vt + r * G::kRowBytes;
-          if constexpr (NW == 1) {
-            vw[i][0] = *(const uint32_t *)(row + 4 * g);
-          } else if constexpr (NW == 2) {
-            const uint2 a = *(const uint2 *)(row + (((g >> 1) ^ G::v_swz(r)) * 16) + 8 * (g & 1));
-            vw[i][0] = a.x, vw[i][1] = a.y;
-          } else {
-#pragma unroll
-            for (int c = 0; c < NW / 4; ++c) {
-              const uint4 a = *(const uint4 *)(row + (((g + 8 * c) ^ G::v_swz(r)) * 16));
-              vw[i][4 * c] = a.x, vw[i][4 * c + 1] = a.y, vw[i][4 * c + 2] = a.z, vw[i][4 * c + 3] = a.w;
-            }
+              for (int e = 0; e < 2; ++e) {
+                const int c = 2 * hh + e;
+                *(float4 *)&sm.merge[warp][r][G::out_dim(j, e, t)] =
+                    make_float4(acc[j][c] * fac[hh], acc[j + 1][c] * fac[hh], acc[j + 2][c] * fac[hh], acc[j + 3][c] * fac[hh]);
+              }
           }
         }
+        __syncthreads();
+#pragma unroll 1
+        for (int e = threadIdx.x; e < min(kPass, rows - r0) * D; e += C::kThreads) {
+          float a = 0.f;
 #pragma unroll
-        for (int w = 0; w < NW; ++w) {
-          if (Q8) {  // four dims of two key pairs: interleave the pair's bytes, then widen two at a time
-            const uint32_t pair[2][2] = {{__byte_perm(vw[0][w], vw[1][w], 0x5140), __byte_perm(vw[0][w], vw[1][w], 0x7362)},
-                                         {__byte_perm(vw[2][w], vw[3][w], 0x5140), __byte_perm(vw[2][w], vw[3][w], 0x7362)}};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint32_t select = e & 1 ? 0x4342 : 0x4140;
-              const uint32_t b0 = codes_bf16(pair[0][e / 2], select), b1 = codes_bf16(pair[1][e / 2], select);
-              mma<false>(acc[4 * w + e], pa[u], b0, b1);
-              if (NR == 16) mma<false>(acc[4 * w + e], pb[u % (NR == 16 ? NT / 2 : 1)], b0, b1);
-            }
-          } else {
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const uint32_t select = e ? 0x7632 : 0x5410;
-              const uint32_t b0 = __byte_perm(vw[0][w], vw[1][w], select), b1 = __byte_perm(vw[2][w], vw[3][w], select);
-              mma<false>(acc[(2 * w + e) % ND], pa[u], b0, b1);
-              if (NR == 16) mma<false>(acc[(2 * w + e) % ND], pb[u % (NR == 16 ? NT / 2 : 1)], b0, b1);
-            }
-          }
+          for (int w = 0; w < kWarps; ++w) a += sm.merge[w][e / D][e % D];
+          if (final) p.out[seg.seq * p.ldo + (int64_t)(seg.g * p.group + r0) * D + e] = f32_to_bf16_bits(a / sm.row_l[r0 + e / D]);
+          else rec[r0 * D + e] = a;
         }
       }
-      __syncwarp();  // the stage is read before the load that reuses it
-    }
-
-    if (NR == 8) {  // the two parts of the weights
-#pragma unroll
-      for (int j = 0; j < ND; ++j) acc[j][0] += acc[j][2], acc[j][1] += acc[j][3];
-    }
-    // ---- the segment is done: the warps' states, each relative to the largest maximum, are added up in shared memory
-#pragma unroll
-    for (int hh = 0; hh < NR / 8; ++hh) {
-      l_part[hh] += __shfl_xor_sync(0xffffffffu, l_part[hh], 1);
-      l_part[hh] += __shfl_xor_sync(0xffffffffu, l_part[hh], 2);
-      if (t == 0) sm.warp_m[warp][g + 8 * hh] = m_run[hh], sm.warp_l[warp][g + 8 * hh] = l_part[hh];
-    }
-    __syncthreads();
-    float fac[NR / 8];
-#pragma unroll
-    for (int hh = 0; hh < NR / 8; ++hh) {
-      float mx = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, sm.warp_m[w][g + 8 * hh]);
-      fac[hh] = ex2(m_run[hh] - (mx == -INFINITY ? 0.f : mx));
-    }
-    if (threadIdx.x < NR) {
-      float mx = -INFINITY, l = 0.f;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, sm.warp_m[w][threadIdx.x]);
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w)
-        l += sm.warp_l[w][threadIdx.x] * ex2(sm.warp_m[w][threadIdx.x] - (mx == -INFINITY ? 0.f : mx));
-      sm.row_m[threadIdx.x] = mx, sm.row_l[threadIdx.x] = l;
-    }
-    const bool whole = seg.start >= x0 && seg.end <= x1;
-    const bool final = MODE == kOwn && whole;
-    const int rows = PREFIX ? kRows : p.group;
-    float *rec = record<D>(p, (int)blockIdx.x + seg.index);
-    constexpr int kPass = S::kPass;
-#pragma unroll 1
-    for (int r0 = 0; r0 < rows; r0 += kPass) {
-      if (r0) __syncthreads();  // the last pass has been read
-#pragma unroll
-      for (int hh = 0; hh < NR / 8; ++hh) {
-        const int r = g + 8 * hh - r0;
-        if (r >= 0 && r < kPass && r + r0 < rows) {
-#pragma unroll
-          for (int j = 0; j < ND; j += 4)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int c = 2 * hh + e;
-              *(float4 *)&sm.merge[warp][r][G::out_dim(j, e, t)] =
-                  make_float4(acc[j][c] * fac[hh], acc[j + 1][c] * fac[hh], acc[j + 2][c] * fac[hh], acc[j + 3][c] * fac[hh]);
-            }
+      if (!final && threadIdx.x < rows) {
+        rec[kRows * D + threadIdx.x] = sm.row_m[threadIdx.x];
+        rec[kRows * D + kRows + threadIdx.x] = sm.row_l[threadIdx.x];
+      }
+      if (MODE != kPrefix && !final) {
+        const int c0 = seg.start / lay.chunk, c1 = (seg.end - 1) / lay.chunk;
+        if (MODE == kOwn) {
+          (split_n ? split[1] : split[0]) = make_int2(seg.index, c0);
+          ++split_n;
+        } else if (seg.start >= x0 && threadIdx.x == 0) {  // (a short segment lies in one CTA wherever the even cuts are)
+          p.parts[seg.index] = make_int2(whole ? (int)blockIdx.x + seg.index : c0 + seg.index, whole ? 1 : c1 - c0 + 1);
         }
       }
-      __syncthreads();
-#pragma unroll 1
-      for (int e = threadIdx.x; e < min(kPass, rows - r0) * D; e += C::kThreads) {
-        float a = 0.f;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) a += sm.merge[w][e / D][e % D];
-        if (final) p.out[seg.seq * p.ldo + (int64_t)(seg.g * p.group + r0) * D + e] = f32_to_bf16_bits(a / sm.row_l[r0 + e / D]);
-        else rec[r0 * D + e] = a;
-      }
+      if (seg.next >= x1) break;
+      seg = next_seg<TILE, PREFIX>(p, sm.cum, sm.len, seg);
+      load_q(seg);
     }
-    if (!final && threadIdx.x < rows) {
-      rec[kRows * D + threadIdx.x] = sm.row_m[threadIdx.x];
-      rec[kRows * D + kRows + threadIdx.x] = sm.row_l[threadIdx.x];
-    }
-    if (MODE != kPrefix && !final) {
-      const int c0 = seg.start / lay.chunk, c1 = (seg.end - 1) / lay.chunk;
-      if (MODE == kOwn) {
-        (split_n ? split[1] : split[0]) = make_int2(seg.index, c0);
-        ++split_n;
-      } else if (seg.start >= x0 && threadIdx.x == 0) {  // (a short segment lies in one CTA wherever the even cuts are)
-        p.parts[seg.index] = make_int2(whole ? (int)blockIdx.x + seg.index : c0 + seg.index, whole ? 1 : c1 - c0 + 1);
-      }
-    }
-    if (seg.next >= x1) break;
-    seg = next_seg<TILE, PREFIX>(p, sm.cum, sm.len, seg);
-    load_q(seg);
-  }
-  cp_wait<0>();
+    cp_wait<0>();
   }
   if (MODE == kBeside) {
     for (int e = blockIdx.x * C::kThreads + threadIdx.x; e < p.m * p.nkv; e += gridDim.x * C::kThreads)
       if (sm.len[e / p.nkv] == 0) p.parts[e] = make_int2(0, 0);
     pdl_wait();  // the prefix's launch: what waits for this one has waited for both
   }
-  if (MODE != kOwn) return;
-  for (int e = blockIdx.x; e < p.m * p.nkv; e += gridDim.x)  // sequences without keys
-    if (sm.len[e / p.nkv] == 0)
-      for (int c = threadIdx.x; c < p.group * D; c += C::kThreads)
-        p.out[(e / p.nkv) * p.ldo + (int64_t)(e % p.nkv) * p.group * D + c] = 0;
-  if (!split_n) return;
-  __threadfence();
-  __syncthreads();
-  if ((int)threadIdx.x < split_n) {
-    const int2 e = threadIdx.x ? split[1] : split[0];
-    const Seg sg = own_seg<TILE>(p, sm.cum, sm.len, e.x / p.nkv, e.x % p.nkv);
-    const int n = (sg.end - 1) / lay.chunk - e.y + 1;
-    const bool last = atomicAdd(p.cnt + e.x, 1u) == (unsigned)(n - 1);
-    if (last) {
-      p.cnt[e.x] = 0u;
-      __threadfence();
-    }
-    sm.last[threadIdx.x] = last ? n : 0;
-  }
-  __syncthreads();
-#pragma unroll 1
-  for (int s = 0; s < split_n; ++s) {
-    const int n = sm.last[s];
-    if (!n) continue;
-    // a warp takes a row, or with fewer rows than warps every parts-th record of one
-    const int2 e = s ? split[1] : split[0];
-    const int parts = p.group < kWarps ? kWarps / p.group : 1, part = parts > 1 ? warp / p.group : 0;
-    uint16_t *out = p.out + (e.x / p.nkv) * p.ldo + (int64_t)(e.x % p.nkv) * p.group * D;
-    const float *rec = record<D>(p, e.y + e.x);
-#pragma unroll 1
-    for (int j = warp - part * p.group; j < p.group && part < parts; j += kWarps) {
-      float a[D / 32];
-      add_records<D, false, 8>(rec + j * D, n, j, nullptr, 0, 0, 0, 0, part, parts, a);
-      if (parts == 1) {
-        store_row(out + j * D + D / 32 * lane, a);
-      } else {
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) sm.fin[warp][D / 32 * lane + i] = a[i];
-      }
-    }
-    if (parts == 1) continue;
+  if constexpr (MODE == kOwn) {
+    for (int e = blockIdx.x; e < p.m * p.nkv; e += gridDim.x)  // sequences without keys
+      if (sm.len[e / p.nkv] == 0)
+        for (int c = threadIdx.x; c < p.group * D; c += C::kThreads)
+          p.out[(e / p.nkv) * p.ldo + (int64_t)(e % p.nkv) * p.group * D + c] = 0;
+    if (!split_n) return;
+    __threadfence();
     __syncthreads();
-    for (int i = threadIdx.x; i < p.group * D; i += C::kThreads) {
-      float v = 0.f;
-      for (int q = 0; q < parts; ++q) v += sm.fin[q * p.group + i / D][i % D];
-      out[i] = f32_to_bf16_bits(v);
+    if ((int)threadIdx.x < split_n) {
+      const int2 e = threadIdx.x ? split[1] : split[0];
+      const Seg sg = own_seg<TILE>(p, sm.cum, sm.len, e.x / p.nkv, e.x % p.nkv);
+      const int n = (sg.end - 1) / lay.chunk - e.y + 1;
+      const bool last = atomicAdd(p.cnt + e.x, 1u) == (unsigned)(n - 1);
+      if (last) {
+        p.cnt[e.x] = 0u;
+        __threadfence();
+      }
+      sm.last[threadIdx.x] = last ? n : 0;
     }
-    __syncthreads();  // sm.fin is free again
+    __syncthreads();
+#pragma unroll 1
+    for (int s = 0; s < split_n; ++s) {
+      const int n = sm.last[s];
+      if (!n) continue;
+      // a warp takes a row, or with fewer rows than warps every parts-th record of one
+      const int2 e = s ? split[1] : split[0];
+      const int parts = p.group < kWarps ? kWarps / p.group : 1, part = parts > 1 ? warp / p.group : 0;
+      uint16_t *out = p.out + (e.x / p.nkv) * p.ldo + (int64_t)(e.x % p.nkv) * p.group * D;
+      const float *rec = record<D>(p, e.y + e.x);
+#pragma unroll 1
+      for (int j = warp - part * p.group; j < p.group && part < parts; j += kWarps) {
+        float a[D / 32];
+        add_records<D, false, 8>(rec + j * D, n, j, nullptr, 0, 0, 0, 0, part, parts, a);
+        if (parts == 1) {
+          store_row(out + j * D + D / 32 * lane, a);
+        } else {
+#pragma unroll
+          for (int i = 0; i < D / 32; ++i) sm.fin[warp][D / 32 * lane + i] = a[i];
+        }
+      }
+      if (parts == 1) continue;
+      __syncthreads();
+      for (int i = threadIdx.x; i < p.group * D; i += C::kThreads) {
+        float v = 0.f;
+        for (int q = 0; q < parts; ++q) v += sm.fin[q * p.group + i / D][i % D];
+        out[i] = f32_to_bf16_bits(v);
+      }
+      __syncthreads();  // sm.fin is free again
+    }
   }
 }
 

@@ -22,6 +22,7 @@ struct AppendParams {
   const int64_t *position;
   int64_t m;
   int nkv, d, ragged;
+  int plain;  // bf16 caches without scales: the rows as they are
   // prologue of a decode step (q non-null): q/k RMSNorm and RoPE as the bf16 append does them
   uint16_t *q_out;
   const uint16_t *q;
@@ -174,12 +175,18 @@ __global__ void __launch_bounds__(kThreads) norm_rope_append_kernel(AppendParams
     for (int i = 0; i < N; ++i) p.q_out[row * p.ldqo + (int64_t)head * D + lane + 32 * i] = f32_to_bf16_bits(x[i]);
     return;
   }
+  const int64_t dst = (head0 + head) * p.cap + slot;
+  if (p.plain) {
+    uint16_t *rows = (uint16_t *)(kind == 1 ? p.k_cache : p.v_cache) + dst * D;
+#pragma unroll
+    for (int i = 0; i < N; ++i) rows[lane + 32 * i] = f32_to_bf16_bits(x[i]);
+    return;
+  }
   float amax = 0.f;
 #pragma unroll
   for (int i = 0; i < N; ++i) amax = fmaxf(amax, fabsf(x[i]));
   amax = warp_max(amax);
   const float s = row_scale(amax);
-  const int64_t dst = (head0 + head) * p.cap + slot;
   int8_t *codes = (kind == 1 ? p.k_cache : p.v_cache) + dst * D;
 #pragma unroll
   for (int i = 0; i < N; ++i) codes[lane + 32 * i] = (int8_t)code_of(x[i], s);
@@ -270,8 +277,9 @@ extern "C" int egpt_kv_append_q8(int8_t *k_cache, float *k_scale, int8_t *v_cach
                                  const void *rope_cos, const void *rope_sin, int64_t rope_base, unsigned flags,
                                  void *stream) {
   clear_error();
-  if (!k_cache || !k_scale || !v_cache || !v_scale || !k || !v || !position)
+  if (!k_cache || !v_cache || !k || !v || !position || (k_scale == nullptr) != (v_scale == nullptr))
     return set_error(EGPT_ERR_ARG, "kv_append_q8: null pointer");
+  if (!k_scale && !q) return set_error(EGPT_ERR_ARG, "kv_append_q8: rows for a bf16 cache (no scales) come with q");
   if (d != 32 && d != 64 && d != 128) return set_error(EGPT_ERR_SHAPE, "kv_append_q8: head_dim must be 32, 64 or 128");
   if (m < 1 || nkv < 1 || cap < 1 || ldk < (int64_t)nkv * d || ldv < (int64_t)nkv * d || m > ((int64_t)1 << 31) / nkv)
     return set_error(EGPT_ERR_SHAPE, "kv_append_q8: bad m, heads, cap or leading dimension");
@@ -283,7 +291,7 @@ extern "C" int egpt_kv_append_q8(int8_t *k_cache, float *k_scale, int8_t *v_cach
   kvq::AppendParams p{};
   p.k_cache = k_cache, p.v_cache = v_cache, p.k_scale = k_scale, p.v_scale = v_scale, p.cap = cap;
   p.k = k, p.v = v, p.ldk = ldk, p.ldv = ldv, p.position = position, p.m = m, p.nkv = nkv, p.d = d;
-  p.ragged = (flags & EGPT_FLAG_RAGGED) != 0;
+  p.ragged = (flags & EGPT_FLAG_RAGGED) != 0, p.plain = !k_scale;
   if (q) {
     if (!q_out) return set_error(EGPT_ERR_ARG, "kv_append_q8: q without q_out");
     if (f32) return set_error(EGPT_ERR_DTYPE, "kv_append_q8: fp32 rows have no norm/RoPE");

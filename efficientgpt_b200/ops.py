@@ -306,8 +306,27 @@ def kv_append_q8(k, v, k_cache, k_scale, v_cache, v_scale, position, *, ragged=F
     *position + i of caches [nkv, cap, d], or (ragged) to slot position[i] of its own heads of caches [M * nkv, cap,
     d] (-1: an idle slot, nothing is written). With q [M, nq * d] the q/k RMSNorm and RoPE of a decode step come first
     (the angle of position rope_base + slot) and the rotated q is returned."""
-    _cuda(k, v, k_cache, k_scale, v_cache, v_scale, position)
-    heads, cap, d = _cache_q8('kv_append_q8', k_cache, k_scale, v_cache, v_scale)
+    _cuda(k_cache, k_scale, v_cache, v_scale)
+    shape = _cache_q8('kv_append_q8', k_cache, k_scale, v_cache, v_scale)
+    return _append(k, v, shape, (k_cache.data_ptr(), k_scale.data_ptr(), v_cache.data_ptr(), v_scale.data_ptr()),
+                   position, ragged, q, q_norm_w, k_norm_w, eps, rope_cos, rope_sin, rope_base, q_out)
+
+
+def kv_append(k, v, cache, position, *, q, ragged=False, q_norm_w=None, k_norm_w=None, eps=1e-6, rope_cos=None,
+              rope_sin=None, rope_base=0, q_out=None):
+    """kv_append_q8 with q, for either kind of cache: (k, k_scale, v, v_scale) in int8 or (k, v) in bf16, which gets the
+    rows as they are."""
+    if len(cache) == 4:
+        return kv_append_q8(k, v, *cache, position, ragged=ragged, q=q, q_norm_w=q_norm_w, k_norm_w=k_norm_w, eps=eps,
+                            rope_cos=rope_cos, rope_sin=rope_sin, rope_base=rope_base, q_out=q_out)
+    heads, cap, _, ptrs = _cache_pair('kv_append', cache, cache[0].shape[-1])
+    return _append(k, v, (heads, cap, cache[0].shape[-1]), ptrs, position, ragged, q, q_norm_w, k_norm_w, eps, rope_cos,
+                   rope_sin, rope_base, q_out)
+
+
+def _append(k, v, shape, ptrs, position, ragged, q, q_norm_w, k_norm_w, eps, rope_cos, rope_sin, rope_base, q_out):
+    heads, cap, d = shape
+    _cuda(k, v, position)
     if k.dim() != 2 or k.stride(1) != 1 or v.stride(-1) != 1:
         raise ValueError('kv_append_q8: k and v must be 2-D tensors with unit column stride')
     m, width = k.shape
@@ -335,9 +354,9 @@ def kv_append_q8(k, v, k_cache, k_scale, v_cache, v_scale, position, *, ragged=F
             raise ValueError('kv_append_q8: q_out must be bf16 rows of the shape of q')
         prologue = (q_out.data_ptr(), q_out.stride(0), q.data_ptr(), q.stride(0), q.shape[1] // d, _p(q_norm_w),
                     _p(k_norm_w), eps, _p(rope_cos), _p(rope_sin), rope_base)
-    rc = L.load().egpt_kv_append_q8(k_cache.data_ptr(), k_scale.data_ptr(), v_cache.data_ptr(), v_scale.data_ptr(), cap,
-                                    k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), position.data_ptr(), m, nkv,
-                                    d, _dt(k), *prologue, L.FLAG_RAGGED if ragged else 0, _raw_stream())
+    rc = L.load().egpt_kv_append_q8(*ptrs, cap, k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0),
+                                    position.data_ptr(), m, nkv, d, _dt(k), *prologue,
+                                    L.FLAG_RAGGED if ragged else 0, _raw_stream())
     if rc:
         L.check(rc, 'kv_append_q8')
     return q_out

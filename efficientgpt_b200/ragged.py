@@ -17,6 +17,11 @@ sequences (egpt_attn_decode with
 EGPT_FLAG_RAGGED | EGPT_FLAG_APPEND: row b's q/k RMSNorm, RoPE at position[b] and K/V append into its own cache
 heads, then its own causal range); the final norm, the lm_head projection over the B rows and a row-wise argmax.
 Prompts are prefilled row by row on the same kernels in 16-row blocks.
+
+kv_dtype=torch.int8 keeps the caches as int8 codes with one scale per row and head (half the bytes per key): a step
+then writes its rows with kv_append_q8 and attends with attn_decode_q8, and a prompt attends to its rows as the cache
+holds them (kv_read_q8), so what a sequence was prefilled with is what it decodes against. RaggedGraphDecoder takes it
+too.
 """
 import torch
 
@@ -46,13 +51,16 @@ def check_ragged(prompts, lengths, count, capacity):
 class RaggedEngine:
     """B sequences with per-row positions on the Qwen3 int8 kernels (weights fused once by Qwen3Engine)."""
 
-    def __init__(self, model, batch, capacity, attn_max_split=8):
+    def __init__(self, model, batch, capacity, attn_max_split=8, kv_dtype=torch.bfloat16, rope_rows=None):
         if not 1 <= batch <= MAX_ROWS:
             raise ValueError(f'batch must be in [1, {MAX_ROWS}]')
-        self.base = Qwen3Engine(model, capacity, step='sequence')
+        if kv_dtype not in (torch.bfloat16, torch.int8):
+            raise ValueError('kv_dtype must be torch.bfloat16 or torch.int8')
+        self.base = Qwen3Engine(model, rope_rows or capacity, step='sequence')
         b = self.base
         self.batch, self.cap, self.device = batch, capacity, b.device
-        self.kv = torch.zeros(b.n_layers, 2, batch * b.nkv, capacity, b.d, dtype=torch.bfloat16, device=b.device)
+        self.q8 = kv_dtype is torch.int8
+        self._alloc_kv()
         self.tokens = torch.zeros(batch, dtype=torch.long, device=b.device)
         self.positions = torch.zeros(batch, dtype=torch.long, device=b.device)
         self.max_split = attn_max_split
@@ -84,16 +92,59 @@ class RaggedEngine:
             self.gemm_ws[(n, k)] = torch.empty(max(need, 16), dtype=torch.uint8, device=self.device)
         return self.gemm_ws[(n, k)]
 
+    def _alloc_kv(self):
+        b = self.base
+        if self.q8:  # per layer (k codes, k scales, v codes, v scales)
+            self.kv = [ops.kv_cache_q8(self.batch * b.nkv, self.cap, b.d, b.device) for _ in range(b.n_layers)]
+            self.q8_ws = ops.attn_q8_ws(self.batch, b.nq, b.nkv, b.d, b.device)
+        else:
+            self.kv = torch.zeros(b.n_layers, 2, self.batch * b.nkv, self.cap, b.d, dtype=torch.bfloat16,
+                                  device=b.device)
+
     def _row_kv(self, row):
         b = self.base
         return self.kv[:, :, row * b.nkv:(row + 1) * b.nkv]
+
+    def _prologue(self, lay):
+        b = self.base
+        return dict(q_norm_w=lay['q_norm'], k_norm_w=lay['k_norm'], eps=b.eps, rope_cos=b.rope_cos, rope_sin=b.rope_sin)
+
+    def _split(self, qkv):
+        """q, k and v columns of the fused projection's rows."""
+        b = self.base
+        return qkv.split((b.nq * b.d, b.nkv * b.d, b.nkv * b.d), dim=1)
+
+    def _attend_prompt(self, row, i, lay, qkv, pos0, ws):
+        """Layer i's attention of a prompt's rows, their keys and values written to row `row`'s cache."""
+        b = self.base
+        if not self.q8:
+            kv = self._row_kv(row)[i]
+            q = ops.qk_norm_rope_kv_append(qkv, kv[0], kv[1], pos0, b.nq, b.nkv, b.d, **self._prologue(lay))
+            k, v = kv[0], kv[1]
+        else:
+            cache = [t[row * b.nkv:(row + 1) * b.nkv] for t in self.kv[i]]
+            q, k, v = self._split(qkv)
+            q = ops.kv_append_q8(k, v, *cache, pos0, q=q, **self._prologue(lay))
+            k, v = ops.kv_read_q8(*cache, 0, qkv.shape[0])
+        return ops.attn_decode(q, k, v, pos0, b.nq, b.nkv, b.d, scale=b.scale, max_split=self.max_split, ws=ws,
+                               ref_softmax=True)
+
+    def _attend_step(self, i, lay, qkv):
+        """Layer i's attention of one step, every row's key and value appended to its cache."""
+        b = self.base
+        if not self.q8:
+            return ops.attn_decode(qkv, self.kv[i, 0], self.kv[i, 1], self.positions, b.nq, b.nkv, b.d, scale=b.scale,
+                                   max_split=self.max_split, ws=self.attn_ws, append=True, ragged=True,
+                                   ref_softmax=True, **self._prologue(lay))
+        q, k, v = self._split(qkv)
+        q = ops.kv_append_q8(k, v, *self.kv[i], self.positions, ragged=True, q=q, **self._prologue(lay))
+        return ops.attn_decode_q8(q, *self.kv[i], self.positions, b.nq, b.nkv, b.d, scale=b.scale, ws=self.q8_ws)
 
     @torch.no_grad()
     def prefill_row(self, row, ids):
         """Prompt ids (int64 [p] on the device) of one row from position 0, on the 16-row-block kernels; leaves the
         row's first generated token and position p."""
         b = self.base
-        kv = self._row_kv(row)
         p = ids.numel()
         pos0 = torch.zeros(1, dtype=torch.long, device=self.device)
         h = ops.embed(ids, b.embed)
@@ -101,11 +152,7 @@ class RaggedEngine:
         for i, lay in enumerate(b.layers):
             x = ops.rmsnorm(h, lay['ln_in'], b.eps)
             qkv = b._linear(x, lay['w_qkv'], lay['s_qkv'])
-            q = ops.qk_norm_rope_kv_append(qkv, kv[i, 0], kv[i, 1], pos0, b.nq, b.nkv, b.d, q_norm_w=lay['q_norm'],
-                                           k_norm_w=lay['k_norm'], eps=b.eps, rope_cos=b.rope_cos,
-                                           rope_sin=b.rope_sin)
-            a = ops.attn_decode(q, kv[i, 0], kv[i, 1], pos0, b.nq, b.nkv, b.d, scale=b.scale,
-                                max_split=self.max_split, ws=ws, ref_softmax=True)
+            a = self._attend_prompt(row, i, lay, qkv, pos0, ws)
             h = b._linear(a, lay['w_o'], lay['s_o'], epilogue=L.EPI_RESIDUAL, residual=h)
             x = ops.rmsnorm(h, lay['ln_post'], b.eps)
             act = b._linear(x, lay['w_gu'], lay['s_gu'], epilogue=L.EPI_SILU_MUL)
@@ -115,6 +162,10 @@ class RaggedEngine:
         self.tokens[row:row + 1].copy_(ops.argmax_rows(logits))
         self.positions[row] = p
 
+    def prefill(self, prompts, lengths):
+        for r in range(self.batch):
+            self.prefill_row(r, prompts[r, :int(lengths[r])].to(self.device))
+
     @torch.no_grad()
     def step(self):
         """One token for every row: tokens <- argmax(model(tokens, positions)); positions += 1 (no host sync)."""
@@ -123,10 +174,7 @@ class RaggedEngine:
         for i, lay in enumerate(b.layers):
             x = ops.rmsnorm(h, lay['ln_in'], b.eps)
             qkv = self._proj(x, lay['w_qkv'], lay['s_qkv'])
-            a = ops.attn_decode(qkv, self.kv[i, 0], self.kv[i, 1], self.positions, b.nq, b.nkv, b.d, scale=b.scale,
-                                max_split=self.max_split, ws=self.attn_ws, append=True, ragged=True,
-                                q_norm_w=lay['q_norm'], k_norm_w=lay['k_norm'], eps=b.eps, rope_cos=b.rope_cos,
-                                rope_sin=b.rope_sin, ref_softmax=True)
+            a = self._attend_step(i, lay, qkv)
             h = self._proj(a, lay['w_o'], lay['s_o'], epilogue=L.EPI_RESIDUAL, residual=h)
             x = ops.rmsnorm(h, lay['ln_post'], b.eps)
             act = self._proj(x, lay['w_gu'], lay['s_gu'], epilogue=L.EPI_SILU_MUL)
@@ -145,8 +193,7 @@ class RaggedEngine:
         if prompts.shape[0] != self.batch:
             raise ValueError('prompts must have the engine batch size')
         out = torch.empty(self.batch, count, dtype=torch.long, device=self.device)
-        for r in range(self.batch):
-            self.prefill_row(r, prompts[r, :int(lengths[r])].to(self.device))
+        self.prefill(prompts, lengths)
         out[:, 0] = self.tokens
         for t in range(1, count):
             self.step()
@@ -158,11 +205,14 @@ class RaggedGraphDecoder:
     """RaggedEngine with the step captured once as a CUDA graph (the reference's RaggedGraphDecoder contract):
     generate(prompts, lengths, count) -> tokens [B, count] (int64, on the device)."""
 
-    def __init__(self, model, batch, capacity):
-        self.engine = RaggedEngine(model, batch, capacity)
+    def __init__(self, model, batch, capacity, kv_dtype=torch.bfloat16):
+        self._init(RaggedEngine(model, batch, capacity, kv_dtype=kv_dtype))
+
+    def _init(self, engine):
+        self.engine = engine
         self.graph = None
-        self.out = torch.zeros(batch, capacity, dtype=torch.long, device=self.engine.device)
-        self.col = torch.zeros(1, dtype=torch.long, device=self.engine.device)
+        self.out = torch.zeros(engine.batch, engine.cap, dtype=torch.long, device=engine.device)
+        self.col = torch.zeros(1, dtype=torch.long, device=engine.device)
 
     def _capture(self):
         eng = self.engine
@@ -191,8 +241,7 @@ class RaggedGraphDecoder:
             raise ValueError('prompts must have the decoder batch size')
         if self.graph is None:
             self._capture()
-        for r in range(eng.batch):
-            eng.prefill_row(r, prompts[r, :int(lengths[r])].to(eng.device))
+        eng.prefill(prompts, lengths)
         self.col.zero_()
         self.out[:, 0] = eng.tokens
         for _ in range(count - 1):

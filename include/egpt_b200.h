@@ -199,7 +199,8 @@ EGPT_API int egpt_attn_prefill(void *out, int64_t ldo, const void *q, int64_t ld
  *   decode step's prologue runs first: q/k RMSNorm (weights nullable) and RoPE (nullable tables bf16 [rows][d/2],
  *   rows >= rope_base + cap; the angle is that of position rope_base + slot) at the rounding points of
  *   egpt_qk_norm_rope_kv_append, rotated q to q_out [m][ldqo] (zeros for an idle row), and the codes are those of the
- *   bf16 rows that call would cache. Slots outside the cache: EGPT_ERR_SHAPE through egpt_device_error.
+ *   bf16 rows that call would cache; then both scales may be NULL too, and the caches (bf16) get those rows
+ *   themselves. Slots outside the cache: EGPT_ERR_SHAPE through egpt_device_error.
  * egpt_kv_read_q8: k_out, v_out [heads][count][d] (bf16 or fp32, out_head_stride elements between heads) = the values
  *   of rows start .. start + count - 1. With starts (device int64, one per heads_per_start heads) rows begin at
  *   start + starts[h / heads_per_start]; slots outside the cache then read as zeros.
