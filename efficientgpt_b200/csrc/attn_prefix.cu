@@ -1,43 +1,59 @@
-// The shared prefix's part of egpt_attn_shared_prefix on the 5th-generation tensor cores (tcgen05): bf16 caches, head_dim
-// 128, batches of more query rows than the mma.sync kernel's tiles are good for (attn_q8.cu has the rule).
+// The shared prefix's part of egpt_attn_shared_prefix on the 5th-generation tensor cores (tcgen05): bf16 and int8 caches,
+// head_dim 64 or 128, batches of more query rows than the mma.sync kernel's tiles are good for (attn_q8.cu has the rule).
 //
 // The (sequence, head) rows of a kv head, up to 128 of them, are the M of the MMAs: row r of tile t is head r % group of
-// sequence t * seqs + r / group. A CTA of 320 threads owns one kv head, one pair of row tiles and one range of 128-key
-// blocks, and runs two streams, each with 128 columns of TMEM for scores and 128 for its output:
+// sequence t * seqs + r / group. A CTA owns one kv head, one pair of row tiles and one range of 128-key blocks, and
+// runs two streams, each with 128 columns of TMEM for scores and D for its output:
 //   two row tiles:  both streams take every block, one tile each, so a block is loaded once for 256 rows;
 //   one row tile:   the streams take alternate blocks of the same rows.
 // Either way one stream's softmax runs under the other's MMAs. Roles:
-//   warp 0    lane 0 issues the TMA loads (this GPU's memory, no multicast): the query tiles, then K blocks into a 3-slot
-//             ring and V blocks into a 2-slot ring, 128-byte swizzle; the cache maps end at the prefix's last key;
+//   warp 0    lane 0 issues the TMA loads (this GPU's memory, no multicast): the query tiles, then K and V blocks, 128-byte
+//             swizzle, into operand rings (bf16) or a ring of raw code tiles (int8); the cache maps end at the prefix's
+//             last key;
 //   warp 1    allocates TMEM; lane 0 issues S = Q K^T and O += P V, P read from TMEM where the scores were (the next
 //             block's scores of the stream are issued after the P.V that reads it, and MMAs run in order);
-//   warps 2-5 and 6-9: the softmax of stream 0 and 1, one row per thread: the row's 128 scores read for their maximum and once
-//             more for the weights, the running maximum (moved only when a block's exceeds it by more than 2^8; O is then rescaled in TMEM, where no P.V
-//             of the stream can be in flight between a block's scores and its weights), weights as bf16 back to
-//             TMEM, partial sums in fp32. Warps whose rows do not exist skip all of it.
-// A stream ends with a partial record (unnormalised output, maximum, sum of each row) for combine_kernel. Weights
-// enter P.V as bf16 relative to the maximum in use, as in the other bf16 attention kernels; everything else is fp32.
-// Every wait is bounded; issued loads and MMAs are drained before the CTA exits.
+//   warps 2-5 and 6-9: the softmax of stream 0 and 1, one row per thread: the row's 128 scores read for their maximum and
+//             once more for the weights, the running maximum moved only when a block's exceeds it by more than 2^8 (O is
+//             then rescaled in TMEM, where no P.V of the stream can be in flight between a block's scores and its
+//             weights), weights as bf16 back to TMEM, partial sums in fp32. Warps whose rows do not exist skip all of it;
+//   warps 10-13 (int8): widen a code tile to bf16, exactly, one key per thread, into the operand rings, and put the
+//             block's scales (the keys' times scale log2(e)) beside them: a key's scale multiplies its column of scores,
+//             a value's its column of weights.
+// A stream ends with a partial record (unnormalised output, maximum, sum of each row) for add_kernel. With bf16 caches
+// weights enter P.V as bf16 relative to the maximum in use, as in the other bf16 attention kernels; with int8 caches as
+// the sum of two bf16 values (16 bits), a second P.V: the values' own rounding is then the only one that counts.
+// Everything else is fp32. Every wait is bounded; issued loads and MMAs are drained before the CTA exits.
 #include "internal.h"
 #include "common.cuh"
 
 namespace egpt {
 namespace apx {
 
-using apf::kHalf;
-using apf::kTile;
+constexpr int kBK = 128, kRowsT = 128;
+constexpr uint32_t kOCol = 256;  // S0 | S1 | O0 | O1, 128 columns each; P_s in S_s: 64 columns, int8: two times 64
+constexpr int record_size(int d) { return kRowsT * (d + 2); }  // floats: [128 rows][d], maxima, sums
 
-constexpr int kD = 128, kBK = 128, kRowsT = 128;
-constexpr int kKStages = 3, kVStages = 2;
-constexpr int kThreads = 64 + 2 * 128;
-constexpr uint32_t kOCol = 256;  // S0 | S1 | O0 | O1, 128 columns each; P_s in the first 64 columns of S_s
-constexpr size_t kSmem = 1024 /* alignment slack */ + (size_t)(2 + kKStages + kVStages) * kTile + 256;
-constexpr int kRecord = kRowsT * (kD + 2);  // floats: [128 rows][128], maxima, sums
+template <int D, bool Q8>
+struct Cfg {
+  static constexpr int kHalves = D / 64;            // 64-column groups of an operand tile
+  static constexpr int kHalf = kRowsT * 128;        // bytes: 128 rows x 64 bf16, one 128-byte swizzle column
+  static constexpr int kTile = kHalves * kHalf;
+  static constexpr int kKStages = Q8 ? 2 : 3, kVStages = 2;
+  static constexpr int kRaw = kBK * D;              // bytes of a code tile
+  static constexpr int kThreads = 64 + 256 + (Q8 ? 128 : 0);
+  static constexpr size_t kScales = Q8 ? 2 * 2 * kBK * 4 : 0;  // two blocks' [ks scale log2(e)][vs]
+  // int8: two code tiles and two blocks' scales behind two query tiles; three and four where the second tile's place is free
+  static constexpr size_t kUsed = (size_t)(2 + kKStages + kVStages) * kTile + (Q8 ? 2 * kRaw : 0) + kScales + 256;
+  static constexpr size_t kSlack = 768;             // alignment: the CTA's shared memory starts 1024-aligned, or nearly
+  static constexpr size_t kSmem = kUsed + kSlack;
+};
 
 struct Args {
-  CUtensorMap qmap;  // q bf16 [m][nq][128], box {64, group, seqs}, 128-byte swizzle
-  CUtensorMap kmap;  // K bf16 [nkv][prefix_len][128] (head stride prefix_cap rows), box {64, 128, 1}
+  CUtensorMap qmap;  // q bf16 [m][nq][D], box {64, group, seqs}, 128-byte swizzle
+  CUtensorMap kmap;  // K bf16 or int8 [nkv][prefix_len][D] (head stride prefix_cap rows), box {64 | D, 128, 1}
   CUtensorMap vmap;
+  const float *ks, *vs;  // int8: [nkv][cap]
+  int64_t cap;
   float *ws;         // records [nkv][pairs][ranges][2 streams]
   int64_t prefix;
   int m, nkv, group;
@@ -46,17 +62,40 @@ struct Args {
   float scale_log2;  // > 0
 };
 
-__global__ void __launch_bounds__(kThreads, 1) attn_prefix_kernel(const __grid_constant__ Args A) {
+__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// The bf16 values of two codes, exactly (as codes_bf16 of attn_q8.cu).
+__device__ __forceinline__ uint32_t widen2(uint32_t codes, uint32_t select) {
+  uint32_t r;
+  const uint32_t pasted = __byte_perm(codes, 0x43434343u, select);
+  asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(pasted & 0xff7fff7fu), "r"((pasted & 0xff80ff80u) | 0x80008000u));
+  return r;
+}
+
+template <int D, bool Q8>
+__global__ void __launch_bounds__(Cfg<D, Q8>::kThreads, 1) attn_prefix_kernel(const __grid_constant__ Args A) {
+  using C = Cfg<D, Q8>;
+  constexpr int kTile = C::kTile, kHalf = C::kHalf, kKStages = C::kKStages, kVStages = C::kVStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);  // 1024-aligned operand tiles
-  uint8_t *sq = smem;                            // two query tiles, each two [128 rows][128 B] halves
+  if ((size_t)(smem - smem_raw) > C::kSlack) {
+    if (threadIdx.x == 0) set_device_error(EGPT_ERR_ALIGN);
+    return;
+  }
+  uint8_t *sq = smem;                            // two query tiles, each of [128 rows][128 B] halves
   uint8_t *sk = sq + 2 * kTile;                  // K slots
   uint8_t *sv = sk + (size_t)kKStages * kTile;   // V slots
-  uint64_t *bars = (uint64_t *)(sv + (size_t)kVStages * kTile);
+  uint8_t *raw0 = sv + (size_t)kVStages * kTile;  // code tiles 0, 1; the third in the second query tile's place
+  float *scales = (float *)(raw0 + (Q8 ? 2 * C::kRaw : 0));
+  uint64_t *bars = (uint64_t *)((uint8_t *)scales + C::kScales);
   uint64_t *q_full = bars, *k_full = q_full + 1, *k_empty = k_full + kKStages, *v_full = k_empty + kKStages;
   uint64_t *v_empty = v_full + kVStages, *s_full = v_empty + kVStages, *p_full = s_full + 2, *o_done = p_full + 2;
-  uint64_t *mma_done = o_done + 2;
-  uint32_t *tmem_slot = (uint32_t *)(mma_done + 1);
+  uint64_t *mma_done = o_done + 2, *raw_full = mma_done + 1, *raw_empty = raw_full + 3;
+  uint64_t *scale_full = raw_empty + 3;
+  uint32_t *tmem_slot = (uint32_t *)(scale_full + 4);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   pdl_wait();
@@ -75,14 +114,16 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefix_kernel(const __grid_c
 
   if (threadIdx.x == 0) {
     gtc::mbar_init(q_full, 1);
-    for (int s = 0; s < kKStages; ++s) gtc::mbar_init(k_full + s, 1), gtc::mbar_init(k_empty + s, 1);
-    for (int s = 0; s < kVStages; ++s) gtc::mbar_init(v_full + s, 1), gtc::mbar_init(v_empty + s, 1);
+    for (int s = 0; s < kKStages; ++s) gtc::mbar_init(k_full + s, Q8 ? 128 : 1), gtc::mbar_init(k_empty + s, 1);
+    for (int s = 0; s < kVStages; ++s) gtc::mbar_init(v_full + s, Q8 ? 128 : 1), gtc::mbar_init(v_empty + s, 1);
     for (int s = 0; s < 2; ++s) {
       gtc::mbar_init(s_full + s, 1);
       gtc::mbar_init(p_full + s, max(1, (rows[s] + 31) / 32) * 32);  // every thread of the warps that have rows
       gtc::mbar_init(o_done + s, 1);
     }
     gtc::mbar_init(mma_done, 1);
+    for (int s = 0; s < 3; ++s) gtc::mbar_init(raw_full + s, 1), gtc::mbar_init(raw_empty + s, 128);
+    for (int s = 0; s < 4; ++s) gtc::mbar_init(scale_full + s, 128);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
@@ -95,44 +136,63 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefix_kernel(const __grid_c
   __syncthreads();
   gtc::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  const int raws = two ? 2 : 3, scale_slots = two ? 2 : 4;  // code tiles in flight (K, V, K, ...), blocks with scales
+  auto raw_tile = [&](int u) { return u < 2 ? raw0 + u * C::kRaw : sq + kTile; };
+  auto scale_of = [&](int b) {  // [ks scale log2(e)][vs] of block b
+    const int j = b % scale_slots;
+    return (j < 2 ? scales : (float *)(sq + kTile + C::kRaw) - 4 * kBK) + j * 2 * kBK;
+  };
 
   if (warp == 0) {
     // ---------------------------------------------------------------- TMA producer
     if (lane == 0) {
       const unsigned qbytes = (unsigned)(A.seqs * A.group) * 128u;  // one half of a query tile
-      gtc::mbar_arrive_tx(q_full, (two ? 4u : 2u) * qbytes);
+      gtc::mbar_arrive_tx(q_full, (two ? 2u : 1u) * C::kHalves * qbytes);
       for (int s = 0; s < (two ? 2 : 1); ++s)
-        for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < C::kHalves; ++h)
           apf::tma_load_3d(sq + s * kTile + h * kHalf, &A.qmap, 64 * h, g * A.group, (2 * pair + s) * A.seqs, q_full);
-      int nk = 0, nv = 0;
-      auto load = [&](int b, const CUtensorMap *map, uint8_t *ring, int stages, uint64_t *full, uint64_t *empty) -> bool {
-        const int slot = b % stages;
-        if (b >= stages && !gtc::mbar_wait(empty + slot, (unsigned)((b / stages) - 1) & 1u)) return false;
-        uint8_t *t = ring + (size_t)slot * kTile;
-        gtc::mbar_arrive_tx(full + slot, kTile);
-        apf::tma_load_3d(t, map, 0, (b0 + b) * kBK, g, full + slot);
-        apf::tma_load_3d(t + kHalf, map, 64, (b0 + b) * kBK, g, full + slot);
-        return true;
-      };
-      auto load_k = [&](int b) -> bool {
-        if (!load(b, &A.kmap, sk, kKStages, k_full, k_empty)) return false;
-        ++nk;
-        return true;
-      };
-      bool ok = load_k(0) && (n < 2 || load_k(1));
-      for (int b = 0; b < n && ok; ++b) {  // K runs two blocks ahead of V: scores come first
-        ok = load(b, &A.vmap, sv, kVStages, v_full, v_empty);
-        if (ok) ++nv;
-        if (ok && b + 2 < n) ok = load_k(b + 2);
+      if constexpr (Q8) {
+        int u = 0;  // tile 2 b is block b's K, 2 b + 1 its V
+        for (; u < 2 * n; ++u) {
+          const int slot = u % raws;
+          if (u >= raws && !gtc::mbar_wait(raw_empty + slot, (unsigned)((u / raws) - 1) & 1u)) break;
+          gtc::mbar_arrive_tx(raw_full + slot, C::kRaw);
+          apf::tma_load_3d(raw_tile(slot), u & 1 ? &A.vmap : &A.kmap, 0, (b0 + u / 2) * kBK, g, raw_full + slot);
+        }
+        for (int t = max(0, u - raws); t < u; ++t) gtc::mbar_drain(raw_full + t % raws, (unsigned)(t / raws) & 1u);
+      } else {
+        int nk = 0, nv = 0;
+        auto load = [&](int b, const CUtensorMap *map, uint8_t *ring, int stages, uint64_t *full, uint64_t *empty) -> bool {
+          const int slot = b % stages;
+          if (b >= stages && !gtc::mbar_wait(empty + slot, (unsigned)((b / stages) - 1) & 1u)) return false;
+          uint8_t *t = ring + (size_t)slot * kTile;
+          gtc::mbar_arrive_tx(full + slot, kTile);
+          for (int h = 0; h < C::kHalves; ++h)
+            apf::tma_load_3d(t + h * kHalf, map, 64 * h, (b0 + b) * kBK, g, full + slot);
+          return true;
+        };
+        auto load_k = [&](int b) -> bool {
+          if (!load(b, &A.kmap, sk, kKStages, k_full, k_empty)) return false;
+          ++nk;
+          return true;
+        };
+        bool ok = load_k(0) && (n < 2 || load_k(1));
+        for (int b = 0; b < n && ok; ++b) {  // K runs two blocks ahead of V: scores come first
+          ok = load(b, &A.vmap, sv, kVStages, v_full, v_empty);
+          if (ok) ++nv;
+          if (ok && b + 2 < n) ok = load_k(b + 2);
+        }
+        for (int b = max(0, nk - kKStages); b < nk; ++b)
+          gtc::mbar_drain(k_full + b % kKStages, (unsigned)(b / kKStages) & 1u);
+        for (int b = max(0, nv - kVStages); b < nv; ++b)
+          gtc::mbar_drain(v_full + b % kVStages, (unsigned)(b / kVStages) & 1u);
       }
-      // none of this CTA's copies may still be landing when it exits
-      gtc::mbar_drain(q_full, 0);
-      for (int b = max(0, nk - kKStages); b < nk; ++b) gtc::mbar_drain(k_full + b % kKStages, (unsigned)(b / kKStages) & 1u);
-      for (int b = max(0, nv - kVStages); b < nv; ++b) gtc::mbar_drain(v_full + b % kVStages, (unsigned)(b / kVStages) & 1u);
+      gtc::mbar_drain(q_full, 0);  // none of this CTA's copies may still be landing when it exits
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMA issuer
     if (lane == 0) {
+      constexpr uint32_t kIdescO = (apf::kIdescO & ~(0x3fu << 17)) | ((uint32_t)(D >> 3) << 17);  // N = D
       auto block_of = [&](int s, int i) { return two ? i : 2 * i + s; };
       // with two row tiles a slot is free once stream 1's MMAs, issued after stream 0's, have read it
       auto issue_scores = [&](int s, int i) -> bool {
@@ -141,7 +201,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefix_kernel(const __grid_c
         gtc::tc_fence_after();
         const uint8_t *q = sq + (two ? s : 0) * kTile, *k = sk + (size_t)slot * kTile;
 #pragma unroll
-        for (int kk = 0; kk < kD / 16; ++kk) {
+        for (int kk = 0; kk < D / 16; ++kk) {
           const uint64_t off = (uint64_t)(2 * (kk & 3));
           apf::umma(tmem + (uint32_t)(128 * s), gtc::sw128_desc(q + (kk >> 2) * kHalf) + off,
                     gtc::sw128_desc(k + (kk >> 2) * kHalf) + off, apf::kIdescS, kk > 0 ? 1u : 0u);
@@ -160,9 +220,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefix_kernel(const __grid_c
           gtc::tc_fence_after();
           const uint8_t *v = sv + (size_t)slot * kTile;
 #pragma unroll
-          for (int kk = 0; kk < kBK / 16; ++kk)  // 16 keys per step: 8 columns of P, 16 rows of 128 bytes of V
-            apf::umma_ts(tmem + kOCol + (uint32_t)(128 * s), tmem + (uint32_t)(128 * s + 8 * kk),
-                         apf::sw128_mn_desc(v + (size_t)kk * 16 * 128), apf::kIdescO, (i > 0 || kk > 0) ? 1u : 0u);
+          for (int part = 0; part < (Q8 ? 2 : 1); ++part)
+#pragma unroll
+            for (int kk = 0; kk < kBK / 16; ++kk)  // 16 keys per step: 8 columns of P, 16 rows of 128 bytes of V
+              apf::umma_ts(tmem + kOCol + (uint32_t)(128 * s), tmem + (uint32_t)(128 * s + 64 * part + 8 * kk),
+                           apf::sw128_mn_desc(v + (size_t)kk * 16 * 128), kIdescO, (i > 0 || part > 0 || kk > 0) ? 1u : 0u);
           if (!two || s == 1) gtc::umma_commit(v_empty + slot);
           if (i + 1 < steps[s]) ok = issue_scores(s, i + 1);
           else gtc::umma_commit(o_done + s);
@@ -170,7 +232,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefix_kernel(const __grid_c
       gtc::umma_commit(mma_done);  // completes once every MMA issued above has finished
       gtc::mbar_drain(mma_done, 0);
     }
-  } else {
+  } else if (warp < 10) {
     // ---------------------------------------------------------------- softmax: one row per thread
     const int s = (warp - 2) >> 2;
     const int quarter = warp & 3;  // TMEM lanes this warp may access: 32 (warp % 4) ..
@@ -180,28 +242,47 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefix_kernel(const __grid_c
       float m_run = -INFINITY, l_sum = 0.f;
       bool ok = true;
       for (int i = 0; i < steps[s] && ok; ++i) {
+        const int b = two ? i : 2 * i + s;
         ok = apf::warp_wait(s_full + s, (unsigned)i & 1u);
+        // (a slot's next phase waits for the P.V of the block that holds it now)
+        if (Q8) ok = ok && apf::warp_wait(scale_full + b % scale_slots, (unsigned)(b / scale_slots) & 1u);
         if (!ok) break;
         gtc::tc_fence_after();
-        const int left = (int)min((int64_t)kBK, A.prefix - (int64_t)(b0 + (two ? i : 2 * i + s)) * kBK);
-        auto load_scores = [&](int c, uint32_t *sc) {  // 32 of the row's scores; -inf past the prefix
-          apf::tmem_ld32(ts + (uint32_t)c, sc);
-          apf::tmem_wait_ld();
+        const float *ks = scale_of(b), *vs = ks + kBK;
+        const uint64_t one2 = apf::f2_pack(A.scale_log2, A.scale_log2);
+        const int left = (int)min((int64_t)kBK, A.prefix - (int64_t)(b0 + b) * kBK);
+        auto mask = [&](int c, uint32_t *sc) {  // -inf past the prefix
           if (left < c + 32) {
 #pragma unroll
             for (int e = 0; e < 32; ++e)
               if (c + e >= left) sc[e] = __float_as_uint(-INFINITY);
           }
         };
+        // scores to log2 units in place: bf16 later, in one fma with the maximum
+        auto scaled = [&](int c, uint32_t *sc) {
+          if constexpr (Q8) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) {
+              const ulonglong2 f = *(const ulonglong2 *)(ks + c + e);
+              const float2 x = apf::f2_unpack(f2_mul(apf::f2_pack(__uint_as_float(sc[e]), __uint_as_float(sc[e + 1])), f.x));
+              const float2 y = apf::f2_unpack(f2_mul(apf::f2_pack(__uint_as_float(sc[e + 2]), __uint_as_float(sc[e + 3])), f.y));
+              sc[e] = __float_as_uint(x.x), sc[e + 1] = __float_as_uint(x.y);
+              sc[e + 2] = __float_as_uint(y.x), sc[e + 3] = __float_as_uint(y.y);
+            }
+          }
+          mask(c, sc);
+        };
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int c = 0; c < kBK; c += 32) {
           uint32_t sc[32];
-          load_scores(c, sc);
+          apf::tmem_ld32(ts + (uint32_t)c, sc);
+          apf::tmem_wait_ld();
+          scaled(c, sc);
 #pragma unroll
           for (int e = 0; e < 32; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(sc[e]));
         }
-        const float bm = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * A.scale_log2;
+        const float bm = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * (Q8 ? 1.f : A.scale_log2);
         float alpha = 1.f;
         if (bm > m_run + apf::kStale) {
           alpha = apf::ex2(m_run - bm);  // 0 on the first block
@@ -210,7 +291,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefix_kernel(const __grid_c
         if (i > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
           // the stream's P.V so far has finished: the scores that were just read completed after it
 #pragma unroll
-          for (int c = 0; c < kD; c += 32) {
+          for (int c = 0; c < D; c += 32) {
             uint32_t o[32];
             apf::tmem_ld32(to + (uint32_t)c, o);
             apf::tmem_wait_ld();
@@ -219,21 +300,49 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefix_kernel(const __grid_c
             apf::tmem_st32(to + (uint32_t)c, o);
           }
         }
-        const uint64_t sc2 = apf::f2_pack(A.scale_log2, A.scale_log2), nm2 = apf::f2_pack(-m_run, -m_run);
+        const uint64_t nm2 = apf::f2_pack(-m_run, -m_run);
         uint64_t sum[2] = {apf::f2_pack(0.f, 0.f), apf::f2_pack(0.f, 0.f)};
-#pragma unroll
-        for (int c = 0; c < kBK; c += 32) {
-          uint32_t sc[32], pk[16];
-          load_scores(c, sc);
+        // weights of 32 keys over scores that have been read: bf16 in columns c / 2 ..; int8: the second parts 64 on
+        auto weights = [&](int c, const uint32_t *sc) {
+          uint32_t pk[16], pl[Q8 ? 16 : 1];
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
-            const float2 x = apf::f2_unpack(apf::f2_fma(
-                apf::f2_pack(__uint_as_float(sc[e]), __uint_as_float(sc[e + 1])), sc2, nm2));
-            const float p0 = apf::ex2(x.x), p1 = apf::ex2(x.y);
-            sum[(e >> 1) & 1] = apf::f2_add(sum[(e >> 1) & 1], apf::f2_pack(p0, p1));
-            pk[e / 2] = gtc::pack_bf16x2(p0, p1);
+            const uint64_t raw = apf::f2_pack(__uint_as_float(sc[e]), __uint_as_float(sc[e + 1]));
+            const float2 x = apf::f2_unpack(Q8 ? apf::f2_add(raw, nm2) : apf::f2_fma(raw, one2, nm2));
+            float2 w = make_float2(apf::ex2(x.x), apf::ex2(x.y));
+            sum[(e >> 1) & 1] = apf::f2_add(sum[(e >> 1) & 1], apf::f2_pack(w.x, w.y));
+            if (Q8) w = apf::f2_unpack(f2_mul(apf::f2_pack(w.x, w.y), *(const uint64_t *)(vs + c + e)));
+            pk[e / 2] = gtc::pack_bf16x2(w.x, w.y);
+            if constexpr (Q8) pl[e / 2] = gtc::pack_bf16x2(w.x - bf16_lo(pk[e / 2]), w.y - bf16_hi(pk[e / 2]));
           }
-          apf::tmem_st16(ts + (uint32_t)(c / 2), pk);  // over scores that have been read
+          apf::tmem_st16(ts + (uint32_t)(c / 2), pk);
+          if constexpr (Q8) apf::tmem_st16(ts + (uint32_t)(64 + c / 2), pl);
+        };
+        if constexpr (Q8) {  // the second parts go over the upper scores: those are read first
+          uint32_t up[2][32];
+          apf::tmem_ld32(ts + 64, up[0]);
+          apf::tmem_ld32(ts + 96, up[1]);
+#pragma unroll
+          for (int c = 0; c < 64; c += 32) {
+            uint32_t sc[32];
+            apf::tmem_ld32(ts + (uint32_t)c, sc);
+            apf::tmem_wait_ld();
+            scaled(c, sc);
+            weights(c, sc);
+          }
+          scaled(64, up[0]);
+          weights(64, up[0]);
+          scaled(96, up[1]);
+          weights(96, up[1]);
+        } else {
+#pragma unroll
+          for (int c = 0; c < kBK; c += 32) {
+            uint32_t sc[32];
+            apf::tmem_ld32(ts + (uint32_t)c, sc);
+            apf::tmem_wait_ld();
+            scaled(c, sc);
+            weights(c, sc);
+          }
         }
         const float2 t = apf::f2_unpack(apf::f2_add(sum[0], sum[1]));
         l_sum = l_sum * alpha + (t.x + t.y);
@@ -243,26 +352,72 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefix_kernel(const __grid_c
       }
       if (ok && apf::warp_wait(o_done + s, 0)) {
         gtc::tc_fence_after();
-        float *rec = A.ws + ((int64_t)blockIdx.x * 2 + s) * kRecord;
+        float *rec = A.ws + ((int64_t)blockIdx.x * 2 + s) * record_size(D);
 #pragma unroll
-        for (int c = 0; c < kD; c += 32) {
+        for (int c = 0; c < D; c += 32) {
           uint32_t o[32];
           apf::tmem_ld32(to + (uint32_t)c, o);
           apf::tmem_wait_ld();
           if (row < rows[s]) {
 #pragma unroll
             for (int e = 0; e < 32; e += 4)
-              *(uint4 *)(rec + row * kD + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+              *(uint4 *)(rec + row * D + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
           }
         }
-        rec[kRowsT * kD + row] = m_run;
-        rec[kRowsT * kD + kRowsT + row] = l_sum;
+        rec[kRowsT * D + row] = m_run;
+        rec[kRowsT * D + kRowsT + row] = l_sum;
       }
     }
     if (!steps[s]) {  // a range of one block: the second stream has no record to add
-      float *rec = A.ws + ((int64_t)blockIdx.x * 2 + s) * kRecord;
-      rec[kRowsT * kD + row] = -INFINITY;
-      rec[kRowsT * kD + kRowsT + row] = 0.f;
+      float *rec = A.ws + ((int64_t)blockIdx.x * 2 + s) * record_size(D);
+      rec[kRowsT * D + row] = -INFINITY;
+      rec[kRowsT * D + kRowsT + row] = 0.f;
+    }
+  } else if constexpr (Q8) {
+    // ---------------------------------------------------------------- widening: one key per thread
+    const int r = (int)threadIdx.x - 320;
+    auto widen = [&](int u, uint8_t *dst) -> bool {  // code tile u to an operand tile
+      const int slot = u % raws;
+      if (!gtc::mbar_wait(raw_full + slot, (unsigned)(u / raws) & 1u)) return false;
+      const uint8_t *src = raw_tile(slot) + r * D;
+      const int swz = D == 128 ? (r & 7) : ((r >> 1) & 3);  // the map's 128- or 64-byte swizzle
+#pragma unroll
+      for (int c = 0; c < D / 16; ++c) {
+        const uint4 w = *(const uint4 *)(src + ((c ^ swz) * 16));
+        uint8_t *half = dst + (c >> 2) * kHalf + r * 128;
+        const int cc = 2 * (c & 3);
+        *(uint4 *)(half + ((cc ^ (r & 7)) * 16)) =
+            make_uint4(widen2(w.x, 0x4140), widen2(w.x, 0x4342), widen2(w.y, 0x4140), widen2(w.y, 0x4342));
+        *(uint4 *)(half + (((cc + 1) ^ (r & 7)) * 16)) =
+            make_uint4(widen2(w.z, 0x4140), widen2(w.z, 0x4342), widen2(w.w, 0x4140), widen2(w.w, 0x4342));
+      }
+      gtc::mbar_arrive(raw_empty + slot);
+      return true;
+    };
+    auto scale_at = [&](const float *p, int b) {
+      const int64_t key = (int64_t)(b0 + b) * kBK + r;
+      return b < n && key < A.prefix ? p[g * A.cap + key] : 0.f;
+    };
+    float next_ks = scale_at(A.ks, 0), next_vs = scale_at(A.vs, 0);
+    for (int b = 0; b < n; ++b) {
+      const float ks = next_ks * A.scale_log2, vs = next_vs;
+      next_ks = scale_at(A.ks, b + 1), next_vs = scale_at(A.vs, b + 1);
+      const int kslot = b % kKStages, vslot = b % kVStages;
+      // an operand slot is free once its MMAs have run, a scale slot once the P.V of its last block has: with two of
+      // them that is block b - 2's, with four b - 4's, which V(b - 2) has waited for
+      if (scale_slots == 2 && b >= 2 && !gtc::mbar_wait(v_empty + vslot, (unsigned)((b / kVStages) - 1) & 1u)) break;
+      float *sc = scale_of(b);
+      sc[r] = ks;
+      sc[kBK + r] = vs;
+      gtc::mbar_arrive(scale_full + b % scale_slots);
+      if (b >= kKStages && !gtc::mbar_wait(k_empty + kslot, (unsigned)((b / kKStages) - 1) & 1u)) break;
+      if (!widen(2 * b, sk + (size_t)kslot * kTile)) break;
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      gtc::mbar_arrive(k_full + kslot);
+      if (b >= kVStages && !gtc::mbar_wait(v_empty + vslot, (unsigned)((b / kVStages) - 1) & 1u)) break;
+      if (!widen(2 * b + 1, sv + (size_t)vslot * kTile)) break;
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      gtc::mbar_arrive(v_full + vslot);
     }
   }
   gtc::tc_fence_before();
@@ -287,43 +442,48 @@ static Shape shape_of(int64_t m, int group, int nkv, int64_t prefix) {
   return s;
 }
 // Floats of the records of any prefix: as many ranges as the SMs allow.
-static size_t record_floats(int64_t m, int group, int nkv) {
+static size_t record_floats(int64_t m, int group, int nkv, int d) {
   const Shape s = shape_of(m, group, nkv, (int64_t)1 << 40);
-  return (size_t)nkv * s.pairs * s.ranges * 2 * kRecord;
+  return (size_t)nkv * s.pairs * s.ranges * 2 * record_size(d);
 }
 
-static cudaError_t launch(Args &A, const void *q, int64_t ldq, const void *k, const void *v, int64_t prefix_cap,
-                          const Shape &sh, cudaStream_t st, bool pdl, bool &maps_ok) {
+template <int D, bool Q8>
+static cudaError_t launch(Args &A, const void *q, int64_t ldq, const void *k, const void *v, const Shape &sh,
+                          cudaStream_t st, bool pdl, bool &maps_ok) {
+  using C = Cfg<D, Q8>;
   auto fn = df::encode_fn();
   maps_ok = fn != nullptr;
   if (!fn) return cudaSuccess;
   const cuuint32_t ones[3] = {1, 1, 1};
-  const cuuint64_t qdims[3] = {kD, (cuuint64_t)A.nkv * A.group, (cuuint64_t)A.m};
-  const cuuint64_t qstrides[2] = {kD * 2, (cuuint64_t)ldq * 2};
+  const cuuint64_t qdims[3] = {D, (cuuint64_t)A.nkv * A.group, (cuuint64_t)A.m};
+  const cuuint64_t qstrides[2] = {D * 2, (cuuint64_t)ldq * 2};
   const cuuint32_t qbox[3] = {64, (cuuint32_t)A.group, (cuuint32_t)sh.seqs};
-  const cuuint64_t kdims[3] = {kD, (cuuint64_t)A.prefix, (cuuint64_t)A.nkv};
-  const cuuint64_t kstrides[2] = {kD * 2, (cuuint64_t)prefix_cap * kD * 2};
-  const cuuint32_t kbox[3] = {64, kBK, 1};
-  auto encode = [&](CUtensorMap *map, const void *p, const cuuint64_t *dims, const cuuint64_t *strides,
+  const int esz = Q8 ? 1 : 2;
+  const cuuint64_t kdims[3] = {D, (cuuint64_t)A.prefix, (cuuint64_t)A.nkv};
+  const cuuint64_t kstrides[2] = {(cuuint64_t)D * esz, (cuuint64_t)A.cap * D * esz};
+  const cuuint32_t kbox[3] = {Q8 ? D : 64, kBK, 1};
+  auto encode = [&](CUtensorMap *map, bool codes, const void *p, const cuuint64_t *dims, const cuuint64_t *strides,
                     const cuuint32_t *box) {
-    return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(p), dims, strides, box, ones,
-              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+    return fn(map, codes ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(p), dims,
+              strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              codes && D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
   };
-  maps_ok = encode(&A.qmap, q, qdims, qstrides, qbox) && encode(&A.kmap, k, kdims, kstrides, kbox) &&
-            encode(&A.vmap, v, kdims, kstrides, kbox);
+  maps_ok = encode(&A.qmap, false, q, qdims, qstrides, qbox) && encode(&A.kmap, Q8, k, kdims, kstrides, kbox) &&
+            encode(&A.vmap, Q8, v, kdims, kstrides, kbox);
   if (!maps_ok) return cudaSuccess;
   static int configured[64] = {0};  // the shared-memory opt-in, per device
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev >= 0 && dev < 64 && !configured[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(attn_prefix_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem);
+    const cudaError_t e = cudaFuncSetAttribute(attn_prefix_kernel<D, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               (int)C::kSmem);
     if (e != cudaSuccess) return e;
     configured[dev] = 1;
   }
   A.seqs = sh.seqs, A.tiles = sh.tiles, A.pairs = sh.pairs, A.ranges = sh.ranges;
-  return launch_kernel((const void *)attn_prefix_kernel, dim3((unsigned)(A.nkv * sh.pairs * sh.ranges)), dim3(kThreads),
-                       kSmem, st, pdl, A);
+  return launch_kernel((const void *)attn_prefix_kernel<D, Q8>, dim3((unsigned)(A.nkv * sh.pairs * sh.ranges)),
+                       dim3(C::kThreads), C::kSmem, st, pdl, A);
 }
 
 }  // namespace apx

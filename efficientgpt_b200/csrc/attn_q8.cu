@@ -887,9 +887,9 @@ __global__ void __launch_bounds__(32 * kAddWarps) add_kernel(const Params p) {
     const int tile = i / p.pre.seqs, pair = tile / 2;
     const bool two = 2 * pair + 1 < p.pre.tiles;  // the pair's streams are two tiles, or both this one
     pre_n = two ? p.pre.ranges : 2 * p.pre.ranges;
-    pre_step = two ? 2 * apx::kRecord : apx::kRecord;
+    pre_step = (two ? 2 : 1) * apx::record_size(D);
     pre_row = (i - tile * p.pre.seqs) * p.group + j, pre_rows = apx::kRowsT;
-    pre0 = p.pre.rec + ((int64_t)(g * p.pre.pairs + pair) * p.pre.ranges * 2 + (two ? tile & 1 : 0)) * apx::kRecord;
+    pre0 = p.pre.rec + ((int64_t)(g * p.pre.pairs + pair) * p.pre.ranges * 2 + (two ? tile & 1 : 0)) * apx::record_size(D);
   } else {
     const int flat = i * p.group + j, seg = g * p.pre.row_tiles + flat / kRows;
     const int start = seg * ceil_div(p.pre.seg_tiles, p.pre.pad) * p.pre.pad;
@@ -958,9 +958,9 @@ static cudaError_t launch_any(Params &p, int d, bool q8, int rows, cudaStream_t 
   if (rows <= 8) return q8 ? launch_d<true, 8, MODE>(p, d, st, pdl) : launch_d<false, 8, MODE>(p, d, st, pdl);
   return q8 ? launch_d<true, 16, MODE>(p, d, st, pdl) : launch_d<false, 16, MODE>(p, d, st, pdl);
 }
-// Whether the prefix goes to attn_prefix_kernel: bf16, head_dim 128, more rows than one tile of the mma.sync kernel.
-static bool prefix_on_tcgen05(const Params &p, int d, bool q8) {
-  return !q8 && d == apx::kD && p.scale_log2 > 0.f && p.m * p.group > kRows;
+// Whether the prefix goes to attn_prefix_kernel: head_dim 64 or 128 and more rows than one tile of the mma.sync kernel.
+static bool prefix_on_tcgen05(const Params &p, int d) {
+  return d >= 64 && p.scale_log2 > 0.f && p.m * p.group > kRows;
 }
 // Arrival counters, then the (first record, records) pairs of the segments.
 static size_t counter_bytes(int64_t m, int nkv) { return ((size_t)m * nkv * 16 + 255) / 256 * 256; }
@@ -993,7 +993,7 @@ extern "C" size_t egpt_attn_q8_ws_bytes(int64_t m, int nq, int nkv, int d) {
   // records: attn_kernel's, one for every pair again, or attn_prefix_kernel's
   const size_t rec = aq8::kRows * ((size_t)d + 2) * 4;
   const size_t small = ((size_t)aq8::max_grid() + (size_t)nkv * aq8::row_tiles(m, nq / nkv)) * rec;
-  const size_t big = d == apx::kD && nq / nkv <= aq8::kRows ? apx::record_floats(m, nq / nkv, nkv) * 4 : 0;
+  const size_t big = (d == 64 || d == 128) && nq / nkv <= aq8::kRows ? apx::record_floats(m, nq / nkv, nkv, d) * 4 : 0;
   return aq8::counter_bytes(m, nkv) + ((size_t)aq8::max_grid() + (size_t)m * nkv) * rec + std::max(small, big);
 }
 
@@ -1045,12 +1045,16 @@ extern "C" int egpt_attn_shared_prefix(void *out, int64_t ldo, const void *q, in
   p.ws = (float *)((char *)ws + aq8::counter_bytes(m, nkv));
   float *pre_rec = p.ws + ((size_t)aq8::max_grid() + (size_t)m * nkv) * aq8::kRows * (d + 2);
   if (prefix_len > 0) {
-    if (aq8::prefix_on_tcgen05(p, d, q8)) {
+    if (aq8::prefix_on_tcgen05(p, d)) {
       apx::Args A{};
       const apx::Shape sh = apx::shape_of(m, p.group, nkv, prefix_len);
       A.ws = pre_rec, A.prefix = prefix_len, A.m = (int)m, A.nkv = nkv, A.group = p.group, A.scale_log2 = p.scale_log2;
+      A.ks = pk_scale, A.vs = pv_scale, A.cap = prefix_cap;
       bool maps_ok = false;
-      const cudaError_t e = apx::launch(A, q, ldq, pk, pv, prefix_cap, sh, st, pdl, maps_ok);
+      const cudaError_t e = d == 128 ? (q8 ? apx::launch<128, true>(A, q, ldq, pk, pv, sh, st, pdl, maps_ok)
+                                           : apx::launch<128, false>(A, q, ldq, pk, pv, sh, st, pdl, maps_ok))
+                                     : (q8 ? apx::launch<64, true>(A, q, ldq, pk, pv, sh, st, pdl, maps_ok)
+                                           : apx::launch<64, false>(A, q, ldq, pk, pv, sh, st, pdl, maps_ok));
       if (!maps_ok) return set_error(EGPT_ERR_ALIGN, "attn_shared_prefix: tensor maps rejected");
       if (e != cudaSuccess) return check_launch(e, "attn_prefix_kernel");
       p.pre.big = 1, p.pre.seqs = sh.seqs, p.pre.tiles = sh.tiles, p.pre.pairs = sh.pairs, p.pre.ranges = sh.ranges;

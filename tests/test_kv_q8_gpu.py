@@ -308,6 +308,7 @@ def _poison(cache, heads, n):
     (128, 6, 2, 33, 257), (64, 16, 2, 3, 0), (128, 2, 2, 64, 4097), (128, 32, 2, 7, 130), (128, 8, 2, 100, 640),
     # row tiles of 128: three of them, a second with one sequence, 126 rows of 128, one key, whole blocks only
     (128, 8, 2, 80, 1500), (128, 16, 1, 9, 300), (128, 9, 3, 50, 129), (128, 4, 1, 20, 1), (128, 16, 4, 64, 12800),
+    (64, 8, 2, 80, 1500), (64, 12, 2, 24, 6000), (64, 4, 1, 40, 20000), (128, 4, 1, 40, 20000), (64, 16, 8, 16, 129),
 ])
 def test_shared_prefix(cuda, q8, d, nq, nkv, m, prefix_len):
     ops = _ops()
