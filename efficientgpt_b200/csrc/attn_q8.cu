@@ -13,7 +13,8 @@
 // segment each (split by the smallest range length that gives every CTA at most one); else they are equal
 // stretches of the flat list of all tiles and may hold several segments (each counted with kExtra tiles more, about
 // what its start and end cost), cut inside a segment only if that is a long one, so that neither many short sequences
-// nor one token next to a document leave CTAs idle. Of a segment's part a warp takes every kWarps-th tile, through
+// nor one token next to a document leave CTAs idle. Many segments of a few tiles each go to the warps whole, which then
+// have nothing to add up (64 sequences of up to 32 keys, 8 kv heads: see make_layout). Of a segment's part a warp takes every kWarps-th tile, through
 // a ring of its own in shared memory (cp.async, rows past the segment's end filled with zeros), running ahead into the
 // next segment; warps only meet at a segment's end.
 //
@@ -76,6 +77,7 @@ struct Layout {
   int total, chunk;
   int pad;    // > 1: a segment takes up a multiple of pad (= chunk) places and every range lies in one segment
   int uncut;  // else equal stretches, and the tiles up to which a segment is not split
+  bool solo;  // no ranges: every warp takes whole segments of its own
 };
 struct Seg {
   int index, start, end, next;  // its number, its tiles in the flat list, and the place after it
@@ -193,12 +195,15 @@ __device__ __forceinline__ int ceil_div_small(int a, int b) {
 
 // cum[i] = places of the sequences before i (one kv head). The ranges: with up to 32 sequences the lanes try eight range
 // lengths from the even share of the tiles to 1.5 times it, and the smallest that gives at most one range per CTA is taken;
-// failing that, and for more sequences, equal stretches. Every thread of the CTA calls it.
+// failing that, and for more sequences, equal stretches, or whole segments to single warps where that takes less time: a
+// CTA's part of a segment costs about one round of its warps' tiles besides its rounds, a warp's half a tile besides
+// its tiles, and the slowest warp has the longest segments. Every thread of the CTA calls it.
 template <typename C>
 __device__ __forceinline__ Layout make_layout(const Params &p, int *cum, int *len_of, int *scratch) {
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, grid = (int)gridDim.x;
   Layout l;
-  l.pad = 1;
+  l.pad = 1, l.solo = false;
+  int segs = 0, rounds = 0, longest = 0;  // segments, their rounds and most tiles, of one kv head
   if (p.m <= 32) {  // every warp for itself
     const int keys = lane < p.m ? seq_len(p, lane) : 0, tiles = ceil_div(keys, C::kTile);
     bool fits = true;
@@ -217,6 +222,11 @@ __device__ __forceinline__ Layout make_layout(const Params &p, int *cum, int *le
       const unsigned good = __ballot_sync(0xffffffffu, p.nkv * parts <= grid);
       fits = good != 0u;
       if (fits) l.pad = __shfl_sync(0xffffffffu, len, __ffs(good) - 1);
+    }
+    if (!fits) {
+      segs = __popc(__ballot_sync(0xffffffffu, tiles > 0));
+      rounds = __reduce_add_sync(0xffffffffu, ceil_div(tiles, C::kWarps));
+      longest = __reduce_max_sync(0xffffffffu, tiles);
     }
     const int places = fits ? ceil_div_small(tiles, l.pad) * l.pad : (tiles ? tiles + C::kExtra : 0);
     int inc = places;
@@ -239,17 +249,28 @@ __device__ __forceinline__ Layout make_layout(const Params &p, int *cum, int *le
       len_of[i] = keys;
       places[e] = tiles ? tiles + C::kExtra : 0;
       sum += places[e];
+      segs += tiles > 0, rounds += ceil_div(tiles, C::kWarps), longest = max(longest, tiles);
     }
+    segs = __reduce_add_sync(0xffffffffu, segs), rounds = __reduce_add_sync(0xffffffffu, rounds);
+    longest = __reduce_max_sync(0xffffffffu, longest);
     int inc = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int up = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += up;
     }
-    if (lane == 31) scratch[warp] = inc;
+    if (lane == 31) {
+      scratch[warp] = inc;
+      scratch[C::kWarps + warp] = segs, scratch[2 * C::kWarps + warp] = rounds, scratch[3 * C::kWarps + warp] = longest;
+    }
     __syncthreads();
     int before = inc - sum;
     for (int w = 0; w < warp; ++w) before += scratch[w];
+    segs = rounds = longest = 0;
+    for (int w = 0; w < C::kWarps; ++w) {
+      segs += scratch[C::kWarps + w], rounds += scratch[2 * C::kWarps + w];
+      longest = max(longest, scratch[3 * C::kWarps + w]);
+    }
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
       cum[t * kPer + e] = before;
@@ -261,6 +282,10 @@ __device__ __forceinline__ Layout make_layout(const Params &p, int *cum, int *le
   l.total = p.nkv * cum[p.m];
   l.chunk = l.pad > 1 ? l.pad : max(1, ceil_div(l.total, grid));
   l.uncut = max(C::kMinChunk, l.chunk / 2);
+  if (l.pad == 1) {
+    const float by_cta = (float)(p.nkv * (segs + rounds)) / (float)grid;
+    l.solo = (float)ceil_div(p.nkv * segs, grid * C::kWarps) * (longest + 0.5f) < by_cta;
+  }
   return l;
 }
 template <int TILE>
@@ -333,7 +358,7 @@ struct Smem {
   float warp_m[kWarps][NR], warp_l[kWarps][NR];  // their maxima and sums
   float row_m[NR], row_l[NR];                    // and the CTA's
   int cum[kMaxBatch + 1], len[kMaxBatch];
-  int scratch[kWarps];
+  int scratch[4 * kWarps];
   int last[2];
 };
 
@@ -434,25 +459,46 @@ __global__ void __launch_bounds__(Cfg<Q8, NR>::kThreads, 1) attn_kernel(const Pa
   pdl_launch_dependents();
   Layout lay;
   if (PREFIX) {
-    lay.chunk = p.pre.chunk, lay.pad = p.pre.pad, lay.uncut = 0;
+    lay.chunk = p.pre.chunk, lay.pad = p.pre.pad, lay.uncut = 0, lay.solo = false;
     lay.total = p.nkv * p.pre.row_tiles * ceil_div(p.pre.seg_tiles, lay.pad) * lay.pad;
   } else {
     lay = make_layout<C>(p, sm.cum, sm.len, sm.scratch);
   }
   int x0 = (int)min((int64_t)lay.total, (int64_t)blockIdx.x * lay.chunk), x1 = min(lay.total, x0 + lay.chunk);
-  if (lay.pad == 1) {  // both cuts at once, in the even and in the odd lanes
+  const int stride = (int)gridDim.x * kWarps;  // whole segments to warps: every stride-th
+  int solo_seg = warp * (int)gridDim.x + (int)blockIdx.x;
+  if (lay.solo) {
+    while (solo_seg < p.m * p.nkv && sm.len[solo_seg / p.nkv] == 0) solo_seg += stride;
+    x0 = 0, x1 = solo_seg < p.m * p.nkv ? lay.total : 0;
+  } else if (lay.pad == 1) {  // both cuts at once, in the even and in the odd lanes
     const int cut = cut_at<TILE, PREFIX>(p, lay, sm.cum, sm.len, (int64_t)(blockIdx.x + (lane & 1)) * lay.chunk);
     x0 = __shfl_sync(0xffffffffu, cut, 0), x1 = __shfl_sync(0xffffffffu, cut, 1);
   }
   int split_n = 0;  // segments that this CTA shares with others: its first, its last
   int2 split[2] = {};  // their number and first CTA
   if (x0 < x1) {
-    Seg seg = find_seg<TILE, PREFIX>(p, sm.cum, sm.len, x0);
+    Seg seg;
+    if (!PREFIX && lay.solo) seg = own_seg<TILE>(p, sm.cum, sm.len, solo_seg / p.nkv, solo_seg % p.nkv);
+    else seg = find_seg<TILE, PREFIX>(p, sm.cum, sm.len, x0);
     if (lay.pad > 1) x1 = min(x1, seg.end);
+    const int first = lay.solo ? 0 : warp, step = lay.solo ? 1 : kWarps;  // this warp's tiles of a segment's part
+    auto advance = [&](Seg &s) -> bool {  // to the next segment of this CTA's range, or of this warp
+      if (!PREFIX && lay.solo) {
+        int i = s.index + stride;
+        while (i < p.m * p.nkv && sm.len[i / p.nkv] == 0) i += stride;
+        if (i >= p.m * p.nkv) return false;
+        s = own_seg<TILE>(p, sm.cum, sm.len, i / p.nkv, i % p.nkv);
+        return true;
+      }
+      if (s.next >= x1) return false;
+      s = next_seg<TILE, PREFIX>(p, sm.cum, sm.len, s);
+      return true;
+    };
 
-    // ---- this warp's loads: every kWarps-th tile of a segment's part, STAGES - 1 tiles ahead. 32 lanes take 512 consecutive bytes
-    // of a full tile at a time; the swizzles split into a part of the lane and one of the step.
-    int lx = x0 + warp, lslot = 0;
+    // ---- this warp's loads, STAGES - 1 tiles ahead. 32 lanes take 512 consecutive bytes of a full tile at a time; the
+    // swizzles split into a part of the lane and one of the step.
+    int lx = max(x0, seg.start) + first, lslot = 0;
+    bool more = true;
     Seg ls = seg;
     constexpr int kStep = 32 / G::kChunks;  // rows per 512 bytes
     const int lr = lane / G::kChunks, lc = lane % G::kChunks;
@@ -460,9 +506,9 @@ __global__ void __launch_bounds__(Cfg<Q8, NR>::kThreads, 1) attn_kernel(const Pa
     const uint32_t k_dst = ring + lr * G::kRowBytes + ((lc ^ G::k_swz(lr)) * 16);
     const uint32_t v_dst = lr * G::kRowBytes + ((lc ^ G::v_swz(lr)) * 16);
     auto load_next = [&]() {
-      while (lx >= ls.end && ls.next < x1) {
-        ls = next_seg<TILE, PREFIX>(p, sm.cum, sm.len, ls);
-        lx = ls.start + warp;
+      while (lx >= ls.end && more) {
+        more = advance(ls);
+        if (more) lx = ls.start + first;
       }
       if (lx < min(ls.end, x1)) {
         const uint32_t st = (uint32_t)(lslot * G::kStageBytes);
@@ -494,7 +540,7 @@ __global__ void __launch_bounds__(Cfg<Q8, NR>::kThreads, 1) attn_kernel(const Pa
         }
       }
       cp_commit();
-      lx += kWarps;
+      lx += step;
       lslot = lslot + 1 == STAGES ? 0 : lslot + 1;
     };
     // the segment's query rows, dims d0 .. d0 + 3 of every 16-dim step: those of the key words that this thread loads
@@ -583,7 +629,7 @@ __global__ void __launch_bounds__(Cfg<Q8, NR>::kThreads, 1) attn_kernel(const Pa
       for (int j = 0; j < ND; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
 
       const int seg_end = min(seg.end, x1);
-      for (int x = max(x0, seg.start) + warp; x < seg_end; x += kWarps) {
+      for (int x = max(x0, seg.start) + first; x < seg_end; x += step) {
         load_next();
         cp_wait<STAGES - 1>();
         __syncwarp();
@@ -741,7 +787,34 @@ __global__ void __launch_bounds__(Cfg<Q8, NR>::kThreads, 1) attn_kernel(const Pa
       for (int hh = 0; hh < NR / 8; ++hh) {
         l_part[hh] += __shfl_xor_sync(0xffffffffu, l_part[hh], 1);
         l_part[hh] += __shfl_xor_sync(0xffffffffu, l_part[hh], 2);
-        if (t == 0) sm.warp_m[warp][g + 8 * hh] = m_run[hh], sm.warp_l[warp][g + 8 * hh] = l_part[hh];
+        if (t == 0 && !lay.solo) sm.warp_m[warp][g + 8 * hh] = m_run[hh], sm.warp_l[warp][g + 8 * hh] = l_part[hh];
+      }
+      if (!PREFIX && lay.solo) {  // the warp's own: to the output, or a record in the segment's slot
+        float *rec = record<D>(p, seg.index);
+        uint16_t *out = p.out + seg.seq * p.ldo + (int64_t)seg.g * p.group * D;
+#pragma unroll
+        for (int hh = 0; hh < NR / 8; ++hh) {
+          const int r = g + 8 * hh;
+          if (r < p.group) {
+            const float inv = 1.f / l_part[hh];
+#pragma unroll
+            for (int j = 0; j < ND; j += 4)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const int c = 2 * hh + e, dim = r * D + G::out_dim(j, e, t);
+                if (MODE == kOwn)
+                  *(uint2 *)(out + dim) = make_uint2(bf16x2(acc[j][c] * inv, acc[j + 1][c] * inv),
+                                                     bf16x2(acc[j + 2][c] * inv, acc[j + 3][c] * inv));
+                else
+                  *(float4 *)(rec + dim) = make_float4(acc[j][c], acc[j + 1][c], acc[j + 2][c], acc[j + 3][c]);
+              }
+            if (MODE != kOwn && t == 0) rec[kRows * D + r] = m_run[hh], rec[kRows * D + kRows + r] = l_part[hh];
+          }
+        }
+        if (MODE == kBeside && lane == 0) p.parts[seg.index] = make_int2(seg.index, 1);
+        if (!advance(seg)) break;
+        load_q(seg);
+        continue;
       }
       __syncthreads();
       float fac[NR / 8];
@@ -806,8 +879,7 @@ __global__ void __launch_bounds__(Cfg<Q8, NR>::kThreads, 1) attn_kernel(const Pa
           p.parts[seg.index] = make_int2(whole ? (int)blockIdx.x + seg.index : c0 + seg.index, whole ? 1 : c1 - c0 + 1);
         }
       }
-      if (seg.next >= x1) break;
-      seg = next_seg<TILE, PREFIX>(p, sm.cum, sm.len, seg);
+      if (!advance(seg)) break;
       load_q(seg);
     }
     cp_wait<0>();

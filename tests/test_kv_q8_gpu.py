@@ -334,6 +334,25 @@ def test_shared_prefix(cuda, q8, d, nq, nkv, m, prefix_len):
     assert L.device_error() == 0
 
 
+@pytest.mark.parametrize('q8', [False, True])
+@pytest.mark.parametrize('nq,nkv,m', [(32, 8, 64), (40, 20, 30), (32, 2, 300)])
+def test_many_short_tails(cuda, q8, nq, nkv, m):
+    """Enough short segments that every warp takes its own (idle slots among them), on the way to the output and to the
+    records that are added to a prefix's."""
+    ops = _ops()
+    gen = _gen(m + q8)
+    d, cap, prefix_len = 128, 40, 150
+    lengths = [(1, 0, 7, 32, 33, 16, 40)[i % 7] for i in range(m)]
+    prefix, own = _cache(gen, nkv, prefix_len, d, q8), _cache(gen, m * nkv, cap, d, q8)
+    for i, n in enumerate(lengths):
+        _poison(own, slice(i * nkv, (i + 1) * nkv), n)
+    q = _randn(gen, m, nq * d).bfloat16()
+    pos = torch.tensor(lengths, device=cuda) - 1
+    for p in (prefix_len, 0):
+        out = ops.attn_shared_prefix(q, prefix, own, pos, p, nq, nkv, d, scale=d ** -0.5)
+        _check(out, q, nq, nkv, d, d ** -0.5, lengths, own, prefix, p)
+
+
 def test_shared_prefix_is_the_decode_of_the_joined_caches(cuda):
     """A prefix shared by all rows or copied in front of every row's own keys: the same attention."""
     ops = _ops()
