@@ -19,7 +19,7 @@
 //   warps 10-13 (int8): widen a code tile to bf16, exactly, one key per thread, into the operand rings, and put the
 //             block's scales (the keys' times scale log2(e)) beside them: a key's scale multiplies its column of scores,
 //             a value's its column of weights.
-// A stream ends with a partial record (unnormalised output, maximum, sum of each row) for add_kernel. With bf16 caches
+// A row tile's range ends with a partial record (unnormalised output, maximum, sum of each row) for add_kernel. With bf16 caches
 // weights enter P.V as bf16 relative to the maximum in use, as in the other bf16 attention kernels; with int8 caches as
 // the sum of two bf16 values (16 bits), a second P.V: the values' own rounding is then the only one that counts.
 // Everything else is fp32. Every wait is bounded; issued loads and MMAs are drained before the CTA exits.
@@ -54,7 +54,7 @@ struct Args {
   CUtensorMap vmap;
   const float *ks, *vs;  // int8: [nkv][cap]
   int64_t cap;
-  float *ws;         // records [nkv][pairs][ranges][2 streams]
+  float *ws;         // records [nkv][pairs][ranges][2 row tiles]
   int64_t prefix;
   int m, nkv, group;
   int seqs;          // sequences per row tile: 128 / group
@@ -66,6 +66,20 @@ __device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
+}
+// Shared memory by its own addresses (a pointer that is one of two places is a generic one to the compiler).
+__device__ __forceinline__ ulonglong2 lds_2x64(uint32_t at) {
+  ulonglong2 r;
+  asm volatile("ld.shared.v2.u64 {%0, %1}, [%2];" : "=l"(r.x), "=l"(r.y) : "r"(at));
+  return r;
+}
+__device__ __forceinline__ uint4 lds_4x32(uint32_t at) {
+  uint4 r;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(at));
+  return r;
+}
+__device__ __forceinline__ void sts_4x32(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 // The bf16 values of two codes, exactly (as codes_bf16 of attn_q8.cu).
 __device__ __forceinline__ uint32_t widen2(uint32_t codes, uint32_t select) {
@@ -248,7 +262,7 @@ __global__ void __launch_bounds__(Cfg<D, Q8>::kThreads, 1) attn_prefix_kernel(co
         if (Q8) ok = ok && apf::warp_wait(scale_full + b % scale_slots, (unsigned)(b / scale_slots) & 1u);
         if (!ok) break;
         gtc::tc_fence_after();
-        const float *ks = scale_of(b), *vs = ks + kBK;
+        const uint32_t ks = Q8 ? smem_u32(scale_of(b)) : 0u, vs = ks + kBK * 4;
         const uint64_t one2 = apf::f2_pack(A.scale_log2, A.scale_log2);
         const int left = (int)min((int64_t)kBK, A.prefix - (int64_t)(b0 + b) * kBK);
         auto mask = [&](int c, uint32_t *sc) {  // -inf past the prefix
@@ -263,7 +277,7 @@ __global__ void __launch_bounds__(Cfg<D, Q8>::kThreads, 1) attn_prefix_kernel(co
           if constexpr (Q8) {
 #pragma unroll
             for (int e = 0; e < 32; e += 4) {
-              const ulonglong2 f = *(const ulonglong2 *)(ks + c + e);
+              const ulonglong2 f = lds_2x64(ks + (uint32_t)(c + e) * 4);
               const float2 x = apf::f2_unpack(f2_mul(apf::f2_pack(__uint_as_float(sc[e]), __uint_as_float(sc[e + 1])), f.x));
               const float2 y = apf::f2_unpack(f2_mul(apf::f2_pack(__uint_as_float(sc[e + 2]), __uint_as_float(sc[e + 3])), f.y));
               sc[e] = __float_as_uint(x.x), sc[e + 1] = __float_as_uint(x.y);
@@ -306,14 +320,20 @@ __global__ void __launch_bounds__(Cfg<D, Q8>::kThreads, 1) attn_prefix_kernel(co
         auto weights = [&](int c, const uint32_t *sc) {
           uint32_t pk[16], pl[Q8 ? 16 : 1];
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            const uint64_t raw = apf::f2_pack(__uint_as_float(sc[e]), __uint_as_float(sc[e + 1]));
-            const float2 x = apf::f2_unpack(Q8 ? apf::f2_add(raw, nm2) : apf::f2_fma(raw, one2, nm2));
-            float2 w = make_float2(apf::ex2(x.x), apf::ex2(x.y));
-            sum[(e >> 1) & 1] = apf::f2_add(sum[(e >> 1) & 1], apf::f2_pack(w.x, w.y));
-            if (Q8) w = apf::f2_unpack(f2_mul(apf::f2_pack(w.x, w.y), *(const uint64_t *)(vs + c + e)));
-            pk[e / 2] = gtc::pack_bf16x2(w.x, w.y);
-            if constexpr (Q8) pl[e / 2] = gtc::pack_bf16x2(w.x - bf16_lo(pk[e / 2]), w.y - bf16_hi(pk[e / 2]));
+          for (int e = 0; e < 32; e += 4) {
+            ulonglong2 vf = make_ulonglong2(0ull, 0ull);
+            if constexpr (Q8) vf = lds_2x64(vs + (uint32_t)(c + e) * 4);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int k = e + 2 * h;
+              const uint64_t raw = apf::f2_pack(__uint_as_float(sc[k]), __uint_as_float(sc[k + 1]));
+              const float2 x = apf::f2_unpack(Q8 ? apf::f2_add(raw, nm2) : apf::f2_fma(raw, one2, nm2));
+              float2 w = make_float2(apf::ex2(x.x), apf::ex2(x.y));
+              sum[h] = apf::f2_add(sum[h], apf::f2_pack(w.x, w.y));
+              if constexpr (Q8) w = apf::f2_unpack(f2_mul(apf::f2_pack(w.x, w.y), h ? vf.y : vf.x));
+              pk[k / 2] = gtc::pack_bf16x2(w.x, w.y);
+              if constexpr (Q8) pl[k / 2] = gtc::pack_bf16x2(w.x - bf16_lo(pk[k / 2]), w.y - bf16_hi(pk[k / 2]));
+            }
           }
           apf::tmem_st16(ts + (uint32_t)(c / 2), pk);
           if constexpr (Q8) apf::tmem_st16(ts + (uint32_t)(64 + c / 2), pl);
@@ -350,28 +370,65 @@ __global__ void __launch_bounds__(Cfg<D, Q8>::kThreads, 1) attn_prefix_kernel(co
         gtc::tc_fence_before();
         gtc::mbar_arrive(p_full + s);
       }
-      if (ok && apf::warp_wait(o_done + s, 0)) {
-        gtc::tc_fence_after();
+      // ---- the record. Once both streams are done the operand tiles are free: a warp's rows go through a place of its
+      // own there, so that they leave in whole lines; alternate blocks' two states are added up first.
+      ok = ok && apf::warp_wait(o_done, 0) && (!steps[1] || apf::warp_wait(o_done + 1, 0));
+      gtc::tc_fence_after();
+      constexpr int kPitch = D + 4;  // floats of a staged row
+      float *stage = (float *)sk + (size_t)(two ? 4 * s + quarter : quarter) * 32 * kPitch;
+      const bool merge = !two && steps[1];
+      float f0 = 1.f, f1 = 0.f;
+      const float *other = stage + lane * kPitch;
+      if (merge) {
+        // stream 1's state to shared memory (maximum and sum in the row's padding), stream 0 takes it
+        if (s == 1 && ok) {
+#pragma unroll
+          for (int c = 0; c < D; c += 32) {
+            uint32_t o[32];
+            apf::tmem_ld32(to + (uint32_t)c, o);
+            apf::tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              *(uint4 *)(stage + lane * kPitch + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          }
+          *(float2 *)(stage + lane * kPitch + D) = make_float2(m_run, l_sum);
+        }
+        asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");  // the quarter's two warps, whatever their waits returned
+        if (s == 0) {
+          const float2 ml = *(const float2 *)(other + D);
+          const float mx = fmaxf(m_run, ml.x), mz = mx == -INFINITY ? 0.f : mx;
+          f0 = apf::ex2(m_run - mz), f1 = apf::ex2(ml.x - mz);
+          m_run = mx, l_sum = l_sum * f0 + ml.y * f1;
+        }
+      }
+      if (ok && !(merge && s == 1)) {
         float *rec = A.ws + ((int64_t)blockIdx.x * 2 + s) * record_size(D);
 #pragma unroll
         for (int c = 0; c < D; c += 32) {
           uint32_t o[32];
           apf::tmem_ld32(to + (uint32_t)c, o);
           apf::tmem_wait_ld();
-          if (row < rows[s]) {
 #pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              *(uint4 *)(rec + row * D + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          for (int e = 0; e < 32; e += 4) {
+            float *at = stage + lane * kPitch + c + e;
+            float4 v = make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 1]), __uint_as_float(o[e + 2]),
+                                   __uint_as_float(o[e + 3]));
+            if (merge) {
+              const float4 w = *(const float4 *)at;
+              v = make_float4(v.x * f0 + w.x * f1, v.y * f0 + w.y * f1, v.z * f0 + w.z * f1, v.w * f0 + w.w * f1);
+            }
+            *(float4 *)at = v;
           }
+        }
+        __syncwarp();
+#pragma unroll 4
+        for (int k = 0; k < D / 4; ++k) {  // 512 consecutive bytes at a time
+          const int r = (128 * k + 4 * lane) / D, c = (128 * k + 4 * lane) % D;
+          if (32 * quarter + r < rows[s]) *(float4 *)(rec + (32 * quarter + r) * D + c) = *(const float4 *)(stage + r * kPitch + c);
         }
         rec[kRowsT * D + row] = m_run;
         rec[kRowsT * D + kRowsT + row] = l_sum;
       }
-    }
-    if (!steps[s]) {  // a range of one block: the second stream has no record to add
-      float *rec = A.ws + ((int64_t)blockIdx.x * 2 + s) * record_size(D);
-      rec[kRowsT * D + row] = -INFINITY;
-      rec[kRowsT * D + kRowsT + row] = 0.f;
     }
   } else if constexpr (Q8) {
     // ---------------------------------------------------------------- widening: one key per thread
@@ -379,17 +436,17 @@ __global__ void __launch_bounds__(Cfg<D, Q8>::kThreads, 1) attn_prefix_kernel(co
     auto widen = [&](int u, uint8_t *dst) -> bool {  // code tile u to an operand tile
       const int slot = u % raws;
       if (!gtc::mbar_wait(raw_full + slot, (unsigned)(u / raws) & 1u)) return false;
-      const uint8_t *src = raw_tile(slot) + r * D;
+      const uint32_t src = smem_u32(raw_tile(slot)) + r * D, to = smem_u32(dst) + r * 128;
       const int swz = D == 128 ? (r & 7) : ((r >> 1) & 3);  // the map's 128- or 64-byte swizzle
 #pragma unroll
       for (int c = 0; c < D / 16; ++c) {
-        const uint4 w = *(const uint4 *)(src + ((c ^ swz) * 16));
-        uint8_t *half = dst + (c >> 2) * kHalf + r * 128;
+        const uint4 w = lds_4x32(src + ((c ^ swz) * 16));
+        const uint32_t half = to + (c >> 2) * kHalf;
         const int cc = 2 * (c & 3);
-        *(uint4 *)(half + ((cc ^ (r & 7)) * 16)) =
-            make_uint4(widen2(w.x, 0x4140), widen2(w.x, 0x4342), widen2(w.y, 0x4140), widen2(w.y, 0x4342));
-        *(uint4 *)(half + (((cc + 1) ^ (r & 7)) * 16)) =
-            make_uint4(widen2(w.z, 0x4140), widen2(w.z, 0x4342), widen2(w.w, 0x4140), widen2(w.w, 0x4342));
+        sts_4x32(half + ((cc ^ (r & 7)) * 16), widen2(w.x, 0x4140), widen2(w.x, 0x4342), widen2(w.y, 0x4140),
+                 widen2(w.y, 0x4342));
+        sts_4x32(half + (((cc + 1) ^ (r & 7)) * 16), widen2(w.z, 0x4140), widen2(w.z, 0x4342), widen2(w.w, 0x4140),
+                 widen2(w.w, 0x4342));
       }
       gtc::mbar_arrive(raw_empty + slot);
       return true;

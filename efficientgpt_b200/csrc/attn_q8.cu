@@ -52,7 +52,7 @@ struct Cache {
 struct Prefix {
   const float *rec;                // null: no prefix
   int big;                         // 1: attn_prefix_kernel's
-  int seqs, tiles, pairs, ranges;  // its shape
+  int seqs, pairs, ranges;         // its shape
   int row_tiles, pad, chunk, seg_tiles;  // else the list of prefix segments, cut as below
 };
 
@@ -782,6 +782,9 @@ __global__ void __launch_bounds__(Cfg<Q8, NR>::kThreads, 1) attn_kernel(const Pa
 #pragma unroll
         for (int j = 0; j < ND; ++j) acc[j][0] += acc[j][2], acc[j][1] += acc[j][3];
       }
+      const Seg done = seg;
+      const bool another = advance(seg);
+      if (another) load_q(seg);  // on its way while this one is added up
       // ---- the segment is done: the warps' states, each relative to the largest maximum, are added up in shared memory
 #pragma unroll
       for (int hh = 0; hh < NR / 8; ++hh) {
@@ -790,8 +793,8 @@ __global__ void __launch_bounds__(Cfg<Q8, NR>::kThreads, 1) attn_kernel(const Pa
         if (t == 0 && !lay.solo) sm.warp_m[warp][g + 8 * hh] = m_run[hh], sm.warp_l[warp][g + 8 * hh] = l_part[hh];
       }
       if (!PREFIX && lay.solo) {  // the warp's own: to the output, or a record in the segment's slot
-        float *rec = record<D>(p, seg.index);
-        uint16_t *out = p.out + seg.seq * p.ldo + (int64_t)seg.g * p.group * D;
+        float *rec = record<D>(p, done.index);
+        uint16_t *out = p.out + done.seq * p.ldo + (int64_t)done.g * p.group * D;
 #pragma unroll
         for (int hh = 0; hh < NR / 8; ++hh) {
           const int r = g + 8 * hh;
@@ -811,9 +814,8 @@ __global__ void __launch_bounds__(Cfg<Q8, NR>::kThreads, 1) attn_kernel(const Pa
             if (MODE != kOwn && t == 0) rec[kRows * D + r] = m_run[hh], rec[kRows * D + kRows + r] = l_part[hh];
           }
         }
-        if (MODE == kBeside && lane == 0) p.parts[seg.index] = make_int2(seg.index, 1);
-        if (!advance(seg)) break;
-        load_q(seg);
+        if (MODE == kBeside && lane == 0) p.parts[done.index] = make_int2(done.index, 1);
+        if (!another) break;
         continue;
       }
       __syncthreads();
@@ -834,10 +836,10 @@ __global__ void __launch_bounds__(Cfg<Q8, NR>::kThreads, 1) attn_kernel(const Pa
           l += sm.warp_l[w][threadIdx.x] * ex2(sm.warp_m[w][threadIdx.x] - (mx == -INFINITY ? 0.f : mx));
         sm.row_m[threadIdx.x] = mx, sm.row_l[threadIdx.x] = l;
       }
-      const bool whole = seg.start >= x0 && seg.end <= x1;
+      const bool whole = done.start >= x0 && done.end <= x1;
       const bool final = MODE == kOwn && whole;
       const int rows = PREFIX ? kRows : p.group;
-      float *rec = record<D>(p, (int)blockIdx.x + seg.index);
+      float *rec = record<D>(p, (int)blockIdx.x + done.index);
       constexpr int kPass = S::kPass;
 #pragma unroll 1
       for (int r0 = 0; r0 < rows; r0 += kPass) {
@@ -862,7 +864,7 @@ __global__ void __launch_bounds__(Cfg<Q8, NR>::kThreads, 1) attn_kernel(const Pa
           float a = 0.f;
 #pragma unroll
           for (int w = 0; w < kWarps; ++w) a += sm.merge[w][e / D][e % D];
-          if (final) p.out[seg.seq * p.ldo + (int64_t)(seg.g * p.group + r0) * D + e] = f32_to_bf16_bits(a / sm.row_l[r0 + e / D]);
+          if (final) p.out[done.seq * p.ldo + (int64_t)(done.g * p.group + r0) * D + e] = f32_to_bf16_bits(a / sm.row_l[r0 + e / D]);
           else rec[r0 * D + e] = a;
         }
       }
@@ -871,16 +873,15 @@ __global__ void __launch_bounds__(Cfg<Q8, NR>::kThreads, 1) attn_kernel(const Pa
         rec[kRows * D + kRows + threadIdx.x] = sm.row_l[threadIdx.x];
       }
       if (MODE != kPrefix && !final) {
-        const int c0 = seg.start / lay.chunk, c1 = (seg.end - 1) / lay.chunk;
+        const int c0 = done.start / lay.chunk, c1 = (done.end - 1) / lay.chunk;
         if (MODE == kOwn) {
-          (split_n ? split[1] : split[0]) = make_int2(seg.index, c0);
+          (split_n ? split[1] : split[0]) = make_int2(done.index, c0);
           ++split_n;
-        } else if (seg.start >= x0 && threadIdx.x == 0) {  // (a short segment lies in one CTA wherever the even cuts are)
-          p.parts[seg.index] = make_int2(whole ? (int)blockIdx.x + seg.index : c0 + seg.index, whole ? 1 : c1 - c0 + 1);
+        } else if (done.start >= x0 && threadIdx.x == 0) {  // (a short segment lies in one CTA wherever the even cuts are)
+          p.parts[done.index] = make_int2(whole ? (int)blockIdx.x + done.index : c0 + done.index, whole ? 1 : c1 - c0 + 1);
         }
       }
-      if (!advance(seg)) break;
-      load_q(seg);
+      if (!another) break;
     }
     cp_wait<0>();
   }
@@ -957,11 +958,9 @@ __global__ void __launch_bounds__(32 * kAddWarps) add_kernel(const Params p) {
   int64_t pre_step;
   if (p.pre.big) {
     const int tile = i / p.pre.seqs, pair = tile / 2;
-    const bool two = 2 * pair + 1 < p.pre.tiles;  // the pair's streams are two tiles, or both this one
-    pre_n = two ? p.pre.ranges : 2 * p.pre.ranges;
-    pre_step = (two ? 2 : 1) * apx::record_size(D);
+    pre_n = p.pre.ranges, pre_step = 2 * apx::record_size(D);
     pre_row = (i - tile * p.pre.seqs) * p.group + j, pre_rows = apx::kRowsT;
-    pre0 = p.pre.rec + ((int64_t)(g * p.pre.pairs + pair) * p.pre.ranges * 2 + (two ? tile & 1 : 0)) * apx::record_size(D);
+    pre0 = p.pre.rec + ((int64_t)(g * p.pre.pairs + pair) * p.pre.ranges * 2 + (tile & 1)) * apx::record_size(D);
   } else {
     const int flat = i * p.group + j, seg = g * p.pre.row_tiles + flat / kRows;
     const int start = seg * ceil_div(p.pre.seg_tiles, p.pre.pad) * p.pre.pad;
@@ -972,7 +971,7 @@ __global__ void __launch_bounds__(32 * kAddWarps) add_kernel(const Params p) {
     pre0 = p.pre.rec + (int64_t)(c0 + seg) * pre_step;
   }
   float a[D / 32];
-  add_records<D, true, 16>(record<D>(p, own.x) + j * D, own.y, j, pre0 + pre_row * D, pre_n, pre_step, pre_row, pre_rows,
+  add_records<D, true, 8>(record<D>(p, own.x) + j * D, own.y, j, pre0 + pre_row * D, pre_n, pre_step, pre_row, pre_rows,
                            0, 1, a);
   store_row(p.out + i * p.ldo + (int64_t)h * D + D / 32 * lane, a);
 }
@@ -1129,7 +1128,7 @@ extern "C" int egpt_attn_shared_prefix(void *out, int64_t ldo, const void *q, in
                                            : apx::launch<64, false>(A, q, ldq, pk, pv, sh, st, pdl, maps_ok));
       if (!maps_ok) return set_error(EGPT_ERR_ALIGN, "attn_shared_prefix: tensor maps rejected");
       if (e != cudaSuccess) return check_launch(e, "attn_prefix_kernel");
-      p.pre.big = 1, p.pre.seqs = sh.seqs, p.pre.tiles = sh.tiles, p.pre.pairs = sh.pairs, p.pre.ranges = sh.ranges;
+      p.pre.big = 1, p.pre.seqs = sh.seqs, p.pre.pairs = sh.pairs, p.pre.ranges = sh.ranges;
     } else {
       aq8::Params a = p;
       a.cache = {(const uint8_t *)pk, (const uint8_t *)pv, pk_scale, pv_scale, prefix_cap};
