@@ -370,8 +370,8 @@ __global__ void __launch_bounds__(Cfg<D, Q8>::kThreads, 1) attn_prefix_kernel(co
         gtc::tc_fence_before();
         gtc::mbar_arrive(p_full + s);
       }
-      // ---- the record. Once both streams are done the operand tiles are free: a warp's rows go through a place of its
-      // own there, so that they leave in whole lines; alternate blocks' two states are added up first.
+      // ---- the record. Once both streams are done the operand tiles are free: a row goes through a place of its own
+      // there and leaves in one bulk copy; alternate blocks' two states are added up first.
       ok = ok && apf::warp_wait(o_done, 0) && (!steps[1] || apf::warp_wait(o_done + 1, 0));
       gtc::tc_fence_after();
       constexpr int kPitch = D + 4;  // floats of a staged row
@@ -420,11 +420,13 @@ __global__ void __launch_bounds__(Cfg<D, Q8>::kThreads, 1) attn_prefix_kernel(co
             *(float4 *)at = v;
           }
         }
-        __syncwarp();
-#pragma unroll 4
-        for (int k = 0; k < D / 4; ++k) {  // 512 consecutive bytes at a time
-          const int r = (128 * k + 4 * lane) / D, c = (128 * k + 4 * lane) % D;
-          if (32 * quarter + r < rows[s]) *(float4 *)(rec + (32 * quarter + r) * D + c) = *(const float4 *)(stage + r * kPitch + c);
+        if (row < rows[s]) {  // the row's own copy engine transfer
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(rec + row * D),
+                       "r"(smem_u32(stage + lane * kPitch)), "n"(D * 4)
+                       : "memory");
+          asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         }
         rec[kRowsT * D + row] = m_run;
         rec[kRowsT * D + kRowsT + row] = l_sum;
@@ -485,7 +487,8 @@ __global__ void __launch_bounds__(Cfg<D, Q8>::kThreads, 1) attn_prefix_kernel(co
   }
 }
 
-// Row tiles, their pairs, and key ranges per kv head and pair: about one CTA per SM, at least two blocks to a range.
+// Row tiles, their pairs, and key ranges per kv head and pair: about one CTA per SM, at least four blocks to a range
+// (a range costs about 5 us besides its blocks, and its record has to be added up).
 struct Shape {
   int seqs, tiles, pairs, ranges;
 };
@@ -495,7 +498,7 @@ static Shape shape_of(int64_t m, int group, int nkv, int64_t prefix) {
   s.tiles = (int)((m + s.seqs - 1) / s.seqs);
   s.pairs = (s.tiles + 1) / 2;
   const int64_t blocks = (prefix + kBK - 1) / kBK;
-  s.ranges = (int)std::max<int64_t>(1, std::min<int64_t>(num_sms() / ((int64_t)nkv * s.pairs), (blocks + 1) / 2));
+  s.ranges = (int)std::max<int64_t>(1, std::min<int64_t>(num_sms() / ((int64_t)nkv * s.pairs), (blocks + 3) / 4));
   return s;
 }
 // Floats of the records of any prefix: as many ranges as the SMs allow.

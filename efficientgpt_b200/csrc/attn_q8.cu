@@ -51,6 +51,7 @@ struct Cache {
 // The prefix's partial records, by the kernel that made them.
 struct Prefix {
   const float *rec;                // null: no prefix
+  int grid;                        // its CTAs
   int big;                         // 1: attn_prefix_kernel's
   int seqs, pairs, ranges;         // its shape
   int row_tiles, pad, chunk, seg_tiles;  // else the list of prefix segments, cut as below
@@ -971,7 +972,7 @@ __global__ void __launch_bounds__(32 * kAddWarps) add_kernel(const Params p) {
     pre0 = p.pre.rec + (int64_t)(c0 + seg) * pre_step;
   }
   float a[D / 32];
-  add_records<D, true, 8>(record<D>(p, own.x) + j * D, own.y, j, pre0 + pre_row * D, pre_n, pre_step, pre_row, pre_rows,
+  add_records<D, true, 10>(record<D>(p, own.x) + j * D, own.y, j, pre0 + pre_row * D, pre_n, pre_step, pre_row, pre_rows,
                            0, 1, a);
   store_row(p.out + i * p.ldo + (int64_t)h * D + D / 32 * lane, a);
 }
@@ -993,11 +994,13 @@ static cudaError_t launch(const Params &p, int grid, cudaStream_t st, bool pdl) 
 
 static int row_tiles(int64_t m, int group) { return (int)((m * group + kRows - 1) / kRows); }
 static int max_grid() { return num_sms(); }
-// CTAs that the sequences' own keys can need: no more than their ranges if each has the fewest keys a range may have.
+// CTAs that the sequences' own keys can need: no more than their ranges if each has the fewest keys a range may have;
+// beside a prefix on less than half of the SMs, those that it leaves free (neither kernel shares an SM).
 template <typename C>
 static int own_grid(const Params &p) {
+  const int free = max_grid() - p.pre.grid;
   const int64_t most = ((p.cache.cap + C::kTile - 1) / C::kTile + C::kMinChunk - 1) / C::kMinChunk;
-  return (int)std::min<int64_t>(max_grid(), most * p.m * p.nkv);
+  return (int)std::min<int64_t>(free >= max_grid() / 2 ? free : max_grid(), most * p.m * p.nkv);
 }
 // How the prefix's segments are cut: as make_layout does it, on the host; returns the grid.
 template <typename C>
@@ -1015,7 +1018,7 @@ static int cut_prefix(Params &p) {
       break;
     }
   }
-  return ceil_div(segs * ceil_div(c.seg_tiles, c.pad) * c.pad, c.chunk);
+  return c.grid = ceil_div(segs * ceil_div(c.seg_tiles, c.pad) * c.pad, c.chunk);
 }
 template <bool Q8, int NR, Mode MODE>
 static cudaError_t launch_d(Params &p, int d, cudaStream_t st, bool pdl) {
@@ -1029,9 +1032,16 @@ static cudaError_t launch_any(Params &p, int d, bool q8, int rows, cudaStream_t 
   if (rows <= 8) return q8 ? launch_d<true, 8, MODE>(p, d, st, pdl) : launch_d<false, 8, MODE>(p, d, st, pdl);
   return q8 ? launch_d<true, 16, MODE>(p, d, st, pdl) : launch_d<false, 16, MODE>(p, d, st, pdl);
 }
-// Whether the prefix goes to attn_prefix_kernel: head_dim 64 or 128 and more rows than one tile of the mma.sync kernel.
-static bool prefix_on_tcgen05(const Params &p, int d) {
-  return d >= 64 && p.scale_log2 > 0.f && p.m * p.group > kRows;
+// Whether the prefix goes to attn_prefix_kernel (head_dim 64 or 128) or to the mma.sync kernel's 16-row tiles, whose time
+// grows with rows x keys: above 1.5 million (query head, key) pairs of the batch for bf16, and for int8, whose tiles the
+// tcgen05 kernel has to widen first, above 3.5 million and 64 rows. Whole calls in us, tcgen05 / mma.sync, rows of
+// each of 8 kv heads at head_dim 128:
+//              64 rows, keys 1024, 4096, 16384     128 rows                         256 rows
+//   bf16       15.3/12.3  17.5/20.6  27.7/43.8     16.6/16.4  18.3/28.2  28.5/72.8   21.9/20.5  24.2/43.2  38.8/131.9
+//   int8       22.9/13.8  25.8/24.0  51.4/49.5     23.4/18.9  26.5/31.8  51.9/79.9   33.5/23.2  35.5/47.8  65.8/141.6
+static bool prefix_on_tcgen05(const Params &p, int64_t keys, int d, bool q8) {
+  const int64_t rows = (int64_t)p.m * p.group, pairs = rows * p.nkv * keys;
+  return d >= 64 && p.scale_log2 > 0.f && (q8 ? rows > 64 && pairs > 3500000 : rows > kRows && pairs > 1500000);
 }
 // Arrival counters, then the (first record, records) pairs of the segments.
 static size_t counter_bytes(int64_t m, int nkv) { return ((size_t)m * nkv * 16 + 255) / 256 * 256; }
@@ -1116,7 +1126,7 @@ extern "C" int egpt_attn_shared_prefix(void *out, int64_t ldo, const void *q, in
   p.ws = (float *)((char *)ws + aq8::counter_bytes(m, nkv));
   float *pre_rec = p.ws + ((size_t)aq8::max_grid() + (size_t)m * nkv) * aq8::kRows * (d + 2);
   if (prefix_len > 0) {
-    if (aq8::prefix_on_tcgen05(p, d)) {
+    if (aq8::prefix_on_tcgen05(p, prefix_len, d, q8)) {
       apx::Args A{};
       const apx::Shape sh = apx::shape_of(m, p.group, nkv, prefix_len);
       A.ws = pre_rec, A.prefix = prefix_len, A.m = (int)m, A.nkv = nkv, A.group = p.group, A.scale_log2 = p.scale_log2;
@@ -1128,6 +1138,7 @@ extern "C" int egpt_attn_shared_prefix(void *out, int64_t ldo, const void *q, in
                                            : apx::launch<64, false>(A, q, ldq, pk, pv, sh, st, pdl, maps_ok));
       if (!maps_ok) return set_error(EGPT_ERR_ALIGN, "attn_shared_prefix: tensor maps rejected");
       if (e != cudaSuccess) return check_launch(e, "attn_prefix_kernel");
+      p.pre.grid = nkv * sh.pairs * sh.ranges;
       p.pre.big = 1, p.pre.seqs = sh.seqs, p.pre.pairs = sh.pairs, p.pre.ranges = sh.ranges;
     } else {
       aq8::Params a = p;
