@@ -9,28 +9,37 @@
 // Work: a segment is one cache head with the query rows that read it: (i, g) with the group's rows for a sequence's
 // own cache, (g, 16 query rows) for the shared prefix, whose rows are all (sequence, head) pairs of kv head g in a
 // row. A segment's keys are cut into tiles of kTile keys and the tiles of a launch into contiguous ranges, one per CTA,
-// on the device, so no length is known to the host. Where the segments allow it ranges are parts of one
-// segment each (split by the smallest range length that gives every CTA at most one); else they are equal
-// stretches of the flat list of all tiles and may hold several segments (each counted with kExtra tiles more, about
-// what its start and end cost), cut inside a segment only if that is a long one, so that neither many short sequences
-// nor one token next to a document leave CTAs idle. Many segments of a few tiles each go to the warps whole, which then
-// have nothing to add up (64 sequences of up to 32 keys, 8 kv heads: see make_layout). Of a segment's part a warp takes every kWarps-th tile, through
-// a ring of its own in shared memory (cp.async, rows past the segment's end filled with zeros), running ahead into the
+// on the device, so no length is known to the host. Where the segments allow it ranges are parts of one segment each
+// (split by the smallest range length that gives every CTA at most one); else they are equal stretches of the flat
+// list of all tiles and may hold several segments (each counted with kExtra tiles more, about what its start and
+// end cost), cut inside a segment only if that is a long one, so that neither many short sequences nor one token
+// next to a document leave CTAs idle. Many segments of a few tiles each go to the warps whole, which then have
+// nothing to add up (make_layout weighs it). Of a segment's part a warp takes every kWarps-th tile, through a ring
+// of its own in shared memory (cp.async, rows past the segment's end filled with zeros), running ahead into the
 // next segment; warps only meet at a segment's end.
 //
 // A prefix runs first, in a launch of its own that leaves partial records (here, or in attn_prefix.cu); the launch over
 // the sequences' own keys is a dependent one that starts beside it and leaves records too, and a third adds both up,
 // a warp to a row.
 //
-// Arithmetic: mma.sync with the query rows as M. Scores of int8 keys, up to 8 rows: q as fixed point X 2^(e - 29), |X| <=
-// 2^30, in four balanced base-256 digits, two of them in the MMA's rows 0-7 and 8-15, so two int8 MMAs per 32 dims
-// give the exact dot products with the codes as they lie in memory, and ks_j multiplies their fp32 value. 16 rows: the
-// codes become f16 exactly (0x6400 | (q + 128) is 1152 + q), and q, scaled by a power of two per row to at most 2^15,
-// too, so the sums are those of the codes in fp32. P.V is in bf16, whose exponents hold every weight times vs_j; its 8 bits
-// would cost a weight 2^-9 of itself, so a weight enters as the sum of two bf16 values (16 bits). With 8 query rows
-// or fewer the second values ride in the MMA's upper 8 rows, which are idle otherwise; 16 rows take a second MMA.
-// Codes become bf16 exactly as (128 + low seven bits) - (128 + sign bit). Sums, maxima and accumulators are fp32; the
-// output is rounded once.
+// Arithmetic: mma.sync with the query rows as M. Scores of int8 keys, up to 8 rows: q as fixed point X 2^(e - 29),
+// |X| <= 2^30, in four balanced base-256 digits, two of them in the MMA's rows 0-7 and 8-15, so two int8 MMAs per 32
+// dims give the exact dot products with the codes as they lie in memory, and ks_j multiplies their fp32 value. 16
+// rows: the codes become f16 exactly (0x6400 | (q + 128) is 1152 + q), and q, scaled by a power of two per row to at
+// most 2^15, too, so the sums are those of the codes in fp32. P.V is in bf16, whose exponents hold every weight times
+// vs_j; its 8 bits would cost a weight 2^-9 of itself, so a weight enters as the sum of two bf16 values (16 bits).
+// With 8 query rows or fewer the second values ride in the MMA's upper 8 rows, which are idle otherwise; 16 rows take
+// a second MMA. Codes become bf16 exactly as (128 + low seven bits) - (128 + sign bit). Sums, maxima and
+// accumulators are fp32; the output is rounded once.
+//
+// What bounds it: HBM for long contexts (the 8 warps' loops run at 5.3 TB/s, 81% of a measured copy: about 800
+// instructions per 32-key tile, a third of them widening V), and for everything else the chain of round trips to L2
+// around them, about 0.5 us each: positions, first tile, and for split segments the fence, the arrival and the other
+// CTAs' records. Measured, d = 128, 8 kv heads, a call on the device: one row of 16 heads over 512 / 2048 / 8192 /
+// 32768 keys 7.7 / 10.7 / 12.6 / 21.8 us (32768: 69.2 MB, 3.2 TB/s); 16 rows of 32 heads over 1 to 8191 keys 24 us;
+// 64 rows over 32 to 512 keys 22 us. Tried: f16 weights (fewer instructions, but weights below 2^-29 of a row's
+// largest vanish), 16 warps with 16-key tiles (one row over 32768 keys 28.4 us for 24.1 then), adding up in every CTA
+// behind a prefix instead of in a third launch (64 rows over 32768 shared keys 81 us for 66).
 #include "internal.h"
 #include "common.cuh"
 
@@ -38,7 +47,7 @@ namespace egpt {
 namespace aq8 {
 
 constexpr int kMaxBatch = 512;
-constexpr int kRows = 16;              // query rows per tile (the M of the MMA), and rows of a partial record
+constexpr int kRows = 16;        // query rows per tile (the M of the MMA), and rows of a partial record
 constexpr int kMinKeys = 512;    // keys of a range at least
 constexpr int kExtraKeys = 512;  // what a segment's start and end cost, in keys
 
@@ -943,7 +952,8 @@ __global__ void __launch_bounds__(Cfg<Q8, NR>::kThreads, 1) attn_kernel(const Pa
   }
 }
 
-// Beside a prefix: one (sequence, head) row per warp, its own records and the prefix's.
+// Beside a prefix: one (sequence, head) row per warp, its own records and the prefix's. Bound by three dependent round
+// trips to L2 (the segment's parts, then two batches of records): 2048 rows of 19 records 5.6 us.
 constexpr int kAddWarps = 4;
 template <int D>
 __global__ void __launch_bounds__(32 * kAddWarps) add_kernel(const Params p) {
@@ -1053,7 +1063,8 @@ static int check(const char *what, int64_t ldo, int64_t ldq, const void *out, co
     return set_error(EGPT_ERR_SHAPE, "%s: nq must be a multiple of nkv, at most %d to one", what, kRows);
   if (m < 1 || m > kMaxBatch || cap < 1 || cap > (1 << 27) || ldq < (int64_t)nq * d || ldo < (int64_t)nq * d)
     return set_error(EGPT_ERR_SHAPE, "%s: bad m (1 to %d), cap or leading dimension", what, kMaxBatch);
-  if (m * nkv * ((cap + 15) / 16) > 0x3fffffff) return set_error(EGPT_ERR_SHAPE, "%s: cache too long for the batch", what);
+  if (nkv > (1 << 24) / m || m * nkv * ((cap + 15) / 16) > 0x1fffffff)
+    return set_error(EGPT_ERR_SHAPE, "%s: cache too long for the batch", what);
   if (!(fabsf(scale) <= 3e38f)) return set_error(EGPT_ERR_ARG, "%s: scale must be finite", what);
   if ((uintptr_t)out % 16 || (uintptr_t)q % 16 || ldq % 8 || ldo % 8)
     return set_error(EGPT_ERR_ALIGN, "%s: q and out must be 16-byte aligned rows", what);

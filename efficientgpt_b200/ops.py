@@ -271,8 +271,12 @@ def silu_mul(gu, inter, out=None):
 # A decode step calls these once or twice per layer, so the wrappers keep to a few microseconds: one pass over the tensors'
 # attributes, plain integers for the pointers, and the raw handle of the current stream.
 
+_I8, _F32, _BF16, _I64 = torch.int8, torch.float32, torch.bfloat16, torch.int64
+_raw_stream_of, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+
+
 def _raw_stream():
-    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+    return _raw_stream_of(_current_device())
 
 
 def kv_cache_q8(heads, cap, d, device):
@@ -284,20 +288,21 @@ def kv_cache_q8(heads, cap, d, device):
 
 def _cache_q8(what, k, ks, v, vs):
     """Checks an int8 cache pair; -> its shape (heads, cap, d)."""
-    shape = k.shape
-    if not (k.dtype is torch.int8 and v.dtype is torch.int8 and ks.dtype is torch.float32
-            and vs.dtype is torch.float32):
+    if k.dtype is not _I8 or v.dtype is not _I8 or ks.dtype is not _F32 or vs.dtype is not _F32:
         raise ValueError(f'{what}: int8 codes and fp32 scales expected')
-    if len(shape) != 3 or v.shape != shape or ks.shape != shape[:2] or vs.shape != shape[:2]:
+    shape = k.shape
+    if len(shape) != 3 or v.shape != shape or ks.shape != shape[:2] or vs.shape != ks.shape:
         raise ValueError(f'{what}: codes [heads, cap, d] and scales [heads, cap] expected')
     if not (k.is_contiguous() and ks.is_contiguous() and v.is_contiguous() and vs.is_contiguous()):
         raise ValueError(f'{what}: caches must be contiguous')
+    if not (k.is_cuda and ks.is_cuda and v.is_cuda and vs.is_cuda):
+        _cuda(k, ks, v, vs)
     return shape
 
 
 def _positions(what, position, n):
-    if position.dtype is not torch.int64 or position.numel() != n or not position.is_contiguous():
-        raise ValueError(f'{what}: position must be a contiguous int64 tensor of {n}')
+    if position.dtype is not _I64 or position.numel() != n or not position.is_contiguous() or not position.is_cuda:
+        raise ValueError(f'{what}: position must be a contiguous int64 CUDA tensor of {n}')
 
 
 def kv_append_q8(k, v, k_cache, k_scale, v_cache, v_scale, position, *, ragged=False, q=None, q_norm_w=None,
@@ -306,7 +311,6 @@ def kv_append_q8(k, v, k_cache, k_scale, v_cache, v_scale, position, *, ragged=F
     *position + i of caches [nkv, cap, d], or (ragged) to slot position[i] of its own heads of caches [M * nkv, cap,
     d] (-1: an idle slot, nothing is written). With q [M, nq * d] the q/k RMSNorm and RoPE of a decode step come first
     (the angle of position rope_base + slot) and the rotated q is returned."""
-    _cuda(k_cache, k_scale, v_cache, v_scale)
     shape = _cache_q8('kv_append_q8', k_cache, k_scale, v_cache, v_scale)
     return _append(k, v, shape, (k_cache.data_ptr(), k_scale.data_ptr(), v_cache.data_ptr(), v_scale.data_ptr()),
                    position, ragged, q, q_norm_w, k_norm_w, eps, rope_cos, rope_sin, rope_base, q_out)
@@ -326,12 +330,15 @@ def kv_append(k, v, cache, position, *, q, ragged=False, q_norm_w=None, k_norm_w
 
 def _append(k, v, shape, ptrs, position, ragged, q, q_norm_w, k_norm_w, eps, rope_cos, rope_sin, rope_base, q_out):
     heads, cap, d = shape
-    _cuda(k, v, position)
-    if k.dim() != 2 or k.stride(1) != 1 or v.stride(-1) != 1:
-        raise ValueError('kv_append_q8: k and v must be 2-D tensors with unit column stride')
-    m, width = k.shape
+    m, width = rows = k.shape
     nkv = width // d
-    if v.shape != k.shape or v.dtype is not k.dtype or nkv * d != width or heads != (nkv * m if ragged else nkv):
+    ldk, unit_k = k.stride()
+    ldv, unit_v = v.stride()
+    if not (k.is_cuda and v.is_cuda):
+        _cuda(k, v)
+    if unit_k != 1 or unit_v != 1:
+        raise ValueError('kv_append_q8: k and v must be 2-D tensors with unit column stride')
+    if v.shape != rows or v.dtype is not k.dtype or nkv * d != width or heads != (nkv * m if ragged else nkv):
         raise ValueError('kv_append_q8: k and v [M, nkv * d] do not fit the caches')
     _positions('kv_append_q8', position, m if ragged else 1)
     prologue = (None, 0, None, 0, 0, None, None, eps, None, None, 0)
@@ -354,9 +361,8 @@ def _append(k, v, shape, ptrs, position, ragged, q, q_norm_w, k_norm_w, eps, rop
             raise ValueError('kv_append_q8: q_out must be bf16 rows of the shape of q')
         prologue = (q_out.data_ptr(), q_out.stride(0), q.data_ptr(), q.stride(0), q.shape[1] // d, _p(q_norm_w),
                     _p(k_norm_w), eps, _p(rope_cos), _p(rope_sin), rope_base)
-    rc = L.load().egpt_kv_append_q8(*ptrs, cap, k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0),
-                                    position.data_ptr(), m, nkv, d, _dt(k), *prologue,
-                                    L.FLAG_RAGGED if ragged else 0, _raw_stream())
+    rc = L.load().egpt_kv_append_q8(*ptrs, cap, k.data_ptr(), ldk, v.data_ptr(), ldv, position.data_ptr(), m, nkv, d,
+                                    _dt(k), *prologue, L.FLAG_RAGGED if ragged else 0, _raw_stream())
     if rc:
         L.check(rc, 'kv_append_q8')
     return q_out
@@ -366,7 +372,6 @@ def kv_read_q8(k_cache, k_scale, v_cache, v_scale, start, count, *, dtype=torch.
     """The values of rows start .. start + count - 1 of an int8 cache: (k, v), each [heads, count, d] bf16 or fp32. An
     int64 tensor `start` of n rows reads every sequence of a ragged cache from its own slot (heads / n heads each;
     slots outside the cache read as zeros). out: the (k, v) tensors to fill, rows contiguous, one head stride."""
-    _cuda(k_cache, k_scale, v_cache, v_scale)
     heads, cap, d = _cache_q8('kv_read_q8', k_cache, k_scale, v_cache, v_scale)
     if out is None:
         k, v = torch.empty((2, heads, count, d), dtype=dtype, device=k_cache.device).unbind(0)
@@ -380,7 +385,6 @@ def kv_read_q8(k_cache, k_scale, v_cache, v_scale, start, count, *, dtype=torch.
         stride = k.stride(0) if heads > 1 else count * d
     starts, group = None, 0
     if torch.is_tensor(start):
-        _cuda(start)
         n = start.numel()
         _positions('kv_read_q8', start, n)
         if n < 1 or heads % n:
@@ -402,19 +406,19 @@ def attn_q8_ws(m, nq, nkv, d, device):
 def _attn_rows(what, q, out, nq, d):
     """Checks q (and out); -> (rows, out)."""
     shape = q.shape
-    if q.dtype is not torch.bfloat16 or len(shape) != 2 or shape[1] != nq * d or q.stride(1) != 1:
+    if q.dtype is not _BF16 or len(shape) != 2 or shape[1] != nq * d or q.stride(1) != 1:
         raise ValueError(f'{what}: q must be bf16 [M, nq * d] with unit column stride')
     if out is None:
         out = torch.empty_like(q)
-    elif out.dtype is not torch.bfloat16 or out.shape != shape or out.stride(1) != 1:
-        raise ValueError(f'{what}: out must be bf16 rows of the shape of q')
+    elif out.dtype is not _BF16 or out.shape != shape or out.stride(1) != 1 or not out.is_cuda:
+        raise ValueError(f'{what}: out must be bf16 CUDA rows of the shape of q')
     return shape[0], out
 
 
 def attn_decode_q8(q, k_cache, k_scale, v_cache, v_scale, position, nq, nkv, d, *, scale, ws=None, out=None):
     """Decode attention over int8 caches [M * nkv, cap, d]: row i of q bf16 [M, nq * d] over the position[i] + 1 keys of
     its own sequence (int64 [M] on the device; -1: an idle slot, zeros) -> bf16 [M, nq * d]."""
-    _cuda(q, k_cache, k_scale, v_cache, v_scale, position, ws, out)
+    _cuda(q, ws)
     m, out = _attn_rows('attn_decode_q8', q, out, nq, d)
     heads, cap, dc = _cache_q8('attn_decode_q8', k_cache, k_scale, v_cache, v_scale)
     if dc != d or heads != m * nkv:
@@ -433,12 +437,12 @@ def attn_decode_q8(q, k_cache, k_scale, v_cache, v_scale, position, nq, nkv, d, 
 
 def _cache_pair(what, cache, d):
     """A bf16 cache (k, v) or an int8 one (k, k_scale, v, v_scale); -> (heads, cap, dtype, pointers)."""
-    _cuda(*cache)
     if len(cache) == 4:
         heads, cap, dc = _cache_q8(what, *cache)
         dt, ptrs = L.EGPT_I8, [t.data_ptr() for t in cache]
     elif len(cache) == 2:
         k, v = cache
+        _cuda(k, v)
         if k.dim() != 3 or k.shape != v.shape or k.dtype is not torch.bfloat16 or v.dtype is not torch.bfloat16 or not (
                 k.is_contiguous() and v.is_contiguous()):
             raise ValueError(f'{what}: bf16 caches must be contiguous [heads, cap, d]')
@@ -456,7 +460,7 @@ def attn_shared_prefix(q, prefix, tails, position, prefix_len, nq, nkv, d, *, sc
     `prefix` (caches [nkv, prefix_cap, d], read once for the batch) and then the position[i] + 1 rows of its own tail
     (`tails`, caches [M * nkv, cap, d]; position int64 [M] counts the tail's slots, -1: none yet). Both are (k, v) in
     bf16 or (k, k_scale, v, v_scale) in int8."""
-    _cuda(q, position, ws, out)
+    _cuda(q, ws)
     m, out = _attn_rows('attn_shared_prefix', q, out, nq, d)
     ph, pcap, pdt, pp = _cache_pair('attn_shared_prefix', prefix, d)
     th, cap, tdt, tp = _cache_pair('attn_shared_prefix', tails, d)

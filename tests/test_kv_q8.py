@@ -9,9 +9,9 @@ X = 16  # an aligned address that is never read
 WS = 1 << 30
 
 
-def _append(k_cache=X, cap=8, k=X, ldk=256, position=X, m=1, nkv=2, d=128, dtype=L.EGPT_BF16, q_out=None, q=None, nq=0,
+def _append(k_cache=X, k_scale=X, v_scale=X, cap=8, k=X, ldk=256, position=X, m=1, nkv=2, d=128, dtype=L.EGPT_BF16, q_out=None, q=None, nq=0,
             norm=None, cos=None, sin=None, base=0):
-    return L.load().egpt_kv_append_q8(k_cache, X, X, X, cap, k, ldk, X, 256, position, m, nkv, d, dtype, q_out, nq * d, q,
+    return L.load().egpt_kv_append_q8(k_cache, k_scale, X, v_scale, cap, k, ldk, X, 256, position, m, nkv, d, dtype, q_out, nq * d, q,
                                       nq * d, nq, norm, None, 1e-6, cos, sin, base, 0, None)
 
 
@@ -42,6 +42,8 @@ def _shared(pk=X, pks=X, pcap=8, plen=4, tk=X, cap=8, m=1, nq=4, nkv=2, d=128, d
     (lambda: _append(q=X, q_out=X, nq=4, cos=X), L.EGPT_ERR_ARG),  # half a RoPE table
     (lambda: _append(q=X, q_out=X, nq=4, base=-1), L.EGPT_ERR_SHAPE),
     (lambda: _append(norm=X), L.EGPT_ERR_ARG),  # a norm without q
+    (lambda: _append(k_scale=None), L.EGPT_ERR_ARG),  # one scale without the other
+    (lambda: _append(k_scale=None, v_scale=None), L.EGPT_ERR_ARG),  # a bf16 cache without q
     (lambda: _read(out=None), L.EGPT_ERR_ARG),
     (lambda: _read(d=256), L.EGPT_ERR_SHAPE),
     (lambda: _read(count=0), L.EGPT_ERR_SHAPE),
@@ -61,6 +63,8 @@ def _shared(pk=X, pks=X, pcap=8, plen=4, tk=X, cap=8, m=1, nq=4, nkv=2, d=128, d
     (lambda: _decode(m=513), L.EGPT_ERR_SHAPE),
     (lambda: _decode(cap=0), L.EGPT_ERR_SHAPE),
     (lambda: _decode(cap=2 ** 40), L.EGPT_ERR_SHAPE),
+    (lambda: _decode(cap=2 ** 27 + 1), L.EGPT_ERR_SHAPE),
+    (lambda: _decode(m=512, cap=2 ** 27), L.EGPT_ERR_SHAPE),  # too many keys for the batch
     (lambda: _decode(ldq=511), L.EGPT_ERR_SHAPE),
     (lambda: _decode(ldq=513), L.EGPT_ERR_ALIGN),
     (lambda: _decode(k=8), L.EGPT_ERR_ALIGN),

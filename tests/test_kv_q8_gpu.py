@@ -155,6 +155,58 @@ def test_append_with_the_step_prologue_quantises_the_rows_of_the_bf16_append(cud
         assert not rag[0][3 * nkv:4 * nkv].any()
 
 
+def test_append_into_a_bf16_cache_stores_the_rows(cuda):
+    """kv_append on a bf16 cache: the rows of egpt_qk_norm_rope_kv_append, in the slots of a ragged batch."""
+    ops = _ops()
+    gen = _gen(44)
+    m, nq, nkv, d, cap, base = 6, 8, 2, 128, 30, 9
+    qkv = _randn(gen, m, (nq + 2 * nkv) * d).bfloat16()
+    wq, wk = (1 + 0.1 * _randn(gen, d)).bfloat16(), (1 + 0.1 * _randn(gen, d)).bfloat16()
+    ang = torch.arange(cap + base, device=cuda)[:, None] * torch.exp(-torch.arange(d // 2, device=cuda) * 0.2)
+    norm = dict(q_norm_w=wq, k_norm_w=wk, eps=1e-6, rope_cos=ang.cos().bfloat16(), rope_sin=ang.sin().bfloat16())
+    pos = torch.tensor([0, 29, -1, 7, 7, 12], device=cuda)
+    cache = tuple(torch.full((m * nkv, cap, d), 3.0, dtype=torch.bfloat16, device=cuda) for _ in range(2))
+    q = ops.kv_append(qkv[:, nq * d:(nq + nkv) * d], qkv[:, (nq + nkv) * d:], cache, pos, q=qkv[:, :nq * d], ragged=True,
+                      rope_base=base, **norm)
+    for i, slot in enumerate(pos.tolist()):
+        h = slice(i * nkv, (i + 1) * nkv)
+        want = [torch.full((nkv, cap + base, d), 3.0, dtype=torch.bfloat16, device=cuda) for _ in range(2)]
+        if slot >= 0:
+            wq_rows = ops.qk_norm_rope_kv_append(qkv[i:i + 1], *want, torch.tensor([base + slot], device=cuda), nq, nkv, d,
+                                                 **norm)
+            assert torch.equal(q[i:i + 1], wq_rows)
+        else:
+            assert not q[i].any()
+        assert torch.equal(cache[0][h], want[0][:, base:]) and torch.equal(cache[1][h], want[1][:, base:])
+
+
+def test_caches_beyond_32_bit_offsets(cuda):
+    """Codes whose offsets pass 2^31 and 2^32: written at the far end, read back and attended to at the near one."""
+    ops = _ops()
+    gen = _gen(45)
+    m, nq, nkv, d, cap = 3, 4, 2, 128, 6_000_000
+    cache = tuple(torch.empty(m * nkv, cap, d, dtype=torch.int8, device=cuda) if i % 2 == 0 else
+                  torch.empty(m * nkv, cap, device=cuda) for i in range(4))
+    near = _cache_q8(gen, m * nkv, 70, d)
+    for t, n in zip(cache, near):
+        t[:, :70] = n
+    rows = _randn(gen, m, 2 * nkv * d).bfloat16()
+    k, v = rows[:, :nkv * d], rows[:, nkv * d:]
+    far = torch.tensor([cap - 1, cap - 2, cap - 1], device=cuda)
+    ops.kv_append_q8(k, v, *cache, far, ragged=True)
+    kr, vr = ops.kv_read_q8(*cache, far, 1, dtype=torch.float32)
+    for x, got in ((k, kr), (v, vr)):
+        q8, s8 = _quantised(x.reshape(m * nkv, d))
+        assert torch.equal(got[:, 0], q8.float() * s8.unsqueeze(-1))
+    q = _randn(gen, m, nq * d).bfloat16()
+    out = ops.attn_decode_q8(q, *cache, torch.tensor([69, 0, 40], device=cuda), nq, nkv, d, scale=d ** -0.5)
+    _check(out, q, nq, nkv, d, d ** -0.5, [70, 1, 41], near)
+    # the whole of the last head's four and a half billion bytes is addressable: its last keys through a long read
+    kr, _ = ops.kv_read_q8(*cache, cap - 1, 1, dtype=torch.float32)
+    q8, s8 = _quantised(k.reshape(m * nkv, d))
+    assert torch.equal(kr[[0, 1, 4, 5], 0], (q8.float() * s8.unsqueeze(-1))[[0, 1, 4, 5]])
+
+
 def test_read_from_device_positions_into_views(cuda):
     ops = _ops()
     gen = _gen(3)
