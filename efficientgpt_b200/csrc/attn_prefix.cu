@@ -24,12 +24,11 @@
 // the sum of two bf16 values (16 bits), a second P.V: the values' own rounding is then the only one that counts.
 // Everything else is fp32. Every wait is bounded; issued loads and MMAs are drained before the CTA exits.
 //
-// What bounds it (d = 128, one step = two streams' blocks): the MMAs of a step take 1.1 us at the measured rate and its
-// exponentials as long, one per clock and four lanes of each SM quarter; a step takes 1.33 us with bf16 caches. 256 rows
-// of each of 8 kv heads over 32768 keys: 47 us with 3 us to the first scores and 3.5 us for the records, 34.4 GFLOP at
-// 730 TFLOP/s (44% of measured); 64 rows: 25 us for the 134 MB of the prefix (5.4 TB/s, 82% of a measured copy). int8: a
-// step takes 2.2 us, the two P.V and twice the softmax's instructions at 128 registers a thread; a larger share of the
-// registers for the softmax warps (setmaxnreg) did not compile.
+// What bounds it (d = 128, one step = two streams' blocks): shared memory, which the MMAs read at 128 bytes a clock. With
+// bf16 caches a step's operands are 256 KB, 1.1 us, as long as its exponentials take (16 a clock); a step takes 1.33 us.
+// 256 rows of each of 8 kv heads over 32768 keys: 47 us with 3 us to the first scores and 3.5 us for the records, 34.4
+// GFLOP at 730 TFLOP/s (44% of measured); 64 rows: 25 us for the 134 MB of the prefix (5.4 TB/s, 82% of a measured
+// copy). int8: the second P.V, the widening and the scales make it 480 KB, 2 us; a step takes 2.2 us.
 #include "internal.h"
 #include "common.cuh"
 
@@ -37,7 +36,7 @@ namespace egpt {
 namespace apx {
 
 constexpr int kBK = 128, kRowsT = 128;
-constexpr uint32_t kOCol = 256;  // S0 | S1 | O0 | O1, 128 columns each; P_s in S_s: 64 columns, int8: two times 64
+constexpr uint32_t kOCol = 256;  // S0 | S1 | O0 | O1, 128 columns each; P_s in S_s
 constexpr int record_size(int d) { return kRowsT * (d + 2); }  // floats: [128 rows][d], maxima, sums
 
 template <int D, bool Q8>
@@ -244,7 +243,8 @@ __global__ void __launch_bounds__(Cfg<D, Q8>::kThreads, 1) attn_prefix_kernel(co
           for (int part = 0; part < (Q8 ? 2 : 1); ++part)
 #pragma unroll
             for (int kk = 0; kk < kBK / 16; ++kk)  // 16 keys per step: 8 columns of P, 16 rows of 128 bytes of V
-              apf::umma_ts(tmem + kOCol + (uint32_t)(128 * s), tmem + (uint32_t)(128 * s + 64 * part + 8 * kk),
+              apf::umma_ts(tmem + kOCol + (uint32_t)(128 * s),
+                           tmem + (uint32_t)(128 * s + (Q8 ? 32 * (kk / 2) + 16 * part + 8 * (kk % 2) : 8 * kk)),
                            apf::sw128_mn_desc(v + (size_t)kk * 16 * 128), kIdescO, (i > 0 || part > 0 || kk > 0) ? 1u : 0u);
           if (!two || s == 1) gtc::umma_commit(v_empty + slot);
           if (i + 1 < steps[s]) ok = issue_scores(s, i + 1);
@@ -302,7 +302,9 @@ __global__ void __launch_bounds__(Cfg<D, Q8>::kThreads, 1) attn_prefix_kernel(co
           scaled(c, sc);
 #pragma unroll
           for (int e = 0; e < 32; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(sc[e]));
+          if (Q8) apf::tmem_st32(ts + (uint32_t)c, sc);  // scaled: the second pass needs no factors from shared memory
         }
+        if (Q8) apf::tmem_wait_st();
         const float bm = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * (Q8 ? 1.f : A.scale_log2);
         float alpha = 1.f;
         if (bm > m_run + apf::kStale) {
@@ -323,7 +325,8 @@ __global__ void __launch_bounds__(Cfg<D, Q8>::kThreads, 1) attn_prefix_kernel(co
         }
         const uint64_t nm2 = apf::f2_pack(-m_run, -m_run);
         uint64_t sum[2] = {apf::f2_pack(0.f, 0.f), apf::f2_pack(0.f, 0.f)};
-        // weights of 32 keys over scores that have been read: bf16 in columns c / 2 ..; int8: the second parts 64 on
+        // weights of 32 keys over scores that have been read: bf16 in columns c / 2 ..; int8 in the 32 columns of their
+        // own scores, the second parts in the upper 16
         auto weights = [&](int c, const uint32_t *sc) {
           uint32_t pk[16], pl[Q8 ? 16 : 1];
 #pragma unroll
@@ -342,34 +345,16 @@ __global__ void __launch_bounds__(Cfg<D, Q8>::kThreads, 1) attn_prefix_kernel(co
               if constexpr (Q8) pl[k / 2] = gtc::pack_bf16x2(w.x - bf16_lo(pk[k / 2]), w.y - bf16_hi(pk[k / 2]));
             }
           }
-          apf::tmem_st16(ts + (uint32_t)(c / 2), pk);
-          if constexpr (Q8) apf::tmem_st16(ts + (uint32_t)(64 + c / 2), pl);
+          apf::tmem_st16(ts + (uint32_t)(Q8 ? c : c / 2), pk);
+          if constexpr (Q8) apf::tmem_st16(ts + (uint32_t)(c + 16), pl);
         };
-        if constexpr (Q8) {  // the second parts go over the upper scores: those are read first
-          uint32_t up[2][32];
-          apf::tmem_ld32(ts + 64, up[0]);
-          apf::tmem_ld32(ts + 96, up[1]);
 #pragma unroll
-          for (int c = 0; c < 64; c += 32) {
-            uint32_t sc[32];
-            apf::tmem_ld32(ts + (uint32_t)c, sc);
-            apf::tmem_wait_ld();
-            scaled(c, sc);
-            weights(c, sc);
-          }
-          scaled(64, up[0]);
-          weights(64, up[0]);
-          scaled(96, up[1]);
-          weights(96, up[1]);
-        } else {
-#pragma unroll
-          for (int c = 0; c < kBK; c += 32) {
-            uint32_t sc[32];
-            apf::tmem_ld32(ts + (uint32_t)c, sc);
-            apf::tmem_wait_ld();
-            scaled(c, sc);
-            weights(c, sc);
-          }
+        for (int c = 0; c < kBK; c += 32) {
+          uint32_t sc[32];
+          apf::tmem_ld32(ts + (uint32_t)c, sc);
+          apf::tmem_wait_ld();
+          if (!Q8) mask(c, sc);
+          weights(c, sc);
         }
         const float2 t = apf::f2_unpack(apf::f2_add(sum[0], sum[1]));
         l_sum = l_sum * alpha + (t.x + t.y);

@@ -374,7 +374,8 @@ def kv_read_q8(k_cache, k_scale, v_cache, v_scale, start, count, *, dtype=torch.
     slots outside the cache read as zeros). out: the (k, v) tensors to fill, rows contiguous, one head stride."""
     heads, cap, d = _cache_q8('kv_read_q8', k_cache, k_scale, v_cache, v_scale)
     if out is None:
-        k, v = torch.empty((2, heads, count, d), dtype=dtype, device=k_cache.device).unbind(0)
+        k = k_cache.new_empty((heads, count, d), dtype=dtype)
+        v = torch.empty_like(k)
         stride = count * d
     else:
         k, v = out
