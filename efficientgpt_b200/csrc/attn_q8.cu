@@ -485,7 +485,7 @@ __global__ void __launch_bounds__(Cfg<Q8, NR>::kThreads, 1) attn_kernel(const Pa
     x0 = __shfl_sync(0xffffffffu, cut, 0), x1 = __shfl_sync(0xffffffffu, cut, 1);
   }
   int split_n = 0;  // segments that this CTA shares with others: its first, its last
-  int2 split[2] = {};  // their number and first CTA
+  int3 split[2] = {};  // their number, first CTA and CTAs
   if (x0 < x1) {
     Seg seg;
     if (!PREFIX && lay.solo) seg = own_seg<TILE>(p, sm.cum, sm.len, solo_seg / p.nkv, solo_seg % p.nkv);
@@ -793,7 +793,7 @@ __global__ void __launch_bounds__(Cfg<Q8, NR>::kThreads, 1) attn_kernel(const Pa
         for (int j = 0; j < ND; ++j) acc[j][0] += acc[j][2], acc[j][1] += acc[j][3];
       }
       const Seg done = seg;
-      const bool another = advance(seg);
+      const bool another = lay.pad == 1 && advance(seg);
       if (another) load_q(seg);  // on its way while this one is added up
       // ---- the segment is done: the warps' states, each relative to the largest maximum, are added up in shared memory
 #pragma unroll
@@ -885,7 +885,7 @@ __global__ void __launch_bounds__(Cfg<Q8, NR>::kThreads, 1) attn_kernel(const Pa
       if (MODE != kPrefix && !final) {
         const int c0 = done.start / lay.chunk, c1 = (done.end - 1) / lay.chunk;
         if (MODE == kOwn) {
-          (split_n ? split[1] : split[0]) = make_int2(done.index, c0);
+          (split_n ? split[1] : split[0]) = make_int3(done.index, c0, c1 - c0 + 1);
           ++split_n;
         } else if (done.start >= x0 && threadIdx.x == 0) {  // (a short segment lies in one CTA wherever the even cuts are)
           p.parts[done.index] = make_int2(whole ? (int)blockIdx.x + done.index : c0 + done.index, whole ? 1 : c1 - c0 + 1);
@@ -906,33 +906,30 @@ __global__ void __launch_bounds__(Cfg<Q8, NR>::kThreads, 1) attn_kernel(const Pa
         for (int c = threadIdx.x; c < p.group * D; c += C::kThreads)
           p.out[(e / p.nkv) * p.ldo + (int64_t)(e % p.nkv) * p.group * D + c] = 0;
     if (!split_n) return;
-    __threadfence();
     __syncthreads();
-    if ((int)threadIdx.x < split_n) {
-      const int2 e = threadIdx.x ? split[1] : split[0];
-      const Seg sg = own_seg<TILE>(p, sm.cum, sm.len, e.x / p.nkv, e.x % p.nkv);
-      const int n = (sg.end - 1) / lay.chunk - e.y + 1;
-      const bool last = atomicAdd(p.cnt + e.x, 1u) == (unsigned)(n - 1);
+    if ((int)threadIdx.x < split_n) {  // (the fence covers the CTA's records, which the barrier ordered before it)
+      const int3 e = threadIdx.x ? split[1] : split[0];
+      __threadfence();
+      const bool last = atomicAdd(p.cnt + e.x, 1u) == (unsigned)(e.z - 1);
       if (last) {
-        p.cnt[e.x] = 0u;
         __threadfence();
+        p.cnt[e.x] = 0u;
       }
-      sm.last[threadIdx.x] = last ? n : 0;
+      sm.last[threadIdx.x] = last;
     }
     __syncthreads();
 #pragma unroll 1
     for (int s = 0; s < split_n; ++s) {
-      const int n = sm.last[s];
-      if (!n) continue;
+      if (!sm.last[s]) continue;
       // a warp takes a row, or with fewer rows than warps every parts-th record of one
-      const int2 e = s ? split[1] : split[0];
+      const int3 e = s ? split[1] : split[0];
       const int parts = p.group < kWarps ? kWarps / p.group : 1, part = parts > 1 ? warp / p.group : 0;
       uint16_t *out = p.out + (e.x / p.nkv) * p.ldo + (int64_t)(e.x % p.nkv) * p.group * D;
       const float *rec = record<D>(p, e.y + e.x);
 #pragma unroll 1
       for (int j = warp - part * p.group; j < p.group && part < parts; j += kWarps) {
         float a[D / 32];
-        add_records<D, false, 8>(rec + j * D, n, j, nullptr, 0, 0, 0, 0, part, parts, a);
+        add_records<D, false, 8>(rec + j * D, e.z, j, nullptr, 0, 0, 0, 0, part, parts, a);
         if (parts == 1) {
           store_row(out + j * D + D / 32 * lane, a);
         } else {

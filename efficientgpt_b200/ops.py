@@ -385,7 +385,7 @@ def kv_read_q8(k_cache, k_scale, v_cache, v_scale, start, count, *, dtype=torch.
             raise ValueError('kv_read_q8: out must be two tensors [heads, count, d] with contiguous rows')
         stride = k.stride(0) if heads > 1 else count * d
     starts, group = None, 0
-    if torch.is_tensor(start):
+    if not isinstance(start, int):
         n = start.numel()
         _positions('kv_read_q8', start, n)
         if n < 1 or heads % n:
