@@ -76,7 +76,7 @@ struct Params {
   int head_share;  // CTAs per kv head
   float scale_log2;
   float *ws;      // partial records of this launch
-  unsigned *cnt;  // arrivals per (sequence, kv head); zero between calls
+  unsigned *cnt;  // arrivals at a split segment, by the first CTA of it; zero between calls
   int2 *parts;    // beside a prefix: first record and records of each (sequence, kv head)
   int keys;       // keys of the shared prefix (the launch over it)
   Prefix pre;     // of the launch over the sequences' own keys: records to add up; of the prefix's: how it is cut
@@ -910,10 +910,10 @@ __global__ void __launch_bounds__(Cfg<Q8, NR>::kThreads, 1) attn_kernel(const Pa
     if ((int)threadIdx.x < split_n) {  // (the fence covers the CTA's records, which the barrier ordered before it)
       const int3 e = threadIdx.x ? split[1] : split[0];
       __threadfence();
-      const bool last = atomicAdd(p.cnt + e.x, 1u) == (unsigned)(e.z - 1);
+      const bool last = atomicAdd(p.cnt + e.y, 1u) == (unsigned)(e.z - 1);
       if (last) {
         __threadfence();
-        p.cnt[e.x] = 0u;
+        p.cnt[e.y] = 0u;
       }
       sm.last[threadIdx.x] = last;
     }
@@ -1050,8 +1050,14 @@ static bool prefix_on_tcgen05(const Params &p, int64_t keys, int d, bool q8) {
   const int64_t rows = (int64_t)p.m * p.group, pairs = rows * p.nkv * keys;
   return d >= 64 && p.scale_log2 > 0.f && (q8 ? rows > 64 && pairs > 3500000 : rows > kRows && pairs > 1500000);
 }
-// Arrival counters, then the (first record, records) pairs of the segments.
-static size_t counter_bytes(int64_t m, int nkv) { return ((size_t)m * nkv * 16 + 255) / 256 * 256; }
+// The workspace: arrival counters, one per CTA (a CTA is the first of at most one split segment) whatever the call's
+// sizes, so that calls of different sizes can share it; the segments' (first record, records) pairs; the records.
+static size_t counter_bytes() { return ((size_t)max_grid() * sizeof(unsigned) + 255) / 256 * 256; }
+static size_t parts_bytes(int64_t m, int nkv) { return ((size_t)m * nkv * sizeof(int2) + 255) / 256 * 256; }
+static void set_workspace(Params &p, void *ws) {
+  p.cnt = (unsigned *)ws, p.parts = (int2 *)((char *)ws + counter_bytes());
+  p.ws = (float *)((char *)p.parts + parts_bytes(p.m, p.nkv));
+}
 
 static int check(const char *what, int64_t ldo, int64_t ldq, const void *out, const void *q, int64_t cap, int64_t m,
                  int nq, int nkv, int d, float scale, const void *ws, size_t ws_bytes) {
@@ -1083,7 +1089,7 @@ extern "C" size_t egpt_attn_q8_ws_bytes(int64_t m, int nq, int nkv, int d) {
   const size_t rec = aq8::kRows * ((size_t)d + 2) * 4;
   const size_t small = ((size_t)aq8::max_grid() + (size_t)nkv * aq8::row_tiles(m, nq / nkv)) * rec;
   const size_t big = (d == 64 || d == 128) && nq / nkv <= aq8::kRows ? apx::record_floats(m, nq / nkv, nkv, d) * 4 : 0;
-  return aq8::counter_bytes(m, nkv) + ((size_t)aq8::max_grid() + (size_t)m * nkv) * rec + std::max(small, big);
+  return aq8::counter_bytes() + aq8::parts_bytes(m, nkv) + ((size_t)aq8::max_grid() + (size_t)m * nkv) * rec + std::max(small, big);
 }
 
 extern "C" int egpt_attn_decode_q8(void *out, int64_t ldo, const void *q, int64_t ldq, const int8_t *k_cache,
@@ -1100,8 +1106,7 @@ extern "C" int egpt_attn_decode_q8(void *out, int64_t ldo, const void *q, int64_
   p.out = (uint16_t *)out, p.ldo = ldo, p.q = (const uint16_t *)q, p.ldq = ldq;
   p.cache = {(const uint8_t *)k_cache, (const uint8_t *)v_cache, k_scale, v_scale, cap};
   p.position = position, p.m = (int)m, p.nkv = nkv, p.group = nq / nkv, p.scale_log2 = scale * 1.4426950408889634f;
-  p.cnt = (unsigned *)ws, p.parts = (int2 *)((char *)ws + (size_t)m * nkv * 8);
-  p.ws = (float *)((char *)ws + aq8::counter_bytes(m, nkv));
+  aq8::set_workspace(p, ws);
   return check_launch(aq8::launch_any<aq8::kOwn>(p, d, true, p.group, (cudaStream_t)stream, (flags & EGPT_FLAG_PDL) != 0),
                       "attn_decode_q8_kernel");
 }
@@ -1130,8 +1135,7 @@ extern "C" int egpt_attn_shared_prefix(void *out, int64_t ldo, const void *q, in
   aq8::Params p{};
   p.out = (uint16_t *)out, p.ldo = ldo, p.q = (const uint16_t *)q, p.ldq = ldq;
   p.position = position, p.m = (int)m, p.nkv = nkv, p.group = nq / nkv, p.scale_log2 = scale * 1.4426950408889634f;
-  p.cnt = (unsigned *)ws, p.parts = (int2 *)((char *)ws + (size_t)m * nkv * 8);
-  p.ws = (float *)((char *)ws + aq8::counter_bytes(m, nkv));
+  aq8::set_workspace(p, ws);
   float *pre_rec = p.ws + ((size_t)aq8::max_grid() + (size_t)m * nkv) * aq8::kRows * (d + 2);
   if (prefix_len > 0) {
     if (aq8::prefix_on_tcgen05(p, prefix_len, d, q8)) {

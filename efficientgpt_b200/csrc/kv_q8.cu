@@ -46,7 +46,12 @@ __device__ __forceinline__ int64_t slot_of(const AppendParams &p, int64_t row, i
   return -1;
 }
 
-__device__ __forceinline__ float row_scale(float amax) { return fmaxf(amax * (1.0f / 127.0f), 1e-12f); }
+// The largest magnitude is kept as its bits, whose order is that of the magnitudes with infinity and NaN at the top: a row
+// that holds one of those gets the scale NaN, so all that reads it sees it.
+__device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+__device__ __forceinline__ float row_scale(uint32_t amax) {
+  return amax >= 0x7f800000u ? NAN : fmaxf(__uint_as_float(amax) * (1.0f / 127.0f), 1e-12f);
+}
 __device__ __forceinline__ int code_of(float x, float s) {
   return (int)fminf(fmaxf(rintf(__fdiv_rn(x, s)), -127.f), 127.f);
 }
@@ -107,11 +112,11 @@ __global__ void __launch_bounds__(kThreads) append_kernel(AppendParams p) {
   const int64_t dst = (head0 + head) * p.cap + slot;
 #pragma unroll
   for (int kv = 0; kv < 2; ++kv) {
-    float amax = 0.f;
+    uint32_t amax = 0u;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(x[kv][e]));
+    for (int e = 0; e < 8; ++e) amax = max(amax, magnitude(x[kv][e]));
 #pragma unroll
-    for (int o = kLanes / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    for (int o = kLanes / 2; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
     if (slot < 0) continue;
     const float s = row_scale(amax);
     *(uint2 *)((kv ? p.v_cache : p.k_cache) + dst * D + e0) = codes_of(x[kv], s);
@@ -185,11 +190,10 @@ __global__ void __launch_bounds__(kThreads) norm_rope_append_kernel(AppendParams
     for (int i = 0; i < N; ++i) rows[lane + 32 * i] = f32_to_bf16_bits(x[i]);
     return;
   }
-  float amax = 0.f;
+  uint32_t amax = 0u;
 #pragma unroll
-  for (int i = 0; i < N; ++i) amax = fmaxf(amax, fabsf(x[i]));
-  amax = warp_max(amax);
-  const float s = row_scale(amax);
+  for (int i = 0; i < N; ++i) amax = max(amax, magnitude(x[i]));
+  const float s = row_scale(__reduce_max_sync(0xffffffffu, amax));
   int8_t *codes = (kind == 1 ? p.k_cache : p.v_cache) + dst * D;
 #pragma unroll
   for (int i = 0; i < N; ++i) codes[lane + 32 * i] = (int8_t)code_of(x[i], s);

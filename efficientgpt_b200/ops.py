@@ -371,7 +371,8 @@ def _append(k, v, shape, ptrs, position, ragged, q, q_norm_w, k_norm_w, eps, rop
 def kv_read_q8(k_cache, k_scale, v_cache, v_scale, start, count, *, dtype=torch.bfloat16, out=None):
     """The values of rows start .. start + count - 1 of an int8 cache: (k, v), each [heads, count, d] bf16 or fp32. An
     int64 tensor `start` of n rows reads every sequence of a ragged cache from its own slot (heads / n heads each;
-    slots outside the cache read as zeros). out: the (k, v) tensors to fill, rows contiguous, one head stride."""
+    slots outside the cache read as zeros). A row that was written with a NaN or an infinity in it reads as NaN. out: the
+    (k, v) tensors to fill, rows contiguous, one head stride."""
     heads, cap, d = _cache_q8('kv_read_q8', k_cache, k_scale, v_cache, v_scale)
     if out is None:
         k = k_cache.new_empty((heads, count, d), dtype=dtype)
@@ -385,12 +386,14 @@ def kv_read_q8(k_cache, k_scale, v_cache, v_scale, start, count, *, dtype=torch.
             raise ValueError('kv_read_q8: out must be two tensors [heads, count, d] with contiguous rows')
         stride = k.stride(0) if heads > 1 else count * d
     starts, group = None, 0
-    if not isinstance(start, int):
+    if isinstance(start, torch.Tensor):
         n = start.numel()
         _positions('kv_read_q8', start, n)
         if n < 1 or heads % n:
             raise ValueError('kv_read_q8: one start for each sequence of the cache')
         starts, group, start = start.data_ptr(), heads // n, 0
+    else:
+        start = int(start)
     rc = L.load().egpt_kv_read_q8(k.data_ptr(), v.data_ptr(), stride, _dt(k), k_cache.data_ptr(), k_scale.data_ptr(),
                                   v_cache.data_ptr(), v_scale.data_ptr(), cap, heads, d, start, starts, group, count, 0,
                                   _raw_stream())
@@ -400,7 +403,8 @@ def kv_read_q8(k_cache, k_scale, v_cache, v_scale, start, count, *, dtype=torch.
 
 
 def attn_q8_ws(m, nq, nkv, d, device):
-    """Workspace of attn_decode_q8 and attn_shared_prefix for m sequences (one per stream that runs them)."""
+    """Workspace of attn_decode_q8 and attn_shared_prefix for m sequences: one per stream that runs them, for calls of
+    every size that needs no more bytes."""
     return torch.zeros(int(L.load().egpt_attn_q8_ws_bytes(m, nq, nkv, d)), dtype=torch.uint8, device=device)
 
 

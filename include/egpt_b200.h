@@ -191,7 +191,8 @@ EGPT_API int egpt_attn_prefill(void *out, int64_t ldo, const void *q, int64_t ld
  * No counterpart in the reference (its static cache holds the activations' dtype). A cache is int8 codes
  * [heads][cap][d] and fp32 scales [heads][cap], a pair of them for keys and for values: row r of head h stands for
  * scale[h][r] * codes[h][r], with the weights' quantiser s = max(max|x| / 127, 1e-12), q = clamp(rint(x / s), -127,
- * 127) (egpt_quantize_rows). d is 32, 64 or 128; codes 16-byte aligned. Values are expected finite.
+ * 127) (egpt_quantize_rows); a row with an infinity or NaN gets the scale NaN. d is 32, 64 or 128; codes 16-byte
+ * aligned.
  *
  * egpt_kv_append_q8: rows i < m of k [m][ldk] and v [m][ldv] (head g at columns g d; dtype bf16 or fp32; 16-byte
  *   aligned rows) into slot *position + i, or with EGPT_FLAG_RAGGED row i into slot position[i] of its own cache heads
@@ -211,8 +212,8 @@ EGPT_API int egpt_attn_prefill(void *out, int64_t ldo, const void *q, int64_t ld
  *   then sequence i's own position[i] + 1 keys (its tail; position counts the tail's slots). cache_dtype EGPT_I8, or
  *   EGPT_BF16 with all scales NULL, for prefix and tails alike. The prefix is read once for the whole batch.
  * The work is cut into equal parts on the device, so a captured graph follows the positions. ws holds
- * egpt_attn_q8_ws_bytes(m, nq, nkv, d) bytes, 16-byte aligned, zero-filled once; calls that can overlap on the GPU
- * need workspaces of their own. Scores, sums and accumulators are fp32, one rounding of the output. */
+ * egpt_attn_q8_ws_bytes(m, nq, nkv, d) bytes or more, 16-byte aligned, zero-filled once; calls of different sizes can
+ * share it one after the other, calls that can overlap on the GPU need workspaces of their own. Scores, sums and accumulators are fp32, one rounding of the output. */
 EGPT_API int egpt_kv_append_q8(int8_t *k_cache, float *k_scale, int8_t *v_cache, float *v_scale, int64_t cap,
                                const void *k, int64_t ldk, const void *v, int64_t ldv, const int64_t *position,
                                int64_t m, int nkv, int d, int dtype, void *q_out, int64_t ldqo, const void *q,

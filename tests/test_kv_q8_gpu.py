@@ -3,8 +3,8 @@
 
 Codes and scales follow from IEEE operations alone (fp32 product, division, rint), so they are compared exactly.
 Attention: with w the exact weights, A = sum w |V| / sum w bounds the effect of rounding every weight by a relative u to
-u A. u is 2^-11 for the f16 weights of the int8 caches and 2^-8 for the bf16 weights of the bf16 caches, the output's own
-rounding 2^-8 |out|; scores are sums of 128 fp32 products and two fp32 roundings more, an error below 2^-14 of the
+u A. u is 2^-11 for the weights of the int8 caches, as f16 would carry them, and 2^-8 for those of the bf16 caches, as bf16
+would (both are carried closer, as the sum of two bf16 values), the output's own rounding 2^-8 |out|; scores are sums of 128 fp32 products and two fp32 roundings more, an error below 2^-14 of the
 score's magnitude sum |q k| scale, which changes a weight by as much relative to itself: 2^-14 (1 + S) A with
 S the largest such sum."""
 import pytest
@@ -227,6 +227,33 @@ def test_read_from_device_positions_into_views(cuda):
     assert buf[:, :, :5].isnan().all() and buf[:, :, 12:].isnan().all()
 
 
+@pytest.mark.parametrize('d', [32, 64, 128])
+@pytest.mark.parametrize('dtype,prologue', [(torch.bfloat16, False), (torch.float32, False), (torch.bfloat16, True)])
+@pytest.mark.parametrize('bad', [float('nan'), float('inf'), float('-inf')])
+def test_a_row_with_nan_or_infinity_reads_as_nan(cuda, d, dtype, prologue, bad):
+    """One bad element marks its own row and head, in keys and values, and the attention over it; the others keep their
+    codes."""
+    ops = _ops()
+    gen = _gen(d)
+    m, nkv, cap = 3, 2, 4
+    rows = _randn(gen, 2, m, nkv * d).to(dtype)
+    poisoned = rows.clone()
+    poisoned[0, 1, d + 5] = poisoned[1, 2, d - 1] = bad
+    q = _randn(gen, m, nkv * d).bfloat16()
+    pos = torch.tensor([1, 0, 3], device=cuda)
+    caches = []
+    for k, v in (rows, poisoned):
+        caches.append(ops.kv_cache_q8(m * nkv, cap, d, cuda))
+        ops.kv_append_q8(k, v, *caches[-1], pos, ragged=True, q=q if prologue else None)
+    (k0, v0), (k1, v1) = (ops.kv_read_q8(*c, 0, cap, dtype=torch.float32) for c in caches)
+    assert k1[1 * nkv + 1, 0].isnan().all() and v1[2 * nkv, 3].isnan().all()
+    out = ops.attn_decode_q8(q, *caches[1], pos, nkv, nkv, d, scale=0.1).view(m * nkv, d)
+    for h in range(m * nkv):
+        assert out[h].isnan().all() if h in (3, 4) else out[h].isfinite().all()
+    k1[1 * nkv + 1, 0], v1[2 * nkv, 3] = k0[1 * nkv + 1, 0], v0[2 * nkv, 3]
+    assert torch.equal(k0, k1) and torch.equal(v0, v1)
+
+
 def test_append_out_of_the_cache_reports_and_writes_nothing(cuda):
     from efficientgpt_b200 import _lib as L
     ops = _ops()
@@ -293,6 +320,28 @@ def test_decode_score_sizes_and_scale_spread(cuda, factor):
     own[1].mul_(own[1].clamp_max(3.0) / own[1])
     out = ops.attn_decode_q8(q, *own, torch.tensor(lengths, device=cuda) - 1, nq, nkv, d, scale=d ** -0.5)
     _check(out, q, nq, nkv, d, d ** -0.5, lengths, own)
+
+
+def test_a_workspace_serves_calls_of_every_size(cuda):
+    """Batches from one sequence to 64 and a shared prefix in turn on the largest call's workspace."""
+    ops = _ops()
+    gen = _gen(13)
+    nq, nkv, d, cap = 16, 8, 128, 1100
+    own = _cache_q8(gen, 64 * nkv, cap, d)
+    q = _randn(gen, 64, nq * d).bfloat16()
+    ws = ops.attn_q8_ws(64, nq, nkv, d, cuda)
+    for m, shared in ((1, 0), (64, 0), (3, 700), (64, 0), (1, 0), (20, 33), (20, 0)):
+        lengths = [cap - 17 * (i % 40) for i in range(m)]
+        heads = [t[:m * nkv] for t in own]
+        pos = torch.tensor(lengths, device=cuda) - 1
+        if shared:
+            out = ops.attn_shared_prefix(q[:m], [t[-nkv:] for t in own], heads, pos, shared, nq, nkv, d, scale=0.1, ws=ws)
+        else:
+            out = ops.attn_decode_q8(q[:m], *heads, pos, nq, nkv, d, scale=0.1, ws=ws)
+        some = range(0, m, 7)  # every seventh sequence
+        rows = lambda t: torch.cat([t[i * nkv:(i + 1) * nkv] for i in some])  # noqa: E731
+        _check(out[::7], q[:m:7], nq, nkv, d, 0.1, [lengths[i] for i in some], [rows(t) for t in heads],
+               [t[-nkv:] for t in own] if shared else None, shared)
 
 
 def test_nan_and_infinity_in_a_query_row_stay_in_its_heads(cuda):
