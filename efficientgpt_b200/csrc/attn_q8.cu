@@ -36,7 +36,7 @@
 // instructions per 32-key tile, a third of them widening V), and for everything else the chain of round trips to L2
 // around them, about 0.5 us each: positions, first tile, and for split segments the fence, the arrival and the other
 // CTAs' records. Measured, d = 128, 8 kv heads, a call on the device: one row of 16 heads over 512 / 2048 / 8192 /
-// 32768 keys 7.7 / 10.7 / 12.6 / 21.8 us (32768: 69.2 MB, 3.2 TB/s); 16 rows of 32 heads over 1 to 8191 keys 24 us;
+// 32768 keys 7.9 / 10.7 / 12.6 / 22.3 us (32768: 69.2 MB, 3.1 TB/s); 16 rows of 32 heads over 1 to 8191 keys 24 us;
 // 64 rows over 32 to 512 keys 22 us. Tried: f16 weights (fewer instructions, but weights below 2^-29 of a row's
 // largest vanish), 16 warps with 16-key tiles (one row over 32768 keys 28.4 us for 24.1 then), adding up in every CTA
 // behind a prefix instead of in a third launch (64 rows over 32768 shared keys 81 us for 66).
@@ -1044,8 +1044,8 @@ static cudaError_t launch_any(Params &p, int d, bool q8, int rows, cudaStream_t 
 // tcgen05 kernel has to widen first, above 3.5 million and 64 rows. Whole calls in us, tcgen05 / mma.sync, rows of
 // each of 8 kv heads at head_dim 128:
 //              64 rows, keys 1024, 4096, 16384     128 rows                         256 rows
-//   bf16       15.3/12.3  17.5/20.6  27.7/43.8     16.6/16.4  18.3/28.2  28.5/72.8   21.9/20.5  24.2/43.2  38.8/131.9
-//   int8       22.9/13.8  25.8/24.0  51.4/49.5     23.4/18.9  26.5/31.8  51.9/79.9   33.5/23.2  35.5/47.8  65.8/141.6
+//   bf16       15.4/12.2  17.9/20.6  28.1/43.8     16.4/16.4  18.5/28.3  28.4/73.0   21.9/20.5  24.3/43.5  39.0/132.3
+//   int8       21.0/13.7  24.6/24.0  49.6/49.6     22.2/19.0  25.0/31.9  49.1/80.2   30.8/23.3  32.8/47.9  61.5/142.3
 static bool prefix_on_tcgen05(const Params &p, int64_t keys, int d, bool q8) {
   const int64_t rows = (int64_t)p.m * p.group, pairs = rows * p.nkv * keys;
   return d >= 64 && p.scale_log2 > 0.f && (q8 ? rows > 64 && pairs > 3500000 : rows > kRows && pairs > 1500000);

@@ -291,7 +291,8 @@ def _cache_q8(what, k, ks, v, vs):
     if k.dtype is not _I8 or v.dtype is not _I8 or ks.dtype is not _F32 or vs.dtype is not _F32:
         raise ValueError(f'{what}: int8 codes and fp32 scales expected')
     shape = k.shape
-    if len(shape) != 3 or v.shape != shape or ks.shape != shape[:2] or vs.shape != ks.shape:
+    heads, cap, _ = shape if len(shape) == 3 else (-1, -1, -1)
+    if v.shape != shape or ks.shape != (heads, cap) or vs.shape != (heads, cap):
         raise ValueError(f'{what}: codes [heads, cap, d] and scales [heads, cap] expected')
     if not (k.is_contiguous() and ks.is_contiguous() and v.is_contiguous() and vs.is_contiguous()):
         raise ValueError(f'{what}: caches must be contiguous')
@@ -375,9 +376,9 @@ def kv_read_q8(k_cache, k_scale, v_cache, v_scale, start, count, *, dtype=torch.
     (k, v) tensors to fill, rows contiguous, one head stride."""
     heads, cap, d = _cache_q8('kv_read_q8', k_cache, k_scale, v_cache, v_scale)
     if out is None:
-        k = k_cache.new_empty((heads, count, d), dtype=dtype)
-        v = torch.empty_like(k)
         stride = count * d
+        k = torch.empty_strided((heads, count, d), (stride, d, 1), dtype=dtype, device=k_cache.device)
+        v = torch.empty_like(k)
     else:
         k, v = out
         _cuda(k, v)

@@ -3,8 +3,8 @@
 
 Codes and scales follow from IEEE operations alone (fp32 product, division, rint), so they are compared exactly.
 Attention: with w the exact weights, A = sum w |V| / sum w bounds the effect of rounding every weight by a relative u to
-u A. u is 2^-11 for the weights of the int8 caches, as f16 would carry them, and 2^-8 for those of the bf16 caches, as bf16
-would (both are carried closer, as the sum of two bf16 values), the output's own rounding 2^-8 |out|; scores are sums of 128 fp32 products and two fp32 roundings more, an error below 2^-14 of the
+u A. u is 2^-11 for the weights of the int8 caches (f16's; they are carried closer, as the sum of two bf16 values) and
+2^-8 for the bf16 weights of the bf16 caches, the output's own rounding 2^-8 |out|; scores are sums of 128 fp32 products and two fp32 roundings more, an error below 2^-14 of the
 score's magnitude sum |q k| scale, which changes a weight by as much relative to itself: 2^-14 (1 + S) A with
 S the largest such sum."""
 import pytest
