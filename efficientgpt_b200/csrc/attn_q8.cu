@@ -18,9 +18,9 @@
 // of its own in shared memory (cp.async, rows past the segment's end filled with zeros), running ahead into the
 // next segment; warps only meet at a segment's end.
 //
-// A prefix runs first, in a launch of its own that leaves partial records (here, or in attn_prefix.cu); the launch over
-// the sequences' own keys is a dependent one that starts beside it and leaves records too, and a third adds both up,
-// a warp to a row.
+// A prefix and the sequences' own keys behind it leave partial records: from one launch, in which the prefix's CTAs come
+// first (4 rows behind 512 bf16 keys a call 15.7 us, 19.5 with a launch for each), or, where attn_prefix.cu takes
+// the prefix, from its launch and a dependent one that starts beside it. A last launch adds both up, a warp to a row.
 //
 // Arithmetic: mma.sync with the query rows as M. Scores of int8 keys, up to 8 rows: q as fixed point X 2^(e - 29),
 // |X| <= 2^30, in four balanced base-256 digits, two of them in the MMA's rows 0-7 and 8-15, so two int8 MMAs per 32
@@ -39,7 +39,7 @@
 // 32768 keys 7.9 / 10.7 / 12.6 / 22.3 us (32768: 69.2 MB, 3.1 TB/s); 16 rows of 32 heads over 1 to 8191 keys 24 us;
 // 64 rows over 32 to 512 keys 22 us. Tried: f16 weights (fewer instructions, but weights below 2^-29 of a row's
 // largest vanish), 16 warps with 16-key tiles (one row over 32768 keys 28.4 us for 24.1 then), adding up in every CTA
-// behind a prefix instead of in a third launch (64 rows over 32768 shared keys 81 us for 66).
+// behind a prefix instead of in a launch for it (64 rows over 32768 shared keys 81 us for 66).
 #include "internal.h"
 #include "common.cuh"
 
@@ -78,8 +78,8 @@ struct Params {
   float *ws;      // partial records of this launch
   unsigned *cnt;  // arrivals at a split segment, by the first CTA of it; zero between calls
   int2 *parts;    // beside a prefix: first record and records of each (sequence, kv head)
-  int keys;       // keys of the shared prefix (the launch over it)
-  Prefix pre;     // of the launch over the sequences' own keys: records to add up; of the prefix's: how it is cut
+  int keys;       // keys of the shared prefix (as its own segments' params)
+  Prefix pre;     // the prefix's records to add up and how its segments are cut
 };
 
 // How the tiles of the launch are cut: a CTA takes `chunk` places of the flat list of segments.
@@ -209,8 +209,8 @@ __device__ __forceinline__ int ceil_div_small(int a, int b) {
 // CTA's part of a segment costs about one round of its warps' tiles besides its rounds, a warp's half a tile besides
 // its tiles, and the slowest warp has the longest segments. Every thread of the CTA calls it.
 template <typename C>
-__device__ __forceinline__ Layout make_layout(const Params &p, int *cum, int *len_of, int *scratch) {
-  const int t = threadIdx.x, lane = t & 31, warp = t >> 5, grid = (int)gridDim.x;
+__device__ __forceinline__ Layout make_layout(const Params &p, int grid, int *cum, int *len_of, int *scratch) {
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   Layout l;
   l.pad = 1, l.solo = false;
   int segs = 0, rounds = 0, longest = 0;  // segments, their rounds and most tiles, of one kv head
@@ -454,7 +454,7 @@ enum Mode { kOwn, kBeside, kPrefix };
 // list, so slots are the pairs' own and a segment's are consecutive. Alone, a segment that one CTA holds goes
 // straight to the output, and a split one's records are added up by the last of its CTAs to get there.
 template <int D, bool Q8, int NR, Mode MODE>
-__global__ void __launch_bounds__(Cfg<Q8, NR>::kThreads, 1) attn_kernel(const Params p) {
+__device__ __forceinline__ void attn_body(const Params &p, int block, int grid) {
   using C = Cfg<Q8, NR>;
   using G = Geo<D, Q8, NR>;
   using S = Smem<D, Q8, NR>;
@@ -465,23 +465,21 @@ __global__ void __launch_bounds__(Cfg<Q8, NR>::kThreads, 1) attn_kernel(const Pa
   extern __shared__ __align__(16) uint8_t smem_raw[];
   S &sm = *(S *)smem_raw;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  if (MODE != kBeside) pdl_wait();  // (what precedes the prefix's launch is done once that has started)
-  pdl_launch_dependents();
   Layout lay;
   if (PREFIX) {
     lay.chunk = p.pre.chunk, lay.pad = p.pre.pad, lay.uncut = 0, lay.solo = false;
     lay.total = p.nkv * p.pre.row_tiles * ceil_div(p.pre.seg_tiles, lay.pad) * lay.pad;
   } else {
-    lay = make_layout<C>(p, sm.cum, sm.len, sm.scratch);
+    lay = make_layout<C>(p, grid, sm.cum, sm.len, sm.scratch);
   }
-  int x0 = (int)min((int64_t)lay.total, (int64_t)blockIdx.x * lay.chunk), x1 = min(lay.total, x0 + lay.chunk);
-  const int stride = (int)gridDim.x * kWarps;  // whole segments to warps: every stride-th
-  int solo_seg = warp * (int)gridDim.x + (int)blockIdx.x;
+  int x0 = (int)min((int64_t)lay.total, (int64_t)block * lay.chunk), x1 = min(lay.total, x0 + lay.chunk);
+  const int stride = grid * kWarps;  // whole segments to warps: every stride-th
+  int solo_seg = warp * grid + block;
   if (lay.solo) {
     while (solo_seg < p.m * p.nkv && sm.len[solo_seg / p.nkv] == 0) solo_seg += stride;
     x0 = 0, x1 = solo_seg < p.m * p.nkv ? lay.total : 0;
   } else if (lay.pad == 1) {  // both cuts at once, in the even and in the odd lanes
-    const int cut = cut_at<TILE, PREFIX>(p, lay, sm.cum, sm.len, (int64_t)(blockIdx.x + (lane & 1)) * lay.chunk);
+    const int cut = cut_at<TILE, PREFIX>(p, lay, sm.cum, sm.len, (int64_t)(block + (lane & 1)) * lay.chunk);
     x0 = __shfl_sync(0xffffffffu, cut, 0), x1 = __shfl_sync(0xffffffffu, cut, 1);
   }
   int split_n = 0;  // segments that this CTA shares with others: its first, its last
@@ -849,7 +847,7 @@ __global__ void __launch_bounds__(Cfg<Q8, NR>::kThreads, 1) attn_kernel(const Pa
       const bool whole = done.start >= x0 && done.end <= x1;
       const bool final = MODE == kOwn && whole;
       const int rows = PREFIX ? kRows : p.group;
-      float *rec = record<D>(p, (int)blockIdx.x + done.index);
+      float *rec = record<D>(p, block + done.index);
       constexpr int kPass = S::kPass;
 #pragma unroll 1
       for (int r0 = 0; r0 < rows; r0 += kPass) {
@@ -888,7 +886,7 @@ __global__ void __launch_bounds__(Cfg<Q8, NR>::kThreads, 1) attn_kernel(const Pa
           (split_n ? split[1] : split[0]) = make_int3(done.index, c0, c1 - c0 + 1);
           ++split_n;
         } else if (done.start >= x0 && threadIdx.x == 0) {  // (a short segment lies in one CTA wherever the even cuts are)
-          p.parts[done.index] = make_int2(whole ? (int)blockIdx.x + done.index : c0 + done.index, whole ? 1 : c1 - c0 + 1);
+          p.parts[done.index] = make_int2(whole ? block + done.index : c0 + done.index, whole ? 1 : c1 - c0 + 1);
         }
       }
       if (!another) break;
@@ -896,12 +894,11 @@ __global__ void __launch_bounds__(Cfg<Q8, NR>::kThreads, 1) attn_kernel(const Pa
     cp_wait<0>();
   }
   if (MODE == kBeside) {
-    for (int e = blockIdx.x * C::kThreads + threadIdx.x; e < p.m * p.nkv; e += gridDim.x * C::kThreads)
+    for (int e = block * C::kThreads + threadIdx.x; e < p.m * p.nkv; e += grid * C::kThreads)
       if (sm.len[e / p.nkv] == 0) p.parts[e] = make_int2(0, 0);
-    pdl_wait();  // the prefix's launch: what waits for this one has waited for both
   }
   if constexpr (MODE == kOwn) {
-    for (int e = blockIdx.x; e < p.m * p.nkv; e += gridDim.x)  // sequences without keys
+    for (int e = block; e < p.m * p.nkv; e += grid)  // sequences without keys
       if (sm.len[e / p.nkv] == 0)
         for (int c = threadIdx.x; c < p.group * D; c += C::kThreads)
           p.out[(e / p.nkv) * p.ldo + (int64_t)(e % p.nkv) * p.group * D + c] = 0;
@@ -949,6 +946,25 @@ __global__ void __launch_bounds__(Cfg<Q8, NR>::kThreads, 1) attn_kernel(const Pa
   }
 }
 
+// The sequences' own keys, alone or beside attn_prefix_kernel's launch.
+template <int D, bool Q8, int NR, Mode MODE>
+__global__ void __launch_bounds__(Cfg<Q8, NR>::kThreads, 1) attn_kernel(const Params p) {
+  if (MODE == kOwn) pdl_wait();  // (what precedes the prefix's launch is done once that has started)
+  pdl_launch_dependents();
+  attn_body<D, Q8, NR, MODE>(p, (int)blockIdx.x, (int)gridDim.x);
+  if (MODE == kBeside) pdl_wait();  // the prefix's launch: what waits for this one has waited for both
+}
+// A prefix (NP query rows in use) and the sequences' own keys (NO) in one launch: the prefix's CTAs first, no CTA waits for
+// another.
+template <int D, bool Q8, int NP, int NO>
+__global__ void __launch_bounds__(Cfg<Q8, NP>::kThreads, 1) attn_both_kernel(const Params pre, const Params own) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int ctas = own.pre.grid;
+  if ((int)blockIdx.x < ctas) attn_body<D, Q8, NP, kPrefix>(pre, (int)blockIdx.x, ctas);
+  else attn_body<D, Q8, NO, kBeside>(own, (int)blockIdx.x - ctas, (int)gridDim.x - ctas);
+}
+
 // Beside a prefix: one (sequence, head) row per warp, its own records and the prefix's. Bound by three dependent round
 // trips to L2 (the segment's parts, then two batches of records): 2048 rows of 19 records 5.6 us.
 constexpr int kAddWarps = 4;
@@ -984,19 +1000,31 @@ __global__ void __launch_bounds__(32 * kAddWarps) add_kernel(const Params p) {
   store_row(p.out + i * p.ldo + (int64_t)h * D + D / 32 * lane, a);
 }
 
-template <int D, bool Q8, int NR, Mode MODE>
-static cudaError_t launch(const Params &p, int grid, cudaStream_t st, bool pdl) {
-  auto fn = attn_kernel<D, Q8, NR, MODE>;
-  const size_t smem = sizeof(Smem<D, Q8, NR>);
-  static int configured[64] = {0};  // the shared-memory opt-in, per device
+// The shared-memory opt-in of a kernel, once per device.
+template <typename F>
+static cudaError_t configure(F *fn, size_t smem, int (&configured)[64]) {
   int dev = 0;
   cudaGetDevice(&dev);
-  if (dev >= 0 && dev < 64 && !configured[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return e;
-    configured[dev] = 1;
-  }
+  if (dev < 0 || dev >= 64 || configured[dev]) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e == cudaSuccess) configured[dev] = 1;
+  return e;
+}
+template <int D, bool Q8, int NR, Mode MODE>
+static cudaError_t launch(const Params &p, int grid, cudaStream_t st, bool pdl) {
+  static int configured[64] = {0};
+  const auto fn = attn_kernel<D, Q8, NR, MODE>;
+  const size_t smem = sizeof(Smem<D, Q8, NR>);
+  if (const cudaError_t e = configure(fn, smem, configured); e != cudaSuccess) return e;
   return launch_kernel((const void *)fn, dim3(grid), dim3(Cfg<Q8, NR>::kThreads), smem, st, pdl, p);
+}
+template <int D, bool Q8, int NP, int NO>
+static cudaError_t launch_both(const Params &pre, const Params &own, int grid, cudaStream_t st, bool pdl) {
+  static int configured[64] = {0};
+  const auto fn = attn_both_kernel<D, Q8, NP, NO>;
+  const size_t smem = std::max(sizeof(Smem<D, Q8, NP>), sizeof(Smem<D, Q8, NO>));
+  if (const cudaError_t e = configure(fn, smem, configured); e != cudaSuccess) return e;
+  return launch_kernel((const void *)fn, dim3(own.pre.grid + grid), dim3(Cfg<Q8, NP>::kThreads), smem, st, pdl, pre, own);
 }
 
 static int row_tiles(int64_t m, int group) { return (int)((m * group + kRows - 1) / kRows); }
@@ -1009,9 +1037,9 @@ static int own_grid(const Params &p) {
   const int64_t most = ((p.cache.cap + C::kTile - 1) / C::kTile + C::kMinChunk - 1) / C::kMinChunk;
   return (int)std::min<int64_t>(free >= max_grid() / 2 ? free : max_grid(), most * p.m * p.nkv);
 }
-// How the prefix's segments are cut: as make_layout does it, on the host; returns the grid.
+// How the prefix's segments are cut: as make_layout does it, on the host.
 template <typename C>
-static int cut_prefix(Params &p) {
+static void cut_prefix(Params &p) {
   Prefix &c = p.pre;
   const int grid = max_grid();
   c.row_tiles = row_tiles(p.m, p.group);
@@ -1025,27 +1053,46 @@ static int cut_prefix(Params &p) {
       break;
     }
   }
-  return c.grid = ceil_div(segs * ceil_div(c.seg_tiles, c.pad) * c.pad, c.chunk);
+  c.grid = ceil_div(segs * ceil_div(c.seg_tiles, c.pad) * c.pad, c.chunk);
 }
 template <bool Q8, int NR, Mode MODE>
 static cudaError_t launch_d(Params &p, int d, cudaStream_t st, bool pdl) {
-  const int grid = MODE == kPrefix ? cut_prefix<Cfg<Q8, NR>>(p) : own_grid<Cfg<Q8, NR>>(p);
+  const int grid = own_grid<Cfg<Q8, NR>>(p);
   p.head_share = grid / p.nkv;
-  return d == 128 ? launch<128, Q8, NR, MODE>(p, grid, st, pdl)
-                  : (d == 64 ? launch<64, Q8, NR, MODE>(p, grid, st, pdl) : launch<32, Q8, NR, MODE>(p, grid, st, pdl));
+  if (d == 128) return launch<128, Q8, NR, MODE>(p, grid, st, pdl);
+  if constexpr (MODE == kOwn)  // (attn_prefix_kernel has no head_dim 32)
+    if (d == 32) return launch<32, Q8, NR, MODE>(p, grid, st, pdl);
+  return launch<64, Q8, NR, MODE>(p, grid, st, pdl);
 }
 template <Mode MODE>
-static cudaError_t launch_any(Params &p, int d, bool q8, int rows, cudaStream_t st, bool pdl) {
-  if (rows <= 8) return q8 ? launch_d<true, 8, MODE>(p, d, st, pdl) : launch_d<false, 8, MODE>(p, d, st, pdl);
+static cudaError_t launch_any(Params &p, int d, bool q8, cudaStream_t st, bool pdl) {
+  if (p.group <= 8) return q8 ? launch_d<true, 8, MODE>(p, d, st, pdl) : launch_d<false, 8, MODE>(p, d, st, pdl);
   return q8 ? launch_d<true, 16, MODE>(p, d, st, pdl) : launch_d<false, 16, MODE>(p, d, st, pdl);
+}
+template <bool Q8, int NP, int NO>
+static cudaError_t launch_both_d(Params &pre, Params &own, int d, cudaStream_t st, bool pdl) {
+  cut_prefix<Cfg<Q8, NP>>(pre);
+  own.pre = pre.pre;
+  const int grid = own_grid<Cfg<Q8, NO>>(own);
+  own.head_share = grid / own.nkv;
+  return d == 128 ? launch_both<128, Q8, NP, NO>(pre, own, grid, st, pdl)
+                  : (d == 64 ? launch_both<64, Q8, NP, NO>(pre, own, grid, st, pdl)
+                             : launch_both<32, Q8, NP, NO>(pre, own, grid, st, pdl));
+}
+static cudaError_t launch_both_any(Params &pre, Params &own, int d, bool q8, cudaStream_t st, bool pdl) {
+  if (own.m * own.group <= 8)
+    return q8 ? launch_both_d<true, 8, 8>(pre, own, d, st, pdl) : launch_both_d<false, 8, 8>(pre, own, d, st, pdl);
+  if (own.group <= 8)
+    return q8 ? launch_both_d<true, 16, 8>(pre, own, d, st, pdl) : launch_both_d<false, 16, 8>(pre, own, d, st, pdl);
+  return q8 ? launch_both_d<true, 16, 16>(pre, own, d, st, pdl) : launch_both_d<false, 16, 16>(pre, own, d, st, pdl);
 }
 // Whether the prefix goes to attn_prefix_kernel (head_dim 64 or 128) or to the mma.sync kernel's 16-row tiles, whose time
 // grows with rows x keys: above 1.5 million (query head, key) pairs of the batch for bf16, and for int8, whose tiles the
 // tcgen05 kernel has to widen first, above 3.5 million and 64 rows. Whole calls in us, tcgen05 / mma.sync, rows of
 // each of 8 kv heads at head_dim 128:
 //              64 rows, keys 1024, 4096, 16384     128 rows                         256 rows
-//   bf16       15.4/12.2  17.9/20.6  28.1/43.8     16.4/16.4  18.5/28.3  28.4/73.0   21.9/20.5  24.3/43.5  39.0/132.3
-//   int8       21.0/13.7  24.6/24.0  49.6/49.6     22.2/19.0  25.0/31.9  49.1/80.2   30.8/23.3  32.8/47.9  61.5/142.3
+//   bf16       15.4/11.8  17.7/20.2  28.1/40.1     16.4/16.5  18.4/27.4  28.5/69.6   22.0/20.4  24.2/39.5  38.6/127.7
+//   int8       21.0/13.2  24.6/23.1  49.6/42.9     22.2/18.7  25.0/30.0  49.1/72.1   30.8/22.7  32.8/41.6  61.5/130.3
 static bool prefix_on_tcgen05(const Params &p, int64_t keys, int d, bool q8) {
   const int64_t rows = (int64_t)p.m * p.group, pairs = rows * p.nkv * keys;
   return d >= 64 && p.scale_log2 > 0.f && (q8 ? rows > 64 && pairs > 3500000 : rows > kRows && pairs > 1500000);
@@ -1107,7 +1154,7 @@ extern "C" int egpt_attn_decode_q8(void *out, int64_t ldo, const void *q, int64_
   p.cache = {(const uint8_t *)k_cache, (const uint8_t *)v_cache, k_scale, v_scale, cap};
   p.position = position, p.m = (int)m, p.nkv = nkv, p.group = nq / nkv, p.scale_log2 = scale * 1.4426950408889634f;
   aq8::set_workspace(p, ws);
-  return check_launch(aq8::launch_any<aq8::kOwn>(p, d, true, p.group, (cudaStream_t)stream, (flags & EGPT_FLAG_PDL) != 0),
+  return check_launch(aq8::launch_any<aq8::kOwn>(p, d, true, (cudaStream_t)stream, (flags & EGPT_FLAG_PDL) != 0),
                       "attn_decode_q8_kernel");
 }
 
@@ -1137,36 +1184,32 @@ extern "C" int egpt_attn_shared_prefix(void *out, int64_t ldo, const void *q, in
   p.position = position, p.m = (int)m, p.nkv = nkv, p.group = nq / nkv, p.scale_log2 = scale * 1.4426950408889634f;
   aq8::set_workspace(p, ws);
   float *pre_rec = p.ws + ((size_t)aq8::max_grid() + (size_t)m * nkv) * aq8::kRows * (d + 2);
-  if (prefix_len > 0) {
-    if (aq8::prefix_on_tcgen05(p, prefix_len, d, q8)) {
-      apx::Args A{};
-      const apx::Shape sh = apx::shape_of(m, p.group, nkv, prefix_len);
-      A.ws = pre_rec, A.prefix = prefix_len, A.m = (int)m, A.nkv = nkv, A.group = p.group, A.scale_log2 = p.scale_log2;
-      A.ks = pk_scale, A.vs = pv_scale, A.cap = prefix_cap;
-      bool maps_ok = false;
-      const cudaError_t e = d == 128 ? (q8 ? apx::launch<128, true>(A, q, ldq, pk, pv, sh, st, pdl, maps_ok)
-                                           : apx::launch<128, false>(A, q, ldq, pk, pv, sh, st, pdl, maps_ok))
-                                     : (q8 ? apx::launch<64, true>(A, q, ldq, pk, pv, sh, st, pdl, maps_ok)
-                                           : apx::launch<64, false>(A, q, ldq, pk, pv, sh, st, pdl, maps_ok));
-      if (!maps_ok) return set_error(EGPT_ERR_ALIGN, "attn_shared_prefix: tensor maps rejected");
-      if (e != cudaSuccess) return check_launch(e, "attn_prefix_kernel");
-      p.pre.grid = nkv * sh.pairs * sh.ranges;
-      p.pre.big = 1, p.pre.seqs = sh.seqs, p.pre.pairs = sh.pairs, p.pre.ranges = sh.ranges;
-    } else {
-      aq8::Params a = p;
-      a.cache = {(const uint8_t *)pk, (const uint8_t *)pv, pk_scale, pv_scale, prefix_cap};
-      a.keys = (int)prefix_len, a.ws = pre_rec;
-      const cudaError_t e = aq8::launch_any<aq8::kPrefix>(a, d, q8, (int)m * p.group, st, pdl);
-      if (e != cudaSuccess) return check_launch(e, "attn_shared_prefix_kernel (prefix)");
-      p.pre = a.pre;
-    }
-    p.pre.rec = pre_rec;
-  }
   p.cache = {(const uint8_t *)tk, (const uint8_t *)tv, tk_scale, tv_scale, cap};
-  if (!p.pre.rec)
-    return check_launch(aq8::launch_any<aq8::kOwn>(p, d, q8, p.group, st, pdl), "attn_shared_prefix_kernel");
-  const cudaError_t e = aq8::launch_any<aq8::kBeside>(p, d, q8, p.group, st, true);
-  if (e != cudaSuccess) return check_launch(e, "attn_shared_prefix_kernel");
+  if (prefix_len == 0) return check_launch(aq8::launch_any<aq8::kOwn>(p, d, q8, st, pdl), "attn_shared_prefix_kernel");
+  p.pre.rec = pre_rec;
+  if (aq8::prefix_on_tcgen05(p, prefix_len, d, q8)) {
+    apx::Args A{};
+    const apx::Shape sh = apx::shape_of(m, p.group, nkv, prefix_len);
+    A.ws = pre_rec, A.prefix = prefix_len, A.m = (int)m, A.nkv = nkv, A.group = p.group, A.scale_log2 = p.scale_log2;
+    A.ks = pk_scale, A.vs = pv_scale, A.cap = prefix_cap;
+    bool maps_ok = false;
+    cudaError_t e = d == 128 ? (q8 ? apx::launch<128, true>(A, q, ldq, pk, pv, sh, st, pdl, maps_ok)
+                                   : apx::launch<128, false>(A, q, ldq, pk, pv, sh, st, pdl, maps_ok))
+                             : (q8 ? apx::launch<64, true>(A, q, ldq, pk, pv, sh, st, pdl, maps_ok)
+                                   : apx::launch<64, false>(A, q, ldq, pk, pv, sh, st, pdl, maps_ok));
+    if (!maps_ok) return set_error(EGPT_ERR_ALIGN, "attn_shared_prefix: tensor maps rejected");
+    if (e != cudaSuccess) return check_launch(e, "attn_prefix_kernel");
+    p.pre.grid = nkv * sh.pairs * sh.ranges;
+    p.pre.big = 1, p.pre.seqs = sh.seqs, p.pre.pairs = sh.pairs, p.pre.ranges = sh.ranges;
+    e = aq8::launch_any<aq8::kBeside>(p, d, q8, st, true);
+    if (e != cudaSuccess) return check_launch(e, "attn_shared_prefix_kernel");
+  } else {
+    aq8::Params a = p;
+    a.cache = {(const uint8_t *)pk, (const uint8_t *)pv, pk_scale, pv_scale, prefix_cap};
+    a.keys = (int)prefix_len, a.ws = pre_rec;
+    const cudaError_t e = aq8::launch_both_any(a, p, d, q8, st, pdl);
+    if (e != cudaSuccess) return check_launch(e, "attn_shared_prefix_both_kernel");
+  }
   const void *fn = d == 128 ? (const void *)aq8::add_kernel<128>
                             : (d == 64 ? (const void *)aq8::add_kernel<64> : (const void *)aq8::add_kernel<32>);
   return check_launch(launch_kernel(fn, dim3((unsigned)((m * nq + aq8::kAddWarps - 1) / aq8::kAddWarps)),
