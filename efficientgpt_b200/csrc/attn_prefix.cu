@@ -87,6 +87,15 @@ __device__ __forceinline__ uint4 lds_4x32(uint32_t at) {
 __device__ __forceinline__ void sts_4x32(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
+// The barrier of the two warps that take it; -> whether both came with ok (every one of the two, whatever its waits returned).
+__device__ __forceinline__ bool both_warps(int barrier, bool ok) {
+  int r;
+  asm volatile("{\n .reg .pred p, q;\n setp.ne.s32 p, %2, 0;\n barrier.cta.red.and.pred q, %1, 64, p;\n selp.s32 %0, 1, 0, q;\n}"
+               : "=r"(r)
+               : "r"(barrier), "r"((int)ok)
+               : "memory");
+  return r != 0;
+}
 // The bf16 values of two codes, exactly (as codes_bf16 of attn_q8.cu).
 __device__ __forceinline__ uint32_t widen2(uint32_t codes, uint32_t select) {
   uint32_t r;
@@ -363,7 +372,8 @@ __global__ void __launch_bounds__(Cfg<D, Q8>::kThreads, 1) attn_prefix_kernel(co
         gtc::mbar_arrive(p_full + s);
       }
       // ---- the record. Once both streams are done the operand tiles are free: a row goes through a place of its own
-      // there and leaves in one bulk copy; alternate blocks' two states are added up first.
+      // there and leaves in one bulk copy; alternate blocks' two states are added up first. Where a wait gave up the sums
+      // are NaN, and with them the outputs: what the record held before is never added up.
       ok = ok && apf::warp_wait(o_done, 0) && (!steps[1] || apf::warp_wait(o_done + 1, 0));
       gtc::tc_fence_after();
       constexpr int kPitch = D + 4;  // floats of a staged row
@@ -385,43 +395,45 @@ __global__ void __launch_bounds__(Cfg<D, Q8>::kThreads, 1) attn_prefix_kernel(co
           }
           *(float2 *)(stage + lane * kPitch + D) = make_float2(m_run, l_sum);
         }
-        asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");  // the quarter's two warps, whatever their waits returned
-        if (s == 0) {
+        ok = both_warps(1 + quarter, ok);
+        if (s == 0 && ok) {
           const float2 ml = *(const float2 *)(other + D);
           const float mx = fmaxf(m_run, ml.x), mz = mx == -INFINITY ? 0.f : mx;
           f0 = apf::ex2(m_run - mz), f1 = apf::ex2(ml.x - mz);
           m_run = mx, l_sum = l_sum * f0 + ml.y * f1;
         }
       }
-      if (ok && !(merge && s == 1)) {
+      if (!(merge && s == 1)) {
         float *rec = A.ws + ((int64_t)blockIdx.x * 2 + s) * record_size(D);
+        if (ok) {
 #pragma unroll
-        for (int c = 0; c < D; c += 32) {
-          uint32_t o[32];
-          apf::tmem_ld32(to + (uint32_t)c, o);
-          apf::tmem_wait_ld();
+          for (int c = 0; c < D; c += 32) {
+            uint32_t o[32];
+            apf::tmem_ld32(to + (uint32_t)c, o);
+            apf::tmem_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 32; e += 4) {
-            float *at = stage + lane * kPitch + c + e;
-            float4 v = make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 1]), __uint_as_float(o[e + 2]),
-                                   __uint_as_float(o[e + 3]));
-            if (merge) {
-              const float4 w = *(const float4 *)at;
-              v = make_float4(v.x * f0 + w.x * f1, v.y * f0 + w.y * f1, v.z * f0 + w.z * f1, v.w * f0 + w.w * f1);
+            for (int e = 0; e < 32; e += 4) {
+              float *at = stage + lane * kPitch + c + e;
+              float4 v = make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 1]), __uint_as_float(o[e + 2]),
+                                     __uint_as_float(o[e + 3]));
+              if (merge) {
+                const float4 w = *(const float4 *)at;
+                v = make_float4(v.x * f0 + w.x * f1, v.y * f0 + w.y * f1, v.z * f0 + w.z * f1, v.w * f0 + w.w * f1);
+              }
+              *(float4 *)at = v;
             }
-            *(float4 *)at = v;
+          }
+          if (row < rows[s]) {  // the row's own copy engine transfer
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(rec + row * D),
+                         "r"(smem_u32(stage + lane * kPitch)), "n"(D * 4)
+                         : "memory");
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
           }
         }
-        if (row < rows[s]) {  // the row's own copy engine transfer
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(rec + row * D),
-                       "r"(smem_u32(stage + lane * kPitch)), "n"(D * 4)
-                       : "memory");
-          asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-          asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-        }
         rec[kRowsT * D + row] = m_run;
-        rec[kRowsT * D + kRowsT + row] = l_sum;
+        rec[kRowsT * D + kRowsT + row] = ok ? l_sum : NAN;
       }
     }
   } else if constexpr (Q8) {

@@ -74,22 +74,21 @@ __device__ __forceinline__ bool mbar_try(uint64_t *bar, unsigned parity) {
                : "memory");
   return ok != 0;
 }
-// Bounded wait; false after a timeout or once another wait of the grid has reported an error.
+// Bounded wait for this CTA's own copies, MMAs and warps; false after a timeout. By time alone: no error elsewhere (a bad
+// position in another kernel, one left from an earlier call) stops what it waits for, and giving up on it would leave the
+// caller with whatever its output held before.
 __device__ bool mbar_wait(uint64_t *bar, unsigned parity) {
   if (mbar_try(bar, parity)) return true;
   const uint64_t t0 = globaltimer_ns();
   for (int it = 0;; ++it) {
     if (mbar_try(bar, parity)) return true;
-    if ((it & 15) == 15) {
-      if (device_error_set()) return false;
-      if (globaltimer_ns() - t0 > kWaitLimitNs) {
-        set_device_error(EGPT_ERR_TIMEOUT);
-        return false;
-      }
+    if ((it & 15) == 15 && globaltimer_ns() - t0 > kWaitLimitNs) {
+      set_device_error(EGPT_ERR_TIMEOUT);
+      return false;
     }
   }
 }
-// Bounded by time only (whatever the error state): used to drain work in flight before the CTA exits.
+// The same without a result: used to drain work in flight before the CTA exits.
 __device__ void mbar_drain(uint64_t *bar, unsigned parity) {
   const uint64_t t0 = globaltimer_ns();
   while (!mbar_try(bar, parity))

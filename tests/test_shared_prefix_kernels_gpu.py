@@ -1,0 +1,76 @@
+"""attn_shared_prefix on each of its prefix kernels, the mma.sync tiles and the tcgen05 kernel, where the shapes and the
+state around a call could lead them astray. Bounds are those of test_kv_q8_gpu.py."""
+import pytest
+import torch
+
+from test_kv_q8_gpu import _cache, _check, _gen, _ops, _poison, _randn
+
+pytestmark = pytest.mark.gpu
+
+# (nq, nkv, m, prefix_len) at head_dim 128: a prefix for the mma.sync tiles and one for the tcgen05 kernel, either dtype
+SMALL, LARGE = (8, 2, 5, 300), (8, 2, 80, 6100)
+
+
+@pytest.fixture(autouse=True)
+def no_error_left():
+    from efficientgpt_b200 import _lib as L
+    L.device_error()
+    yield
+    L.device_error()
+
+
+@pytest.mark.parametrize('q8', [False, True])
+@pytest.mark.parametrize('shape', [SMALL, LARGE])
+def test_a_position_outside_the_cache_costs_its_own_row_alone(cuda, q8, shape):
+    """It is reported, its row attends to the prefix alone, and the other rows are right; and so is a call that starts with
+    the error still set, on a workspace that holds the records of other queries."""
+    from efficientgpt_b200 import _lib as L
+    ops = _ops()
+    nq, nkv, m, prefix_len = shape
+    gen = _gen(m + q8)
+    d, cap = 128, 20
+    prefix, own = _cache(gen, nkv, prefix_len, d, q8), _cache(gen, m * nkv, cap, d, q8)
+    ws = ops.attn_q8_ws(m, nq, nkv, d, cuda)
+    lengths = [i % (cap + 1) for i in range(m)]
+    pos = torch.tensor(lengths, device=cuda) - 1
+    bad = pos.clone()
+    bad[1], bad[3] = cap, -2
+    run = lambda q, p: ops.attn_shared_prefix(q, prefix, own, p, prefix_len, nq, nkv, d, scale=d ** -0.5, ws=ws)  # noqa: E731
+    for _ in range(3):
+        run(_randn(gen, m, nq * d).bfloat16(), pos)  # records of other queries
+        q = _randn(gen, m, nq * d).bfloat16()
+        out = run(q, bad)
+        assert L.device_error(clear=False) == L.EGPT_ERR_SHAPE
+        _check(out, q, nq, nkv, d, d ** -0.5, [0 if i in (1, 3) else n for i, n in enumerate(lengths)], own, prefix,
+               prefix_len)
+        q = _randn(gen, m, nq * d).bfloat16()
+        out = run(q, pos)
+        assert L.device_error() == L.EGPT_ERR_SHAPE
+        _check(out, q, nq, nkv, d, d ** -0.5, lengths, own, prefix, prefix_len)
+
+
+def test_an_error_left_by_another_call_does_not_reach_the_tensor_core_kernels(cuda):
+    """The GEMM, the prefill and the one-row decode attention give the same bits with a device error set as without."""
+    from efficientgpt_b200 import _lib as L
+    ops = _ops()
+    gen = _gen(5)
+    x = _randn(gen, 300, 2048).bfloat16()
+    w = torch.randint(-127, 128, (4096, 2048), dtype=torch.int8, device=cuda, generator=gen)
+    s = (0.01 * torch.rand(4096, device=cuda, generator=gen)).bfloat16()
+    nq, nkv, d, cap = 16, 8, 128, 3000
+    k, v = (_randn(gen, nkv, cap, d).bfloat16() for _ in range(2))
+    q = _randn(gen, 2900, nq * d).bfloat16()
+    last = torch.tensor([cap - 1], device=cuda)
+    ws = ops.attn_ws(1, nq, nkv, d, 16, cuda)
+    runs = [lambda out: ops.gemm_i8_tc(x, w, s, out=out),
+            lambda out: ops.gemm_i8_tc(x[:16], w, s, double_round=False, out=out),
+            lambda out: ops.attn_prefill(q, k, v, 50, nq, nkv, d, scale=d ** -0.5, out=out),
+            lambda out: ops.attn_decode(q[:1], k, v, last, nq, nkv, d, scale=d ** -0.5, ws=ws, out=out)]
+    want = [run(None) for run in runs]
+    row = torch.ones(1, 64, dtype=torch.bfloat16, device=cuda)
+    ops.kv_append_q8(row, row, *ops.kv_cache_q8(1, 4, 64, cuda), last)  # slot 2999 of 4
+    assert L.device_error(clear=False) == L.EGPT_ERR_SHAPE
+    for run, ref in zip(runs, want):
+        out = torch.full_like(ref, float('nan'))
+        assert torch.equal(run(out), ref)
+    assert L.device_error() == L.EGPT_ERR_SHAPE
