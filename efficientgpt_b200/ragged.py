@@ -218,9 +218,10 @@ class RaggedGraphDecoder:
         eng = self.engine
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
-        with torch.cuda.stream(side):  # warm-up outside capture
+        with torch.cuda.stream(side):  # warm-up outside capture, each from the start (the last request's place is left)
             for _ in range(2):
                 eng.positions.zero_()
+                self.col.zero_()
                 self._replay_body()
         torch.cuda.current_stream().wait_stream(side)
         torch.cuda.synchronize()
