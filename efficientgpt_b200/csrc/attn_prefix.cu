@@ -332,7 +332,8 @@ __global__ void __launch_bounds__(Cfg<D, Q8>::kThreads, 1) attn_prefix_kernel(co
             apf::tmem_st32(to + (uint32_t)c, o);
           }
         }
-        const uint64_t nm2 = apf::f2_pack(-m_run, -m_run);
+        const float base = m_run == -INFINITY ? 0.f : m_run;  // (every score so far is -inf: their weights are zeros)
+        const uint64_t nm2 = apf::f2_pack(-base, -base);
         uint64_t sum[2] = {apf::f2_pack(0.f, 0.f), apf::f2_pack(0.f, 0.f)};
         // weights of 32 keys over scores that have been read: bf16 in columns c / 2 ..; int8 in the 32 columns of their
         // own scores, the second parts in the upper 16

@@ -74,3 +74,34 @@ def test_an_error_left_by_another_call_does_not_reach_the_tensor_core_kernels(cu
         out = torch.full_like(ref, float('nan'))
         assert torch.equal(run(out), ref)
     assert L.device_error() == L.EGPT_ERR_SHAPE
+
+
+ONE_TILE = (32, 8, 28, 4100)  # 112 rows of each kv head: alternate blocks of one row tile
+
+
+@pytest.mark.parametrize('q8', [False, True])
+@pytest.mark.parametrize('shape', [SMALL, ONE_TILE, LARGE])
+def test_keys_with_scores_of_minus_infinity_weigh_nothing(cuda, q8, shape):
+    """Whole blocks of them, from a range's first key on: the attention is that over the other keys."""
+    ops = _ops()
+    nq, nkv, m, prefix_len = shape
+    gen = _gen(m + 7 + q8)
+    d, cap = 128, 9
+    prefix, own = _cache(gen, nkv, prefix_len, d, q8), _cache(gen, m * nkv, cap, d, q8)
+    lengths = [i % (cap + 1) for i in range(m)]
+    q = _randn(gen, m, nq, d)
+    q[..., 0] = q[..., 0].abs() + 0.5
+    q = q.bfloat16().view(m, nq * d)
+    away = torch.zeros(prefix_len, dtype=torch.bool, device=cuda)
+    for start, end in ((0, 0.13), (0.4, 0.45), (0.55, 0.8), (0.97, 1)):
+        away[int(start * prefix_len):int(end * prefix_len)] = True
+    if q8:  # -127 of a scale near fp32's largest: past -3.4e38 after any q of half or more
+        prefix[0][:, away] = 0
+        prefix[0][:, away, 0] = -127
+        prefix[1][:, away] = 3e38
+    else:
+        prefix[0][:, away, 0] = float('-inf')
+    pos = torch.tensor(lengths, device=cuda) - 1
+    out = ops.attn_shared_prefix(q, prefix, own, pos, prefix_len, nq, nkv, d, scale=d ** -0.5)
+    seen = [t[:, ~away] for t in prefix]
+    _check(out, q, nq, nkv, d, d ** -0.5, lengths, own, seen, seen[0].shape[1])
