@@ -4,7 +4,7 @@
 //                             over the L_i = position[i] + 1 keys of sequence i's own cache;
 //   egpt_attn_shared_prefix:  the same over prefix_len keys held once and then sequence i's own L_i keys (its tail).
 // K[j] = ks_j kq_j and V[j] = vs_j vq_j for int8 codes kq, vq with one scale per row and head (kv_q8.cu). GQA: head h
-// reads kv head h / group. A row without any key gives zeros.
+// reads kv head h / group. A row without any key, or whose scores are all -inf, gives zeros.
 //
 // Work: a segment is one cache head with the query rows that read it: (i, g) with the group's rows for a sequence's
 // own cache, (g, 16 query rows) for the shared prefix, whose rows are all (sequence, head) pairs of kv head g in a
@@ -127,6 +127,8 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// A row's accumulators over their sum; a sum of zero (no key, or every score -inf) gives zeros.
+__device__ __forceinline__ float inverse_sum(float sum) { return sum == 0.f ? 0.f : 1.f / sum; }
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -436,7 +438,7 @@ __device__ __forceinline__ void add_records(const float *own0, int own_n, int ro
       c += BATCH * parts;
     } while (c < cnt);
   }
-  const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
+  const float inv = inverse_sum(lsum);
 #pragma unroll
   for (int e = 0; e < N; ++e) a[e] *= inv;
 }
@@ -807,7 +809,7 @@ __device__ __forceinline__ void attn_body(const Params &p, int block, int grid) 
         for (int hh = 0; hh < NR / 8; ++hh) {
           const int r = g + 8 * hh;
           if (r < p.group) {
-            const float inv = 1.f / l_part[hh];
+            const float inv = inverse_sum(l_part[hh]);
 #pragma unroll
             for (int j = 0; j < ND; j += 4)
 #pragma unroll
@@ -872,8 +874,12 @@ __device__ __forceinline__ void attn_body(const Params &p, int block, int grid) 
           float a = 0.f;
 #pragma unroll
           for (int w = 0; w < kWarps; ++w) a += sm.merge[w][e / D][e % D];
-          if (final) p.out[done.seq * p.ldo + (int64_t)(done.g * p.group + r0) * D + e] = f32_to_bf16_bits(a / sm.row_l[r0 + e / D]);
-          else rec[r0 * D + e] = a;
+          if (final) {
+            const float l = sm.row_l[r0 + e / D];
+            p.out[done.seq * p.ldo + (int64_t)(done.g * p.group + r0) * D + e] = f32_to_bf16_bits(l == 0.f ? 0.f : a / l);
+          } else {
+            rec[r0 * D + e] = a;
+          }
         }
       }
       if (!final && threadIdx.x < rows) {

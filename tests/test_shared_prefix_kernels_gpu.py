@@ -105,3 +105,35 @@ def test_keys_with_scores_of_minus_infinity_weigh_nothing(cuda, q8, shape):
     out = ops.attn_shared_prefix(q, prefix, own, pos, prefix_len, nq, nkv, d, scale=d ** -0.5)
     seen = [t[:, ~away] for t in prefix]
     _check(out, q, nq, nkv, d, d ** -0.5, lengths, own, seen, seen[0].shape[1])
+
+
+@pytest.mark.parametrize('q8', [False, True])
+@pytest.mark.parametrize('nq,nkv,m,cap,prefix_len', [
+    (4, 2, 1, 300, 0), (32, 2, 1, 300, 0), (4, 2, 1, 20000, 0), (4, 2, 3, 9000, 0),  # one CTA's, split between CTAs
+    (32, 8, 64, 40, 0), (32, 2, 300, 40, 0),                                        # a warp's
+    (8, 2, 5, 60, 300), (32, 2, 5, 60, 300), (32, 8, 64, 40, 150), (32, 8, 28, 40, 4100), (8, 2, 80, 60, 6100)])
+def test_a_row_whose_scores_are_all_minus_infinity_gives_zeros(cuda, q8, nq, nkv, m, cap, prefix_len):
+    """However its keys are cut: as a row without keys. The other kv heads' rows are right."""
+    ops = _ops()
+    gen = _gen(m + cap + q8)
+    d = 128
+    prefix, own = _cache(gen, nkv, max(prefix_len, 1), d, q8), _cache(gen, m * nkv, cap, d, q8)
+    q = _randn(gen, m, nq, d)
+    q[..., 0] = q[..., 0].abs() + 0.5
+    q = q.bfloat16().view(m, nq * d)
+    for cache, heads in ((prefix, slice(0, None, nkv)), (own, slice(0, None, nkv))):  # kv head 0's keys
+        if q8:
+            cache[0][heads] = 0
+            cache[0][heads, :, 0] = -127
+            cache[1][heads] = 3e38
+        else:
+            cache[0][heads, :, 0] = float('-inf')
+    lengths = [cap - i % 3 for i in range(m)]
+    pos = torch.tensor(lengths, device=cuda) - 1
+    out = ops.attn_shared_prefix(q, prefix, own, pos, prefix_len, nq, nkv, d, scale=d ** -0.5).view(m, nkv, -1, d)
+    assert (out[:, 0] == 0).all()
+    rest = lambda t: t.view(-1, nkv, *t.shape[1:])[:, 1:].flatten(0, 1)  # noqa: E731
+    some = slice(0, None, max(1, m // 9))
+    _check(out[some, 1:].reshape(len(lengths[some]), -1), q.view(m, nkv, -1, d)[some, 1:].reshape(len(lengths[some]), -1),
+           nq - nq // nkv, nkv - 1, d, d ** -0.5, lengths[some],
+           [rest(t.view(m, nkv, *t.shape[1:])[some].flatten(0, 1)) for t in own], [rest(t) for t in prefix], prefix_len)
