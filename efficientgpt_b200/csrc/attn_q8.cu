@@ -848,7 +848,7 @@ __device__ __forceinline__ void attn_body(const Params &p, int block, int grid) 
       }
       const bool whole = done.start >= x0 && done.end <= x1;
       const bool final = MODE == kOwn && whole;
-      const int rows = PREFIX ? kRows : p.group;
+      const int rows = PREFIX ? NR : p.group;  // of the record, whose stride is kRows either way
       float *rec = record<D>(p, block + done.index);
       constexpr int kPass = S::kPass;
 #pragma unroll 1

@@ -137,3 +137,28 @@ def test_a_row_whose_scores_are_all_minus_infinity_gives_zeros(cuda, q8, nq, nkv
     _check(out[some, 1:].reshape(len(lengths[some]), -1), q.view(m, nkv, -1, d)[some, 1:].reshape(len(lengths[some]), -1),
            nq - nq // nkv, nkv - 1, d, d ** -0.5, lengths[some],
            [rest(t.view(m, nkv, *t.shape[1:])[some].flatten(0, 1)) for t in own], [rest(t) for t in prefix], prefix_len)
+
+
+@pytest.mark.parametrize('q8', [False, True])
+@pytest.mark.parametrize('d,nq,nkv,m,prefix_len', [(128, 16, 8, 4, 512), (64, 4, 4, 8, 3000), (32, 6, 2, 1, 33)])
+def test_records_of_few_rows_leave_the_others_alone(cuda, q8, d, nq, nkv, m, prefix_len):
+    """Up to 8 query rows behind a prefix: the workspace's prefix records hold 16 rows each (accumulators, then maxima, then
+    sums), of which the upper 8 are not written."""
+    from efficientgpt_b200 import _lib as L
+    ops = _ops()
+    gen = _gen(d + q8)
+    prefix, own = _cache(gen, nkv, prefix_len, d, q8), _cache(gen, m * nkv, 5, d, q8)
+    q = _randn(gen, m, nq * d).bfloat16()
+    ws = ops.attn_q8_ws(m, nq, nkv, d, cuda)
+    up = lambda n: (n + 255) // 256 * 256  # noqa: E731
+    sms, record = L.load().egpt_num_sms(), 16 * (d + 2) * 4
+    first = up(4 * sms) + up(8 * m * nkv) + (sms + m * nkv) * record  # counters, parts and the records of own keys
+    records = ws[first:first + (sms + nkv) * record].view(torch.float32).view(-1, 16 * (d + 2))
+    records.fill_(7.0)
+    lengths = [i % 6 for i in range(m)]
+    out = ops.attn_shared_prefix(q, prefix, own, torch.tensor(lengths, device=cuda) - 1, prefix_len, nq, nkv, d,
+                                 scale=d ** -0.5, ws=ws)
+    _check(out, q, nq, nkv, d, d ** -0.5, lengths, own, prefix, prefix_len)
+    assert (records[:, :8 * d] != 7).any() and (records[:, 16 * d:16 * d + 8] != 7).any()
+    assert (records[:, 8 * d:16 * d] == 7).all()
+    assert (records[:, 16 * d + 8:16 * d + 16] == 7).all() and (records[:, 16 * d + 24:] == 7).all()
