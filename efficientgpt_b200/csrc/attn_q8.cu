@@ -40,12 +40,15 @@
 // 64 rows over 32 to 512 keys 22 us. Tried: f16 weights (fewer instructions, but weights below 2^-29 of a row's
 // largest vanish), 16 warps with 16-key tiles (one row over 32768 keys 28.4 us for 24.1 then), adding up in every CTA
 // behind a prefix instead of in a launch for it (64 rows over 32768 shared keys 81 us for 66).
+#include <cmath>
+
 #include "internal.h"
 #include "common.cuh"
 
 namespace egpt {
 namespace aq8 {
 
+constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kMaxBatch = 512;
 constexpr int kRows = 16;        // query rows per tile (the M of the MMA), and rows of a partial record
 constexpr int kMinKeys = 512;    // keys of a range at least
@@ -1121,7 +1124,7 @@ static int check(const char *what, int64_t ldo, int64_t ldq, const void *out, co
     return set_error(EGPT_ERR_SHAPE, "%s: bad m (1 to %d), cap or leading dimension", what, kMaxBatch);
   if (nkv > (1 << 24) / m || m * nkv * ((cap + 15) / 16) > 0x1fffffff)
     return set_error(EGPT_ERR_SHAPE, "%s: cache too long for the batch", what);
-  if (!(fabsf(scale) <= 3e38f)) return set_error(EGPT_ERR_ARG, "%s: scale must be finite", what);
+  if (!std::isfinite(scale * kLog2e)) return set_error(EGPT_ERR_ARG, "%s: scale log2(e) must be finite", what);
   if ((uintptr_t)out % 16 || (uintptr_t)q % 16 || ldq % 8 || ldo % 8)
     return set_error(EGPT_ERR_ALIGN, "%s: q and out must be 16-byte aligned rows", what);
   if (!ws || ws_bytes < egpt_attn_q8_ws_bytes(m, nq, nkv, d))
@@ -1158,7 +1161,7 @@ extern "C" int egpt_attn_decode_q8(void *out, int64_t ldo, const void *q, int64_
   aq8::Params p{};
   p.out = (uint16_t *)out, p.ldo = ldo, p.q = (const uint16_t *)q, p.ldq = ldq;
   p.cache = {(const uint8_t *)k_cache, (const uint8_t *)v_cache, k_scale, v_scale, cap};
-  p.position = position, p.m = (int)m, p.nkv = nkv, p.group = nq / nkv, p.scale_log2 = scale * 1.4426950408889634f;
+  p.position = position, p.m = (int)m, p.nkv = nkv, p.group = nq / nkv, p.scale_log2 = scale * aq8::kLog2e;
   aq8::set_workspace(p, ws);
   return check_launch(aq8::launch_any<aq8::kOwn>(p, d, true, (cudaStream_t)stream, (flags & EGPT_FLAG_PDL) != 0),
                       "attn_decode_q8_kernel");
@@ -1187,7 +1190,7 @@ extern "C" int egpt_attn_shared_prefix(void *out, int64_t ldo, const void *q, in
   const bool pdl = (flags & EGPT_FLAG_PDL) != 0;
   aq8::Params p{};
   p.out = (uint16_t *)out, p.ldo = ldo, p.q = (const uint16_t *)q, p.ldq = ldq;
-  p.position = position, p.m = (int)m, p.nkv = nkv, p.group = nq / nkv, p.scale_log2 = scale * 1.4426950408889634f;
+  p.position = position, p.m = (int)m, p.nkv = nkv, p.group = nq / nkv, p.scale_log2 = scale * aq8::kLog2e;
   aq8::set_workspace(p, ws);
   float *pre_rec = p.ws + ((size_t)aq8::max_grid() + (size_t)m * nkv) * aq8::kRows * (d + 2);
   p.cache = {(const uint8_t *)tk, (const uint8_t *)tv, tk_scale, tv_scale, cap};

@@ -109,3 +109,12 @@ def test_wrappers_refuse_cpu_tensors_and_bad_layouts():
         ops._cache_q8('x', cache[0][:, ::2], cache[1][:, ::2], cache[2][:, ::2], cache[3][:, ::2])
     with pytest.raises(ValueError, match='fp32 scales'):
         ops._cache_q8('x', cache[0], cache[1].half(), cache[2], cache[3].half())
+
+
+@pytest.mark.parametrize('scale', [2.4e38, 3e38, -2.4e38, float('-inf')])
+def test_a_scale_that_is_infinite_in_log2_units_is_refused(scale):
+    """Scores are taken in log2 units: scale log2(e) has to be a finite fp32 value too (scale up to 2.35e38)."""
+    assert _decode(scale=scale) == L.EGPT_ERR_ARG
+    assert L.load().egpt_attn_shared_prefix(X, 512, X, 512, X, X, X, X, 8, 4, X, X, X, X, 8, X, 1, 4, 2, 128, scale, L.EGPT_I8,
+                                            X, WS, 0, None) == L.EGPT_ERR_ARG
+    assert 'log2' in L.last_error()
