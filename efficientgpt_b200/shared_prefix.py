@@ -122,12 +122,21 @@ class SharedPrefixEngine(RaggedEngine):
 
 
 class SharedPrefixGraphDecoder(RaggedGraphDecoder):
-    """SharedPrefixEngine with the step captured once per prefix as a CUDA graph: set_prefix(ids), then any number of
-    generate(prompts, lengths, count) -> tokens [B, count] (int64, on the device)."""
+    """SharedPrefixEngine with the step captured as a CUDA graph: set_prefix(ids), then any number of
+    generate(prompts, lengths, count) -> tokens [B, count] (int64, on the device). The captured step holds the prefix's
+    length, so a prefix of another length is captured anew at the next request."""
 
     def __init__(self, model, batch, prefix_capacity, capacity, kv_dtype=torch.bfloat16):
         self._init(SharedPrefixEngine(model, batch, prefix_capacity, capacity, kv_dtype=kv_dtype))
 
     def set_prefix(self, ids):
         self.engine.set_prefix(ids)
-        self.graph = None  # the step holds the prefix length
+
+    def _capture(self):
+        super()._capture()
+        self.captured_len = self.engine.prefix_len
+
+    def generate(self, prompts, lengths, count):
+        if self.graph is not None and self.captured_len != self.engine.prefix_len:
+            self.graph = None
+        return super().generate(prompts, lengths, count)

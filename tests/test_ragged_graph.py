@@ -90,3 +90,35 @@ def test_every_prefix_answers_the_largest_request(cuda):
         want = eng.generate_eager(prompts, lengths, cap - 1)
         dec.set_prefix(prefix)
         assert torch.equal(dec.generate(prompts, lengths, cap - 1), want)
+
+
+def test_a_prefix_of_another_length_is_captured_however_it_was_set(monkeypatch):
+    from efficientgpt_b200.shared_prefix import SharedPrefixGraphDecoder
+    dec = SharedPrefixGraphDecoder.__new__(SharedPrefixGraphDecoder)
+    dec._init(_Engine(1, 8))
+    _stub_cuda(monkeypatch, dec)
+    captured = []
+    capture = dec._capture
+    dec._capture = lambda: (captured.append(dec.engine.prefix_len), capture())
+    for setter, n in ((dec.set_prefix, 5), (dec.set_prefix, 5), (dec.engine.set_prefix, 3), (dec.set_prefix, 5)):
+        setter(torch.zeros(n, dtype=torch.long))
+        for _ in range(2):
+            dec.generate(torch.tensor([[1]]), torch.tensor([1]), 4)
+    assert captured == [5, 3, 5]
+
+
+@pytest.mark.gpu
+def test_a_prefix_set_on_the_engine_is_the_one_that_is_decoded_behind(cuda):
+    from efficientgpt_b200.int8_linear import quantize_model
+    from efficientgpt_b200.shared_prefix import SharedPrefixEngine, SharedPrefixGraphDecoder
+    cfg = gi.tiny_config()
+    cfg.initializer_range = 0.05
+    model = gi.build_model(cfg, seed=3).cuda()
+    quantize_model(model, scale_dtype=torch.bfloat16)
+    ids = torch.randint(0, 512, (90,), generator=torch.Generator().manual_seed(9)).cuda()
+    prompts, lengths = torch.tensor([[5, 9], [6, 2]]).cuda(), torch.tensor([2, 1])
+    dec, eng = SharedPrefixGraphDecoder(model, 2, 90, 30), SharedPrefixEngine(model, 2, 90, 30)
+    for prefix in (ids[:20], ids, ids[:3], ids[40:43]):
+        eng.set_prefix(prefix)
+        dec.engine.set_prefix(prefix)
+        assert torch.equal(dec.generate(prompts, lengths, 24), eng.generate_eager(prompts, lengths, 24))
