@@ -78,6 +78,7 @@ SIGNATURES = {
     'egpt_attn_decode_q8': (I32, [P, I64, P, I64, P, P, P, P, I64, P, I64, I32, I32, I32, F32, P, SZ, U32, P]),
     'egpt_attn_shared_prefix': (I32, [P, I64, P, I64, P, P, P, P, I64, I64, P, P, P, P, I64, P, I64, I32, I32, I32, F32,
                                       I32, P, SZ, U32, P]),
+    'egpt_attn_shared_prefix_on_tcgen05': (I32, [I64, I32, I32, I32, I64, F32, I32]),
     'egpt_argmax_rows': (I32, [P, P, I64, I64, I64, I32, P]),
     'egpt_sample_ws_bytes': (SZ, [I64]),
     'egpt_attn_prefill': (I32, [P, I64, P, I64, P, P, I64, I64, I64, I32, I32, I32, F32, P]),

@@ -1102,9 +1102,9 @@ static cudaError_t launch_both_any(Params &pre, Params &own, int d, bool q8, cud
 //              64 rows, keys 1024, 4096, 16384     128 rows                         256 rows
 //   bf16       15.4/11.8  17.7/20.2  28.1/40.1     16.4/16.5  18.4/27.4  28.5/69.6   22.0/20.4  24.2/39.5  38.6/127.7
 //   int8       21.0/13.2  24.6/23.1  49.6/42.9     22.2/18.7  25.0/30.0  49.1/72.1   30.8/22.7  32.8/41.6  61.5/130.3
-static bool prefix_on_tcgen05(const Params &p, int64_t keys, int d, bool q8) {
-  const int64_t rows = (int64_t)p.m * p.group, pairs = rows * p.nkv * keys;
-  return d >= 64 && p.scale_log2 > 0.f && (q8 ? rows > 64 && pairs > 3500000 : rows > kRows && pairs > 1500000);
+static bool prefix_on_tcgen05(int64_t m, int group, int nkv, int64_t keys, int d, float scale, bool q8) {
+  const int64_t rows = m * group, pairs = rows * nkv * keys;
+  return d >= 64 && scale > 0.f && (q8 ? rows > 64 && pairs > 3500000 : rows > kRows && pairs > 1500000);
 }
 // The workspace: arrival counters, one per CTA (a CTA is the first of at most one split segment) whatever the call's
 // sizes, so that calls of different sizes can share it; the segments' (first record, records) pairs; the records.
@@ -1167,6 +1167,12 @@ extern "C" int egpt_attn_decode_q8(void *out, int64_t ldo, const void *q, int64_
                       "attn_decode_q8_kernel");
 }
 
+extern "C" int egpt_attn_shared_prefix_on_tcgen05(int64_t m, int nq, int nkv, int d, int64_t prefix_len, float scale,
+                                                  int cache_dtype) {
+  return m >= 1 && nkv >= 1 && nq >= nkv && (d == 64 || d == 128) && prefix_len >= 1 &&
+         aq8::prefix_on_tcgen05(m, nq / nkv, nkv, prefix_len, d, scale * aq8::kLog2e, cache_dtype == EGPT_I8);
+}
+
 extern "C" int egpt_attn_shared_prefix(void *out, int64_t ldo, const void *q, int64_t ldq, const void *pk,
                                        const float *pk_scale, const void *pv, const float *pv_scale, int64_t prefix_cap,
                                        int64_t prefix_len, const void *tk, const float *tk_scale, const void *tv,
@@ -1196,7 +1202,7 @@ extern "C" int egpt_attn_shared_prefix(void *out, int64_t ldo, const void *q, in
   p.cache = {(const uint8_t *)tk, (const uint8_t *)tv, tk_scale, tv_scale, cap};
   if (prefix_len == 0) return check_launch(aq8::launch_any<aq8::kOwn>(p, d, q8, st, pdl), "attn_shared_prefix_kernel");
   p.pre.rec = pre_rec;
-  if (aq8::prefix_on_tcgen05(p, prefix_len, d, q8)) {
+  if (aq8::prefix_on_tcgen05(m, p.group, nkv, prefix_len, d, p.scale_log2, q8)) {
     apx::Args A{};
     const apx::Shape sh = apx::shape_of(m, p.group, nkv, prefix_len);
     A.ws = pre_rec, A.prefix = prefix_len, A.m = (int)m, A.nkv = nkv, A.group = p.group, A.scale_log2 = p.scale_log2;

@@ -237,6 +237,9 @@ EGPT_API int egpt_attn_shared_prefix(void *out, int64_t ldo, const void *q, int6
                                      const float *tv_scale, int64_t cap, const int64_t *position, int64_t m, int nq,
                                      int nkv, int d, float scale, int cache_dtype, void *ws, size_t ws_bytes,
                                      unsigned flags, void *stream);
+/* 1 if a call of these sizes takes its prefix to the tcgen05 kernel, 0 if to the mma.sync tiles (or there is none). */
+EGPT_API int egpt_attn_shared_prefix_on_tcgen05(int64_t m, int nq, int nkv, int d, int64_t prefix_len, float scale,
+                                                int cache_dtype);
 
 /* ---- argmax over rows of bf16/fp32 logits -----------------------------------------------------------
  * replaces: logits[:, -1].argmax(-1) (research/realmodel/fast_decode.py:48,84): first index on ties. */

@@ -118,3 +118,13 @@ def test_a_scale_that_is_infinite_in_log2_units_is_refused(scale):
     assert L.load().egpt_attn_shared_prefix(X, 512, X, 512, X, X, X, X, 8, 4, X, X, X, X, 8, X, 1, 4, 2, 128, scale, L.EGPT_I8,
                                             X, WS, 0, None) == L.EGPT_ERR_ARG
     assert 'log2' in L.last_error()
+
+
+def test_the_query_for_the_prefix_kernel():
+    on = L.load().egpt_attn_shared_prefix_on_tcgen05
+    for dtype in (L.EGPT_BF16, L.EGPT_I8):
+        assert on(64, 32, 8, 128, 32768, 0.1, dtype) == 1
+        assert on(64, 32, 8, 64, 32768, 0.1, dtype) == 1
+        for args in ((64, 32, 8, 32, 32768, 0.1), (64, 32, 8, 128, 32768, -0.1), (64, 32, 8, 128, 32768, 0.0),
+                     (4, 16, 8, 128, 512, 0.1), (64, 32, 8, 128, 0, 0.1), (0, 32, 8, 128, 9, 0.1), (64, 32, 0, 128, 9, 0.1)):
+            assert on(*args, dtype) == 0

@@ -162,3 +162,76 @@ def test_records_of_few_rows_leave_the_others_alone(cuda, q8, d, nq, nkv, m, pre
     assert (records[:, :8 * d] != 7).any() and (records[:, 16 * d:16 * d + 8] != 7).any()
     assert (records[:, 8 * d:16 * d] == 7).all()
     assert (records[:, 16 * d + 8:16 * d + 16] == 7).all() and (records[:, 16 * d + 24:] == 7).all()
+
+
+def _on_tcgen05(m, nq, nkv, d, prefix_len, q8):
+    from efficientgpt_b200 import _lib as L
+    return L.load().egpt_attn_shared_prefix_on_tcgen05(m, nq, nkv, d, prefix_len, d ** -0.5, L.EGPT_I8 if q8 else L.EGPT_BF16)
+
+
+def _shared_prefix_case(cuda, q8, d, nq, nkv, m, prefix_len, seqs):
+    """Against fp64 on the sequences `seqs` (every row is run), NaN in all that must not be read, strided rows of q and
+    out; twice on one workspace, with the same bits."""
+    ops = _ops()
+    gen = _gen(m * 31 + prefix_len + q8 + d)
+    cap = 40
+    lengths = [(0, 1, 40, 17, 16, 33)[i % 6] for i in range(m)]
+    prefix, own = _cache(gen, nkv, prefix_len + 5, d, q8), _cache(gen, m * nkv, cap, d, q8)
+    _poison(prefix, slice(None), prefix_len)
+    for i, n in enumerate(lengths):
+        _poison(own, slice(i * nkv, (i + 1) * nkv), n)
+    q = _randn(gen, m, nq * d + 24).bfloat16()[:, 8:8 + nq * d]
+    wide = torch.full((m, nq * d + 16), 5.0, dtype=torch.bfloat16, device=cuda)
+    out = wide[:, 8:8 + nq * d]
+    ws, pos = ops.attn_q8_ws(m, nq, nkv, d, cuda), torch.tensor(lengths, device=cuda) - 1
+    run = lambda rows: ops.attn_shared_prefix(rows, prefix, own, pos, prefix_len, nq, nkv, d, scale=d ** -0.5, ws=ws, out=out)  # noqa: E731
+    first = run(q).clone()
+    run(_randn(gen, m, nq * d).bfloat16())  # records of other queries
+    assert torch.equal(run(q), first)
+    assert (wide[:, :8] == 5).all() and (wide[:, 8 + nq * d:] == 5).all()
+    heads = [i * nkv + g for i in seqs for g in range(nkv)]
+    _check(out[seqs], q[seqs], nq, nkv, d, d ** -0.5, [lengths[i] for i in seqs], [t[heads] for t in own], prefix, prefix_len)
+    from efficientgpt_b200 import _lib as L
+    assert L.device_error() == 0
+
+
+@pytest.mark.parametrize('q8', [False, True])
+@pytest.mark.parametrize('d', [64, 128])
+@pytest.mark.parametrize('nq,nkv,m,prefix_len', [
+    # one row tile of 128 rows, its blocks taken in turn by two streams: 3 and 4 blocks to a range, the last one of 4 keys;
+    # whole blocks; 126 rows (groups of 3 and 9); 16 heads to one
+    (32, 8, 28, 4100), (32, 8, 28, 5120), (6, 2, 42, 14001), (27, 3, 14, 9500), (16, 1, 8, 28001),
+    # one row tile, ranges of one block, of two and of three
+    (220, 220, 128, 127), (110, 110, 128, 250), (80, 80, 128, 384),
+    # two row tiles: the second with one sequence; partly filled; full
+    (32, 8, 33, 3500), (6, 2, 60, 9999), (64, 4, 16, 3700),
+    # three; 64, over one block
+    (8, 2, 80, 6100), (64, 4, 512, 110)])
+def test_every_shape_of_the_tcgen05_prefix(cuda, q8, d, nq, nkv, m, prefix_len):
+    assert _on_tcgen05(m, nq, nkv, d, prefix_len, q8)
+    step = max(1, m * nkv // 400)  # the ends of every row tile and some between
+    tile = 128 // (nq // nkv)
+    seqs = sorted({i for i in range(m) if i % step == 0 or i % tile in (0, tile - 1) and m * nkv < 3000} | {m - 1})
+    _shared_prefix_case(cuda, q8, d, nq, nkv, m, prefix_len, seqs)
+
+
+@pytest.mark.parametrize('d', [64, 128])
+@pytest.mark.parametrize('nq,nkv,m,prefix_len', [(4, 1, 5, 80001), (4, 4, 40, 10000), (6, 2, 11, 25000)])
+def test_bf16_prefixes_of_few_rows_on_tcgen05(cuda, d, nq, nkv, m, prefix_len):
+    """17 to 64 rows of each kv head: two or three of the four warps of a stream have none."""
+    assert _on_tcgen05(m, nq, nkv, d, prefix_len, False) and not _on_tcgen05(m, nq, nkv, d, prefix_len, True)
+    _shared_prefix_case(cuda, False, d, nq, nkv, m, prefix_len, list(range(m)))
+
+
+@pytest.mark.parametrize('q8', [False, True])
+@pytest.mark.parametrize('d,nq,nkv,m,prefix_len', [(128, 16, 8, 16, 700), (64, 40, 5, 6, 300), (32, 32, 8, 64, 9000)])
+def test_prefixes_on_the_mma_tiles(cuda, q8, d, nq, nkv, m, prefix_len):
+    assert not _on_tcgen05(m, nq, nkv, d, prefix_len, q8)
+    _shared_prefix_case(cuda, q8, d, nq, nkv, m, prefix_len, list(range(0, m, 5)))
+
+
+def test_the_shapes_above_take_the_kernels_they_name(cuda):
+    for q8 in (False, True):
+        for shape, want in ((SMALL, 0), (LARGE, 1), (ONE_TILE, 1)):
+            nq, nkv, m, prefix_len = shape
+            assert _on_tcgen05(m, nq, nkv, 128, prefix_len, q8) == want
