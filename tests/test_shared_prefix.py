@@ -168,3 +168,40 @@ def test_engine_refusals(cuda):
         eng.set_prefix(torch.zeros(17, dtype=torch.long))
     with pytest.raises(ValueError, match='prefix length'):
         eng.set_prefix(torch.zeros(0, dtype=torch.long))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('kv_dtype,heads', [(torch.bfloat16, 8), (torch.int8, 16)])
+def test_long_prefix_on_the_tcgen05_kernel_decodes_as_the_joined_sequences(cuda, kv_dtype, heads):
+    """A batch and a prefix that take attn_shared_prefix to the tcgen05 kernel, in the engine (4 query heads
+    to one with bf16 caches, the most that the ragged engine takes; 8 with int8, whose rule wants more than 64 rows)."""
+    from efficientgpt_b200 import _lib as L
+    from efficientgpt_b200.int8_linear import quantize_model
+    from efficientgpt_b200.ragged import RaggedEngine
+    from efficientgpt_b200.shared_prefix import SharedPrefixEngine
+    cfg = gi.tiny_config()
+    cfg.initializer_range = 0.05
+    cfg.hidden_size, cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim = 256, heads, 2, 128
+    cfg.max_position_embeddings = 16384
+    model = gi.build_model(cfg, seed=3).cuda()
+    quantize_model(model, scale_dtype=torch.bfloat16)
+    batch, prefix = 16, 14001
+    assert L.load().egpt_attn_shared_prefix_on_tcgen05(
+        batch, heads, 2, 128, prefix, 128 ** -0.5, L.EGPT_I8 if kv_dtype is torch.int8 else L.EGPT_BF16)
+    prompts, lengths = _batch(batch, 21, seed=4)
+    ids = torch.randint(0, 512, (prefix,), generator=torch.Generator().manual_seed(5)).cuda()
+    shared = SharedPrefixEngine(model, batch, prefix, 40, kv_dtype=kv_dtype)
+    shared.set_prefix(ids)
+    shared.prefill(prompts.cuda(), lengths)
+    joined = RaggedEngine(model, batch, prefix + 40, kv_dtype=kv_dtype)
+    nkv = shared.base.nkv
+    for i in range(shared.base.n_layers):
+        for dst, head, tail in zip(joined.kv[i], shared.prefix[i], shared.kv[i]):
+            for r in range(batch):
+                h = slice(r * nkv, (r + 1) * nkv)
+                dst[h, :prefix] = head
+                dst[h, prefix:] = tail[h]
+    joined.tokens.copy_(shared.tokens)
+    joined.positions.copy_(shared.positions + prefix)
+    _follow(shared, joined, 6)
+    assert L.device_error() == 0
