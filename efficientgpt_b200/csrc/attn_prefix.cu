@@ -22,13 +22,17 @@
 // A row tile's range ends with a partial record (unnormalised output, maximum, sum of each row) for add_kernel. With bf16 caches
 // weights enter P.V as bf16 relative to the maximum in use, as in the other bf16 attention kernels; with int8 caches as
 // the sum of two bf16 values (16 bits), a second P.V: the values' own rounding is then the only one that counts.
-// Everything else is fp32. Every wait is bounded; issued loads and MMAs are drained before the CTA exits.
+// Everything else is fp32. Every wait is bounded by time; issued loads and MMAs are drained before the CTA exits.
 //
-// What bounds it (d = 128, one step = two streams' blocks): shared memory, which the MMAs read at 128 bytes a clock. With
-// bf16 caches a step's operands are 256 KB, 1.1 us, as long as its exponentials take (16 a clock); a step takes 1.33 us.
-// 256 rows of each of 8 kv heads over 32768 keys: 47 us with 3 us to the first scores and 3.5 us for the records, 34.4
-// GFLOP at 730 TFLOP/s (44% of measured); 64 rows: 25 us for the 134 MB of the prefix (5.4 TB/s, 82% of a measured
-// copy). int8: the second P.V, the widening and the scales make it 480 KB, 2 us; a step takes 2.2 us.
+// What bounds it (d = 128, one step = two streams' blocks): the chain of a stream's step, not a unit. P lies over S, so a
+// stream's next scores wait for its P.V, and its step is scores, softmax and P.V in a row: the scores are read twice, 32
+// columns at a time, each read waited for, and P.V starts once all 128 weights of every row are written; the other stream
+// hides part of that. With 256 rows of each of 8 kv heads a step takes 2.2 us with bf16 caches (by the slope over 32768 to
+// 131072 keys), where the MMAs' reads of shared memory (192 KB at 128 bytes a clock) are 0.8 us and the exponentials (16
+// a clock) 1.0, and 5.1 us with int8, whose scaled scores go back to TMEM between the two reads, whose weights enter
+// twice and whose codes are widened by four warps in the order of the blocks. Whole calls on the device, 256 rows over
+// 32768 keys without own keys: 50 us bf16 (34.4 GFLOP, 690 TFLOP/s, 41% of measured), 99 us int8; 64 rows: 35 us bf16
+// (134 MB, 3.8 TB/s; each further 32768 keys add 18.5 us, which is HBM), 72 us int8.
 #include "internal.h"
 #include "common.cuh"
 
@@ -87,13 +91,15 @@ __device__ __forceinline__ uint4 lds_4x32(uint32_t at) {
 __device__ __forceinline__ void sts_4x32(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
-// The barrier of the two warps that take it; -> whether both came with ok (every one of the two, whatever its waits returned).
+// The barrier of the two warps that take it (both do, whatever their waits returned); -> whether both came with ok.
 __device__ __forceinline__ bool both_warps(int barrier, bool ok) {
   int r;
-  asm volatile("{\n .reg .pred p, q;\n setp.ne.s32 p, %2, 0;\n barrier.cta.red.and.pred q, %1, 64, p;\n selp.s32 %0, 1, 0, q;\n}"
-               : "=r"(r)
-               : "r"(barrier), "r"((int)ok)
-               : "memory");
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.s32 p, %2, 0;\n"
+      " barrier.cta.red.and.pred q, %1, 64, p;\n selp.s32 %0, 1, 0, q;\n}"
+      : "=r"(r)
+      : "r"(barrier), "r"((int)ok)
+      : "memory");
   return r != 0;
 }
 // The bf16 values of two codes, exactly (as codes_bf16 of attn_q8.cu).

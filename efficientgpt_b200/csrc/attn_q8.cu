@@ -20,7 +20,8 @@
 //
 // A prefix and the sequences' own keys behind it leave partial records: from one launch, in which the prefix's CTAs come
 // first (4 rows behind 512 bf16 keys a call 15.7 us, 19.5 with a launch for each), or, where attn_prefix.cu takes
-// the prefix, from its launch and a dependent one that starts beside it. A last launch adds both up, a warp to a row.
+// the prefix, from its launch and a dependent one: on the SMs that the prefix leaves free where those are at least half
+// (a short prefix), else as its CTAs end. A last launch adds both up, a warp to a row.
 //
 // Arithmetic: mma.sync with the query rows as M. Scores of int8 keys, up to 8 rows: q as fixed point X 2^(e - 29),
 // |X| <= 2^30, in four balanced base-256 digits, two of them in the MMA's rows 0-7 and 8-15, so two int8 MMAs per 32
@@ -33,11 +34,11 @@
 // accumulators are fp32; the output is rounded once.
 //
 // What bounds it: HBM for long contexts (the 8 warps' loops run at 5.3 TB/s, 81% of a measured copy: about 800
-// instructions per 32-key tile, a third of them widening V), and for everything else the chain of round trips to L2
-// around them, about 0.5 us each: positions, first tile, and for split segments the fence, the arrival and the other
-// CTAs' records. Measured, d = 128, 8 kv heads, a call on the device: one row of 16 heads over 512 / 2048 / 8192 /
-// 32768 keys 7.9 / 10.7 / 12.6 / 22.3 us (32768: 69.2 MB, 3.1 TB/s); 16 rows of 32 heads over 1 to 8191 keys 24 us;
-// 64 rows over 32 to 512 keys 22 us. Tried: f16 weights (fewer instructions, but weights below 2^-29 of a row's
+// instructions per 32-key tile, a third of them widening V), and for everything else the way in (positions, cuts, first
+// tile: 3 us) and out (the warps' merge, and for split segments the fence, the arrival and the other CTAs' records: 5 us
+// with 18 of those), whose parts have not been timed apart. Measured, d = 128, 8 kv heads, a call on the device: one row
+// of 16 heads over 512 / 2048 / 8192 / 32768 keys 8.2 / 10.8 / 12.7 / 22.1 us (32768: 69.2 MB, 3.1 TB/s); 16 rows of
+// 32 heads over 1 to 8191 keys 24 us; 64 rows over 32 to 512 keys 22 us. Tried: f16 weights (fewer instructions, but weights below 2^-29 of a row's
 // largest vanish), 16 warps with 16-key tiles (one row over 32768 keys 28.4 us for 24.1 then), adding up in every CTA
 // behind a prefix instead of in a launch for it (64 rows over 32768 shared keys 81 us for 66).
 #include <cmath>
@@ -1097,8 +1098,8 @@ static cudaError_t launch_both_any(Params &pre, Params &own, int d, bool q8, cud
 }
 // Whether the prefix goes to attn_prefix_kernel (head_dim 64 or 128) or to the mma.sync kernel's 16-row tiles, whose time
 // grows with rows x keys: above 1.5 million (query head, key) pairs of the batch for bf16, and for int8, whose tiles the
-// tcgen05 kernel has to widen first, above 3.5 million and 64 rows. Whole calls in us, tcgen05 / mma.sync, rows of
-// each of 8 kv heads at head_dim 128:
+// tcgen05 kernel has to widen first, above 3.5 million and 64 rows. Measured at 8 kv heads and head_dim 128 alone, and
+// there 1.6 us off at 256 bf16 rows x 1024 keys. Whole calls in us, tcgen05 / mma.sync, rows of each kv head:
 //              64 rows, keys 1024, 4096, 16384     128 rows                         256 rows
 //   bf16       15.4/11.8  17.7/20.2  28.1/40.1     16.4/16.5  18.4/27.4  28.5/69.6   22.0/20.4  24.2/39.5  38.6/127.7
 //   int8       21.0/13.2  24.6/23.1  49.6/42.9     22.2/18.7  25.0/30.0  49.1/72.1   30.8/22.7  32.8/41.6  61.5/130.3

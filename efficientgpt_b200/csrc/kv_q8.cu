@@ -5,9 +5,9 @@
 // rows (quantize_rows_kernel); a code stands for q s. A scale per row and head keeps every key's and value's error
 // within half a step of its own largest element whatever its neighbours hold, and lets a row be written without
 // touching another one. All kernels here are single passes, bound by HBM for long stretches and by the launch and two
-// round trips to memory for a few rows. Measured with 8 heads of 128: 4096 prompt rows written in 10.8 us (25.3 MB,
-// 2.3 TB/s; 14 us with a division per element), one row in 2.3 us; 32768 rows read
-// back in 38.2 us (203.4 MB, 5.3 TB/s, 81% of a measured copy), one row in 1.6 us.
+// round trips to memory for a few rows. Measured with 8 heads of 128: 4096 prompt rows of bf16 written in 11.5 us
+// (25.4 MB, 2.2 TB/s), of fp32 in 9.6 us (42.2 MB), one row in 2.6 us; 32768 rows read back in 38.6 us (203.4 MB,
+// 5.3 TB/s, 81% of a measured copy).
 #include "internal.h"
 #include "common.cuh"
 
@@ -57,7 +57,8 @@ __device__ __forceinline__ int code_of(float x, float s) {
 }
 
 // Codes of eight elements, one to a byte. A product with 1 / s is within 2^-15 of the quotient, so it decides every code
-// whose quotient is not that near to a half; the others (about one in ten thousand) take the division. The rounding is
+// whose quotient is not that near to a half. One within 1e-4 of a half (one element in 5000) sends its thread's eight
+// to the division (one thread in 625, one warp in 20). The rounding is
 // that of a sum with 1.5 2^23, whose low byte is the code (|x / s| < 127.5 by the choice of s: nothing to clamp).
 __device__ __forceinline__ uint2 codes_of(const float (&x)[8], float s) {
   constexpr float kMagic = 12582912.f;
@@ -80,7 +81,7 @@ __device__ __forceinline__ uint2 codes_of(const float (&x)[8], float s) {
 
 // Rows as they are: D / 8 lanes hold a row, 16 bytes (bf16) or 32 bytes (fp32) each, so it is read once and its maximum
 // needs a few shuffles; a thread takes the K and the V piece of one (row, head), heads innermost as they lie in the rows
-// (4096 rows of 8 heads: 12 us; with the rows innermost, as they lie in the cache, 16).
+// (with the rows innermost, as they lie in the cache, a third slower).
 template <int D, bool F32>
 __global__ void __launch_bounds__(kThreads) append_kernel(AppendParams p) {
   constexpr int kLanes = D / 8, kRows = kThreads / kLanes;
@@ -126,7 +127,9 @@ __global__ void __launch_bounds__(kThreads) append_kernel(AppendParams p) {
 
 // With the decode step's prologue: one warp per head vector of q, k or v (lane l: elements l + 32 i). The norm's sum
 // is added in the order of head_norm_rope's block sum, so q and the row that is quantised have the bits that
-// egpt_qk_norm_rope_kv_append writes.
+// egpt_qk_norm_rope_kv_append writes. 32 q heads, 8 kv heads of 128: one row 2.7 us, 16 ragged rows 3.1 us, both a launch;
+// 4096 rows 60 us int8, 54 us into bf16 caches (92 and 101 MB, 14 and 15 us of HBM): bound by its 2-byte loads and 1- and
+// 2-byte stores, a warp to a vector.
 template <int D>
 __global__ void __launch_bounds__(kThreads) norm_rope_append_kernel(AppendParams p) {
   constexpr int N = D / 32;
@@ -212,7 +215,7 @@ struct ReadParams {
 
 // out[h][r] = q s of row start + r of head h (blockIdx.y; K, then V, in blockIdx.z): 16 codes (one 16-byte load) per
 // thread and row, D / 16 threads to a row, ROWS rows' loads on their way at once: four where that still fills the GPU
-// (32768 rows of 8 heads: 37.9 us, 43.0 with one), one for short stretches (257 rows of 6 heads: 2.2 us, 3.1 with four).
+// (32768 rows of 8 heads: 38.6 us, 43.0 with one), one for short stretches (257 rows of 6 heads: 2.2 us, 3.1 with four).
 template <int D, bool F32, int ROWS>
 __global__ void __launch_bounds__(kThreads) read_kernel(ReadParams p) {
   constexpr int kLanes = D / 16, kStep = kThreads / kLanes;

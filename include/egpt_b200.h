@@ -211,7 +211,8 @@ EGPT_API int egpt_attn_prefill(void *out, int64_t ldo, const void *q, int64_t ld
  * egpt_attn_shared_prefix: the same over prefix_len keys that all m sequences share (caches [nkv][prefix_cap][d]) and
  *   then sequence i's own position[i] + 1 keys (its tail; position counts the tail's slots). cache_dtype EGPT_I8, or
  *   EGPT_BF16 with all scales NULL, for prefix and tails alike. The prefix is read once for the whole batch.
- * A position outside the cache counts as -1 in the attention calls and is reported as EGPT_ERR_SHAPE through
+ * Infinite or NaN values that are attended to give infinite or NaN outputs (a row of a bf16 cache; an int8 row reads as
+ * NaN); those past a sequence's length or the prefix are not read. A position outside the cache counts as -1 in the attention calls and is reported as EGPT_ERR_SHAPE through
  * egpt_device_error; the other rows are not affected, nor is a later call by an error that is still set.
  * The work is cut into equal parts on the device, so a captured graph follows the positions. ws holds
  * egpt_attn_q8_ws_bytes(m, nq, nkv, d) bytes or more, 16-byte aligned, zero-filled once; calls of different sizes can
