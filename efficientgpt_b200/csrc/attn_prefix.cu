@@ -102,10 +102,12 @@ __device__ __forceinline__ bool both_warps(int barrier, bool ok) {
       : "memory");
   return r != 0;
 }
-// The bf16 values of two codes, exactly (as codes_bf16 of attn_q8.cu).
+// The bf16 values of two codes: 0x43 above a byte is 128 + its low seven bits, doubled scale if the sign bit is set; the
+// two parts of the byte apart are 128 + low bits and 128 or 256, and their difference is the code, exactly.
 __device__ __forceinline__ uint32_t widen2(uint32_t codes, uint32_t select) {
   uint32_t r;
   const uint32_t pasted = __byte_perm(codes, 0x43434343u, select);
+  // (the second part with its sign set: a sum is one instruction, a difference two)
   asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(pasted & 0xff7fff7fu), "r"((pasted & 0xff80ff80u) | 0x80008000u));
   return r;
 }

@@ -126,11 +126,9 @@ struct Geo {
   }
 };
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
+using apf::ex2;
+using apx::widen2;
+
 // A row's accumulators over their sum; a sum of zero (no key, or every score -inf) gives zeros.
 __device__ __forceinline__ float inverse_sum(float sum) { return sum == 0.f ? 0.f : 1.f / sum; }
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src) {
@@ -178,16 +176,6 @@ __device__ __forceinline__ uint32_t codes_f16(uint32_t biased, uint32_t select) 
   uint32_t r;
   const uint32_t pasted = __byte_perm(biased, 0x64646464u, select);
   asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(pasted), "r"(0x64806480u));
-  return r;
-}
-
-// The bf16 values of two codes: 0x43 above a byte is 128 + its low seven bits, doubled scale if the sign bit is set; the
-// two parts of the byte apart are 128 + low bits and 128 or 256, and their difference is the code, exactly.
-__device__ __forceinline__ uint32_t codes_bf16(uint32_t codes, uint32_t select) {
-  uint32_t r;
-  const uint32_t pasted = __byte_perm(codes, 0x43434343u, select);
-  // (the second part with its sign set: a sum is one instruction, a difference two)
-  asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(pasted & 0xff7fff7fu), "r"((pasted & 0xff80ff80u) | 0x80008000u));
   return r;
 }
 
@@ -774,7 +762,7 @@ __device__ __forceinline__ void attn_body(const Params &p, int block, int grid) 
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 const uint32_t select = e & 1 ? 0x4342 : 0x4140;
-                const uint32_t b0 = codes_bf16(pair[0][e / 2], select), b1 = codes_bf16(pair[1][e / 2], select);
+                const uint32_t b0 = widen2(pair[0][e / 2], select), b1 = widen2(pair[1][e / 2], select);
                 mma<false>(acc[4 * w + e], pa[u], b0, b1);
                 if (NR == 16) mma<false>(acc[4 * w + e], pb[u % (NR == 16 ? NT / 2 : 1)], b0, b1);
               }
