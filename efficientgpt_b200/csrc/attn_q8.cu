@@ -59,6 +59,10 @@ struct Cache {
   const uint8_t *k, *v;
   const float *ks, *vs;  // null: bf16 rows
   int64_t cap;
+  // in pages (paged.cu): a pool, and for each sequence the pages of its slots
+  const int32_t *table;
+  int64_t ldt, pages;
+  int shift;  // log2 of the rows of a page
 };
 
 // The prefix's partial records, by the kernel that made them.
@@ -447,7 +451,7 @@ enum Mode { kOwn, kBeside, kPrefix };
 // NR: query rows in use, 8 or 16. A (CTA, segment) pair leaves its record in slot CTA + segment: both only grow along the
 // list, so slots are the pairs' own and a segment's are consecutive. Alone, a segment that one CTA holds goes
 // straight to the output, and a split one's records are added up by the last of its CTAs to get there.
-template <int D, bool Q8, int NR, Mode MODE>
+template <int D, bool Q8, int NR, Mode MODE, bool PAGED = false>
 __device__ __forceinline__ void attn_body(const Params &p, int block, int grid) {
   using C = Cfg<Q8, NR>;
   using G = Geo<D, Q8, NR>;
@@ -507,20 +511,60 @@ __device__ __forceinline__ void attn_body(const Params &p, int block, int grid) 
     const uint32_t ring = smem_u32(sm.ring[warp][0]);
     const uint32_t k_dst = ring + lr * G::kRowBytes + ((lc ^ G::k_swz(lr)) * 16);
     const uint32_t v_dst = lr * G::kRowBytes + ((lc ^ G::v_swz(lr)) * 16);
-    auto load_next = [&]() {
+    auto settle = [&]() {  // at the next tile that there is
       while (lx >= ls.end && more) {
         more = advance(ls);
         if (more) lx = ls.start + first;
       }
+    };
+    // pages: the page of row lane % TILE of the next tile, asked for a tile ahead (-1: none, the row reads as zeros)
+    int page = -1;
+    auto find_page = [&]() {
+      settle();
+      const int key = (lx - ls.start) * TILE + lane % TILE;
+      page = -1;
+      if (lx < min(ls.end, x1) && key < ls.len) {
+        page = __ldg(p.cache.table + ls.seq * p.cache.ldt + (key >> p.cache.shift));
+        if (page < 0 || page >= p.cache.pages) {
+          set_device_error(EGPT_ERR_SHAPE);
+          page = -1;
+        }
+      }
+    };
+    if (PAGED) find_page();
+    auto load_next = [&]() {
+      if (!PAGED) settle();
       if (lx < min(ls.end, x1)) {
         const uint32_t st = (uint32_t)(lslot * G::kStageBytes);
         const Cache &c = p.cache;
-        const int key0 = (lx - ls.start) * TILE, left = ls.len - key0;
-        const int64_t row0 = (PREFIX ? ls.g : (int64_t)ls.seq * p.nkv + ls.g) * c.cap + key0;
+        const int key0 = (lx - ls.start) * TILE;
+        int left = ls.len - key0;
+        int64_t row0;
+        if (PAGED) {
+          const int at = __shfl_sync(0xffffffffu, page, 0);
+          row0 = (((int64_t)at * p.nkv + ls.g) << c.shift) + (key0 & ((1 << c.shift) - 1));
+          if (at < 0 && (1 << c.shift) >= TILE) row0 = left = 0;
+        } else {
+          row0 = (PREFIX ? ls.g : (int64_t)ls.seq * p.nkv + ls.g) * c.cap + key0;
+        }
         const uint8_t *kb = c.k + row0 * G::kRowBytes + lane * 16, *vb = c.v + row0 * G::kRowBytes + lane * 16;
         // v_swz(it kStep + lr) = v_swz(it kStep) ^ v_swz(lr) (the row bits it uses do not carry)
         const uint32_t kd = st + k_dst, vd = st + ring + TILE * G::kRowBytes;
-        if (left >= TILE) {
+        int64_t scale_row = row0 + (lane < left ? lane : 0);
+        bool scale_in = lane < left;
+        if (PAGED && (1 << c.shift) < TILE) {  // a tile of several pages
+          const int mask = (1 << c.shift) - 1;
+#pragma unroll
+          for (int it = 0; it < TILE / kStep; ++it) {
+            const int r = it * kStep + lr, at = __shfl_sync(0xffffffffu, page, r);
+            const bool in = r < left && at >= 0;
+            const int64_t row = in ? (((int64_t)at * p.nkv + ls.g) << c.shift) + ((key0 + r) & mask) : 0;
+            cp16z(kd + it * 512, c.k + row * G::kRowBytes + lc * 16, in ? 16 : 0);
+            cp16z(vd + (v_dst ^ (G::v_swz(it * kStep) * 16)) + it * 512, c.v + row * G::kRowBytes + lc * 16, in ? 16 : 0);
+          }
+          scale_in = lane < left && page >= 0;
+          scale_row = scale_in ? (((int64_t)page * p.nkv + ls.g) << c.shift) + ((key0 + lane) & mask) : 0;
+        } else if (left >= TILE) {
 #pragma unroll
           for (int it = 0; it < TILE / kStep; ++it) {
             cp16(kd + it * 512, kb + it * 512);
@@ -536,13 +580,13 @@ __device__ __forceinline__ void attn_body(const Params &p, int block, int grid) 
         }
         if (Q8) {
           const uint32_t sc = ring + st + 2 * TILE * G::kRowBytes + lane * 4;  // [ks of the tile][vs of the tile]
-          const bool in = lane < left;
-          cp4(sc, c.ks + row0 + (in ? lane : 0), in ? 4 : 0);
-          cp4(sc + TILE * 4, c.vs + row0 + (in ? lane : 0), in ? 4 : 0);
+          cp4(sc, c.ks + scale_row, scale_in ? 4 : 0);
+          cp4(sc + TILE * 4, c.vs + scale_row, scale_in ? 4 : 0);
         }
       }
       cp_commit();
       lx += step;
+      if (PAGED) find_page();
       lslot = lslot + 1 == STAGES ? 0 : lslot + 1;
     };
     // the segment's query rows, dims d0 .. d0 + 3 of every 16-dim step: those of the key words that this thread loads
@@ -945,11 +989,11 @@ __device__ __forceinline__ void attn_body(const Params &p, int block, int grid) 
 }
 
 // The sequences' own keys, alone or beside attn_prefix_kernel's launch.
-template <int D, bool Q8, int NR, Mode MODE>
+template <int D, bool Q8, int NR, Mode MODE, bool PAGED>
 __global__ void __launch_bounds__(Cfg<Q8, NR>::kThreads, 1) attn_kernel(const Params p) {
   if (MODE == kOwn) pdl_wait();  // (what precedes the prefix's launch is done once that has started)
   pdl_launch_dependents();
-  attn_body<D, Q8, NR, MODE>(p, (int)blockIdx.x, (int)gridDim.x);
+  attn_body<D, Q8, NR, MODE, PAGED>(p, (int)blockIdx.x, (int)gridDim.x);
   if (MODE == kBeside) pdl_wait();  // the prefix's launch: what waits for this one has waited for both
 }
 // A prefix (NP query rows in use) and the sequences' own keys (NO) in one launch: the prefix's CTAs first, no CTA waits for
@@ -1008,10 +1052,10 @@ static cudaError_t configure(F *fn, size_t smem, int (&configured)[64]) {
   if (e == cudaSuccess) configured[dev] = 1;
   return e;
 }
-template <int D, bool Q8, int NR, Mode MODE>
+template <int D, bool Q8, int NR, Mode MODE, bool PAGED>
 static cudaError_t launch(const Params &p, int grid, cudaStream_t st, bool pdl) {
   static int configured[64] = {0};
-  const auto fn = attn_kernel<D, Q8, NR, MODE>;
+  const auto fn = attn_kernel<D, Q8, NR, MODE, PAGED>;
   const size_t smem = sizeof(Smem<D, Q8, NR>);
   if (const cudaError_t e = configure(fn, smem, configured); e != cudaSuccess) return e;
   return launch_kernel((const void *)fn, dim3(grid), dim3(Cfg<Q8, NR>::kThreads), smem, st, pdl, p);
@@ -1053,19 +1097,19 @@ static void cut_prefix(Params &p) {
   }
   c.grid = ceil_div(segs * ceil_div(c.seg_tiles, c.pad) * c.pad, c.chunk);
 }
-template <bool Q8, int NR, Mode MODE>
+template <bool Q8, int NR, Mode MODE, bool PAGED>
 static cudaError_t launch_d(Params &p, int d, cudaStream_t st, bool pdl) {
   const int grid = own_grid<Cfg<Q8, NR>>(p);
   p.head_share = grid / p.nkv;
-  if (d == 128) return launch<128, Q8, NR, MODE>(p, grid, st, pdl);
+  if (d == 128) return launch<128, Q8, NR, MODE, PAGED>(p, grid, st, pdl);
   if constexpr (MODE == kOwn)  // (attn_prefix_kernel has no head_dim 32)
-    if (d == 32) return launch<32, Q8, NR, MODE>(p, grid, st, pdl);
-  return launch<64, Q8, NR, MODE>(p, grid, st, pdl);
+    if (d == 32) return launch<32, Q8, NR, MODE, PAGED>(p, grid, st, pdl);
+  return launch<64, Q8, NR, MODE, PAGED>(p, grid, st, pdl);
 }
-template <Mode MODE>
+template <Mode MODE, bool PAGED = false>
 static cudaError_t launch_any(Params &p, int d, bool q8, cudaStream_t st, bool pdl) {
-  if (p.group <= 8) return q8 ? launch_d<true, 8, MODE>(p, d, st, pdl) : launch_d<false, 8, MODE>(p, d, st, pdl);
-  return q8 ? launch_d<true, 16, MODE>(p, d, st, pdl) : launch_d<false, 16, MODE>(p, d, st, pdl);
+  if (p.group <= 8) return q8 ? launch_d<true, 8, MODE, PAGED>(p, d, st, pdl) : launch_d<false, 8, MODE, PAGED>(p, d, st, pdl);
+  return q8 ? launch_d<true, 16, MODE, PAGED>(p, d, st, pdl) : launch_d<false, 16, MODE, PAGED>(p, d, st, pdl);
 }
 template <bool Q8, int NP, int NO>
 static cudaError_t launch_both_d(Params &pre, Params &own, int d, cudaStream_t st, bool pdl) {
@@ -1149,11 +1193,33 @@ extern "C" int egpt_attn_decode_q8(void *out, int64_t ldo, const void *q, int64_
     return set_error(EGPT_ERR_ALIGN, "attn_decode_q8: caches must be 16-byte aligned");
   aq8::Params p{};
   p.out = (uint16_t *)out, p.ldo = ldo, p.q = (const uint16_t *)q, p.ldq = ldq;
-  p.cache = {(const uint8_t *)k_cache, (const uint8_t *)v_cache, k_scale, v_scale, cap};
+  p.cache = {(const uint8_t *)k_cache, (const uint8_t *)v_cache, k_scale, v_scale, cap, nullptr, 0, 0, 0};
   p.position = position, p.m = (int)m, p.nkv = nkv, p.group = nq / nkv, p.scale_log2 = scale * aq8::kLog2e;
   aq8::set_workspace(p, ws);
   return check_launch(aq8::launch_any<aq8::kOwn>(p, d, true, (cudaStream_t)stream, (flags & EGPT_FLAG_PDL) != 0),
                       "attn_decode_q8_kernel");
+}
+
+extern "C" int egpt_attn_decode_paged(void *out, int64_t ldo, const void *q, int64_t ldq, const void *k_pages,
+                                      const float *k_scale, const void *v_pages, const float *v_scale, int64_t pages,
+                                      int page_size, const int32_t *table, int64_t ldt, int64_t columns,
+                                      const int64_t *position, int64_t m, int nq, int nkv, int d, float scale, void *ws,
+                                      size_t ws_bytes, unsigned flags, void *stream) {
+  clear_error();
+  pgd::Pool pool{};
+  if (int rc = pgd::pool_of("attn_decode_paged", pool, k_pages, k_scale, v_pages, v_scale, pages, page_size, table, ldt, columns,
+                            m, nkv, d))
+    return rc;
+  if (!out || !q || !position) return set_error(EGPT_ERR_ARG, "attn_decode_paged: null pointer");
+  if (int rc = aq8::check("attn_decode_paged", ldo, ldq, out, q, pool.cap, m, nq, nkv, d, scale, ws, ws_bytes)) return rc;
+  aq8::Params p{};
+  p.out = (uint16_t *)out, p.ldo = ldo, p.q = (const uint16_t *)q, p.ldq = ldq;
+  p.cache = {(const uint8_t *)k_pages, (const uint8_t *)v_pages, k_scale, v_scale, pool.cap, table, ldt, pages, pool.shift};
+  p.position = position, p.m = (int)m, p.nkv = nkv, p.group = nq / nkv, p.scale_log2 = scale * aq8::kLog2e;
+  aq8::set_workspace(p, ws);
+  return check_launch(
+      aq8::launch_any<aq8::kOwn, true>(p, d, k_scale != nullptr, (cudaStream_t)stream, (flags & EGPT_FLAG_PDL) != 0),
+      "attn_decode_paged_kernel");
 }
 
 extern "C" int egpt_attn_shared_prefix_on_tcgen05(int64_t m, int nq, int nkv, int d, int64_t prefix_len, float scale,
@@ -1188,7 +1254,7 @@ extern "C" int egpt_attn_shared_prefix(void *out, int64_t ldo, const void *q, in
   p.position = position, p.m = (int)m, p.nkv = nkv, p.group = nq / nkv, p.scale_log2 = scale * aq8::kLog2e;
   aq8::set_workspace(p, ws);
   float *pre_rec = p.ws + ((size_t)aq8::max_grid() + (size_t)m * nkv) * aq8::kRows * (d + 2);
-  p.cache = {(const uint8_t *)tk, (const uint8_t *)tv, tk_scale, tv_scale, cap};
+  p.cache = {(const uint8_t *)tk, (const uint8_t *)tv, tk_scale, tv_scale, cap, nullptr, 0, 0, 0};
   if (prefix_len == 0) return check_launch(aq8::launch_any<aq8::kOwn>(p, d, q8, st, pdl), "attn_shared_prefix_kernel");
   p.pre.rec = pre_rec;
   if (aq8::prefix_on_tcgen05(m, p.group, nkv, prefix_len, d, p.scale_log2, q8)) {
@@ -1209,7 +1275,7 @@ extern "C" int egpt_attn_shared_prefix(void *out, int64_t ldo, const void *q, in
     if (e != cudaSuccess) return check_launch(e, "attn_shared_prefix_kernel");
   } else {
     aq8::Params a = p;
-    a.cache = {(const uint8_t *)pk, (const uint8_t *)pv, pk_scale, pv_scale, prefix_cap};
+    a.cache = {(const uint8_t *)pk, (const uint8_t *)pv, pk_scale, pv_scale, prefix_cap, nullptr, 0, 0, 0};
     a.keys = (int)prefix_len, a.ws = pre_rec;
     const cudaError_t e = aq8::launch_both_any(a, p, d, q8, st, pdl);
     if (e != cudaSuccess) return check_launch(e, "attn_shared_prefix_both_kernel");

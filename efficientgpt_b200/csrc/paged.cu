@@ -1,0 +1,329 @@
+// The paged KV cache: a batch's key and value rows written to the pages of their sequences, and read back.
+//
+// A pool is `pages` pages of S rows (S a power of two) for every kv head, K and V apart: [page][kv head][S][d], bf16 rows
+// or int8 codes with one fp32 scale a row (kv_q8.cu's quantiser). table[i][c] names the page of slots c S .. c S + S - 1 of
+// sequence i (-1: none). A page's rows of one head lie together, so that attention streams S d elements at a time and
+// a tensor of one page is the contiguous caches' [heads][cap][d] with cap = S.
+#include "internal.h"
+#include "common.cuh"
+
+namespace egpt {
+namespace pgd {
+
+constexpr int kThreads = 256;
+
+struct Pool {
+  void *k, *v;
+  float *ks, *vs;  // null: bf16 rows
+  int64_t pages;
+  int shift;  // log2 of the rows of a page
+  int nkv;
+  const int32_t *table;
+  int64_t ldt, cap;  // slots that a table row has pages for
+};
+
+// The pool row of slot `slot` of sequence `seq` and kv head 0 (head h: + h << shift), -1 without a page; a name outside the
+// pool is reported.
+__device__ __forceinline__ int64_t row_of(const Pool &p, int64_t seq, int64_t slot) {
+  const int32_t page = p.table[seq * p.ldt + (slot >> p.shift)];
+  if (page >= 0 && page < p.pages) return (((int64_t)page * p.nkv) << p.shift) + (slot & ((1 << p.shift) - 1));
+  if (page != -1) set_device_error(EGPT_ERR_SHAPE);
+  return -1;
+}
+
+struct AppendParams {
+  Pool pool;
+  const uint16_t *q, *k, *v;
+  uint16_t *q_out;
+  int64_t ldq, ldk, ldv, ldqo;
+  const int64_t *position, *starts;  // starts null: row i is sequence i's
+  int seqs, m, nq;
+  const uint16_t *q_norm_w, *k_norm_w;
+  float eps;
+  const void *rope_cos, *rope_sin;
+  int rope_f32;
+  int64_t rope_rows, rope_base;
+};
+
+__device__ __forceinline__ void load8(float (&x)[8], const uint16_t *src) {
+  const uint4 a = *(const uint4 *)src;
+  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[2 * e] = bf16_lo(w[e]), x[2 * e + 1] = bf16_hi(w[e]);
+}
+__device__ __forceinline__ void load8(float (&x)[8], const float *src) {
+  const float4 a = ((const float4 *)src)[0], b = ((const float4 *)src)[1];
+  x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+}
+__device__ __forceinline__ uint4 bf16x8(const float (&x)[8]) {
+  uint32_t y[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    y[e] = (uint32_t)f32_to_bf16_bits(x[2 * e]) | ((uint32_t)f32_to_bf16_bits(x[2 * e + 1]) << 16);
+  return make_uint4(y[0], y[1], y[2], y[3]);
+}
+
+// One head vector of q, k or v to D / 16 lanes: lane l holds dims 8 l .. 8 l + 7 and the D / 2 further on that the half-layout
+// rotation pairs them with, so a row is read once in 16-byte pieces, the rotation stays inside a lane, and the norm and
+// the quantiser's maximum take a few shuffles. Norm and rotation are fp32 and rounded once, to bf16 or to a code.
+template <int D, bool Q8>
+__global__ void __launch_bounds__(kThreads) append_kernel(const AppendParams p) {
+  constexpr int kLanes = D / 16, kHalf = D / 2;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int e0 = (int)(threadIdx.x % kLanes) * 8;
+  const unsigned item = blockIdx.x * (unsigned)(kThreads / kLanes) + threadIdx.x / kLanes;
+  const unsigned vectors = p.nq + 2 * p.pool.nkv;
+  const bool live = item < (unsigned)p.m * vectors;
+  const unsigned row = live ? item / vectors : 0, vec = live ? item - row * vectors : 0;
+  const int kind = vec < (unsigned)p.nq ? 0 : (vec < (unsigned)(p.nq + p.pool.nkv) ? 1 : 2);  // q, k, v
+  const int head = (int)vec - (kind == 0 ? 0 : (kind == 1 ? p.nq : p.nq + p.pool.nkv));
+  const uint16_t *src = (kind == 0 ? p.q + row * p.ldq : (kind == 1 ? p.k + row * p.ldk : p.v + row * p.ldv)) +
+                        (int64_t)head * D + e0;
+  float lo[8], hi[8];
+  load8(lo, src);
+  load8(hi, src + kHalf);
+
+  // the row's sequence and slot
+  int64_t seq = row, slot = -1;
+  bool ours = live;  // rows outside every sequence stay as they are
+  if (p.starts) {
+    int a = 0, b = p.seqs + 1;  // the last start at or before the row is in [a, b) if there is one
+    while (b - a > 1) {
+      const int mid = (a + b) >> 1;
+      if (p.starts[mid] <= (int64_t)row) a = mid;
+      else b = mid;
+    }
+    seq = a;
+    ours = live && a < p.seqs && p.starts[a] <= (int64_t)row;
+  }
+  int64_t dst = -1;
+  if (ours) {
+    const int64_t first = p.position[seq];
+    slot = first + (p.starts ? (int64_t)row - p.starts[seq] : 0);
+    const bool in = first >= 0 && slot >= 0 && slot < p.pool.cap && (!p.rope_cos || slot < p.rope_rows - p.rope_base);
+    if (!in && first != -1) set_device_error(EGPT_ERR_SHAPE);  // -1: an idle slot of the batch
+    if (!in) slot = -1;
+    if (slot >= 0 && kind != 0) {
+      dst = row_of(p.pool, seq, slot);
+      if (dst < 0) set_device_error(EGPT_ERR_SHAPE);
+    }
+  }
+  const uint16_t *norm_w = kind == 0 ? p.q_norm_w : (kind == 1 ? p.k_norm_w : nullptr);
+  float ss = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) ss = fmaf(lo[e], lo[e], fmaf(hi[e], hi[e], ss));
+#pragma unroll
+  for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  if (norm_w) {
+    const float inv = rsqrtf(ss / (float)D + p.eps);
+    float w[8];
+    load8(w, norm_w + e0);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) lo[e] = lo[e] * inv * w[e];
+    load8(w, norm_w + kHalf + e0);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) hi[e] = hi[e] * inv * w[e];
+  }
+  if (kind != 2 && p.rope_cos && slot >= 0) {
+    const int64_t at = (slot + p.rope_base) * kHalf + e0;
+    float c[8], s[8];
+    if (p.rope_f32) {
+      load8(c, (const float *)p.rope_cos + at);
+      load8(s, (const float *)p.rope_sin + at);
+    } else {
+      load8(c, (const uint16_t *)p.rope_cos + at);
+      load8(s, (const uint16_t *)p.rope_sin + at);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float a = lo[e], b = hi[e];
+      lo[e] = a * c[e] - b * s[e];
+      hi[e] = b * c[e] + a * s[e];
+    }
+  }
+  uint32_t amax = 0u;
+  if (Q8) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) amax = max(amax, max(kvq::magnitude(lo[e]), kvq::magnitude(hi[e])));
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  }
+  if (kind == 0) {
+    if (!ours) return;
+    const uint4 zero = make_uint4(0u, 0u, 0u, 0u);  // a row without a slot has no position to rotate to
+    uint16_t *out = p.q_out + row * p.ldqo + (int64_t)head * D + e0;
+    *(uint4 *)out = slot >= 0 ? bf16x8(lo) : zero;
+    *(uint4 *)(out + kHalf) = slot >= 0 ? bf16x8(hi) : zero;
+    return;
+  }
+  if (dst < 0) return;
+  dst += (int64_t)head << p.pool.shift;
+  if (Q8) {
+    const float s = kvq::row_scale(amax);
+    int8_t *codes = (int8_t *)(kind == 1 ? p.pool.k : p.pool.v) + dst * D + e0;
+    *(uint2 *)codes = kvq::codes_of(lo, s);
+    *(uint2 *)(codes + kHalf) = kvq::codes_of(hi, s);
+    if (e0 == 0) (kind == 1 ? p.pool.ks : p.pool.vs)[dst] = s;
+  } else {
+    uint16_t *out = (uint16_t *)(kind == 1 ? p.pool.k : p.pool.v) + dst * D + e0;
+    *(uint4 *)out = bf16x8(lo);
+    *(uint4 *)(out + kHalf) = bf16x8(hi);
+  }
+}
+
+struct ReadParams {
+  Pool pool;
+  void *k_out, *v_out;
+  int64_t out_head;  // elements between the heads of the outputs
+  int64_t start, count;
+  const int64_t *starts;  // nullable: every sequence's first slot
+  int seqs;
+};
+
+// out[i nkv + h][r] = row start_i + r of head h of sequence i: 16 stored bytes a thread, of K and of V.
+template <int D, bool Q8, bool F32>
+__global__ void __launch_bounds__(kThreads) read_kernel(const ReadParams p) {
+  constexpr int kElems = Q8 ? 16 : 8, kLanes = D / kElems, kRows = kThreads / kLanes;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int e0 = (int)(threadIdx.x % kLanes) * kElems;
+  for (int h = blockIdx.y; h < p.seqs * p.pool.nkv; h += gridDim.y) {
+    const int seq = h / p.pool.nkv, head = h - seq * p.pool.nkv;
+    const int64_t start = p.starts ? p.starts[seq] : p.start;
+    for (int64_t r = (int64_t)blockIdx.x * kRows + threadIdx.x / kLanes; r < p.count; r += (int64_t)gridDim.x * kRows) {
+      const int64_t slot = start + r;
+      int64_t src = slot >= 0 && slot < p.pool.cap ? row_of(p.pool, seq, slot) : -1;
+      if (src >= 0) src += (int64_t)head << p.pool.shift;
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) {
+        const uint8_t *rows = (const uint8_t *)(kv ? p.pool.v : p.pool.k) + (src * D + e0) * (Q8 ? 1 : 2);
+        const uint4 c = src >= 0 ? *(const uint4 *)rows : make_uint4(0u, 0u, 0u, 0u);
+        const float s = Q8 && src >= 0 ? (kv ? p.pool.vs : p.pool.ks)[src] : 0.f;
+        const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+        const int64_t at = (int64_t)h * p.out_head + r * D + e0;
+        void *out = kv ? p.v_out : p.k_out;
+        if constexpr (!Q8 && !F32) {
+          *(uint4 *)((uint16_t *)out + at) = c;
+        } else {
+#pragma unroll
+          for (int e = 0; e < kElems; e += 8) {
+            float y[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int j = e + i;
+              if (Q8) y[i] = (float)(int8_t)(w[j / 4] >> (8 * (j % 4))) * s;
+              else y[i] = j % 2 ? bf16_hi(w[(j / 2) % 4]) : bf16_lo(w[(j / 2) % 4]);
+            }
+            if (F32) {
+              float4 *dst = (float4 *)((float *)out + at + e);
+              dst[0] = make_float4(y[0], y[1], y[2], y[3]);
+              dst[1] = make_float4(y[4], y[5], y[6], y[7]);
+            } else {
+              *(uint4 *)((uint16_t *)out + at + e) = bf16x8(y);
+            }
+          }
+        }
+      }
+    }
+  }
+}
+
+template <int D>
+static const void *append_fn(bool q8) {
+  return q8 ? (const void *)append_kernel<D, true> : (const void *)append_kernel<D, false>;
+}
+template <int D>
+static const void *read_fn(bool q8, bool f32) {
+  if (q8) return f32 ? (const void *)read_kernel<D, true, true> : (const void *)read_kernel<D, true, false>;
+  return f32 ? (const void *)read_kernel<D, false, true> : (const void *)read_kernel<D, false, false>;
+}
+
+// Checks a pool and its table; fills `p`.
+static int pool_of(const char *what, Pool &p, const void *k, const float *ks, const void *v, const float *vs, int64_t pages,
+                   int page_size, const int32_t *table, int64_t ldt, int64_t columns, int64_t seqs, int nkv, int d) {
+  if (!k || !v || !table || (ks == nullptr) != (vs == nullptr)) return set_error(EGPT_ERR_ARG, "%s: null pointer", what);
+  if (d != 32 && d != 64 && d != 128) return set_error(EGPT_ERR_SHAPE, "%s: head_dim must be 32, 64 or 128", what);
+  if (page_size < 1 || page_size > 1024 || (page_size & (page_size - 1)))
+    return set_error(EGPT_ERR_SHAPE, "%s: the rows of a page must be a power of two up to 1024", what);
+  if (pages < 1 || pages > 0x7fffffff || nkv < 1 || nkv > 4096 || seqs < 1 || seqs > (1 << 20) || columns < 1 || ldt < columns ||
+      columns > (1 << 27) / page_size)
+    return set_error(EGPT_ERR_SHAPE, "%s: bad pages, heads, sequences or table", what);
+  if ((uintptr_t)k % 16 || (uintptr_t)v % 16 || (uintptr_t)ks % 4 || (uintptr_t)vs % 4 || (uintptr_t)table % 4)
+    return set_error(EGPT_ERR_ALIGN, "%s: pages must be 16-byte aligned", what);
+  p.k = (void *)k, p.v = (void *)v, p.ks = (float *)ks, p.vs = (float *)vs, p.pages = pages, p.nkv = nkv;
+  p.shift = 0;
+  while ((1 << p.shift) < page_size) ++p.shift;
+  p.table = table, p.ldt = ldt, p.cap = columns * page_size;
+  return EGPT_OK;
+}
+
+}  // namespace pgd
+}  // namespace egpt
+
+using namespace egpt;
+
+extern "C" int egpt_kv_append_paged(void *k_pages, float *k_scale, void *v_pages, float *v_scale, int64_t pages,
+                                    int page_size, const int32_t *table, int64_t ldt, int64_t columns, int64_t seqs,
+                                    const void *k, int64_t ldk, const void *v, int64_t ldv, const int64_t *position,
+                                    const int64_t *starts, int64_t m, int nkv, int d, void *q_out, int64_t ldqo, const void *q,
+                                    int64_t ldq, int nq, const void *q_norm_w, const void *k_norm_w, float eps,
+                                    const void *rope_cos, const void *rope_sin, int rope_dtype, int64_t rope_rows,
+                                    int64_t rope_base, unsigned flags, void *stream) {
+  clear_error();
+  pgd::AppendParams p{};
+  if (int rc = pgd::pool_of("kv_append_paged", p.pool, k_pages, k_scale, v_pages, v_scale, pages, page_size, table, ldt, columns,
+                            seqs, nkv, d))
+    return rc;
+  if (!k || !v || !position || (q == nullptr) != (q_out == nullptr) || (rope_cos == nullptr) != (rope_sin == nullptr))
+    return set_error(EGPT_ERR_ARG, "kv_append_paged: null pointer");
+  if (!q && q_norm_w) return set_error(EGPT_ERR_ARG, "kv_append_paged: a q norm without q");
+  if (!q) nq = 0, ldq = ldqo = 0;
+  if (m < 1 || ldk < (int64_t)nkv * d || ldv < (int64_t)nkv * d || (q && (nq < 1 || nq > (1 << 16))) || ldq < (int64_t)nq * d ||
+      ldqo < (int64_t)nq * d || (!starts && m != seqs))
+    return set_error(EGPT_ERR_SHAPE, "kv_append_paged: bad m, heads or leading dimension (without starts a row a sequence)");
+  if (rope_cos && rope_dtype != EGPT_BF16 && rope_dtype != EGPT_F32)
+    return set_error(EGPT_ERR_DTYPE, "kv_append_paged: RoPE tables are bf16 or fp32");
+  if (rope_cos && (rope_base < 0 || rope_rows < 1 || rope_base >= rope_rows))
+    return set_error(EGPT_ERR_SHAPE, "kv_append_paged: bad rope_rows or rope_base");
+  if ((uintptr_t)k % 16 || (uintptr_t)v % 16 || (uintptr_t)q % 16 || (uintptr_t)q_out % 16 || ldk % 8 || ldv % 8 || ldq % 8 ||
+      ldqo % 8 || (uintptr_t)rope_cos % 16 || (uintptr_t)rope_sin % 16 || (uintptr_t)q_norm_w % 16 || (uintptr_t)k_norm_w % 16)
+    return set_error(EGPT_ERR_ALIGN, "kv_append_paged: rows, norm weights and RoPE tables must be 16-byte aligned");
+  const int64_t vectors = nq + 2 * (int64_t)nkv, per_cta = pgd::kThreads / (d / 16);
+  if (m > 0x7fffffff / vectors) return set_error(EGPT_ERR_SHAPE, "kv_append_paged: too many rows");
+  p.q = (const uint16_t *)q, p.k = (const uint16_t *)k, p.v = (const uint16_t *)v, p.q_out = (uint16_t *)q_out;
+  p.ldq = ldq, p.ldk = ldk, p.ldv = ldv, p.ldqo = ldqo, p.position = position, p.starts = starts;
+  p.seqs = (int)seqs, p.m = (int)m, p.nq = nq;
+  p.q_norm_w = (const uint16_t *)q_norm_w, p.k_norm_w = (const uint16_t *)k_norm_w, p.eps = eps;
+  p.rope_cos = rope_cos, p.rope_sin = rope_sin, p.rope_f32 = rope_dtype == EGPT_F32;
+  p.rope_rows = rope_rows, p.rope_base = rope_base;
+  const void *fn = d == 128 ? pgd::append_fn<128>(k_scale) : (d == 64 ? pgd::append_fn<64>(k_scale) : pgd::append_fn<32>(k_scale));
+  return check_launch(launch_kernel(fn, dim3((unsigned)((m * vectors + per_cta - 1) / per_cta)), dim3(pgd::kThreads), 0,
+                                    (cudaStream_t)stream, (flags & EGPT_FLAG_PDL) != 0, p),
+                      "kv_append_paged_kernel");
+}
+
+extern "C" int egpt_kv_read_paged(void *k_out, void *v_out, int64_t out_head_stride, int dtype, const void *k_pages,
+                                  const float *k_scale, const void *v_pages, const float *v_scale, int64_t pages,
+                                  int page_size, const int32_t *table, int64_t ldt, int64_t columns, int64_t seqs, int nkv,
+                                  int d, int64_t start, const int64_t *starts, int64_t count, unsigned flags, void *stream) {
+  clear_error();
+  pgd::ReadParams p{};
+  if (int rc = pgd::pool_of("kv_read_paged", p.pool, k_pages, k_scale, v_pages, v_scale, pages, page_size, table, ldt, columns,
+                            seqs, nkv, d))
+    return rc;
+  if (!k_out || !v_out) return set_error(EGPT_ERR_ARG, "kv_read_paged: null pointer");
+  if (dtype != EGPT_BF16 && dtype != EGPT_F32) return set_error(EGPT_ERR_DTYPE, "kv_read_paged: the output is bf16 or fp32");
+  if (count < 1 || count > (1 << 27) || out_head_stride < count * d || (!starts && (start < 0 || start > p.pool.cap - count)))
+    return set_error(EGPT_ERR_SHAPE, "kv_read_paged: rows [start, start + count) outside the table, or bad output stride");
+  const bool f32 = dtype == EGPT_F32, q8 = k_scale != nullptr;
+  if ((uintptr_t)k_out % 16 || (uintptr_t)v_out % 16 || (out_head_stride * (f32 ? 4 : 2)) % 16)
+    return set_error(EGPT_ERR_ALIGN, "kv_read_paged: outputs must be 16-byte aligned");
+  p.k_out = k_out, p.v_out = v_out, p.out_head = out_head_stride, p.start = start, p.count = count, p.starts = starts;
+  p.seqs = (int)seqs;
+  const int64_t per_cta = pgd::kThreads / (d / (q8 ? 16 : 8)), heads = seqs * nkv;
+  const dim3 grid((unsigned)std::min<int64_t>((count + per_cta - 1) / per_cta, 1 << 16), (unsigned)std::min<int64_t>(heads, 65535));
+  const void *fn = d == 128 ? pgd::read_fn<128>(q8, f32) : (d == 64 ? pgd::read_fn<64>(q8, f32) : pgd::read_fn<32>(q8, f32));
+  return check_launch(launch_kernel(fn, grid, dim3(pgd::kThreads), 0, (cudaStream_t)stream, (flags & EGPT_FLAG_PDL) != 0, p),
+                      "kv_read_paged_kernel");
+}

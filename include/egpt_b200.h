@@ -242,6 +242,60 @@ EGPT_API int egpt_attn_shared_prefix(void *out, int64_t ldo, const void *q, int6
 EGPT_API int egpt_attn_shared_prefix_on_tcgen05(int64_t m, int nq, int nkv, int d, int64_t prefix_len, float scale,
                                                 int cache_dtype);
 
+/* ---- KV cache in pages ------------------------------------------------------------------------------
+ * No counterpart in the reference. A pool is `pages` pages of page_size rows (a power of two up to 1024) for every kv
+ * head, K and V apart: [pages][nkv][page_size][d], bf16, or int8 codes with fp32 scales [pages][nkv][page_size] (k_scale,
+ * v_scale; NULL: bf16). table (int32, row stride ldt) names the pages of a sequence's slots in order, `columns` of
+ * them: slot s of sequence i lies in page table[i ldt + s / page_size] (-1: no page). Sequences may share pages. d 32, 64
+ * or 128; pool, rows and tables 16-byte aligned. Positions, starts and the table are read on the device. Reported
+ * through egpt_device_error (EGPT_ERR_SHAPE), without effect on other rows: a slot outside the table, a row or key
+ * on a page that is -1 or outside the pool.
+ *
+ * egpt_kv_append_paged: m rows of k and v bf16 (leading dimensions ldk, ldv) to the pages. Without `starts` row i is
+ * sequence i's, for slot position[i] (-1: an idle slot of the batch, nothing is written); with starts (int64 [seqs + 1],
+ * ascending) rows starts[i] .. starts[i + 1] - 1 are sequence i's, for slots position[i], position[i] + 1, ...; rows
+ * outside all sequences are left alone. With k_norm_w bf16 [d] / q_norm_w the k and q heads are RMS-normed, with
+ * rope_cos, rope_sin [rope_rows][d / 2] (rope_dtype bf16 or fp32) rotated (half layout) to position rope_base + slot, in
+ * fp32 and rounded once, to bf16 or to a code. q [m][nq d] (nullable) goes to q_out, which may be q; rows without a
+ * slot become zeros. Two rows for one slot leave either.
+ *
+ * egpt_kv_read_paged: rows start .. start + count - 1 of every sequence (starts: NULL, or int64 [seqs] on the device in
+ * place of start) into k_out and v_out, bf16 or fp32 [seqs nkv][count][d] with out_head_stride elements between the heads;
+ * slots outside the table and pages of -1 read as zeros (not reported).
+ *
+ * egpt_attn_decode_paged: softmax(scale q K^T) V of row i of q bf16 [m][nq d] over the position[i] + 1 keys of sequence i
+ * (m sequences; -1: an idle slot, zeros), GQA with at most 16 query heads to a kv head. Keys on pages that are -1 or
+ * outside the pool count as zeros. Workspace as egpt_attn_decode_q8's (egpt_attn_q8_ws_bytes, zero-filled once). */
+EGPT_API int egpt_kv_append_paged(void *k_pages, float *k_scale, void *v_pages, float *v_scale, int64_t pages,
+                                  int page_size, const int32_t *table, int64_t ldt, int64_t columns, int64_t seqs,
+                                  const void *k, int64_t ldk, const void *v, int64_t ldv, const int64_t *position,
+                                  const int64_t *starts, int64_t m, int nkv, int d, void *q_out, int64_t ldqo,
+                                  const void *q, int64_t ldq, int nq, const void *q_norm_w, const void *k_norm_w,
+                                  float eps, const void *rope_cos, const void *rope_sin, int rope_dtype,
+                                  int64_t rope_rows, int64_t rope_base, unsigned flags, void *stream);
+EGPT_API int egpt_kv_read_paged(void *k_out, void *v_out, int64_t out_head_stride, int dtype, const void *k_pages,
+                                const float *k_scale, const void *v_pages, const float *v_scale, int64_t pages,
+                                int page_size, const int32_t *table, int64_t ldt, int64_t columns, int64_t seqs, int nkv,
+                                int d, int64_t start, const int64_t *starts, int64_t count, unsigned flags, void *stream);
+EGPT_API int egpt_attn_decode_paged(void *out, int64_t ldo, const void *q, int64_t ldq, const void *k_pages,
+                                    const float *k_scale, const void *v_pages, const float *v_scale, int64_t pages,
+                                    int page_size, const int32_t *table, int64_t ldt, int64_t columns,
+                                    const int64_t *position, int64_t m, int nq, int nkv, int d, float scale, void *ws,
+                                    size_t ws_bytes, unsigned flags, void *stream);
+
+/* ---- log probabilities of tokens --------------------------------------------------------------------
+ * No counterpart in the reference. For every row of logits (bf16 or fp32, leading dimension ldx, v <= 2^20 columns):
+ * logp[r] = log softmax(x_r)[tokens[r]] (tokens nullable; -1: no token, 0; another id outside [0, v): NaN and
+ * EGPT_ERR_SHAPE through egpt_device_error), entropy[r] in nats, and the `top` (0 to 32) most likely tokens in order (of
+ * equal logits the lowest id first) with their log probabilities, top_ids and top_logp [m][top]. -inf logits are masked
+ * tokens; a row of nothing else has log probabilities -inf and entropy 0; a NaN or +inf makes the row's results NaN.
+ * Workspace: egpt_token_logprobs_ws_bytes(m, v) bytes (0 for many rows), zero-filled once by the caller, left so
+ * where it matters; it serves calls of every size that needs no more. Deterministic. */
+EGPT_API size_t egpt_token_logprobs_ws_bytes(int64_t m, int64_t v);
+EGPT_API int egpt_token_logprobs(float *logp, float *entropy, int64_t *top_ids, float *top_logp, const void *logits,
+                                 int64_t ldx, int dtype, int64_t m, int64_t v, const int64_t *tokens, int top, void *ws,
+                                 size_t ws_bytes, unsigned flags, void *stream);
+
 /* ---- argmax over rows of bf16/fp32 logits -----------------------------------------------------------
  * replaces: logits[:, -1].argmax(-1) (research/realmodel/fast_decode.py:48,84): first index on ties. */
 EGPT_API int egpt_argmax_rows(int64_t *out, const void *logits, int64_t rows, int64_t n, int64_t ld, int dtype, void *stream);
