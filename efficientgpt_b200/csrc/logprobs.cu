@@ -87,13 +87,8 @@ struct Sums {
   float m, s, w;  // maximum (-inf: none yet), sum of 2^((x - m) log2 e), the same times its exponent
 };
 __device__ __forceinline__ void rescale(Sums &a, float m) {  // m >= a.m
-  if (a.m == -INFINITY) {
-    a.s = a.w = 0.f;
-  } else {
-    const float t = (a.m - m) * kLog2e, f = exp2f(t);
-    a.w = f == 0.f ? 0.f : f * fmaf(t, a.s, a.w), a.s *= f;
-  }
-  a.m = m;
+  const float t = fmaxf((a.m - m) * kLog2e, -1000.f), f = apf::ex2(t);  // (2^-1000 is 0, and 0 times it too)
+  a.w = f * fmaf(t, a.s, a.w), a.s *= f, a.m = m;
 }
 __device__ __forceinline__ void join(Sums &a, Sums b) {
   const float m = fmaxf(a.m, b.m);
@@ -101,78 +96,178 @@ __device__ __forceinline__ void join(Sums &a, Sums b) {
   rescale(a, m), rescale(b, m);
   a.s += b.s, a.w += b.w;
 }
+// The sums of N neighbouring lanes in all of them, the lower lane's first.
+template <int N>
+__device__ __forceinline__ void join_lanes(Sums &a) {
+#pragma unroll
+  for (int o = 1; o < N; o <<= 1) {
+    Sums b;
+    b.m = __shfl_xor_sync(0xffffffffu, a.m, o);
+    b.s = __shfl_xor_sync(0xffffffffu, a.s, o);
+    b.w = __shfl_xor_sync(0xffffffffu, a.w, o);
+    if (threadIdx.x & o) {
+      const Sums t = a;
+      a = b, b = t;
+    }
+    join(a, b);
+  }
+}
 template <int E>
 __device__ __forceinline__ void take(Sums &a, const float (&y)[E], float largest) {
   if (largest > a.m) rescale(a, largest);
   const float m = a.m == -INFINITY ? 0.f : a.m;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    const float t = fmaxf((y[e] - m) * kLog2e, -1000.f);  // (2^-1000 is 0, and 0 times it too)
+    const float t = fmaxf((y[e] - m) * kLog2e, -1000.f);
     const float f = apf::ex2(t);
     a.s += f, a.w = fmaf(f, t, a.w);
   }
 }
 
-// The `top` largest of a warp's keys (hi, then the lower index first: lo = ~index), N a lane; lane j gets the j-th. Keys of 0 are
-// none.
-template <int N>
-__device__ __forceinline__ uint2 select(uint32_t (&hi)[N], uint32_t (&lo)[N], int top) {
-  const int lane = threadIdx.x & 31;
-  uint2 mine = make_uint2(0u, 0u);
-#pragma unroll 1
-  for (int j = 0; j < top; ++j) {
-    uint32_t bh = 0u, bl = 0u;
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (hi[i] > bh || (hi[i] == bh && lo[i] > bl)) bh = hi[i], bl = lo[i];
-    const uint32_t mh = __reduce_max_sync(0xffffffffu, bh);
-    if (mh == 0u) break;
-    const uint32_t ml = __reduce_max_sync(0xffffffffu, bh == mh ? bl : 0u);
-    if (lane == j) mine = make_uint2(mh, ml);
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (hi[i] == mh && lo[i] == ml) hi[i] = 0u;
+// Two fp32 operations an instruction.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 halves(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// A whole chunk (16 bytes) into sums kept in pairs; -> its largest value, NaN if there is one.
+struct Sums2 {
+  float m;
+  uint64_t s, w;
+};
+template <int E>
+__device__ __forceinline__ float take2(Sums2 &a, uint4 c) {
+  uint32_t v[4] = {c.x, c.y, c.z, c.w};
+  float largest;
+  if (E == 8) {
+    const uint32_t mx = max2_nan(max2_nan(v[0], v[1]), max2_nan(v[2], v[3]));
+    largest = max_nan(bf16_lo(mx), bf16_hi(mx));
+  } else {
+    largest = max_nan(max_nan(__uint_as_float(v[0]), __uint_as_float(v[1])),
+                      max_nan(__uint_as_float(v[2]), __uint_as_float(v[3])));
   }
-  return mine;
+  if (largest > a.m || !(fabsf(a.m) <= 1e36f)) {
+    const float2 s = halves(a.s), w = halves(a.w);
+    Sums t = {a.m, s.x + s.y, w.x + w.y};
+    if (largest > t.m) rescale(t, largest);
+    a.m = t.m;
+    if (!(fabsf(t.m) <= 1e36f)) {  // nothing yet, or differences that can overflow: one at a time
+      float y[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        y[e] = E == 4 ? __uint_as_float(v[e % 4]) : (e % 2 ? bf16_hi(v[(e / 2) % 4]) : bf16_lo(v[(e / 2) % 4]));
+      take<E>(t, y, largest);
+      a.s = pair(t.s, 0.f), a.w = pair(t.w, 0.f);
+      return largest;
+    }
+    a.s = pair(t.s, 0.f), a.w = pair(t.w, 0.f);
+  }
+  const uint64_t less = pair(-a.m, -a.m), log2e = pair(kLog2e, kLog2e);
+#pragma unroll
+  for (int i = 0; i < E / 2; ++i) {
+    // no lower than -1e37 (0xfcf0, as bf16 -9.97e36), whose weight is 0 and exponent finite: -inf would give 0 times infinity
+    uint64_t x;
+    if (E == 8) {
+      const uint32_t t = max2(v[i % 4], 0xfcf0fcf0u);
+      x = pair(bf16_lo(t), bf16_hi(t));
+    } else {
+      x = pair(fmaxf(__uint_as_float(v[(2 * i) % 4]), -1e37f), fmaxf(__uint_as_float(v[(2 * i + 1) % 4]), -1e37f));
+    }
+    const uint64_t t = mul2(add2(x, less), log2e);
+    const float2 th = halves(t);
+    const uint64_t f = pair(apf::ex2(th.x), apf::ex2(th.y));
+    a.s = add2(a.s, f), a.w = fma2(f, t, a.w);
+  }
+  return largest;
 }
 
+constexpr int kFew = 48;        // how many threads at most have a key that passes the selection's first step
+constexpr int kKeysEach = 33;   // keys of a thread at most: 2^20 fp32 logits off the 16-byte grid are 8193 groups
 struct Smem {
   Sums sums[kWarps];
   uint32_t largest[kWarps];
-  uint2 cand[kWarps][kMaxTop];  // the warps' selections
-  uint2 best[kMaxTop];
-  uint2 found[kMaxTop * kMaxTop];  // elements of the selected groups
+  uint2 cand[kFew * kKeysEach];  // keys that may be among the first
+  uint2 best[kMaxTop];    // the first ones in order: value, ~index
+  int group[kMaxTop];
   int count, last;
   float m, log_s;
-  uint32_t keys[1];  // the row's groups, where no other CTA has some
+  uint32_t keys[1];  // the row's groups (where no other CTA has some), then the elements of the selected ones
 };
+__device__ __forceinline__ bool before(uint2 a, uint2 b) { return a.x > b.x || (a.x == b.x && a.y > b.y); }
 
-// The `top` largest of keys get(0 .. n - 1), in order, into sm.best (0 where there are fewer). Every thread calls it.
+// The `top` first of the keys get(0 .. n - 1) (value, ~index: all different), in order, into sm.best (value 0: fewer than top), n <=
+// kKeysEach kThreads. A threshold is found by bisection that `top` to kFew threads' first keys reach, so at most kKeysEach
+// kFew keys do, mostly a few more than top; those are ranked by counting. Every thread calls it.
 template <typename F>
-__device__ __forceinline__ void select_block(Smem &sm, int n, int top, F get) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  uint2 mine = make_uint2(0u, 0u);
-  for (int i0 = warp * 128; i0 < n; i0 += kWarps * 128) {
-    uint32_t hi[5], lo[5];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int at = i0 + 32 * i + lane;
-      const uint2 k = at < n ? get(at) : make_uint2(0u, 0u);
-      hi[i] = k.x, lo[i] = k.y;
-    }
-    hi[4] = mine.x, lo[4] = mine.y;
-    mine = select<5>(hi, lo, top);
+__device__ __forceinline__ void select(Smem &sm, int n, int top, F get) {
+  const int t = threadIdx.x;
+  uint2 first = make_uint2(0u, 0u);
+  for (int i = t; i < n; i += kThreads) {
+    const uint2 k = get(i);
+    if (before(k, first)) first = k;
   }
-  sm.cand[warp][lane] = mine;
-  __syncthreads();
-  if (warp == 0) {
-    uint32_t hi[kWarps], lo[kWarps];
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const uint2 k = lane < top ? sm.cand[w][lane] : make_uint2(0u, 0u);
-      hi[w] = k.x, lo[w] = k.y;
+  if (t == 0) sm.count = 0;
+  if (t < kMaxTop) sm.best[t] = make_uint2(0u, 0u);
+  uint2 lo = make_uint2(0u, 1u);  // every key reaches it
+  if (__syncthreads_count(before(first, make_uint2(0u, 0u))) > kFew) {
+    uint2 hi = make_uint2(0xffffffffu, 0xffffffffu);
+    for (;;) {
+      // halfway in the values, then in the indices
+      uint2 mid = make_uint2(lo.x + (hi.x - lo.x) / 2, 0u);
+      if (hi.x - lo.x <= 1u) mid = hi.x == lo.x ? make_uint2(lo.x, lo.y + (hi.y - lo.y) / 2) : make_uint2(hi.x, 0u);
+      if (hi.x == lo.x && mid.y == lo.y) mid.y = hi.y;
+      const int reach = __syncthreads_count(!before(mid, first));
+      if (reach >= top) lo = mid;
+      else hi = make_uint2(mid.y ? mid.x : mid.x - 1u, mid.y - 1u);
+      if (reach >= top && reach <= kFew) break;
     }
-    sm.best[lane] = select<kWarps>(hi, lo, top);
+  }
+  for (int i = t; i < n; i += kThreads) {
+    const uint2 k = get(i);
+    if (k.x != 0u && !before(lo, k)) sm.cand[atomicAdd(&sm.count, 1)] = k;
+  }
+  __syncthreads();
+  const int count = sm.count;
+  for (int i = t; i < count; i += kThreads) {
+    const uint2 k = sm.cand[i];
+    int rank = 0;
+    for (int j = 0; j < count; ++j) rank += before(sm.cand[j], k);
+    if (rank < top) sm.best[rank] = k;
   }
   __syncthreads();
 }
@@ -188,46 +283,50 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const Params p) {
   const Row<T> r(p, row);
   const int g0 = (int)((int64_t)r.groups * split / p.splits), g1 = (int)((int64_t)r.groups * (split + 1) / p.splits);
   uint32_t *keys = p.splits == 1 ? sm.keys : p.keys + (int64_t)row * p.key_stride;
-  Sums a = {-INFINITY, 0.f, 0.f};
   uint32_t largest = 0u;
-  for (int g = g0 + warp; g < g1; g += U * kWarps) {
-    float y[U][E];
-    bool any[U];
+  auto note = [&](int g, uint32_t key) {
+    key = __reduce_max_sync(0xffffffffu, key);
+    largest = max(largest, key);
+    if (p.top && lane == 0) keys[g] = key;
+  };
+  // groups that lie inside the row whole, U loads on their way at once
+  const int whole0 = max(g0, r.off ? 1 : 0), whole1 = min(g1, (r.v + r.off) / (32 * E));
+  Sums2 a2 = {-INFINITY, 0u, 0u};
+  for (int g = whole0 + warp; g < whole1; g += U * kWarps) {
+    uint4 c[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      any[u] = false;
-      if (g + u * kWarps < g1) any[u] = r.load((g + u * kWarps) * 32 + lane, y[u]);
+      c[u] = make_uint4(0u, 0u, 0u, 0u);
+      if (g + u * kWarps < whole1) c[u] = __ldg((const uint4 *)(r.x - r.off) + (g + u * kWarps) * 32 + lane);
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (g + u * kWarps >= g1) break;
-      float mx = y[u][0];
-      bool nan = false;
-#pragma unroll
-      for (int e = 0; e < E; ++e) mx = fmaxf(mx, y[u][e]), nan |= y[u][e] != y[u][e];
-      if (any[u]) take<E>(a, y[u], mx);
-      const uint32_t key = __reduce_max_sync(0xffffffffu, any[u] ? (nan ? 0xffffffffu : key_of(mx)) : 0u);
-      largest = max(largest, key);
-      if (p.top && lane == 0) keys[g + u * kWarps] = key;
-    }
+    for (int u = 0; u < U; ++u)
+      if (g + u * kWarps < whole1) note(g + u * kWarps, key_of(take2<E>(a2, c[u])));
   }
+  const float2 s2 = halves(a2.s), w2 = halves(a2.w);
+  Sums a = {a2.m, s2.x + s2.y, w2.x + w2.y};
+  // the first and the last one otherwise
+  const int ends[2] = {r.off ? 0 : -1, r.groups - 1 >= (r.v + r.off) / (32 * E) && (r.groups > 1 || !r.off) ? r.groups - 1 : -1};
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    Sums b;
-    b.m = __shfl_xor_sync(0xffffffffu, a.m, o);
-    b.s = __shfl_xor_sync(0xffffffffu, a.s, o);
-    b.w = __shfl_xor_sync(0xffffffffu, a.w, o);
-    if (lane & o) {  // the same order in both lanes
-      const Sums t = a;
-      a = b, b = t;
-    }
-    join(a, b);
+  for (int i = 0; i < 2; ++i) {
+    if (warp != i || ends[i] < g0 || ends[i] >= g1) continue;
+    float y[E], mx = -INFINITY;
+    const bool any = r.load(ends[i] * 32 + lane, y);
+#pragma unroll
+    for (int e = 0; e < E; ++e) mx = max_nan(mx, y[e]);
+    if (any) take<E>(a, y, mx);
+    note(ends[i], any ? key_of(mx) : 0u);
   }
+  join_lanes<32>(a);
   if (lane == 0) sm.sums[warp] = a, sm.largest[warp] = largest;
   __syncthreads();
+  if (warp == 0) {
+    a = lane < kWarps ? sm.sums[lane] : Sums{-INFINITY, 0.f, 0.f};
+    join_lanes<kWarps>(a);
+    largest = __reduce_max_sync(0xffffffffu, lane < kWarps ? sm.largest[lane] : 0u);
+  }
   if (p.splits > 1) {
     if (threadIdx.x == 0) {
-      for (int w = 1; w < kWarps; ++w) join(a, sm.sums[w]), largest = max(largest, sm.largest[w]);
       p.parts[(int64_t)row * p.splits + split] = make_float4(a.m, a.s, a.w, __uint_as_float(largest));
       __threadfence();  // the record and (by the barrier) the keys
       const bool last = atomicAdd(p.cnt + row, 1u) == (unsigned)p.splits - 1u;
@@ -239,41 +338,23 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const Params p) {
     }
     __syncthreads();
     if (!sm.last) return;
-  }
-  // ---- the row: all sums, in the order of the parts (warp 0: a lane takes some, then the lanes')
-  const int n = p.splits > 1 ? p.splits : kWarps;
-  if (warp == 0) {
-    a = {-INFINITY, 0.f, 0.f}, largest = 0u;
-    for (int i = lane; i < n; i += 32) {
-      Sums b;
-      uint32_t k;
-      if (p.splits > 1) {
+    if (warp == 0) {  // the row's parts: a lane takes every 32nd, then the lanes'
+      a = {-INFINITY, 0.f, 0.f}, largest = 0u;
+      for (int i = lane; i < p.splits; i += 32) {
         const float4 t = __ldcg(p.parts + (int64_t)row * p.splits + i);
-        b = {t.x, t.y, t.z}, k = __float_as_uint(t.w);
-      } else {
-        b = sm.sums[i], k = sm.largest[i];
+        join(a, Sums{t.x, t.y, t.z});
+        largest = max(largest, __float_as_uint(t.w));
       }
-      join(a, b);
-      largest = max(largest, k);
+      join_lanes<32>(a);
+      largest = __reduce_max_sync(0xffffffffu, largest);
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      Sums b;
-      b.m = __shfl_xor_sync(0xffffffffu, a.m, o);
-      b.s = __shfl_xor_sync(0xffffffffu, a.s, o);
-      b.w = __shfl_xor_sync(0xffffffffu, a.w, o);
-      if (lane & o) {
-        const Sums t = a;
-        a = b, b = t;
-      }
-      join(a, b);
-    }
-    largest = __reduce_max_sync(0xffffffffu, largest);
+  }
+  if (warp == 0) {
     const bool none = largest == kNegInf, bad = largest >= kInf;
     // of a row of -inf alone, log p is that too: x - 0 - 0
     const float m = bad ? NAN : (none ? 0.f : a.m), log_s = none ? 0.f : log2f(a.s) * kLn2;
     if (lane == 0) {
-      sm.m = m, sm.log_s = log_s, sm.count = 0;
+      sm.m = m, sm.log_s = log_s;
       p.entropy[row] = bad ? NAN : (none ? 0.f : fmaxf(0.f, log_s - a.w / a.s * kLn2));
       if (p.tokens) {
         const int64_t t = p.tokens[row];
@@ -285,33 +366,26 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const Params p) {
     }
   }
   if (!p.top) return;
-  __syncthreads();
-  // ---- the groups with the top tokens, then their elements that can be some
+  // ---- the groups with the top tokens, then the first of their elements
   const bool split_keys = p.splits > 1;
-  select_block(sm, r.groups, p.top, [&](int i) { return make_uint2(split_keys ? __ldcg(keys + i) : keys[i], ~(uint32_t)i); });
+  select(sm, r.groups, p.top, [&](int i) { return make_uint2(split_keys ? __ldcg(keys + i) : keys[i], ~(uint32_t)i); });
   const int groups = min(p.top, r.groups);
-  const uint32_t least = r.groups < p.top ? 1u : sm.best[p.top - 1].x;
-#pragma unroll 1
+  if (threadIdx.x < groups) sm.group[threadIdx.x] = (int)~sm.best[threadIdx.x].y;
+  uint32_t *elems = sm.keys;  // the groups' own keys are done with
   for (int j = warp; j < groups; j += kWarps) {
     const int c = (int)~sm.best[j].y * 32 + lane;
     float y[E];
-    uint32_t hi[E], lo[E];
     r.load(c, y);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const int i = c * E - r.off + e;
-      hi[e] = i >= 0 && i < r.v ? key_of(y[e]) : 0u, lo[e] = ~(uint32_t)i;
-      if (hi[e] < least) hi[e] = 0u;
+      elems[(j * 32 + lane) * E + e] = i >= 0 && i < r.v ? key_of(y[e]) : 0u;
     }
-    const uint2 mine = select<E>(hi, lo, p.top);
-    const unsigned have = __ballot_sync(0xffffffffu, mine.x != 0u);
-    int at = 0;
-    if (lane == 0) at = atomicAdd(&sm.count, __popc(have));
-    at = __shfl_sync(0xffffffffu, at, 0);
-    if (mine.x != 0u) sm.found[at + lane] = mine;
   }
   __syncthreads();
-  select_block(sm, sm.count, p.top, [&](int i) { return sm.found[i]; });
+  select(sm, groups * 32 * E, p.top, [&](int i) {
+    return make_uint2(elems[i], ~(uint32_t)(sm.group[i / (32 * E)] * 32 * E + i % (32 * E) - r.off));
+  });
   if (threadIdx.x < p.top) {
     const uint2 k = sm.best[threadIdx.x];
     p.top_ids[(int64_t)row * p.top + threadIdx.x] = (int64_t)(~k.y);
@@ -365,7 +439,8 @@ extern "C" int egpt_token_logprobs(float *logp, float *entropy, int64_t *top_ids
   p.logp = logp, p.entropy = entropy, p.top_logp = top_logp, p.top_ids = top_ids;
   p.cnt = (unsigned *)ws, p.parts = (float4 *)((char *)ws + lgp::kSplitRows * sizeof(unsigned));
   p.keys = (uint32_t *)(p.parts + m * p.splits), p.key_stride = (lgp::most_groups(v, f32) + 3) / 4 * 4;
-  const size_t smem = sizeof(lgp::Smem) + (p.splits == 1 && top ? (size_t)lgp::most_groups(v, f32) * sizeof(uint32_t) : 0);
+  const int words = std::max(p.splits == 1 ? lgp::most_groups(v, f32) : 0, top * lgp::group_elems(f32));
+  const size_t smem = sizeof(lgp::Smem) + (top ? words * sizeof(uint32_t) : 0);
   const void *fn = f32 ? (const void *)lgp::logprobs_kernel<float> : (const void *)lgp::logprobs_kernel<uint16_t>;
   return check_launch(launch_kernel(fn, dim3((unsigned)p.splits, (unsigned)m), dim3(lgp::kThreads), smem, (cudaStream_t)stream,
                                     (flags & EGPT_FLAG_PDL) != 0, p),
