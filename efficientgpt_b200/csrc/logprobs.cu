@@ -20,7 +20,8 @@ namespace lgp {
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kMaxTop = 32;
 constexpr int kMaxVocab = 1 << 20;
-constexpr int kSplitRows = 512;   // rows that may be split, and arrival counters
+constexpr int kResident = 4;      // CTAs of an SM
+constexpr int kSplitRows = 4096;  // arrival counters: more than the CTAs of a GPU
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr uint32_t kNegInf = 0x007fffffu, kInf = 0xff800000u;  // keys of the infinities; above kInf NaN, below kNegInf nothing
 
@@ -28,19 +29,19 @@ struct Params {
   const void *x;
   int64_t ldx;
   const int64_t *tokens;  // nullable
-  int m, v, top, splits;
+  int m, v, top;
+  int whole, splits;  // rows of a CTA each; CTAs of each of the others
   float *logp, *entropy, *top_logp;
   int64_t *top_ids;
   unsigned *cnt;   // arrivals of a split row, zero between calls
-  float4 *parts;   // [m][splits] maximum, sum, weighted sum, largest key
-  uint32_t *keys;  // [m][most groups]
+  float4 *parts;   // [split rows][splits] maximum, sum, weighted sum, largest key
+  uint32_t *keys;  // [split rows][most groups]
   int key_stride;
 };
 
-// Keys in the order of the values: -inf < ... < +inf < NaN, zeros alike.
+// Keys in the order of the values: -inf < ... < +inf < NaN (0x7fffffff, as a sum gives it), zeros alike.
 __device__ __forceinline__ uint32_t key_of(float x) {
   const uint32_t b = __float_as_uint(__fadd_rn(x, 0.f));
-  if ((b & 0x7fffffffu) > 0x7f800000u) return 0xffffffffu;
   return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float value_of(uint32_t key) {
@@ -84,10 +85,21 @@ struct Row {
 };
 
 struct Sums {
-  float m, s, w;  // maximum (-inf: none yet), sum of 2^((x - m) log2 e), the same times its exponent
+  float m, s, w;  // reference (-inf: none yet), sum of 2^exponent(x, m), the same times its exponent
 };
+// (x - m) log2 e. For m up to 1e4 as x log2 e less m log2 e, rounded: what that is off (4e-4 at most) is the same for all x and
+// cancels in log p and in the entropy; beyond, where it grows and x log2 e can overflow, as the difference times log2 e.
+__device__ __forceinline__ bool plain_range(float m) { return fabsf(m) <= 1e4f; }
+__device__ __forceinline__ float exponent(float x, float m) {
+  return plain_range(m) ? fmaf(x, kLog2e, -__fmul_rn(m, kLog2e)) : (x - m) * kLog2e;
+}
+__device__ __forceinline__ float log_prob(float x, float m, float log_s) {
+  return (plain_range(m) && plain_range(x) ? exponent(x, m) * kLn2 : x - m) - log_s;
+}
 __device__ __forceinline__ void rescale(Sums &a, float m) {  // m >= a.m
-  const float t = fmaxf((a.m - m) * kLog2e, -1000.f), f = apf::ex2(t);  // (2^-1000 is 0, and 0 times it too)
+  float t = plain_range(a.m) && plain_range(m) ? __fmul_rn(a.m, kLog2e) - __fmul_rn(m, kLog2e) : (a.m - m) * kLog2e;
+  t = fmaxf(t, -1000.f);  // (2^-1000 is 0, and 0 times it too)
+  const float f = apf::ex2(t);
   a.w = f * fmaf(t, a.s, a.w), a.s *= f, a.m = m;
 }
 __device__ __forceinline__ void join(Sums &a, Sums b) {
@@ -118,7 +130,7 @@ __device__ __forceinline__ void take(Sums &a, const float (&y)[E], float largest
   const float m = a.m == -INFINITY ? 0.f : a.m;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    const float t = fmaxf((y[e] - m) * kLog2e, -1000.f);
+    const float t = fmaxf(exponent(y[e], m), -1000.f);
     const float f = apf::ex2(t);
     a.s += f, a.w = fmaf(f, t, a.w);
   }
@@ -138,11 +150,6 @@ __device__ __forceinline__ float2 halves(uint64_t v) {
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
 __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
@@ -165,39 +172,20 @@ __device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b) {
   asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
-// A whole chunk (16 bytes) into sums kept in pairs; -> its largest value, NaN if there is one.
-struct Sums2 {
-  float m;
-  uint64_t s, w;
-};
+// The largest element of a whole chunk (16 bytes), NaN if there is one.
 template <int E>
-__device__ __forceinline__ float take2(Sums2 &a, uint4 c) {
-  uint32_t v[4] = {c.x, c.y, c.z, c.w};
-  float largest;
+__device__ __forceinline__ float largest_of(uint4 c) {
   if (E == 8) {
-    const uint32_t mx = max2_nan(max2_nan(v[0], v[1]), max2_nan(v[2], v[3]));
-    largest = max_nan(bf16_lo(mx), bf16_hi(mx));
-  } else {
-    largest = max_nan(max_nan(__uint_as_float(v[0]), __uint_as_float(v[1])),
-                      max_nan(__uint_as_float(v[2]), __uint_as_float(v[3])));
+    const uint32_t mx = max2_nan(max2_nan(c.x, c.y), max2_nan(c.z, c.w));
+    return max_nan(bf16_lo(mx), bf16_hi(mx));
   }
-  if (largest > a.m || !(fabsf(a.m) <= 1e36f)) {
-    const float2 s = halves(a.s), w = halves(a.w);
-    Sums t = {a.m, s.x + s.y, w.x + w.y};
-    if (largest > t.m) rescale(t, largest);
-    a.m = t.m;
-    if (!(fabsf(t.m) <= 1e36f)) {  // nothing yet, or differences that can overflow: one at a time
-      float y[E];
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        y[e] = E == 4 ? __uint_as_float(v[e % 4]) : (e % 2 ? bf16_hi(v[(e / 2) % 4]) : bf16_lo(v[(e / 2) % 4]));
-      take<E>(t, y, largest);
-      a.s = pair(t.s, 0.f), a.w = pair(t.w, 0.f);
-      return largest;
-    }
-    a.s = pair(t.s, 0.f), a.w = pair(t.w, 0.f);
-  }
-  const uint64_t less = pair(-a.m, -a.m), log2e = pair(kLog2e, kLog2e);
+  return max_nan(max_nan(__uint_as_float(c.x), __uint_as_float(c.y)), max_nan(__uint_as_float(c.z), __uint_as_float(c.w)));
+}
+// Its elements into sums kept in pairs, relative to m (of the plain range).
+template <int E>
+__device__ __forceinline__ void take2(uint64_t &s, uint64_t &w, float m, uint4 c) {
+  const uint32_t v[4] = {c.x, c.y, c.z, c.w};
+  const uint64_t less = pair(-__fmul_rn(m, kLog2e), -__fmul_rn(m, kLog2e)), log2e = pair(kLog2e, kLog2e);
 #pragma unroll
   for (int i = 0; i < E / 2; ++i) {
     // no lower than -1e37 (0xfcf0, as bf16 -9.97e36), whose weight is 0 and exponent finite: -inf would give 0 times infinity
@@ -208,21 +196,21 @@ __device__ __forceinline__ float take2(Sums2 &a, uint4 c) {
     } else {
       x = pair(fmaxf(__uint_as_float(v[(2 * i) % 4]), -1e37f), fmaxf(__uint_as_float(v[(2 * i + 1) % 4]), -1e37f));
     }
-    const uint64_t t = mul2(add2(x, less), log2e);
+    const uint64_t t = fma2(x, log2e, less);
     const float2 th = halves(t);
     const uint64_t f = pair(apf::ex2(th.x), apf::ex2(th.y));
-    a.s = add2(a.s, f), a.w = fma2(f, t, a.w);
+    s = add2(s, f), w = fma2(f, t, w);
   }
-  return largest;
 }
 
-constexpr int kFew = 48;        // how many threads at most have a key that passes the selection's first step
+constexpr int kMore = 8;        // threads more than asked for that may have a key which passes the selection's first step
 constexpr int kKeysEach = 33;   // keys of a thread at most: 2^20 fp32 logits off the 16-byte grid are 8193 groups
 struct Smem {
   Sums sums[kWarps];
   uint32_t largest[kWarps];
-  uint2 cand[kFew * kKeysEach];  // keys that may be among the first
+  uint2 cand[(kMaxTop + kMore) * kKeysEach];  // keys that may be among the first
   uint2 best[kMaxTop];    // the first ones in order: value, ~index
+  uint2 range[kWarps];
   int group[kMaxTop];
   int count, last;
   float m, log_s;
@@ -231,41 +219,60 @@ struct Smem {
 __device__ __forceinline__ bool before(uint2 a, uint2 b) { return a.x > b.x || (a.x == b.x && a.y > b.y); }
 
 // The `top` first of the keys get(0 .. n - 1) (value, ~index: all different), in order, into sm.best (value 0: fewer than top), n <=
-// kKeysEach kThreads. A threshold is found by bisection that `top` to kFew threads' first keys reach, so at most kKeysEach
-// kFew keys do, mostly a few more than top; those are ranked by counting. Every thread calls it.
+// kKeysEach kThreads. A threshold is found by bisection that the first keys of `top` to top + kMore threads reach, so at most
+// kKeysEach keys of each of those do, mostly a few more than top; they are ranked by counting. Every thread calls it.
 template <typename F>
 __device__ __forceinline__ void select(Smem &sm, int n, int top, F get) {
-  const int t = threadIdx.x;
-  uint2 first = make_uint2(0u, 0u);
-  for (int i = t; i < n; i += kThreads) {
+  constexpr int kHeld = 4;  // keys of a thread in registers
+  const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
+  uint2 held[kHeld], first = make_uint2(0u, 0u);
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) {
+    held[i] = make_uint2(0u, 0u);
+    if (t + i * kThreads < n) held[i] = get(t + i * kThreads);
+  }
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i)
+    if (before(held[i], first)) first = held[i];
+  for (int i = t + kHeld * kThreads; i < n; i += kThreads) {
     const uint2 k = get(i);
     if (before(k, first)) first = k;
   }
+  // the least and the largest value of the threads' first keys, between which the threshold's is
+  const uint32_t warp_lo = __reduce_min_sync(0xffffffffu, first.x), warp_hi = __reduce_max_sync(0xffffffffu, first.x);
+  if (lane == 0) sm.range[warp] = make_uint2(warp_lo, warp_hi);
   if (t == 0) sm.count = 0;
   if (t < kMaxTop) sm.best[t] = make_uint2(0u, 0u);
   uint2 lo = make_uint2(0u, 1u);  // every key reaches it
-  if (__syncthreads_count(before(first, make_uint2(0u, 0u))) > kFew) {
-    uint2 hi = make_uint2(0xffffffffu, 0xffffffffu);
+  if (__syncthreads_count(first.x != 0u) > top + kMore) {
+    uint2 hi = make_uint2(0u, 0xffffffffu);
+    lo.x = 0xffffffffu;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) lo.x = min(lo.x, sm.range[w].x), hi.x = max(hi.x, sm.range[w].y);
+    lo.y = 0u;  // (an index of 0 is no key's; a value of 0 none's either, so that all of them count as reaching it)
     for (;;) {
       // halfway in the values, then in the indices
       uint2 mid = make_uint2(lo.x + (hi.x - lo.x) / 2, 0u);
       if (hi.x - lo.x <= 1u) mid = hi.x == lo.x ? make_uint2(lo.x, lo.y + (hi.y - lo.y) / 2) : make_uint2(hi.x, 0u);
       if (hi.x == lo.x && mid.y == lo.y) mid.y = hi.y;
-      const int reach = __syncthreads_count(!before(mid, first));
+      const int reach = __syncthreads_count(first.x != 0u && !before(mid, first));
       if (reach >= top) lo = mid;
       else hi = make_uint2(mid.y ? mid.x : mid.x - 1u, mid.y - 1u);
-      if (reach >= top && reach <= kFew) break;
+      if (reach >= top && reach <= top + kMore) break;
     }
   }
-  for (int i = t; i < n; i += kThreads) {
-    const uint2 k = get(i);
+  auto offer = [&](uint2 k) {
     if (k.x != 0u && !before(lo, k)) sm.cand[atomicAdd(&sm.count, 1)] = k;
-  }
+  };
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) offer(held[i]);
+  for (int i = t + kHeld * kThreads; i < n; i += kThreads) offer(get(i));
   __syncthreads();
   const int count = sm.count;
   for (int i = t; i < count; i += kThreads) {
     const uint2 k = sm.cand[i];
     int rank = 0;
+#pragma unroll 8
     for (int j = 0; j < count; ++j) rank += before(sm.cand[j], k);
     if (rank < top) sm.best[rank] = k;
   }
@@ -273,38 +280,84 @@ __device__ __forceinline__ void select(Smem &sm, int n, int top, F get) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) logprobs_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads, kResident) logprobs_kernel(const Params p) {
   constexpr int E = Row<T>::E, U = 4;
   extern __shared__ __align__(16) uint8_t smem_raw[];
   Smem &sm = *(Smem *)smem_raw;
   pdl_wait();
   pdl_launch_dependents();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = blockIdx.y, split = blockIdx.x;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, cut = (int)blockIdx.x - p.whole;
+  // this CTA's row, its part and the row's parts
+  const int at = cut < 0 ? 0 : cut / p.splits, row = cut < 0 ? (int)blockIdx.x : p.whole + at;
+  const int split = cut < 0 ? 0 : cut - at * p.splits, splits = cut < 0 ? 1 : p.splits;
+  float x_token = 0.f;  // asked for early: the last of the row's CTAs needs it
+  int64_t token = -1;
+  if (threadIdx.x == 0 && p.tokens) token = p.tokens[row];
   const Row<T> r(p, row);
-  const int g0 = (int)((int64_t)r.groups * split / p.splits), g1 = (int)((int64_t)r.groups * (split + 1) / p.splits);
-  uint32_t *keys = p.splits == 1 ? sm.keys : p.keys + (int64_t)row * p.key_stride;
+  const int g0 = (int)((int64_t)r.groups * split / splits), g1 = (int)((int64_t)r.groups * (split + 1) / splits);
+  if (token >= 0 && token < p.v) x_token = Row<T>::widen(r.x[token]);
+  uint32_t *keys = splits == 1 ? sm.keys : p.keys + (int64_t)at * p.key_stride;
   uint32_t largest = 0u;
   auto note = [&](int g, uint32_t key) {
     key = __reduce_max_sync(0xffffffffu, key);
-    largest = max(largest, key);
     if (p.top && lane == 0) keys[g] = key;
+    return key;
   };
-  // groups that lie inside the row whole, U loads on their way at once
+  // Groups that lie inside the row whole, U loads on their way at once. A warp's sums are relative to the largest element of its
+  // first U groups, and to a later one's only where that is 4 more (weights up to e^4 and a few exponents that are rescaled).
   const int whole0 = max(g0, r.off ? 1 : 0), whole1 = min(g1, (r.v + r.off) / (32 * E));
-  Sums2 a2 = {-INFINITY, 0u, 0u};
-  for (int g = whole0 + warp; g < whole1; g += U * kWarps) {
-    uint4 c[U];
+  Sums a = {-INFINITY, 0.f, 0.f};
+  uint64_t s2 = 0u, w2 = 0u;
+  auto load = [&](int g, auto &c) {  // of groups g, g + kWarps, ...
+    const uint4 *src = (const uint4 *)(r.x - r.off) + g * 32 + lane;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      c[u] = make_uint4(0u, 0u, 0u, 0u);
-      if (g + u * kWarps < whole1) c[u] = __ldg((const uint4 *)(r.x - r.off) + (g + u * kWarps) * 32 + lane);
+    for (int u = 0; u < (int)(sizeof(c) / sizeof(c[0])); ++u) c[u] = __ldg(src + u * kWarps * 32);
+  };
+  auto add = [&](int g, const auto &c) {
+    constexpr int N = (int)(sizeof(c) / sizeof(c[0]));
+    uint32_t most = 0u;
+#pragma unroll
+    for (int u = 0; u < N; ++u) most = max(most, note(g + u * kWarps, key_of(largest_of<E>(c[u]))));
+    largest = max(largest, most);
+    const float mx = value_of(most);  // the same in all lanes, as a.m is
+    if (!(mx <= a.m + 4.f) || !plain_range(a.m)) {
+      const float2 s = halves(s2), w = halves(w2);
+      a.s += s.x + s.y, a.w += w.x + w.y, s2 = w2 = 0u;
+      if (mx > a.m) rescale(a, mx);
+      if (!plain_range(a.m)) {  // nothing yet, or far from 0: one element at a time
+#pragma unroll 1
+        for (int u = 0; u < N; ++u) {
+          float y[E];
+          r.load((g + u * kWarps) * 32 + lane, y);
+          take<E>(a, y, -INFINITY);
+        }
+        return;
+      }
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (g + u * kWarps < whole1) note(g + u * kWarps, key_of(take2<E>(a2, c[u])));
+    for (int u = 0; u < N; ++u) take2<E>(s2, w2, a.m, c[u]);
+  };
+  int g = whole0 + warp;
+  constexpr int kStep = U * kWarps, kSpan = kStep - kWarps;
+  if (g + kSpan < whole1) {  // the next ones on their way while these are added
+    uint4 c[U], next[U];
+    load(g, c);
+    for (; g + kStep + kSpan < whole1; g += kStep) {
+      load(g + kStep, next);
+      add(g, c);
+#pragma unroll
+      for (int u = 0; u < U; ++u) c[u] = next[u];
+    }
+    add(g, c);
+    g += kStep;
   }
-  const float2 s2 = halves(a2.s), w2 = halves(a2.w);
-  Sums a = {a2.m, s2.x + s2.y, w2.x + w2.y};
+  for (; g < whole1; g += kWarps) {
+    uint4 c[1];
+    load(g, c);
+    add(g, c);
+  }
+  const float2 s = halves(s2), w = halves(w2);
+  a.s += s.x + s.y, a.w += w.x + w.y;
   // the first and the last one otherwise
   const int ends[2] = {r.off ? 0 : -1, r.groups - 1 >= (r.v + r.off) / (32 * E) && (r.groups > 1 || !r.off) ? r.groups - 1 : -1};
 #pragma unroll
@@ -315,7 +368,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const Params p) {
 #pragma unroll
     for (int e = 0; e < E; ++e) mx = max_nan(mx, y[e]);
     if (any) take<E>(a, y, mx);
-    note(ends[i], any ? key_of(mx) : 0u);
+    largest = max(largest, note(ends[i], any ? key_of(mx) : 0u));
   }
   join_lanes<32>(a);
   if (lane == 0) sm.sums[warp] = a, sm.largest[warp] = largest;
@@ -325,23 +378,25 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const Params p) {
     join_lanes<kWarps>(a);
     largest = __reduce_max_sync(0xffffffffu, lane < kWarps ? sm.largest[lane] : 0u);
   }
-  if (p.splits > 1) {
+  if (splits > 1) {
     if (threadIdx.x == 0) {
-      p.parts[(int64_t)row * p.splits + split] = make_float4(a.m, a.s, a.w, __uint_as_float(largest));
+      p.parts[(int64_t)at * splits + split] = make_float4(a.m, a.s, a.w, __uint_as_float(largest));
       __threadfence();  // the record and (by the barrier) the keys
-      const bool last = atomicAdd(p.cnt + row, 1u) == (unsigned)p.splits - 1u;
+      const bool last = atomicAdd(p.cnt + at, 1u) == (unsigned)splits - 1u;
       if (last) {
         __threadfence();
-        p.cnt[row] = 0u;
+        p.cnt[at] = 0u;
       }
       sm.last = last;
     }
     __syncthreads();
     if (!sm.last) return;
+    if (p.top)  // (a thread reads its own ones again)
+      for (int i = threadIdx.x; i < r.groups; i += kThreads) sm.keys[i] = __ldcg(keys + i);
     if (warp == 0) {  // the row's parts: a lane takes every 32nd, then the lanes'
       a = {-INFINITY, 0.f, 0.f}, largest = 0u;
-      for (int i = lane; i < p.splits; i += 32) {
-        const float4 t = __ldcg(p.parts + (int64_t)row * p.splits + i);
+      for (int i = lane; i < splits; i += 32) {
+        const float4 t = __ldcg(p.parts + (int64_t)at * splits + i);
         join(a, Sums{t.x, t.y, t.z});
         largest = max(largest, __float_as_uint(t.w));
       }
@@ -351,24 +406,23 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const Params p) {
   }
   if (warp == 0) {
     const bool none = largest == kNegInf, bad = largest >= kInf;
-    // of a row of -inf alone, log p is that too: x - 0 - 0
+    // of a row of -inf alone, log p is that too
+    if (!none && !bad) rescale(a, value_of(largest));
     const float m = bad ? NAN : (none ? 0.f : a.m), log_s = none ? 0.f : log2f(a.s) * kLn2;
     if (lane == 0) {
       sm.m = m, sm.log_s = log_s;
       p.entropy[row] = bad ? NAN : (none ? 0.f : fmaxf(0.f, log_s - a.w / a.s * kLn2));
       if (p.tokens) {
-        const int64_t t = p.tokens[row];
         float lp = 0.f;  // -1: no token
-        if (t >= 0 && t < p.v) lp = Row<T>::widen(r.x[t]) - m - log_s;
-        else if (t != -1) set_device_error(EGPT_ERR_SHAPE), lp = NAN;
+        if (token >= 0 && token < p.v) lp = log_prob(x_token, m, log_s);
+        else if (token != -1) set_device_error(EGPT_ERR_SHAPE), lp = NAN;
         p.logp[row] = lp;
       }
     }
   }
   if (!p.top) return;
   // ---- the groups with the top tokens, then the first of their elements
-  const bool split_keys = p.splits > 1;
-  select(sm, r.groups, p.top, [&](int i) { return make_uint2(split_keys ? __ldcg(keys + i) : keys[i], ~(uint32_t)i); });
+  select(sm, r.groups, p.top, [&](int i) { return make_uint2(sm.keys[i], ~(uint32_t)i); });
   const int groups = min(p.top, r.groups);
   if (threadIdx.x < groups) sm.group[threadIdx.x] = (int)~sm.best[threadIdx.x].y;
   uint32_t *elems = sm.keys;  // the groups' own keys are done with
@@ -389,21 +443,28 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const Params p) {
   if (threadIdx.x < p.top) {
     const uint2 k = sm.best[threadIdx.x];
     p.top_ids[(int64_t)row * p.top + threadIdx.x] = (int64_t)(~k.y);
-    p.top_logp[(int64_t)row * p.top + threadIdx.x] = value_of(k.x) - sm.m - sm.log_s;
+    p.top_logp[(int64_t)row * p.top + threadIdx.x] = log_prob(value_of(k.x), sm.m, sm.log_s);
   }
 }
 
 static int group_elems(bool f32) { return 512 / (f32 ? 4 : 2); }
 // Groups of a row at most (a row may start inside a 16-byte chunk).
 static int most_groups(int64_t v, bool f32) { return (int)((v + 16 / (f32 ? 4 : 2) - 1 + group_elems(f32) - 1) / group_elems(f32)); }
-// CTAs of a row: about two for every SM, each with 16 groups (two loads a warp) at least; rows alone fill the GPU otherwise.
-static int splits_of(int64_t m, int64_t v, bool f32) {
-  const int64_t want = std::min<int64_t>(2 * num_sms() / m, most_groups(v, f32) / 16);
-  return m > kSplitRows ? 1 : (int)std::max<int64_t>(1, want);
+// The rows in full waves of CTAs take one each. Those behind them are split where two parts or more of each fit into one wave, with
+// 16 groups (two loads a warp) a part at least. More parts than that cost more than the places they fill: a part ends
+// with a fence, an arrival and an idle stream (1024 rows of 151936 bf16 logits, 432 of them behind a wave of 592: 69 us
+// whole, 80 us in quarters).
+static void cut(int64_t m, int64_t v, bool f32, int &whole, int &splits) {
+  const int wave = std::min(num_sms() * kResident, kSplitRows), rest = (int)(m % wave);
+  splits = rest ? std::max(1, std::min(wave / rest, most_groups(v, f32) / 16)) : 1;
+  whole = splits > 1 ? (int)m - rest : (int)m;
 }
 static size_t ws_bytes(int64_t m, int64_t v, bool f32) {
-  if (splits_of(m, v, f32) == 1) return 0;
-  return kSplitRows * sizeof(unsigned) + (size_t)m * (splits_of(m, v, f32) * sizeof(float4) + (most_groups(v, f32) + 3) / 4 * 16);
+  int whole, splits;
+  cut(m, v, f32, whole, splits);
+  if (splits == 1) return 0;
+  return kSplitRows * sizeof(unsigned) +
+         (size_t)(m - whole) * (splits * sizeof(float4) + (most_groups(v, f32) + 3) / 4 * 4 * sizeof(uint32_t));
 }
 
 }  // namespace lgp
@@ -430,7 +491,7 @@ extern "C" int egpt_token_logprobs(float *logp, float *entropy, int64_t *top_ids
     return set_error(EGPT_ERR_SHAPE, "token_logprobs: top must be in [0, %d] and no more than the vocabulary", lgp::kMaxTop);
   if ((uintptr_t)logits % (f32 ? 4 : 2)) return set_error(EGPT_ERR_ALIGN, "token_logprobs: logits must be aligned to their type");
   lgp::Params p{};
-  p.splits = lgp::splits_of(m, v, f32);
+  lgp::cut(m, v, f32, p.whole, p.splits);
   if (p.splits > 1) {
     if (!ws || ws_bytes < lgp::ws_bytes(m, v, f32)) return set_error(EGPT_ERR_WORKSPACE, "token_logprobs: workspace too small");
     if ((uintptr_t)ws % 16) return set_error(EGPT_ERR_ALIGN, "token_logprobs: workspace must be 16-byte aligned");
@@ -438,11 +499,11 @@ extern "C" int egpt_token_logprobs(float *logp, float *entropy, int64_t *top_ids
   p.x = logits, p.ldx = ldx, p.tokens = tokens, p.m = (int)m, p.v = (int)v, p.top = top;
   p.logp = logp, p.entropy = entropy, p.top_logp = top_logp, p.top_ids = top_ids;
   p.cnt = (unsigned *)ws, p.parts = (float4 *)((char *)ws + lgp::kSplitRows * sizeof(unsigned));
-  p.keys = (uint32_t *)(p.parts + m * p.splits), p.key_stride = (lgp::most_groups(v, f32) + 3) / 4 * 4;
-  const int words = std::max(p.splits == 1 ? lgp::most_groups(v, f32) : 0, top * lgp::group_elems(f32));
+  p.keys = (uint32_t *)(p.parts + (m - p.whole) * p.splits), p.key_stride = (lgp::most_groups(v, f32) + 3) / 4 * 4;
+  const int words = std::max(lgp::most_groups(v, f32), top * lgp::group_elems(f32));
   const size_t smem = sizeof(lgp::Smem) + (top ? words * sizeof(uint32_t) : 0);
   const void *fn = f32 ? (const void *)lgp::logprobs_kernel<float> : (const void *)lgp::logprobs_kernel<uint16_t>;
-  return check_launch(launch_kernel(fn, dim3((unsigned)p.splits, (unsigned)m), dim3(lgp::kThreads), smem, (cudaStream_t)stream,
+  return check_launch(launch_kernel(fn, dim3((unsigned)(p.whole + (m - p.whole) * p.splits)), dim3(lgp::kThreads), smem, (cudaStream_t)stream,
                                     (flags & EGPT_FLAG_PDL) != 0, p),
                       "token_logprobs_kernel");
 }
