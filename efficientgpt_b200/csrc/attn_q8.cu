@@ -54,6 +54,10 @@ constexpr int kMaxBatch = 512;
 constexpr int kRows = 16;        // query rows per tile (the M of the MMA), and rows of a partial record
 constexpr int kMinKeys = 512;    // keys of a range at least
 constexpr int kExtraKeys = 512;  // what a segment's start and end cost, in keys
+// Over pages, whose segments are cut wherever the even cuts fall, but nearer to an end than the margin at that end: no CTA
+// has more than its share, where leaving short segments whole gave some half as much again (64 rows over 200 to
+// 16000 bf16 keys 181 -> 155 us, 478 MB of int8 174 -> 140).
+constexpr int kMarginKeys = 256, kPagedExtraKeys = 256;
 
 struct Cache {
   const uint8_t *k, *v;
@@ -111,6 +115,7 @@ struct Cfg {
   static constexpr int kTile = Q8 ? 32 : 16;  // keys per warp tile: K and V 4 KB each at d = 128
   static constexpr int kStages = NR == 8 ? 3 : 2;
   static constexpr int kMinChunk = kMinKeys / kTile, kExtra = kExtraKeys / kTile;
+  static constexpr int kMargin = kMarginKeys / kTile, kPagedExtra = kPagedExtraKeys / kTile;
 };
 template <int D, bool Q8, int NR>
 struct Geo {
@@ -206,7 +211,7 @@ __device__ __forceinline__ int ceil_div_small(int a, int b) {
 // failing that, and for more sequences, equal stretches, or whole segments to single warps where that takes less time: a
 // CTA's part of a segment costs about one round of its warps' tiles besides its rounds, a warp's half a tile besides
 // its tiles, and the slowest warp has the longest segments. Every thread of the CTA calls it.
-template <typename C>
+template <typename C, bool PAGED>
 __device__ __forceinline__ Layout make_layout(const Params &p, int grid, int *cum, int *len_of, int *scratch) {
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   Layout l;
@@ -228,7 +233,7 @@ __device__ __forceinline__ Layout make_layout(const Params &p, int grid, int *cu
       parts += __shfl_xor_sync(0xffffffffu, parts, 8);
       parts += __shfl_xor_sync(0xffffffffu, parts, 16);
       const unsigned good = __ballot_sync(0xffffffffu, p.nkv * parts <= grid);
-      fits = good != 0u;
+      fits = good != 0u && !PAGED;
       if (fits) l.pad = __shfl_sync(0xffffffffu, len, __ffs(good) - 1);
     }
     if (!fits) {
@@ -236,7 +241,7 @@ __device__ __forceinline__ Layout make_layout(const Params &p, int grid, int *cu
       rounds = __reduce_add_sync(0xffffffffu, ceil_div(tiles, C::kWarps));
       longest = __reduce_max_sync(0xffffffffu, tiles);
     }
-    const int places = fits ? ceil_div_small(tiles, l.pad) * l.pad : (tiles ? tiles + C::kExtra : 0);
+    const int places = fits ? ceil_div_small(tiles, l.pad) * l.pad : (tiles ? tiles + (PAGED ? C::kPagedExtra : C::kExtra) : 0);
     int inc = places;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -255,7 +260,7 @@ __device__ __forceinline__ Layout make_layout(const Params &p, int grid, int *cu
     for (int e = 0; e < kPer; ++e) {
       const int i = t * kPer + e, keys = i < p.m ? seq_len(p, i) : 0, tiles = ceil_div(keys, C::kTile);
       len_of[i] = keys;
-      places[e] = tiles ? tiles + C::kExtra : 0;
+      places[e] = tiles ? tiles + (PAGED ? C::kPagedExtra : C::kExtra) : 0;
       sum += places[e];
       segs += tiles > 0, rounds += ceil_div(tiles, C::kWarps), longest = max(longest, tiles);
     }
@@ -288,7 +293,7 @@ __device__ __forceinline__ Layout make_layout(const Params &p, int grid, int *cu
     __syncthreads();
   }
   l.total = p.nkv * cum[p.m];
-  l.chunk = l.pad > 1 ? l.pad : max(1, ceil_div(l.total, grid));
+  l.chunk = l.pad > 1 ? l.pad : max(PAGED ? 2 * C::kMargin : 1, ceil_div(l.total, grid));
   l.uncut = max(C::kMinChunk, l.chunk / 2);
   if (l.pad == 1) {
     const float by_cta = (float)(p.nkv * (segs + rounds)) / (float)grid;
@@ -343,10 +348,14 @@ __device__ __forceinline__ Seg next_seg(const Params &p, const int *cum, const i
   return own_seg<TILE>(p, cum, len_of, i, 0);
 }
 // Where a stretch whose even cut is place x begins: not past the tiles of a segment, nor inside a short one.
-template <int TILE, bool PREFIX>
+template <int TILE, bool PREFIX, int MARGIN>
 __device__ __noinline__ int cut_at(const Params &p, const Layout &l, const int *cum, const int *len_of, int64_t x) {
   if (x >= l.total) return l.total;
   const Seg s = find_seg<TILE, PREFIX>(p, cum, len_of, (int)x);
+  if (MARGIN) {
+    if (x >= s.end) return s.next;
+    return x - s.start < MARGIN ? s.start : (s.end - x < MARGIN ? s.next : (int)x);
+  }
   return x >= s.end || (x > s.start && s.end - s.start <= l.uncut) ? s.next : (int)x;
 }
 // A partial record: kRows rows of (D accumulators), then kRows maxima and kRows sums.
@@ -468,7 +477,7 @@ __device__ __forceinline__ void attn_body(const Params &p, int block, int grid) 
     lay.chunk = p.pre.chunk, lay.pad = p.pre.pad, lay.uncut = 0, lay.solo = false;
     lay.total = p.nkv * p.pre.row_tiles * ceil_div(p.pre.seg_tiles, lay.pad) * lay.pad;
   } else {
-    lay = make_layout<C>(p, grid, sm.cum, sm.len, sm.scratch);
+    lay = make_layout<C, PAGED>(p, grid, sm.cum, sm.len, sm.scratch);
   }
   int x0 = (int)min((int64_t)lay.total, (int64_t)block * lay.chunk), x1 = min(lay.total, x0 + lay.chunk);
   const int stride = grid * kWarps;  // whole segments to warps: every stride-th
@@ -477,7 +486,7 @@ __device__ __forceinline__ void attn_body(const Params &p, int block, int grid) 
     while (solo_seg < p.m * p.nkv && sm.len[solo_seg / p.nkv] == 0) solo_seg += stride;
     x0 = 0, x1 = solo_seg < p.m * p.nkv ? lay.total : 0;
   } else if (lay.pad == 1) {  // both cuts at once, in the even and in the odd lanes
-    const int cut = cut_at<TILE, PREFIX>(p, lay, sm.cum, sm.len, (int64_t)(block + (lane & 1)) * lay.chunk);
+    const int cut = cut_at<TILE, PREFIX, PAGED ? C::kMargin : 0>(p, lay, sm.cum, sm.len, (int64_t)(block + (lane & 1)) * lay.chunk);
     x0 = __shfl_sync(0xffffffffu, cut, 0), x1 = __shfl_sync(0xffffffffu, cut, 1);
   }
   int split_n = 0;  // segments that this CTA shares with others: its first, its last
@@ -923,7 +932,12 @@ __device__ __forceinline__ void attn_body(const Params &p, int block, int grid) 
         rec[kRows * D + kRows + threadIdx.x] = sm.row_l[threadIdx.x];
       }
       if (MODE != kPrefix && !final) {
-        const int c0 = done.start / lay.chunk, c1 = (done.end - 1) / lay.chunk;
+        int c0 = done.start / lay.chunk, c1 = (done.end - 1) / lay.chunk;
+        if (PAGED && lay.pad == 1) {  // where cut_at has moved the cuts
+          const int b0 = (c0 + 1) * lay.chunk, b1 = c1 * lay.chunk;
+          c1 -= b1 - done.start >= C::kMargin && done.end - b1 < C::kMargin;
+          c0 += b0 < done.end && b0 - done.start < C::kMargin;
+        }
         if (MODE == kOwn) {
           (split_n ? split[1] : split[0]) = make_int3(done.index, c0, c1 - c0 + 1);
           ++split_n;
