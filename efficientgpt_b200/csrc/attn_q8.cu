@@ -113,7 +113,7 @@ struct Cfg {
   static constexpr int kWarps = 8;
   static constexpr int kThreads = 32 * kWarps;
   static constexpr int kTile = Q8 ? 32 : 16;  // keys per warp tile: K and V 4 KB each at d = 128
-  static constexpr int kStages = NR == 8 ? 3 : 2;
+  static constexpr int kStages = NR <= 8 ? 3 : 2;
   static constexpr int kMinChunk = kMinKeys / kTile, kExtra = kExtraKeys / kTile;
   static constexpr int kMargin = kMarginKeys / kTile, kPagedExtra = kPagedExtraKeys / kTile;
 };
@@ -366,7 +366,7 @@ __device__ __forceinline__ float *record(const Params &p, int index) {
 
 template <int D, bool Q8, int NR>
 struct Smem {
-  static constexpr int kWarps = Cfg<Q8, NR>::kWarps, kPass = NR / 2;
+  static constexpr int kWarps = Cfg<Q8, NR>::kWarps, kPass = NR == 4 ? 4 : NR / 2;
   uint8_t ring[kWarps][Cfg<Q8, NR>::kStages][Geo<D, Q8, NR>::kStageBytes];
   union {
     float merge[kWarps][kPass][D];  // the warps' accumulators, kPass rows at a time
@@ -454,10 +454,40 @@ __device__ __forceinline__ void store_row(uint16_t *dst, const float (&a)[N]) {
   else *dst = f32_to_bf16_bits(a[0]);
 }
 
+// x of the lanes that hold the scores of row r % 4 (up to four rows).
+__device__ __forceinline__ float of_row(float x, int r) { return __shfl_sync(0xffffffffu, x, (r & 3) * 4); }
+// Every (row, output dim, value of that and the next three dims) of a thread's accumulators to f, times the row's factor.
+template <int D, bool Q8, int NR, int ND, int HH, typename F>
+__device__ __forceinline__ void for_rows(const float (&acc)[ND][4], const float (&factor)[HH], int g, int t, F f) {
+  if constexpr (NR == 4) {
+    const float f0 = of_row(factor[0], 2 * t), f1 = of_row(factor[0], 2 * t + 1);
+    if (t >= 2) return;
+#pragma unroll
+    for (int j = 0; j < ND; j += 2)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const float x = c ? f1 : f0;
+        f(2 * t + c, D / 8 * g + 2 * j, make_float4(acc[j][c] * x, acc[j][2 + c] * x, acc[j + 1][c] * x, acc[j + 1][2 + c] * x));
+      }
+  } else {
+#pragma unroll
+    for (int hh = 0; hh < HH; ++hh)
+#pragma unroll
+      for (int j = 0; j < ND; j += 4)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int c = 2 * hh + e;
+          const float x = factor[hh];
+          f(g + 8 * hh, Geo<D, Q8, NR>::out_dim(j, e, t),
+            make_float4(acc[j][c] * x, acc[j + 1][c] * x, acc[j + 2][c] * x, acc[j + 3][c] * x));
+        }
+  }
+}
+
 // The keys of a launch: the sequences' own, alone or beside a prefix, or the prefix's.
 enum Mode { kOwn, kBeside, kPrefix };
 
-// NR: query rows in use, 8 or 16. A (CTA, segment) pair leaves its record in slot CTA + segment: both only grow along the
+// NR: query rows in use, 8 or 16, or over int8 pages 4. A (CTA, segment) pair leaves its record in slot CTA + segment: both only grow along the
 // list, so slots are the pairs' own and a segment's are consecutive. Alone, a segment that one CTA holds goes
 // straight to the output, and a split one's records are added up by the last of its CTAs to get there.
 template <int D, bool Q8, int NR, Mode MODE, bool PAGED = false>
@@ -466,9 +496,16 @@ __device__ __forceinline__ void attn_body(const Params &p, int block, int grid) 
   using G = Geo<D, Q8, NR>;
   using S = Smem<D, Q8, NR>;
   constexpr int kWarps = C::kWarps, STAGES = C::kStages;
-  constexpr int TILE = G::kTile, NT = TILE / 8, ND = D / 8;
+  constexpr int TILE = G::kTile, NT = TILE / 8, ND = NR == 4 ? D / 16 : D / 8;
   constexpr bool PREFIX = MODE == kPrefix;
-  constexpr bool PLANES = Q8 && NR == 8;  // scores by int8 MMAs on the digits of q
+  constexpr bool PLANES = Q8 && NR <= 8;  // scores by int8 MMAs on the digits of q
+  // Up to four rows: all four digits of a row fill the scores' MMA (digits 3, 2, 1, 0 of row r in its rows r, 4 + r, 8 + r, 12
+  // + r), half as many as for eight rows, and P.V is taken the other way round, with V^T as M and as N the rows' weights,
+  // first values and then second ones, which lie in the lanes as the scores leave them: again half the MMAs, and
+  // half the accumulators. Lanes of rows g and g + 4 hold the same row's scores.
+  constexpr bool FOUR = NR == 4;
+  constexpr int HH = FOUR ? 1 : NR / 8;
+  static_assert(!FOUR || (Q8 && MODE == kOwn), "four rows: int8, the sequences' own keys");
   extern __shared__ __align__(16) uint8_t smem_raw[];
   S &sm = *(S *)smem_raw;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -599,11 +636,11 @@ __device__ __forceinline__ void attn_body(const Params &p, int block, int grid) 
       lslot = lslot + 1 == STAGES ? 0 : lslot + 1;
     };
     // the segment's query rows, dims d0 .. d0 + 3 of every 16-dim step: those of the key words that this thread loads
-    uint2 qw[NR / 8][D / 16];
+    uint2 qw[HH][D / 16];
     auto load_q = [&](const Seg &sg) {
 #pragma unroll
-      for (int hh = 0; hh < NR / 8; ++hh) {
-        const int r = g + 8 * hh;
+      for (int hh = 0; hh < HH; ++hh) {
+        const int r = FOUR ? g & 3 : g + 8 * hh;
         int64_t tok = -1;
         int h = 0;
         if (PREFIX) {
@@ -628,10 +665,10 @@ __device__ __forceinline__ void attn_body(const Params &p, int block, int grid) 
     int cslot = 0;
     for (;;) {
       // ---- the segment's query rows as MMA fragments
-      uint32_t qa[PLANES ? D / 32 : D / 16][PLANES ? 8 : 4];
+      uint32_t qa[PLANES ? D / 32 : D / 16][PLANES && !FOUR ? 8 : 4];
       float rowfac[2] = {p.scale_log2, p.scale_log2};  // and for int8 the power of two that q was divided by
 #pragma unroll
-      for (int hh = 0; hh < NR / 8; ++hh) {
+      for (int hh = 0; hh < HH; ++hh) {
         const uint2(&w)[D / 16] = qw[hh];
         uint32_t amax2 = 0u;  // the largest magnitudes of the even and odd elements, as bf16 bits (NaN above infinity)
 #pragma unroll
@@ -664,6 +701,10 @@ __device__ __forceinline__ void attn_body(const Params &p, int block, int grid) 
               d[2] = __byte_perm(hi01, hi23, 0x5410), d[3] = __byte_perm(hi01, hi23, 0x7632);
               // MMA 0: planes 3 and 2 in rows g and g + 8; MMA 1: planes 1 and 0
               const int c = 2 * (s & 1);
+              if constexpr (FOUR) {
+                qa[s / 2][c] = g < 4 ? d[3] : d[2], qa[s / 2][c + 1] = g < 4 ? d[1] : d[0];
+                continue;
+              }
               qa[s / 2][c] = d[3], qa[s / 2][c + 1] = d[2], qa[s / 2][4 + c] = d[1], qa[s / 2][4 + c + 1] = d[0];
             } else {
               qa[s][hh] = f16x2(y[0], y[1]), qa[s][hh + 2] = f16x2(y[2], y[3]);
@@ -716,7 +757,17 @@ __device__ __forceinline__ void attn_body(const Params &p, int block, int grid) 
           }
           float2 ks = make_float2(1.f, 1.f);
           if (Q8) ks = *(const float2 *)(ksc + 8 * nt + 2 * t), vs[nt] = *(const float2 *)(vsc + 8 * nt + 2 * t);
-          if constexpr (PLANES) {
+          if constexpr (FOUR) {
+            int x[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int s = 0; s < D / 32; ++s) mma_i8(x, qa[s], kw[2 * s], kw[2 * s + 1]);
+            // digits 3 and 1 here, 2 and 0 in the lane of row g + 4 (sums up to 2^21, exact in fp32), or the other way round
+            const float unit = g < 4 ? 256.f : 1.f;
+            const float a = fmaf((float)x[0], 65536.f, (float)x[2]) * unit, b = fmaf((float)x[1], 65536.f, (float)x[3]) * unit;
+            sc[nt][0] = (a + __shfl_xor_sync(0xffffffffu, a, 16)) * (rowfac[0] * ks.x);
+            sc[nt][1] = (b + __shfl_xor_sync(0xffffffffu, b, 16)) * (rowfac[0] * ks.y);
+            sc[nt][2] = sc[nt][3] = 0.f;
+          } else if constexpr (PLANES) {
             int hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
 #pragma unroll
             for (int s = 0; s < D / 32; ++s) {
@@ -739,7 +790,7 @@ __device__ __forceinline__ void attn_body(const Params &p, int block, int grid) 
               }
             }
 #pragma unroll
-            for (int hh = 0; hh < NR / 8; ++hh) sc[nt][2 * hh] *= rowfac[hh] * ks.x, sc[nt][2 * hh + 1] *= rowfac[hh] * ks.y;
+            for (int hh = 0; hh < HH; ++hh) sc[nt][2 * hh] *= rowfac[hh] * ks.x, sc[nt][2 * hh + 1] *= rowfac[hh] * ks.y;
           }
         }
         if (left < TILE) {  // the segment's last tile
@@ -752,7 +803,7 @@ __device__ __forceinline__ void attn_body(const Params &p, int block, int grid) 
         }
         float ms[2], alpha[2] = {1.f, 1.f};
 #pragma unroll
-        for (int hh = 0; hh < NR / 8; ++hh) {
+        for (int hh = 0; hh < HH; ++hh) {
           float mx = -INFINITY;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) mx = fmaxf(mx, fmaxf(sc[nt][2 * hh], sc[nt][2 * hh + 1]));
@@ -769,21 +820,27 @@ __device__ __forceinline__ void attn_body(const Params &p, int block, int grid) 
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-          for (int hh = 0; hh < NR / 8; ++hh) {
+          for (int hh = 0; hh < HH; ++hh) {
             float p0 = ex2(sc[nt][2 * hh] - ms[hh]), p1 = ex2(sc[nt][2 * hh + 1] - ms[hh]);
             l_part[hh] += p0 + p1;
             if (Q8) p0 *= vs[nt].x, p1 *= vs[nt].y;  // (past the segment's end both are zeros)
             const uint32_t hi = bf16x2(p0, p1), lo = bf16x2(p0 - bf16_lo(hi), p1 - bf16_hi(hi));
+            if constexpr (FOUR) {
+              pa[nt / 2][nt % 2] = g < 4 ? hi : lo;
+              continue;
+            }
             pa[nt / 2][2 * (nt % 2) + hh] = hi;
             if (NR == 16) pb[nt / 2][2 * (nt % 2) + hh] = lo;
             else pa[nt / 2][2 * (nt % 2) + 1] = lo;
           }
         }
         if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+          float column0 = 1.f, column1 = 1.f;  // of the accumulators' columns 2t, 2t + 1
+          if (FOUR) column0 = of_row(alpha[0], 2 * t), column1 = of_row(alpha[0], 2 * t + 1);
 #pragma unroll
           for (int j = 0; j < ND; ++j)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) acc[j][c] *= alpha[NR == 16 ? c / 2 : 0];
+            for (int c = 0; c < 4; ++c) acc[j][c] *= FOUR ? (c & 1 ? column1 : column0) : alpha[NR == 16 ? c / 2 : 0];
         }
         // ---- P.V: step u takes keys 16 u .. 16 u + 15; this thread's pairs are keys 2t, 2t + 1 and 2t + 8, 2t + 9 of them
 #pragma unroll
@@ -812,12 +869,21 @@ __device__ __forceinline__ void attn_body(const Params &p, int block, int grid) 
             if (Q8) {  // four dims of two key pairs: interleave the pair's bytes, then widen two at a time
               const uint32_t pair[2][2] = {{__byte_perm(vw[0][w], vw[1][w], 0x5140), __byte_perm(vw[0][w], vw[1][w], 0x7362)},
                                            {__byte_perm(vw[2][w], vw[3][w], 0x5140), __byte_perm(vw[2][w], vw[3][w], 0x7362)}};
+              if constexpr (FOUR) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  const uint32_t a[4] = {widen2(pair[0][e], 0x4140), widen2(pair[0][e], 0x4342), widen2(pair[1][e], 0x4140),
+                                         widen2(pair[1][e], 0x4342)};
+                  mma<false>(acc[2 * w + e], a, pa[u][0], pa[u][1]);
+                }
+                continue;
+              }
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 const uint32_t select = e & 1 ? 0x4342 : 0x4140;
                 const uint32_t b0 = widen2(pair[0][e / 2], select), b1 = widen2(pair[1][e / 2], select);
-                mma<false>(acc[4 * w + e], pa[u], b0, b1);
-                if (NR == 16) mma<false>(acc[4 * w + e], pb[u % (NR == 16 ? NT / 2 : 1)], b0, b1);
+                mma<false>(acc[(4 * w + e) % ND], pa[u], b0, b1);
+                if (NR == 16) mma<false>(acc[(4 * w + e) % ND], pb[u % (NR == 16 ? NT / 2 : 1)], b0, b1);
               }
             } else {
 #pragma unroll
@@ -837,49 +903,49 @@ __device__ __forceinline__ void attn_body(const Params &p, int block, int grid) 
 #pragma unroll
         for (int j = 0; j < ND; ++j) acc[j][0] += acc[j][2], acc[j][1] += acc[j][3];
       }
+      if (FOUR) {  // columns 2t, 2t + 1 are rows (2t) % 4, (2t + 1) % 4
+#pragma unroll
+        for (int j = 0; j < ND; ++j)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) acc[j][c] += __shfl_xor_sync(0xffffffffu, acc[j][c], 2);
+      }
       const Seg done = seg;
       const bool another = lay.pad == 1 && advance(seg);
       if (another) load_q(seg);  // on its way while this one is added up
       // ---- the segment is done: the warps' states, each relative to the largest maximum, are added up in shared memory
 #pragma unroll
-      for (int hh = 0; hh < NR / 8; ++hh) {
+      for (int hh = 0; hh < HH; ++hh) {
         l_part[hh] += __shfl_xor_sync(0xffffffffu, l_part[hh], 1);
         l_part[hh] += __shfl_xor_sync(0xffffffffu, l_part[hh], 2);
-        if (t == 0 && !lay.solo) sm.warp_m[warp][g + 8 * hh] = m_run[hh], sm.warp_l[warp][g + 8 * hh] = l_part[hh];
+        if (t == 0 && (!FOUR || g < 4) && !lay.solo) sm.warp_m[warp][g + 8 * hh] = m_run[hh], sm.warp_l[warp][g + 8 * hh] = l_part[hh];
       }
       if (!PREFIX && lay.solo) {  // the warp's own: to the output, or a record in the segment's slot
         float *rec = record<D>(p, done.index);
         uint16_t *out = p.out + done.seq * p.ldo + (int64_t)done.g * p.group * D;
+        float inv[HH];
 #pragma unroll
-        for (int hh = 0; hh < NR / 8; ++hh) {
+        for (int hh = 0; hh < HH; ++hh) inv[hh] = MODE == kOwn ? inverse_sum(l_part[hh]) : 1.f;
+        for_rows<D, Q8, NR>(acc, inv, g, t, [&](int r, int dim, float4 v) {
+          if (r >= p.group) return;
+          if (MODE == kOwn) *(uint2 *)(out + r * D + dim) = make_uint2(bf16x2(v.x, v.y), bf16x2(v.z, v.w));
+          else *(float4 *)(rec + r * D + dim) = v;
+        });
+#pragma unroll
+        for (int hh = 0; hh < HH; ++hh) {
           const int r = g + 8 * hh;
-          if (r < p.group) {
-            const float inv = inverse_sum(l_part[hh]);
-#pragma unroll
-            for (int j = 0; j < ND; j += 4)
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const int c = 2 * hh + e, dim = r * D + G::out_dim(j, e, t);
-                if (MODE == kOwn)
-                  *(uint2 *)(out + dim) = make_uint2(bf16x2(acc[j][c] * inv, acc[j + 1][c] * inv),
-                                                     bf16x2(acc[j + 2][c] * inv, acc[j + 3][c] * inv));
-                else
-                  *(float4 *)(rec + dim) = make_float4(acc[j][c], acc[j + 1][c], acc[j + 2][c], acc[j + 3][c]);
-              }
-            if (MODE != kOwn && t == 0) rec[kRows * D + r] = m_run[hh], rec[kRows * D + kRows + r] = l_part[hh];
-          }
+          if (MODE != kOwn && t == 0 && r < p.group) rec[kRows * D + r] = m_run[hh], rec[kRows * D + kRows + r] = l_part[hh];
         }
         if (MODE == kBeside && lane == 0) p.parts[done.index] = make_int2(done.index, 1);
         if (!another) break;
         continue;
       }
       __syncthreads();
-      float fac[NR / 8];
+      float fac[HH];
 #pragma unroll
-      for (int hh = 0; hh < NR / 8; ++hh) {
+      for (int hh = 0; hh < HH; ++hh) {
         float mx = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, sm.warp_m[w][g + 8 * hh]);
+        for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, sm.warp_m[w][FOUR ? g & 3 : g + 8 * hh]);
         fac[hh] = ex2(m_run[hh] - (mx == -INFINITY ? 0.f : mx));
       }
       if (threadIdx.x < NR) {
@@ -899,20 +965,9 @@ __device__ __forceinline__ void attn_body(const Params &p, int block, int grid) 
 #pragma unroll 1
       for (int r0 = 0; r0 < rows; r0 += kPass) {
         if (r0) __syncthreads();  // the last pass has been read
-#pragma unroll
-        for (int hh = 0; hh < NR / 8; ++hh) {
-          const int r = g + 8 * hh - r0;
-          if (r >= 0 && r < kPass && r + r0 < rows) {
-#pragma unroll
-            for (int j = 0; j < ND; j += 4)
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const int c = 2 * hh + e;
-                *(float4 *)&sm.merge[warp][r][G::out_dim(j, e, t)] =
-                    make_float4(acc[j][c] * fac[hh], acc[j + 1][c] * fac[hh], acc[j + 2][c] * fac[hh], acc[j + 3][c] * fac[hh]);
-              }
-          }
-        }
+        for_rows<D, Q8, NR>(acc, fac, g, t, [&](int r, int dim, float4 v) {
+          if (r >= r0 && r < r0 + kPass && r < rows) *(float4 *)&sm.merge[warp][r - r0][dim] = v;
+        });
         __syncthreads();
 #pragma unroll 1
         for (int e = threadIdx.x; e < min(kPass, rows - r0) * D; e += C::kThreads) {
@@ -1122,6 +1177,8 @@ static cudaError_t launch_d(Params &p, int d, cudaStream_t st, bool pdl) {
 }
 template <Mode MODE, bool PAGED = false>
 static cudaError_t launch_any(Params &p, int d, bool q8, cudaStream_t st, bool pdl) {
+  if constexpr (PAGED)
+    if (q8 && p.group <= 4) return launch_d<true, 4, MODE, PAGED>(p, d, st, pdl);
   if (p.group <= 8) return q8 ? launch_d<true, 8, MODE, PAGED>(p, d, st, pdl) : launch_d<false, 8, MODE, PAGED>(p, d, st, pdl);
   return q8 ? launch_d<true, 16, MODE, PAGED>(p, d, st, pdl) : launch_d<false, 16, MODE, PAGED>(p, d, st, pdl);
 }
