@@ -57,7 +57,7 @@ constexpr int kExtraKeys = 512;  // what a segment's start and end cost, in keys
 // Over pages, whose segments are cut wherever the even cuts fall, but nearer to an end than the margin at that end: no CTA
 // has more than its share, where leaving short segments whole gave some half as much again (64 rows over 200 to
 // 16000 bf16 keys 181 -> 155 us, 478 MB of int8 174 -> 140).
-constexpr int kMarginKeys = 256, kPagedExtraKeys = 256;
+constexpr int kMarginKeys = 256;
 
 struct Cache {
   const uint8_t *k, *v;
@@ -110,12 +110,16 @@ struct Seg {
 // Shape of a CTA (one per SM) by type and query rows.
 template <bool Q8, int NR>
 struct Cfg {
-  static constexpr int kWarps = 8;
+  // (up to four rows need fewer registers and take more warps: 64 rows over 3544 int8 keys 104 us with 8, 96 with 12)
+  static constexpr int kWarps = NR == 4 ? 12 : 8;
   static constexpr int kThreads = 32 * kWarps;
   static constexpr int kTile = Q8 ? 32 : 16;  // keys per warp tile: K and V 4 KB each at d = 128
-  static constexpr int kStages = NR <= 8 ? 3 : 2;
+  static constexpr int kStages = NR == 8 ? 3 : 2;
   static constexpr int kMinChunk = kMinKeys / kTile, kExtra = kExtraKeys / kTile;
-  static constexpr int kMargin = kMarginKeys / kTile, kPagedExtra = kPagedExtraKeys / kTile;
+  // what a segment costs besides its tiles over pages, where its warps' merge comes in between two segments' loads: with 256,
+  // 512, 768 int8 keys 64 rows over 200 to 16000 take 155, 128, 122 us (bf16: no difference there, and for 16 rows of 33
+  // to 288 12.1, 9.8, 9.7)
+  static constexpr int kMargin = kMarginKeys / kTile, kPagedExtra = (Q8 ? 768 : 512) / kTile;
 };
 template <int D, bool Q8, int NR>
 struct Geo {
@@ -254,12 +258,12 @@ __device__ __forceinline__ Layout make_layout(const Params &p, int grid, int *cu
     }
     __syncthreads();
   } else {
-    constexpr int kPer = kMaxBatch / C::kThreads;
+    constexpr int kPer = (kMaxBatch + C::kThreads - 1) / C::kThreads;
     int places[kPer], sum = 0;
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
       const int i = t * kPer + e, keys = i < p.m ? seq_len(p, i) : 0, tiles = ceil_div(keys, C::kTile);
-      len_of[i] = keys;
+      if (i < kMaxBatch) len_of[i] = keys;
       places[e] = tiles ? tiles + (PAGED ? C::kPagedExtra : C::kExtra) : 0;
       sum += places[e];
       segs += tiles > 0, rounds += ceil_div(tiles, C::kWarps), longest = max(longest, tiles);
@@ -286,7 +290,7 @@ __device__ __forceinline__ Layout make_layout(const Params &p, int grid, int *cu
     }
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
-      cum[t * kPer + e] = before;
+      if (t * kPer + e < kMaxBatch) cum[t * kPer + e] = before;
       before += places[e];
     }
     if (t == C::kThreads - 1) cum[kMaxBatch] = before;
@@ -366,7 +370,7 @@ __device__ __forceinline__ float *record(const Params &p, int index) {
 
 template <int D, bool Q8, int NR>
 struct Smem {
-  static constexpr int kWarps = Cfg<Q8, NR>::kWarps, kPass = NR == 4 ? 4 : NR / 2;
+  static constexpr int kWarps = Cfg<Q8, NR>::kWarps, kPass = NR / 2;
   uint8_t ring[kWarps][Cfg<Q8, NR>::kStages][Geo<D, Q8, NR>::kStageBytes];
   union {
     float merge[kWarps][kPass][D];  // the warps' accumulators, kPass rows at a time
@@ -809,7 +813,8 @@ __device__ __forceinline__ void attn_body(const Params &p, int block, int grid) 
           for (int nt = 0; nt < NT; ++nt) mx = fmaxf(mx, fmaxf(sc[nt][2 * hh], sc[nt][2 * hh + 1]));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-          const float m_new = fmaxf(m_run[hh], mx);
+          // (over pages the maximum in use moves only for one 2^8 larger: weights up to that and few rescaled sums)
+          const float m_new = PAGED && mx <= m_run[hh] + 8.f ? m_run[hh] : fmaxf(m_run[hh], mx);
           ms[hh] = m_new == -INFINITY ? 0.f : m_new;
           alpha[hh] = ex2(m_run[hh] - ms[hh]);
           m_run[hh] = m_new;
