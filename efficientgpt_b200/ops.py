@@ -486,14 +486,19 @@ def attn_shared_prefix(q, prefix, tails, position, prefix_len, nq, nkv, d, *, sc
 # ---- KV cache in pages: a pool of pages, named by a table, for sequences that come and go ----
 
 
-def _here(what, *ts):
-    """Every tensor on the current device, whose stream the call goes to (the first of them is one)."""
-    device = ts[0].get_device()
+def _here(what, device, *ts):
+    """Refuses tensors on another device than `device`, the current one, whose stream the call goes to."""
     for t in ts:
         if t is not None and t.get_device() != device:
-            device = -1
+            raise ValueError(f'{what}: CUDA tensors on the current device expected (there is no CPU path)')
+
+
+def _device_of(what, t):
+    """The device of t, which has to be the current one."""
+    device = t.get_device()
     if device < 0 or device != _current_device():
         raise ValueError(f'{what}: CUDA tensors on the current device expected (there is no CPU path)')
+    return device
 
 
 def kv_pages(pages, nkv, page_size, d, device, dtype=torch.bfloat16):
@@ -509,7 +514,7 @@ def kv_pages(pages, nkv, page_size, d, device, dtype=torch.bfloat16):
 
 
 def _pool(what, pages, table):
-    """Checks a pool and its table int32 [M, columns]; -> (shape of the pool, its four pointers, the table's arguments)."""
+    """Checks a pool and its table int32 [M, columns]; -> (shape of the pool, the C arguments for both, M, device)."""
     if len(pages) == 2:
         k, v = pages
         ks = vs = None
@@ -525,13 +530,16 @@ def _pool(what, pages, table):
     shape = k.shape
     if len(shape) != 4 or v.shape != shape or not (k.is_contiguous() and v.is_contiguous()):
         raise ValueError(f'{what}: contiguous pages [pages, nkv, page_size, d] expected')
-    if table.dtype is not torch.int32 or table.dim() != 2 or table.stride(1) != 1:
+    if table.dtype is not torch.int32 or table.dim() != 2:
         raise ValueError(f'{what}: the table must be int32 [M, columns] with unit column stride')
-    _here(what, k, ks, v, vs, table)
-    ptrs = (k.data_ptr(), ks.data_ptr(), v.data_ptr(), vs.data_ptr()) if ks is not None else (k.data_ptr(), None, v.data_ptr(),
-                                                                                              None)
     seqs, columns = table.shape
-    return shape, ptrs + (shape[0], shape[2], table.data_ptr(), table.stride(0) if seqs > 1 else columns, columns), seqs
+    ldt, unit = table.stride()
+    if unit != 1 and columns > 1:
+        raise ValueError(f'{what}: the table must be int32 [M, columns] with unit column stride')
+    device = _device_of(what, k)
+    _here(what, device, v, table, ks, vs)
+    return shape, (k.data_ptr(), None if ks is None else ks.data_ptr(), v.data_ptr(), None if vs is None else vs.data_ptr(),
+                   shape[0], shape[2], table.data_ptr(), ldt if seqs > 1 else columns, columns), seqs, device
 
 
 def kv_append_paged(k, v, pages, table, position, *, starts=None, q=None, q_norm_w=None, k_norm_w=None, eps=1e-6,
@@ -542,13 +550,14 @@ def kv_append_paged(k, v, pages, table, position, *, starts=None, q=None, q_norm
     left alone. k_norm_w / q_norm_w: RMSNorm of the k / q heads; rope_cos, rope_sin (bf16 or fp32 [rows, d / 2]): rotation to
     position rope_base + slot. With q [M, nq * d] the normed and rotated q is returned (in q_out, which may be q; rows
     without a slot are zeros). Norm and rotation are fp32 and rounded once, to bf16 or to an int8 pool's codes."""
-    shape, pool, seqs = _pool('kv_append_paged', pages, table)
-    nkv, d = shape[1], shape[3]
-    m, width = k.shape
-    if k.dtype is not _BF16 or v.dtype is not _BF16 or v.shape != k.shape or width != nkv * d or k.stride(1) != 1 or v.stride(
-            1) != 1:
+    (_, nkv, _, d), pool, seqs, device = _pool('kv_append_paged', pages, table)
+    rows = k.shape
+    m = rows[0]
+    ldk, unit_k = k.stride()
+    ldv, unit_v = v.stride()
+    if k.dtype is not _BF16 or v.dtype is not _BF16 or rows[1] != nkv * d or v.shape != rows or unit_k != 1 or unit_v != 1:
         raise ValueError('kv_append_paged: k and v must be bf16 [M, nkv * d] with unit column stride')
-    _here('kv_append_paged', k, v, position, starts, q, q_norm_w, k_norm_w, rope_cos, rope_sin, q_out)
+    _here('kv_append_paged', device, k, v, position, starts, q_norm_w, k_norm_w, rope_cos, rope_sin)
     if position.dtype is not _I64 or position.shape != (seqs,) or not position.is_contiguous():
         raise ValueError('kv_append_paged: position must be a contiguous int64 tensor of one slot a sequence')
     if starts is None:
@@ -556,32 +565,40 @@ def kv_append_paged(k, v, pages, table, position, *, starts=None, q=None, q_norm
             raise ValueError('kv_append_paged: without starts there is one row a sequence')
     elif starts.dtype is not _I64 or starts.shape != (seqs + 1,) or not starts.is_contiguous():
         raise ValueError('kv_append_paged: starts must be a contiguous int64 tensor of sequences + 1')
+    else:
+        starts = starts.data_ptr()
+    norms = []
     for w in (q_norm_w, k_norm_w):
-        if w is not None and (w.dtype is not _BF16 or w.numel() != d or not w.is_contiguous()):
-            raise ValueError('kv_append_paged: norm weights must be bf16 [d]')
+        if w is not None:
+            if w.dtype is not _BF16 or w.numel() != d or not w.is_contiguous():
+                raise ValueError('kv_append_paged: norm weights must be bf16 [d]')
+            w = w.data_ptr()
+        norms.append(w)
     rope = (None, None, 0, 0)
-    if (rope_cos is None) != (rope_sin is None):
-        raise ValueError('kv_append_paged: rope_cos and rope_sin come together')
-    if rope_cos is not None:
-        if (rope_cos.dim() != 2 or rope_cos.shape[1] != d // 2 or rope_sin.shape != rope_cos.shape
-                or rope_sin.dtype is not rope_cos.dtype or not (rope_cos.is_contiguous() and rope_sin.is_contiguous())):
+    if rope_cos is not None and rope_sin is not None:
+        length = rope_cos.shape
+        if (len(length) != 2 or length[1] != d // 2 or rope_sin.shape != length or rope_sin.dtype is not rope_cos.dtype
+                or not (rope_cos.is_contiguous() and rope_sin.is_contiguous())):
             raise ValueError('kv_append_paged: RoPE tables must be contiguous [rows, d / 2] of one dtype')
-        rope = (rope_cos.data_ptr(), rope_sin.data_ptr(), _dt(rope_cos), rope_cos.shape[0])
-    rows = (None, 0, None, 0, 0)
+        rope = (rope_cos.data_ptr(), rope_sin.data_ptr(), _dt(rope_cos), length[0])
+    elif rope_cos is not rope_sin:
+        raise ValueError('kv_append_paged: rope_cos and rope_sin come together')
+    queries = (None, 0, None, 0, 0)
     if q is not None:
-        if q.dtype is not _BF16 or q.dim() != 2 or q.shape[0] != m or q.shape[1] % d or q.stride(1) != 1:
+        width = q.shape
+        ldq, unit = q.stride()
+        if q.dtype is not _BF16 or len(width) != 2 or width[0] != m or width[1] % d or unit != 1:
             raise ValueError('kv_append_paged: q must be bf16 [M, nq * d] with unit column stride')
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=_BF16, device=q.device)
-        elif q_out.dtype is not _BF16 or q_out.shape != q.shape or q_out.stride(1) != 1:
+            q_out = torch.empty_like(q)
+        elif q_out.dtype is not _BF16 or q_out.shape != width or q_out.stride(1) != 1:
             raise ValueError('kv_append_paged: q_out must be bf16 rows of the shape of q')
-        rows = (q_out.data_ptr(), q_out.stride(0), q.data_ptr(), q.stride(0), q.shape[1] // d)
+        _here('kv_append_paged', device, q, q_out)
+        queries = (q_out.data_ptr(), q_out.stride(0), q.data_ptr(), ldq, width[1] // d)
     elif q_norm_w is not None or q_out is not None:
         raise ValueError('kv_append_paged: q_norm_w and q_out need q')
-    rc = L.load().egpt_kv_append_paged(
-        *pool, seqs, k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), position.data_ptr(),
-        None if starts is None else starts.data_ptr(), m, nkv, d, *rows, None if q_norm_w is None else q_norm_w.data_ptr(),
-        None if k_norm_w is None else k_norm_w.data_ptr(), eps, *rope, rope_base, 0, _raw_stream())
+    rc = L.load().egpt_kv_append_paged(*pool, seqs, k.data_ptr(), ldk, v.data_ptr(), ldv, position.data_ptr(), starts, m, nkv, d,
+                                       *queries, *norms, eps, *rope, rope_base, 0, _raw_stream_of(device))
     if rc:
         L.check(rc, 'kv_append_paged')
     return q_out
@@ -591,27 +608,27 @@ def kv_read_paged(pages, table, start, count, *, dtype=torch.bfloat16, out=None)
     """The rows start .. start + count - 1 of every sequence of the table (start: an int, or int64 [M] on the device): (k,
     v), each [M * nkv, count, d] bf16 or fp32; slots outside the table and pages of -1 read as zeros. out: the (k, v)
     tensors to fill, rows contiguous, one head stride."""
-    shape, pool, seqs = _pool('kv_read_paged', pages, table)
-    nkv, d = shape[1], shape[3]
+    (_, nkv, _, d), pool, seqs, device = _pool('kv_read_paged', pages, table)
     heads = seqs * nkv
     if out is None:
-        k, v = (torch.empty((heads, count, d), dtype=dtype, device=table.device) for _ in range(2))
+        k = pages[0].new_empty((heads, count, d), dtype=dtype)
+        v = torch.empty_like(k)
         stride = count * d
     else:
         k, v = out
-        _here('kv_read_paged', k, v)
+        _here('kv_read_paged', device, k, v)
         if (k.shape != (heads, count, d) or v.shape != k.shape or k.stride() != v.stride() or k.dtype is not v.dtype
                 or (count > 1 and k.stride(1) != d) or k.stride(2) != 1):
             raise ValueError('kv_read_paged: out must be two tensors [M * nkv, count, d] with contiguous rows')
         stride = k.stride(0) if heads > 1 else count * d
     starts = None
     if isinstance(start, torch.Tensor):
-        _here('kv_read_paged', start)
+        _here('kv_read_paged', device, start)
         if start.dtype is not _I64 or start.shape != (seqs,) or not start.is_contiguous():
             raise ValueError('kv_read_paged: start must be an int or a contiguous int64 tensor of one slot a sequence')
         starts, start = start.data_ptr(), 0
     rc = L.load().egpt_kv_read_paged(k.data_ptr(), v.data_ptr(), stride, _dt(k), *pool, seqs, nkv, d, start, starts, count, 0,
-                                     _raw_stream())
+                                     _raw_stream_of(device))
     if rc:
         L.check(rc, 'kv_read_paged')
     return k, v
@@ -625,8 +642,8 @@ def attn_paged_ws(m, nq, nkv, d, device):
 def attn_decode_paged(q, pages, table, position, nq, nkv, d, *, scale, ws=None, out=None):
     """Decode attention over pages: row i of q bf16 [M, nq * d] over the position[i] + 1 keys of sequence i (int64 [M] on the
     device; -1: an idle slot, zeros), whose pages row i of `table` names -> bf16 [M, nq * d]."""
-    shape, pool, seqs = _pool('attn_decode_paged', pages, table)
-    _here('attn_decode_paged', q, position, ws, out)
+    shape, pool, seqs, device = _pool('attn_decode_paged', pages, table)
+    _here('attn_decode_paged', device, q, position, ws)
     m, out = _attn_rows('attn_decode_paged', q, out, nq, d)
     if shape[1] != nkv or shape[3] != d or seqs != m:
         raise ValueError('attn_decode_paged: pages [pages, nkv, page_size, d] and a table row for each row of q expected')
@@ -634,8 +651,10 @@ def attn_decode_paged(q, pages, table, position, nq, nkv, d, *, scale, ws=None, 
         raise ValueError('attn_decode_paged: position must be a contiguous int64 tensor of one slot a sequence')
     if ws is None:
         ws = attn_paged_ws(m, nq, nkv, d, q.device)
+    if out.get_device() != device:
+        _here('attn_decode_paged', device, out)
     rc = L.load().egpt_attn_decode_paged(out.data_ptr(), out.stride(0), q.data_ptr(), q.stride(0), *pool, position.data_ptr(), m,
-                                         nq, nkv, d, scale, ws.data_ptr(), ws.numel(), 0, _raw_stream())
+                                         nq, nkv, d, scale, ws.data_ptr(), ws.numel(), 0, _raw_stream_of(device))
     if rc:
         L.check(rc, 'attn_decode_paged')
     return out
@@ -656,30 +675,33 @@ def token_logprobs(logits, tokens=None, *, top=0, ws=None, out=None):
     in nats, and its `top` (up to 32) most likely tokens in order, of equal ones the lowest id first. fp32 and int64. logprob is
     None without tokens, the last two are without top. -inf logits are masked tokens; a row of nothing else has log
     probabilities -inf and entropy 0, one with a NaN or +inf has NaN. out: the four tensors to fill (contiguous)."""
-    _here('token_logprobs', logits, tokens, ws)
-    if logits.dim() != 2 or logits.stride(1) != 1:
+    device = _device_of('token_logprobs', logits)
+    _here('token_logprobs', device, tokens, ws)
+    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise ValueError('token_logprobs: logits must be [M, V] with unit column stride')
     m, v = logits.shape
     if tokens is not None and (tokens.dtype is not _I64 or tokens.shape != (m,) or not tokens.is_contiguous()):
         raise ValueError('token_logprobs: tokens must be a contiguous int64 tensor of one id a row')
+    lp = ids = tlp = None
     if out is None:
-        dev = logits.device
-        lp = None if tokens is None else torch.empty(m, dtype=_F32, device=dev)
-        ent = torch.empty(m, dtype=_F32, device=dev)
-        ids = torch.empty((m, top), dtype=_I64, device=dev) if top else None
-        tlp = torch.empty((m, top), dtype=_F32, device=dev) if top else None
+        ent = logits.new_empty((m,), dtype=_F32)
+        if tokens is not None:
+            lp = torch.empty_like(ent)
+        if top:
+            tlp = logits.new_empty((m, top), dtype=_F32)
+            ids = torch.empty_like(tlp, dtype=_I64)
     else:
         lp, ent, ids, tlp = out
-        _here('token_logprobs', logits, *out)
+        _here('token_logprobs', device, *out)
         for t, dt, shape in ((lp, _F32, (m,)), (ent, _F32, (m,)), (ids, _I64, (m, top)), (tlp, _F32, (m, top))):
             if t is not None and (t.dtype is not dt or t.shape != shape or not t.is_contiguous()):
                 raise ValueError('token_logprobs: out must be fp32 [M], fp32 [M], int64 [M, top] and fp32 [M, top]')
     if ws is None:
         ws = token_logprobs_ws(m, v, logits.device)
-    rc = L.load().egpt_token_logprobs(None if lp is None else lp.data_ptr(), _p(ent), _p(ids), _p(tlp), logits.data_ptr(),
-                                      logits.stride(0) if m > 1 else v, _dt(logits), m, v,
-                                      None if tokens is None else tokens.data_ptr(), top, ws.data_ptr(), ws.numel(), 0,
-                                      _raw_stream())
+    rc = L.load().egpt_token_logprobs(
+        None if lp is None else lp.data_ptr(), None if ent is None else ent.data_ptr(), None if ids is None else ids.data_ptr(),
+        None if tlp is None else tlp.data_ptr(), logits.data_ptr(), logits.stride(0) if m > 1 else v, _dt(logits), m, v,
+        None if tokens is None else tokens.data_ptr(), top, ws.data_ptr(), ws.numel(), 0, _raw_stream_of(device))
     if rc:
         L.check(rc, 'token_logprobs')
     return lp, ent, ids, tlp

@@ -150,7 +150,10 @@ def test_tensors_of_another_device_are_refused(monkeypatch):
             return self.device
 
     monkeypatch.setattr(ops, '_current_device', lambda: 0)
-    ops._here('x', On(0), None, On(0))
-    for ts in ((On(1), On(1)), (On(0), On(1)), (On(0), None, On(-1)), (On(-1),)):
+    assert ops._device_of('x', On(0)) == 0
+    ops._here('x', 0, On(0), None, On(0))
+    for device in (1, -1):
         with pytest.raises(ValueError, match='current device'):
-            ops._here('x', *ts)
+            ops._device_of('x', On(device))
+        with pytest.raises(ValueError, match='current device'):
+            ops._here('x', 0, On(0), None, On(device))
