@@ -4,8 +4,9 @@ Drop-in for the research/realmodel path of BagelsFun/efficientgpt: `int8_linear`
 `fast_decode.GraphGreedyDecoder` (and `SampledGraphDecoder` with `sampling`: temperature, top-k, top-p, inverse
 CDF on the device), `backend.BucketedGraphDecoder` (the request-sized decoder pool of HFBackend), plus
 `ragged.RaggedGraphDecoder` (up to 16 sequences of different lengths, bf16 or int8 KV cache),
-`shared_prefix.SharedPrefixGraphDecoder` (the same behind a prefix that is held and read once), `tp.TPQwen3Engine` (tensor parallelism)
-and `nanogpt` (config 1), with the
+`shared_prefix.SharedPrefixGraphDecoder` (the same behind a prefix that is held and read once),
+`paged.PagedGraphDecoder` and `paged.PagedEngine` (sequences that come and go out of a pool of KV pages, with the log
+probabilities of their answers), `tp.TPQwen3Engine` (tensor parallelism) and `nanogpt` (config 1), with the
 arithmetic in hand-written CUDA (libegpt_b200.so, C-ABI in
 include/egpt_b200.h). Submodules import lazily so the package imports without a GPU.
 """
@@ -26,6 +27,9 @@ def __getattr__(name):
         return getattr(m, name)
     if name in ('SharedPrefixEngine', 'SharedPrefixGraphDecoder'):  # batches under one shared prefix
         from . import shared_prefix as m
+        return getattr(m, name)
+    if name in ('PagedEngine', 'PagedGraphDecoder', 'PagePool'):  # sequences out of a pool of KV pages
+        from . import paged as m
         return getattr(m, name)
     if name in ('SamplingConfig', 'draw_uniforms', 'sample'):
         from . import sampling as m

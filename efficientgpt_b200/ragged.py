@@ -28,6 +28,7 @@ import torch
 from . import _lib as L
 from . import ops
 from .engine import Qwen3Engine
+from .prefill import _proj as prefill_proj
 
 MAX_ROWS = 16
 
@@ -113,6 +114,19 @@ class RaggedEngine:
         """q, k and v columns of the fused projection's rows."""
         b = self.base
         return qkv.split((b.nq * b.d, b.nkv * b.d, b.nkv * b.d), dim=1)
+
+    def _layers(self, ids, attend):
+        """The rows `ids` (int64 [n]) through all layers, attend(i, lay, qkv) -> attention rows; -> hidden [n, H]."""
+        b = self.base
+        h = ops.embed(ids, b.embed)
+        for i, lay in enumerate(b.layers):
+            x = ops.rmsnorm(h, lay['ln_in'], b.eps)
+            a = attend(i, lay, prefill_proj(x, lay['w_qkv'], lay['s_qkv']))
+            h = prefill_proj(a, lay['w_o'], lay['s_o'], residual=h)
+            x = ops.rmsnorm(h, lay['ln_post'], b.eps)
+            act = ops.silu_mul(prefill_proj(x, lay['w_gu'], lay['s_gu']), b.inter)
+            h = prefill_proj(act, lay['w_down'], lay['s_down'], residual=h)
+        return h
 
     def _attend_prompt(self, row, i, lay, qkv, pos0, ws):
         """Layer i's attention of a prompt's rows, their keys and values written to row `row`'s cache."""
@@ -214,13 +228,16 @@ class RaggedGraphDecoder:
         self.out = torch.zeros(engine.batch, engine.cap, dtype=torch.long, device=engine.device)
         self.col = torch.zeros(1, dtype=torch.long, device=engine.device)
 
+    def _park(self):
+        """Puts the rows where a step without a request may run (a capture's warm-up)."""
+        self.engine.positions.zero_()
+
     def _capture(self):
-        eng = self.engine
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(side):  # warm-up outside capture, each from the start (the last request's place is left)
             for _ in range(2):
-                eng.positions.zero_()
+                self._park()
                 self.col.zero_()
                 self._replay_body()
         torch.cuda.current_stream().wait_stream(side)

@@ -49,19 +49,6 @@ class SharedPrefixEngine(RaggedEngine):
             dst.copy_(src)
         return out
 
-    def _layers(self, ids, attend):
-        """The rows `ids` (int64 [n]) through all layers, attend(i, lay, qkv) -> attention rows; -> hidden [n, H]."""
-        b = self.base
-        h = ops.embed(ids, b.embed)
-        for i, lay in enumerate(b.layers):
-            x = ops.rmsnorm(h, lay['ln_in'], b.eps)
-            a = attend(i, lay, _proj(x, lay['w_qkv'], lay['s_qkv']))
-            h = _proj(a, lay['w_o'], lay['s_o'], residual=h)
-            x = ops.rmsnorm(h, lay['ln_post'], b.eps)
-            act = ops.silu_mul(_proj(x, lay['w_gu'], lay['s_gu']), b.inter)
-            h = _proj(act, lay['w_down'], lay['s_down'], residual=h)
-        return h
-
     @torch.no_grad()
     def set_prefix(self, ids):
         """Prefill the shared prefix (int64 [p]); the rows of an earlier prefix and all tails are forgotten."""

@@ -1,0 +1,285 @@
+"""Decoding out of a pool of KV pages (paged.PagedEngine, paged.PagedGraphDecoder) on small Qwen3 models.
+
+Two engines whose caches hold the same values differ by roundings only: attention sums in other orders, and keys that are
+normed and rotated with one rounding instead of the reference's five. A relative 2^-8 of the attention's rows at most, which
+the residual stream carries to the logits with a gain of a few: logits are held to a relative 2^-6 in the 2-norm of a row
+(four such roundings), as those of the other engines with their own caches."""
+import pytest
+import torch
+
+import golden_inputs as gi
+
+LOGIT_TOL = 2.0 ** -6
+
+
+# ------------------------------------------------------------------------------------------------- pages, on the CPU
+def test_page_pool():
+    from efficientgpt_b200.paged import PagePool
+    pool = PagePool(5)
+    a = pool.take(2)
+    b = pool.take(3)
+    assert sorted(a + b) == [0, 1, 2, 3, 4] and pool.free == 0
+    with pytest.raises(RuntimeError, match='1 pages asked for, 0 of 5 free'):
+        pool.take(1)
+    pool.give(a)
+    assert pool.free == 2 and pool.take(2) == a and pool.take(0) == []
+    with pytest.raises(ValueError):
+        PagePool(0)
+
+
+# ------------------------------------------------------------------------------------------------- engines
+def _model(d, seed=3):
+    from efficientgpt_b200.int8_linear import quantize_model
+    cfg = gi.tiny_config()
+    cfg.initializer_range = 0.05
+    if d == 128:
+        cfg.hidden_size, cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim = 256, 8, 2, 128
+        cfg.max_position_embeddings = 4096
+    model = gi.build_model(cfg, seed=seed).cuda()
+    quantize_model(model, scale_dtype=torch.bfloat16)
+    return model
+
+
+def _batch(batch, longest, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    lengths = torch.randint(1, longest + 1, (batch,), generator=g)
+    lengths[0] = longest
+    lengths[-1] = 1
+    return torch.randint(0, 512, (batch, longest), generator=g), lengths
+
+
+def _ids(n, seed):
+    return torch.randint(0, 512, (n,), generator=torch.Generator().manual_seed(seed)).cuda()
+
+
+def _close(a, b):
+    a, b = a.double(), b.double()
+    off = (a - b).norm(dim=-1) / b.norm(dim=-1)
+    assert (off <= LOGIT_TOL).all(), off
+
+
+def _rows(eng, row, layer):
+    """The cached rows of a sequence, as ragged caches hold them: [heads, length, d] (and scales)."""
+    n = eng.lengths[row]
+    at = torch.arange(n, device='cuda')
+    pages = eng.table[row, at // eng.page_size].long()
+    return [t[pages, :, at % eng.page_size].transpose(0, 1) for t in eng.kv[layer]]
+
+
+def _no_error():
+    from efficientgpt_b200 import _lib as L
+    assert L.device_error() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('kv_dtype', [torch.bfloat16, torch.int8])
+@pytest.mark.parametrize('d,batch,page', [(32, 3, 8), (128, 1, 16), (128, 16, 16), (128, 6, 64)])
+def test_decodes_as_the_ragged_engine_on_the_same_rows(cuda, kv_dtype, d, batch, page):
+    from efficientgpt_b200.paged import PagedEngine
+    from efficientgpt_b200.ragged import RaggedEngine
+    model = _model(d)
+    prompts, lengths = _batch(batch, 37)
+    eng = PagedEngine(model, batch, 16 * batch, 64, page_size=page, kv_dtype=kv_dtype)
+    eng.prefill(prompts, lengths)
+    ref = RaggedEngine(model, batch, 64, kv_dtype=kv_dtype)
+    nkv = ref.base.nkv
+    for i in range(ref.base.n_layers):
+        for r in range(batch):
+            for dst, src in zip(ref.kv[i], _rows(eng, r, i)):
+                dst[r * nkv:(r + 1) * nkv, :eng.lengths[r]] = src
+    ref.tokens.copy_(eng.tokens)
+    ref.positions.copy_(eng.positions)
+    assert ref.positions.tolist() == lengths.tolist() == eng.lengths
+    for _ in range(6):
+        ref.tokens.copy_(eng.tokens)
+        eng.step()
+        ref.step()
+        _close(eng.logits, ref.logits)
+    assert eng.positions.tolist() == eng.lengths == [n + 6 for n in lengths.tolist()]
+    assert [len(h) for h in eng.held] == [-(-n // page) for n in eng.lengths]
+    _no_error()
+
+
+@pytest.mark.gpu
+def test_prefill_fills_the_pages_with_the_ragged_caches_rows(cuda):
+    """Keys and values of a prompt against RaggedEngine's prefill of it: within the roundings of the layers below."""
+    from efficientgpt_b200.paged import PagedEngine
+    from efficientgpt_b200.ragged import RaggedEngine
+    model = _model(128)
+    prompts, lengths = _batch(3, 45)
+    eng = PagedEngine(model, 3, 20, 60)
+    eng.prefill(prompts, lengths)
+    ref = RaggedEngine(model, 3, 60)
+    ref.prefill(prompts.cuda(), lengths)
+    for i in range(ref.base.n_layers):
+        for r in range(3):
+            n = int(lengths[r])
+            for dst, src in zip(ref.kv[i], _rows(eng, r, i)):
+                want = dst[r * ref.base.nkv:(r + 1) * ref.base.nkv, :n].double()
+                assert (src.double() - want).norm() <= LOGIT_TOL * want.norm()
+    _no_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('kv_dtype', [torch.bfloat16, torch.int8])
+def test_graph_equals_eager_and_gives_what_token_logprobs_gives(cuda, kv_dtype):
+    """Tokens and log probabilities of the captured step, request after request, against eager steps; every value against
+    log_softmax of the eager engine's logits in 64 bits (V = 512: an error below 2^-18, see test_logprobs_gpu)."""
+    from efficientgpt_b200.paged import PagedEngine, PagedGraphDecoder
+    model = _model(128)
+    batch, count, top = 5, 24, 3
+    dec = PagedGraphDecoder(model, batch, 40, 48, page_size=8, kv_dtype=kv_dtype, top_logprobs=top)
+    for seed in (0, 1):
+        prompts, lengths = _batch(batch, 20, seed)
+        tokens, lp, ent, ids, tlp = dec.generate(prompts.cuda(), lengths.cuda(), count)
+        assert tokens.shape == lp.shape == ent.shape == (batch, count) and ids.shape == tlp.shape == (batch, count, top)
+        eng = PagedEngine(model, batch, 40, 48, page_size=8, kv_dtype=kv_dtype, top_logprobs=top)
+        eng.prefill(prompts, lengths)
+        for t in range(count):
+            for got, want in ((tokens, eng.tokens), (lp, eng.logprob), (ent, eng.entropy), (ids, eng.top_ids),
+                              (tlp, eng.top_logprob)):
+                assert torch.equal(got[:, t], want), t
+            assert torch.equal(ids[:, t, 0], tokens[:, t]) and torch.equal(tlp[:, t, 0], lp[:, t])
+            if t:
+                exact = torch.log_softmax(eng.logits.double(), -1)
+                assert (lp[:, t] - exact.gather(1, tokens[:, t:t + 1]).squeeze(1)).abs().max() <= 2.0 ** -18 * 8
+                assert (ent[:, t] + (exact.exp() * exact).sum(-1)).abs().max() <= 2.0 ** -18 * 8
+            if t + 1 < count:
+                eng.step()
+    assert torch.equal(PagedGraphDecoder(model, batch, 40, 48, page_size=8, kv_dtype=kv_dtype).generate(
+        prompts.cuda(), lengths.cuda(), count), tokens)
+    _no_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('kv_dtype', [torch.bfloat16, torch.int8])
+def test_sequences_come_and_go(cuda, kv_dtype):
+    """Rows that join and leave between steps, on pages that others left: every step's logits as those of the sequence alone."""
+    from efficientgpt_b200.paged import PagedEngine
+    model = _model(128)
+    eng = PagedEngine(model, 4, 14, 80, page_size=8, kv_dtype=kv_dtype)
+    alone = {}
+
+    def follow(row):
+        solo, last = alone[row]
+        solo.tokens.copy_(last)
+        solo.step()
+        _close(eng.logits[row:row + 1], solo.logits)
+        alone[row] = (solo, eng.tokens[row:row + 1].clone())
+
+    def join(n, seed):
+        row = eng.add(_ids(n, seed))
+        solo = PagedEngine(model, 1, 14, 80, page_size=8, kv_dtype=kv_dtype)
+        solo.add(_ids(n, seed))
+        alone[row] = (solo, eng.tokens[row:row + 1].clone())
+        return row
+
+    def steps(n):
+        for _ in range(n):
+            eng.step()
+            for row in alone:
+                follow(row)
+
+    a, b = join(30, 1), join(3, 2)
+    steps(7)
+    c = join(17, 3)
+    steps(3)
+    eng.release(a)
+    del alone[a]
+    steps(2)
+    d = join(33, 4)  # on the first one's row and pages
+    assert d == a
+    steps(6)
+    for row in (b, c, d):
+        eng.release(row)
+    assert eng.pool.free == 14 and eng.positions.tolist() == [-1] * 4 and (eng.table == -1).all()
+    eng.step()  # nothing to do: idle rows alone
+    assert eng.positions.tolist() == [-1] * 4
+    _no_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('d', [32, 128])
+@pytest.mark.parametrize('kv_dtype', [torch.bfloat16, torch.int8])
+def test_a_conversation_goes_on_where_it_was(cuda, d, kv_dtype):
+    """extend() behind the cached tokens against one prompt of all of them."""
+    from efficientgpt_b200.paged import PagedEngine
+    model = _model(d)
+    eng = PagedEngine(model, 2, 40, 96, page_size=8, kv_dtype=kv_dtype)
+    other = eng.add(_ids(9, 8))
+    row = eng.add(_ids(21, 5))
+    said = _ids(21, 5).tolist()
+    for _ in range(4):
+        said.append(int(eng.tokens[row]))
+        eng.step()
+    said.append(int(eng.tokens[row]))
+    eng.extend(row, _ids(19, 6))
+    said += _ids(19, 6).tolist()
+    whole = PagedEngine(model, 1, 40, 96, page_size=8, kv_dtype=kv_dtype)
+    whole.add(torch.tensor(said))
+    assert eng.lengths[row] == whole.lengths[0] == len(said)
+    eng.tokens[row] = whole.tokens[0]
+    eng.step()
+    whole.step()
+    _close(eng.logits[row:row + 1], whole.logits)
+    assert eng.lengths[other] == 14
+    _no_error()
+
+
+@pytest.mark.gpu
+def test_scores_of_a_text(cuda):
+    """score(): each token's log probability under the step that generates it, for a text that the engine wrote itself."""
+    from efficientgpt_b200.paged import PagedEngine
+    model = _model(128)
+    eng = PagedEngine(model, 2, 30, 90, page_size=8, top_logprobs=2)
+    row = eng.add(_ids(12, 9))
+    text, lps = _ids(12, 9).tolist(), []
+    for _ in range(30):
+        text.append(int(eng.tokens[row]))
+        lps.append(float(eng.logprob[row]))
+        eng.step()
+    free = eng.pool.free
+    lp, ent, ids, tlp = eng.score(torch.tensor(text), top=2, rows_at_once=16)
+    assert eng.pool.free == free and lp.shape == ent.shape == (41,) and ids.shape == tlp.shape == (41, 2)
+    # logits within 2^-6 of their norm differ by at most that norm a logit; both log probabilities move by no more
+    size = float(eng.logits[row].double().norm()) * LOGIT_TOL
+    assert (lp[11:].cpu().double() - torch.tensor(lps)).abs().max() <= 2 * size
+    assert (lp <= 0).all() and (tlp[:, 0] >= lp).all() and (ent >= 0).all()
+    only = eng.score(torch.tensor(text))
+    assert torch.equal(only[0], lp) and only[2] is None
+    _no_error()
+
+
+@pytest.mark.gpu
+def test_refusals_leave_the_engine_as_it_was(cuda):
+    from efficientgpt_b200.paged import PagedEngine, PagedGraphDecoder
+    model = _model(32)
+    eng = PagedEngine(model, 2, 6, 40, page_size=8)
+    row = eng.add(_ids(20, 1))
+    logits = None
+    for call, error in ((lambda: eng.add(_ids(33, 2)), RuntimeError), (lambda: eng.add(_ids(41, 2)), ValueError),
+                        (lambda: eng.add_all([_ids(1, 2), _ids(2, 2)]), RuntimeError), (lambda: eng.add(_ids(0, 2)), ValueError),
+                        (lambda: eng.extend(row, _ids(30, 2)), ValueError), (lambda: eng.extend(1, _ids(3, 2)), ValueError),
+                        (lambda: eng.score(_ids(1, 2)), ValueError), (lambda: eng.score(_ids(30, 2)), RuntimeError)):
+        with pytest.raises(error):
+            call()
+        assert eng.pool.free == 3 and eng.lengths == [20, 0] and len(eng.held[0]) == 3 and not eng.held[1]
+        assert (eng.table >= 0).sum() == 3
+    for _ in range(20):
+        eng.step()
+        logits = eng.logits[row].clone()
+    assert torch.isfinite(logits.float()).all() and eng.lengths[row] == 40
+    with pytest.raises(ValueError, match='capacity'):
+        eng.step()
+    eng.release(row)
+    eng.add_all([_ids(8, 3), _ids(33, 4)])  # one and five pages: all six
+    with pytest.raises(RuntimeError, match='free'):
+        eng.step()
+    for kw in (dict(page_size=12), dict(capacity=0), dict(top_logprobs=33), dict(pages=0)):
+        with pytest.raises(ValueError):
+            PagedEngine(model, 2, **{**dict(pages=6, capacity=40), **kw})
+    dec = PagedGraphDecoder(model, 2, 4, 40, page_size=8)
+    with pytest.raises(RuntimeError, match='free'):
+        dec.generate(torch.zeros(2, 20, dtype=torch.long).cuda(), torch.tensor([20, 20]).cuda(), 4)
+    assert dec.generate(torch.zeros(2, 8, dtype=torch.long).cuda(), torch.tensor([8, 3]).cuda(), 4).shape == (2, 4)
+    _no_error()
