@@ -216,6 +216,7 @@ struct Smem {
   float m, log_s;
   uint32_t keys[1];  // the row's groups (where no other CTA has some), then the elements of the selected ones
 };
+static_assert(sizeof(Smem) + 4 * (kMaxVocab / 128 + 1) <= 48 * 1024, "no opt-in: the most groups, 128 fp32 logits each");
 __device__ __forceinline__ bool before(uint2 a, uint2 b) { return a.x > b.x || (a.x == b.x && a.y > b.y); }
 
 // The `top` first of the keys get(0 .. n - 1) (value, ~index: all different), in order, into sm.best (value 0: fewer than top), n <=

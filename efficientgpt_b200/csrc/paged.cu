@@ -291,8 +291,8 @@ static int pool_of(const char *what, Pool &p, const void *k, const float *ks, co
   if (d != 32 && d != 64 && d != 128) return set_error(EGPT_ERR_SHAPE, "%s: head_dim must be 32, 64 or 128", what);
   if (page_size < 1 || page_size > 1024 || (page_size & (page_size - 1)))
     return set_error(EGPT_ERR_SHAPE, "%s: the rows of a page must be a power of two up to 1024", what);
-  if (pages < 1 || pages > 0x7fffffff || nkv < 1 || nkv > 4096 || seqs < 1 || seqs > (1 << 20) || columns < 1 || ldt < columns ||
-      columns > (1 << 27) / page_size)
+  if (pages < 1 || pages > 0x7fffffff || nkv < 1 || nkv > 4096 || seqs < 1 || seqs > (1 << 30) / nkv || columns < 1 ||
+      ldt < columns || columns > (1 << 27) / page_size)
     return set_error(EGPT_ERR_SHAPE, "%s: bad pages, heads, sequences or table", what);
   if ((uintptr_t)k % 16 || (uintptr_t)v % 16 || (uintptr_t)ks % 4 || (uintptr_t)vs % 4 || (uintptr_t)table % 4)
     return set_error(EGPT_ERR_ALIGN, "%s: pages must be 16-byte aligned", what);

@@ -549,7 +549,8 @@ def kv_append_paged(k, v, pages, table, position, *, starts=None, q=None, q_norm
     [sequences + 1]) rows starts[i] .. starts[i + 1] - 1 to the slots from position[i] on; rows outside all sequences are
     left alone. k_norm_w / q_norm_w: RMSNorm of the k / q heads; rope_cos, rope_sin (bf16 or fp32 [rows, d / 2]): rotation to
     position rope_base + slot. With q [M, nq * d] the normed and rotated q is returned (in q_out, which may be q; rows
-    without a slot are zeros). Norm and rotation are fp32 and rounded once, to bf16 or to an int8 pool's codes."""
+    without a slot are zeros). Norm and rotation are fp32 and rounded once, to bf16 or to an int8 pool's codes. Two rows for
+    one slot leave elements of both."""
     (_, nkv, _, d), pool, seqs, device = _pool('kv_append_paged', pages, table)
     rows = k.shape
     m = rows[0]
@@ -557,6 +558,8 @@ def kv_append_paged(k, v, pages, table, position, *, starts=None, q=None, q_norm
     ldv, unit_v = v.stride()
     if k.dtype is not _BF16 or v.dtype is not _BF16 or rows[1] != nkv * d or v.shape != rows or unit_k != 1 or unit_v != 1:
         raise ValueError('kv_append_paged: k and v must be bf16 [M, nkv * d] with unit column stride')
+    if m == 1:  # (one row's stride is anything)
+        ldk = ldv = rows[1]
     _here('kv_append_paged', device, k, v, position, starts, q_norm_w, k_norm_w, rope_cos, rope_sin)
     if position.dtype is not _I64 or position.shape != (seqs,) or not position.is_contiguous():
         raise ValueError('kv_append_paged: position must be a contiguous int64 tensor of one slot a sequence')
@@ -594,7 +597,10 @@ def kv_append_paged(k, v, pages, table, position, *, starts=None, q=None, q_norm
         elif q_out.dtype is not _BF16 or q_out.shape != width or q_out.stride(1) != 1:
             raise ValueError('kv_append_paged: q_out must be bf16 rows of the shape of q')
         _here('kv_append_paged', device, q, q_out)
-        queries = (q_out.data_ptr(), q_out.stride(0), q.data_ptr(), ldq, width[1] // d)
+        ldo = q_out.stride(0)
+        if m == 1:
+            ldq = ldo = width[1]
+        queries = (q_out.data_ptr(), ldo, q.data_ptr(), ldq, width[1] // d)
     elif q_norm_w is not None or q_out is not None:
         raise ValueError('kv_append_paged: q_norm_w and q_out need q')
     rc = L.load().egpt_kv_append_paged(*pool, seqs, k.data_ptr(), ldk, v.data_ptr(), ldv, position.data_ptr(), starts, m, nkv, d,
@@ -653,8 +659,9 @@ def attn_decode_paged(q, pages, table, position, nq, nkv, d, *, scale, ws=None, 
         ws = attn_paged_ws(m, nq, nkv, d, q.device)
     if out.get_device() != device:
         _here('attn_decode_paged', device, out)
-    rc = L.load().egpt_attn_decode_paged(out.data_ptr(), out.stride(0), q.data_ptr(), q.stride(0), *pool, position.data_ptr(), m,
-                                         nq, nkv, d, scale, ws.data_ptr(), ws.numel(), 0, _raw_stream_of(device))
+    ldo, ldq = (out.stride(0), q.stride(0)) if m > 1 else (nq * d, nq * d)
+    rc = L.load().egpt_attn_decode_paged(out.data_ptr(), ldo, q.data_ptr(), ldq, *pool, position.data_ptr(), m, nq, nkv, d,
+                                         scale, ws.data_ptr(), ws.numel(), 0, _raw_stream_of(device))
     if rc:
         L.check(rc, 'attn_decode_paged')
     return out

@@ -257,7 +257,7 @@ EGPT_API int egpt_attn_shared_prefix_on_tcgen05(int64_t m, int nq, int nkv, int 
  * outside all sequences are left alone. With k_norm_w bf16 [d] / q_norm_w the k and q heads are RMS-normed, with
  * rope_cos, rope_sin [rope_rows][d / 2] (rope_dtype bf16 or fp32) rotated (half layout) to position rope_base + slot, in
  * fp32 and rounded once, to bf16 or to a code. q [m][nq d] (nullable) goes to q_out, which may be q; rows without a
- * slot become zeros. Two rows for one slot leave either.
+ * slot become zeros. Two rows for one slot leave elements of both.
  *
  * egpt_kv_read_paged: rows start .. start + count - 1 of every sequence (starts: NULL, or int64 [seqs] on the device in
  * place of start) into k_out and v_out, bf16 or fp32 [seqs nkv][count][d] with out_head_stride elements between the heads;

@@ -62,6 +62,8 @@ def _logprobs(logp=X, entropy=X, ids=X, tlp=X, x=X, ldx=100, dtype=L.EGPT_BF16, 
     (lambda: _append(cos=X, sin=X, dtype=L.EGPT_I8), L.EGPT_ERR_DTYPE),
     (lambda: _append(cos=X, sin=X, base=-1), L.EGPT_ERR_SHAPE),
     (lambda: _append(cos=X, sin=X, rows=4, base=4), L.EGPT_ERR_SHAPE),
+    (lambda: _append(seqs=2 ** 29 + 1, m=2 ** 29 + 1, starts=X), L.EGPT_ERR_SHAPE),  # too many heads of all sequences
+    (lambda: _read(seqs=2 ** 29 + 1), L.EGPT_ERR_SHAPE),
     (lambda: _read(out=None), L.EGPT_ERR_ARG),
     (lambda: _read(kp=8), L.EGPT_ERR_ALIGN),
     (lambda: _read(dtype=L.EGPT_I8), L.EGPT_ERR_DTYPE),

@@ -205,6 +205,24 @@ def test_norm_and_rotation(cuda, q8, angles, d, nq, nkv, norm):
     _no_error()
 
 
+def test_one_row_of_any_stride(cuda):
+    """The row stride of a single row, and of a table with one sequence, is anything."""
+    ops = _ops()
+    gen = _gen(6)
+    nq, nkv, d = 4, 2, 64
+    flat = _randn(gen, (nq + 2 * nkv) * d).bfloat16()
+    q, k, v = (t.as_strided((1, t.numel()), (3, 1)) for t in flat.split((nq * d, nkv * d, nkv * d)))
+    table = torch.tensor([1, 0], dtype=torch.int32, device=cuda).as_strided((1, 2), (1, 1))
+    pos = torch.tensor([17], device=cuda)
+    pool = _pool(gen, 2, nkv, 16, d, False)
+    got = ops.kv_append_paged(k, v, pool, table, pos, q=q)
+    assert torch.equal(got, q) and torch.equal(pool[0][0, :, 1].flatten(), k[0]) and torch.equal(pool[1][0, :, 1].flatten(), v[0])
+    out = torch.empty(nq * d, dtype=torch.bfloat16, device=cuda).as_strided((1, nq * d), (5, 1))
+    ops.attn_decode_paged(q, pool, table, pos, nq, nkv, d, scale=0.2, out=out)
+    keys, values = (_rows_of(t, table, 0, 0, 18) for t in _values(pool))
+    _check_one(out[0], q[0], nq, nkv, d, 0.2, keys, values)
+
+
 def test_rows_of_nan_and_infinity(cuda):
     """bf16 pages hold them; an int8 row that has one gets the scale NaN, and the rows beside it nothing of it."""
     ops = _ops()
