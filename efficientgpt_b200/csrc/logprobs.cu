@@ -21,6 +21,8 @@ constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kMaxTop = 32;
 constexpr int kMaxVocab = 1 << 20;
 constexpr int kResident = 4;      // CTAs of an SM
+constexpr int kAtOnce = 4, kRing = 2;  // groups that a warp loads at once, and how many times that is on its way
+constexpr int kRingBytes = kRing * kAtOnce * 512 * kWarps;
 constexpr int kSplitRows = 4096;  // arrival counters: more than the CTAs of a GPU
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr uint32_t kNegInf = 0x007fffffu, kInf = 0xff800000u;  // keys of the infinities; above kInf NaN, below kNegInf nothing
@@ -216,7 +218,9 @@ struct Smem {
   float m, log_s;
   uint32_t keys[1];  // the row's groups (where no other CTA has some), then the elements of the selected ones
 };
-static_assert(sizeof(Smem) + 4 * (kMaxVocab / 128 + 1) <= 48 * 1024, "no opt-in: the most groups, 128 fp32 logits each");
+constexpr int kMostGroups = kMaxVocab / 128 + 1;  // of fp32 logits, in a row off the 16-byte grid
+constexpr size_t kMostSmem = kRingBytes + sizeof(Smem) + 4 * kMostGroups;
+static_assert(kMostGroups >= kMaxTop * 256 && kMostGroups <= kKeysEach * kThreads && kMostSmem <= 100 * 1024, "sizes");
 __device__ __forceinline__ bool before(uint2 a, uint2 b) { return a.x > b.x || (a.x == b.x && a.y > b.y); }
 
 // The `top` first of the keys get(0 .. n - 1) (value, ~index: all different), in order, into sm.best (value 0: fewer than top), n <=
@@ -282,9 +286,9 @@ __device__ __forceinline__ void select(Smem &sm, int n, int top, F get) {
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads, kResident) logprobs_kernel(const Params p) {
-  constexpr int E = Row<T>::E, U = 4;
-  extern __shared__ __align__(16) uint8_t smem_raw[];
-  Smem &sm = *(Smem *)smem_raw;
+  constexpr int E = Row<T>::E, U = kAtOnce;
+  extern __shared__ __align__(16) uint8_t smem_raw[];  // the warps' rings, then Smem
+  Smem &sm = *(Smem *)(smem_raw + kRingBytes);
   pdl_wait();
   pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, cut = (int)blockIdx.x - p.whole;
@@ -309,12 +313,7 @@ __global__ void __launch_bounds__(kThreads, kResident) logprobs_kernel(const Par
   const int whole0 = max(g0, r.off ? 1 : 0), whole1 = min(g1, (r.v + r.off) / (32 * E));
   Sums a = {-INFINITY, 0.f, 0.f};
   uint64_t s2 = 0u, w2 = 0u;
-  auto load = [&](int g, auto &c) {  // of groups g, g + kWarps, ...
-    const uint4 *src = (const uint4 *)(r.x - r.off) + g * 32 + lane;
-#pragma unroll
-    for (int u = 0; u < (int)(sizeof(c) / sizeof(c[0])); ++u) c[u] = __ldg(src + u * kWarps * 32);
-  };
-  auto add = [&](int g, const auto &c) {
+  auto add = [&](int g, const auto &c) {  // groups g, g + kWarps, ...
     constexpr int N = (int)(sizeof(c) / sizeof(c[0]));
     uint32_t most = 0u;
 #pragma unroll
@@ -340,21 +339,34 @@ __global__ void __launch_bounds__(kThreads, kResident) logprobs_kernel(const Par
   };
   int g = whole0 + warp;
   constexpr int kStep = U * kWarps, kSpan = kStep - kWarps;
-  if (g + kSpan < whole1) {  // the next ones on their way while these are added
-    uint4 c[U], next[U];
-    load(g, c);
-    for (; g + kStep + kSpan < whole1; g += kStep) {
-      load(g + kStep, next);
-      add(g, c);
+  if (g + kSpan < whole1) {  // the next ones on their way while these are added (in shared memory: registers are full)
+    uint4 *mine = (uint4 *)smem_raw + warp * (kRing * U * 32) + lane;  // a lane reads what it has copied itself
+    int fetch = g;
+    auto copy = [&](int slot) {
+      if (fetch + kSpan < whole1)
 #pragma unroll
-      for (int u = 0; u < U; ++u) c[u] = next[u];
+        for (int u = 0; u < U; ++u)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(mine + (slot * U + u) * 32)),
+                       "l"((const uint4 *)(r.x - r.off) + (fetch + u * kWarps) * 32 + lane)
+                       : "memory");
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      fetch += kStep;
+    };
+#pragma unroll
+    for (int i = 0; i < kRing; ++i) copy(i);
+    for (int slot = 0; g + kSpan < whole1; g += kStep) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 1) : "memory");
+      uint4 c[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) c[u] = mine[(slot * U + u) * 32];
+      copy(slot);
+      slot = slot + 1 == kRing ? 0 : slot + 1;
+      add(g, c);
     }
-    add(g, c);
-    g += kStep;
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
   }
   for (; g < whole1; g += kWarps) {
-    uint4 c[1];
-    load(g, c);
+    const uint4 c[1] = {__ldg((const uint4 *)(r.x - r.off) + g * 32 + lane)};
     add(g, c);
   }
   const float2 s = halves(s2), w = halves(w2);
@@ -502,8 +514,16 @@ extern "C" int egpt_token_logprobs(float *logp, float *entropy, int64_t *top_ids
   p.cnt = (unsigned *)ws, p.parts = (float4 *)((char *)ws + lgp::kSplitRows * sizeof(unsigned));
   p.keys = (uint32_t *)(p.parts + (m - p.whole) * p.splits), p.key_stride = (lgp::most_groups(v, f32) + 3) / 4 * 4;
   const int words = std::max(lgp::most_groups(v, f32), top * lgp::group_elems(f32));
-  const size_t smem = sizeof(lgp::Smem) + (top ? words * sizeof(uint32_t) : 0);
+  const size_t smem = lgp::kRingBytes + sizeof(lgp::Smem) + (top ? words * sizeof(uint32_t) : 0);
   const void *fn = f32 ? (const void *)lgp::logprobs_kernel<float> : (const void *)lgp::logprobs_kernel<uint16_t>;
+  static int configured[2][64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !configured[f32][dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)lgp::kMostSmem);
+    if (e != cudaSuccess) return check_launch(e, "token_logprobs_kernel");
+    if (dev >= 0 && dev < 64) configured[f32][dev] = 1;
+  }
   return check_launch(launch_kernel(fn, dim3((unsigned)(p.whole + (m - p.whole) * p.splits)), dim3(lgp::kThreads), smem, (cudaStream_t)stream,
                                     (flags & EGPT_FLAG_PDL) != 0, p),
                       "token_logprobs_kernel");
