@@ -486,18 +486,24 @@ def attn_shared_prefix(q, prefix, tails, position, prefix_len, nq, nkv, d, *, sc
 # ---- KV cache in pages: a pool of pages, named by a table, for sequences that come and go ----
 
 
+# Every tensor of a call has to be on the current device, whose stream the call goes to. (The checks stand in line: a call of
+# these has up to fourteen tensors, and a loop over them costs as much as all else.)
+_I32 = torch.int32
+_ELSEWHERE = '%s: CUDA tensors on the current device expected (there is no CPU path)'
+
+
 def _here(what, device, *ts):
-    """Refuses tensors on another device than `device`, the current one, whose stream the call goes to."""
+    """Refuses tensors on another device than `device`, which is the current one."""
     for t in ts:
         if t is not None and t.get_device() != device:
-            raise ValueError(f'{what}: CUDA tensors on the current device expected (there is no CPU path)')
+            raise ValueError(_ELSEWHERE % what)
 
 
 def _device_of(what, t):
     """The device of t, which has to be the current one."""
     device = t.get_device()
     if device < 0 or device != _current_device():
-        raise ValueError(f'{what}: CUDA tensors on the current device expected (there is no CPU path)')
+        raise ValueError(_ELSEWHERE % what)
     return device
 
 
@@ -530,16 +536,27 @@ def _pool(what, pages, table):
     shape = k.shape
     if len(shape) != 4 or v.shape != shape or not (k.is_contiguous() and v.is_contiguous()):
         raise ValueError(f'{what}: contiguous pages [pages, nkv, page_size, d] expected')
-    if table.dtype is not torch.int32 or table.dim() != 2:
+    names = table.shape
+    if table.dtype is not _I32 or len(names) != 2 or not (table.is_contiguous() or table.stride(1) == 1):
         raise ValueError(f'{what}: the table must be int32 [M, columns] with unit column stride')
-    seqs, columns = table.shape
-    ldt, unit = table.stride()
-    if unit != 1 and columns > 1:
-        raise ValueError(f'{what}: the table must be int32 [M, columns] with unit column stride')
-    device = _device_of(what, k)
-    _here(what, device, v, table, ks, vs)
-    return shape, (k.data_ptr(), None if ks is None else ks.data_ptr(), v.data_ptr(), None if vs is None else vs.data_ptr(),
-                   shape[0], shape[2], table.data_ptr(), ldt if seqs > 1 else columns, columns), seqs, device
+    seqs, columns = names
+    device = k.get_device()
+    if device < 0 or device != _current_device() or v.get_device() != device or table.get_device() != device or (
+            ks is not None and (ks.get_device() != device or vs.get_device() != device)):
+        raise ValueError(_ELSEWHERE % what)
+    ldt = columns if table.is_contiguous() else table.stride(0)
+    if ks is None:
+        return shape, (k.data_ptr(), None, v.data_ptr(), None, shape[0], shape[2], table.data_ptr(), ldt, columns), seqs, device
+    return shape, (k.data_ptr(), ks.data_ptr(), v.data_ptr(), vs.data_ptr(), shape[0], shape[2], table.data_ptr(), ldt,
+                   columns), seqs, device
+
+
+def _norm_weight(w, d, device):
+    if w.dtype is not _BF16 or w.numel() != d or not w.is_contiguous():
+        raise ValueError('kv_append_paged: norm weights must be bf16 [d]')
+    if w.get_device() != device:
+        raise ValueError(_ELSEWHERE % 'kv_append_paged')
+    return w.data_ptr()
 
 
 def kv_append_paged(k, v, pages, table, position, *, starts=None, q=None, q_norm_w=None, k_norm_w=None, eps=1e-6,
@@ -560,30 +577,31 @@ def kv_append_paged(k, v, pages, table, position, *, starts=None, q=None, q_norm
         raise ValueError('kv_append_paged: k and v must be bf16 [M, nkv * d] with unit column stride')
     if m == 1:  # (one row's stride is anything)
         ldk = ldv = rows[1]
-    _here('kv_append_paged', device, k, v, position, starts, q_norm_w, k_norm_w, rope_cos, rope_sin)
-    if position.dtype is not _I64 or position.shape != (seqs,) or not position.is_contiguous():
+    if k.get_device() != device or v.get_device() != device or position.get_device() != device:
+        raise ValueError(_ELSEWHERE % 'kv_append_paged')
+    if position.dtype is not _I64 or position.numel() != seqs or not position.is_contiguous():
         raise ValueError('kv_append_paged: position must be a contiguous int64 tensor of one slot a sequence')
     if starts is None:
         if m != seqs:
             raise ValueError('kv_append_paged: without starts there is one row a sequence')
-    elif starts.dtype is not _I64 or starts.shape != (seqs + 1,) or not starts.is_contiguous():
+    elif starts.dtype is not _I64 or starts.numel() != seqs + 1 or not starts.is_contiguous():
         raise ValueError('kv_append_paged: starts must be a contiguous int64 tensor of sequences + 1')
     else:
+        _here('kv_append_paged', device, starts)
         starts = starts.data_ptr()
-    norms = []
-    for w in (q_norm_w, k_norm_w):
-        if w is not None:
-            if w.dtype is not _BF16 or w.numel() != d or not w.is_contiguous():
-                raise ValueError('kv_append_paged: norm weights must be bf16 [d]')
-            w = w.data_ptr()
-        norms.append(w)
+    if q_norm_w is not None:
+        q_norm_w = _norm_weight(q_norm_w, d, device)
+    if k_norm_w is not None:
+        k_norm_w = _norm_weight(k_norm_w, d, device)
     rope = (None, None, 0, 0)
     if rope_cos is not None and rope_sin is not None:
-        length = rope_cos.shape
-        if (len(length) != 2 or length[1] != d // 2 or rope_sin.shape != length or rope_sin.dtype is not rope_cos.dtype
+        length, kind = rope_cos.shape, rope_cos.dtype
+        if (len(length) != 2 or length[1] != d // 2 or rope_sin.shape != length or rope_sin.dtype is not kind
                 or not (rope_cos.is_contiguous() and rope_sin.is_contiguous())):
             raise ValueError('kv_append_paged: RoPE tables must be contiguous [rows, d / 2] of one dtype')
-        rope = (rope_cos.data_ptr(), rope_sin.data_ptr(), _dt(rope_cos), length[0])
+        if rope_cos.get_device() != device or rope_sin.get_device() != device:
+            raise ValueError(_ELSEWHERE % 'kv_append_paged')
+        rope = (rope_cos.data_ptr(), rope_sin.data_ptr(), L.EGPT_BF16 if kind is _BF16 else _dt(rope_cos), length[0])
     elif rope_cos is not rope_sin:
         raise ValueError('kv_append_paged: rope_cos and rope_sin come together')
     queries = (None, 0, None, 0, 0)
@@ -596,15 +614,17 @@ def kv_append_paged(k, v, pages, table, position, *, starts=None, q=None, q_norm
             q_out = torch.empty_like(q)
         elif q_out.dtype is not _BF16 or q_out.shape != width or q_out.stride(1) != 1:
             raise ValueError('kv_append_paged: q_out must be bf16 rows of the shape of q')
-        _here('kv_append_paged', device, q, q_out)
-        ldo = q_out.stride(0)
+        if q.get_device() != device or q_out.get_device() != device:
+            raise ValueError(_ELSEWHERE % 'kv_append_paged')
         if m == 1:
             ldq = ldo = width[1]
+        else:
+            ldo = q_out.stride(0)
         queries = (q_out.data_ptr(), ldo, q.data_ptr(), ldq, width[1] // d)
     elif q_norm_w is not None or q_out is not None:
         raise ValueError('kv_append_paged: q_norm_w and q_out need q')
     rc = L.load().egpt_kv_append_paged(*pool, seqs, k.data_ptr(), ldk, v.data_ptr(), ldv, position.data_ptr(), starts, m, nkv, d,
-                                       *queries, *norms, eps, *rope, rope_base, 0, _raw_stream_of(device))
+                                       *queries, q_norm_w, k_norm_w, eps, *rope, rope_base, 0, _raw_stream_of(device))
     if rc:
         L.check(rc, 'kv_append_paged')
     return q_out
@@ -617,7 +637,8 @@ def kv_read_paged(pages, table, start, count, *, dtype=torch.bfloat16, out=None)
     (_, nkv, _, d), pool, seqs, device = _pool('kv_read_paged', pages, table)
     heads = seqs * nkv
     if out is None:
-        k = pages[0].new_empty((heads, count, d), dtype=dtype)
+        like = pages[0]
+        k = like.new_empty((heads, count, d)) if like.dtype is dtype else like.new_empty((heads, count, d), dtype=dtype)
         v = torch.empty_like(k)
         stride = count * d
     else:
@@ -630,7 +651,7 @@ def kv_read_paged(pages, table, start, count, *, dtype=torch.bfloat16, out=None)
     starts = None
     if isinstance(start, torch.Tensor):
         _here('kv_read_paged', device, start)
-        if start.dtype is not _I64 or start.shape != (seqs,) or not start.is_contiguous():
+        if start.dtype is not _I64 or start.numel() != seqs or not start.is_contiguous():
             raise ValueError('kv_read_paged: start must be an int or a contiguous int64 tensor of one slot a sequence')
         starts, start = start.data_ptr(), 0
     rc = L.load().egpt_kv_read_paged(k.data_ptr(), v.data_ptr(), stride, _dt(k), *pool, seqs, nkv, d, start, starts, count, 0,
@@ -649,16 +670,16 @@ def attn_decode_paged(q, pages, table, position, nq, nkv, d, *, scale, ws=None, 
     """Decode attention over pages: row i of q bf16 [M, nq * d] over the position[i] + 1 keys of sequence i (int64 [M] on the
     device; -1: an idle slot, zeros), whose pages row i of `table` names -> bf16 [M, nq * d]."""
     shape, pool, seqs, device = _pool('attn_decode_paged', pages, table)
-    _here('attn_decode_paged', device, q, position, ws)
     m, out = _attn_rows('attn_decode_paged', q, out, nq, d)
     if shape[1] != nkv or shape[3] != d or seqs != m:
         raise ValueError('attn_decode_paged: pages [pages, nkv, page_size, d] and a table row for each row of q expected')
-    if position.dtype is not _I64 or position.shape != (m,) or not position.is_contiguous():
+    if position.dtype is not _I64 or position.numel() != m or not position.is_contiguous():
         raise ValueError('attn_decode_paged: position must be a contiguous int64 tensor of one slot a sequence')
     if ws is None:
         ws = attn_paged_ws(m, nq, nkv, d, q.device)
-    if out.get_device() != device:
-        _here('attn_decode_paged', device, out)
+    if (q.get_device() != device or position.get_device() != device or ws.get_device() != device
+            or out.get_device() != device):
+        raise ValueError(_ELSEWHERE % 'attn_decode_paged')
     ldo, ldq = (out.stride(0), q.stride(0)) if m > 1 else (nq * d, nq * d)
     rc = L.load().egpt_attn_decode_paged(out.data_ptr(), ldo, q.data_ptr(), ldq, *pool, position.data_ptr(), m, nq, nkv, d,
                                          scale, ws.data_ptr(), ws.numel(), 0, _raw_stream_of(device))
