@@ -70,8 +70,8 @@ __device__ __forceinline__ void widen8(float (&x)[8], uint4 a) {
 }
 
 // A warp takes one row, or every parts-th of its turns: so the row's sequence, slot and page are found once (the starts 32 at a
-// time), the angles are read once, and several heads' loads are on their way under that. In a turn D / 16 lanes hold a head
-// vector of q, k or v: lane l dims 8 l .. 8 l + 7 and the D / 2 further on that the half-layout rotation pairs them
+// time), the angles are read once, and the next turn's loads are on their way under this one's work. A turn takes heads of
+// one kind, q, k or v, D / 16 lanes to a head: lane l dims 8 l .. 8 l + 7 and the D / 2 further on that the half-layout rotation pairs them
 // with, so a vector is read once in 16-byte pieces, the rotation stays inside a lane, and the norm and the quantiser's
 // maximum take a few shuffles. Norm and rotation are fp32 and rounded once, to bf16 or to a code.
 template <int D, bool Q8>
@@ -83,20 +83,24 @@ __global__ void __launch_bounds__(kThreads, 4) append_kernel(const AppendParams 
   const unsigned unit = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
   const int row = (int)(unit / (unsigned)p.parts), part = (int)(unit - (unsigned)row * p.parts);
   if (row >= p.m) return;
-  const int vectors = p.nq + 2 * p.pool.nkv;
-  auto source = [&](int vec) {
-    const uint16_t *x = vec < p.nq ? p.q + row * p.ldq + (int64_t)vec * D
-                                   : (vec < p.nq + p.pool.nkv ? p.k + row * p.ldk + (int64_t)(vec - p.nq) * D
-                                                              : p.v + row * p.ldv + (int64_t)(vec - p.nq - p.pool.nkv) * D);
-    return x + e0;
+  const int q_turns = (p.nq + kGroups - 1) / kGroups, kv_turns = (p.pool.nkv + kGroups - 1) / kGroups;
+  const int turns = q_turns + 2 * kv_turns;
+  const uint16_t *q_row = p.q + row * p.ldq + e0, *k_row = p.k + row * p.ldk + e0, *v_row = p.v + row * p.ldv + e0;
+  // a turn's head of q (kind 0), k or v for this group, and whether there is one
+  auto head_of = [&](int turn, int &kind) {
+    kind = (turn >= q_turns) + (turn >= q_turns + kv_turns);
+    const int head = (turn - (kind ? q_turns : 0) - (kind == 2 ? kv_turns : 0)) * kGroups + group;
+    return head < (kind ? p.pool.nkv : p.nq) ? head : -1;
   };
-  auto load = [&](uint4 (&x)[2], int vec) {
-    if (vec < vectors) x[0] = *(const uint4 *)source(vec), x[1] = *(const uint4 *)(source(vec) + kHalf);
+  auto load = [&](uint4 (&x)[2], int turn) {
+    int kind;
+    const int head = turn < turns ? head_of(turn, kind) : -1;
+    if (head < 0) return;
+    const uint16_t *src = (kind == 0 ? q_row : (kind == 1 ? k_row : v_row)) + head * D;
+    x[0] = *(const uint4 *)src, x[1] = *(const uint4 *)(src + kHalf);
   };
   uint4 next[2] = {};
-  int vec = part * kGroups + group;
-  const int step = p.parts * kGroups;
-  load(next, vec);
+  load(next, part);
 
   // the row's sequence and slot
   int64_t seq = row, at = 0;
@@ -129,21 +133,21 @@ __global__ void __launch_bounds__(kThreads, 4) append_kernel(const AppendParams 
       load8(s, (const uint16_t *)p.rope_sin + angle);
     }
   }
-  // turns of the warp's first group, which has the most
-  for (int turns = (vectors - part * kGroups + step - 1) / step; turns > 0; --turns, vec += step) {
+  for (int turn = part; turn < turns; turn += p.parts) {
     const uint4 x[2] = {next[0], next[1]};
-    load(next, vec + step);  // on its way under this turn
-    const bool is_q = vec < p.nq, is_k = !is_q && vec < p.nq + p.pool.nkv;
+    load(next, turn + p.parts);  // on its way under this turn
+    int kind;
+    const int head = head_of(turn, kind);
     float lo[8], hi[8];
     widen8(lo, x[0]);
     widen8(hi, x[1]);
-    const uint16_t *norm_w = vec >= vectors ? nullptr : (is_q ? p.q_norm_w : (is_k ? p.k_norm_w : nullptr));
-    float ss = 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) ss = fmaf(lo[e], lo[e], fmaf(hi[e], hi[e], ss));
-#pragma unroll
-    for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    const uint16_t *norm_w = kind == 0 ? p.q_norm_w : (kind == 1 ? p.k_norm_w : nullptr);
     if (norm_w) {
+      float ss = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ss = fmaf(lo[e], lo[e], fmaf(hi[e], hi[e], ss));
+#pragma unroll
+      for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
       const float inv = rsqrtf(ss / (float)D + p.eps);
       float w[8];
       load8(w, norm_w + e0);
@@ -153,7 +157,7 @@ __global__ void __launch_bounds__(kThreads, 4) append_kernel(const AppendParams 
 #pragma unroll
       for (int e = 0; e < 8; ++e) hi[e] = hi[e] * inv * w[e];
     }
-    if ((is_q || is_k) && p.rope_cos && in) {
+    if (kind != 2 && p.rope_cos && in) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float a = lo[e], b = hi[e];
@@ -162,28 +166,28 @@ __global__ void __launch_bounds__(kThreads, 4) append_kernel(const AppendParams 
       }
     }
     uint32_t amax = 0u;
-    if (Q8) {
+    if (Q8 && kind != 0) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) amax = max(amax, max(kvq::magnitude(lo[e]), kvq::magnitude(hi[e])));
 #pragma unroll
       for (int o = kLanes / 2; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
     }
-    if (vec >= vectors) continue;
-    if (is_q) {
+    if (head < 0) continue;
+    if (kind == 0) {
       const uint4 zero = make_uint4(0u, 0u, 0u, 0u);  // a row without a slot has no position to rotate to
-      uint16_t *out = p.q_out + row * p.ldqo + (int64_t)vec * D + e0;
+      uint16_t *out = p.q_out + row * p.ldqo + head * D + e0;
       *(uint4 *)out = in ? bf16x8(lo) : zero;
       *(uint4 *)(out + kHalf) = in ? bf16x8(hi) : zero;
     } else if (dst >= 0) {
-      const int64_t to = dst + ((int64_t)(vec - p.nq - (is_k ? 0 : p.pool.nkv)) << p.pool.shift);
+      const int64_t to = dst + ((int64_t)head << p.pool.shift);
       if (Q8) {
         const float scale = kvq::row_scale(amax);
-        int8_t *codes = (int8_t *)(is_k ? p.pool.k : p.pool.v) + to * D + e0;
+        int8_t *codes = (int8_t *)(kind == 1 ? p.pool.k : p.pool.v) + to * D + e0;
         *(uint2 *)codes = kvq::codes_of(lo, scale);
         *(uint2 *)(codes + kHalf) = kvq::codes_of(hi, scale);
-        if (e0 == 0) (is_k ? p.pool.ks : p.pool.vs)[to] = scale;
+        if (e0 == 0) (kind == 1 ? p.pool.ks : p.pool.vs)[to] = scale;
       } else {
-        uint16_t *out = (uint16_t *)(is_k ? p.pool.k : p.pool.v) + to * D + e0;
+        uint16_t *out = (uint16_t *)(kind == 1 ? p.pool.k : p.pool.v) + to * D + e0;
         *(uint4 *)out = bf16x8(lo);
         *(uint4 *)(out + kHalf) = bf16x8(hi);
       }
@@ -341,7 +345,7 @@ extern "C" int egpt_kv_append_paged(void *k_pages, float *k_scale, void *v_pages
   p.seqs = (int)seqs, p.m = (int)m, p.nq = nq;
   // four turns of a row's heads to a warp (4096 rows of 48 heads 21.8 us, 22.5 with two; with all twelve 21.6, but 3400 rows
   // 31.6 for 26.3), fewer as long as that makes no more than 16 warps an SM
-  const int64_t turns = (vectors * (d / 16) + 31) / 32;
+  const int64_t groups = 512 / d, turns = (nq + groups - 1) / groups + 2 * ((nkv + groups - 1) / groups);
   p.parts = (int)std::max<int64_t>((turns + 3) / 4, std::min<int64_t>(turns, 16 * num_sms() / m));
   p.q_norm_w = (const uint16_t *)q_norm_w, p.k_norm_w = (const uint16_t *)k_norm_w, p.eps = eps;
   p.rope_cos = rope_cos, p.rope_sin = rope_sin, p.rope_f32 = rope_dtype == EGPT_F32;
