@@ -705,11 +705,8 @@ __device__ __forceinline__ void attn_body(const Params &p, int block, int grid) 
               d[2] = __byte_perm(hi01, hi23, 0x5410), d[3] = __byte_perm(hi01, hi23, 0x7632);
               // MMA 0: planes 3 and 2 in rows g and g + 8; MMA 1: planes 1 and 0
               const int c = 2 * (s & 1);
-              if constexpr (FOUR) {
-                qa[s / 2][c] = g < 4 ? d[3] : d[2], qa[s / 2][c + 1] = g < 4 ? d[1] : d[0];
-                continue;
-              }
-              qa[s / 2][c] = d[3], qa[s / 2][c + 1] = d[2], qa[s / 2][4 + c] = d[1], qa[s / 2][4 + c + 1] = d[0];
+              if constexpr (FOUR) qa[s / 2][c] = g < 4 ? d[3] : d[2], qa[s / 2][c + 1] = g < 4 ? d[1] : d[0];
+              else qa[s / 2][c] = d[3], qa[s / 2][c + 1] = d[2], qa[s / 2][4 + c] = d[1], qa[s / 2][4 + c + 1] = d[0];
             } else {
               qa[s][hh] = f16x2(y[0], y[1]), qa[s][hh + 2] = f16x2(y[2], y[3]);
             }
@@ -832,11 +829,11 @@ __device__ __forceinline__ void attn_body(const Params &p, int block, int grid) 
             const uint32_t hi = bf16x2(p0, p1), lo = bf16x2(p0 - bf16_lo(hi), p1 - bf16_hi(hi));
             if constexpr (FOUR) {
               pa[nt / 2][nt % 2] = g < 4 ? hi : lo;
-              continue;
+            } else {
+              pa[nt / 2][2 * (nt % 2) + hh] = hi;
+              if (NR == 16) pb[nt / 2][2 * (nt % 2) + hh] = lo;
+              else pa[nt / 2][2 * (nt % 2) + 1] = lo;
             }
-            pa[nt / 2][2 * (nt % 2) + hh] = hi;
-            if (NR == 16) pb[nt / 2][2 * (nt % 2) + hh] = lo;
-            else pa[nt / 2][2 * (nt % 2) + 1] = lo;
           }
         }
         if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
@@ -881,14 +878,14 @@ __device__ __forceinline__ void attn_body(const Params &p, int block, int grid) 
                                          widen2(pair[1][e], 0x4342)};
                   mma<false>(acc[2 * w + e], a, pa[u][0], pa[u][1]);
                 }
-                continue;
-              }
+              } else {
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const uint32_t select = e & 1 ? 0x4342 : 0x4140;
-                const uint32_t b0 = widen2(pair[0][e / 2], select), b1 = widen2(pair[1][e / 2], select);
-                mma<false>(acc[(4 * w + e) % ND], pa[u], b0, b1);
-                if (NR == 16) mma<false>(acc[(4 * w + e) % ND], pb[u % (NR == 16 ? NT / 2 : 1)], b0, b1);
+                for (int e = 0; e < 4; ++e) {
+                  const uint32_t select = e & 1 ? 0x4342 : 0x4140;
+                  const uint32_t b0 = widen2(pair[0][e / 2], select), b1 = widen2(pair[1][e / 2], select);
+                  mma<false>(acc[(4 * w + e) % ND], pa[u], b0, b1);
+                  if (NR == 16) mma<false>(acc[(4 * w + e) % ND], pb[u % (NR == 16 ? NT / 2 : 1)], b0, b1);
+                }
               }
             } else {
 #pragma unroll
