@@ -82,6 +82,7 @@ SIGNATURES = {
     'egpt_kv_append_paged': (I32, [P, P, P, P, I64, I32, P, I64, I64, I64, P, I64, P, I64, P, P, I64, I32, I32, P, I64, P, I64,
                                    I32, P, P, F32, P, P, I32, I64, I64, U32, P]),
     'egpt_kv_read_paged': (I32, [P, P, I64, I32, P, P, P, P, I64, I32, P, I64, I64, I64, I32, I32, I64, P, I64, U32, P]),
+    'egpt_attn_paged_ws_bytes': (SZ, [I64, I32, I32, I32]),
     'egpt_attn_decode_paged': (I32, [P, I64, P, I64, P, P, P, P, I64, I32, P, I64, I64, P, I64, I32, I32, I32, F32, P, SZ, U32,
                                      P]),
     'egpt_token_logprobs_ws_bytes': (SZ, [I64, I64]),

@@ -107,11 +107,12 @@ struct Seg {
   int len;                // keys
 };
 
-// Shape of a CTA (one per SM) by type and query rows.
-template <bool Q8, int NR>
+// Shape of a CTA by type and query rows. PAGED: over pages, 1 or 2 CTAs to an SM, that many times fewer warps each.
+template <bool Q8, int NR, int PAGED = 0>
 struct Cfg {
   // (up to four rows need fewer registers and take more warps: 64 rows over 3544 int8 keys 104 us with 8, 96 with 12)
-  static constexpr int kWarps = NR == 4 ? 12 : 8;
+  static constexpr int kCtas = PAGED == 2 ? 2 : 1;  // of an SM
+  static constexpr int kWarps = (NR == 4 ? 12 : 8) / kCtas;
   static constexpr int kThreads = 32 * kWarps;
   static constexpr int kTile = Q8 ? 32 : 16;  // keys per warp tile: K and V 4 KB each at d = 128
   static constexpr int kStages = NR == 8 ? 3 : 2;
@@ -121,11 +122,11 @@ struct Cfg {
   // to 288 12.1, 9.8, 9.7)
   static constexpr int kMargin = kMarginKeys / kTile, kPagedExtra = (Q8 ? 768 : 512) / kTile;
 };
-template <int D, bool Q8, int NR>
+template <int D, bool Q8, int NR, int PAGED = 0>
 struct Geo {
   static constexpr int kRowBytes = Q8 ? D : 2 * D;
   static constexpr int kChunks = kRowBytes / 16;
-  static constexpr int kTile = Cfg<Q8, NR>::kTile;
+  static constexpr int kTile = Cfg<Q8, NR, PAGED>::kTile;
   static constexpr int kStageBytes = 2 * kTile * kRowBytes + (Q8 ? 2 * kTile * 4 : 0);
   static constexpr int kRun = (!Q8 && D == 128) ? 8 : D / 8;  // consecutive output dims of one thread
   // chunk permutations of a row so that the fragment reads of 8 lanes hit 8 different 16-byte banks
@@ -215,7 +216,7 @@ __device__ __forceinline__ int ceil_div_small(int a, int b) {
 // failing that, and for more sequences, equal stretches, or whole segments to single warps where that takes less time: a
 // CTA's part of a segment costs about one round of its warps' tiles besides its rounds, a warp's half a tile besides
 // its tiles, and the slowest warp has the longest segments. Every thread of the CTA calls it.
-template <typename C, bool PAGED>
+template <typename C, int PAGED>
 __device__ __forceinline__ Layout make_layout(const Params &p, int grid, int *cum, int *len_of, int *scratch) {
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   Layout l;
@@ -368,10 +369,10 @@ __device__ __forceinline__ float *record(const Params &p, int index) {
   return p.ws + (int64_t)index * kRows * (D + 2);
 }
 
-template <int D, bool Q8, int NR>
+template <int D, bool Q8, int NR, int PAGED = 0>
 struct Smem {
-  static constexpr int kWarps = Cfg<Q8, NR>::kWarps, kPass = NR / 2;
-  uint8_t ring[kWarps][Cfg<Q8, NR>::kStages][Geo<D, Q8, NR>::kStageBytes];
+  static constexpr int kWarps = Cfg<Q8, NR, PAGED>::kWarps, kPass = NR / 2;
+  uint8_t ring[kWarps][Cfg<Q8, NR, PAGED>::kStages][Geo<D, Q8, NR, PAGED>::kStageBytes];
   union {
     float merge[kWarps][kPass][D];  // the warps' accumulators, kPass rows at a time
     float fin[kWarps][D];           // shares of a row's records
@@ -494,11 +495,11 @@ enum Mode { kOwn, kBeside, kPrefix };
 // NR: query rows in use, 8 or 16, or over int8 pages 4. A (CTA, segment) pair leaves its record in slot CTA + segment: both only grow along the
 // list, so slots are the pairs' own and a segment's are consecutive. Alone, a segment that one CTA holds goes
 // straight to the output, and a split one's records are added up by the last of its CTAs to get there.
-template <int D, bool Q8, int NR, Mode MODE, bool PAGED = false>
+template <int D, bool Q8, int NR, Mode MODE, int PAGED = 0>
 __device__ __forceinline__ void attn_body(const Params &p, int block, int grid) {
-  using C = Cfg<Q8, NR>;
-  using G = Geo<D, Q8, NR>;
-  using S = Smem<D, Q8, NR>;
+  using C = Cfg<Q8, NR, PAGED>;
+  using G = Geo<D, Q8, NR, PAGED>;
+  using S = Smem<D, Q8, NR, PAGED>;
   constexpr int kWarps = C::kWarps, STAGES = C::kStages;
   constexpr int TILE = G::kTile, NT = TILE / 8, ND = NR == 4 ? D / 16 : D / 8;
   constexpr bool PREFIX = MODE == kPrefix;
@@ -1060,8 +1061,8 @@ __device__ __forceinline__ void attn_body(const Params &p, int block, int grid) 
 }
 
 // The sequences' own keys, alone or beside attn_prefix_kernel's launch.
-template <int D, bool Q8, int NR, Mode MODE, bool PAGED>
-__global__ void __launch_bounds__(Cfg<Q8, NR>::kThreads, 1) attn_kernel(const Params p) {
+template <int D, bool Q8, int NR, Mode MODE, int PAGED>
+__global__ void __launch_bounds__(Cfg<Q8, NR, PAGED>::kThreads, Cfg<Q8, NR, PAGED>::kCtas) attn_kernel(const Params p) {
   if (MODE == kOwn) pdl_wait();  // (what precedes the prefix's launch is done once that has started)
   pdl_launch_dependents();
   attn_body<D, Q8, NR, MODE, PAGED>(p, (int)blockIdx.x, (int)gridDim.x);
@@ -1123,13 +1124,13 @@ static cudaError_t configure(F *fn, size_t smem, int (&configured)[64]) {
   if (e == cudaSuccess) configured[dev] = 1;
   return e;
 }
-template <int D, bool Q8, int NR, Mode MODE, bool PAGED>
+template <int D, bool Q8, int NR, Mode MODE, int PAGED>
 static cudaError_t launch(const Params &p, int grid, cudaStream_t st, bool pdl) {
   static int configured[64] = {0};
   const auto fn = attn_kernel<D, Q8, NR, MODE, PAGED>;
-  const size_t smem = sizeof(Smem<D, Q8, NR>);
+  const size_t smem = sizeof(Smem<D, Q8, NR, PAGED>);
   if (const cudaError_t e = configure(fn, smem, configured); e != cudaSuccess) return e;
-  return launch_kernel((const void *)fn, dim3(grid), dim3(Cfg<Q8, NR>::kThreads), smem, st, pdl, p);
+  return launch_kernel((const void *)fn, dim3(grid), dim3(Cfg<Q8, NR, PAGED>::kThreads), smem, st, pdl, p);
 }
 template <int D, bool Q8, int NP, int NO>
 static cudaError_t launch_both(const Params &pre, const Params &own, int grid, cudaStream_t st, bool pdl) {
@@ -1146,9 +1147,9 @@ static int max_grid() { return num_sms(); }
 // beside a prefix on less than half of the SMs, those that it leaves free (neither kernel shares an SM).
 template <typename C>
 static int own_grid(const Params &p) {
-  const int free = max_grid() - p.pre.grid;
+  const int all = max_grid() * C::kCtas, free = all - p.pre.grid;
   const int64_t most = ((p.cache.cap + C::kTile - 1) / C::kTile + C::kMinChunk - 1) / C::kMinChunk;
-  return (int)std::min<int64_t>(free >= max_grid() / 2 ? free : max_grid(), most * p.m * p.nkv);
+  return (int)std::min<int64_t>(free >= all / 2 ? free : all, most * p.m * p.nkv);
 }
 // How the prefix's segments are cut: as make_layout does it, on the host.
 template <typename C>
@@ -1168,21 +1169,25 @@ static void cut_prefix(Params &p) {
   }
   c.grid = ceil_div(segs * ceil_div(c.seg_tiles, c.pad) * c.pad, c.chunk);
 }
-template <bool Q8, int NR, Mode MODE, bool PAGED>
+template <bool Q8, int NR, Mode MODE, int PAGED>
 static cudaError_t launch_d(Params &p, int d, cudaStream_t st, bool pdl) {
-  const int grid = own_grid<Cfg<Q8, NR>>(p);
+  const int grid = own_grid<Cfg<Q8, NR, PAGED>>(p);
   p.head_share = grid / p.nkv;
   if (d == 128) return launch<128, Q8, NR, MODE, PAGED>(p, grid, st, pdl);
   if constexpr (MODE == kOwn)  // (attn_prefix_kernel has no head_dim 32)
     if (d == 32) return launch<32, Q8, NR, MODE, PAGED>(p, grid, st, pdl);
   return launch<64, Q8, NR, MODE, PAGED>(p, grid, st, pdl);
 }
-template <Mode MODE, bool PAGED = false>
+template <Mode MODE, int PAGED = 0>
 static cudaError_t launch_any(Params &p, int d, bool q8, cudaStream_t st, bool pdl) {
-  if constexpr (PAGED)
-    if (q8 && p.group <= 4) return launch_d<true, 4, MODE, PAGED>(p, d, st, pdl);
-  if (p.group <= 8) return q8 ? launch_d<true, 8, MODE, PAGED>(p, d, st, pdl) : launch_d<false, 8, MODE, PAGED>(p, d, st, pdl);
-  return q8 ? launch_d<true, 16, MODE, PAGED>(p, d, st, pdl) : launch_d<false, 16, MODE, PAGED>(p, d, st, pdl);
+  if constexpr (PAGED == 2) {  // bf16 alone
+    return p.group <= 8 ? launch_d<false, 8, MODE, 2>(p, d, st, pdl) : launch_d<false, 16, MODE, 2>(p, d, st, pdl);
+  } else {
+    if constexpr (PAGED)
+      if (q8 && p.group <= 4) return launch_d<true, 4, MODE, PAGED>(p, d, st, pdl);
+    if (p.group <= 8) return q8 ? launch_d<true, 8, MODE, PAGED>(p, d, st, pdl) : launch_d<false, 8, MODE, PAGED>(p, d, st, pdl);
+    return q8 ? launch_d<true, 16, MODE, PAGED>(p, d, st, pdl) : launch_d<false, 16, MODE, PAGED>(p, d, st, pdl);
+  }
 }
 template <bool Q8, int NP, int NO>
 static cudaError_t launch_both_d(Params &pre, Params &own, int d, cudaStream_t st, bool pdl) {
@@ -1215,6 +1220,11 @@ static bool prefix_on_tcgen05(int64_t m, int group, int nkv, int64_t keys, int d
 // The workspace: arrival counters, one per CTA (a CTA is the first of at most one split segment) whatever the call's
 // sizes, so that calls of different sizes can share it; the segments' (first record, records) pairs; the records.
 static size_t counter_bytes() { return ((size_t)max_grid() * sizeof(unsigned) + 255) / 256 * 256; }
+// Over pages: counters for twice as many CTAs, and the records.
+static size_t paged_counter_bytes() { return (2 * (size_t)num_sms() * sizeof(unsigned) + 255) / 256 * 256; }
+static size_t paged_ws_bytes(int64_t m, int nkv, int d) {
+  return paged_counter_bytes() + (2 * (size_t)num_sms() + (size_t)m * nkv) * kRows * (d + 2) * sizeof(float);
+}
 static size_t parts_bytes(int64_t m, int nkv) { return ((size_t)m * nkv * sizeof(int2) + 255) / 256 * 256; }
 static void set_workspace(Params &p, void *ws) {
   p.cnt = (unsigned *)ws, p.parts = (int2 *)((char *)ws + counter_bytes());
@@ -1222,7 +1232,7 @@ static void set_workspace(Params &p, void *ws) {
 }
 
 static int check(const char *what, int64_t ldo, int64_t ldq, const void *out, const void *q, int64_t cap, int64_t m,
-                 int nq, int nkv, int d, float scale, const void *ws, size_t ws_bytes) {
+                 int nq, int nkv, int d, float scale, const void *ws, size_t ws_bytes, bool paged = false) {
   if (d != 32 && d != 64 && d != 128) return set_error(EGPT_ERR_SHAPE, "%s: head_dim must be 32, 64 or 128", what);
   if (nq < 1 || nkv < 1 || nq % nkv || nq / nkv > kRows)
     return set_error(EGPT_ERR_SHAPE, "%s: nq must be a multiple of nkv, at most %d to one", what, kRows);
@@ -1233,7 +1243,7 @@ static int check(const char *what, int64_t ldo, int64_t ldq, const void *out, co
   if (!std::isfinite(scale * kLog2e)) return set_error(EGPT_ERR_ARG, "%s: scale log2(e) must be finite", what);
   if ((uintptr_t)out % 16 || (uintptr_t)q % 16 || ldq % 8 || ldo % 8)
     return set_error(EGPT_ERR_ALIGN, "%s: q and out must be 16-byte aligned rows", what);
-  if (!ws || ws_bytes < egpt_attn_q8_ws_bytes(m, nq, nkv, d))
+  if (!ws || ws_bytes < (paged ? egpt_attn_paged_ws_bytes(m, nq, nkv, d) : egpt_attn_q8_ws_bytes(m, nq, nkv, d)))
     return set_error(EGPT_ERR_WORKSPACE, "%s: workspace too small", what);
   if ((uintptr_t)ws % 16) return set_error(EGPT_ERR_ALIGN, "%s: workspace must be 16-byte aligned", what);
   return EGPT_OK;
@@ -1273,6 +1283,11 @@ extern "C" int egpt_attn_decode_q8(void *out, int64_t ldo, const void *q, int64_
                       "attn_decode_q8_kernel");
 }
 
+extern "C" size_t egpt_attn_paged_ws_bytes(int64_t m, int nq, int nkv, int d) {
+  if (m < 1 || nkv < 1 || nq < nkv || d < 1) return 0;
+  return aq8::paged_ws_bytes(m, nkv, d);
+}
+
 extern "C" int egpt_attn_decode_paged(void *out, int64_t ldo, const void *q, int64_t ldq, const void *k_pages,
                                       const float *k_scale, const void *v_pages, const float *v_scale, int64_t pages,
                                       int page_size, const int32_t *table, int64_t ldt, int64_t columns,
@@ -1284,15 +1299,21 @@ extern "C" int egpt_attn_decode_paged(void *out, int64_t ldo, const void *q, int
                             m, nkv, d))
     return rc;
   if (!out || !q || !position) return set_error(EGPT_ERR_ARG, "attn_decode_paged: null pointer");
-  if (int rc = aq8::check("attn_decode_paged", ldo, ldq, out, q, pool.cap, m, nq, nkv, d, scale, ws, ws_bytes)) return rc;
+  if (int rc = aq8::check("attn_decode_paged", ldo, ldq, out, q, pool.cap, m, nq, nkv, d, scale, ws, ws_bytes, true))
+    return rc;
   aq8::Params p{};
   p.out = (uint16_t *)out, p.ldo = ldo, p.q = (const uint16_t *)q, p.ldq = ldq;
   p.cache = {(const uint8_t *)k_pages, (const uint8_t *)v_pages, k_scale, v_scale, pool.cap, table, ldt, pages, pool.shift};
   p.position = position, p.m = (int)m, p.nkv = nkv, p.group = nq / nkv, p.scale_log2 = scale * aq8::kLog2e;
-  aq8::set_workspace(p, ws);
-  return check_launch(
-      aq8::launch_any<aq8::kOwn, true>(p, d, k_scale != nullptr, (cudaStream_t)stream, (flags & EGPT_FLAG_PDL) != 0),
-      "attn_decode_paged_kernel");
+  p.cnt = (unsigned *)ws, p.ws = (float *)((char *)ws + aq8::paged_counter_bytes());
+  // With many segments two CTAs to an SM, so that one's loads go on while the other one's warps meet at a segment's end; with
+  // few of them that only makes more records to add up. bf16, 64 rows of 8 kv heads over 200 to 16000 keys 160 us with
+  // one, 149 with two, 40 over 200 to 9000 84 / 80; 16 over 33 to 288 9.7 / 10.6, one over 32768 29.8 / 31.7. int8 gains
+  // for short segments alone (64 over 100 to 600 30 / 25, but over 200 to 16000 120 / 125) and stays with one.
+  const bool q8 = k_scale != nullptr, pdl = (flags & EGPT_FLAG_PDL) != 0, two = !q8 && m * nkv >= 2 * (int64_t)num_sms();
+  return check_launch(two ? aq8::launch_any<aq8::kOwn, 2>(p, d, q8, (cudaStream_t)stream, pdl)
+                          : aq8::launch_any<aq8::kOwn, 1>(p, d, q8, (cudaStream_t)stream, pdl),
+                      "attn_decode_paged_kernel");
 }
 
 extern "C" int egpt_attn_shared_prefix_on_tcgen05(int64_t m, int nq, int nkv, int d, int64_t prefix_len, float scale,

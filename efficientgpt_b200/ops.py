@@ -662,8 +662,9 @@ def kv_read_paged(pages, table, start, count, *, dtype=torch.bfloat16, out=None)
 
 
 def attn_paged_ws(m, nq, nkv, d, device):
-    """Workspace of attn_decode_paged for m sequences (attn_q8_ws: one per stream, for calls that need no more bytes)."""
-    return attn_q8_ws(m, nq, nkv, d, device)
+    """Workspace of attn_decode_paged for m sequences: one per stream that runs it, for calls of every size that needs no more
+    bytes."""
+    return torch.zeros(int(L.load().egpt_attn_paged_ws_bytes(m, nq, nkv, d)), dtype=torch.uint8, device=device)
 
 
 def attn_decode_paged(q, pages, table, position, nq, nkv, d, *, scale, ws=None, out=None):

@@ -265,7 +265,8 @@ EGPT_API int egpt_attn_shared_prefix_on_tcgen05(int64_t m, int nq, int nkv, int 
  *
  * egpt_attn_decode_paged: softmax(scale q K^T) V of row i of q bf16 [m][nq d] over the position[i] + 1 keys of sequence i
  * (m sequences; -1: an idle slot, zeros), GQA with at most 16 query heads to a kv head. Keys on pages that are -1 or
- * outside the pool count as zeros. Workspace as egpt_attn_decode_q8's (egpt_attn_q8_ws_bytes, zero-filled once). */
+ * outside the pool count as zeros. Workspace: egpt_attn_paged_ws_bytes bytes, 16-byte aligned, zero-filled once; it
+ * serves calls of every size that needs no more, one after the other. */
 EGPT_API int egpt_kv_append_paged(void *k_pages, float *k_scale, void *v_pages, float *v_scale, int64_t pages,
                                   int page_size, const int32_t *table, int64_t ldt, int64_t columns, int64_t seqs,
                                   const void *k, int64_t ldk, const void *v, int64_t ldv, const int64_t *position,
@@ -277,6 +278,7 @@ EGPT_API int egpt_kv_read_paged(void *k_out, void *v_out, int64_t out_head_strid
                                 const float *k_scale, const void *v_pages, const float *v_scale, int64_t pages,
                                 int page_size, const int32_t *table, int64_t ldt, int64_t columns, int64_t seqs, int nkv,
                                 int d, int64_t start, const int64_t *starts, int64_t count, unsigned flags, void *stream);
+EGPT_API size_t egpt_attn_paged_ws_bytes(int64_t m, int nq, int nkv, int d);
 EGPT_API int egpt_attn_decode_paged(void *out, int64_t ldo, const void *q, int64_t ldq, const void *k_pages,
                                     const float *k_scale, const void *v_pages, const float *v_scale, int64_t pages,
                                     int page_size, const int32_t *table, int64_t ldt, int64_t columns,
