@@ -1,8 +1,9 @@
-// Decode attention of a batch over int8 KV caches, and over a prefix that the whole batch shares (int8 or bf16).
+// Decode attention of a batch over int8 KV caches, over a prefix that the whole batch shares and over pages (int8 or bf16).
 //
 //   egpt_attn_decode_q8:      out[i, h] = sum_j w_j V[j] / sum_j w_j,  w_j = 2^(scale log2(e) q[i, h] . K[j]),
 //                             over the L_i = position[i] + 1 keys of sequence i's own cache;
-//   egpt_attn_shared_prefix:  the same over prefix_len keys held once and then sequence i's own L_i keys (its tail).
+//   egpt_attn_shared_prefix:  the same over prefix_len keys held once and then sequence i's own L_i keys (its tail);
+//   egpt_attn_decode_paged:   the same over the L_i keys that sequence i has in the pages of a pool (paged.cu).
 // K[j] = ks_j kq_j and V[j] = vs_j vq_j for int8 codes kq, vq with one scale per row and head (kv_q8.cu). GQA: head h
 // reads kv head h / group. A row without any key, or whose scores are all -inf, gives zeros.
 //
@@ -41,6 +42,19 @@
 // 32 heads over 1 to 8191 keys 24 us; 64 rows over 32 to 512 keys 22 us. Tried: f16 weights (fewer instructions, but weights below 2^-29 of a row's
 // largest vanish), 16 warps with 16-key tiles (one row over 32768 keys 28.4 us for 24.1 then), adding up in every CTA
 // behind a prefix instead of in a launch for it (64 rows over 32768 shared keys 81 us for 66).
+//
+// Over pages (the PAGED instantiations): a warp asks for the names of a tile's pages one tile ahead, a lane to a row, and
+// takes a tile that lies in one page as it takes a contiguous one; a tile of several smaller pages is gathered row by
+// row (int8 tiles of 32 keys from 16-row pages 113 us where 32-row pages take 96). Segments are cut wherever the even
+// shares fall, maxima move for a factor of 2^8 only, int8 keys with up to four query rows have MMAs and twelve warps of
+// their own, and many bf16 segments two CTAs an SM. What bounds it: HBM, once the loops run (bf16 6.3, int8 5.9 TB/s over
+// one long sequence); besides it 5 us of way in and launch, 3.9 us of way out for split segments (fence and arrival 1.3,
+// adding 18 records up 2.6), and 2 to 3 us a segment in between, most of it warps that wait for the others' last tile.
+// Measured, d = 128, 8 kv heads, on the device: 64 rows of 32 heads over 200 to 16000 bf16 keys 151 us (906 MB, 6.0 TB/s),
+// int8 in 32-row pages 120 us (653 MB); one row over 211 / 2048 / 32768 bf16 keys 6.3 / 11.8 / 30 us; 16 rows of 16 heads
+// over 33 to 8191 int8 keys 27 us. Tried: stretches of single warps without any meeting (records of all of them to add
+// up, and registers for it that spill: int8 112 us where whole CTAs take 96), P.V of a tile under the next one's scores
+// (no faster), merges by two warps a row (no faster: the wait for the last tile is what counts).
 #include <cmath>
 
 #include "internal.h"

@@ -3,7 +3,10 @@
 // A pool is `pages` pages of S rows (S a power of two) for every kv head, K and V apart: [page][kv head][S][d], bf16 rows
 // or int8 codes with one fp32 scale a row (kv_q8.cu's quantiser). table[i][c] names the page of slots c S .. c S + S - 1 of
 // sequence i (-1: none). A page's rows of one head lie together, so that attention streams S d elements at a time and
-// a tensor of one page is the contiguous caches' [heads][cap][d] with cap = S.
+// a tensor of one page is the contiguous caches' [heads][cap][d] with cap = S. Single passes: few rows are bound by the launch
+// and the round trips to memory that find their place (one row 2.9 us on the device), prompts by instructions (3370 rows of
+// 48 heads with norm and rotation 21 us, 84 MB, 4.0 TB/s; 310 instructions for 16 elements a lane), reads by HBM (32768 rows of
+// 8 heads 42 us from int8, 203 MB, 4.8 TB/s, 45 us from bf16, 268 MB, 6.0 TB/s).
 #include "internal.h"
 #include "common.cuh"
 

@@ -355,6 +355,15 @@ def test_attention_over_long_and_many_sequences(cuda, q8, lengths, nq, nkv, size
 
 
 @pytest.mark.parametrize('q8', [False, True])
+@pytest.mark.parametrize('d,nq,nkv,size', [(32, 8, 8, 16), (64, 24, 8, 8), (64, 40, 4, 16), (128, 32, 8, 16), (128, 72, 8, 32)])
+def test_attention_of_many_segments(cuda, q8, d, nq, nkv, size):
+    """More (sequence, kv head) pairs than two for every SM: none, one and a thousand keys beside each other."""
+    lengths = [(53 * i * i) % 301 for i in range(90)] + [0, 1, 1100]
+    _check_all(_ops(), _gen(d + nq), lengths, nq, nkv, d, size, q8)
+    _no_error()
+
+
+@pytest.mark.parametrize('q8', [False, True])
 @pytest.mark.parametrize('scale', [0.0, -0.05, 3.0])
 def test_attention_scales(cuda, q8, scale):
     _check_all(_ops(), _gen(8), [600, 5], 8, 2, 128, 16, q8, scale=scale)
