@@ -96,17 +96,22 @@ struct Row {
 struct Sums {
   float m, s, w;  // reference (-inf: none yet), sum of 2^exponent(x, m), the same times its exponent
 };
-// (x - m) log2 e. For m up to 1e4 as x log2 e less m log2 e, rounded: what that is off (4e-4 at most) is the same for all x and
-// cancels in log p and in the entropy; beyond, where it grows and x log2 e can overflow, as the difference times log2 e.
+// (x - m) log2 e. For m up to 1e4 as x log2 e less m log2 e, rounded: what that is off (residual(m), 5e-4 at most) is the same for
+// all x and cancels in log p and in the entropy, or is put back where it meets a sum that does not have it; beyond, where it grows
+// and x log2 e can overflow, as the difference times log2 e.
 __device__ __forceinline__ bool plain_range(float m) { return fabsf(m) <= 1e4f; }
 __device__ __forceinline__ float exponent(float x, float m) {
   return plain_range(m) ? fmaf(x, kLog2e, -__fmul_rn(m, kLog2e)) : (x - m) * kLog2e;
 }
+__device__ __forceinline__ float residual(float m) {  // m log2 e, rounded, less m log2 e
+  return plain_range(m) ? -fmaf(m, kLog2e, -__fmul_rn(m, kLog2e)) : 0.f;
+}
 __device__ __forceinline__ float log_prob(float x, float m, float log_s) {
-  return (plain_range(m) && plain_range(x) ? exponent(x, m) * kLn2 : x - m) - log_s;
+  return plain_range(m) && plain_range(x) ? exponent(x, m) * kLn2 - log_s : x - m - fmaf(residual(m), kLn2, log_s);
 }
 __device__ __forceinline__ void rescale(Sums &a, float m) {  // m >= a.m
-  float t = plain_range(a.m) && plain_range(m) ? __fmul_rn(a.m, kLog2e) - __fmul_rn(m, kLog2e) : (a.m - m) * kLog2e;
+  float t = plain_range(a.m) && plain_range(m) ? __fmul_rn(a.m, kLog2e) - __fmul_rn(m, kLog2e)
+                                               : fmaf(a.m - m, kLog2e, residual(a.m) - residual(m));
   t = fmaxf(t, -1000.f);  // (2^-1000 is 0, and 0 times it too)
   const float f = apf::ex2(t);
   a.w = f * fmaf(t, a.s, a.w), a.s *= f, a.m = m;

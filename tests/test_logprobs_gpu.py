@@ -79,6 +79,8 @@ def _logits(kind, m, v, dtype, seed):
         x = x * torch.finfo(dtype).max / 8
     elif kind == 'large':  # differences that overflow
         x = (x * (torch.finfo(dtype).max / 2)).clamp(-torch.finfo(dtype).max, torch.finfo(dtype).max)
+    elif kind in ('far', 'far below'):  # 1e4 or -1e4, where x log2 e has an error of 5e-4, and both sides of that
+        x = x * 2 + (1e4 if kind == 'far' else -1e4)
     elif kind == 'zeros':  # of both signs: one value
         x = torch.where(x > 0, 0.0, -0.0)
     return x.to(dtype)
@@ -86,7 +88,7 @@ def _logits(kind, m, v, dtype, seed):
 
 @pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize('kind', ['normal', 'peaked', 'flat', 'constant', 'rising', 'falling', 'masked', 'lowest', 'huge', 'large',
-                                  'zeros'])
+                                  'zeros', 'far', 'far below'])
 @pytest.mark.parametrize('m,v,top', [(1, 1, 1), (3, 5, 5), (2, 65, 32), (1, 2049, 1), (7, 50257, 20), (2, 151936, 32),
                                      (300, 1000, 8), (1, 9000, 0)])
 def test_against_64_bits(cuda, dtype, kind, m, v, top):
