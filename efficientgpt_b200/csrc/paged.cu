@@ -209,8 +209,10 @@ struct ReadParams {
 
 // out[i nkv + h][r] = row start_i + r of head h of sequence i: eight elements a thread, of K and of V, so that neighbouring
 // threads write neighbouring 16-byte pieces (with sixteen codes a thread, whose two pieces leave one after the other, 32768
-// rows of 8 heads 44.6 us, now 41.3), ROWS rows' on their way at once (four where that still fills the GPU, one for short
-// stretches).
+// rows of 8 heads 44.6 us, now 41.3), ROWS rows' on their way at once (two where that fills the GPU twice over, one for
+// shorter stretches: 4096 rows 7.4 us, with two 7.9; four and eight leave too few threads to an SM: 41.5 and 51.2 us for
+// the 32768, two 39.7). The stores are marked as passing through, like the loads (without and with: 39.7 and 39.0 us, bf16
+// pages 44.9 and 43.5).
 template <int D, bool Q8, bool F32, int ROWS>
 __global__ void __launch_bounds__(kThreads) read_kernel(const ReadParams p) {
   constexpr int kElems = 8, kLanes = D / kElems, kStep = kThreads / kLanes;
@@ -254,7 +256,7 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const ReadParams p) {
           const int64_t at = (int64_t)h * p.out_head + r * D + e0;
           void *out = kv ? p.v_out : p.k_out;
           if constexpr (!Q8 && !F32) {
-            *(uint4 *)((uint16_t *)out + at) = x[i][kv];
+            __stcs((uint4 *)((uint16_t *)out + at), x[i][kv]);
           } else {
             float y[8];
 #pragma unroll
@@ -265,10 +267,10 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const ReadParams p) {
             }
             if (F32) {
               float4 *dst = (float4 *)((float *)out + at);
-              dst[0] = make_float4(y[0], y[1], y[2], y[3]);
-              dst[1] = make_float4(y[4], y[5], y[6], y[7]);
+              __stcs(dst, make_float4(y[0], y[1], y[2], y[3]));
+              __stcs(dst + 1, make_float4(y[4], y[5], y[6], y[7]));
             } else {
-              *(uint4 *)((uint16_t *)out + at) = bf16x8(y);
+              __stcs((uint4 *)((uint16_t *)out + at), bf16x8(y));
             }
           }
         }
@@ -378,10 +380,10 @@ extern "C" int egpt_kv_read_paged(void *k_out, void *v_out, int64_t out_head_str
   p.k_out = k_out, p.v_out = v_out, p.out_head = out_head_stride, p.start = start, p.count = count, p.starts = starts;
   p.seqs = (int)seqs;
   const int64_t heads = seqs * nkv, lanes = d / 8;
-  const bool four = heads * count * lanes >= (int64_t)num_sms() * 4 * 4 * pgd::kThreads;
-  const int64_t per_cta = (four ? 4 : 1) * pgd::kThreads / lanes;
+  const bool two = heads * count * lanes >= (int64_t)num_sms() * 4 * 4 * pgd::kThreads;
+  const int64_t per_cta = (two ? 2 : 1) * pgd::kThreads / lanes;
   const dim3 grid((unsigned)std::min<int64_t>((count + per_cta - 1) / per_cta, 1 << 16), (unsigned)std::min<int64_t>(heads, 65535));
-  const void *fn = four ? pgd::read_fn<4>(d, q8, f32) : pgd::read_fn<1>(d, q8, f32);
+  const void *fn = two ? pgd::read_fn<2>(d, q8, f32) : pgd::read_fn<1>(d, q8, f32);
   return check_launch(launch_kernel(fn, grid, dim3(pgd::kThreads), 0, (cudaStream_t)stream, (flags & EGPT_FLAG_PDL) != 0, p),
                       "kv_read_paged_kernel");
 }
