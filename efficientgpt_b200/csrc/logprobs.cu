@@ -13,9 +13,9 @@
 // probabilities NaN; a row of -inf alone has log p = -inf and entropy 0.
 //
 // What bounds it: many rows of bf16 the arithmetic (one exponential and 8.5 instructions an element; 1024 rows of 151936
-// 55.6 us without top tokens, 5.6 TB/s, and 63.7 with one: a row's two selections are 2 us each, in which its CTA loads
-// nothing), of fp32 HBM (512 rows 50.8 us, 6.1 TB/s); few rows the chain of round trips (one row 6.4 us without, 9.9 with one
-// and 12.5 with twenty top tokens). Tried: the loads ahead in registers (66.5 us: they leave no more than four CTAs an
+// 54.6 us without top tokens, 5.7 TB/s, and 62.5 with one: a row's two selections are 2 us each, in which its CTA loads
+// nothing), of fp32 HBM (512 rows 50.5 us, 6.2 TB/s); few rows the chain of round trips (one row 5.7 us without, 9.1 with one
+// and 11.8 with twenty top tokens). Tried: the loads ahead in registers (66.5 us: they leave no more than four CTAs an
 // SM either way and cost moves), 128 threads a CTA (65.0, but 96 with twenty top tokens for 77), parts of all rows of a last
 // wave (80).
 #include "internal.h"
@@ -97,8 +97,8 @@ struct Sums {
   float m, s, w;  // reference (-inf: none yet), sum of 2^exponent(x, m), the same times its exponent
 };
 // (x - m) log2 e. For m up to 1e4 as x log2 e less m log2 e, rounded: what that is off (residual(m), 5e-4 at most) is the same for
-// all x and cancels in log p and in the entropy, or is put back where it meets a sum that does not have it; beyond, where it grows
-// and x log2 e can overflow, as the difference times log2 e.
+// all x and cancels in the entropy; log p and a change of m put it back. Beyond, where it grows and x log2 e can overflow, as the
+// difference times log2 e.
 __device__ __forceinline__ bool plain_range(float m) { return fabsf(m) <= 1e4f; }
 __device__ __forceinline__ float exponent(float x, float m) {
   return plain_range(m) ? fmaf(x, kLog2e, -__fmul_rn(m, kLog2e)) : (x - m) * kLog2e;
@@ -107,22 +107,25 @@ __device__ __forceinline__ float residual(float m) {  // m log2 e, rounded, less
   return plain_range(m) ? -fmaf(m, kLog2e, -__fmul_rn(m, kLog2e)) : 0.f;
 }
 __device__ __forceinline__ float log_prob(float x, float m, float log_s) {
-  return plain_range(m) && plain_range(x) ? exponent(x, m) * kLn2 - log_s : x - m - fmaf(residual(m), kLn2, log_s);
+  return x - m - fmaf(residual(m), kLn2, log_s);
+}
+// The exponent that takes sums from one reference to another, from <= to. (2^-1000 is 0, and 0 times it too; of two -inf, whose
+// difference is NaN, the sums are 0.)
+__device__ __forceinline__ float moved(float from, float to) {
+  return fmaxf(fmaf(from - to, kLog2e, residual(from) - residual(to)), -1000.f);
 }
 __device__ __forceinline__ void rescale(Sums &a, float m) {  // m >= a.m
-  float t = plain_range(a.m) && plain_range(m) ? __fmul_rn(a.m, kLog2e) - __fmul_rn(m, kLog2e)
-                                               : fmaf(a.m - m, kLog2e, residual(a.m) - residual(m));
-  t = fmaxf(t, -1000.f);  // (2^-1000 is 0, and 0 times it too)
-  const float f = apf::ex2(t);
+  const float t = moved(a.m, m), f = apf::ex2(t);
   a.w = f * fmaf(t, a.s, a.w), a.s *= f, a.m = m;
 }
-__device__ __forceinline__ void join(Sums &a, Sums b) {
-  const float m = fmaxf(a.m, b.m);
-  if (m == -INFINITY) return;
-  rescale(a, m), rescale(b, m);
-  a.s += b.s, a.w += b.w;
+// The same for (a, b) and (b, a), to the bit. One exponential: with both sums moved to the maximum one row takes 1.9 us longer.
+__device__ __forceinline__ void join(Sums &a, const Sums &b) {
+  const bool less = a.m < b.m;
+  const Sums lo = less ? a : b, hi = less ? b : a;
+  const float t = moved(lo.m, hi.m), f = apf::ex2(t);
+  a.s = fmaf(f, lo.s, hi.s), a.w = fmaf(f, fmaf(t, lo.s, lo.w), hi.w), a.m = hi.m;
 }
-// The sums of N neighbouring lanes in all of them, the lower lane's first.
+// The sums of N neighbouring lanes in all of them.
 template <int N>
 __device__ __forceinline__ void join_lanes(Sums &a) {
 #pragma unroll
@@ -131,10 +134,6 @@ __device__ __forceinline__ void join_lanes(Sums &a) {
     b.m = __shfl_xor_sync(0xffffffffu, a.m, o);
     b.s = __shfl_xor_sync(0xffffffffu, a.s, o);
     b.w = __shfl_xor_sync(0xffffffffu, a.w, o);
-    if (threadIdx.x & o) {
-      const Sums t = a;
-      a = b, b = t;
-    }
     join(a, b);
   }
 }
