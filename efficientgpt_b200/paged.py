@@ -103,16 +103,8 @@ class PagedEngine(RaggedEngine):
         b = self.base
         counts = [p.numel() for p in parts]
         before = [self.lengths[r] for r in rows]
-        held = [len(self.held[r]) for r in rows]
-        try:
-            for r, f, n in zip(rows, before, counts):
-                self.reserve(r, f + n)
-        except (RuntimeError, ValueError):  # what the others of them were given goes back
-            for r, have in zip(rows, held):
-                self.pool.give(self.held[r][have:])
-                self.held[r] = self.held[r][:have]
-                self.table[r, have:] = -1
-            raise
+        for r, f, n in zip(rows, before, counts):
+            self.reserve(r, f + n)
         index = torch.tensor(rows, device=self.device)
         table = self.table[index]
         position = torch.tensor(before, device=self.device)
@@ -150,10 +142,18 @@ class PagedEngine(RaggedEngine):
 
     def _prefill_rows(self, rows, parts):
         b = self.base
-        h, index, last = self._run(rows, parts)
-        logits = _proj(ops.rmsnorm(h[last], b.final_norm, b.eps), b.w_lm, b.s_lm)
-        tokens = ops.argmax_rows(logits)
-        self._answer(logits, tokens, index)
+        before = [(len(self.held[r]), self.lengths[r]) for r in rows]
+        try:
+            h, index, last = self._run(rows, parts)
+            logits = _proj(ops.rmsnorm(h[last], b.final_norm, b.eps), b.w_lm, b.s_lm)
+            tokens = ops.argmax_rows(logits)
+            self._answer(logits, tokens, index)
+        except Exception:  # too few pages, or too little memory for the prompts: the rows are as they were
+            for r, (have, length) in zip(rows, before):
+                self.pool.give(self.held[r][have:])
+                self.held[r], self.lengths[r] = self.held[r][:have], length
+                self.table[r, have:] = -1
+            raise
         self.tokens[index] = tokens
         self.positions[index] = torch.tensor([self.lengths[r] for r in rows], device=self.device)
         self.idle[index] = False

@@ -283,3 +283,32 @@ def test_refusals_leave_the_engine_as_it_was(cuda):
         dec.generate(torch.zeros(2, 20, dtype=torch.long).cuda(), torch.tensor([20, 20]).cuda(), 4)
     assert dec.generate(torch.zeros(2, 8, dtype=torch.long).cuda(), torch.tensor([8, 3]).cuda(), 4).shape == (2, 4)
     _no_error()
+
+
+@pytest.mark.gpu
+def test_prompts_that_fail_on_the_way_give_their_pages_back(cuda, monkeypatch):
+    from efficientgpt_b200 import ops
+    from efficientgpt_b200.paged import PagedEngine
+    model = _model(32)
+    eng = PagedEngine(model, 3, 12, 40, page_size=8)
+    row = eng.add(_ids(20, 1))
+    free, table, token = eng.pool.free, eng.table.clone(), eng.tokens.clone()
+
+    def fail(*args, **kw):
+        raise RuntimeError('out of memory')
+
+    for name in ('kv_read_paged', 'argmax_rows'):  # in a layer; behind all of them
+        with monkeypatch.context() as m:
+            m.setattr(ops, name, fail)
+            for call in (lambda: eng.add(_ids(9, 2)), lambda: eng.extend(row, _ids(9, 2)), lambda: eng.add_all([_ids(9, 2)] * 2)):
+                with pytest.raises(RuntimeError, match='memory'):
+                    call()
+                assert eng.pool.free == free and eng.lengths == [20, 0, 0] and torch.equal(eng.table, table)
+                assert eng.positions.tolist() == [20, -1, -1] and torch.equal(eng.tokens, token)
+    other = PagedEngine(model, 1, 12, 40, page_size=8)
+    other.add(_ids(20, 1))
+    for e in (eng, other):
+        e.extend(0, _ids(9, 2))
+        e.step()
+    _close(eng.logits[:1], other.logits)
+    _no_error()
