@@ -73,8 +73,13 @@ class PagedEngine(RaggedEngine):
         self.q8_ws = ops.attn_paged_ws(self.batch, b.nq, b.nkv, b.d, b.device)
 
     # ---- rows and their pages
+    def _check_row(self, row):
+        if not 0 <= row < self.batch:
+            raise ValueError(f'row {row} of a batch of {self.batch}')
+
     def reserve(self, row, length):
         """Pages for the row's first `length` tokens; all of them or, where the pool has too few, none."""
+        self._check_row(row)
         if length > self.cap:
             raise ValueError(f'{length} tokens exceed the capacity {self.cap}')
         have = len(self.held[row])
@@ -86,6 +91,7 @@ class PagedEngine(RaggedEngine):
 
     def release(self, row):
         """The row's sequence leaves: its pages are free again, the row idle."""
+        self._check_row(row)
         self.pool.give(self.held[row])
         self.held[row], self.lengths[row] = [], 0
         self.table[row] = -1
@@ -183,6 +189,7 @@ class PagedEngine(RaggedEngine):
     @torch.no_grad()
     def extend(self, row, ids):
         """The sequence goes on with `ids` behind its newest token (which is run with them)."""
+        self._check_row(row)
         if not self.held[row]:
             raise ValueError(f'row {row} has no sequence')
         self._prefill_rows([row], [torch.cat([self.tokens[row:row + 1], self._ids(ids)])])
@@ -190,6 +197,8 @@ class PagedEngine(RaggedEngine):
     @torch.no_grad()
     def prefill(self, prompts, lengths):
         """All rows anew: right-padded prompts [batch, Pmax] and their lengths."""
+        if len(prompts) != self.batch or len(lengths) != self.batch:
+            raise ValueError('prefill takes a prompt and its length for every row')
         self.reset()
         self._prefill_rows(list(range(self.batch)), [self._ids(prompts[r, :int(n)]) for r, n in enumerate(lengths)])
 

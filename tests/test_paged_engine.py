@@ -312,3 +312,20 @@ def test_prompts_that_fail_on_the_way_give_their_pages_back(cuda, monkeypatch):
         e.step()
     _close(eng.logits[:1], other.logits)
     _no_error()
+
+
+@pytest.mark.gpu
+def test_rows_outside_the_batch_are_refused(cuda):
+    """-1 among them, which an index of a list or a tensor takes for the last one."""
+    from efficientgpt_b200.paged import PagedEngine
+    eng = PagedEngine(_model(32), 2, 12, 40, page_size=8)
+    eng.add_all([_ids(5, 1), _ids(9, 2)])
+    for row in (-1, 2):
+        for call in (lambda: eng.extend(row, _ids(3, 3)), lambda: eng.release(row), lambda: eng.reserve(row, 20)):
+            with pytest.raises(ValueError, match='batch of 2'):
+                call()
+    for prompts, lengths in ((torch.zeros(1, 4, dtype=torch.long), [4]), (torch.zeros(2, 4, dtype=torch.long), [4]),
+                             (torch.zeros(3, 4, dtype=torch.long), [4, 4, 4])):
+        with pytest.raises(ValueError, match='every row'):
+            eng.prefill(prompts, lengths)
+    assert eng.lengths == [5, 9] and eng.pool.free == 9 and eng.positions.tolist() == [5, 9]
