@@ -703,7 +703,8 @@ def token_logprobs(logits, tokens=None, *, top=0, ws=None, out=None):
     stride): the log probability of tokens[i] (int64 [M]; -1: no token, 0) under softmax(logits[i]), the entropy of that
     in nats, and its `top` (up to 32) most likely tokens in order, of equal ones the lowest id first. fp32 and int64. logprob is
     None without tokens, the last two are without top. -inf logits are masked tokens; a row of nothing else has log
-    probabilities -inf and entropy 0, one with a NaN or +inf has NaN. out: the four tensors to fill (contiguous)."""
+    probabilities -inf and entropy 0, one with a NaN or +inf has NaN. out: the four tensors to fill (contiguous), None
+    for those."""
     device = _device_of('token_logprobs', logits)
     _here('token_logprobs', device, tokens, ws)
     if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
@@ -725,6 +726,8 @@ def token_logprobs(logits, tokens=None, *, top=0, ws=None, out=None):
         for t, dt, shape in ((lp, _F32, (m,)), (ent, _F32, (m,)), (ids, _I64, (m, top)), (tlp, _F32, (m, top))):
             if t is not None and (t.dtype is not dt or t.shape != shape or not t.is_contiguous()):
                 raise ValueError('token_logprobs: out must be fp32 [M], fp32 [M], int64 [M, top] and fp32 [M, top]')
+        if (lp is None) is not (tokens is None) or (not top and (ids is not None or tlp is not None)):
+            raise ValueError('token_logprobs: the first of out goes with tokens, the last two with top (else None)')
     if ws is None:
         ws = token_logprobs_ws(m, v, logits.device)
     rc = L.load().egpt_token_logprobs(

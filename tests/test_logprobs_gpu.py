@@ -174,3 +174,20 @@ def test_one_workspace_for_calls_of_every_size_and_replays(cuda):
         _check(x, tokens, 3, out)
         again = ops.token_logprobs(x, tokens, top=3)
         assert all(torch.equal(a, b) for a, b in zip(out, again))
+
+
+def test_outputs_that_nothing_would_fill_are_refused(cuda):
+    ops = _ops()
+    x = torch.randn(3, 100, device='cuda')
+    tokens = torch.tensor([5, -1, 99], device='cuda')
+    f = lambda *shape: torch.full(shape, 7.0, device='cuda')
+    i = lambda *shape: torch.full(shape, 7, device='cuda')
+    for t, top, out in ((None, 0, (f(3), f(3), None, None)), (tokens, 0, (None, f(3), None, None)),
+                        (tokens, 0, (f(3), f(3), i(3, 0), f(3, 0))), (tokens, 2, (f(3), f(3), i(3, 2), None)),
+                        (tokens, 2, (f(3), f(3), None, f(3, 2))), (tokens, 2, (f(3), None, i(3, 2), f(3, 2)))):
+        with pytest.raises(ValueError, match='token_logprobs'):
+            ops.token_logprobs(x, t, top=top, out=out)
+    want = ops.token_logprobs(x, tokens, top=2)
+    got = ops.token_logprobs(x, tokens, top=2, out=(f(3), f(3), i(3, 2), f(3, 2)))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert torch.equal(ops.token_logprobs(x, out=(None, f(3), None, None))[1], want[1])
