@@ -4,9 +4,10 @@
 // or int8 codes with one fp32 scale a row (kv_q8.cu's quantiser). table[i][c] names the page of slots c S .. c S + S - 1 of
 // sequence i (-1: none). A page's rows of one head lie together, so that attention streams S d elements at a time and
 // a tensor of one page is the contiguous caches' [heads][cap][d] with cap = S. Single passes: few rows are bound by the launch
-// and the round trips to memory that find their place (one row 2.9 us on the device), prompts by instructions (3370 rows of
-// 48 heads with norm and rotation 21 us, 84 MB, 4.0 TB/s; 310 instructions for 16 elements a lane), reads by HBM (32768 rows of
-// 8 heads 42 us from int8, 203 MB, 4.8 TB/s, 45 us from bf16, 268 MB, 6.0 TB/s).
+// and the round trips to memory that find their place (one row 2.5 us on the device), prompts by that and by instructions
+// (3370 rows of 48 heads with norm and rotation 19.4 us, 85 MB, 4.4 TB/s; 235 instructions for 16 elements a lane, without norm
+// and rotation 5.3 TB/s), reads by HBM (32768 rows of 8 heads 39 us from int8, 203 MB, 5.2 TB/s, 43.5 us from bf16, 268 MB,
+// 6.2 TB/s).
 #include "internal.h"
 #include "common.cuh"
 
@@ -14,6 +15,7 @@ namespace egpt {
 namespace pgd {
 
 constexpr int kThreads = 256;
+constexpr int kTurns = 4;  // of a warp at most, each of 32 lanes' heads of a row
 
 struct Pool {
   void *k, *v;
@@ -41,7 +43,6 @@ struct AppendParams {
   int64_t ldq, ldk, ldv, ldqo;
   const int64_t *position, *starts;  // starts null: row i is sequence i's
   int seqs, m, nq;
-  int parts;  // warps that share a row's heads
   const uint16_t *q_norm_w, *k_norm_w;
   float eps;
   const void *rope_cos, *rope_sin;
@@ -49,16 +50,6 @@ struct AppendParams {
   int64_t rope_rows, rope_base;
 };
 
-__device__ __forceinline__ void load8(float (&x)[8], const uint16_t *src) {
-  const uint4 a = *(const uint4 *)src;
-  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-  for (int e = 0; e < 4; ++e) x[2 * e] = bf16_lo(w[e]), x[2 * e + 1] = bf16_hi(w[e]);
-}
-__device__ __forceinline__ void load8(float (&x)[8], const float *src) {
-  const float4 a = ((const float4 *)src)[0], b = ((const float4 *)src)[1];
-  x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-}
 __device__ __forceinline__ uint4 bf16x8(const float (&x)[8]) {
   uint32_t y[4];
 #pragma unroll
@@ -66,44 +57,149 @@ __device__ __forceinline__ uint4 bf16x8(const float (&x)[8]) {
   return make_uint4(y[0], y[1], y[2], y[3]);
 }
 
-__device__ __forceinline__ void widen8(float (&x)[8], uint4 a) {
-  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+// Eight fp32 values in pairs: two operations an instruction.
+struct Eight {
+  uint64_t v[4];
+};
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 halves(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ Eight widen8(uint4 a) {
+  return {{pair(bf16_lo(a.x), bf16_hi(a.x)), pair(bf16_lo(a.y), bf16_hi(a.y)), pair(bf16_lo(a.z), bf16_hi(a.z)),
+           pair(bf16_lo(a.w), bf16_hi(a.w))}};
+}
+__device__ __forceinline__ Eight load8(const void *src, int64_t at, bool f32) {
+  if (!f32) return widen8(*(const uint4 *)((const uint16_t *)src + at));
+  const float4 a = ((const float4 *)((const float *)src + at))[0], b = ((const float4 *)((const float *)src + at))[1];
+  return {{pair(a.x, a.y), pair(a.z, a.w), pair(b.x, b.y), pair(b.z, b.w)}};
+}
+__device__ __forceinline__ void unpack(float (&y)[8], const Eight &x) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) x[2 * e] = bf16_lo(w[e]), x[2 * e + 1] = bf16_hi(w[e]);
+  for (int e = 0; e < 4; ++e) {
+    const float2 h = halves(x.v[e]);
+    y[2 * e] = h.x, y[2 * e + 1] = h.y;
+  }
+}
+
+__device__ __forceinline__ void copy16(void *dst, const void *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+
+// A head of q (KIND 0), k (1) or v (2): norm, rotation by the angles' cosines and sines, and out to `dst` (where `store`).
+template <int D, bool Q8, int KIND>
+__device__ __forceinline__ void append_head(const AppendParams &p, const uint4 (&x)[2], const Eight &cosine, const Eight &sine,
+                                            int e0, bool store, void *dst, float *scale_dst) {
+  constexpr int kLanes = D / 16, kHalf = D / 2;
+  constexpr bool kCodes = Q8 && KIND != 0;
+  const uint16_t *norm_w = KIND == 0 ? p.q_norm_w : (KIND == 1 ? p.k_norm_w : nullptr);
+  const bool turned = KIND != 2 && p.rope_cos;
+  uint4 y0 = x[0], y1 = x[1];
+  if (kCodes || norm_w || turned) {
+    Eight lo = widen8(x[0]), hi = widen8(x[1]);
+    if (norm_w) {
+      uint64_t s2 = 0u;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s2 = fma2(lo.v[e], lo.v[e], fma2(hi.v[e], hi.v[e], s2));
+      const float2 s = halves(s2);
+      float ss = s.x + s.y;
+#pragma unroll
+      for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      const float inv = rsqrtf(ss / (float)D + p.eps);
+      const Eight w0 = widen8(*(const uint4 *)(norm_w + e0)), w1 = widen8(*(const uint4 *)(norm_w + kHalf + e0));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        lo.v[e] = mul2(mul2(lo.v[e], pair(inv, inv)), w0.v[e]);
+        hi.v[e] = mul2(mul2(hi.v[e], pair(inv, inv)), w1.v[e]);
+      }
+    }
+    if (turned) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 a = halves(mul2(lo.v[e], cosine.v[e])), b = halves(hi.v[e]), s = halves(sine.v[e]);
+        hi.v[e] = fma2(lo.v[e], sine.v[e], mul2(hi.v[e], cosine.v[e]));
+        lo.v[e] = pair(fmaf(-b.x, s.x, a.x), fmaf(-b.y, s.y, a.y));
+      }
+    }
+    float l[8], h[8];
+    unpack(l, lo), unpack(h, hi);
+    if (kCodes) {
+      uint32_t amax = 0u;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) amax = max(amax, max(kvq::magnitude(l[e]), kvq::magnitude(h[e])));
+#pragma unroll
+      for (int o = kLanes / 2; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+      if (!store) return;
+      const float scale = kvq::row_scale(amax);
+      *(uint2 *)dst = kvq::codes_of(l, scale);
+      *(uint2 *)((int8_t *)dst + kHalf) = kvq::codes_of(h, scale);
+      if (e0 == 0) *scale_dst = scale;
+      return;
+    }
+    y0 = bf16x8(l), y1 = bf16x8(h);
+  }
+  if (!store) return;
+  *(uint4 *)dst = y0;
+  *(uint4 *)((uint16_t *)dst + kHalf) = y1;
 }
 
 // A warp takes one row, or every parts-th of its turns: so the row's sequence, slot and page are found once (the starts 32 at a
-// time), the angles are read once, and the next turn's loads are on their way under this one's work. A turn takes heads of
-// one kind, q, k or v, D / 16 lanes to a head: lane l dims 8 l .. 8 l + 7 and the D / 2 further on that the half-layout rotation pairs them
-// with, so a vector is read once in 16-byte pieces, the rotation stays inside a lane, and the norm and the quantiser's
-// maximum take a few shuffles. Norm and rotation are fp32 and rounded once, to bf16 or to a code.
+// time), the angles are read once, and all of its heads are on their way to shared memory before that (with one turn ahead in
+// registers 20.1 us for 19.4). A turn takes heads of one kind, q, k or v, D / 16 lanes to a head: lane l dims 8 l .. 8 l + 7
+// and the D / 2 further on that the half-layout rotation pairs them with, so a vector is read once in 16-byte pieces, the
+// rotation stays inside a lane, and the norm and the quantiser's maximum take a few shuffles. Norm and rotation are fp32 and
+// rounded once, to bf16 or to a code. (The norm weights in shared memory as fp32: 21.8 us, for the barrier.)
 template <int D, bool Q8>
 __global__ void __launch_bounds__(kThreads, 4) append_kernel(const AppendParams p) {
-  constexpr int kLanes = D / 16, kHalf = D / 2, kGroups = 32 / kLanes;
+  constexpr int kLanes = D / 16, kHalf = D / 2, kGroups = 32 / kLanes, kBytes = Q8 ? 1 : 2;
   pdl_wait();
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31, group = lane / kLanes, e0 = (lane % kLanes) * 8;
-  const unsigned unit = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
-  const int row = (int)(unit / (unsigned)p.parts), part = (int)(unit - (unsigned)row * p.parts);
+  const int row = (int)blockIdx.x * (kThreads / 32) + (int)(threadIdx.x >> 5), part = (int)blockIdx.y, parts = (int)gridDim.y;
   if (row >= p.m) return;
-  const int q_turns = (p.nq + kGroups - 1) / kGroups, kv_turns = (p.pool.nkv + kGroups - 1) / kGroups;
-  const int turns = q_turns + 2 * kv_turns;
+  const int nq = p.nq, nkv = p.pool.nkv;
+  const int q_turns = (nq + kGroups - 1) / kGroups, kv_turns = (nkv + kGroups - 1) / kGroups, k_end = q_turns + kv_turns;
   const uint16_t *q_row = p.q + row * p.ldq + e0, *k_row = p.k + row * p.ldk + e0, *v_row = p.v + row * p.ldv + e0;
-  // a turn's head of q (kind 0), k or v for this group, and whether there is one
-  auto head_of = [&](int turn, int &kind) {
-    kind = (turn >= q_turns) + (turn >= q_turns + kv_turns);
-    const int head = (turn - (kind ? q_turns : 0) - (kind == 2 ? kv_turns : 0)) * kGroups + group;
-    return head < (kind ? p.pool.nkv : p.nq) ? head : -1;
+  __shared__ uint4 inputs[kThreads / 32][kTurns][2][32];  // a lane reads what it has copied itself
+  uint4 (*mine)[2][32] = inputs[threadIdx.x >> 5];
+  int turn = part;
+#pragma unroll
+  for (int i = 0; i < kTurns; ++i) {
+    const int t = part + i * parts;
+    const uint16_t *src = q_row;
+    int head = t * kGroups + group, heads = nq;
+    if (t >= q_turns) head -= q_turns * kGroups, src = k_row, heads = nkv;
+    if (t >= k_end) head -= kv_turns * kGroups, src = v_row;
+    if (head < heads) {
+      src += head * D;
+      copy16(&mine[i][0][lane], src), copy16(&mine[i][1][lane], src + kHalf);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  int taken = 0;
+  auto take = [&](uint4 (&x)[2]) {  // the next turn's
+    if (taken == 0) asm volatile("cp.async.wait_group %0;" ::"n"(kTurns - 1) : "memory");
+    else if (taken == 1) asm volatile("cp.async.wait_group %0;" ::"n"(kTurns - 2) : "memory");
+    else asm volatile("cp.async.wait_group 0;" ::: "memory");
+    x[0] = mine[taken][0][lane], x[1] = mine[taken][1][lane];
+    ++taken, turn += parts;
   };
-  auto load = [&](uint4 (&x)[2], int turn) {
-    int kind;
-    const int head = turn < turns ? head_of(turn, kind) : -1;
-    if (head < 0) return;
-    const uint16_t *src = (kind == 0 ? q_row : (kind == 1 ? k_row : v_row)) + head * D;
-    x[0] = *(const uint4 *)src, x[1] = *(const uint4 *)(src + kHalf);
-  };
-  uint4 next[2] = {};
-  load(next, part);
 
   // the row's sequence and slot
   int64_t seq = row, at = 0;
@@ -111,90 +207,56 @@ __global__ void __launch_bounds__(kThreads, 4) append_kernel(const AppendParams 
     int n = 0;
     for (int i = 0; i <= p.seqs; i += 32) {
       const int64_t s = i + lane <= p.seqs ? p.starts[i + lane] : INT64_MAX;
-      n += __popc(__ballot_sync(0xffffffffu, s <= (int64_t)row));
+      const int here = __popc(__ballot_sync(0xffffffffu, s <= (int64_t)row));
+      if (here) at = (int64_t)row - __shfl_sync(0xffffffffu, s, here - 1);
+      n += here;
     }
-    if (n == 0 || n > p.seqs) return;  // rows outside every sequence stay as they are
+    if (n == 0 || n > p.seqs) {  // rows outside every sequence stay as they are
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      return;
+    }
     seq = n - 1;
-    at = (int64_t)row - p.starts[seq];
   }
   const int64_t first = p.position[seq];
-  int64_t slot = first + at, dst = -1;
-  const bool in = first >= 0 && first < p.pool.cap && at >= 0 && slot < p.pool.cap && (!p.rope_cos || slot < p.rope_rows - p.rope_base);
-  if (!in && first != -1) set_device_error(EGPT_ERR_SHAPE);  // -1: an idle slot of the batch
-  if (in) {
-    dst = row_of(p.pool, seq, slot);
-    if (dst < 0) set_device_error(EGPT_ERR_SHAPE);
+  const int64_t slot = first + at;
+  const bool in = first >= 0 && first < p.pool.cap && at >= 0 && slot < p.pool.cap &&
+                  (!p.rope_cos || slot < p.rope_rows - p.rope_base);
+  uint16_t *q_out = p.q_out + row * p.ldqo + e0;
+  if (!in) {  // no position to rotate to: q is zeros
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if (first != -1) set_device_error(EGPT_ERR_SHAPE);  // -1: an idle slot of the batch
+    for (; turn < q_turns; turn += parts) {
+      const int head = turn * kGroups + group;
+      if (head >= nq) break;
+      *(uint4 *)(q_out + head * D) = *(uint4 *)(q_out + head * D + kHalf) = make_uint4(0u, 0u, 0u, 0u);
+    }
+    return;
   }
-  float c[8], s[8];
-  if (in && p.rope_cos) {
+  const int64_t dst = row_of(p.pool, seq, slot);
+  if (dst < 0) set_device_error(EGPT_ERR_SHAPE);
+  Eight cosine, sine;
+  if (p.rope_cos) {
     const int64_t angle = (slot + p.rope_base) * kHalf + e0;
-    if (p.rope_f32) {
-      load8(c, (const float *)p.rope_cos + angle);
-      load8(s, (const float *)p.rope_sin + angle);
-    } else {
-      load8(c, (const uint16_t *)p.rope_cos + angle);
-      load8(s, (const uint16_t *)p.rope_sin + angle);
-    }
+    cosine = load8(p.rope_cos, angle, p.rope_f32), sine = load8(p.rope_sin, angle, p.rope_f32);
   }
-  for (int turn = part; turn < turns; turn += p.parts) {
-    const uint4 x[2] = {next[0], next[1]};
-    load(next, turn + p.parts);  // on its way under this turn
-    int kind;
-    const int head = head_of(turn, kind);
-    float lo[8], hi[8];
-    widen8(lo, x[0]);
-    widen8(hi, x[1]);
-    const uint16_t *norm_w = kind == 0 ? p.q_norm_w : (kind == 1 ? p.k_norm_w : nullptr);
-    if (norm_w) {
-      float ss = 0.f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) ss = fmaf(lo[e], lo[e], fmaf(hi[e], hi[e], ss));
-#pragma unroll
-      for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      const float inv = rsqrtf(ss / (float)D + p.eps);
-      float w[8];
-      load8(w, norm_w + e0);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) lo[e] = lo[e] * inv * w[e];
-      load8(w, norm_w + kHalf + e0);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) hi[e] = hi[e] * inv * w[e];
-    }
-    if (kind != 2 && p.rope_cos && in) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float a = lo[e], b = hi[e];
-        lo[e] = a * c[e] - b * s[e];
-        hi[e] = b * c[e] + a * s[e];
-      }
-    }
-    uint32_t amax = 0u;
-    if (Q8 && kind != 0) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) amax = max(amax, max(kvq::magnitude(lo[e]), kvq::magnitude(hi[e])));
-#pragma unroll
-      for (int o = kLanes / 2; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    }
-    if (head < 0) continue;
-    if (kind == 0) {
-      const uint4 zero = make_uint4(0u, 0u, 0u, 0u);  // a row without a slot has no position to rotate to
-      uint16_t *out = p.q_out + row * p.ldqo + head * D + e0;
-      *(uint4 *)out = in ? bf16x8(lo) : zero;
-      *(uint4 *)(out + kHalf) = in ? bf16x8(hi) : zero;
-    } else if (dst >= 0) {
-      const int64_t to = dst + ((int64_t)head << p.pool.shift);
-      if (Q8) {
-        const float scale = kvq::row_scale(amax);
-        int8_t *codes = (int8_t *)(kind == 1 ? p.pool.k : p.pool.v) + to * D + e0;
-        *(uint2 *)codes = kvq::codes_of(lo, scale);
-        *(uint2 *)(codes + kHalf) = kvq::codes_of(hi, scale);
-        if (e0 == 0) (kind == 1 ? p.pool.ks : p.pool.vs)[to] = scale;
-      } else {
-        uint16_t *out = (uint16_t *)(kind == 1 ? p.pool.k : p.pool.v) + to * D + e0;
-        *(uint4 *)out = bf16x8(lo);
-        *(uint4 *)(out + kHalf) = bf16x8(hi);
-      }
-    }
+  uint4 x[2];
+  while (turn < q_turns) {
+    const int head = turn * kGroups + group;
+    take(x);
+    append_head<D, Q8, 0>(p, x, cosine, sine, e0, head < nq, q_out + head * D, nullptr);
+  }
+  uint8_t *k_dst = (uint8_t *)p.pool.k + (dst * D + e0) * kBytes, *v_dst = (uint8_t *)p.pool.v + (dst * D + e0) * kBytes;
+  while (turn < k_end) {
+    const int head = (turn - q_turns) * kGroups + group, skip = head << p.pool.shift;  // rows to the head's
+    take(x);
+    append_head<D, Q8, 1>(p, x, cosine, sine, e0, head < nkv && dst >= 0, k_dst + (int64_t)skip * (D * kBytes),
+                          p.pool.ks + dst + skip);
+  }
+  while (turn < k_end + kv_turns) {
+    const int head = (turn - k_end) * kGroups + group, skip = head << p.pool.shift;
+    take(x);
+    append_head<D, Q8, 2>(p, x, cosine, sine, e0, head < nkv && dst >= 0, v_dst + (int64_t)skip * (D * kBytes),
+                          p.pool.vs + dst + skip);
   }
 }
 
@@ -348,15 +410,15 @@ extern "C" int egpt_kv_append_paged(void *k_pages, float *k_scale, void *v_pages
   p.q = (const uint16_t *)q, p.k = (const uint16_t *)k, p.v = (const uint16_t *)v, p.q_out = (uint16_t *)q_out;
   p.ldq = ldq, p.ldk = ldk, p.ldv = ldv, p.ldqo = ldqo, p.position = position, p.starts = starts;
   p.seqs = (int)seqs, p.m = (int)m, p.nq = nq;
-  // four turns of a row's heads to a warp (4096 rows of 48 heads 21.8 us, 22.5 with two; with all twelve 21.6, but 3400 rows
-  // 31.6 for 26.3), fewer as long as that makes no more than 16 warps an SM
+  // kTurns turns of a row's heads to a warp (4096 rows of 48 heads 22.0 us, 22.2 with three, 22.8 with six; 3370 rows 19.4, 19.1
+  // and 20.3), fewer as long as that makes no more than 16 warps an SM
   const int64_t groups = 512 / d, turns = (nq + groups - 1) / groups + 2 * ((nkv + groups - 1) / groups);
-  p.parts = (int)std::max<int64_t>((turns + 3) / 4, std::min<int64_t>(turns, 16 * num_sms() / m));
+  const int64_t parts = std::max<int64_t>((turns + pgd::kTurns - 1) / pgd::kTurns, std::min<int64_t>(turns, 16 * num_sms() / m));
   p.q_norm_w = (const uint16_t *)q_norm_w, p.k_norm_w = (const uint16_t *)k_norm_w, p.eps = eps;
   p.rope_cos = rope_cos, p.rope_sin = rope_sin, p.rope_f32 = rope_dtype == EGPT_F32;
   p.rope_rows = rope_rows, p.rope_base = rope_base;
   const void *fn = d == 128 ? pgd::append_fn<128>(k_scale) : (d == 64 ? pgd::append_fn<64>(k_scale) : pgd::append_fn<32>(k_scale));
-  return check_launch(launch_kernel(fn, dim3((unsigned)((m * p.parts + per_cta - 1) / per_cta)), dim3(pgd::kThreads), 0,
+  return check_launch(launch_kernel(fn, dim3((unsigned)((m + per_cta - 1) / per_cta), (unsigned)parts), dim3(pgd::kThreads), 0,
                                     (cudaStream_t)stream, (flags & EGPT_FLAG_PDL) != 0, p),
                       "kv_append_paged_kernel");
 }
