@@ -6,7 +6,7 @@
 // a tensor of one page is the contiguous caches' [heads][cap][d] with cap = S. Single passes: few rows are bound by the launch
 // and the round trips to memory that find their place (one row 2.5 us on the device), prompts by that and by instructions
 // (3370 rows of 48 heads with norm and rotation 19.4 us, 85 MB, 4.4 TB/s; 235 instructions for 16 elements a lane, without norm
-// and rotation 5.3 TB/s), reads by HBM (32768 rows of 8 heads 39 us from int8, 203 MB, 5.2 TB/s, 43.5 us from bf16, 268 MB,
+// and rotation 5.3 TB/s), reads by HBM (32768 rows of 8 heads 36 us from int8, 203 MB, 5.7 TB/s, 43 us from bf16, 268 MB,
 // 6.2 TB/s).
 #include "internal.h"
 #include "common.cuh"
@@ -15,6 +15,7 @@ namespace egpt {
 namespace pgd {
 
 constexpr int kThreads = 256;
+constexpr int kMostSlots = 1 << 27;  // of a table row, and rows of a read
 constexpr int kTurns = 4;  // of a warp at most, each of 32 lanes' heads of a row
 
 struct Pool {
@@ -274,24 +275,25 @@ struct ReadParams {
 // rows of 8 heads 44.6 us, now 41.3), ROWS rows' on their way at once (two where that fills the GPU twice over, one for
 // shorter stretches: 4096 rows 7.4 us, with two 7.9; four and eight leave too few threads to an SM: 41.5 and 51.2 us for
 // the 32768, two 39.7). The stores are marked as passing through, like the loads (without and with: 39.7 and 39.0 us, bf16
-// pages 44.9 and 43.5).
+// pages 44.9 and 43.5). Sequence and head come from the grid and slots are 32 bits (a division and 64-bit slots a row: 39.0 us
+// for 35.8), in 32 registers, so that an SM has all its threads (40 registers and 10% fewer instructions: 38.1).
 template <int D, bool Q8, bool F32, int ROWS>
 __global__ void __launch_bounds__(kThreads) read_kernel(const ReadParams p) {
   constexpr int kElems = 8, kLanes = D / kElems, kStep = kThreads / kLanes;
   pdl_wait();
   pdl_launch_dependents();
-  const int e0 = (int)(threadIdx.x % kLanes) * kElems;
-  for (int h = blockIdx.y; h < p.seqs * p.pool.nkv; h += gridDim.y) {
-    const int seq = h / p.pool.nkv, head = h - seq * p.pool.nkv;
-    const int64_t start = p.starts ? p.starts[seq] : p.start;
-    for (int64_t r0 = (int64_t)blockIdx.x * kStep * ROWS + threadIdx.x / kLanes; r0 < p.count;
-         r0 += (int64_t)gridDim.x * kStep * ROWS) {
+  const int e0 = (int)(threadIdx.x % kLanes) * kElems, head = (int)blockIdx.y, count = (int)p.count;
+  for (int seq = blockIdx.z; seq < p.seqs; seq += gridDim.z) {
+    // rows before slot 0 and behind the last one are zeros (any start further off is as good)
+    const int start = (int)min(max(p.starts ? p.starts[seq] : p.start, (int64_t)-kMostSlots), p.pool.cap);
+    const int64_t out0 = ((int64_t)seq * p.pool.nkv + head) * p.out_head + e0;
+    for (int r0 = (int)blockIdx.x * (kStep * ROWS) + (int)threadIdx.x / kLanes; r0 < count; r0 += (int)gridDim.x * (kStep * ROWS)) {
       uint4 x[ROWS][2];  // (codes: half of it)
       float scale[ROWS][2];
 #pragma unroll
       for (int i = 0; i < ROWS; ++i) {
-        const int64_t r = r0 + i * kStep, slot = start + r;
-        int64_t src = r < p.count && slot >= 0 && slot < p.pool.cap ? row_of(p.pool, seq, slot) : -1;
+        const int r = r0 + i * kStep, slot = start + r;
+        int64_t src = r < count && slot >= 0 && slot < (int)p.pool.cap ? row_of(p.pool, seq, slot) : -1;
         if (src >= 0) src += (int64_t)head << p.pool.shift;
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
@@ -310,12 +312,12 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const ReadParams p) {
       }
 #pragma unroll
       for (int i = 0; i < ROWS; ++i) {
-        const int64_t r = r0 + i * kStep;
-        if (r >= p.count) break;
+        const int r = r0 + i * kStep;
+        if (r >= count) break;
+        const int64_t at = out0 + (int64_t)r * D;
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
           const uint32_t w[4] = {x[i][kv].x, x[i][kv].y, x[i][kv].z, x[i][kv].w};
-          const int64_t at = (int64_t)h * p.out_head + r * D + e0;
           void *out = kv ? p.v_out : p.k_out;
           if constexpr (!Q8 && !F32) {
             __stcs((uint4 *)((uint16_t *)out + at), x[i][kv]);
@@ -363,7 +365,7 @@ static int pool_of(const char *what, Pool &p, const void *k, const float *ks, co
   if (page_size < 1 || page_size > 1024 || (page_size & (page_size - 1)))
     return set_error(EGPT_ERR_SHAPE, "%s: the rows of a page must be a power of two up to 1024", what);
   if (pages < 1 || pages > 0x7fffffff || nkv < 1 || nkv > 4096 || seqs < 1 || seqs > (1 << 30) / nkv || columns < 1 ||
-      ldt < columns || columns > (1 << 27) / page_size)
+      ldt < columns || columns > kMostSlots / page_size)
     return set_error(EGPT_ERR_SHAPE, "%s: bad pages, heads, sequences or table", what);
   if ((uintptr_t)k % 16 || (uintptr_t)v % 16 || (uintptr_t)ks % 4 || (uintptr_t)vs % 4 || (uintptr_t)table % 4)
     return set_error(EGPT_ERR_ALIGN, "%s: pages must be 16-byte aligned", what);
@@ -434,17 +436,18 @@ extern "C" int egpt_kv_read_paged(void *k_out, void *v_out, int64_t out_head_str
     return rc;
   if (!k_out || !v_out) return set_error(EGPT_ERR_ARG, "kv_read_paged: null pointer");
   if (dtype != EGPT_BF16 && dtype != EGPT_F32) return set_error(EGPT_ERR_DTYPE, "kv_read_paged: the output is bf16 or fp32");
-  if (count < 1 || count > (1 << 27) || out_head_stride < count * d || (!starts && (start < 0 || start > p.pool.cap - count)))
+  if (count < 1 || count > pgd::kMostSlots || out_head_stride < count * d || (!starts && (start < 0 || start > p.pool.cap - count)))
     return set_error(EGPT_ERR_SHAPE, "kv_read_paged: rows [start, start + count) outside the table, or bad output stride");
   const bool f32 = dtype == EGPT_F32, q8 = k_scale != nullptr;
   if ((uintptr_t)k_out % 16 || (uintptr_t)v_out % 16 || (out_head_stride * (f32 ? 4 : 2)) % 16)
     return set_error(EGPT_ERR_ALIGN, "kv_read_paged: outputs must be 16-byte aligned");
   p.k_out = k_out, p.v_out = v_out, p.out_head = out_head_stride, p.start = start, p.count = count, p.starts = starts;
   p.seqs = (int)seqs;
-  const int64_t heads = seqs * nkv, lanes = d / 8;
-  const bool two = heads * count * lanes >= (int64_t)num_sms() * 4 * 4 * pgd::kThreads;
+  const int64_t lanes = d / 8;
+  const bool two = seqs * nkv * count * lanes >= (int64_t)num_sms() * 4 * 4 * pgd::kThreads;
   const int64_t per_cta = (two ? 2 : 1) * pgd::kThreads / lanes;
-  const dim3 grid((unsigned)std::min<int64_t>((count + per_cta - 1) / per_cta, 1 << 16), (unsigned)std::min<int64_t>(heads, 65535));
+  const dim3 grid((unsigned)std::min<int64_t>((count + per_cta - 1) / per_cta, 1 << 16), (unsigned)nkv,
+                  (unsigned)std::min<int64_t>(seqs, 65535));
   const void *fn = two ? pgd::read_fn<2>(d, q8, f32) : pgd::read_fn<1>(d, q8, f32);
   return check_launch(launch_kernel(fn, grid, dim3(pgd::kThreads), 0, (cudaStream_t)stream, (flags & EGPT_FLAG_PDL) != 0, p),
                       "kv_read_paged_kernel");

@@ -479,3 +479,26 @@ def test_one_workspace_for_calls_of_every_size_and_replays(cuda):
                 _check_one(out[i], q[i], 32, 8, 128, 0.1, k, v)
         _check_all(ops, gen, [700, 80], 32, 8, 128, 16, False, ws=ws)
     _no_error()
+
+
+@pytest.mark.parametrize('q8', [False, True])
+def test_reads_of_many_sequences_and_from_any_start(cuda, q8):
+    """More sequences than a grid's third dimension has places; starts as far off as their type goes read as zeros."""
+    ops = _ops()
+    gen = _gen(4)
+    m, size, pages, columns, count = 66000, 2, 5, 3, 3
+    pool = _pool(gen, pages, 1, size, 32, q8)
+    table = torch.randint(0, pages, (m, columns), generator=gen, device=cuda, dtype=torch.int32)
+    start = torch.randint(-4, columns * size + 3, (m,), generator=gen, device=cuda)
+    far = torch.tensor([-2 ** 63, 2 ** 63 - 1, -2 ** 31 - 1, 2 ** 31, 2 ** 32, -2 ** 32, 2 ** 27, -2 ** 27], device=cuda)
+    start[100:108], start[-8:] = far, far
+    values = [t.float() for t in _values([t.float() if t.dtype != torch.int8 else t for t in pool])]
+    got = ops.kv_read_paged(pool, table, start, count)
+    slots = start.clamp(-8, columns * size)[:, None] + torch.arange(count, device=cuda)
+    inside = (slots >= 0) & (slots < columns * size)
+    at = slots.clamp(0, columns * size - 1)
+    page = table.gather(1, at // size).long()
+    for x, y in zip(values, got):
+        want = torch.where(inside[..., None], x[page, 0, at % size], torch.zeros((), device=cuda))
+        assert torch.equal(y, want.bfloat16())
+    _no_error()
