@@ -46,7 +46,7 @@
 // Over pages (the PAGED instantiations): a warp asks for the names of a tile's pages one tile ahead, a lane to a row, and
 // takes a tile that lies in one page as it takes a contiguous one; a tile of several smaller pages is gathered row by
 // row (int8 tiles of 32 keys from 16-row pages 113 us where 32-row pages take 96). Segments are cut wherever the even
-// shares fall, maxima move for a factor of 2^8 only, int8 keys with up to four query rows have MMAs and twelve warps of
+// shares fall, int8 keys with up to four query rows have MMAs and twelve warps of
 // their own, and many bf16 segments two CTAs an SM. What bounds it: HBM, once the loops run (bf16 6.3, int8 5.9 TB/s over
 // one long sequence); besides it 5 us of way in and launch, 3.9 us of way out for split segments (fence and arrival 1.3,
 // adding 18 records up 2.6), and 2 to 3 us a segment in between, most of it warps that wait for the others' last tile.
@@ -825,8 +825,7 @@ __device__ __forceinline__ void attn_body(const Params &p, int block, int grid) 
           for (int nt = 0; nt < NT; ++nt) mx = fmaxf(mx, fmaxf(sc[nt][2 * hh], sc[nt][2 * hh + 1]));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-          // (over pages the maximum in use moves only for one 2^8 larger: weights up to that and few rescaled sums)
-          const float m_new = PAGED && mx <= m_run[hh] + 8.f ? m_run[hh] : fmaxf(m_run[hh], mx);
+          const float m_new = fmaxf(m_run[hh], mx);
           ms[hh] = m_new == -INFINITY ? 0.f : m_new;
           alpha[hh] = ex2(m_run[hh] - ms[hh]);
           m_run[hh] = m_new;

@@ -502,3 +502,36 @@ def test_reads_of_many_sequences_and_from_any_start(cuda, q8):
         want = torch.where(inside[..., None], x[page, 0, at % size], torch.zeros((), device=cuda))
         assert torch.equal(y, want.bfloat16())
     _no_error()
+
+
+@pytest.mark.parametrize('q8', [False, True])
+@pytest.mark.parametrize('group', [1, 8, 16])
+@pytest.mark.parametrize('m', [1, 3])
+def test_attend_values_near_the_types_largest_behind_a_rising_maximum(cuda, m, group, q8):
+    """Values of 2^120 to 2^121 under weights that grow by 2^7.5 along the sequence: the weighted mean is finite, and so is
+    every sum of the values under weights up to 1 (11 of them: below 2^125)."""
+    import math
+    ops = _ops()
+    n, d, page, nkv = 400, 128, 32, 2
+    nq, columns = nkv * group, -(-n // page)
+    shape = (m * columns, nkv, page, d)
+    table = torch.arange(m * columns, device=cuda, dtype=torch.int32).view(m, columns)
+    score = torch.full((columns * page,), -300.0, device=cuda)
+    score[:8] = 0.0
+    score[[128, 256, 384]] = 7.5  # in the second, third and fourth tiles of the warp that has the first, by the shape of a CTA
+    k = torch.zeros(shape, device=cuda)
+    k.view(m, columns, nkv, page, d)[..., 0] = score.view(columns, 1, page)
+    v = (0.5 + 0.5 * torch.rand(shape, device=cuda, generator=_gen(group))) * 2.0 ** 121
+    pool = [k.bfloat16(), v.bfloat16()]
+    kd, vd = (t.double() for t in pool)
+    if q8:
+        pool = [t for x in (k, v) for t in _quantised(x)]
+        kd, vd = (pool[i].double() * pool[i + 1].double()[..., None] for i in (0, 2))
+    q = torch.zeros(m, nq, d, dtype=torch.bfloat16, device=cuda)
+    q[..., 0] = 1
+    got = ops.attn_decode_paged(q.view(m, -1), pool, table, torch.full((m,), n - 1, device=cuda), nq, nkv, d, scale=math.log(2))
+    kd, vd = (t.view(m, columns, nkv, page, d).transpose(1, 2).reshape(m, nkv, columns * page, d)[:, :, :n] for t in (kd, vd))
+    w = torch.softmax(math.log(2) * kd[..., 0], -1)
+    want = (w[..., None] * vd).sum(2).repeat_interleave(group, 1).reshape(m, -1)
+    assert ((got.double() - want).abs() <= (2.0 ** -8 + U) * want).all()
+    _no_error()
