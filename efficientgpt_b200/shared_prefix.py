@@ -99,6 +99,9 @@ class SharedPrefixEngine(RaggedEngine):
         self.tokens.copy_(ops.argmax_rows(_proj(x, b.w_lm, b.s_lm)))
         self.positions.copy_(torch.tensor(lens, device=self.device))
 
+    def prefill_row(self, row, ids):
+        raise NotImplementedError('prefill_row: the rows behind a prefix are prefilled together, by prefill')
+
     def _attend_step(self, i, lay, qkv):
         b = self.base
         q, k, v = self._split(qkv)

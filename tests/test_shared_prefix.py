@@ -205,3 +205,18 @@ def test_long_prefix_on_the_tcgen05_kernel_decodes_as_the_joined_sequences(cuda,
     joined.positions.copy_(shared.positions + prefix)
     _follow(shared, joined, 6)
     assert L.device_error() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('kv_dtype', [torch.bfloat16, torch.int8])
+def test_a_row_alone_is_not_prefilled(cuda, kv_dtype):
+    """The ragged engine's way would leave the prefix out (tokens of another text); a refusal leaves everything as it was."""
+    from efficientgpt_b200.shared_prefix import SharedPrefixEngine
+    eng = SharedPrefixEngine(_model(32), 2, 20, 20, kv_dtype=kv_dtype)
+    prompts, lengths = _batch(2, 5)
+    eng.set_prefix(prompts[0].cuda())
+    eng.prefill(prompts.cuda(), lengths)
+    tokens, positions = eng.tokens.clone(), eng.positions.clone()
+    with pytest.raises(NotImplementedError, match='prefill_row'):
+        eng.prefill_row(0, prompts[0].cuda())
+    assert torch.equal(eng.tokens, tokens) and torch.equal(eng.positions, positions)
