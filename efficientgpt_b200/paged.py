@@ -194,13 +194,28 @@ class PagedEngine(RaggedEngine):
             raise ValueError(f'row {row} has no sequence')
         self._prefill_rows([row], [torch.cat([self.tokens[row:row + 1], self._ids(ids)])])
 
+    def _check_anew(self, lengths, counts):
+        """Whether sequences with prompts of `lengths` tokens, that grow to counts tokens, have room in an empty pool."""
+        for n, count in zip(lengths, counts):
+            if n < 1 or count > self.cap:
+                raise ValueError(f'a prompt of {n} tokens, a sequence of {count}: at least one, and the capacity is {self.cap}')
+        need = sum(-(-n // self.page_size) for n in counts)
+        if need > self.pool.pages:
+            raise RuntimeError(f'{need} pages asked for, {self.pool.pages} of {self.pool.pages} free once every row has left')
+
     @torch.no_grad()
     def prefill(self, prompts, lengths):
-        """All rows anew: right-padded prompts [batch, Pmax] and their lengths."""
-        if len(prompts) != self.batch or len(lengths) != self.batch:
+        """All rows anew: right-padded prompts [batch, Pmax] and their lengths. The sequences that there are leave once
+        the prompts are found to fit."""
+        if prompts.dim() != 2 or len(prompts) != self.batch or len(lengths) != self.batch:
             raise ValueError('prefill takes a prompt and its length for every row')
+        lengths = [int(n) for n in lengths]
+        if max(lengths) > prompts.shape[1]:
+            raise ValueError(f'a length of {max(lengths)} of prompts [{self.batch}, {prompts.shape[1]}]')
+        self._check_anew(lengths, lengths)
+        parts = [self._ids(prompts[r, :n]) for r, n in enumerate(lengths)]
         self.reset()
-        self._prefill_rows(list(range(self.batch)), [self._ids(prompts[r, :int(n)]) for r, n in enumerate(lengths)])
+        self._prefill_rows(list(range(self.batch)), parts)
 
     @torch.no_grad()
     def score(self, ids, top=0, rows_at_once=512):
@@ -276,6 +291,8 @@ class PagedGraphDecoder(RaggedGraphDecoder):
         check_ragged(prompts, lengths, count, eng.cap)
         if prompts.shape[0] != eng.batch:
             raise ValueError('prompts must have the decoder batch size')
+        lengths = lengths.tolist()
+        eng._check_anew(lengths, [n + count - 1 for n in lengths])
         eng.reset()
         if self.graph is None:
             self._capture()

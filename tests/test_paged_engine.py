@@ -329,3 +329,31 @@ def test_rows_outside_the_batch_are_refused(cuda):
         with pytest.raises(ValueError, match='every row'):
             eng.prefill(prompts, lengths)
     assert eng.lengths == [5, 9] and eng.pool.free == 9 and eng.positions.tolist() == [5, 9]
+
+
+@pytest.mark.gpu
+def test_prompts_that_do_not_fit_leave_the_sequences_that_there_are(cuda):
+    """prefill and generate begin all rows anew, but not for prompts that have no place."""
+    from efficientgpt_b200.paged import PagedEngine, PagedGraphDecoder
+    model = _model(32)
+    dec = PagedGraphDecoder(model, 2, 6, 40, page_size=8)
+    long = torch.zeros(2, 41, dtype=torch.long)
+    for eng in (PagedEngine(model, 2, 6, 40, page_size=8), dec.engine):
+        eng.add_all([_ids(5, 1), _ids(9, 2)])
+        tokens, table = eng.tokens.clone(), eng.table.clone()
+        for prompts, lengths, error in ((long[:, :12], [4, 0], ValueError), (long[:, :12], [4, -1], ValueError),
+                                        (long[:, :12], [4, 13], ValueError), (long, [41, 1], ValueError),
+                                        (long[0], [1, 1], ValueError), (long, [33, 9], RuntimeError)):
+            with pytest.raises(error):
+                eng.prefill(prompts, lengths)
+            assert eng.lengths == [5, 9] and eng.pool.free == 3 and eng.positions.tolist() == [5, 9]
+            assert torch.equal(eng.tokens, tokens) and torch.equal(eng.table, table)
+        if eng is dec.engine:
+            with pytest.raises(RuntimeError, match='free'):
+                dec.generate(long[:, :20].cuda(), torch.tensor([20, 20]).cuda(), 6)  # 4 pages each by the last token
+            assert eng.lengths == [5, 9] and torch.equal(eng.tokens, tokens) and torch.equal(eng.table, table)
+        eng.step()
+        assert eng.lengths == [6, 10]
+        eng.prefill(long, [32, 16])  # all pages, those of the sequences among them
+        assert eng.lengths == [32, 16] and eng.pool.free == 0
+    _no_error()
