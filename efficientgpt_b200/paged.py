@@ -194,14 +194,14 @@ class PagedEngine(RaggedEngine):
             raise ValueError(f'row {row} has no sequence')
         self._prefill_rows([row], [torch.cat([self.tokens[row:row + 1], self._ids(ids)])])
 
-    def _check_anew(self, lengths, counts):
-        """Whether sequences with prompts of `lengths` tokens, that grow to counts tokens, have room in an empty pool."""
+    def _check_anew(self, lengths, counts, free):
+        """Whether sequences with prompts of `lengths` tokens, that grow to counts tokens, have room in `free` pages."""
         for n, count in zip(lengths, counts):
             if n < 1 or count > self.cap:
                 raise ValueError(f'a prompt of {n} tokens, a sequence of {count}: at least one, and the capacity is {self.cap}')
         need = sum(-(-n // self.page_size) for n in counts)
-        if need > self.pool.pages:
-            raise RuntimeError(f'{need} pages asked for, {self.pool.pages} of {self.pool.pages} free once every row has left')
+        if need > free:
+            raise RuntimeError(f'{need} pages asked for, {free} of {self.pool.pages} free once the rows have left')
 
     @torch.no_grad()
     def prefill(self, prompts, lengths):
@@ -212,10 +212,19 @@ class PagedEngine(RaggedEngine):
         lengths = [int(n) for n in lengths]
         if max(lengths) > prompts.shape[1]:
             raise ValueError(f'a length of {max(lengths)} of prompts [{self.batch}, {prompts.shape[1]}]')
-        self._check_anew(lengths, lengths)
+        self._check_anew(lengths, lengths, self.pool.pages)
         parts = [self._ids(prompts[r, :n]) for r, n in enumerate(lengths)]
         self.reset()
         self._prefill_rows(list(range(self.batch)), parts)
+
+    @torch.no_grad()
+    def prefill_row(self, row, ids):
+        """One row anew with the prompt `ids` (int64 [p]). A sequence that it has leaves once the prompt is found to fit."""
+        self._check_row(row)
+        ids = self._ids(ids)
+        self._check_anew([ids.numel()], [ids.numel()], self.pool.free + len(self.held[row]))
+        self.release(row)
+        self._prefill_rows([row], [ids])
 
     @torch.no_grad()
     def score(self, ids, top=0, rows_at_once=512):
@@ -292,7 +301,7 @@ class PagedGraphDecoder(RaggedGraphDecoder):
         if prompts.shape[0] != eng.batch:
             raise ValueError('prompts must have the decoder batch size')
         lengths = lengths.tolist()
-        eng._check_anew(lengths, [n + count - 1 for n in lengths])
+        eng._check_anew(lengths, [n + count - 1 for n in lengths], eng.pool.pages)
         eng.reset()
         if self.graph is None:
             self._capture()

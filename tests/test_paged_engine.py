@@ -357,3 +357,29 @@ def test_prompts_that_do_not_fit_leave_the_sequences_that_there_are(cuda):
         eng.prefill(long, [32, 16])  # all pages, those of the sequences among them
         assert eng.lengths == [32, 16] and eng.pool.free == 0
     _no_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('kv_dtype', [torch.bfloat16, torch.int8])
+def test_one_row_anew(cuda, kv_dtype):
+    """prefill_row, which the ragged engine has too: on a free row, on one with a sequence, and refused as a whole."""
+    from efficientgpt_b200.paged import PagedEngine
+    model = _model(128)
+    eng = PagedEngine(model, 2, 8, 40, page_size=8, kv_dtype=kv_dtype)
+    row = eng.add(_ids(30, 1))
+    eng.prefill_row(1, _ids(11, 2))
+    eng.prefill_row(row, _ids(33, 3))  # five pages, of which four were the row's own
+    assert eng.lengths == [33, 11] and eng.positions.tolist() == [33, 11] and eng.pool.free == 1
+    want = PagedEngine(model, 2, 8, 40, page_size=8, kv_dtype=kv_dtype)
+    want.add_all([_ids(33, 3), _ids(11, 2)])
+    for e in (eng, want):
+        e.tokens.copy_(want.tokens)
+        e.step()
+    _close(eng.logits, want.logits)
+    table = eng.table.clone()
+    for at, ids, error in ((0, _ids(41, 1), ValueError), (1, _ids(25, 1), RuntimeError), (0, _ids(0, 1), ValueError),
+                           (2, _ids(1, 1), ValueError), (-1, _ids(1, 1), ValueError)):
+        with pytest.raises(error):
+            eng.prefill_row(at, ids)
+        assert eng.lengths == [34, 12] and torch.equal(eng.table, table) and eng.positions.tolist() == [34, 12]
+    _no_error()
