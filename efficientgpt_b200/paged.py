@@ -77,9 +77,17 @@ class PagedEngine(RaggedEngine):
         if not 0 <= row < self.batch:
             raise ValueError(f'row {row} of a batch of {self.batch}')
 
-    def reserve(self, row, length):
-        """Pages for the row's first `length` tokens; all of them or, where the pool has too few, none."""
+    def _check_sequence(self, row):
         self._check_row(row)
+        if not self.held[row]:
+            raise ValueError(f'row {row} has no sequence')
+
+    def reserve(self, row, length):
+        """Pages for the first `length` tokens of the row's sequence; all of them or, where the pool has too few, none."""
+        self._check_sequence(row)  # (a row that holds pages is taken for one with a sequence)
+        self._reserve(row, length)
+
+    def _reserve(self, row, length):
         if length > self.cap:
             raise ValueError(f'{length} tokens exceed the capacity {self.cap}')
         have = len(self.held[row])
@@ -110,7 +118,7 @@ class PagedEngine(RaggedEngine):
         counts = [p.numel() for p in parts]
         before = [self.lengths[r] for r in rows]
         for r, f, n in zip(rows, before, counts):
-            self.reserve(r, f + n)
+            self._reserve(r, f + n)
         index = torch.tensor(rows, device=self.device)
         table = self.table[index]
         position = torch.tensor(before, device=self.device)
@@ -189,9 +197,7 @@ class PagedEngine(RaggedEngine):
     @torch.no_grad()
     def extend(self, row, ids):
         """The sequence goes on with `ids` behind its newest token (which is run with them)."""
-        self._check_row(row)
-        if not self.held[row]:
-            raise ValueError(f'row {row} has no sequence')
+        self._check_sequence(row)
         self._prefill_rows([row], [torch.cat([self.tokens[row:row + 1], self._ids(ids)])])
 
     def _check_anew(self, lengths, counts, free):

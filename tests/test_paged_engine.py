@@ -383,3 +383,21 @@ def test_one_row_anew(cuda, kv_dtype):
             eng.prefill_row(at, ids)
         assert eng.lengths == [34, 12] and torch.equal(eng.table, table) and eng.positions.tolist() == [34, 12]
     _no_error()
+
+
+@pytest.mark.gpu
+def test_pages_are_reserved_for_sequences_alone(cuda):
+    """Pages of a row without a sequence made it count as one: steps advanced its length, extend ran on what it had not cached."""
+    from efficientgpt_b200.paged import PagedEngine
+    eng = PagedEngine(_model(32), 2, 6, 40, page_size=8)
+    row = eng.add(_ids(5, 1))
+    with pytest.raises(ValueError, match='no sequence'):
+        eng.reserve(1, 9)
+    eng.reserve(row, 17)
+    assert eng.pool.free == 3 and eng.held[1] == []
+    eng.step()
+    assert eng.lengths == [6, 0] and eng.positions.tolist() == [6, -1]
+    with pytest.raises(ValueError, match='no sequence'):
+        eng.extend(1, _ids(2, 2))
+    assert eng.add(_ids(9, 2)) == 1 and eng.pool.free == 1
+    _no_error()
