@@ -10,6 +10,8 @@ batch's rows to their pages (kv_append_paged: q/k norm and rotation on the way, 
 log probability of every answered token, the distribution's entropy and its most likely tokens come with it
 (token_logprobs); score() gives them for a prompt's own tokens.
 """
+import contextlib
+
 import torch
 
 from . import ops
@@ -93,23 +95,46 @@ class PagedEngine(RaggedEngine):
         have = len(self.held[row])
         need = -(-length // self.page_size)
         if need > have:
-            pages = self.pool.take(need - have)
-            self.table[row, have:need] = torch.tensor(pages, dtype=torch.int32).to(self.device)
-            self.held[row] += pages
+            self.held[row] += self.pool.take(need - have)
+            self.table[row, have:need] = torch.tensor(self.held[row][have:], dtype=torch.int32).to(self.device)
 
     def release(self, row):
         """The row's sequence leaves: its pages are free again, the row idle."""
         self._check_row(row)
-        self.pool.give(self.held[row])
-        self.held[row], self.lengths[row] = [], 0
         self.table[row] = -1
         self.positions[row] = -1
         self.idle[row] = True
+        self._give_back(row, 0, 0)
+
+    def _give_back(self, row, have, length):
+        """The row keeps its first `have` pages and `length` tokens."""
+        pages = self.held[row][have:]
+        self.held[row], self.lengths[row] = self.held[row][:have], length
+        self.pool.give(pages)  # (last: an interrupt may lose pages here, but none is ever free and held)
 
     def reset(self):
         for row in range(self.batch):
             if self.held[row]:
                 self.release(row)
+
+    @contextlib.contextmanager
+    def _all_or_nothing(self):
+        """A change of the batch, whole or, whatever ends it (too few pages, too little memory, an interrupt), not at all: every
+        row's pages, length, newest token and its log probabilities are as they were. (What it cached lies behind the lengths.)"""
+        before = [(len(pages), length) for pages, length in zip(self.held, self.lengths)]
+        state = [self.tokens, self.positions, self.idle]
+        if self.top is not None:
+            state += [self.logprob, self.entropy, self.top_ids, self.top_logprob]
+        saved = [t.clone() for t in state]
+        try:
+            yield
+        except BaseException:
+            for r, (have, length) in enumerate(before):
+                self.table[r, have:] = -1
+                self._give_back(r, have, length)
+            for t, old in zip(state, saved):
+                t.copy_(old)
+            raise
 
     # ---- prompts
     def _run(self, rows, parts):
@@ -156,21 +181,14 @@ class PagedEngine(RaggedEngine):
 
     def _prefill_rows(self, rows, parts):
         b = self.base
-        before = [(len(self.held[r]), self.lengths[r]) for r in rows]
-        try:
+        with self._all_or_nothing():
             h, index, last = self._run(rows, parts)
             logits = _proj(ops.rmsnorm(h[last], b.final_norm, b.eps), b.w_lm, b.s_lm)
             tokens = ops.argmax_rows(logits)
             self._answer(logits, tokens, index)
-        except Exception:  # too few pages, or too little memory for the prompts: the rows are as they were
-            for r, (have, length) in zip(rows, before):
-                self.pool.give(self.held[r][have:])
-                self.held[r], self.lengths[r] = self.held[r][:have], length
-                self.table[r, have:] = -1
-            raise
-        self.tokens[index] = tokens
-        self.positions[index] = torch.tensor([self.lengths[r] for r in rows], device=self.device)
-        self.idle[index] = False
+            self.tokens[index] = tokens
+            self.positions[index] = torch.tensor([self.lengths[r] for r in rows], device=self.device)
+            self.idle[index] = False
 
     def _ids(self, ids):
         ids = ids.reshape(-1).to(device=self.device, dtype=torch.int64)
@@ -270,11 +288,12 @@ class PagedEngine(RaggedEngine):
     def step(self):
         """One token for every row that has a sequence."""
         live = [r for r in range(self.batch) if self.held[r]]
-        for r in live:
-            self.reserve(r, self.lengths[r] + 1)
-        self._step()
-        for r in live:
-            self.lengths[r] += 1
+        with self._all_or_nothing():
+            for r in live:
+                self._reserve(r, self.lengths[r] + 1)
+            self._step()
+            for r in live:
+                self.lengths[r] += 1
 
 
 class PagedGraphDecoder(RaggedGraphDecoder):
@@ -312,16 +331,20 @@ class PagedGraphDecoder(RaggedGraphDecoder):
         if self.graph is None:
             self._capture()
         eng.prefill(prompts, lengths)
-        for r in range(eng.batch):
-            eng.reserve(r, eng.lengths[r] + count - 1)
-        self.col.zero_()
-        self.out[:, 0] = eng.tokens
-        for buf, t in self.kept:
-            buf[0] = t
-        for _ in range(count - 1):
-            self.graph.replay()
-        for r in range(eng.batch):
-            eng.lengths[r] += count - 1
+        try:
+            for r in range(eng.batch):
+                eng.reserve(r, eng.lengths[r] + count - 1)
+            self.col.zero_()
+            self.out[:, 0] = eng.tokens
+            for buf, t in self.kept:
+                buf[0] = t
+            for _ in range(count - 1):
+                self.graph.replay()
+            for r in range(eng.batch):
+                eng.lengths[r] += count - 1
+        except BaseException:  # an interrupt between replays: how many have run is not known
+            eng.reset()
+            raise
         tokens = self.out[:, :count].clone()
         if not self.kept:
             return tokens

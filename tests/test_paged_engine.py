@@ -401,3 +401,65 @@ def test_pages_are_reserved_for_sequences_alone(cuda):
         eng.extend(1, _ids(2, 2))
     assert eng.add(_ids(9, 2)) == 1 and eng.pool.free == 1
     _no_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('error', [RuntimeError, KeyboardInterrupt])
+def test_whatever_ends_a_change_of_the_batch_leaves_it_as_it_was(cuda, monkeypatch, error):
+    """Prompts and steps that end anywhere, an interrupt among the ends: pages, lengths, tokens and log probabilities are those
+    from before, and the sequences go on as if nothing had been."""
+    from efficientgpt_b200 import ops
+    from efficientgpt_b200.paged import PagedEngine
+    model = _model(32)
+    eng, same = (PagedEngine(model, 3, 12, 40, page_size=8, top_logprobs=2) for _ in range(2))
+    for e in (eng, same):
+        e.add(_ids(16, 1))  # two full pages: the next step needs a third
+
+    def state():
+        return [eng.tokens, eng.positions, eng.idle, eng.table, eng.logprob, eng.entropy, eng.top_ids, eng.top_logprob]
+
+    before = [t.clone() for t in state()]
+
+    def fail(*args, **kw):
+        raise error
+
+    calls = [lambda: eng.add(_ids(9, 2)), lambda: eng.extend(0, _ids(9, 2)), eng.step]
+    places = [(ops, 'kv_append_paged'), (ops, 'argmax_rows'), (ops, 'token_logprobs'), (torch, 'tensor')]
+    for where, name in places:  # in a layer; behind all of them; behind the steps' tokens and positions; between a row's pages
+        for call in calls:
+            with monkeypatch.context() as m:
+                m.setattr(where, name, fail)
+                with pytest.raises(error):
+                    call()
+            assert eng.pool.free == 10 and eng.lengths == [16, 0, 0] and [len(h) for h in eng.held] == [2, 0, 0]
+            assert all(torch.equal(a, b) for a, b in zip(state(), before)), (name, call)
+    for _ in range(3):
+        eng.step()
+        same.step()
+        assert torch.equal(eng.tokens[:1], same.tokens[:1]) and torch.equal(eng.logits[:1], same.logits[:1])
+    assert eng.lengths == [19, 0, 0] and sorted(eng.pool._free + eng.held[0]) == list(range(12))
+    _no_error()
+
+
+@pytest.mark.gpu
+def test_an_interrupted_request_leaves_no_sequences(cuda, monkeypatch):
+    from efficientgpt_b200.paged import PagedGraphDecoder
+    dec = PagedGraphDecoder(_model(32), 2, 12, 40, page_size=8)
+    prompts, lengths = torch.zeros(2, 8, dtype=torch.long).cuda(), torch.tensor([8, 3]).cuda()
+    want = dec.generate(prompts, lengths, 6)
+    replay, left = dec.graph.replay, [2]
+
+    class Graph:
+        def replay(self):
+            if not left[0]:
+                raise KeyboardInterrupt
+            left[0] -= 1
+            replay()
+
+    with monkeypatch.context() as m:
+        m.setattr(dec, 'graph', Graph())
+        with pytest.raises(KeyboardInterrupt):
+            dec.generate(prompts, lengths, 6)
+    assert dec.engine.lengths == [0, 0] and dec.engine.pool.free == 12 and dec.engine.positions.tolist() == [-1, -1]
+    assert torch.equal(dec.generate(prompts, lengths, 6), want)
+    _no_error()
