@@ -259,6 +259,8 @@ class PagedEngine(RaggedEngine):
         ids = self._ids(ids)
         if ids.numel() < 2:
             raise ValueError('a text to score has at least two tokens')
+        if not 1 <= rows_at_once <= 65535:
+            raise ValueError('rows_at_once must be in [1, 65535]')
         row = next((r for r in range(self.batch) if not self.held[r]), None)
         if row is None:
             raise RuntimeError('no free row')

@@ -463,3 +463,20 @@ def test_an_interrupted_request_leaves_no_sequences(cuda, monkeypatch):
     assert dec.engine.lengths == [0, 0] and dec.engine.pool.free == 12 and dec.engine.positions.tolist() == [-1, -1]
     assert torch.equal(dec.generate(prompts, lengths, 6), want)
     _no_error()
+
+
+@pytest.mark.gpu
+def test_scores_by_any_number_of_rows_at_once(cuda):
+    """Every row has its score whatever the pieces; no number of rows gave no scores and no error."""
+    from efficientgpt_b200.paged import PagedEngine
+    eng = PagedEngine(_model(32), 1, 5, 40, page_size=8)
+    want = eng.score(_ids(9, 2), top=1)
+    assert all(t.shape[0] == 8 for t in want)
+    for rows in (0, -1, 65536):
+        with pytest.raises(ValueError, match='rows_at_once'):
+            eng.score(_ids(9, 2), rows_at_once=rows)
+    for rows in (3, 65535):
+        got = eng.score(_ids(9, 2), top=1, rows_at_once=rows)
+        assert all(a.shape == b.shape for a, b in zip(got, want)) and torch.equal(got[2], want[2])
+    assert eng.pool.free == 5 and eng.held == [[]]
+    _no_error()
