@@ -86,6 +86,7 @@ SIGNATURES = {
     'egpt_attn_decode_paged': (I32, [P, I64, P, I64, P, P, P, P, I64, I32, P, I64, I64, P, I64, I32, I32, I32, F32, P, SZ, U32,
                                      P]),
     'egpt_token_logprobs_ws_bytes': (SZ, [I64, I64]),
+    'egpt_token_logprobs_max_ws_bytes': (SZ, [I64, I64]),
     'egpt_token_logprobs': (I32, [P, P, P, P, P, I64, I32, I64, I64, P, I32, P, SZ, U32, P]),
     'egpt_argmax_rows': (I32, [P, P, I64, I64, I64, I32, P]),
     'egpt_sample_ws_bytes': (SZ, [I64]),

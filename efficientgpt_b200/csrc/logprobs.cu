@@ -501,6 +501,13 @@ extern "C" size_t egpt_token_logprobs_ws_bytes(int64_t m, int64_t v) {
   return std::max(lgp::ws_bytes(m, v, false), lgp::ws_bytes(m, v, true));
 }
 
+extern "C" size_t egpt_token_logprobs_max_ws_bytes(int64_t m, int64_t v) {
+  size_t most = 0;  // the rows behind the last full wave decide: m of less than two waves have all there are
+  for (int64_t rows = 1; rows <= std::min<int64_t>(m, 2 * lgp::kSplitRows); ++rows)
+    most = std::max(most, egpt_token_logprobs_ws_bytes(rows, v));
+  return most;
+}
+
 extern "C" int egpt_token_logprobs(float *logp, float *entropy, int64_t *top_ids, float *top_logp, const void *logits,
                                    int64_t ldx, int dtype, int64_t m, int64_t v, const int64_t *tokens, int top, void *ws,
                                    size_t ws_bytes, unsigned flags, void *stream) {

@@ -693,9 +693,9 @@ def attn_decode_paged(q, pages, table, position, nq, nkv, d, *, scale, ws=None, 
 
 
 def token_logprobs_ws(m, v, device):
-    """Workspace of token_logprobs for up to m rows of v logits (zeroed; every call leaves it usable for the next): one per
-    stream. Many rows need none."""
-    return torch.zeros(int(L.load().egpt_token_logprobs_ws_bytes(m, v)), dtype=torch.uint8, device=device)
+    """Workspace of token_logprobs for up to m rows of up to v logits (zeroed; every call leaves it usable for the next): one
+    per stream."""
+    return torch.zeros(int(L.load().egpt_token_logprobs_max_ws_bytes(m, v)), dtype=torch.uint8, device=device)
 
 
 def token_logprobs(logits, tokens=None, *, top=0, ws=None, out=None):
@@ -729,7 +729,7 @@ def token_logprobs(logits, tokens=None, *, top=0, ws=None, out=None):
         if (lp is None) is not (tokens is None) or (not top and (ids is not None or tlp is not None)):
             raise ValueError('token_logprobs: the first of out goes with tokens, the last two with top (else None)')
     if ws is None:
-        ws = token_logprobs_ws(m, v, logits.device)
+        ws = torch.zeros(int(L.load().egpt_token_logprobs_ws_bytes(m, v)), dtype=torch.uint8, device=logits.device)
     rc = L.load().egpt_token_logprobs(
         None if lp is None else lp.data_ptr(), None if ent is None else ent.data_ptr(), None if ids is None else ids.data_ptr(),
         None if tlp is None else tlp.data_ptr(), logits.data_ptr(), logits.stride(0) if m > 1 else v, _dt(logits), m, v,

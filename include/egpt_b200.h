@@ -291,9 +291,11 @@ EGPT_API int egpt_attn_decode_paged(void *out, int64_t ldo, const void *q, int64
  * EGPT_ERR_SHAPE through egpt_device_error), entropy[r] in nats, and the `top` (0 to 32) most likely tokens in order (of
  * equal logits the lowest id first) with their log probabilities, top_ids and top_logp [m][top]. -inf logits are masked
  * tokens; a row of nothing else has log probabilities -inf and entropy 0; a NaN or +inf makes the row's results NaN.
- * Workspace: egpt_token_logprobs_ws_bytes(m, v) bytes (0 for many rows), zero-filled once by the caller, left so
- * where it matters; it serves calls of every size that needs no more. Deterministic. */
+ * Workspace: egpt_token_logprobs_ws_bytes(m, v) bytes for m rows (0 for some numbers of rows; fewer rows can need more), or
+ * egpt_token_logprobs_max_ws_bytes(m, v) for every call of up to m rows of up to v logits. Zero-filled once by the caller, left
+ * so where it matters; it serves calls of every size that needs no more. Deterministic. */
 EGPT_API size_t egpt_token_logprobs_ws_bytes(int64_t m, int64_t v);
+EGPT_API size_t egpt_token_logprobs_max_ws_bytes(int64_t m, int64_t v);
 EGPT_API int egpt_token_logprobs(float *logp, float *entropy, int64_t *top_ids, float *top_logp, const void *logits,
                                  int64_t ldx, int dtype, int64_t m, int64_t v, const int64_t *tokens, int top, void *ws,
                                  size_t ws_bytes, unsigned flags, void *stream);

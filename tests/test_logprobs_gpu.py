@@ -191,3 +191,15 @@ def test_outputs_that_nothing_would_fill_are_refused(cuda):
     got = ops.token_logprobs(x, tokens, top=2, out=(f(3), f(3), i(3, 2), f(3, 2)))
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     assert torch.equal(ops.token_logprobs(x, out=(None, f(3), None, None))[1], want[1])
+
+
+@pytest.mark.parametrize('rows', [64, 400, 592])
+def test_a_workspace_for_up_to_m_rows_serves_every_fewer(cuda, rows):
+    ops = _ops()
+    v = 151936
+    ws = ops.token_logprobs_ws(rows, v, cuda)
+    for m, width, dtype in ((rows, v, torch.bfloat16), (1, v, torch.bfloat16), (24, v, torch.float32), (3, 100, torch.bfloat16),
+                            (64, 50257, torch.float32), (1, v, torch.float32), (rows // 2, v, torch.bfloat16)):
+        x = _logits('normal', m, width, dtype, m)
+        tokens = x.float().argmax(-1)
+        _check(x, tokens, 5, ops.token_logprobs(x, tokens, top=5, ws=ws))

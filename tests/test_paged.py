@@ -159,3 +159,16 @@ def test_tensors_of_another_device_are_refused(monkeypatch):
             ops._device_of('x', On(device))
         with pytest.raises(ValueError, match='current device'):
             ops._here('x', 0, On(0), None, On(device))
+
+
+def test_a_logprobs_workspace_for_up_to_m_rows_serves_every_fewer():
+    """The size for m rows is no measure of it: the rows behind the last full wave of CTAs decide."""
+    one, most = L.load().egpt_token_logprobs_ws_bytes, L.load().egpt_token_logprobs_max_ws_bytes
+    for v in (65, 4097, 50257, 151936, 2 ** 20):
+        need = [one(m, v) for m in range(1, 1300)]
+        for m in (1, 2, 24, 296, 400, 592, 593, 1024, 1299):
+            assert most(m, v) == max(need[:m])
+            assert all(most(m, w) <= most(m, v) for w in (1, v // 3, v - 1))
+    assert most(512, 151936) > one(512, 151936)
+    assert most(65535, 151936) == most(10 ** 9, 151936) == max(one(m, 151936) for m in range(1, 9000))
+    assert most(0, 5) == most(-1, 5) == most(1, 0) == most(1, 2 ** 21) == 0
