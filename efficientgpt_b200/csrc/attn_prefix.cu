@@ -72,11 +72,6 @@ struct Args {
   float scale_log2;  // > 0
 };
 
-__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 // Shared memory by its own addresses (a pointer that is one of two places is a generic one to the compiler).
 __device__ __forceinline__ ulonglong2 lds_2x64(uint32_t at) {
   ulonglong2 r;
@@ -287,7 +282,7 @@ __global__ void __launch_bounds__(Cfg<D, Q8>::kThreads, 1) attn_prefix_kernel(co
         if (!ok) break;
         gtc::tc_fence_after();
         const uint32_t ks = Q8 ? smem_u32(scale_of(b)) : 0u, vs = ks + kBK * 4;
-        const uint64_t one2 = apf::f2_pack(A.scale_log2, A.scale_log2);
+        const uint64_t one2 = f2_pack(A.scale_log2, A.scale_log2);
         const int left = (int)min((int64_t)kBK, A.prefix - (int64_t)(b0 + b) * kBK);
         auto mask = [&](int c, uint32_t *sc) {  // -inf past the prefix
           if (left < c + 32) {
@@ -302,8 +297,8 @@ __global__ void __launch_bounds__(Cfg<D, Q8>::kThreads, 1) attn_prefix_kernel(co
 #pragma unroll
             for (int e = 0; e < 32; e += 4) {
               const ulonglong2 f = lds_2x64(ks + (uint32_t)(c + e) * 4);
-              const float2 x = apf::f2_unpack(f2_mul(apf::f2_pack(__uint_as_float(sc[e]), __uint_as_float(sc[e + 1])), f.x));
-              const float2 y = apf::f2_unpack(f2_mul(apf::f2_pack(__uint_as_float(sc[e + 2]), __uint_as_float(sc[e + 3])), f.y));
+              const float2 x = f2_unpack(f2_mul(f2_pack(__uint_as_float(sc[e]), __uint_as_float(sc[e + 1])), f.x));
+              const float2 y = f2_unpack(f2_mul(f2_pack(__uint_as_float(sc[e + 2]), __uint_as_float(sc[e + 3])), f.y));
               sc[e] = __float_as_uint(x.x), sc[e + 1] = __float_as_uint(x.y);
               sc[e + 2] = __float_as_uint(y.x), sc[e + 3] = __float_as_uint(y.y);
             }
@@ -341,8 +336,8 @@ __global__ void __launch_bounds__(Cfg<D, Q8>::kThreads, 1) attn_prefix_kernel(co
           }
         }
         const float base = m_run == -INFINITY ? 0.f : m_run;  // (every score so far is -inf: their weights are zeros)
-        const uint64_t nm2 = apf::f2_pack(-base, -base);
-        uint64_t sum[2] = {apf::f2_pack(0.f, 0.f), apf::f2_pack(0.f, 0.f)};
+        const uint64_t nm2 = f2_pack(-base, -base);
+        uint64_t sum[2] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
         // weights of 32 keys over scores that have been read: bf16 in columns c / 2 ..; int8 in the 32 columns of their
         // own scores, the second parts in the upper 16
         auto weights = [&](int c, const uint32_t *sc) {
@@ -354,11 +349,11 @@ __global__ void __launch_bounds__(Cfg<D, Q8>::kThreads, 1) attn_prefix_kernel(co
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               const int k = e + 2 * h;
-              const uint64_t raw = apf::f2_pack(__uint_as_float(sc[k]), __uint_as_float(sc[k + 1]));
-              const float2 x = apf::f2_unpack(Q8 ? apf::f2_add(raw, nm2) : apf::f2_fma(raw, one2, nm2));
+              const uint64_t raw = f2_pack(__uint_as_float(sc[k]), __uint_as_float(sc[k + 1]));
+              const float2 x = f2_unpack(Q8 ? f2_add(raw, nm2) : f2_fma(raw, one2, nm2));
               float2 w = make_float2(apf::ex2(x.x), apf::ex2(x.y));
-              sum[h] = apf::f2_add(sum[h], apf::f2_pack(w.x, w.y));
-              if constexpr (Q8) w = apf::f2_unpack(f2_mul(apf::f2_pack(w.x, w.y), h ? vf.y : vf.x));
+              sum[h] = f2_add(sum[h], f2_pack(w.x, w.y));
+              if constexpr (Q8) w = f2_unpack(f2_mul(f2_pack(w.x, w.y), h ? vf.y : vf.x));
               pk[k / 2] = gtc::pack_bf16x2(w.x, w.y);
               if constexpr (Q8) pl[k / 2] = gtc::pack_bf16x2(w.x - bf16_lo(pk[k / 2]), w.y - bf16_hi(pk[k / 2]));
             }
@@ -374,7 +369,7 @@ __global__ void __launch_bounds__(Cfg<D, Q8>::kThreads, 1) attn_prefix_kernel(co
           if (!Q8) mask(c, sc);
           weights(c, sc);
         }
-        const float2 t = apf::f2_unpack(apf::f2_add(sum[0], sum[1]));
+        const float2 t = f2_unpack(f2_add(sum[0], sum[1]));
         l_sum = l_sum * alpha + (t.x + t.y);
         apf::tmem_wait_st();
         gtc::tc_fence_before();

@@ -149,27 +149,6 @@ __device__ __forceinline__ void take(Sums &a, const float (&y)[E], float largest
   }
 }
 
-// Two fp32 operations an instruction.
-__device__ __forceinline__ uint64_t pair(float lo, float hi) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-__device__ __forceinline__ float2 halves(uint64_t v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -198,21 +177,21 @@ __device__ __forceinline__ float largest_of(uint4 c) {
 template <int E>
 __device__ __forceinline__ void take2(uint64_t &s, uint64_t &w, float m, uint4 c) {
   const uint32_t v[4] = {c.x, c.y, c.z, c.w};
-  const uint64_t less = pair(-__fmul_rn(m, kLog2e), -__fmul_rn(m, kLog2e)), log2e = pair(kLog2e, kLog2e);
+  const uint64_t less = f2_pack(-__fmul_rn(m, kLog2e), -__fmul_rn(m, kLog2e)), log2e = f2_pack(kLog2e, kLog2e);
 #pragma unroll
   for (int i = 0; i < E / 2; ++i) {
     // no lower than -1e37 (0xfcf0, as bf16 -9.97e36), whose weight is 0 and exponent finite: -inf would give 0 times infinity
     uint64_t x;
     if (E == 8) {
       const uint32_t t = max2(v[i % 4], 0xfcf0fcf0u);
-      x = pair(bf16_lo(t), bf16_hi(t));
+      x = f2_pack(bf16_lo(t), bf16_hi(t));
     } else {
-      x = pair(fmaxf(__uint_as_float(v[(2 * i) % 4]), -1e37f), fmaxf(__uint_as_float(v[(2 * i + 1) % 4]), -1e37f));
+      x = f2_pack(fmaxf(__uint_as_float(v[(2 * i) % 4]), -1e37f), fmaxf(__uint_as_float(v[(2 * i + 1) % 4]), -1e37f));
     }
-    const uint64_t t = fma2(x, log2e, less);
-    const float2 th = halves(t);
-    const uint64_t f = pair(apf::ex2(th.x), apf::ex2(th.y));
-    s = add2(s, f), w = fma2(f, t, w);
+    const uint64_t t = f2_fma(x, log2e, less);
+    const float2 th = f2_unpack(t);
+    const uint64_t f = f2_pack(apf::ex2(th.x), apf::ex2(th.y));
+    s = f2_add(s, f), w = f2_fma(f, t, w);
   }
 }
 
@@ -332,7 +311,7 @@ __global__ void __launch_bounds__(kThreads, kResident) logprobs_kernel(const Par
     largest = max(largest, most);
     const float mx = value_of(most);  // the same in all lanes, as a.m is
     if (!(mx <= a.m + 4.f) || !plain_range(a.m)) {
-      const float2 s = halves(s2), w = halves(w2);
+      const float2 s = f2_unpack(s2), w = f2_unpack(w2);
       a.s += s.x + s.y, a.w += w.x + w.y, s2 = w2 = 0u;
       if (mx > a.m) rescale(a, mx);
       if (!plain_range(a.m)) {  // nothing yet, or far from 0: one element at a time
@@ -380,7 +359,7 @@ __global__ void __launch_bounds__(kThreads, kResident) logprobs_kernel(const Par
     const uint4 c[1] = {__ldg((const uint4 *)(r.x - r.off) + g * 32 + lane)};
     add(g, c);
   }
-  const float2 s = halves(s2), w = halves(w2);
+  const float2 s = f2_unpack(s2), w = f2_unpack(w2);
   a.s += s.x + s.y, a.w += w.x + w.y;
   // the first and the last one otherwise
   const int ends[2] = {r.off ? 0 : -1, r.groups - 1 >= (r.v + r.off) / (32 * E) && (r.groups > 1 || !r.off) ? r.groups - 1 : -1};

@@ -62,39 +62,19 @@ __device__ __forceinline__ uint4 bf16x8(const float (&x)[8]) {
 struct Eight {
   uint64_t v[4];
 };
-__device__ __forceinline__ uint64_t pair(float lo, float hi) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-__device__ __forceinline__ float2 halves(uint64_t v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
 __device__ __forceinline__ Eight widen8(uint4 a) {
-  return {{pair(bf16_lo(a.x), bf16_hi(a.x)), pair(bf16_lo(a.y), bf16_hi(a.y)), pair(bf16_lo(a.z), bf16_hi(a.z)),
-           pair(bf16_lo(a.w), bf16_hi(a.w))}};
+  return {{f2_pack(bf16_lo(a.x), bf16_hi(a.x)), f2_pack(bf16_lo(a.y), bf16_hi(a.y)), f2_pack(bf16_lo(a.z), bf16_hi(a.z)),
+           f2_pack(bf16_lo(a.w), bf16_hi(a.w))}};
 }
 __device__ __forceinline__ Eight load8(const void *src, int64_t at, bool f32) {
   if (!f32) return widen8(*(const uint4 *)((const uint16_t *)src + at));
   const float4 a = ((const float4 *)((const float *)src + at))[0], b = ((const float4 *)((const float *)src + at))[1];
-  return {{pair(a.x, a.y), pair(a.z, a.w), pair(b.x, b.y), pair(b.z, b.w)}};
+  return {{f2_pack(a.x, a.y), f2_pack(a.z, a.w), f2_pack(b.x, b.y), f2_pack(b.z, b.w)}};
 }
 __device__ __forceinline__ void unpack(float (&y)[8], const Eight &x) {
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    const float2 h = halves(x.v[e]);
+    const float2 h = f2_unpack(x.v[e]);
     y[2 * e] = h.x, y[2 * e + 1] = h.y;
   }
 }
@@ -117,8 +97,8 @@ __device__ __forceinline__ void append_head(const AppendParams &p, const uint4 (
     if (norm_w) {
       uint64_t s2 = 0u;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s2 = fma2(lo.v[e], lo.v[e], fma2(hi.v[e], hi.v[e], s2));
-      const float2 s = halves(s2);
+      for (int e = 0; e < 4; ++e) s2 = f2_fma(lo.v[e], lo.v[e], f2_fma(hi.v[e], hi.v[e], s2));
+      const float2 s = f2_unpack(s2);
       float ss = s.x + s.y;
 #pragma unroll
       for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
@@ -126,16 +106,16 @@ __device__ __forceinline__ void append_head(const AppendParams &p, const uint4 (
       const Eight w0 = widen8(*(const uint4 *)(norm_w + e0)), w1 = widen8(*(const uint4 *)(norm_w + kHalf + e0));
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        lo.v[e] = mul2(mul2(lo.v[e], pair(inv, inv)), w0.v[e]);
-        hi.v[e] = mul2(mul2(hi.v[e], pair(inv, inv)), w1.v[e]);
+        lo.v[e] = f2_mul(f2_mul(lo.v[e], f2_pack(inv, inv)), w0.v[e]);
+        hi.v[e] = f2_mul(f2_mul(hi.v[e], f2_pack(inv, inv)), w1.v[e]);
       }
     }
     if (turned) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float2 a = halves(mul2(lo.v[e], cosine.v[e])), b = halves(hi.v[e]), s = halves(sine.v[e]);
-        hi.v[e] = fma2(lo.v[e], sine.v[e], mul2(hi.v[e], cosine.v[e]));
-        lo.v[e] = pair(fmaf(-b.x, s.x, a.x), fmaf(-b.y, s.y, a.y));
+        const float2 a = f2_unpack(f2_mul(lo.v[e], cosine.v[e])), b = f2_unpack(hi.v[e]), s = f2_unpack(sine.v[e]);
+        hi.v[e] = f2_fma(lo.v[e], sine.v[e], f2_mul(hi.v[e], cosine.v[e]));
+        lo.v[e] = f2_pack(fmaf(-b.x, s.x, a.x), fmaf(-b.y, s.y, a.y));
       }
     }
     float l[8], h[8];
