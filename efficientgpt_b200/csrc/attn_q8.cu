@@ -44,17 +44,18 @@
 // behind a prefix instead of in a launch for it (64 rows over 32768 shared keys 81 us for 66).
 //
 // Over pages (the PAGED instantiations): a warp asks for the names of a tile's pages one tile ahead, a lane to a row, and
-// takes a tile that lies in one page as it takes a contiguous one; a tile of several smaller pages is gathered row by
-// row (int8 tiles of 32 keys from 16-row pages 113 us where 32-row pages take 96). Segments are cut wherever the even
-// shares fall, int8 keys with up to four query rows have MMAs and twelve warps of
-// their own, and many bf16 segments two CTAs an SM. What bounds it: HBM, once the loops run (bf16 6.3, int8 5.9 TB/s over
-// one long sequence); besides it 5 us of way in and launch, 3.9 us of way out for split segments (fence and arrival 1.3,
-// adding 18 records up 2.6), and 2 to 3 us a segment in between, most of it warps that wait for the others' last tile.
-// Measured, d = 128, 8 kv heads, on the device: 64 rows of 32 heads over 200 to 16000 bf16 keys 151 us (906 MB, 6.0 TB/s),
-// int8 in 32-row pages 120 us (653 MB); one row over 211 / 2048 / 32768 bf16 keys 6.3 / 11.8 / 30 us; 16 rows of 16 heads
-// over 33 to 8191 int8 keys 27 us. Tried: stretches of single warps without any meeting (records of all of them to add
-// up, and registers for it that spill: int8 112 us where whole CTAs take 96), P.V of a tile under the next one's scores
-// (no faster), merges by two warps a row (no faster: the wait for the last tile is what counts).
+// takes a tile that lies in one page as it takes a contiguous one; a tile of several smaller pages is gathered row by row (64
+// rows of 32 heads over 3544 int8 keys, 480 MB, 114 us from 16-row pages where 32-row pages take 96). Segments are cut
+// wherever the even shares fall, int8 keys with up to four query rows have MMAs and twelve warps of their own, and many bf16
+// segments two CTAs an SM. (A maximum that moves for a factor of 2^8 only saves up to 1%, but then weights up to 2^8 overflow
+// the sums of values that large, and a reference above the maximum loses the smallest weights.) What bounds it: HBM, once the
+// loops run (bf16 6.3, int8 5.9 TB/s over one long sequence); besides it 5 us of way in and launch, 3.9 us of way out for
+// split segments (fence and arrival 1.3, adding 18 records up 2.6), and 2 to 3 us a segment in between, most of it warps that
+// wait for the others' last tile. Measured, d = 128, 8 kv heads, on the device: 64 rows of 32 heads over 200 to 16000 bf16
+// keys 147 to 151 us (906 MB, 6.1 TB/s), int8 in 32-row pages 119 us (653 MB); one row over 211 / 2048 / 32768 bf16 keys 6.3 /
+// 12.9 / 29 us; 16 rows of 16 heads over 33 to 8191 int8 keys 26.5 us. Tried: stretches of single warps without any meeting
+// (records of all of them to add up, and registers for it that spill: int8 112 us where whole CTAs take 96), P.V of a tile
+// under the next one's scores (no faster), merges by two warps a row (no faster: the wait for the last tile is what counts).
 #include <cmath>
 
 #include "internal.h"
@@ -69,8 +70,8 @@ constexpr int kRows = 16;        // query rows per tile (the M of the MMA), and 
 constexpr int kMinKeys = 512;    // keys of a range at least
 constexpr int kExtraKeys = 512;  // what a segment's start and end cost, in keys
 // Over pages, whose segments are cut wherever the even cuts fall, but nearer to an end than the margin at that end: no CTA
-// has more than its share, where leaving short segments whole gave some half as much again (64 rows over 200 to
-// 16000 bf16 keys 181 -> 155 us, 478 MB of int8 174 -> 140).
+// has more than its share, where leaving short segments whole gives some half as much again (64 rows over 200 to
+// 16000 bf16 keys take 17% longer then, 478 MB of int8 24%).
 constexpr int kMarginKeys = 256;
 
 struct Cache {
@@ -131,9 +132,9 @@ struct Cfg {
   static constexpr int kTile = Q8 ? 32 : 16;  // keys per warp tile: K and V 4 KB each at d = 128
   static constexpr int kStages = NR == 8 ? 3 : 2;
   static constexpr int kMinChunk = kMinKeys / kTile, kExtra = kExtraKeys / kTile;
-  // what a segment costs besides its tiles over pages, where its warps' merge comes in between two segments' loads: with 256,
-  // 512, 768 int8 keys 64 rows over 200 to 16000 take 155, 128, 122 us (bf16: no difference there, and for 16 rows of 33
-  // to 288 12.1, 9.8, 9.7)
+  // what a segment costs besides its tiles over pages, where its warps' merge comes in between two segments' loads: with 256
+  // and 512 int8 keys 64 rows over 200 to 16000 take 27% and 5% longer than with 768 (bf16: no difference there, and for 16 rows
+  // of 33 to 288 25% and 1%)
   static constexpr int kMargin = kMarginKeys / kTile, kPagedExtra = (Q8 ? 768 : 512) / kTile;
 };
 template <int D, bool Q8, int NR, int PAGED = 0>

@@ -2,22 +2,27 @@
 //
 //   log p(t) = x_t - m - ln s,   s = sum_j e^(x_j - m),   H = ln s - (1/s) sum_j e^(x_j - m) (x_j - m),   m = max_j x_j;
 //   the `top` largest logits (of equal ones the lowest index first) with their log p.
-// Every thread keeps a running maximum, sum and weighted sum (fp32, base-2 exponents) of its elements, rescaled when the
-// maximum moves. A row is cut into groups of 512 consecutive bytes, one load of a warp each, whose largest value is kept
-// as an ordered 32-bit key (one redux). The top tokens lie in the `top` groups that come first by (largest value, index):
-// each of those holds an element that comes before all of any other group's. So they are found from the keys and
-// read once more, whatever the logits look like: sorted, constant or mostly masked ones cost no more than others.
+// Every thread keeps a sum and a weighted sum (fp32, base-2 exponents) of its elements, relative to a reference that all
+// lanes of its warp share: the largest element of the warp's first groups, and a later one only where that is 4 more, so
+// that weights go up to e^4 and few sums are rescaled; warps and CTAs are joined relative to the larger reference, and in
+// the end to the row's maximum. A row is cut into groups of 512 consecutive bytes, one load of a warp each, whose largest
+// value is kept as an ordered 32-bit key (one redux). The top tokens lie in the `top` groups that come first by (largest
+// value, index): each of those holds an element that comes before all of any other group's. So they are found from the keys
+// and read once more, whatever the logits look like. (Many equal logits, which the selection has to tell apart by their
+// index, cost up to a quarter more over 1024 rows and up to 18 us over a few; warps that have seen nothing but -inf, or a
+// reference beyond 1e4, take one element at a time: 1024 rows with five tokens left 100 us, far from 0 120 us.)
 //
 // Few rows are split over CTAs, each of which leaves its sums and its groups' keys in the workspace; the last of a row's
 // CTAs to arrive adds them up in their order (results do not depend on timing). A NaN or +inf logit makes a row's
 // probabilities NaN; a row of -inf alone has log p = -inf and entropy 0.
 //
 // What bounds it: many rows of bf16 the arithmetic (one exponential and 8.5 instructions an element; 1024 rows of 151936
-// 54.6 us without top tokens, 5.7 TB/s, and 62.5 with one: a row's two selections are 2 us each, in which its CTA loads
-// nothing), of fp32 HBM (512 rows 50.5 us, 6.2 TB/s); few rows the chain of round trips (one row 5.7 us without, 9.1 with one
-// and 11.8 with twenty top tokens). Tried: the loads ahead in registers (66.5 us: they leave no more than four CTAs an
-// SM either way and cost moves), 128 threads a CTA (65.0, but 96 with twenty top tokens for 77), parts of all rows of a last
-// wave (80).
+// 54.4 us without top tokens, 5.7 TB/s, 62.2 with one and 75 with twenty: a row's two selections are 2 us each, in which
+// its CTA loads nothing), of fp32 HBM (512 rows 49.5 us, 6.3 TB/s); rows that do not fill waves of CTAs the places left
+// empty (300, 512 and 740 rows 31, 39 and 54 us with one top token, whose bytes take 14, 24 and 34); few rows the chain of
+// round trips (one row 5.8 us without, 9.3 with one and 11.9 with twenty top tokens). Tried: the loads ahead in registers (4%
+// longer: they leave no more than four CTAs an SM either way and cost moves), 128 threads a CTA (2% longer, a quarter
+// with twenty top tokens), parts of all rows of a last wave (a quarter longer).
 #include "internal.h"
 #include "common.cuh"
 
@@ -298,8 +303,7 @@ __global__ void __launch_bounds__(kThreads, kResident) logprobs_kernel(const Par
     if (p.top && lane == 0) keys[g] = key;
     return key;
   };
-  // Groups that lie inside the row whole, U loads on their way at once. A warp's sums are relative to the largest element of its
-  // first U groups, and to a later one's only where that is 4 more (weights up to e^4 and a few exponents that are rescaled).
+  // Groups that lie inside the row whole, U loads on their way at once.
   const int whole0 = max(g0, r.off ? 1 : 0), whole1 = min(g1, (r.v + r.off) / (32 * E));
   Sums a = {-INFINITY, 0.f, 0.f};
   uint64_t s2 = 0u, w2 = 0u;
@@ -455,8 +459,8 @@ static int group_elems(bool f32) { return 512 / (f32 ? 4 : 2); }
 static int most_groups(int64_t v, bool f32) { return (int)((v + 16 / (f32 ? 4 : 2) - 1 + group_elems(f32) - 1) / group_elems(f32)); }
 // The rows in full waves of CTAs take one each. Those behind them are split where two parts or more of each fit into one wave, with
 // 16 groups (two loads a warp) a part at least. More parts than that cost more than the places they fill: a part ends
-// with a fence, an arrival and an idle stream (1024 rows of 151936 bf16 logits, 432 of them behind a wave of 592: 69 us
-// whole, 80 us in quarters).
+// with a fence, an arrival and an idle stream (1024 rows of 151936 bf16 logits, 432 of them behind a wave of 592, take 16%
+// longer in quarters than whole).
 static void cut(int64_t m, int64_t v, bool f32, int &whole, int &splits) {
   const int wave = std::min(num_sms() * kResident, kSplitRows), rest = (int)(m % wave);
   splits = rest ? std::max(1, std::min(wave / rest, most_groups(v, f32) / 16)) : 1;

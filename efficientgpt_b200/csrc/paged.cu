@@ -4,10 +4,11 @@
 // or int8 codes with one fp32 scale a row (kv_q8.cu's quantiser). table[i][c] names the page of slots c S .. c S + S - 1 of
 // sequence i (-1: none). A page's rows of one head lie together, so that attention streams S d elements at a time and
 // a tensor of one page is the contiguous caches' [heads][cap][d] with cap = S. Single passes: few rows are bound by the launch
-// and the round trips to memory that find their place (one row 2.5 us on the device), prompts by that and by instructions
-// (3370 rows of 48 heads with norm and rotation 19.4 us, 85 MB, 4.4 TB/s; 235 instructions for 16 elements a lane, without norm
-// and rotation 5.3 TB/s), reads by HBM (32768 rows of 8 heads 36 us from int8, 203 MB, 5.7 TB/s, 43 us from bf16, 268 MB,
-// 6.2 TB/s).
+// and the round trips to memory that find their place (one row 2.4 us on the device), prompts by waiting, for neither HBM nor
+// the issue slots are full (3370 rows of 48 heads with norm and rotation 17.7 us, 85 MB, 4.8 TB/s, 58% of the issue slots;
+// without both 5.9 TB/s; 4096 rows into int8 pages 22.5 us, 94 MB, 4.2 TB/s, and into bf16 ones 20.8, 102 MB, 4.9 TB/s): every
+// wave of CTAs goes through its rows' look-ups (start, position, page, angles) together before it works on them. Reads are
+// bound by HBM (32768 rows of 8 heads 36 us from int8, 203 MB, 5.7 TB/s, 43 us from bf16, 268 MB, 6.2 TB/s).
 #include "internal.h"
 #include "common.cuh"
 
@@ -141,11 +142,11 @@ __device__ __forceinline__ void append_head(const AppendParams &p, const uint4 (
 }
 
 // A warp takes one row, or every parts-th of its turns: so the row's sequence, slot and page are found once (the starts 32 at a
-// time), the angles are read once, and all of its heads are on their way to shared memory before that (with one turn ahead in
-// registers 20.1 us for 19.4). A turn takes heads of one kind, q, k or v, D / 16 lanes to a head: lane l dims 8 l .. 8 l + 7
+// time), the angles are read once, and all of its heads are on their way to shared memory before that (4% less time than with
+// one turn ahead in registers). A turn takes heads of one kind, q, k or v, D / 16 lanes to a head: lane l dims 8 l .. 8 l + 7
 // and the D / 2 further on that the half-layout rotation pairs them with, so a vector is read once in 16-byte pieces, the
 // rotation stays inside a lane, and the norm and the quantiser's maximum take a few shuffles. Norm and rotation are fp32 and
-// rounded once, to bf16 or to a code. (The norm weights in shared memory as fp32: 21.8 us, for the barrier.)
+// rounded once, to bf16 or to a code. (With the norm weights in shared memory as fp32 12% longer, for the barrier.)
 template <int D, bool Q8>
 __global__ void __launch_bounds__(kThreads, 4) append_kernel(const AppendParams p) {
   constexpr int kLanes = D / 16, kHalf = D / 2, kGroups = 32 / kLanes, kBytes = Q8 ? 1 : 2;
@@ -251,12 +252,12 @@ struct ReadParams {
 };
 
 // out[i nkv + h][r] = row start_i + r of head h of sequence i: eight elements a thread, of K and of V, so that neighbouring
-// threads write neighbouring 16-byte pieces (with sixteen codes a thread, whose two pieces leave one after the other, 32768
-// rows of 8 heads 44.6 us, now 41.3), ROWS rows' on their way at once (two where that fills the GPU twice over, one for
-// shorter stretches: 4096 rows 7.4 us, with two 7.9; four and eight leave too few threads to an SM: 41.5 and 51.2 us for
-// the 32768, two 39.7). The stores are marked as passing through, like the loads (without and with: 39.7 and 39.0 us, bf16
-// pages 44.9 and 43.5). Sequence and head come from the grid and slots are 32 bits (a division and 64-bit slots a row: 39.0 us
-// for 35.8), in 32 registers, so that an SM has all its threads (40 registers and 10% fewer instructions: 38.1).
+// threads write neighbouring 16-byte pieces (sixteen codes a thread, whose two pieces leave one after the other, take 8% longer
+// for 32768 int8 rows of 8 heads), ROWS rows' on their way at once (two where that fills the GPU twice over: one takes 4% longer
+// for those 32768 rows, and four and eight, which leave too few threads to an SM, 5% and 29%; one for shorter stretches:
+// two take 7% longer for 4096 rows). The stores are marked as passing through, like the loads (2% less, over bf16 pages 3%).
+// Sequence and head come from the grid and slots are 32 bits (a division and 64-bit slots a row: 9% longer), in 32 registers,
+// so that an SM has all its threads (40 registers and 10% fewer instructions: 6% longer).
 template <int D, bool Q8, bool F32, int ROWS>
 __global__ void __launch_bounds__(kThreads) read_kernel(const ReadParams p) {
   constexpr int kElems = 8, kLanes = D / kElems, kStep = kThreads / kLanes;
@@ -392,8 +393,8 @@ extern "C" int egpt_kv_append_paged(void *k_pages, float *k_scale, void *v_pages
   p.q = (const uint16_t *)q, p.k = (const uint16_t *)k, p.v = (const uint16_t *)v, p.q_out = (uint16_t *)q_out;
   p.ldq = ldq, p.ldk = ldk, p.ldv = ldv, p.ldqo = ldqo, p.position = position, p.starts = starts;
   p.seqs = (int)seqs, p.m = (int)m, p.nq = nq;
-  // kTurns turns of a row's heads to a warp (4096 rows of 48 heads 22.0 us, 22.2 with three, 22.8 with six; 3370 rows 19.4, 19.1
-  // and 20.3), fewer as long as that makes no more than 16 warps an SM
+  // kTurns turns of a row's heads to a warp (three take 1% longer for 4096 rows of 48 heads and 2% less for 3370, six 4% and 5%
+  // longer), fewer as long as that makes no more than 16 warps an SM
   const int64_t groups = 512 / d, turns = (nq + groups - 1) / groups + 2 * ((nkv + groups - 1) / groups);
   const int64_t parts = std::max<int64_t>((turns + pgd::kTurns - 1) / pgd::kTurns, std::min<int64_t>(turns, 16 * num_sms() / m));
   p.q_norm_w = (const uint16_t *)q_norm_w, p.k_norm_w = (const uint16_t *)k_norm_w, p.eps = eps;

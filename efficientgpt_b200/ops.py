@@ -631,8 +631,9 @@ def kv_append_paged(k, v, pages, table, position, *, starts=None, q=None, q_norm
 
 
 def kv_read_paged(pages, table, start, count, *, dtype=torch.bfloat16, out=None):
-    """The rows start .. start + count - 1 of every sequence of the table (start: an int, or int64 [M] on the device): (k,
-    v), each [M * nkv, count, d] bf16 or fp32; slots outside the table and pages of -1 read as zeros. out: the (k, v)
+    """The rows start .. start + count - 1 of every sequence of the table (start: an int, with all rows inside the table, or
+    int64 [M] on the device, whose rows outside it read as zeros): (k, v), each [M * nkv, count, d] bf16 or fp32; pages of -1
+    read as zeros. out: the (k, v)
     tensors to fill, rows contiguous, one head stride."""
     (_, nkv, _, d), pool, seqs, device = _pool('kv_read_paged', pages, table)
     heads = seqs * nkv

@@ -259,9 +259,9 @@ EGPT_API int egpt_attn_shared_prefix_on_tcgen05(int64_t m, int nq, int nkv, int 
  * fp32 and rounded once, to bf16 or to a code. q [m][nq d] (nullable) goes to q_out, which may be q; rows without a
  * slot become zeros. Two rows for one slot leave elements of both.
  *
- * egpt_kv_read_paged: rows start .. start + count - 1 of every sequence (starts: NULL, or int64 [seqs] on the device in
- * place of start) into k_out and v_out, bf16 or fp32 [seqs nkv][count][d] with out_head_stride elements between the heads;
- * slots outside the table and pages of -1 read as zeros (not reported).
+ * egpt_kv_read_paged: rows start .. start + count - 1 of every sequence into k_out and v_out, bf16 or fp32 [seqs nkv][count][d]
+ * with out_head_stride elements between the heads. With starts NULL all of them have to lie inside the table; starts (int64
+ * [seqs] on the device) takes the place of start, and slots outside the table read as zeros, as pages of -1 do (not reported).
  *
  * egpt_attn_decode_paged: softmax(scale q K^T) V of row i of q bf16 [m][nq d] over the position[i] + 1 keys of sequence i
  * (m sequences; -1: an idle slot, zeros), GQA with at most 16 query heads to a kv head. Keys on pages that are -1 or
